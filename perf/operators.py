@@ -213,7 +213,8 @@ def _operator(case):
 
     if case["kind"] in ("delta", "train"):
         return O.GatedDelta(case["dtype"], case["batch"], case["tokens"], case["key_heads"], case["value_heads"],
-                            case["key_dim"], case["value_dim"], sequences=case["sequences"] or None)
+                            case["key_dim"], case["value_dim"], sequences=case["sequences"] or None,
+                            states=case["state"])
     if case["kind"] in ("norm", "norm_back"):
         return O.NormBlock(case["dtype"], case["rows"], case["width"], norm=case["norm"], pre=case["pre"],
                            gate=case["gate"], dropout=case["dropout"], scale=RESIDUAL_SCALE, eps=EPS,
