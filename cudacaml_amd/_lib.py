@@ -25,7 +25,8 @@ c_cp = ctypes.c_char_p
 c_i64 = ctypes.c_int64
 P = ctypes.POINTER
 
-# name -> (restype, argtypes); every symbol the headers declare.
+# name -> (restype, argtypes); every symbol cchip_runtime.h and
+# cchip_backend.h declare (cchip_operators.h: OPERATOR_SIGNATURES below).
 SIGNATURES = {
     # cchip_runtime.h
     "cchip_last_error": (c_cp, []),
@@ -92,6 +93,57 @@ SIGNATURES = {
     "cchip_program_timing_each": (c_int, [c_vp, c_int, P(ctypes.c_double), P(c_int), P(ctypes.c_double)]),
 }
 
+
+
+# ---- cchip_operators.h --------------------------------------------------------
+
+c_i32 = ctypes.c_int32
+c_u64 = ctypes.c_uint64
+
+
+class GatedDeltaDesc(ctypes.Structure):
+    _fields_ = [("dtype", c_int), ("batch", c_i64), ("tokens", c_i64), ("sequences", c_i64), ("key_heads", c_int),
+                ("value_heads", c_int), ("key_dim", c_int), ("value_dim", c_int), ("states", c_int),
+                ("scale", ctypes.c_float)]
+
+
+class Heads(ctypes.Structure):
+    _fields_ = [("data", c_vp), ("batch", c_i64), ("token", c_i64), ("head", c_i64)]
+
+
+class GatedDeltaIO(ctypes.Structure):
+    _fields_ = [(n, Heads) for n in ("q", "k", "v", "g", "beta", "o", "d_o", "dq", "dk", "dv", "dg", "dbeta")] + [
+        (n, c_vp) for n in ("offsets", "state", "state_out", "dstate_out", "dstate", "saved")]
+
+
+class DropDesc(ctypes.Structure):
+    _fields_ = [("p", ctypes.c_double), ("seed", c_u64), ("offset", c_u64), ("step", c_vp)]
+
+
+class Rows(ctypes.Structure):
+    _fields_ = [("data", c_vp), ("row", c_i64)]
+
+
+class NormBlockDesc(ctypes.Structure):
+    _fields_ = [("dtype", c_int), ("weight_dtype", c_int), ("rows", c_i64), ("width", c_i64), ("post", c_int),
+                ("pre", c_int), ("gate", c_int), ("scale", ctypes.c_float), ("eps", ctypes.c_float)]
+
+
+class NormParams(ctypes.Structure):
+    _fields_ = [(n, c_vp) for n in ("post_weight", "post_bias", "channel_scale", "pre_weight", "pre_bias")]
+
+
+OPERATOR_SIGNATURES = {
+    "cchip_gated_delta_sizes": (c_int, [P(GatedDeltaDesc), P(c_size), P(c_size)]),
+    "cchip_gated_delta_forward": (c_int, [P(GatedDeltaDesc), P(GatedDeltaIO), c_vp, c_size, c_vp]),
+    "cchip_gated_delta_backward": (c_int, [P(GatedDeltaDesc), P(GatedDeltaIO), c_vp, c_size, c_vp]),
+    "cchip_dropout": (c_int, [c_int, c_i64, c_i64, P(DropDesc), ctypes.c_float, Rows, Rows, Rows, c_vp]),
+    "cchip_norm_block_forward": (c_int, [P(NormBlockDesc), P(DropDesc), P(NormParams)] + [Rows] * 5 + [c_vp]),
+    "cchip_norm_block_workspace": (c_int, [P(NormBlockDesc), P(c_size)]),
+    "cchip_norm_block_backward": (c_int, [P(NormBlockDesc), P(DropDesc), P(NormParams), P(NormParams)] + [Rows] * 8
+                                  + [c_vp, c_size, c_vp]),
+}
+
 _lib = None
 
 
@@ -109,7 +161,7 @@ def lib():
             "cudacaml_amd: %s is not built; run __graft_entry__.build() or python -m cudacaml_amd.build" % LIB_PATH
         )
     L = ctypes.CDLL(LIB_PATH)
-    for name, (res, args) in SIGNATURES.items():
+    for name, (res, args) in list(SIGNATURES.items()) + list(OPERATOR_SIGNATURES.items()):
         f = getattr(L, name)
         f.restype = res
         f.argtypes = args

@@ -1,10 +1,10 @@
 """Builds ``libcchip.so`` (the runtime + Backend_hip C-ABI) in-tree.
 
-The library is host code over the HIP runtime and hiprtc; the kernels it
-runs are generated per graph and compiled by hiprtc for gfx950 at
-``compile`` time. Its own device code (``csrc/*.hip``, built for gfx950
-here) is the static scratch of the allocation-free entry point and the
-kernel that clears it. ``check_templates`` JIT-compiles a representative set of
+The library is host code over the HIP runtime and hiprtc; the kernels a
+graph runs are generated and compiled by hiprtc for gfx950 at ``compile``
+time. Its own device code (``csrc/*.hip``, built for gfx950 here) is the
+layer operators and the static scratch of the allocation-free entry point
+with the kernel that clears it. ``check_templates`` JIT-compiles a representative set of
 generated modules without a GPU, so template errors surface at build time.
 """
 
@@ -13,6 +13,8 @@ from __future__ import annotations
 import glob
 import os
 import subprocess
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libcchip.so")
@@ -33,23 +35,30 @@ def build(verbose=False, asan=False):
     srcs = sorted(glob.glob(os.path.join(HERE, "csrc", "*.cpp"))) + sorted(glob.glob(os.path.join(HERE, "csrc", "*.hip")))
     out = ASAN_LIB if asan else LIB
     tmp = out + ".tmp%d" % os.getpid()
-    cmd = [
-        os.path.join(ROCM, "bin", "hipcc"),
-        "--offload-arch=gfx950", "-O1" if asan else "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+    hipcc = os.path.join(ROCM, "bin", "hipcc")
+    flags = [
+        "--offload-arch=gfx950", "-O1" if asan else "-O2", "-std=c++17", "-fPIC", "-Wall",
         "-Wno-unused-function",
         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         "-D__HIP_PLATFORM_AMD__",
         "-I" + os.path.join(ROCM, "include"),
     ]
-    if asan:
-        cmd += ["-g", "-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fno-omit-frame-pointer"]
-    cmd += ["-o", tmp] + srcs + [
-        "-L" + os.path.join(ROCM, "lib"), "-Wl,-rpath," + os.path.join(ROCM, "lib"),
-        "-lhiprtc", "-lamdhip64",
-    ]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True)
+    sanitize = ["-g", "-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fno-omit-frame-pointer"] if asan else []
+
+    def run(cmd):
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.run(cmd, check=True)
+
+    # One compilation a source, as many at once as the machine is allowed.
+    jobs = int(os.environ.get("MAX_JOBS") or min(8, os.cpu_count() or 1))
+    with tempfile.TemporaryDirectory(prefix="cchip-build-") as work, ThreadPoolExecutor(max(1, jobs)) as pool:
+        objs = [os.path.join(work, os.path.basename(s) + ".o") for s in srcs]
+        list(pool.map(run, [[hipcc] + flags + sanitize + ["-c", "-o", o, s] for s, o in zip(srcs, objs)]))
+        run([hipcc, "--offload-arch=gfx950", "-shared"] + sanitize + ["-o", tmp] + objs + [
+            "-L" + os.path.join(ROCM, "lib"), "-Wl,-rpath," + os.path.join(ROCM, "lib"),
+            "-lhiprtc", "-lamdhip64",
+        ])
     os.replace(tmp, out)
     return out
 

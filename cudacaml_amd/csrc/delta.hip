@@ -1,0 +1,190 @@
+// Gated delta rule: the entry points of cchip_operators.h, their checks, and
+// where a call's buffers lie in `saved` and the workspace.
+
+#include "delta.hpp"
+
+#include <cmath>
+
+using namespace cchip;
+using namespace cchip::op;
+
+namespace {
+
+// Up to this many tokens a sequence the recurrence runs token by token.
+constexpr int64_t kStepTokens = 8;
+
+struct Layout {
+  int64_t slots, slot_heads;
+  size_t record, record_back, states, us;  // bytes, all slots and heads; states: [key_dim][value_dim], us: [64][value_dim]
+};
+
+size_t up16(size_t n) { return (n + 15) / 16 * 16; }
+
+void check_op(const cchip_gated_delta *op) {
+  if (!op) throw InvalidArgument("gated delta: no descriptor");
+  if (op->dtype != CCHIP_F32 && op->dtype != CCHIP_BF16 && op->dtype != CCHIP_F16)
+    throw InvalidArgument(strf("gated delta: dtype %d is not f32, bf16 or f16", op->dtype));
+  if (op->batch < 0 || op->tokens < 0 || op->sequences < 0 || op->tokens > (int64_t(1) << 31) - 64)
+    throw InvalidArgument("gated delta: batch, tokens and sequences are not negative and tokens below 2^31 - 64");
+  if (op->sequences > 0 && op->batch != 1) throw InvalidArgument("gated delta: packed sequences have a batch of 1");
+  if (op->key_heads < 1 || op->value_heads < 1 || op->value_heads % op->key_heads)
+    throw InvalidArgument(strf("gated delta: %d value heads are not a multiple of %d key heads", op->value_heads, op->key_heads));
+  if (op->key_dim < 1 || op->key_dim > 128) throw InvalidArgument(strf("gated delta: key_dim %d is not in 1 .. 128", op->key_dim));
+  if (op->value_dim < 1 || op->value_dim > 4096)
+    throw InvalidArgument(strf("gated delta: value_dim %d is not in 1 .. 4096", op->value_dim));
+  if (!std::isfinite(op->scale)) throw InvalidArgument("gated delta: scale is not finite");
+}
+
+int64_t count_sequences(const cchip_gated_delta &op) { return op.sequences ? op.sequences : op.batch; }
+
+Layout layout_of(const cchip_gated_delta &op) {
+  Layout p;
+  // batch and sequences below 2^31, so nothing here overflows
+  if (op.batch >= (int64_t(1) << 31) || op.sequences >= (int64_t(1) << 31)) throw InvalidArgument("gated delta: too many sequences");
+  p.slots = op.sequences ? op.tokens / kChunk + op.sequences : op.batch * ((op.tokens + kChunk - 1) / kChunk);
+  p.slot_heads = p.slots * op.value_heads;
+  const int64_t blocks = (op.value_dim + 15) / 16;
+  if (p.slots > INT32_MAX || p.slot_heads > INT32_MAX || (count_sequences(op) * op.value_heads + 8) * blocks > INT32_MAX)
+    throw InvalidArgument("gated delta: more chunks, heads and value columns than a launch can have");
+  with_mode(op, [&](auto m) {
+    typedef decltype(m) M;
+    p.record = up16(size_t(p.slot_heads) * record_bytes<M>(false));
+    p.record_back = up16(size_t(p.slot_heads) * record_bytes<M>(true));
+    p.states = up16(size_t(p.slot_heads) * op.key_dim * op.value_dim * sizeof(typename M::Saved));
+    p.us = up16(size_t(p.slot_heads) * kChunk * op.value_dim * sizeof(typename M::Saved));
+  });
+  return p;
+}
+
+bool steps(const cchip_gated_delta &op, const cchip_gated_delta_io &io) {
+  return !op.sequences && !io.saved && op.tokens <= kStepTokens;
+}
+
+int element_size(const cchip_gated_delta &op) { return op.dtype == CCHIP_F32 ? 4 : 2; }
+
+Heads heads_of(const cchip_gated_delta &op, const cchip_heads &x, const char *name, bool written, int heads, int dim) {
+  if (op.batch * op.tokens == 0) return {static_cast<char *>(x.data), x.batch, x.token, x.head};
+  if (!x.data) throw InvalidArgument(strf("gated delta: no %s", name));
+  if (reinterpret_cast<uintptr_t>(x.data) % element_size(op))
+    throw InvalidArgument(strf("gated delta: %s is not aligned to its elements", name));
+  if (written && ((op.batch > 1 && x.batch == 0) || (op.tokens > 1 && x.token == 0) || (heads > 1 && std::llabs(x.head) < dim)))
+    throw InvalidArgument(strf("gated delta: elements of %s overlap", name));
+  return {static_cast<char *>(x.data), x.batch, x.token, x.head};
+}
+
+bool vector_rows(const cchip_gated_delta &op, const Heads &x, int dim) {
+  const int n = 16 / element_size(op);
+  return aligned16(x.p) && x.b % n == 0 && x.t % n == 0 && x.h % n == 0 && dim % 8 == 0;
+}
+
+DeltaArgs args_of(const cchip_gated_delta &op, const cchip_gated_delta_io &io, bool back) {
+  DeltaArgs a = {};
+  const int hk = op.key_heads, hv = op.value_heads, dk = op.key_dim, dv = op.value_dim;
+  a.q = heads_of(op, io.q, "q", false, hk, dk);
+  a.k = heads_of(op, io.k, "k", false, hk, dk);
+  a.v = heads_of(op, io.v, "v", false, hv, dv);
+  a.g = heads_of(op, io.g, "g", false, hv, 1);
+  a.beta = heads_of(op, io.beta, "beta", false, hv, 1);
+  if (op.sequences ? !io.offsets : io.offsets != nullptr)
+    throw InvalidArgument(op.sequences ? "gated delta: packed sequences need offsets" : "gated delta: offsets without packed sequences");
+  if (!op.states && (io.state || io.state_out || io.dstate || io.dstate_out))
+    throw InvalidArgument("gated delta: a state for an operator made without states");
+  a.vec_qk = vector_rows(op, a.q, dk) && vector_rows(op, a.k, dk);
+  a.vec_v = vector_rows(op, a.v, dv);
+  if (back) {
+    if (!io.saved) throw InvalidArgument("gated delta: the backward pass needs what the forward pass saved");
+    a.d_o = heads_of(op, io.d_o, "the gradient of o", false, hv, dv);
+    a.gq = heads_of(op, io.dq, "dq", true, hk, dk);
+    a.gk = heads_of(op, io.dk, "dk", true, hk, dk);
+    a.gv = heads_of(op, io.dv, "dv", true, hv, dv);
+    a.gg = heads_of(op, io.dg, "dg", true, hv, 1);
+    a.gbeta = heads_of(op, io.dbeta, "dbeta", true, hv, 1);
+    a.vec_v = a.vec_v && vector_rows(op, a.d_o, dv);
+    a.dstate_out = io.dstate_out;
+    a.dstate = io.dstate;
+  } else {
+    a.o = heads_of(op, io.o, "o", true, hv, dv);
+    a.state = io.state;
+    a.state_out = io.state_out;
+  }
+  if (!aligned16(io.saved)) throw InvalidArgument("gated delta: saved is not aligned to 16 bytes");
+  a.offsets = io.offsets;
+  a.tokens = op.tokens;
+  a.sequences = count_sequences(op);
+  a.chunks = int((op.tokens + kChunk - 1) / kChunk);
+  a.hk = hk;
+  a.hv = hv;
+  a.dk = dk;
+  a.dv = dv;
+  a.scale = op.scale;
+  return a;
+}
+
+void check_workspace(const void *workspace, size_t have, size_t need) {
+  if (have < need || (need && !workspace) || !aligned16(workspace))
+    throw InvalidArgument(strf("gated delta: the workspace needs %zu bytes aligned to 16, has %zu", need, workspace ? have : 0));
+}
+
+size_t workspace_bytes_of(const cchip_gated_delta &op, const Layout &p) {
+  (void)op;
+  return std::max(p.record, p.states + p.us);
+}
+
+void lay_out(DeltaArgs &a, const Layout &p, char *saved) {
+  a.records = saved;
+  a.states = saved + p.record_back;
+  a.us = a.states + p.states;
+}
+
+}  // namespace
+
+extern "C" {
+
+int cchip_gated_delta_sizes(const cchip_gated_delta *op, size_t *workspace, size_t *saved) {
+  return guarded([&] {
+    check_op(op);
+    const Layout p = layout_of(*op);
+    if (workspace) *workspace = workspace_bytes_of(*op, p);
+    if (saved) *saved = p.record_back + p.states + p.us;
+  });
+}
+
+int cchip_gated_delta_forward(const cchip_gated_delta *op, const cchip_gated_delta_io *io, void *workspace,
+                              size_t workspace_bytes, void *stream) {
+  return guarded([&] {
+    check_op(op);
+    if (!io) throw InvalidArgument("gated delta: no tensors");
+    const Layout p = layout_of(*op);
+    DeltaArgs a = args_of(*op, *io, false);
+    a.slots = p.slots;
+    if (a.sequences == 0) return;
+    if (steps(*op, *io)) return delta_step_launch(*op, a, (hipStream_t)stream);
+    if (io->saved) {
+      lay_out(a, p, static_cast<char *>(io->saved));
+    } else {
+      check_workspace(workspace, workspace_bytes, p.record);
+      a.records = static_cast<char *>(workspace);
+    }
+    if (p.slots) delta_chunk_launch(*op, a, io->saved != nullptr, (hipStream_t)stream);
+    delta_forward_launch(*op, a, io->saved != nullptr, (hipStream_t)stream);
+  });
+}
+
+int cchip_gated_delta_backward(const cchip_gated_delta *op, const cchip_gated_delta_io *io, void *workspace,
+                               size_t workspace_bytes, void *stream) {
+  return guarded([&] {
+    check_op(op);
+    if (!io) throw InvalidArgument("gated delta: no tensors");
+    const Layout p = layout_of(*op);
+    DeltaArgs a = args_of(*op, *io, true);
+    a.slots = p.slots;
+    if (a.sequences == 0) return;
+    lay_out(a, p, static_cast<char *>(io->saved));
+    check_workspace(workspace, workspace_bytes, p.states + p.us);
+    a.grads = static_cast<char *>(workspace);
+    a.ys = a.grads + p.states;
+    delta_backward_launch(*op, a, (hipStream_t)stream);
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,209 @@
+// The norm block: entry points, checks, and the sum over workgroups that
+// ends the parameters' gradients.
+
+#include "norm_block.hpp"
+
+#include <cmath>
+
+namespace cchip {
+namespace op {
+
+extern template void norm_forward_launch<bf16>(const NormArgs &, hipStream_t);
+extern template void norm_forward_launch<f16>(const NormArgs &, hipStream_t);
+extern template void norm_forward_launch<float>(const NormArgs &, hipStream_t);
+extern template void norm_backward_launch<bf16>(const NormArgs &, bool, int, hipStream_t);
+extern template void norm_backward_launch<f16>(const NormArgs &, bool, int, hipStream_t);
+extern template void norm_backward_launch<float>(const NormArgs &, bool, int, hipStream_t);
+
+namespace {
+
+struct ColumnArgs {
+  const float *partial;
+  void *to[kParams];
+  int groups, sums, width;
+  bool f32;
+};
+
+// 32 columns of one parameter a workgroup; 8 threads a column sum every 8th
+// workgroup's share, and thread 0 those 8, in order.
+template <typename T>
+__global__ __launch_bounds__(256) void norm_columns(const ColumnArgs a) {
+  __shared__ float part[8][33];
+  const int col = threadIdx.x % 32, turn = threadIdx.x / 32, s = blockIdx.y;
+  const int c = int(blockIdx.x) * 32 + col;
+  float q = 0.0f;
+  if (c < a.width && a.to[s])
+    for (int g = turn; g < a.groups; g += 8) q += a.partial[(int64_t(g) * a.sums + s) * a.width + c];
+  part[turn][col] = q;
+  __syncthreads();
+  if (turn || c >= a.width || !a.to[s]) return;
+  float x = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; i++) x += part[i][col];
+  if (a.f32) static_cast<float *>(a.to[s])[c] = x;
+  else static_cast<T *>(a.to[s])[c] = T(x);
+}
+
+void check_op(const cchip_norm_block *op) {
+  const char *who = "norm block";
+  if (!op) throw InvalidArgument("norm block: no descriptor");
+  check_rows_type(who, op->dtype);
+  if (op->weight_dtype != op->dtype && op->weight_dtype != CCHIP_F32)
+    throw InvalidArgument("norm block: parameters are of the operator's dtype or f32");
+  if (op->rows < 0 || op->rows >= (int64_t(1) << 32)) throw InvalidArgument("norm block: rows are below 2^32");
+  if (op->width < 1 || op->width > 32768)
+    throw InvalidArgument(strf("norm block: width %lld is not in 1 .. 32768", (long long)op->width));
+  for (int kind : {op->post, op->pre})
+    if (kind != CCHIP_NORM_NONE && kind != CCHIP_NORM_RMS && kind != CCHIP_NORM_LAYER)
+      throw InvalidArgument(strf("norm block: unknown norm %d", kind));
+  if (op->gate != CCHIP_GATE_NONE && op->gate != CCHIP_GATE_SIGMOID && op->gate != CCHIP_GATE_SILU)
+    throw InvalidArgument(strf("norm block: unknown gate %d", op->gate));
+  if (!std::isfinite(op->scale) || !(op->eps >= 0.0f) || !std::isfinite(op->eps))
+    throw InvalidArgument("norm block: scale is finite and eps finite and not negative");
+}
+
+NormArgs args_of(const cchip_norm_block &op, const cchip_drop *drop, const cchip_norm_params *params) {
+  NormArgs a = {};
+  a.rows = uint32_t(op.rows);
+  a.width = int(op.width);
+  a.post = op.post;
+  a.pre = op.pre;
+  a.act = op.gate;
+  a.scale = op.scale;
+  a.eps = op.eps;
+  a.weights_f32 = op.weight_dtype == CCHIP_F32;
+  a.drop = drop_of(drop);
+  if (params) {
+    a.post_weight = params->post_weight;
+    a.post_bias = params->post_bias;
+    a.channel_scale = params->channel_scale;
+    a.pre_weight = params->pre_weight;
+    a.pre_bias = params->pre_bias;
+  }
+  for (const void *p : {a.post_weight, a.post_bias, a.channel_scale, a.pre_weight, a.pre_bias})
+    if (reinterpret_cast<uintptr_t>(p) % (a.weights_f32 ? 4 : 2))
+      throw InvalidArgument("norm block: a parameter is not aligned to its elements");
+  if (op.post == CCHIP_NORM_NONE && (a.post_weight || a.post_bias))
+    throw InvalidArgument("norm block: parameters of a post norm that there is not");
+  if (op.pre == CCHIP_NORM_NONE && (a.pre_weight || a.pre_bias))
+    throw InvalidArgument("norm block: parameters of a pre norm that there is not");
+  return a;
+}
+
+// Workgroups of a backward pass: enough to fill the chip four times over,
+// and at least 4 rows each so that the sums left over stay small beside the
+// rows.
+int groups_of(const cchip_norm_block &op) {
+  const int64_t at_a_time = rows_at_a_time(int(op.width));
+  const int64_t sets = (op.rows + at_a_time - 1) / at_a_time;
+  return int(std::min<int64_t>(kMostGroups, (sets + 3) / 4));
+}
+
+}  // namespace
+}  // namespace op
+}  // namespace cchip
+
+using namespace cchip;
+using namespace cchip::op;
+
+extern "C" {
+
+int cchip_norm_block_forward(const cchip_norm_block *op, const cchip_drop *drop, const cchip_norm_params *params,
+                             cchip_rows y, cchip_rows gate, cchip_rows residual, cchip_rows h, cchip_rows n,
+                             void *stream) {
+  return guarded([&] {
+    const char *who = "norm block";
+    check_op(op);
+    NormArgs a = args_of(*op, drop, params);
+    const bool pre = op->pre != CCHIP_NORM_NONE, gated = op->gate != CCHIP_GATE_NONE;
+    if (op->rows == 0) return;
+    if (pre != (n.data != nullptr)) throw InvalidArgument("norm block: n is given if and only if there is a pre norm");
+    if (gated != (gate.data != nullptr)) throw InvalidArgument("norm block: a gate is given if and only if the operator has one");
+    a.y = rows_of(who, "y", op->dtype, op->rows, op->width, y, false, true);
+    a.gate = rows_of(who, "gate", op->dtype, op->rows, op->width, gate, false, false);
+    a.residual = rows_of(who, "residual", op->dtype, op->rows, op->width, residual, false, false);
+    a.h = rows_of(who, "h", op->dtype, op->rows, op->width, h, true, true);
+    a.n = rows_of(who, "n", op->dtype, op->rows, op->width, n, true, false);
+    a.vec = true;
+    for (const Rows *r : {&a.y, &a.gate, &a.residual, &a.h, &a.n}) a.vec = a.vec && vector_rows(*r, op->dtype);
+    with_rows_type(op->dtype, [&](auto t) { norm_forward_launch<decltype(t)>(a, (hipStream_t)stream); });
+    check_launch(who);
+  });
+}
+
+int cchip_norm_block_workspace(const cchip_norm_block *op, size_t *bytes) {
+  return guarded([&] {
+    check_op(op);
+    if (bytes) *bytes = size_t(groups_of(*op)) * kParams * op->width * sizeof(float);
+  });
+}
+
+int cchip_norm_block_backward(const cchip_norm_block *op, const cchip_drop *drop, const cchip_norm_params *params,
+                              const cchip_norm_grads *grads, cchip_rows y, cchip_rows gate, cchip_rows h,
+                              cchip_rows dh, cchip_rows dn, cchip_rows dy, cchip_rows dgate, cchip_rows dresidual,
+                              void *workspace, size_t workspace_bytes, void *stream) {
+  return guarded([&] {
+    const char *who = "norm block";
+    check_op(op);
+    NormArgs a = args_of(*op, drop, params);
+    const bool pre = op->pre != CCHIP_NORM_NONE, gated = op->gate != CCHIP_GATE_NONE;
+    ColumnArgs c = {};
+    if (grads) {
+      c.to[kPostWeight] = grads->post_weight;
+      c.to[kChannelScale] = grads->channel_scale;
+      c.to[kPreWeight] = grads->pre_weight;
+      c.to[kPostBias] = grads->post_bias;
+      c.to[kPreBias] = grads->pre_bias;
+    }
+    bool any = false;
+    for (void *p : c.to) {
+      any = any || p;
+      if (reinterpret_cast<uintptr_t>(p) % (a.weights_f32 ? 4 : 2))
+        throw InvalidArgument("norm block: a parameter's gradient is not aligned to its elements");
+    }
+    if ((c.to[kPostWeight] || c.to[kPostBias]) && op->post == CCHIP_NORM_NONE)
+      throw InvalidArgument("norm block: gradients of a post norm that there is not");
+    if ((c.to[kPreWeight] || c.to[kPreBias]) && !pre) throw InvalidArgument("norm block: gradients of a pre norm that there is not");
+    const bool bias = c.to[kPostBias] || c.to[kPreBias];
+    if (op->rows > 0) {
+      if (pre != (dn.data != nullptr) || pre != (h.data != nullptr))
+        throw InvalidArgument("norm block: h and dn are given if and only if there is a pre norm");
+      if (gated != (gate.data != nullptr)) throw InvalidArgument("norm block: a gate is given if and only if the operator has one");
+      if (!gated && dgate.data) throw InvalidArgument("norm block: the gradient of a gate that there is not");
+      a.y = rows_of(who, "y", op->dtype, op->rows, op->width, y, false, true);
+      a.gate = rows_of(who, "gate", op->dtype, op->rows, op->width, gate, false, false);
+      a.h = rows_of(who, "h", op->dtype, op->rows, op->width, h, false, false);
+      a.dh = rows_of(who, "dh", op->dtype, op->rows, op->width, dh, false, true);
+      a.dn = rows_of(who, "dn", op->dtype, op->rows, op->width, dn, false, false);
+      a.dy = rows_of(who, "dy", op->dtype, op->rows, op->width, dy, true, true);
+      a.dgate = rows_of(who, "dgate", op->dtype, op->rows, op->width, dgate, true, false);
+      a.dresidual = rows_of(who, "dresidual", op->dtype, op->rows, op->width, dresidual, true, false);
+      a.vec = true;
+      for (const Rows *r : {&a.y, &a.gate, &a.h, &a.dh, &a.dn, &a.dy, &a.dgate, &a.dresidual})
+        a.vec = a.vec && vector_rows(*r, op->dtype);
+    }
+    const int groups = groups_of(*op);
+    if (any) {
+      const size_t need = size_t(groups) * (bias ? 5 : 3) * op->width * sizeof(float);
+      if (workspace_bytes < need || (need && !workspace) || reinterpret_cast<uintptr_t>(workspace) % 4)
+        throw InvalidArgument(strf("norm block: the workspace needs %zu bytes aligned to 4, has %zu", need, workspace ? workspace_bytes : 0));
+      a.partial = static_cast<float *>(workspace);
+    }
+    if (groups)
+      with_rows_type(op->dtype, [&](auto t) { norm_backward_launch<decltype(t)>(a, bias, groups, (hipStream_t)stream); });
+    check_launch(who);
+    if (!any) return;
+    c.partial = a.partial;
+    c.groups = groups;
+    c.sums = bias ? 5 : 3;
+    c.width = a.width;
+    c.f32 = a.weights_f32;
+    with_rows_type(op->dtype, [&](auto t) {
+      typedef decltype(t) T;
+      hipLaunchKernelGGL((norm_columns<T>), dim3((a.width + 31) / 32, c.sums), dim3(256), 0, (hipStream_t)stream, c);
+    });
+    check_launch(who);
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,361 @@
+// The norm block's kernels (cchip_operators.h states what they compute). One
+// element type is instantiated a file: norm_block_bf16.hip and the like.
+#pragma once
+
+#include "rows.hpp"
+
+namespace cchip {
+namespace op {
+
+struct NormArgs {
+  Rows y, gate, residual, h, n;                 // forward
+  Rows dh, dn, dy, dgate, dresidual;            // backward (reads y, gate, h)
+  const void *post_weight, *post_bias, *channel_scale, *pre_weight, *pre_bias;
+  float *partial;  // backward: [workgroup][parameter][width]
+  uint32_t rows;
+  int width, post, pre, act;
+  bool weights_f32, vec;
+  float scale, eps;
+  Drop drop;
+};
+
+// Row sums over LANES threads: every one gets the sum. `at` is a scratch of
+// a float a wave and set, two sets, used in turn.
+template <int LANES>
+struct RowSum {
+  float (*at)[LANES > 64 ? LANES / 64 : 1];
+  int set;
+  __device__ __forceinline__ float operator()(float x) {
+    if (LANES == 16) return sum16(x);
+    x = sum64(x);
+    if (LANES == 64) return x;
+    const int w = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) at[set][w] = x;
+    __syncthreads();
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < (LANES > 64 ? LANES / 64 : 1); i++) s += at[set][i];
+    set ^= 1;
+    return s;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void load_params(float (&w)[8], const void *p, bool f32, int at, int n, float none) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) w[i] = none;
+  if (!p) return;
+#pragma unroll
+  for (int i = 0; i < 8; i++)
+    if (i < n) w[i] = f32 ? static_cast<const float *>(p)[at + i] : float(static_cast<const T *>(p)[at + i]);
+}
+
+// x becomes (x - mean) / sqrt(mean of squares + eps); returns what it was
+// multiplied by. Sums of squares are of centred values: nothing cancels.
+template <int LANES, int V>
+__device__ __forceinline__ float normalise(float (&x)[V][8], int kind, float inv_width, float eps, RowSum<LANES> &sum,
+                                           int lane, int width) {
+  if (kind == CCHIP_NORM_LAYER) {
+    float s = 0.0f;
+#pragma unroll
+    for (int v = 0; v < V; v++)
+#pragma unroll
+      for (int i = 0; i < 8; i++) s += x[v][i];
+    const float mean = sum(s) * inv_width;
+#pragma unroll
+    for (int v = 0; v < V; v++)
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[v][i] = (v * LANES + lane) * 8 + i < width ? x[v][i] - mean : 0.0f;
+  }
+  float q = 0.0f;
+#pragma unroll
+  for (int v = 0; v < V; v++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) q += x[v][i] * x[v][i];
+  const float inv = 1.0f / sqrtf(sum(q) * inv_width + eps);
+#pragma unroll
+  for (int v = 0; v < V; v++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[v][i] *= inv;
+  return inv;
+}
+
+__device__ __forceinline__ float sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }
+
+// A row to LANES threads, 8 neighbouring columns a thread and step, held in
+// registers from the one read of it to the writes.
+template <typename T, int LANES, int V>
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_forward(const NormArgs a) {
+  constexpr int kRows = LANES < 256 ? 256 / LANES : 1;
+  __shared__ float scratch[2][LANES > 64 ? LANES / 64 : 1];
+  RowSum<LANES> sum = {scratch, 0};
+  const int lane = threadIdx.x % LANES;
+  const int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / LANES;
+  if (row >= a.rows) return;
+  const float inv_width = 1.0f / float(a.width);
+
+  Raw8<T> y[V], z[V], x[V];
+  int n[V];
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    const int c = (v * LANES + lane) * 8;
+    n[v] = a.width - c < 0 ? 0 : a.width - c > 8 ? 8 : a.width - c;
+    y[v] = load8<T>(row_at<T>(a.y, row) + c, n[v], a.vec);
+  }
+  if (a.act != CCHIP_GATE_NONE)
+#pragma unroll
+    for (int v = 0; v < V; v++) z[v] = load8<T>(row_at<T>(a.gate, row) + (v * LANES + lane) * 8, n[v], a.vec);
+  if (a.residual.p)
+#pragma unroll
+    for (int v = 0; v < V; v++) x[v] = load8<T>(row_at<T>(a.residual, row) + (v * LANES + lane) * 8, n[v], a.vec);
+
+  float h[V][8];
+#pragma unroll
+  for (int v = 0; v < V; v++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) h[v][i] = float(y[v].x[i]);
+  if (a.post != CCHIP_NORM_NONE) normalise<LANES, V>(h, a.post, inv_width, a.eps, sum, lane, a.width);
+  const float up = a.scale * a.drop.up;
+  const uint64_t offset = a.drop.bar ? offset_of(a.drop) : 0;
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    const int g = v * LANES + lane, c = g * 8;
+    float w[8], b[8], t[8];
+    load_params<T>(w, a.post_weight, a.weights_f32, c, n[v], 1.0f);
+    load_params<T>(b, a.post_bias, a.weights_f32, c, n[v], 0.0f);
+    load_params<T>(t, a.channel_scale, a.weights_f32, c, n[v], 1.0f);
+    const uint32_t bits = a.drop.bar && n[v] ? keep_bits(a.drop, offset, uint32_t(row), g) : 0xFFu;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      float e = h[v][i] * w[i] + b[i];
+      if (a.act != CCHIP_GATE_NONE) {
+        const float zi = float(z[v].x[i]), s = sigmoid(zi);
+        e *= a.act == CCHIP_GATE_SILU ? zi * s : s;
+      }
+      e = bits >> i & 1 ? e * up * t[i] : 0.0f;
+      if (a.residual.p) e += float(x[v].x[i]);
+      h[v][i] = i < n[v] ? e : 0.0f;
+    }
+    store8<T>(row_at<T>(a.h, row) + c, h[v], n[v], a.vec);
+  }
+  if (a.pre == CCHIP_NORM_NONE) return;
+  normalise<LANES, V>(h, a.pre, inv_width, a.eps, sum, lane, a.width);
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    const int c = (v * LANES + lane) * 8;
+    float w[8], b[8];
+    load_params<T>(w, a.pre_weight, a.weights_f32, c, n[v], 1.0f);
+    load_params<T>(b, a.pre_bias, a.weights_f32, c, n[v], 0.0f);
+#pragma unroll
+    for (int i = 0; i < 8; i++) h[v][i] = h[v][i] * w[i] + b[i];
+    store8<T>(row_at<T>(a.n, row) + c, h[v], n[v], a.vec);
+  }
+}
+
+// d becomes the gradient of what `normalise` read, from that of what it
+// gave: (d - mean(d) - xhat mean(d xhat)) inv, the first mean of a layer norm.
+template <int LANES, int V>
+__device__ __forceinline__ void normalise_back(float (&d)[V][8], const float (&xhat)[V][8], int kind, float inv,
+                                               float inv_width, RowSum<LANES> &sum) {
+  float p = 0.0f, q = 0.0f;
+#pragma unroll
+  for (int v = 0; v < V; v++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      p += d[v][i] * xhat[v][i];
+      q += d[v][i];
+    }
+  p = sum(p) * inv_width;
+  q = kind == CCHIP_NORM_LAYER ? sum(q) * inv_width : 0.0f;
+#pragma unroll
+  for (int v = 0; v < V; v++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) d[v][i] = (d[v][i] - xhat[v][i] * p - q) * inv;
+}
+
+// The parameters' gradients in the order of their sums; without Bias the
+// second and the last are not made.
+enum Param { kPostWeight, kChannelScale, kPreWeight, kPostBias, kPreBias, kParams };
+
+// As norm_forward, a workgroup taking every gridDim-th set of rows so that it
+// can sum the parameters' gradients of its columns in registers; they are
+// left in `partial` and added up by norm_columns.
+template <typename T, int LANES, int V, bool Gate, bool Pre, bool Bias>
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_backward(const NormArgs a) {
+  constexpr int kRows = LANES < 256 ? 256 / LANES : 1, kThreads = LANES < 256 ? 256 : LANES;
+  constexpr int kSums = Bias ? 5 : 3;
+  __shared__ float scratch[2][LANES > 64 ? LANES / 64 : 1];
+  RowSum<LANES> sum = {scratch, 0};
+  const int lane = threadIdx.x % LANES;
+  const float inv_width = 1.0f / float(a.width);
+  const float up = a.scale * a.drop.up;
+  const uint64_t offset = a.drop.bar ? offset_of(a.drop) : 0;
+  float acc[kSums][V][8] = {};
+  int n[V];
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    const int c = (v * LANES + lane) * 8;
+    n[v] = a.width - c < 0 ? 0 : a.width - c > 8 ? 8 : a.width - c;
+  }
+  for (int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / LANES; row < a.rows; row += int64_t(gridDim.x) * kRows) {
+    Raw8<T> ry[V], rz[V], rh[V], rdh[V], rdn[V];
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      const int c = (v * LANES + lane) * 8;
+      if (Pre) rh[v] = load8<T>(row_at<T>(a.h, row) + c, n[v], a.vec);
+      if (Pre) rdn[v] = load8<T>(row_at<T>(a.dn, row) + c, n[v], a.vec);
+      rdh[v] = load8<T>(row_at<T>(a.dh, row) + c, n[v], a.vec);
+      ry[v] = load8<T>(row_at<T>(a.y, row) + c, n[v], a.vec);
+      if (Gate) rz[v] = load8<T>(row_at<T>(a.gate, row) + c, n[v], a.vec);
+    }
+    float d[V][8], x[V][8];
+    if (Pre) {
+#pragma unroll
+      for (int v = 0; v < V; v++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[v][i] = float(rh[v].x[i]);
+      const float inv = normalise<LANES, V>(x, a.pre, inv_width, a.eps, sum, lane, a.width);
+#pragma unroll
+      for (int v = 0; v < V; v++) {
+        float w[8];
+        load_params<T>(w, a.pre_weight, a.weights_f32, (v * LANES + lane) * 8, n[v], 1.0f);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float dn = float(rdn[v].x[i]);
+          acc[kPreWeight][v][i] += dn * x[v][i];
+          if (Bias) acc[kPreBias][v][i] += dn;
+          d[v][i] = i < n[v] ? dn * w[i] : 0.0f;
+        }
+      }
+      normalise_back<LANES, V>(d, x, a.pre, inv, inv_width, sum);
+#pragma unroll
+      for (int v = 0; v < V; v++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) d[v][i] += float(rdh[v].x[i]);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; v++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) d[v][i] = float(rdh[v].x[i]);
+    }
+    if (a.dresidual.p)
+#pragma unroll
+      for (int v = 0; v < V; v++) store8<T>(row_at<T>(a.dresidual, row) + (v * LANES + lane) * 8, d[v], n[v], a.vec);
+
+#pragma unroll
+    for (int v = 0; v < V; v++)
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[v][i] = float(ry[v].x[i]);
+    float inv = 1.0f;
+    if (a.post != CCHIP_NORM_NONE) inv = normalise<LANES, V>(x, a.post, inv_width, a.eps, sum, lane, a.width);
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      const int g = v * LANES + lane, c = g * 8;
+      float w[8], b[8], t[8], dz[8];
+      load_params<T>(w, a.post_weight, a.weights_f32, c, n[v], 1.0f);
+      load_params<T>(b, a.post_bias, a.weights_f32, c, n[v], 0.0f);
+      load_params<T>(t, a.channel_scale, a.weights_f32, c, n[v], 1.0f);
+      const uint32_t bits = a.drop.bar && n[v] ? keep_bits(a.drop, offset, uint32_t(row), g) : 0xFFu;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const bool keep = bits >> i & 1 && i < n[v];
+        const float e = x[v][i] * w[i] + b[i];
+        float act = 1.0f, slope = 0.0f;
+        if (Gate) {
+          const float z = float(rz[v].x[i]), s = sigmoid(z);
+          act = a.act == CCHIP_GATE_SILU ? z * s : s;
+          slope = a.act == CCHIP_GATE_SILU ? s * (1.0f + z * (1.0f - s)) : s * (1.0f - s);
+        }
+        const float du = keep ? d[v][i] * up : 0.0f;
+        acc[kChannelScale][v][i] += keep ? du * e * act : 0.0f;
+        const float db = du * t[i], da = db * act;
+        if (Gate) dz[i] = keep ? db * e * slope : 0.0f;
+        acc[kPostWeight][v][i] += da * x[v][i];
+        if (Bias) acc[kPostBias][v][i] += da;
+        d[v][i] = da * w[i];
+      }
+      if (Gate && a.dgate.p) store8<T>(row_at<T>(a.dgate, row) + c, dz, n[v], a.vec);
+    }
+    if (a.post != CCHIP_NORM_NONE) normalise_back<LANES, V>(d, x, a.post, inv, inv_width, sum);
+#pragma unroll
+    for (int v = 0; v < V; v++) store8<T>(row_at<T>(a.dy, row) + (v * LANES + lane) * 8, d[v], n[v], a.vec);
+  }
+  if (!a.partial) return;
+  if (kRows > 1) {
+    // the workgroup's rows side by side: sum them in the order of the rows
+    __shared__ float side[kThreads * 8];
+#pragma unroll
+    for (int s = 0; s < kSums; s++)
+#pragma unroll
+      for (int v = 0; v < V; v++) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; i++) side[threadIdx.x * 8 + i] = acc[s][v][i];
+        __syncthreads();
+        for (int i = threadIdx.x; i < LANES * 8; i += kThreads) {
+          float q = 0.0f;
+          for (int r = 0; r < kRows; r++) q += side[r * LANES * 8 + i];
+          const int c = v * LANES * 8 + i;
+          if (c < a.width) a.partial[(int64_t(blockIdx.x) * kSums + s) * a.width + c] = q;
+        }
+      }
+  } else {
+#pragma unroll
+    for (int s = 0; s < kSums; s++)
+#pragma unroll
+      for (int v = 0; v < V; v++)
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          if (i < n[v]) a.partial[(int64_t(blockIdx.x) * kSums + s) * a.width + (v * LANES + lane) * 8 + i] = acc[s][v][i];
+  }
+}
+
+constexpr int kMostGroups = 1024;  // workgroups of a backward pass
+
+template <typename T>
+void norm_forward_launch(const NormArgs &a, hipStream_t stream);
+template <typename T>
+void norm_backward_launch(const NormArgs &a, bool bias, int groups, hipStream_t stream);
+
+// Rows a workgroup takes at a time for a width.
+inline int rows_at_a_time(int width) { return width <= 128 ? 16 : width <= 512 ? 4 : 1; }
+
+// Calls f(lanes, steps) with the smallest shape that holds a row: few lanes
+// for short rows, so that none idles, and no more than 16 columns a thread
+// up to 16384, so that a backward pass's five sums stay in registers.
+template <typename F>
+void with_shape(int width, F &&f) {
+  if (width <= 128) f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
+  else if (width <= 512) f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
+  else if (width <= 2048) f(std::integral_constant<int, 256>(), std::integral_constant<int, 1>());
+  else if (width <= 4096) f(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
+  else if (width <= 8192) f(std::integral_constant<int, 512>(), std::integral_constant<int, 2>());
+  else if (width <= 16384) f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
+  else f(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
+}
+
+#define CCHIP_NORM_BLOCK_LAUNCHERS(T)                                                                              \
+  template <>                                                                                                      \
+  void norm_forward_launch<T>(const NormArgs &a, hipStream_t stream) {                                             \
+    with_shape(a.width, [&](auto lanes, auto steps) {                                                              \
+      constexpr int L = decltype(lanes)::value, V = decltype(steps)::value;                                        \
+      constexpr int kRows = L < 256 ? 256 / L : 1;                                                                 \
+      hipLaunchKernelGGL((norm_forward<T, L, V>), dim3(unsigned((int64_t(a.rows) + kRows - 1) / kRows)),           \
+                         dim3(L < 256 ? 256 : L), 0, stream, a);                                                   \
+    });                                                                                                            \
+  }                                                                                                                \
+  template <>                                                                                                      \
+  void norm_backward_launch<T>(const NormArgs &a, bool bias, int groups, hipStream_t stream) {                     \
+    with_shape(a.width, [&](auto lanes, auto steps) {                                                              \
+      constexpr int L = decltype(lanes)::value, V = decltype(steps)::value;                                        \
+      const bool gate = a.act != CCHIP_GATE_NONE, pre = a.pre != CCHIP_NORM_NONE;                                  \
+      auto *k = gate ? (pre ? (bias ? norm_backward<T, L, V, true, true, true> : norm_backward<T, L, V, true, true, false>)      \
+                            : (bias ? norm_backward<T, L, V, true, false, true> : norm_backward<T, L, V, true, false, false>))   \
+                     : (pre ? (bias ? norm_backward<T, L, V, false, true, true> : norm_backward<T, L, V, false, true, false>)    \
+                            : (bias ? norm_backward<T, L, V, false, false, true> : norm_backward<T, L, V, false, false, false>));\
+      hipLaunchKernelGGL(k, dim3(unsigned(groups)), dim3(L < 256 ? 256 : L), 0, stream, a);                        \
+    });                                                                                                            \
+  }
+
+}  // namespace op
+}  // namespace cchip

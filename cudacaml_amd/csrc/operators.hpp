@@ -1,0 +1,209 @@
+// What the layer operators (delta*.hip, norm_block.hip, dropout.hip) share:
+// element types, raw loads at any alignment, matrix-core fragments held in
+// one to three bf16 planes, and the counter-based generator.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "internal.hpp"
+
+namespace cchip {
+namespace op {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// Eight neighbouring elements as they lie in memory. `vec`: p is aligned to
+// 16 bytes and all eight exist; otherwise the first `valid` are read one by
+// one and the rest are zero.
+template <typename T>
+struct Raw8 {
+  T x[8];
+};
+
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8(const T *p, int valid, bool vec) {
+  Raw8<T> r;
+  if (vec && valid == 8) {
+    const uint4 *s = reinterpret_cast<const uint4 *>(p);
+    uint4 *d = reinterpret_cast<uint4 *>(&r);
+#pragma unroll
+    for (int i = 0; i < int(sizeof(T) * 8 / 16); i++) d[i] = s[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) r.x[i] = i < valid ? p[i] : T(0.0f);
+  }
+  return r;
+}
+
+// x as the sum of N bf16 values, each the rounding of what the ones before
+// it leave: 8, 16 and 24 bits of x for N = 1, 2 and 3 (24 hold every f32, 11
+// every f16).
+template <int N>
+__device__ __forceinline__ void split(float x, bf16 (&out)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    out[i] = bf16(x);
+    x -= float(out[i]);
+  }
+}
+
+// A matrix-core operand of 16 rows (or columns) and 32 terms: lane l holds
+// row l % 16, terms 8 (l / 16) .. + 7, in N planes.
+template <int N>
+struct Frag {
+  bf16x8 p[N];
+};
+
+template <int N, typename T>
+__device__ __forceinline__ Frag<N> frag_of(const Raw8<T> &r) {
+  Frag<N> f;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    if constexpr (N == 1 && sizeof(T) == 2) {
+      f.p[0][i] = bf16(r.x[i]);
+    } else {
+      bf16 s[N];
+      split<N>(float(r.x[i]), s);
+#pragma unroll
+      for (int n = 0; n < N; n++) f.p[n][i] = s[n];
+    }
+  }
+  return f;
+}
+
+// Fragment of a matrix in LDS stored [row][term], rows of `ld` elements (a
+// multiple of 8), planes `plane` elements apart: one 16-byte read a plane.
+template <int N>
+__device__ __forceinline__ Frag<N> frag_row(const bf16 *m, int plane, int ld, int row0, int term0) {
+  const int l = threadIdx.x & 63;
+  const bf16 *p = m + (row0 + (l & 15)) * ld + term0 + (l >> 4) * 8;
+  Frag<N> f;
+#pragma unroll
+  for (int n = 0; n < N; n++) f.p[n] = *reinterpret_cast<const bf16x8 *>(p + n * plane);
+  return f;
+}
+
+// The same of a matrix stored [term][row]: the transposing LDS read. Of 16
+// lanes each gives the address of 4 neighbouring elements, 4 lanes to a
+// stored row; lane i gets column i of those 4 rows of 16.
+template <int N>
+__device__ __forceinline__ Frag<N> frag_col(const bf16 *m, int plane, int ld, int row0, int term0) {
+  typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+  const int l = threadIdx.x & 63;
+  const bf16 *p = m + (term0 + (l >> 4) * 8 + ((l >> 2) & 3)) * ld + row0 + (l & 3) * 4;
+  Frag<N> f;
+#pragma unroll
+  for (int n = 0; n < N; n++) {
+    union {
+      i16x4 h[2];
+      bf16x8 v;
+    } u;
+    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(p + n * plane));
+    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(p + n * plane + 4 * ld));
+    f.p[n] = u.v;
+  }
+  return f;
+}
+
+// c += a b^T over 32 terms. Planes i and j are multiplied while i + j is
+// below the larger count: the terms left out are as small as what splitting
+// dropped. Small terms first. Lane l holds rows 4 (l / 16) .. + 3 of column
+// l % 16.
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mma(f32x4 c, const Frag<NA> &a, const Frag<NB> &b) {
+  constexpr int M = NA > NB ? NA : NB;
+#pragma unroll
+  for (int s = M - 1; s >= 0; s--)
+#pragma unroll
+    for (int i = 0; i < NA; i++) {
+      const int j = s - i;
+      if (j >= 0 && j < NB) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[j], c, 0, 0, 0);
+    }
+  return c;
+}
+
+// Four rows of one column of a product into LDS, stored [column][row].
+template <int N>
+__device__ __forceinline__ void put_column(bf16 *at, int plane, const f32x4 &c) {
+  bf16x4 v[N];
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    bf16 s[N];
+    split<N>(c[r], s);
+#pragma unroll
+    for (int n = 0; n < N; n++) v[n][r] = s[n];
+  }
+#pragma unroll
+  for (int n = 0; n < N; n++) *reinterpret_cast<bf16x4 *>(at + n * plane) = v[n];
+}
+
+template <int N>
+__device__ __forceinline__ void put_frag(bf16 *at, int plane, const Frag<N> &f) {
+#pragma unroll
+  for (int n = 0; n < N; n++) *reinterpret_cast<bf16x8 *>(at + n * plane) = f.p[n];
+}
+
+// Sum over the 16 lanes of a row of lanes (every lane gets it).
+__device__ __forceinline__ float sum16(float x) {
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) x += __shfl_xor(x, d, 64);
+  return x;
+}
+
+__device__ __forceinline__ float sum64(float x) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d, 64);
+  return x;
+}
+
+// Philox-4x32-10 (Salmon, Moraes, Dror and Shaw, SC'11), the generator of
+// cudacaml_amd/rng.py: ten rounds, the key bumped after the first nine.
+__device__ __forceinline__ uint4 philox(uint4 c, uint2 k) {
+#pragma unroll
+  for (int r = 0; r < 10; r++) {
+    const uint64_t a = uint64_t(0xD2511F53u) * c.x, b = uint64_t(0xCD9E8D57u) * c.z;
+    c = make_uint4(uint32_t(b >> 32) ^ c.y ^ k.x, uint32_t(b), uint32_t(a >> 32) ^ c.w ^ k.y, uint32_t(a));
+    k.x += 0x9E3779B9u;
+    k.y += 0xBB67AE85u;
+  }
+  return c;
+}
+
+// Which of columns 8 group .. + 7 of a row dropout keeps, as bits: the
+// 16-bit halves of philox((group, row, offset), seed), low half first,
+// against `bar` = round(65536 p).
+struct Drop {
+  uint64_t seed, offset;
+  const uint64_t *step;  // device counter added to offset, or null
+  uint32_t bar;          // 0: everything is kept and nothing is drawn
+  float up;              // 65536 / (65536 - bar), 0 if nothing is kept
+};
+
+__device__ __forceinline__ uint32_t keep_bits(const Drop &d, uint64_t offset, uint32_t row, uint32_t group) {
+  const uint4 w = philox(make_uint4(group, row, uint32_t(offset), uint32_t(offset >> 32)),
+                         make_uint2(uint32_t(d.seed), uint32_t(d.seed >> 32)));
+  const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+  uint32_t bits = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    bits |= uint32_t((x[i] & 0xFFFFu) >= d.bar) << (2 * i);
+    bits |= uint32_t((x[i] >> 16) >= d.bar) << (2 * i + 1);
+  }
+  return bits;
+}
+
+// ---- host side --------------------------------------------------------------
+
+inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+inline void check_launch(const char *what) { check_hip(hipGetLastError(), what); }
+
+}  // namespace op
+}  // namespace cchip

@@ -1,0 +1,73 @@
+// Matrices of rows for the dropout and the norm block: addressing, stores,
+// dropout's parameters and the checks of arguments they share.
+#pragma once
+
+#include <cstdlib>
+
+#include "../../include/cchip_operators.h"
+#include "operators.hpp"
+
+namespace cchip {
+namespace op {
+
+struct Rows {
+  char *p;
+  int64_t row;  // elements
+};
+
+template <typename T>
+__device__ __forceinline__ T *row_at(const Rows &x, uint64_t row) {
+  return reinterpret_cast<T *>(x.p) + int64_t(row) * x.row;
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T *p, const float (&x)[8], int n, bool vec) {
+  Raw8<T> r;
+#pragma unroll
+  for (int i = 0; i < 8; i++) r.x[i] = T(x[i]);
+  if (vec && n == 8) {
+    const uint4 *s = reinterpret_cast<const uint4 *>(&r);
+    uint4 *d = reinterpret_cast<uint4 *>(p);
+#pragma unroll
+    for (int i = 0; i < int(sizeof(T) * 8 / 16); i++) d[i] = s[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (i < n) p[i] = r.x[i];
+  }
+}
+
+__device__ __forceinline__ uint64_t offset_of(const Drop &d) { return d.offset + (d.step ? *d.step : 0); }
+
+// The kernel's form of a probability and seed; null: nothing is dropped.
+Drop drop_of(const cchip_drop *d);
+
+inline void check_rows_type(const char *who, int dtype) {
+  if (dtype != CCHIP_F32 && dtype != CCHIP_BF16 && dtype != CCHIP_F16)
+    throw InvalidArgument(strf("%s: dtype %d is not f32, bf16 or f16", who, dtype));
+}
+
+inline Rows rows_of(const char *who, const char *name, int dtype, int64_t rows, int64_t cols, const cchip_rows &x,
+                    bool written, bool needed) {
+  if (!x.data) {
+    if (needed) throw InvalidArgument(strf("%s: no %s", who, name));
+    return {nullptr, 0};
+  }
+  if (reinterpret_cast<uintptr_t>(x.data) % (dtype == CCHIP_F32 ? 4 : 2))
+    throw InvalidArgument(strf("%s: %s is not aligned to its elements", who, name));
+  if (written && rows > 1 && std::llabs(x.row) < cols) throw InvalidArgument(strf("%s: rows of %s overlap", who, name));
+  return {static_cast<char *>(x.data), x.row};
+}
+
+// Whether every row begins at a multiple of 16 bytes (true of no matrix).
+inline bool vector_rows(const Rows &x, int dtype) { return aligned16(x.p) && x.row % (dtype == CCHIP_F32 ? 4 : 8) == 0; }
+
+template <typename F>
+void with_rows_type(int dtype, F &&f) {
+  if (dtype == CCHIP_F32) f(float());
+  else if (dtype == CCHIP_F16) f(f16());
+  else f(bf16());
+}
+
+}  // namespace op
+}  // namespace cchip

@@ -1,0 +1,182 @@
+/*
+ * cchip operators: layer operators of language models on device-resident
+ * data, next to the graphs of cchip_backend.h. The array DSL cannot express
+ * them: its scans carry scalars, its tensors have no 16-bit types, and a
+ * fused norm, gate, dropout and residual is several of its kernels. Like
+ * cchip_program_run_resident_noalloc every call only issues work on `stream`
+ * (NULL: the default stream), allocates nothing and may be captured into a
+ * HIP graph; synchronise the stream before reading results on the host.
+ *
+ * Status codes and cchip_last_error() are those of cchip_runtime.h: a shape,
+ * type, stride or missing buffer that an operator does not take is
+ * CCHIP_INVALID_ARGUMENT before any device work.
+ */
+#ifndef CCHIP_OPERATORS_H
+#define CCHIP_OPERATORS_H
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include "cchip_runtime.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Element types of the operators (the codes of cchip_backend.h go on). */
+#define CCHIP_F32 0
+#define CCHIP_BF16 5
+#define CCHIP_F16 6
+
+/* ---- Gated delta rule ---------------------------------------------------- */
+
+/*
+ * A linear recurrence whose state S is a key_dim x value_dim matrix, one for
+ * each sequence and value head:
+ *
+ *   u_t = beta_t (v_t - exp(g_t) S_{t-1}^T k_t)
+ *   S_t = exp(g_t) S_{t-1} + k_t u_t^T
+ *   o_t = scale S_t^T q_t
+ *
+ * q and k have key_heads heads, v and o value_heads, a multiple of it: value
+ * head h goes with key head h / (value_heads / key_heads). g and beta have
+ * value_heads values a token and, like all tensors below, the type `dtype`;
+ * states are f32, [sequence][value head][key_dim][value_dim], contiguous.
+ * With `sequences` 0 the rows of the batch are the sequences; otherwise batch
+ * is 1 and sequence i is the tokens offsets[i] .. offsets[i + 1] - 1 (i32 on
+ * the device, `sequences` + 1 values from 0 to tokens, not decreasing;
+ * values out of that range are clamped to it). A sequence may be empty: its
+ * last state is its first.
+ *
+ * `states` non-zero: sequences begin from `state` (NULL: zeros) and their
+ * last states or the gradients of their first ones are wanted; the products
+ * that make a state then keep 24 bits of f32 operands. With `states` zero,
+ * those arguments are NULL and bf16 operands are rounded to 8 bits once per
+ * 64 tokens. Sums and states are f32 either way.
+ *
+ * A NaN or infinity in a token reaches the outputs of its own sequence and
+ * value heads from the 64-token chunk it stands in onwards, in the backward
+ * pass those up to that chunk's end.
+ */
+typedef struct {
+  int dtype;
+  int64_t batch, tokens, sequences;
+  int key_heads, value_heads, key_dim, value_dim; /* key_dim <= 128 */
+  int states;
+  float scale;
+} cchip_gated_delta;
+
+/* A tensor [batch][token][head][dim]: the distances, in elements, of
+   neighbours along the first three; the elements of a head are adjacent. g
+   and beta have no last dimension. */
+typedef struct {
+  void *data;
+  int64_t batch, token, head;
+} cchip_heads;
+
+typedef struct {
+  cchip_heads q, k, v, g, beta;
+  cchip_heads o;                       /* forward: written */
+  cchip_heads d_o;                     /* backward: read */
+  cchip_heads dq, dk, dv, dg, dbeta;   /* backward: written */
+  const int32_t *offsets;
+  const float *state;                  /* forward: read */
+  float *state_out;                    /* forward: written; may be `state` */
+  const float *dstate_out;             /* backward: gradient of state_out, NULL: zero */
+  float *dstate;                       /* backward: gradient of state, NULL: not wanted */
+  void *saved;                         /* forward: written (NULL: no backward pass follows); backward: read */
+} cchip_gated_delta_io;
+
+/* Bytes of workspace that a forward or backward call needs (it holds nothing
+   between calls; calls that overlap need one each) and of `saved`. Both are
+   aligned to 16 bytes. */
+int cchip_gated_delta_sizes(const cchip_gated_delta *op, size_t *workspace, size_t *saved);
+int cchip_gated_delta_forward(const cchip_gated_delta *op, const cchip_gated_delta_io *io, void *workspace,
+                              size_t workspace_bytes, void *stream);
+int cchip_gated_delta_backward(const cchip_gated_delta *op, const cchip_gated_delta_io *io, void *workspace,
+                               size_t workspace_bytes, void *stream);
+
+/* ---- Dropout ------------------------------------------------------------- */
+
+/*
+ * Column c of row r is kept iff half c % 8 (16 bits, low halves first) of
+ * Philox-4x32-10 at counter (c / 8, r, offset, offset >> 32) and key (seed,
+ * seed >> 32) is at least round(65536 p). A kept value is scaled by
+ * 65536 / (65536 - round(65536 p)); one that is not is zero whatever it was.
+ * The mask is never stored: the backward pass draws it again. It does not
+ * depend on strides. `step`, if not NULL, is a device word added to offset
+ * when the kernel runs, so that a captured graph draws anew on each replay.
+ */
+typedef struct {
+  double p; /* 0 <= p <= 1 */
+  uint64_t seed, offset;
+  const uint64_t *step;
+} cchip_drop;
+
+/* A matrix: rows `row` elements apart, the elements of a row adjacent. */
+typedef struct {
+  void *data;
+  int64_t row;
+} cchip_rows;
+
+/* out = residual + scale drop(x), residual.data NULL: no residual. The
+   gradient of x is the same call on the gradient of out, without residual.
+   out may be x or residual. rows < 2^32, cols < 2^35. */
+int cchip_dropout(int dtype, int64_t rows, int64_t cols, const cchip_drop *drop, float scale, cchip_rows x,
+                  cchip_rows residual, cchip_rows out, void *stream);
+
+/* ---- Norm block ---------------------------------------------------------- */
+
+/*
+ * What stands between a block and the next one, on each row of `width`:
+ *
+ *   a = norm(y) post_weight + post_bias      (post: the norm, or none)
+ *   b = a act(gate)                          (gate: none, sigmoid or silu)
+ *   h = residual + scale channel_scale drop(b)
+ *   n = norm(h) pre_weight + pre_bias        (pre: the next block's norm, or none)
+ *
+ * norm(x) is x / sqrt(mean(x^2) + eps), of x minus its mean for a layer
+ * norm. Every parameter vector may be NULL (1 or 0 in its place), of type
+ * dtype or f32. Rows of every tensor are apart by a stride of its own.
+ */
+#define CCHIP_NORM_NONE 0
+#define CCHIP_NORM_RMS 1
+#define CCHIP_NORM_LAYER 2
+#define CCHIP_GATE_NONE 0
+#define CCHIP_GATE_SIGMOID 1
+#define CCHIP_GATE_SILU 2
+
+typedef struct {
+  int dtype, weight_dtype;
+  int64_t rows, width; /* rows < 2^32, width <= 32768 */
+  int post, pre, gate;
+  float scale, eps;
+} cchip_norm_block;
+
+typedef struct {
+  const void *post_weight, *post_bias, *channel_scale, *pre_weight, *pre_bias;
+} cchip_norm_params;
+
+typedef struct {
+  void *post_weight, *post_bias, *channel_scale, *pre_weight, *pre_bias; /* NULL: not wanted */
+} cchip_norm_grads;
+
+/* h may be `residual` or y, n may be y. n is NULL iff pre is none. */
+int cchip_norm_block_forward(const cchip_norm_block *op, const cchip_drop *drop, const cchip_norm_params *params,
+                             cchip_rows y, cchip_rows gate, cchip_rows residual, cchip_rows h, cchip_rows n,
+                             void *stream);
+/* From y, gate, the forward pass's h (needed iff pre is not none), and the
+   gradients dh and dn of its results: the gradients of y, gate and residual
+   (dresidual.data NULL: not wanted) and of the parameters, summed over rows
+   in f32 in an order that does not change from run to run. */
+int cchip_norm_block_workspace(const cchip_norm_block *op, size_t *bytes);
+int cchip_norm_block_backward(const cchip_norm_block *op, const cchip_drop *drop, const cchip_norm_params *params,
+                              const cchip_norm_grads *grads, cchip_rows y, cchip_rows gate, cchip_rows h,
+                              cchip_rows dh, cchip_rows dn, cchip_rows dy, cchip_rows dgate, cchip_rows dresidual,
+                              void *workspace, size_t workspace_bytes, void *stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif
