@@ -72,11 +72,6 @@ Heads heads_of(const cchip_gated_delta &op, const cchip_heads &x, const char *na
   return {static_cast<char *>(x.data), x.batch, x.token, x.head};
 }
 
-bool vector_rows(const cchip_gated_delta &op, const Heads &x, int dim) {
-  const int n = 16 / element_size(op);
-  return aligned16(x.p) && x.b % n == 0 && x.t % n == 0 && x.h % n == 0 && dim % 8 == 0;
-}
-
 DeltaArgs args_of(const cchip_gated_delta &op, const cchip_gated_delta_io &io, bool back) {
   DeltaArgs a = {};
   const int hk = op.key_heads, hv = op.value_heads, dk = op.key_dim, dv = op.value_dim;
@@ -89,8 +84,6 @@ DeltaArgs args_of(const cchip_gated_delta &op, const cchip_gated_delta_io &io, b
     throw InvalidArgument(op.sequences ? "gated delta: packed sequences need offsets" : "gated delta: offsets without packed sequences");
   if (!op.states && (io.state || io.state_out || io.dstate || io.dstate_out))
     throw InvalidArgument("gated delta: a state for an operator made without states");
-  a.vec_qk = vector_rows(op, a.q, dk) && vector_rows(op, a.k, dk);
-  a.vec_v = vector_rows(op, a.v, dv);
   if (back) {
     if (!io.saved) throw InvalidArgument("gated delta: the backward pass needs what the forward pass saved");
     a.d_o = heads_of(op, io.d_o, "the gradient of o", false, hv, dv);
@@ -99,7 +92,6 @@ DeltaArgs args_of(const cchip_gated_delta &op, const cchip_gated_delta_io &io, b
     a.gv = heads_of(op, io.dv, "dv", true, hv, dv);
     a.gg = heads_of(op, io.dg, "dg", true, hv, 1);
     a.gbeta = heads_of(op, io.dbeta, "dbeta", true, hv, 1);
-    a.vec_v = a.vec_v && vector_rows(op, a.d_o, dv);
     a.dstate_out = io.dstate_out;
     a.dstate = io.dstate;
   } else {

@@ -50,8 +50,6 @@ struct DeltaArgs {
   int chunks;  // of a row of the batch; unused where packed
   int hk, hv, dk, dv;
   float scale;
-  bool vec_qk;  // rows of q and k can be read 16 bytes at a time
-  bool vec_v;   // v, d_o
 };
 
 // What a chunk and value head have that depends on no state: matrices as
@@ -134,9 +132,9 @@ __device__ __forceinline__ T *out_at(const Heads &x, int64_t row, int64_t token,
 // Eight elements of token `t` of a chunk from element `d` on, of a head of
 // `dim`; zeros past the chunk or the head.
 template <typename T>
-__device__ __forceinline__ Raw8<T> load_head8(const Heads &x, const Chunk &c, int head, int t, int d, int dim, bool vec) {
+__device__ __forceinline__ Raw8<T> load_head8(const Heads &x, const Chunk &c, int head, int t, int d, int dim) {
   const int n = t < c.len ? (dim - d < 0 ? 0 : dim - d > 8 ? 8 : dim - d) : 0;
-  return load8<T>(at<T>(x, c.row, c.first + t, head) + d, n, vec);
+  return load8<T>(at<T>(x, c.row, c.first + t, head) + d, n);
 }
 
 template <typename Mode>

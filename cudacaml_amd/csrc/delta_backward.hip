@@ -71,12 +71,12 @@ __global__ __launch_bounds__(256) void delta_reverse(const DeltaArgs a, int bloc
     const float *dec = reinterpret_cast<const float *>(rec + R::Decay);
     for (int at = tid; at < 64 * (DK / 8); at += 256) {
       const int t = at / (DK / 8), d = at % (DK / 8) * 8;
-      put_frag<NI>(ks + t * LDK + d, KP, frag_of<NI>(load_head8<T>(a.k, c, hk, t, d, a.dk, a.vec_qk)));
-      put_frag<NI>(qs + t * LDK + d, KP, frag_of<NI>(load_head8<T>(a.q, c, hk, t, d, a.dk, a.vec_qk)));
+      put_frag<NI>(ks + t * LDK + d, KP, frag_of<NI>(load_head8<T>(a.k, c, hk, t, d, a.dk)));
+      put_frag<NI>(qs + t * LDK + d, KP, frag_of<NI>(load_head8<T>(a.q, c, hk, t, d, a.dk)));
     }
     for (int at = tid; at < 64 * (BV / 8); at += 256) {
       const int t = at / (BV / 8), d = at % (BV / 8) * 8;
-      const Raw8<T> raw = load_head8<T>(a.d_o, c, h, t, dv0 + d, a.dv, a.vec_v);
+      const Raw8<T> raw = load_head8<T>(a.d_o, c, h, t, dv0 + d, a.dv);
       put_frag<NI>(os + t * LDV + d, VP, frag_of<NI>(raw));
       const float f = a.scale * dec[t];
       Raw8<float> up;
@@ -215,8 +215,8 @@ __global__ __launch_bounds__(256) void delta_gradients(const DeltaArgs a) {
 
   for (int at = tid; at < 64 * (DK / 8); at += 256) {
     const int t = at / (DK / 8), d = at % (DK / 8) * 8;
-    put_frag<NI>(ks + t * LDK + d, KP, frag_of<NI>(load_head8<T>(a.k, c, hk, t, d, a.dk, a.vec_qk)));
-    put_frag<NI>(qs + t * LDK + d, KP, frag_of<NI>(load_head8<T>(a.q, c, hk, t, d, a.dk, a.vec_qk)));
+    put_frag<NI>(ks + t * LDK + d, KP, frag_of<NI>(load_head8<T>(a.k, c, hk, t, d, a.dk)));
+    put_frag<NI>(qs + t * LDK + d, KP, frag_of<NI>(load_head8<T>(a.q, c, hk, t, d, a.dk)));
   }
   // element (t, d) of K or Q as its planes add up
   auto value = [&](const bf16 *m, int t, int d) {
@@ -234,7 +234,6 @@ __global__ __launch_bounds__(256) void delta_gradients(const DeltaArgs a) {
     const Saved *E = reinterpret_cast<const Saved *>(a.grads) + slot_head * a.dk * a.dv;
     const Saved *U = reinterpret_cast<const Saved *>(a.us) + slot_head * kChunk * a.dv;
     const Saved *Y = reinterpret_cast<const Saved *>(a.ys) + slot_head * kChunk * a.dv;
-    const bool vec = a.dv % 8 == 0;
     __syncthreads();
     if (w == 0) {
       const float g = l < c.len ? float(*at<T>(a.g, c.row, c.first + l, h)) : 0.0f;
@@ -252,8 +251,8 @@ __global__ __launch_bounds__(256) void delta_gradients(const DeltaArgs a) {
     for (int v0 = 0; v0 < a.dv; v0 += 32) {
       const int v = v0 + 8 * quad, t = 16 * w + col;
       const int nv = a.dv - v < 0 ? 0 : a.dv - v > 8 ? 8 : a.dv - v;
-      const Raw8<T> ro = load_head8<T>(a.d_o, c, h, t, v, a.dv, a.vec_v), rv = load_head8<T>(a.v, c, h, t, v, a.dv, a.vec_v);
-      const Raw8<Saved> ry = load8<Saved>(Y + int64_t(t) * a.dv + v, nv, vec), ru = load8<Saved>(U + int64_t(t) * a.dv + v, nv, vec);
+      const Raw8<T> ro = load_head8<T>(a.d_o, c, h, t, v, a.dv), rv = load_head8<T>(a.v, c, h, t, v, a.dv);
+      const Raw8<Saved> ry = load8<Saved>(Y + int64_t(t) * a.dv + v, nv), ru = load8<Saved>(U + int64_t(t) * a.dv + v, nv);
 #pragma unroll
       for (int i = 0; i < 8; i++) yv += float(ry.x[i]) * float(rv.x[i]);
       const Frag<NI> fo = frag_of<NI>(ro);
@@ -263,7 +262,7 @@ __global__ __launch_bounds__(256) void delta_gradients(const DeltaArgs a) {
       for (int i = tid; i < DK * 4; i += 256) {
         const int x = i / 4, y = v0 + i % 4 * 8;
         const int n = x < a.dk && y < a.dv ? (a.dv - y > 8 ? 8 : a.dv - y) : 0;
-        const Raw8<Saved> rs = load8<Saved>(S + int64_t(x) * a.dv + y, n, vec), re = load8<Saved>(E + int64_t(x) * a.dv + y, n, vec);
+        const Raw8<Saved> rs = load8<Saved>(S + int64_t(x) * a.dv + y, n), re = load8<Saved>(E + int64_t(x) * a.dv + y, n);
 #pragma unroll
         for (int j = 0; j < 8; j++) se += float(rs.x[j]) * float(re.x[j]);
         put_frag<NB>(ss + x * LDS + i % 4 * 8, SP, frag_of<NB>(rs));
@@ -286,7 +285,7 @@ __global__ __launch_bounds__(256) void delta_gradients(const DeltaArgs a) {
       for (int i = tid; i < DK * 4; i += 256) {
         const int x = i / 4, y = v0 + i % 4 * 8;
         const int n = x < a.dk && y < a.dv ? (a.dv - y > 8 ? 8 : a.dv - y) : 0;
-        put_frag<NB>(ss + x * LDS + i % 4 * 8, SP, frag_of<NB>(load8<Saved>(E + int64_t(x) * a.dv + y, n, vec)));
+        put_frag<NB>(ss + x * LDS + i % 4 * 8, SP, frag_of<NB>(load8<Saved>(E + int64_t(x) * a.dv + y, n)));
       }
       __syncthreads();
 #pragma unroll
@@ -344,12 +343,10 @@ __global__ __launch_bounds__(256) void delta_gradients(const DeltaArgs a) {
         across += pair;
         db[r] -= s < t ? yu[j][r] * d * kk[j][r] : 0.0f;
       }
-      across += __shfl_xor(across, 16, 64);
-      across += __shfl_xor(across, 32, 64);
+      across = sum_rows(across);
       if (quad == 0) down[w][16 * j + col] = across;
     }
-    yv += __shfl_xor(yv, 16, 64);
-    yv += __shfl_xor(yv, 32, 64);  // lane c: of row 16 w + c % 16
+    yv = sum_rows(yv);  // lane c: of row 16 w + c % 16
     float end = 0.0f;
 #pragma unroll
     for (int r = 0; r < 4; r++) {
@@ -358,8 +355,7 @@ __global__ __launch_bounds__(256) void delta_gradients(const DeltaArgs a) {
       const float f = sum16(from_last[r]);
       end += f;
     }
-    end = end + __shfl_xor(end, 16, 64);
-    end = end + __shfl_xor(end, 32, 64);
+    end = sum_rows(end);
     se = sum64(se);
     if (l == 0) total[w] = end + se * dec[63];
     __syncthreads();  // every wave is done with the slice; down and total are there

@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256) void delta_chunk(const DeltaArgs a) {
   }
   for (int i = tid; i < 64 * (DK / 8); i += 256) {
     const int t = i / (DK / 8), d = i % (DK / 8) * 8;
-    put_frag<NI>(ks + t * LD + d, KPlane, frag_of<NI>(load_head8<T>(a.k, c, hk, t, d, a.dk, a.vec_qk)));
+    put_frag<NI>(ks + t * LD + d, KPlane, frag_of<NI>(load_head8<T>(a.k, c, hk, t, d, a.dk)));
   }
   for (int i = tid; i < 64 * kPad; i += 256) tm[i] = 0.0f;
   __syncthreads();
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256) void delta_chunk(const DeltaArgs a) {
 #pragma unroll
   for (int d = 0; d < DK; d += 32) {
     const Frag<NI> fk = frag_row<NI>(ks, KPlane, LD, 16 * w, d);
-    const Frag<NI> fq = frag_of<NI>(load_head8<T>(a.q, c, hk, 16 * w + col, d + quad * 8, a.dk, a.vec_qk));
+    const Frag<NI> fq = frag_of<NI>(load_head8<T>(a.q, c, hk, 16 * w + col, d + quad * 8, a.dk));
 #pragma unroll
     for (int j = 0; j < 4; j++)
       if (j <= w) {

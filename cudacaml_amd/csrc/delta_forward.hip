@@ -72,10 +72,10 @@ __global__ __launch_bounds__(256) void delta_forward(const DeltaArgs a, int bloc
 #pragma unroll
     for (int j = 0; j < DK / 32; j++) {
       const int at = tid + 256 * j;
-      n.k[j] = load_head8<T>(a.k, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk, a.vec_qk);
+      n.k[j] = load_head8<T>(a.k, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk);
     }
 #pragma unroll
-    for (int j = 0; j < DK / 32; j++) n.q[j] = load_head8<T>(a.q, c, hk, 16 * w + col, 32 * j + 8 * quad, a.dk, a.vec_qk);
+    for (int j = 0; j < DK / 32; j++) n.q[j] = load_head8<T>(a.q, c, hk, 16 * w + col, 32 * j + 8 * quad, a.dk);
 #pragma unroll
     for (int b = 0; b < 2; b++)
       if (b == 0 || w >= 2) {  // T and P end at the diagonal

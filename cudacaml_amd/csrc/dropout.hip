@@ -18,7 +18,6 @@ struct DropoutArgs {
   int64_t cols;
   float scale;
   Drop drop;
-  bool vec;
 };
 
 // A thread a group of 8 columns. One call of the generator serves all 8, at
@@ -33,16 +32,16 @@ __global__ __launch_bounds__(256) void dropout(const DropoutArgs a) {
   const uint32_t group = uint32_t(i - row * a.per_row);
   const int64_t col = int64_t(group) * 8;
   const int n = a.cols - col > 8 ? 8 : int(a.cols - col);
-  const Raw8<T> x = load8<T>(row_at<T>(a.x, row) + col, n, a.vec);
+  const Raw8<T> x = load8<T>(row_at<T>(a.x, row) + col, n);
   const bool add = a.residual.p != nullptr;
   Raw8<T> r = {};
-  if (add) r = load8<T>(row_at<T>(a.residual, row) + col, n, a.vec);
+  if (add) r = load8<T>(row_at<T>(a.residual, row) + col, n);
   const uint32_t bits = a.drop.bar ? keep_bits(a.drop, offset_of(a.drop), uint32_t(row), group) : 0xFFu;
   const float up = a.scale * a.drop.up;
   float out[8];
 #pragma unroll
   for (int j = 0; j < 8; j++) out[j] = (bits >> j & 1 ? up * float(x.x[j]) : 0.0f) + (add ? float(r.x[j]) : 0.0f);
-  store8<T>(row_at<T>(a.out, row) + col, out, n, a.vec);
+  store8<T>(row_at<T>(a.out, row) + col, out, n);
 }
 
 }  // namespace
@@ -80,7 +79,6 @@ extern "C" int cchip_dropout(int dtype, int64_t rows, int64_t cols, const cchip_
     if ((a.groups + 255) / 256 > uint64_t(INT32_MAX)) throw InvalidArgument("dropout: more elements than a launch can have");
     a.cols = cols;
     a.scale = scale;
-    a.vec = vector_rows(a.x, dtype) && vector_rows(a.residual, dtype) && vector_rows(a.out, dtype);
     with_rows_type(dtype, [&](auto t) {
       typedef decltype(t) T;
       hipLaunchKernelGGL((dropout<T>), dim3(unsigned((a.groups + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a);

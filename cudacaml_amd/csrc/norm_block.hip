@@ -24,22 +24,25 @@ struct ColumnArgs {
   bool f32;
 };
 
-// 32 columns of one parameter a workgroup; 8 threads a column sum every 8th
-// workgroup's share, and thread 0 those 8, in order.
+// 32 columns of one parameter a workgroup; 32 threads a column each sum
+// every 32nd workgroup's share, and one of them those 32, in order.
 template <typename T>
-__global__ __launch_bounds__(256) void norm_columns(const ColumnArgs a) {
-  __shared__ float part[8][33];
+__global__ __launch_bounds__(1024) void norm_columns(const ColumnArgs a) {
+  __shared__ float part[32][33];
   const int col = threadIdx.x % 32, turn = threadIdx.x / 32, s = blockIdx.y;
   const int c = int(blockIdx.x) * 32 + col;
+  if (!a.to[s]) return;
   float q = 0.0f;
-  if (c < a.width && a.to[s])
-    for (int g = turn; g < a.groups; g += 8) q += a.partial[(int64_t(g) * a.sums + s) * a.width + c];
+  if (c < a.width) {
+#pragma unroll 8
+    for (int g = turn; g < a.groups; g += 32) q += a.partial[(int64_t(g) * a.sums + s) * a.width + c];
+  }
   part[turn][col] = q;
   __syncthreads();
-  if (turn || c >= a.width || !a.to[s]) return;
+  if (turn || c >= a.width) return;
   float x = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 8; i++) x += part[i][col];
+  for (int i = 0; i < 32; i++) x += part[i][col];
   if (a.f32) static_cast<float *>(a.to[s])[c] = x;
   else static_cast<T *>(a.to[s])[c] = T(x);
 }
@@ -90,13 +93,12 @@ NormArgs args_of(const cchip_norm_block &op, const cchip_drop *drop, const cchip
   return a;
 }
 
-// Workgroups of a backward pass: enough to fill the chip four times over,
-// and at least 4 rows each so that the sums left over stay small beside the
-// rows.
+// Workgroups of a backward pass: as many as run at once, and at least 4 rows
+// each so that the sums they leave stay small beside the rows.
 int groups_of(const cchip_norm_block &op) {
   const int64_t at_a_time = rows_at_a_time(int(op.width));
   const int64_t sets = (op.rows + at_a_time - 1) / at_a_time;
-  return int(std::min<int64_t>(kMostGroups, (sets + 3) / 4));
+  return int(std::min<int64_t>(resident_groups(int(op.width)), (sets + 3) / 4));
 }
 
 }  // namespace
@@ -124,8 +126,6 @@ int cchip_norm_block_forward(const cchip_norm_block *op, const cchip_drop *drop,
     a.residual = rows_of(who, "residual", op->dtype, op->rows, op->width, residual, false, false);
     a.h = rows_of(who, "h", op->dtype, op->rows, op->width, h, true, true);
     a.n = rows_of(who, "n", op->dtype, op->rows, op->width, n, true, false);
-    a.vec = true;
-    for (const Rows *r : {&a.y, &a.gate, &a.residual, &a.h, &a.n}) a.vec = a.vec && vector_rows(*r, op->dtype);
     with_rows_type(op->dtype, [&](auto t) { norm_forward_launch<decltype(t)>(a, (hipStream_t)stream); });
     check_launch(who);
   });
@@ -164,7 +164,7 @@ int cchip_norm_block_backward(const cchip_norm_block *op, const cchip_drop *drop
     if ((c.to[kPostWeight] || c.to[kPostBias]) && op->post == CCHIP_NORM_NONE)
       throw InvalidArgument("norm block: gradients of a post norm that there is not");
     if ((c.to[kPreWeight] || c.to[kPreBias]) && !pre) throw InvalidArgument("norm block: gradients of a pre norm that there is not");
-    const bool bias = c.to[kPostBias] || c.to[kPreBias];
+    const bool bias = c.to[kPostBias] || c.to[kPreBias] || a.post_bias;
     if (op->rows > 0) {
       if (pre != (dn.data != nullptr) || pre != (h.data != nullptr))
         throw InvalidArgument("norm block: h and dn are given if and only if there is a pre norm");
@@ -178,9 +178,6 @@ int cchip_norm_block_backward(const cchip_norm_block *op, const cchip_drop *drop
       a.dy = rows_of(who, "dy", op->dtype, op->rows, op->width, dy, true, true);
       a.dgate = rows_of(who, "dgate", op->dtype, op->rows, op->width, dgate, true, false);
       a.dresidual = rows_of(who, "dresidual", op->dtype, op->rows, op->width, dresidual, true, false);
-      a.vec = true;
-      for (const Rows *r : {&a.y, &a.gate, &a.h, &a.dh, &a.dn, &a.dy, &a.dgate, &a.dresidual})
-        a.vec = a.vec && vector_rows(*r, op->dtype);
     }
     const int groups = groups_of(*op);
     if (any) {
@@ -200,7 +197,7 @@ int cchip_norm_block_backward(const cchip_norm_block *op, const cchip_drop *drop
     c.f32 = a.weights_f32;
     with_rows_type(op->dtype, [&](auto t) {
       typedef decltype(t) T;
-      hipLaunchKernelGGL((norm_columns<T>), dim3((a.width + 31) / 32, c.sums), dim3(256), 0, (hipStream_t)stream, c);
+      hipLaunchKernelGGL((norm_columns<T>), dim3((a.width + 31) / 32, c.sums), dim3(1024), 0, (hipStream_t)stream, c);
     });
     check_launch(who);
   });

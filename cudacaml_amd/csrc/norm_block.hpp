@@ -14,7 +14,7 @@ struct NormArgs {
   float *partial;  // backward: [workgroup][parameter][width]
   uint32_t rows;
   int width, post, pre, act;
-  bool weights_f32, vec;
+  bool weights_f32;
   float scale, eps;
   Drop drop;
 };
@@ -40,14 +40,21 @@ struct RowSum {
   }
 };
 
+// Eight of a parameter vector; `none` where there is none.
 template <typename T>
 __device__ __forceinline__ void load_params(float (&w)[8], const void *p, bool f32, int at, int n, float none) {
+  if (!p) {
 #pragma unroll
-  for (int i = 0; i < 8; i++) w[i] = none;
-  if (!p) return;
+    for (int i = 0; i < 8; i++) w[i] = none;
+  } else if (f32) {
+    const Raw8<float> r = load8<float>(static_cast<const float *>(p) + at, n);
 #pragma unroll
-  for (int i = 0; i < 8; i++)
-    if (i < n) w[i] = f32 ? static_cast<const float *>(p)[at + i] : float(static_cast<const T *>(p)[at + i]);
+    for (int i = 0; i < 8; i++) w[i] = r.x[i];
+  } else {
+    const Raw8<T> r = load8<T>(static_cast<const T *>(p) + at, n);
+#pragma unroll
+    for (int i = 0; i < 8; i++) w[i] = float(r.x[i]);
+  }
 }
 
 // x becomes (x - mean) / sqrt(mean of squares + eps); returns what it was
@@ -83,72 +90,81 @@ __device__ __forceinline__ float normalise(float (&x)[V][8], int kind, float inv
 __device__ __forceinline__ float sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }
 
 // A row to LANES threads, 8 neighbouring columns a thread and step, held in
-// registers from the one read of it to the writes.
+// registers from the one read of it to the writes. A workgroup takes every
+// gridDim-th set of rows and keeps the parameters of its columns.
 template <typename T, int LANES, int V>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_forward(const NormArgs a) {
   constexpr int kRows = LANES < 256 ? 256 / LANES : 1;
   __shared__ float scratch[2][LANES > 64 ? LANES / 64 : 1];
   RowSum<LANES> sum = {scratch, 0};
   const int lane = threadIdx.x % LANES;
-  const int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / LANES;
-  if (row >= a.rows) return;
   const float inv_width = 1.0f / float(a.width);
+  const float up = a.scale * a.drop.up;
+  const uint64_t offset = a.drop.bar ? offset_of(a.drop) : 0;
 
-  Raw8<T> y[V], z[V], x[V];
+  // (yhat w + b) up t, as one product and sum
+  float w[V][8], b[V][8], pw[V][8], pb[V][8];
   int n[V];
 #pragma unroll
   for (int v = 0; v < V; v++) {
     const int c = (v * LANES + lane) * 8;
     n[v] = a.width - c < 0 ? 0 : a.width - c > 8 ? 8 : a.width - c;
-    y[v] = load8<T>(row_at<T>(a.y, row) + c, n[v], a.vec);
-  }
-  if (a.act != CCHIP_GATE_NONE)
-#pragma unroll
-    for (int v = 0; v < V; v++) z[v] = load8<T>(row_at<T>(a.gate, row) + (v * LANES + lane) * 8, n[v], a.vec);
-  if (a.residual.p)
-#pragma unroll
-    for (int v = 0; v < V; v++) x[v] = load8<T>(row_at<T>(a.residual, row) + (v * LANES + lane) * 8, n[v], a.vec);
-
-  float h[V][8];
-#pragma unroll
-  for (int v = 0; v < V; v++)
-#pragma unroll
-    for (int i = 0; i < 8; i++) h[v][i] = float(y[v].x[i]);
-  if (a.post != CCHIP_NORM_NONE) normalise<LANES, V>(h, a.post, inv_width, a.eps, sum, lane, a.width);
-  const float up = a.scale * a.drop.up;
-  const uint64_t offset = a.drop.bar ? offset_of(a.drop) : 0;
-#pragma unroll
-  for (int v = 0; v < V; v++) {
-    const int g = v * LANES + lane, c = g * 8;
-    float w[8], b[8], t[8];
-    load_params<T>(w, a.post_weight, a.weights_f32, c, n[v], 1.0f);
-    load_params<T>(b, a.post_bias, a.weights_f32, c, n[v], 0.0f);
+    float t[8];
     load_params<T>(t, a.channel_scale, a.weights_f32, c, n[v], 1.0f);
-    const uint32_t bits = a.drop.bar && n[v] ? keep_bits(a.drop, offset, uint32_t(row), g) : 0xFFu;
+    load_params<T>(w[v], a.post_weight, a.weights_f32, c, n[v], 1.0f);
+    load_params<T>(b[v], a.post_bias, a.weights_f32, c, n[v], 0.0f);
+    load_params<T>(pw[v], a.pre_weight, a.weights_f32, c, n[v], 1.0f);
+    load_params<T>(pb[v], a.pre_bias, a.weights_f32, c, n[v], 0.0f);
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      float e = h[v][i] * w[i] + b[i];
-      if (a.act != CCHIP_GATE_NONE) {
-        const float zi = float(z[v].x[i]), s = sigmoid(zi);
-        e *= a.act == CCHIP_GATE_SILU ? zi * s : s;
-      }
-      e = bits >> i & 1 ? e * up * t[i] : 0.0f;
-      if (a.residual.p) e += float(x[v].x[i]);
-      h[v][i] = i < n[v] ? e : 0.0f;
+      w[v][i] *= up * t[i];
+      b[v][i] *= up * t[i];
     }
-    store8<T>(row_at<T>(a.h, row) + c, h[v], n[v], a.vec);
   }
-  if (a.pre == CCHIP_NORM_NONE) return;
-  normalise<LANES, V>(h, a.pre, inv_width, a.eps, sum, lane, a.width);
+  for (int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / LANES; row < a.rows; row += int64_t(gridDim.x) * kRows) {
+    Raw8<T> y[V], z[V], x[V];
 #pragma unroll
-  for (int v = 0; v < V; v++) {
-    const int c = (v * LANES + lane) * 8;
-    float w[8], b[8];
-    load_params<T>(w, a.pre_weight, a.weights_f32, c, n[v], 1.0f);
-    load_params<T>(b, a.pre_bias, a.weights_f32, c, n[v], 0.0f);
+    for (int v = 0; v < V; v++) y[v] = load8<T>(row_at<T>(a.y, row) + (v * LANES + lane) * 8, n[v]);
+    if (a.act != CCHIP_GATE_NONE)
 #pragma unroll
-    for (int i = 0; i < 8; i++) h[v][i] = h[v][i] * w[i] + b[i];
-    store8<T>(row_at<T>(a.n, row) + c, h[v], n[v], a.vec);
+      for (int v = 0; v < V; v++) z[v] = load8<T>(row_at<T>(a.gate, row) + (v * LANES + lane) * 8, n[v]);
+    if (a.residual.p)
+#pragma unroll
+      for (int v = 0; v < V; v++) x[v] = load8<T>(row_at<T>(a.residual, row) + (v * LANES + lane) * 8, n[v]);
+    uint32_t bits[V];  // drawn while the row is on its way
+#pragma unroll
+    for (int v = 0; v < V; v++)
+      bits[v] = a.drop.bar ? keep_bits(a.drop, offset, uint32_t(row), v * LANES + lane) : 0xFFu;
+
+    float h[V][8];
+#pragma unroll
+    for (int v = 0; v < V; v++)
+#pragma unroll
+      for (int i = 0; i < 8; i++) h[v][i] = float(y[v].x[i]);
+    if (a.post != CCHIP_NORM_NONE) normalise<LANES, V>(h, a.post, inv_width, a.eps, sum, lane, a.width);
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        float e = h[v][i] * w[v][i] + b[v][i];
+        if (a.act != CCHIP_GATE_NONE) {
+          const float zi = float(z[v].x[i]), s = sigmoid(zi);
+          e *= a.act == CCHIP_GATE_SILU ? zi * s : s;
+        }
+        e = bits[v] >> i & 1 ? e : 0.0f;
+        if (a.residual.p) e += float(x[v].x[i]);
+        h[v][i] = i < n[v] ? e : 0.0f;
+      }
+      store8<T>(row_at<T>(a.h, row) + (v * LANES + lane) * 8, h[v], n[v]);
+    }
+    if (a.pre == CCHIP_NORM_NONE) continue;
+    normalise<LANES, V>(h, a.pre, inv_width, a.eps, sum, lane, a.width);
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) h[v][i] = h[v][i] * pw[v][i] + pb[v][i];
+      store8<T>(row_at<T>(a.n, row) + (v * LANES + lane) * 8, h[v], n[v]);
+    }
   }
 }
 
@@ -173,8 +189,8 @@ __device__ __forceinline__ void normalise_back(float (&d)[V][8], const float (&x
     for (int i = 0; i < 8; i++) d[v][i] = (d[v][i] - xhat[v][i] * p - q) * inv;
 }
 
-// The parameters' gradients in the order of their sums; without Bias the
-// second and the last are not made.
+// The parameters' gradients in the order of their sums; without Bias there
+// are no biases and the last two are not made.
 enum Param { kPostWeight, kChannelScale, kPreWeight, kPostBias, kPreBias, kParams };
 
 // As norm_forward, a workgroup taking every gridDim-th set of rows so that it
@@ -191,22 +207,27 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_backward(const
   const float up = a.scale * a.drop.up;
   const uint64_t offset = a.drop.bar ? offset_of(a.drop) : 0;
   float acc[kSums][V][8] = {};
+  float w[V][8], b[V][8], t[V][8], pw[V][8];
   int n[V];
 #pragma unroll
   for (int v = 0; v < V; v++) {
     const int c = (v * LANES + lane) * 8;
     n[v] = a.width - c < 0 ? 0 : a.width - c > 8 ? 8 : a.width - c;
+    load_params<T>(w[v], a.post_weight, a.weights_f32, c, n[v], 1.0f);
+    load_params<T>(b[v], Bias ? a.post_bias : nullptr, a.weights_f32, c, n[v], 0.0f);
+    load_params<T>(t[v], a.channel_scale, a.weights_f32, c, n[v], 1.0f);
+    if (Pre) load_params<T>(pw[v], a.pre_weight, a.weights_f32, c, n[v], 1.0f);
   }
   for (int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / LANES; row < a.rows; row += int64_t(gridDim.x) * kRows) {
     Raw8<T> ry[V], rz[V], rh[V], rdh[V], rdn[V];
 #pragma unroll
     for (int v = 0; v < V; v++) {
       const int c = (v * LANES + lane) * 8;
-      if (Pre) rh[v] = load8<T>(row_at<T>(a.h, row) + c, n[v], a.vec);
-      if (Pre) rdn[v] = load8<T>(row_at<T>(a.dn, row) + c, n[v], a.vec);
-      rdh[v] = load8<T>(row_at<T>(a.dh, row) + c, n[v], a.vec);
-      ry[v] = load8<T>(row_at<T>(a.y, row) + c, n[v], a.vec);
-      if (Gate) rz[v] = load8<T>(row_at<T>(a.gate, row) + c, n[v], a.vec);
+      if (Pre) rh[v] = load8<T>(row_at<T>(a.h, row) + c, n[v]);
+      if (Pre) rdn[v] = load8<T>(row_at<T>(a.dn, row) + c, n[v]);
+      rdh[v] = load8<T>(row_at<T>(a.dh, row) + c, n[v]);
+      ry[v] = load8<T>(row_at<T>(a.y, row) + c, n[v]);
+      if (Gate) rz[v] = load8<T>(row_at<T>(a.gate, row) + c, n[v]);
     }
     float d[V][8], x[V][8];
     if (Pre) {
@@ -217,14 +238,12 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_backward(const
       const float inv = normalise<LANES, V>(x, a.pre, inv_width, a.eps, sum, lane, a.width);
 #pragma unroll
       for (int v = 0; v < V; v++) {
-        float w[8];
-        load_params<T>(w, a.pre_weight, a.weights_f32, (v * LANES + lane) * 8, n[v], 1.0f);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
           const float dn = float(rdn[v].x[i]);
           acc[kPreWeight][v][i] += dn * x[v][i];
           if (Bias) acc[kPreBias][v][i] += dn;
-          d[v][i] = i < n[v] ? dn * w[i] : 0.0f;
+          d[v][i] = i < n[v] ? dn * pw[v][i] : 0.0f;
         }
       }
       normalise_back<LANES, V>(d, x, a.pre, inv, inv_width, sum);
@@ -240,7 +259,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_backward(const
     }
     if (a.dresidual.p)
 #pragma unroll
-      for (int v = 0; v < V; v++) store8<T>(row_at<T>(a.dresidual, row) + (v * LANES + lane) * 8, d[v], n[v], a.vec);
+      for (int v = 0; v < V; v++) store8<T>(row_at<T>(a.dresidual, row) + (v * LANES + lane) * 8, d[v], n[v]);
 
 #pragma unroll
     for (int v = 0; v < V; v++)
@@ -251,15 +270,12 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_backward(const
 #pragma unroll
     for (int v = 0; v < V; v++) {
       const int g = v * LANES + lane, c = g * 8;
-      float w[8], b[8], t[8], dz[8];
-      load_params<T>(w, a.post_weight, a.weights_f32, c, n[v], 1.0f);
-      load_params<T>(b, a.post_bias, a.weights_f32, c, n[v], 0.0f);
-      load_params<T>(t, a.channel_scale, a.weights_f32, c, n[v], 1.0f);
-      const uint32_t bits = a.drop.bar && n[v] ? keep_bits(a.drop, offset, uint32_t(row), g) : 0xFFu;
+      float dz[8];
+      const uint32_t bits = a.drop.bar ? keep_bits(a.drop, offset, uint32_t(row), g) : 0xFFu;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
         const bool keep = bits >> i & 1 && i < n[v];
-        const float e = x[v][i] * w[i] + b[i];
+        const float e = Bias ? x[v][i] * w[v][i] + b[v][i] : x[v][i] * w[v][i];
         float act = 1.0f, slope = 0.0f;
         if (Gate) {
           const float z = float(rz[v].x[i]), s = sigmoid(z);
@@ -268,17 +284,17 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_backward(const
         }
         const float du = keep ? d[v][i] * up : 0.0f;
         acc[kChannelScale][v][i] += keep ? du * e * act : 0.0f;
-        const float db = du * t[i], da = db * act;
+        const float db = du * t[v][i], da = db * act;
         if (Gate) dz[i] = keep ? db * e * slope : 0.0f;
         acc[kPostWeight][v][i] += da * x[v][i];
         if (Bias) acc[kPostBias][v][i] += da;
-        d[v][i] = da * w[i];
+        d[v][i] = da * w[v][i];
       }
-      if (Gate && a.dgate.p) store8<T>(row_at<T>(a.dgate, row) + c, dz, n[v], a.vec);
+      if (Gate && a.dgate.p) store8<T>(row_at<T>(a.dgate, row) + c, dz, n[v]);
     }
     if (a.post != CCHIP_NORM_NONE) normalise_back<LANES, V>(d, x, a.post, inv, inv_width, sum);
 #pragma unroll
-    for (int v = 0; v < V; v++) store8<T>(row_at<T>(a.dy, row) + (v * LANES + lane) * 8, d[v], n[v], a.vec);
+    for (int v = 0; v < V; v++) store8<T>(row_at<T>(a.dy, row) + (v * LANES + lane) * 8, d[v], n[v]);
   }
   if (!a.partial) return;
   if (kRows > 1) {
@@ -310,8 +326,6 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_backward(const
   }
 }
 
-constexpr int kMostGroups = 1024;  // workgroups of a backward pass
-
 template <typename T>
 void norm_forward_launch(const NormArgs &a, hipStream_t stream);
 template <typename T>
@@ -320,16 +334,19 @@ void norm_backward_launch(const NormArgs &a, bool bias, int groups, hipStream_t 
 // Rows a workgroup takes at a time for a width.
 inline int rows_at_a_time(int width) { return width <= 128 ? 16 : width <= 512 ? 4 : 1; }
 
+// Workgroups that run at once: 8 of 256 threads a unit, fewer of more.
+inline int resident_groups(int width) { return width <= 2048 ? 1024 : width <= 4096 ? 512 : 256; }
+
 // Calls f(lanes, steps) with the smallest shape that holds a row: few lanes
-// for short rows, so that none idles, and no more than 16 columns a thread
-// up to 16384, so that a backward pass's five sums stay in registers.
+// for short rows, so that none idles, and 8 columns a thread up to 8192, so
+// that a backward pass's parameters and sums stay in registers.
 template <typename F>
 void with_shape(int width, F &&f) {
   if (width <= 128) f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
   else if (width <= 512) f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
   else if (width <= 2048) f(std::integral_constant<int, 256>(), std::integral_constant<int, 1>());
-  else if (width <= 4096) f(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
-  else if (width <= 8192) f(std::integral_constant<int, 512>(), std::integral_constant<int, 2>());
+  else if (width <= 4096) f(std::integral_constant<int, 512>(), std::integral_constant<int, 1>());
+  else if (width <= 8192) f(std::integral_constant<int, 1024>(), std::integral_constant<int, 1>());
   else if (width <= 16384) f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
   else f(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
 }
@@ -340,7 +357,9 @@ void with_shape(int width, F &&f) {
     with_shape(a.width, [&](auto lanes, auto steps) {                                                              \
       constexpr int L = decltype(lanes)::value, V = decltype(steps)::value;                                        \
       constexpr int kRows = L < 256 ? 256 / L : 1;                                                                 \
-      hipLaunchKernelGGL((norm_forward<T, L, V>), dim3(unsigned((int64_t(a.rows) + kRows - 1) / kRows)),           \
+      const int64_t sets = (int64_t(a.rows) + kRows - 1) / kRows;                                                  \
+      const int most = 2 * resident_groups(a.width);                                                               \
+      hipLaunchKernelGGL((norm_forward<T, L, V>), dim3(unsigned(sets < most ? sets : most)),                       \
                          dim3(L < 256 ? 256 : L), 0, stream, a);                                                   \
     });                                                                                                            \
   }                                                                                                                \

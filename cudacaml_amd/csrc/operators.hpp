@@ -19,20 +19,24 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// Eight neighbouring elements as they lie in memory. `vec`: p is aligned to
-// 16 bytes and all eight exist; otherwise the first `valid` are read one by
-// one and the rest are zero.
+// Eight neighbouring elements as they lie in memory: 16-byte accesses at any
+// alignment that the elements have (the hardware takes them; what counts is
+// how many lines they touch) where all eight exist; otherwise the first
+// `valid` one by one, the rest zero.
 template <typename T>
 struct Raw8 {
   T x[8];
 };
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+
 template <typename T>
-__device__ __forceinline__ Raw8<T> load8(const T *p, int valid, bool vec) {
+__device__ __forceinline__ Raw8<T> load8(const T *p, int valid) {
   Raw8<T> r;
-  if (vec && valid == 8) {
-    const uint4 *s = reinterpret_cast<const uint4 *>(p);
-    uint4 *d = reinterpret_cast<uint4 *>(&r);
+  if (valid == 8) {
+    const u32x4_any *s = reinterpret_cast<const u32x4_any *>(p);
+    u32x4 *d = reinterpret_cast<u32x4 *>(&r);
 #pragma unroll
     for (int i = 0; i < int(sizeof(T) * 8 / 16); i++) d[i] = s[i];
   } else {
@@ -150,18 +154,32 @@ __device__ __forceinline__ void put_frag(bf16 *at, int plane, const Frag<N> &f) 
   for (int n = 0; n < N; n++) *reinterpret_cast<bf16x8 *>(at + n * plane) = f.p[n];
 }
 
-// Sum over the 16 lanes of a row of lanes (every lane gets it).
+// Sum over the 16 lanes of a row of lanes by rotations within it, and over
+// the wave by swapping its rows and then its halves: every lane gets it, and
+// nothing goes through LDS.
 __device__ __forceinline__ float sum16(float x) {
-#pragma unroll
-  for (int d = 1; d < 16; d *= 2) x += __shfl_xor(x, d, 64);
+#define CCHIP_ROTATED(x, n) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + n, 0xf, 0xf, true))
+  x += CCHIP_ROTATED(x, 8);
+  x += CCHIP_ROTATED(x, 4);
+  x += CCHIP_ROTATED(x, 2);
+  x += CCHIP_ROTATED(x, 1);
+#undef CCHIP_ROTATED
   return x;
 }
 
-__device__ __forceinline__ float sum64(float x) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d, 64);
-  return x;
+// x of the same column summed over the four rows of 16 lanes.
+__device__ __forceinline__ float sum_rows(float x) {
+  uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  x = __builtin_bit_cast(float, a0) + __builtin_bit_cast(float, a1);
+  u = __builtin_bit_cast(uint32_t, x);
+  const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return __builtin_bit_cast(float, b0) + __builtin_bit_cast(float, b1);
 }
+
+__device__ __forceinline__ float sum64(float x) { return sum_rows(sum16(x)); }
 
 // Philox-4x32-10 (Salmon, Moraes, Dror and Shaw, SC'11), the generator of
 // cudacaml_amd/rng.py: ten rounds, the key bumped after the first nine.

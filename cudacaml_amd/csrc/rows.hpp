@@ -21,13 +21,13 @@ __device__ __forceinline__ T *row_at(const Rows &x, uint64_t row) {
 }
 
 template <typename T>
-__device__ __forceinline__ void store8(T *p, const float (&x)[8], int n, bool vec) {
+__device__ __forceinline__ void store8(T *p, const float (&x)[8], int n) {
   Raw8<T> r;
 #pragma unroll
   for (int i = 0; i < 8; i++) r.x[i] = T(x[i]);
-  if (vec && n == 8) {
-    const uint4 *s = reinterpret_cast<const uint4 *>(&r);
-    uint4 *d = reinterpret_cast<uint4 *>(p);
+  if (n == 8) {
+    const u32x4 *s = reinterpret_cast<const u32x4 *>(&r);
+    u32x4_any *d = reinterpret_cast<u32x4_any *>(p);
 #pragma unroll
     for (int i = 0; i < int(sizeof(T) * 8 / 16); i++) d[i] = s[i];
   } else {
@@ -58,9 +58,6 @@ inline Rows rows_of(const char *who, const char *name, int dtype, int64_t rows, 
   if (written && rows > 1 && std::llabs(x.row) < cols) throw InvalidArgument(strf("%s: rows of %s overlap", who, name));
   return {static_cast<char *>(x.data), x.row};
 }
-
-// Whether every row begins at a multiple of 16 bytes (true of no matrix).
-inline bool vector_rows(const Rows &x, int dtype) { return aligned16(x.p) && x.row % (dtype == CCHIP_F32 ? 4 : 8) == 0; }
 
 template <typename F>
 void with_rows_type(int dtype, F &&f) {
