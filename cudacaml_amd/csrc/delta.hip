@@ -15,10 +15,8 @@ constexpr int64_t kStepTokens = 8;
 
 struct Layout {
   int64_t slots, slot_heads;
-  size_t record, record_back, states, us;  // bytes, all slots and heads; states: [key_dim][value_dim], us: [64][value_dim]
+  size_t record, record_back, states, us;  // bytes, all slots and heads
 };
-
-size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 
 void check_op(const cchip_gated_delta *op) {
   if (!op) throw InvalidArgument("gated delta: no descriptor");
@@ -37,21 +35,23 @@ void check_op(const cchip_gated_delta *op) {
 
 int64_t count_sequences(const cchip_gated_delta &op) { return op.sequences ? op.sequences : op.batch; }
 
+int padded_value_dim(const cchip_gated_delta &op) { return (op.value_dim + 31) / 32 * 32; }
+
 Layout layout_of(const cchip_gated_delta &op) {
   Layout p;
   // batch and sequences below 2^31, so nothing here overflows
   if (op.batch >= (int64_t(1) << 31) || op.sequences >= (int64_t(1) << 31)) throw InvalidArgument("gated delta: too many sequences");
   p.slots = op.sequences ? op.tokens / kChunk + op.sequences : op.batch * ((op.tokens + kChunk - 1) / kChunk);
   p.slot_heads = p.slots * op.value_heads;
-  const int64_t blocks = (op.value_dim + 15) / 16;
+  const int64_t blocks = padded_value_dim(op) / 16;
   if (p.slots > INT32_MAX || p.slot_heads > INT32_MAX || (count_sequences(op) * op.value_heads + 8) * blocks > INT32_MAX)
     throw InvalidArgument("gated delta: more chunks, heads and value columns than a launch can have");
   with_mode(op, [&](auto m) {
     typedef decltype(m) M;
-    p.record = up16(size_t(p.slot_heads) * record_bytes<M>(false));
-    p.record_back = up16(size_t(p.slot_heads) * record_bytes<M>(true));
-    p.states = up16(size_t(p.slot_heads) * op.key_dim * op.value_dim * sizeof(typename M::Saved));
-    p.us = up16(size_t(p.slot_heads) * kChunk * op.value_dim * sizeof(typename M::Saved));
+    p.record = size_t(p.slot_heads) * record_bytes<M>(false);
+    p.record_back = size_t(p.slot_heads) * record_bytes<M>(true);
+    p.states = size_t(p.slot_heads) * padded_key_dim(op.key_dim) * padded_value_dim(op) * sizeof(typename M::Saved);
+    p.us = size_t(p.slot_heads) * kChunk * padded_value_dim(op) * sizeof(float);
   });
   return p;
 }
@@ -67,6 +67,8 @@ Heads heads_of(const cchip_gated_delta &op, const cchip_heads &x, const char *na
   if (!x.data) throw InvalidArgument(strf("gated delta: no %s", name));
   if (reinterpret_cast<uintptr_t>(x.data) % element_size(op))
     throw InvalidArgument(strf("gated delta: %s is not aligned to its elements", name));
+  // within a chunk elements are counted in 32 bits
+  if (x.token < 0 || x.token > (int64_t(1) << 23)) throw InvalidArgument(strf("gated delta: tokens of %s are not 0 to 2^23 elements apart", name));
   if (written && ((op.batch > 1 && x.batch == 0) || (op.tokens > 1 && x.token == 0) || (heads > 1 && std::llabs(x.head) < dim)))
     throw InvalidArgument(strf("gated delta: elements of %s overlap", name));
   return {static_cast<char *>(x.data), x.batch, x.token, x.head};
@@ -108,6 +110,7 @@ DeltaArgs args_of(const cchip_gated_delta &op, const cchip_gated_delta_io &io, b
   a.hv = hv;
   a.dk = dk;
   a.dv = dv;
+  a.dvp = padded_value_dim(op);
   a.scale = op.scale;
   return a;
 }
@@ -125,7 +128,7 @@ size_t workspace_bytes_of(const cchip_gated_delta &op, const Layout &p) {
 void lay_out(DeltaArgs &a, const Layout &p, char *saved) {
   a.records = saved;
   a.states = saved + p.record_back;
-  a.us = a.states + p.states;
+  a.us = reinterpret_cast<float *>(a.states + p.states);
 }
 
 }  // namespace
@@ -174,7 +177,7 @@ int cchip_gated_delta_backward(const cchip_gated_delta *op, const cchip_gated_de
     lay_out(a, p, static_cast<char *>(io->saved));
     check_workspace(workspace, workspace_bytes, p.states + p.us);
     a.grads = static_cast<char *>(workspace);
-    a.ys = a.grads + p.states;
+    a.ys = reinterpret_cast<float *>(a.grads + p.states);
     delta_backward_launch(*op, a, (hipStream_t)stream);
   });
 }

@@ -18,6 +18,8 @@
 // state as it is.
 #pragma once
 
+#include <type_traits>
+
 #include "../../include/cchip_operators.h"
 #include "operators.hpp"
 
@@ -41,41 +43,50 @@ struct DeltaArgs {
   const float *dstate_out;
   float *dstate;
   char *records;  // one a (slot, value head)
-  char *states;   // saved S before each chunk, [key_dim][value_dim]; null if there is no backward pass
-  char *us;       // saved U, [64][value_dim]
-  char *grads;    // backward: dS after each chunk
-  char *ys;       // backward: Y
+  // of each (slot, value head), rows of dvp elements; what pads a head is zero
+  char *states;   // saved S before the chunk, [DK][dvp]; null if there is no backward pass
+  float *us;      // saved U, [64][dvp]
+  char *grads;    // backward: dS after the chunk
+  float *ys;      // backward: Y
   int64_t tokens, sequences;  // sequences: of the packed batch, or its rows
   int64_t slots;
   int chunks;  // of a row of the batch; unused where packed
   int hk, hv, dk, dv;
+  int dvp;     // dv rounded up to 32
   float scale;
 };
+
+// Element type, then the planes: NI of an input, NS of what makes a state
+// (S, T, X and U in their products), NO of S and P where they make only an
+// output, NU of U and Y where they make only outputs. Saved is the type that
+// S and dS are kept in for the backward pass, read back in NB planes.
+//
+// A product loses the most precise operand's worth of the other's rounding:
+// 2^-9 of a value in one plane of bf16, 2^-17 in two. bf16 results are
+// rounded to 2^-9 themselves, and each of theirs comes through one operand
+// in one plane and no more (2.3e-3 in the 2-norm where their own rounding
+// alone is 1.7e-3); states in f32 take three planes.
+template <typename T_, int NI_, int NS_, int NO_, int NU_, typename Saved_, int NB_>
+struct Mode {
+  typedef T_ T;
+  typedef Saved_ Saved;
+  static constexpr int NI = NI_, NS = NS_, NO = NO_, NU = NU_, NB = NB_;
+};
+typedef Mode<bf16, 1, 2, 1, 2, bf16, 1> ModeBf16;   // bf16 in and out
+typedef Mode<bf16, 1, 3, 1, 2, bf16, 1> ModeBf16S;  // with f32 states in or out
+typedef Mode<f16, 2, 3, 2, 2, float, 2> ModeF16;
+typedef Mode<float, 3, 3, 3, 3, float, 3> ModeF32;
 
 // What a chunk and value head have that depends on no state: matrices as
 // fragments of 16 rows and 32 terms, [row block][term block][lane][8], in
 // planes, and the decays.
-template <int NS, int NO>
+template <typename M>
 struct Record {
   static constexpr int kPlane = 64 * 64 * 2;
-  static constexpr int T = 0, P = NS * kPlane, Decay = P + NO * kPlane;  // Gam, G, beta: 64 f32 each
-  static constexpr int Tt = Decay + 768, Pt = Tt + NS * kPlane;          // transposed, for the backward pass
-  static constexpr int64_t bytes(bool back) { return back ? Pt + NS * kPlane : Tt; }
+  static constexpr int T = 0, P = M::NS * kPlane, Decay = P + M::NO * kPlane;  // Gam, G, beta: 64 f32 each
+  static constexpr int Tt = Decay + 768, Pt = Tt + M::NS * kPlane;             // transposed, for the backward pass
+  static constexpr int64_t bytes(bool back) { return back ? Pt + M::NS * kPlane : Tt; }
 };
-
-// Element type, planes of an input, of what makes a state, of what makes
-// only an output, and the type that states are saved in for the backward
-// pass with the planes they are read back in.
-template <typename T_, int NI_, int NS_, int NO_, typename Saved_, int NB_>
-struct Mode {
-  typedef T_ T;
-  typedef Saved_ Saved;
-  static constexpr int NI = NI_, NS = NS_, NO = NO_, NB = NB_;
-};
-typedef Mode<bf16, 1, 1, 1, bf16, 1> ModeBf16;    // bf16 in and out
-typedef Mode<bf16, 1, 3, 1, bf16, 1> ModeBf16S;   // with f32 states in or out
-typedef Mode<f16, 2, 3, 2, float, 2> ModeF16;
-typedef Mode<float, 3, 3, 3, float, 3> ModeF32;
 
 // A chunk: `first` is its first token, in the packed batch or in row `row`.
 struct Chunk {
@@ -130,22 +141,84 @@ __device__ __forceinline__ T *out_at(const Heads &x, int64_t row, int64_t token,
 }
 
 // Eight elements of token `t` of a chunk from element `d` on, of a head of
-// `dim`; zeros past the chunk or the head.
-template <typename T>
+// `dim` (a multiple of 8 if Fast): always loads, of an element that exists
+// where the one asked for does not, so that nothing branches and loads stay
+// in flight; keep_head8 makes what is past the chunk or the head zero once
+// they are needed.
+template <bool Fast, typename T>
 __device__ __forceinline__ Raw8<T> load_head8(const Heads &x, const Chunk &c, int head, int t, int d, int dim) {
-  const int n = t < c.len ? (dim - d < 0 ? 0 : dim - d > 8 ? 8 : dim - d) : 0;
-  return load8<T>(at<T>(x, c.row, c.first + t, head) + d, n);
+  const char *base = x.p + (c.row * x.b + c.first * x.t + head * x.h) * int64_t(sizeof(T));
+  const uint32_t row = uint32_t(t < c.len ? t : c.len - 1) * uint32_t(x.t);
+  Raw8<T> r;
+  if (Fast) {
+    const u32x4_any *s = reinterpret_cast<const u32x4_any *>(base + (row + uint32_t(d < dim ? d : dim - 8)) * uint32_t(sizeof(T)));
+    u32x4 *to = reinterpret_cast<u32x4 *>(&r);
+#pragma unroll
+    for (int i = 0; i < int(sizeof(T) * 8 / 16); i++) to[i] = s[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      r.x[i] = *reinterpret_cast<const T *>(base + (row + uint32_t(d + i < dim ? d + i : dim - 1)) * uint32_t(sizeof(T)));
+  }
+  return r;
+}
+
+template <bool Fast, typename T>
+__device__ __forceinline__ Raw8<T> keep_head8(Raw8<T> r, const Chunk &c, int t, int d, int dim) {
+  if (Fast) {
+    const bool live = t < c.len && d < dim;
+    u32x4 *x = reinterpret_cast<u32x4 *>(&r);
+#pragma unroll
+    for (int i = 0; i < int(sizeof(T) * 8 / 16); i++) x[i] = live ? x[i] : u32x4{};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) r.x[i] = t < c.len && d + i < dim ? r.x[i] : T(0.0f);
+  }
+  return r;
+}
+
+template <bool Fast, typename T>
+__device__ __forceinline__ Raw8<T> head8(const Heads &x, const Chunk &c, int head, int t, int d, int dim) {
+  return keep_head8<Fast>(load_head8<Fast, T>(x, c, head, t, d, dim), c, t, d, dim);
+}
+
+// One element in the same way.
+template <typename T>
+__device__ __forceinline__ T load_head1(const Heads &x, const Chunk &c, int head, int t, int d, int dim) {
+  const char *base = x.p + (c.row * x.b + c.first * x.t + head * x.h) * int64_t(sizeof(T));
+  const uint32_t row = uint32_t(t < c.len ? t : c.len - 1) * uint32_t(x.t);
+  return *reinterpret_cast<const T *>(base + (row + uint32_t(d < dim ? d : dim - 1)) * uint32_t(sizeof(T)));
+}
+
+// The first N planes of a fragment.
+template <int N, int M>
+__device__ __forceinline__ Frag<N> first_planes(const Frag<M> &f) {
+  Frag<N> r;
+#pragma unroll
+  for (int i = 0; i < N; i++) r.p[i] = f.p[i];
+  return r;
 }
 
 template <typename Mode>
 int64_t record_bytes(bool back) {
-  return Record<Mode::NS, Mode::NO>::bytes(back);
+  return Record<Mode>::bytes(back);
 }
 
 void delta_chunk_launch(const cchip_gated_delta &op, const DeltaArgs &a, bool back, hipStream_t stream);
 void delta_forward_launch(const cchip_gated_delta &op, const DeltaArgs &a, bool back, hipStream_t stream);
 void delta_backward_launch(const cchip_gated_delta &op, const DeltaArgs &a, hipStream_t stream);
 void delta_step_launch(const cchip_gated_delta &op, const DeltaArgs &a, hipStream_t stream);
+
+inline int padded_key_dim(int dk) { return dk <= 64 ? 64 : 128; }
+
+// Whether heads are read 8 elements at a time.
+inline bool fast(const DeltaArgs &a) { return a.dk % 8 == 0 && a.dv % 8 == 0; }
+
+template <typename F>
+void with_bool(bool x, F &&f) {
+  if (x) f(std::true_type());
+  else f(std::false_type());
+}
 
 // Calls f with the Mode of an operator.
 template <typename F>

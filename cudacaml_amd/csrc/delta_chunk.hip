@@ -49,11 +49,11 @@ __device__ __forceinline__ void put_block(float *to, const f32x4 &c, float sign)
 // lower triangle T_ij = -T_ii sum_m A_im T_mj, a diagonal of blocks at a
 // time. All of it is f32: entries of T add up 64 products deep, and every
 // state after the chunk carries what they lose.
-template <typename M, int DK, bool Back>
+template <typename M, int DK, bool Back, bool Fast>
 __global__ __launch_bounds__(256) void delta_chunk(const DeltaArgs a) {
   typedef typename M::T T;
   constexpr int NI = M::NI, LD = DK + 8, KPlane = 64 * LD;
-  typedef Record<M::NS, M::NO> R;
+  typedef Record<M> R;
   __shared__ __align__(16) bf16 ks[NI * KPlane];
   __shared__ __align__(16) float am[64 * kPad], tm[64 * kPad];
   __shared__ double cs[64];
@@ -87,9 +87,17 @@ __global__ __launch_bounds__(256) void delta_chunk(const DeltaArgs a) {
     dec[64 + l] = expf(float(last - s));
     dec[128 + l] = beta;
   }
-  for (int i = tid; i < 64 * (DK / 8); i += 256) {
-    const int t = i / (DK / 8), d = i % (DK / 8) * 8;
-    put_frag<NI>(ks + t * LD + d, KPlane, frag_of<NI>(load_head8<T>(a.k, c, hk, t, d, a.dk)));
+  Raw8<T> rk[DK / 32], rq[DK / 32];
+#pragma unroll
+  for (int j = 0; j < DK / 32; j++) {
+    const int i = tid + 256 * j;
+    rk[j] = load_head8<Fast, T>(a.k, c, hk, i / (DK / 8), i % (DK / 8) * 8, a.dk);
+    rq[j] = load_head8<Fast, T>(a.q, c, hk, 16 * w + col, 32 * j + quad * 8, a.dk);
+  }
+#pragma unroll
+  for (int j = 0; j < DK / 32; j++) {
+    const int i = tid + 256 * j, t = i / (DK / 8), d = i % (DK / 8) * 8;
+    put_frag<NI>(ks + t * LD + d, KPlane, frag_of<NI>(keep_head8<Fast>(rk[j], c, t, d, a.dk)));
   }
   for (int i = tid; i < 64 * kPad; i += 256) tm[i] = 0.0f;
   __syncthreads();
@@ -98,7 +106,7 @@ __global__ __launch_bounds__(256) void delta_chunk(const DeltaArgs a) {
 #pragma unroll
   for (int d = 0; d < DK; d += 32) {
     const Frag<NI> fk = frag_row<NI>(ks, KPlane, LD, 16 * w, d);
-    const Frag<NI> fq = frag_of<NI>(load_head8<T>(a.q, c, hk, 16 * w + col, d + quad * 8, a.dk));
+    const Frag<NI> fq = frag_of<NI>(keep_head8<Fast>(rq[d / 32], c, 16 * w + col, d + quad * 8, a.dk));
 #pragma unroll
     for (int j = 0; j < 4; j++)
       if (j <= w) {
@@ -171,9 +179,13 @@ void delta_chunk_launch(const cchip_gated_delta &op, const DeltaArgs &a, bool ba
   const int64_t grid = a.slots * a.hv;
   with_mode(op, [&](auto m) {
     typedef decltype(m) M;
-    auto *k = a.dk <= 64 ? (back ? delta_chunk<M, 64, true> : delta_chunk<M, 64, false>)
-                         : (back ? delta_chunk<M, 128, true> : delta_chunk<M, 128, false>);
-    hipLaunchKernelGGL(k, dim3(unsigned(grid)), dim3(256), 0, stream, a);
+    with_bool(back, [&](auto b) {
+      with_bool(fast(a), [&](auto f) {
+        constexpr bool B = decltype(b)::value, F = decltype(f)::value;
+        auto *k = a.dk <= 64 ? delta_chunk<M, 64, B, F> : delta_chunk<M, 128, B, F>;
+        hipLaunchKernelGGL(k, dim3(unsigned(grid)), dim3(256), 0, stream, a);
+      });
+    });
   });
   check_launch("gated delta: chunks");
 }
