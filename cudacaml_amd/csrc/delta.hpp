@@ -43,9 +43,10 @@ struct DeltaArgs {
   const float *dstate_out;
   float *dstate;
   char *records;  // one a (slot, value head)
-  // of each (slot, value head), rows of dvp elements; what pads a head is zero
-  char *states;   // saved S before the chunk, [DK][dvp]; null if there is no backward pass
-  float *us;      // saved U, [64][dvp]
+  // of each (slot, value head), in blocks of 32 value columns (put_block);
+  // what pads a head is zero
+  char *states;   // saved S before the chunk, DK rows; null if there is no backward pass
+  float *us;      // saved U, 64 rows
   char *grads;    // backward: dS after the chunk
   float *ys;      // backward: Y
   int64_t tokens, sequences;  // sequences: of the packed batch, or its rows
@@ -182,12 +183,141 @@ __device__ __forceinline__ Raw8<T> head8(const Heads &x, const Chunk &c, int hea
   return keep_head8<Fast>(load_head8<Fast, T>(x, c, head, t, d, dim), c, t, d, dim);
 }
 
-// One element in the same way.
+// Four in the same way, as f32, and the store of four.
 template <typename T>
-__device__ __forceinline__ T load_head1(const Heads &x, const Chunk &c, int head, int t, int d, int dim) {
+struct Raw4 {
+  T x[4];
+};
+template <typename T>
+struct Vector4;
+template <>
+struct Vector4<float> {
+  typedef u32x4_any type;
+};
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+template <>
+struct Vector4<bf16> {
+  typedef u32x2_any type;
+};
+template <>
+struct Vector4<f16> {
+  typedef u32x2_any type;
+};
+
+template <bool Fast, typename T>
+__device__ __forceinline__ Raw4<T> load_head4(const Heads &x, const Chunk &c, int head, int t, int d, int dim) {
   const char *base = x.p + (c.row * x.b + c.first * x.t + head * x.h) * int64_t(sizeof(T));
   const uint32_t row = uint32_t(t < c.len ? t : c.len - 1) * uint32_t(x.t);
-  return *reinterpret_cast<const T *>(base + (row + uint32_t(d < dim ? d : dim - 1)) * uint32_t(sizeof(T)));
+  Raw4<T> r;
+  if (Fast) {
+    typedef typename Vector4<T>::type V;
+    *reinterpret_cast<V *>(&r) = *reinterpret_cast<const V *>(base + (row + uint32_t(d < dim ? d : dim - 4)) * uint32_t(sizeof(T)));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      r.x[i] = *reinterpret_cast<const T *>(base + (row + uint32_t(d + i < dim ? d + i : dim - 1)) * uint32_t(sizeof(T)));
+  }
+  return r;
+}
+
+template <bool Fast, typename T>
+__device__ __forceinline__ void store_head4(const Heads &x, const Chunk &c, int head, int t, int d, int dim, const f32x4 &v) {
+  if (t >= c.len || d >= dim) return;
+  char *base = x.p + (c.row * x.b + c.first * x.t + head * x.h) * int64_t(sizeof(T));
+  char *to = base + (uint32_t(t) * uint32_t(x.t) + uint32_t(d)) * uint32_t(sizeof(T));
+  Raw4<T> r;
+#pragma unroll
+  for (int i = 0; i < 4; i++) r.x[i] = T(v[i]);
+  if (Fast) {
+    typedef typename Vector4<T>::type V;
+    *reinterpret_cast<V *>(to) = *reinterpret_cast<const V *>(&r);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (d + i < dim) reinterpret_cast<T *>(to)[i] = r.x[i];
+  }
+}
+
+// A lane of a transposed product has, of BV value columns, those from
+// BV / 4 quad on: TV = BV / 16 fragments' worth of four, read with frag_v.
+template <int N, int TV>
+__device__ __forceinline__ Frag<N> frag_v(const bf16 *m, int plane, int ld, int j, int term0) {
+  return frag_col<N, 4 * TV>(m, plane, ld, 4 * j, term0);
+}
+
+// A lane's 4 TV elements of token t of a tensor, zero past the chunk or the
+// head, and their store.
+template <typename T, int TV>
+struct RawV {
+  T x[4 * TV];
+};
+
+template <bool Fast, typename T, int TV>
+__device__ __forceinline__ RawV<T, TV> load_v(const Heads &x, const Chunk &c, int head, int t, int d, int dim) {
+  union {
+    RawV<T, TV> v;
+    Raw4<T> r4;
+    Raw8<T> r8;
+  } u;
+  if constexpr (TV == 2) u.r8 = load_head8<Fast, T>(x, c, head, t, d, dim);
+  else u.r4 = load_head4<Fast, T>(x, c, head, t, d, dim);
+  return u.v;
+}
+
+template <bool Fast, typename T, int TV>
+__device__ __forceinline__ void store_v(const Heads &x, const Chunk &c, int head, int t, int d, int dim, const f32x4 (&v)[TV]) {
+  if (t >= c.len || d >= dim) return;
+  char *base = x.p + (c.row * x.b + c.first * x.t + head * x.h) * int64_t(sizeof(T));
+  char *to = base + (uint32_t(t) * uint32_t(x.t) + uint32_t(d)) * uint32_t(sizeof(T));
+  union {
+    RawV<T, TV> r;
+    u32x4 w[sizeof(RawV<T, TV>) >= 16 ? sizeof(RawV<T, TV>) / 16 : 1];
+    uint64_t half;
+  } u;
+#pragma unroll
+  for (int i = 0; i < 4 * TV; i++) u.r.x[i] = T(v[i / 4][i % 4]);
+  if (Fast) {
+    if constexpr (sizeof(u.r) >= 16) {
+#pragma unroll
+      for (int i = 0; i < int(sizeof(u.r) / 16); i++) reinterpret_cast<u32x4_any *>(to)[i] = u.w[i];
+    } else {
+      *reinterpret_cast<u32x2_any *>(to) = __builtin_bit_cast(u32x2_any, u.half);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4 * TV; i++)
+      if (d + i < dim) reinterpret_cast<T *>(to)[i] = u.r.x[i];
+  }
+}
+
+// Buffers between kernels hold value columns in blocks of 32, [block][row][32]:
+// a workgroup writes whole lines, and a reader takes a block in one piece.
+// `y`: the lane's first column of the block.
+template <typename T, int TV>
+__device__ __forceinline__ void put_block(char *rows, int row, int y, const f32x4 (&v)[TV]) {
+  union {
+    RawV<T, TV> r;
+    u32x4 w[sizeof(RawV<T, TV>) >= 16 ? sizeof(RawV<T, TV>) / 16 : 1];
+    uint64_t half;
+  } u;
+#pragma unroll
+  for (int i = 0; i < 4 * TV; i++) u.r.x[i] = T(v[i / 4][i % 4]);
+  char *to = rows + uint32_t(row * 32 + y) * uint32_t(sizeof(T));
+  if constexpr (sizeof(u.r) >= 16) {
+#pragma unroll
+    for (int i = 0; i < int(sizeof(u.r) / 16); i++) reinterpret_cast<u32x4 *>(to)[i] = u.w[i];
+  } else {
+    *reinterpret_cast<uint64_t *>(to) = u.half;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ Raw8<T> load_block8(const char *rows, uint32_t at) {
+  Raw8<T> r;
+#pragma unroll
+  for (int i = 0; i < int(sizeof(T) * 8 / 16); i++)
+    reinterpret_cast<u32x4 *>(&r)[i] = reinterpret_cast<const u32x4 *>(rows + at * uint32_t(sizeof(T)))[i];
+  return r;
 }
 
 // The first N planes of a fragment.

@@ -26,21 +26,20 @@ namespace cchip {
 namespace op {
 namespace {
 
-// The counterpart of delta_forward: BV value columns of a head, E in
-// registers, each chunk's rows asked for while the one after it is computed.
+// The counterpart of delta_forward, laid out like it: BV value columns of a
+// head, E in registers, each chunk's rows asked for while the one after it is
+// computed.
 template <typename M, int DK, int BV, bool Fast>
 __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int blocks) {
   typedef typename M::T T;
   typedef typename M::Saved Saved;
   constexpr int NI = M::NI, NS = M::NS;
-  constexpr int LDK = DK + 8, LDT = 72, LDV = BV + 8;
-  constexpr int KP = 64 * LDK, SP = BV * LDK, XP = BV * LDT, VP = 64 * LDV;
+  constexpr int LDK = DK + 8, LDV = BV + 8;
+  constexpr int KP = 64 * LDK, EP = DK * LDV, XP = 64 * LDV;
   constexpr int TK = DK / 64, TV = BV / 16;
   typedef Record<M> R;
-  __shared__ __align__(16) bf16 ks[NI * KP], qs[NI * KP], et[NS * SP], xt[NS * XP], os[NI * VP], gs[NS * VP];
-  static_assert(SP >= XP || DK < 128, "Z does not fit where E was");
-  __shared__ __align__(16) bf16 own[DK < 128 ? NS * XP : 8];
-  bf16 *const zt = DK < 128 ? own : et;  // E is done with when Z is made
+  __shared__ __align__(16) bf16 ks[NI * KP], qs[NI * KP], es[NS * EP], xs[NS * XP], os[NI * XP], gs[NS * XP];
+  bf16 *const zs = es;  // E is done with when Z is made
 
   const int64_t group = blockIdx.x / (8 * blocks);
   const int rest = int(blockIdx.x - group * 8 * blocks);
@@ -52,20 +51,20 @@ __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int b
   const int chunks = int((sq.len + kChunk - 1) / kChunk);
 
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, quad = l >> 4, col = l & 15;
-  const int row0 = w * (DK / 4) + quad * 4;
+  const int x0 = w * (DK / 4) + col, y0 = 4 * TV * quad, t = 16 * w + col;
   const int ot = tid / (BV / 8), od = tid % (BV / 8) * 8;  // this thread's piece of dO, if it has one
   const bool has_o = tid < 64 * (BV / 8);
 
   f32x4 e[TK][TV];
-  const int64_t state_at = lane_id * a.dk * a.dv;
+  const int64_t state_at = lane_id * a.dk * a.dv + dv0;
 #pragma unroll
   for (int i = 0; i < TK; i++)
 #pragma unroll
     for (int j = 0; j < TV; j++)
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const int x = row0 + 16 * i + r, y = dv0 + 16 * j + col;
-        e[i][j][r] = a.dstate_out && x < a.dk && y < a.dv ? a.dstate_out[state_at + int64_t(x) * a.dv + y] : 0.0f;
+        const int x = x0 + 16 * i, y = y0 + 4 * j + r;
+        e[i][j][r] = a.dstate_out && x < a.dk && dv0 + y < a.dv ? a.dstate_out[state_at + int64_t(x) * a.dv + y] : 0.0f;
       }
 
   auto chunk = [&](int i) {
@@ -75,7 +74,7 @@ __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int b
   auto record = [&](int i) { return a.records + ((sq.slot + i) * a.hv + h) * R::bytes(true); };
   Raw8<T> rk[DK / 32], rq[DK / 32], ro;
   Frag<NS> tt[2], pt[2];  // rows 16 w .. of T^T and P^T: terms from the diagonal on
-  float og;
+  float og, gam, last, beta, end;
   auto fetch = [&](int i) {
     const Chunk c = chunk(i);
 #pragma unroll
@@ -89,131 +88,147 @@ __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int b
       og = reinterpret_cast<const float *>(record(i) + R::Decay)[ot];
     }
   };
+  auto fetch_end = [&](int i) { end = reinterpret_cast<const float *>(record(i) + R::Decay)[63]; };
+  auto fragment = [&](const char *from, int b) {
+    return *reinterpret_cast<const bf16x8 *>(from + uint32_t((w * 2 + b) * 1024 + l * 16));
+  };
   auto fetch_p = [&](int i) {
 #pragma unroll
     for (int b = 0; b < 2; b++)
       if (b == 1 || w < 2)
 #pragma unroll
-        for (int p = 0; p < NS; p++)
-          pt[b].p[p] = reinterpret_cast<const bf16x8 *>(record(i) + R::Pt + p * 8192)[(w * 2 + b) * 64 + l];
+        for (int p = 0; p < NS; p++) pt[b].p[p] = fragment(record(i) + R::Pt + p * 8192, b);
   };
   auto fetch_t = [&](int i) {
 #pragma unroll
     for (int b = 0; b < 2; b++)
       if (b == 1 || w < 2)
 #pragma unroll
-        for (int p = 0; p < NS; p++)
-          tt[b].p[p] = reinterpret_cast<const bf16x8 *>(record(i) + R::Tt + p * 8192)[(w * 2 + b) * 64 + l];
+        for (int p = 0; p < NS; p++) tt[b].p[p] = fragment(record(i) + R::Tt + p * 8192, b);
+    const float *dec = reinterpret_cast<const float *>(record(i) + R::Decay);
+    gam = dec[t];
+    last = dec[64 + t];
+    beta = dec[128 + t];
   };
   if (chunks > 0) {
     fetch(chunks - 1);
     fetch_p(chunks - 1);
     fetch_t(chunks - 1);
+    fetch_end(chunks - 1);
   }
   for (int ci = chunks - 1; ci >= 0; ci--) {
     const Chunk c = chunk(ci);
     const int next = ci ? ci - 1 : 0;
     const int64_t slot_head = (sq.slot + ci) * a.hv + h;
-    const float *dec = reinterpret_cast<const float *>(record(ci) + R::Decay);
 #pragma unroll
     for (int j = 0; j < DK / 32; j++) {
-      const int at = tid + 256 * j, t = at / (DK / 8), d = at % (DK / 8) * 8;
-      put_frag<NI>(ks + t * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rk[j], c, t, d, a.dk)));
-      put_frag<NI>(qs + t * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rq[j], c, t, d, a.dk)));
+      const int at = tid + 256 * j, kt = at / (DK / 8), d = at % (DK / 8) * 8;
+      put_frag<NI>(ks + kt * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rk[j], c, kt, d, a.dk)));
+      put_frag<NI>(qs + kt * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rq[j], c, kt, d, a.dk)));
     }
     if (has_o) {
       const Raw8<T> raw = keep_head8<Fast>(ro, c, ot, dv0 + od, a.dv);
-      put_frag<NI>(os + ot * LDV + od, VP, frag_of<NI>(raw));
+      put_frag<NI>(os + ot * LDV + od, XP, frag_of<NI>(raw));
       const float f = a.scale * og;
       Raw8<float> up;
 #pragma unroll
       for (int i = 0; i < 8; i++) up.x[i] = f * float(raw.x[i]);
-      put_frag<NS>(gs + ot * LDV + od, VP, frag_of<NS>(up));
+      put_frag<NS>(gs + ot * LDV + od, XP, frag_of<NS>(up));
     }
 #pragma unroll
     for (int i = 0; i < TK; i++)
 #pragma unroll
-      for (int j = 0; j < TV; j++) put_column<NS>(et + (16 * j + col) * LDK + row0 + 16 * i, SP, e[i][j]);
-    float gam[4], last[4], beta[4];
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const int t = 16 * w + 4 * quad + r;
-      gam[r] = dec[t];
-      last[r] = dec[64 + t];
-      beta[r] = dec[128 + t];
-    }
-    const float end = dec[63];
+      for (int j = 0; j < TV; j++) put_four<NS>(es + (x0 + 16 * i) * LDV + y0 + 4 * j, EP, e[i][j]);
     __syncthreads();
     fetch(next);
-    Saved *es = reinterpret_cast<Saved *>(a.grads) + slot_head * DK * a.dvp + dv0;
+    char *to = a.grads + (slot_head * a.dvp + dv0 / 32 * 32) * DK * int64_t(sizeof(Saved));
 #pragma unroll
-    for (int i = 0; i < TK; i++)
-#pragma unroll
-      for (int j = 0; j < TV; j++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) es[(row0 + 16 * i + r) * a.dvp + 16 * j + col] = Saved(e[i][j][r]);
+    for (int i = 0; i < TK; i++) put_block<Saved, TV>(to, x0 + 16 * i, dv0 % 32 + y0, e[i]);
 
     f32x4 ke[TV] = {}, du[TV] = {};
+    {
+      // operands first, products after: one wait for LDS, not one a product
+      Frag<NI> fk[DK / 32], fo[2][TV];
+      Frag<NS> fe[DK / 32][TV];
 #pragma unroll
-    for (int d = 0; d < DK; d += 32) {
-      const Frag<NI> fk = frag_row<NI>(ks, KP, LDK, 16 * w, d);
+      for (int d = 0; d < DK / 32; d++) {
+        fk[d] = frag_row<NI>(ks, KP, LDK, 16 * w, 32 * d);
 #pragma unroll
-      for (int j = 0; j < TV; j++) ke[j] = mma(ke[j], fk, frag_row<NS>(et, SP, LDK, 16 * j, d));
+        for (int j = 0; j < TV; j++) fe[d][j] = frag_v<NS, TV>(es, EP, LDV, j, 32 * d);
+      }
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int j = 0; j < TV; j++) fo[b][j] = frag_v<NI, TV>(os, XP, LDV, j, 32 * b);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int d = 0; d < DK / 32; d++)
+#pragma unroll
+        for (int j = 0; j < TV; j++) ke[j] = mma(ke[j], fe[d][j], fk[d]);
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+        if (b == 1 || w < 2)
+#pragma unroll
+          for (int j = 0; j < TV; j++) du[j] = mma(du[j], fo[b][j], pt[b]);
     }
-#pragma unroll
-    for (int b = 0; b < 2; b++)
-      if (b == 1 || w < 2)
-#pragma unroll
-        for (int j = 0; j < TV; j++) du[j] = mma(du[j], pt[b], frag_col<NI>(os, VP, LDV, 16 * j, 32 * b));
     fetch_p(next);
 #pragma unroll
     for (int j = 0; j < TV; j++) {
-#pragma unroll
-      for (int r = 0; r < 4; r++) du[j][r] = a.scale * du[j][r] + last[r] * ke[j][r];
-      put_column<NS>(xt + (16 * j + col) * LDT + 16 * w + 4 * quad, XP, du[j]);
+      du[j] = a.scale * du[j] + last * ke[j];
+      put_four<NS>(xs + t * LDV + y0 + 4 * j, XP, du[j]);
     }
     __syncthreads();
     f32x4 y[TV] = {};
+    {
+      Frag<NS> fx[2][TV];
 #pragma unroll
-    for (int b = 0; b < 2; b++)
-      if (b == 1 || w < 2)
+      for (int b = 0; b < 2; b++)
 #pragma unroll
-        for (int j = 0; j < TV; j++) y[j] = mma(y[j], tt[b], frag_row<NS>(xt, XP, LDT, 16 * j, 32 * b));
-    fetch_t(next);
-    float *ys = a.ys + slot_head * kChunk * a.dvp + dv0;
+        for (int j = 0; j < TV; j++) fx[b][j] = frag_v<NS, TV>(xs, XP, LDV, j, 32 * b);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+        if (b == 1 || w < 2)
+#pragma unroll
+          for (int j = 0; j < TV; j++) y[j] = mma(y[j], fx[b][j], tt[b]);
+    }
+    put_block<float, TV>(reinterpret_cast<char *>(a.ys + (slot_head * a.dvp + dv0 / 32 * 32) * kChunk), t, dv0 % 32 + y0, y);
 #pragma unroll
     for (int j = 0; j < TV; j++) {
-      f32x4 z;
-#pragma unroll
-      for (int r = 0; r < 4; r++) z[r] = -gam[r] * beta[r] * y[j][r];
-      put_column<NS>(zt + (16 * j + col) * LDT + 16 * w + 4 * quad, XP, z);
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int t = 16 * w + 4 * quad + r, v = 16 * j + col;
-        ys[t * a.dvp + v] = y[j][r];
-        if (t < c.len && dv0 + v < a.dv) out_at<T>(a.gv, c.row, c.first + t, h)[dv0 + v] = T(beta[r] * y[j][r]);
-      }
+      put_four<NS>(zs + t * LDV + y0 + 4 * j, EP, (-gam * beta) * y[j]);
+      y[j] *= beta;
     }
+    store_v<Fast, T, TV>(a.gv, c, h, t, dv0 + y0, a.dv, y);
+    fetch_t(next);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < TK; i++)
 #pragma unroll
       for (int j = 0; j < TV; j++) e[i][j] *= end;
+    fetch_end(next);
 #pragma unroll
     for (int b = 0; b < 2; b++) {
       Frag<NS> fg[TV], fz[TV];
+      Frag<NI> fq[TK], fk[TK];
 #pragma unroll
       for (int j = 0; j < TV; j++) {
-        fg[j] = frag_col<NS>(gs, VP, LDV, 16 * j, 32 * b);
-        fz[j] = frag_row<NS>(zt, XP, LDT, 16 * j, 32 * b);
+        fg[j] = frag_v<NS, TV>(gs, XP, LDV, j, 32 * b);
+        fz[j] = frag_v<NS, TV>(zs, EP, LDV, j, 32 * b);
       }
 #pragma unroll
       for (int i = 0; i < TK; i++) {
-        const Frag<NI> fq = frag_col<NI>(qs, KP, LDK, w * (DK / 4) + 16 * i, 32 * b);
-        const Frag<NI> fk = frag_col<NI>(ks, KP, LDK, w * (DK / 4) + 16 * i, 32 * b);
-#pragma unroll
-        for (int j = 0; j < TV; j++) e[i][j] = mma(mma(e[i][j], fq, fg[j]), fk, fz[j]);
+        fq[i] = frag_col<NI>(qs, KP, LDK, w * (DK / 4) + 16 * i, 32 * b);
+        fk[i] = frag_col<NI>(ks, KP, LDK, w * (DK / 4) + 16 * i, 32 * b);
       }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < TK; i++)
+#pragma unroll
+        for (int j = 0; j < TV; j++) e[i][j] = mma(e[i][j], fg[j], fq[i]);
+#pragma unroll
+      for (int i = 0; i < TK; i++)
+#pragma unroll
+        for (int j = 0; j < TV; j++) e[i][j] = mma(e[i][j], fz[j], fk[i]);
     }
     __syncthreads();
   }
@@ -224,25 +239,17 @@ __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int b
       for (int j = 0; j < TV; j++)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-          const int x = row0 + 16 * i + r, y = dv0 + 16 * j + col;
-          if (x < a.dk && y < a.dv) a.dstate[state_at + int64_t(x) * a.dv + y] = e[i][j][r];
+          const int x = x0 + 16 * i, y = y0 + 4 * j + r;
+          if (x < a.dk && dv0 + y < a.dv) a.dstate[state_at + int64_t(x) * a.dv + y] = e[i][j][r];
         }
-}
-
-// Eight neighbouring elements of an inner buffer, which has no ragged edges.
-template <typename T>
-__device__ __forceinline__ Raw8<T> load_inner8(const T *p) {
-  Raw8<T> r;
-#pragma unroll
-  for (int i = 0; i < int(sizeof(T) * 8 / 16); i++) reinterpret_cast<u32x4 *>(&r)[i] = reinterpret_cast<const u32x4 *>(p)[i];
-  return r;
 }
 
 // A workgroup of eight waves a chunk and key head, its value heads one after
 // another (so dQ and dK of a shared head are summed in registers, in an order
-// that is always the same). Wave w has rows 16 (w % 4) .. of every product
-// and half w / 4 of its columns; S, E and U pass through LDS 32 value columns
-// at a time, the next 32 being read while the products of these are made.
+// that is always the same). Products are taken transposed, as in the forward
+// pass: wave w has tokens 16 (w % 4) .. of each and half w / 4 of the rest,
+// and a lane one token. S, E and U pass through LDS 32 value columns at a
+// time, the next 32 being read while the products of these are made.
 template <typename M, int DK, bool Fast>
 __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
   typedef typename M::T T;
@@ -255,7 +262,8 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
   constexpr int kSlices = (kBoth ? 2 : 1) * NB * SP + NU * UP, kMs = (kBoth ? 2 : 1) * NB * MP;
   __shared__ __align__(16) bf16 ks[NI * KP], qs[NI * KP], slice[kSlices > kMs ? kSlices : kMs];
   __shared__ double cs[64];
-  __shared__ float down[4][64], row_c[2][64], row_b[2][64], total[8];
+  __shared__ __align__(16) float down[4][64];
+  __shared__ float row_c[2][64], row_b[2][64], total[8];
   bf16 *const us = slice, *const ss = slice + NU * UP, *const es = kBoth ? ss + NB * SP : ss;
   bf16 *const ms = slice, *const bs = kBoth ? slice + NB * MP : slice;
 
@@ -265,6 +273,9 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
   if (c.len == 0) return;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, quad = l >> 4, col = l & 15;
   const int wr = w & 3, half = w >> 2;
+  const int t = 16 * wr + col;                  // this lane's token
+  const int x0 = 16 * JK * half + 4 * quad;     // its part of a key: x0 + 16 j + r
+  const int s0 = 32 * half + 4 * quad;          // and of the tokens before it: s0 + 16 j + r
 
   {
     Raw8<T> rk[DK / 64], rq[DK / 64];
@@ -276,43 +287,47 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
     }
 #pragma unroll
     for (int j = 0; j < DK / 64; j++) {
-      const int at = tid + 512 * j, t = at / (DK / 8), d = at % (DK / 8) * 8;
-      put_frag<NI>(ks + t * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rk[j], c, t, d, a.dk)));
-      put_frag<NI>(qs + t * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rq[j], c, t, d, a.dk)));
+      const int at = tid + 512 * j, kt = at / (DK / 8), d = at % (DK / 8) * 8;
+      put_frag<NI>(ks + kt * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rk[j], c, kt, d, a.dk)));
+      put_frag<NI>(qs + kt * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rq[j], c, kt, d, a.dk)));
     }
   }
-  // element (t, d) of K or Q as its planes add up
-  auto value = [&](const bf16 *m, int t, int d) {
-    float x = 0.0f;
+  // four elements of this lane's row of K or Q as their planes add up
+  auto value4 = [&](const bf16 *m, int d) {
+    f32x4 x = {};
 #pragma unroll
-    for (int p = NI - 1; p >= 0; p--) x += float(m[p * KP + t * LDK + d]);
+    for (int p = NI - 1; p >= 0; p--) {
+      const bf16x4 v = *reinterpret_cast<const bf16x4 *>(m + p * KP + t * LDK + d);
+#pragma unroll
+      for (int r = 0; r < 4; r++) x[r] += float(v[r]);
+    }
     return x;
   };
   // this thread's pieces of a slice: of S and E (row sx), and of U (row ux)
-  const int sx = tid / 4, sv = tid % 4 * 8, ux = (tid & 255) / 4, uv = tid % 4 * 8;
+  const int sx = tid / 4, sv = tid % 4 * 8, ux = (tid & 255) / 4;
   const bool has_s = sx < DK, has_u = tid < 256;
-  const int t_own = 16 * wr + col;
 
   f32x4 dq[JK] = {}, dk[JK] = {};
   for (int h = hk * per; h < (hk + 1) * per; h++) {
     const int64_t slot_head = slot * a.hv + h;
     const float *dec = reinterpret_cast<const float *>(a.records + slot_head * R::bytes(true) + R::Decay);
-    const Saved *S = reinterpret_cast<const Saved *>(a.states) + slot_head * DK * a.dvp;
-    const Saved *E = reinterpret_cast<const Saved *>(a.grads) + slot_head * DK * a.dvp;
-    const float *U = a.us + slot_head * kChunk * a.dvp, *Y = a.ys + slot_head * kChunk * a.dvp;
+    const char *S = a.states + slot_head * DK * a.dvp * int64_t(sizeof(Saved));
+    const char *E = a.grads + slot_head * DK * a.dvp * int64_t(sizeof(Saved));
+    const char *U = reinterpret_cast<const char *>(a.us + slot_head * kChunk * a.dvp);
+    const char *Y = reinterpret_cast<const char *>(a.ys + slot_head * kChunk * a.dvp);
 
     Raw8<Saved> rs, re;
     Raw8<float> ru, ry;
     Raw8<T> ro, rv;
     auto fetch = [&](int v0) {
       if (has_s) {
-        rs = load_inner8(S + sx * a.dvp + v0 + sv);
-        re = load_inner8(E + sx * a.dvp + v0 + sv);
+        rs = load_block8<Saved>(S, uint32_t(v0 * DK + sx * 32 + sv));
+        re = load_block8<Saved>(E, uint32_t(v0 * DK + sx * 32 + sv));
       }
-      if (has_u) ru = load_inner8(U + ux * a.dvp + v0 + uv);
-      ry = load_inner8(Y + t_own * a.dvp + v0 + 8 * quad);
-      ro = load_head8<Fast, T>(a.d_o, c, h, t_own, v0 + 8 * quad, a.dv);
-      rv = load_head8<Fast, T>(a.v, c, h, t_own, v0 + 8 * quad, a.dv);
+      if (has_u) ru = load_block8<float>(U, uint32_t(v0 * 64 + ux * 32 + sv));
+      ry = load_block8<float>(Y, uint32_t(v0 * 64 + t * 32 + 8 * quad));
+      ro = load_head8<Fast, T>(a.d_o, c, h, t, v0 + 8 * quad, a.dv);
+      rv = load_head8<Fast, T>(a.v, c, h, t, v0 + 8 * quad, a.dv);
     };
     fetch(0);
     double run = 0.0;  // the running sum of g, as delta_chunk makes it
@@ -329,14 +344,14 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
     if (w == 0) cs[l] = run;
 
     f32x4 os[JK] = {}, ys[JK] = {}, ue[JK] = {}, ou[2] = {}, yu[2] = {};
-    float yv = 0.0f, se = 0.0f;  // yv: of row t_own, this lane's columns
+    float yv = 0.0f, se = 0.0f;  // yv: this lane's columns
     for (int v0 = 0; v0 < a.dvp; v0 += 32) {
-      const Frag<NI> fo = frag_of<NI>(keep_head8<Fast>(ro, c, t_own, v0 + 8 * quad, a.dv));
+      const Frag<NI> fo = frag_of<NI>(keep_head8<Fast>(ro, c, t, v0 + 8 * quad, a.dv));
       const Frag<NU> fy = frag_of<NU>(ry);
-      const Raw8<T> v = keep_head8<Fast>(rv, c, t_own, v0 + 8 * quad, a.dv);
+      const Raw8<T> v = keep_head8<Fast>(rv, c, t, v0 + 8 * quad, a.dv);
 #pragma unroll
       for (int i = 0; i < 8; i++) yv += ry.x[i] * float(v.x[i]);
-      if (has_u) put_frag<NU>(us + ux * LDS + uv, UP, frag_of<NU>(ru));
+      if (has_u) put_frag<NU>(us + ux * LDS + sv, UP, frag_of<NU>(ru));
       Raw8<Saved> late = re;
       if (has_s) {
 #pragma unroll
@@ -351,50 +366,42 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
       for (int j = 0; j < JK; j++) {
         const int x = 16 * (JK * half + j);
         const Frag<NB> fs = frag_row<NB>(ss, SP, LDS, x, 0);
-        os[j] = mma(os[j], fo, fs);
-        ys[j] = mma(ys[j], fy, fs);
-        if (kBoth) ue[j] = mma(ue[j], fu, frag_row<NB>(es, SP, LDS, x, 0));
+        os[j] = mma(os[j], fs, fo);
+        ys[j] = mma(ys[j], fs, fy);
+        if (kBoth) ue[j] = mma(ue[j], frag_row<NB>(es, SP, LDS, x, 0), fu);
       }
 #pragma unroll
       for (int j = 0; j < 2; j++)
         if (2 * half + j <= wr) {
           const Frag<NU> f = frag_row<NU>(us, UP, LDS, 16 * (2 * half + j), 0);
-          ou[j] = mma(ou[j], fo, f);
-          yu[j] = mma(yu[j], fy, f);
+          ou[j] = mma(ou[j], f, fo);
+          yu[j] = mma(yu[j], f, fy);
         }
       __syncthreads();
       if (!kBoth) {
         if (has_s) put_frag<NB>(es + sx * LDS + sv, SP, frag_of<NB>(late));
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < JK; j++) ue[j] = mma(ue[j], fu, frag_row<NB>(es, SP, LDS, 16 * (JK * half + j), 0));
+        for (int j = 0; j < JK; j++) ue[j] = mma(ue[j], frag_row<NB>(es, SP, LDS, 16 * (JK * half + j), 0), fu);
         __syncthreads();
       }
     }
 
-    // this lane's rows t = 16 wr + 4 quad + r
-    float gam[4], last[4], beta[4], dc[4], db[4], end = 0.0f;
+    const float gam = dec[t], last = dec[64 + t], beta = dec[128 + t];
+    float dc = 0.0f, db = half == 0 ? yv : 0.0f, end = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const int t = 16 * wr + 4 * quad + r;
-      gam[r] = dec[t];
-      last[r] = dec[64 + t];
-      beta[r] = dec[128 + t];
-      dc[r] = db[r] = 0.0f;
-    }
-#pragma unroll
-    for (int j = 0; j < JK; j++)
+    for (int j = 0; j < JK; j++) {
+      const f32x4 kv = value4(ks, x0 + 16 * j), qv = value4(qs, x0 + 16 * j);
+      const f32x4 o = (a.scale * gam) * os[j], y = gam * ys[j], u = last * ue[j];
+      dq[j] += o;
+      dk[j] += u - beta * y;
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const int t = 16 * wr + 4 * quad + r, d = 16 * (JK * half + j) + col;
-        const float kv = value(ks, t, d), qv = value(qs, t, d);
-        const float o = a.scale * gam[r] * os[j][r], y = gam[r] * ys[j][r], u = last[r] * ue[j][r];
-        dq[j][r] += o;
-        dk[j][r] += u - beta[r] * y;
-        dc[r] += qv * o - beta[r] * kv * y - kv * u;
-        db[r] -= kv * y;
-        end += kv * u;
+        dc += qv[r] * o[r] - kv[r] * (beta * y[r] + u[r]);
+        db -= kv[r] * y[r];
+        end += kv[r] * u[r];
       }
+    }
     f32x4 kk[2] = {}, qk[2] = {};
 #pragma unroll
     for (int d = 0; d < DK; d += 32) {
@@ -403,41 +410,34 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
       for (int j = 0; j < 2; j++)
         if (2 * half + j <= wr) {
           const Frag<NI> fs = frag_row<NI>(ks, KP, LDK, 16 * (2 * half + j), d);
-          kk[j] = mma(kk[j], fk, fs);
-          qk[j] = mma(qk[j], fq, fs);
+          kk[j] = mma(kk[j], fs, fk);
+          qk[j] = mma(qk[j], fs, fq);
         }
     }
     f32x4 b[2];
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-      float across = 0.0f;
-      f32x4 m;
+      f32x4 m, across;
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const int t = 16 * wr + 4 * quad + r, s = 16 * (2 * half + j) + col;
+        const int s = s0 + 16 * j + r;
         const float d = s <= t ? expf(float(cs[t] - cs[s])) : 0.0f;
         m[r] = s <= t ? a.scale * d * ou[j][r] : 0.0f;
-        b[j][r] = s < t ? -beta[r] * d * yu[j][r] : 0.0f;
+        b[j][r] = s < t ? -beta * d * yu[j][r] : 0.0f;
         const float pair = m[r] * qk[j][r] + b[j][r] * kk[j][r];
-        dc[r] += pair;
-        across += pair;
-        db[r] -= s < t ? yu[j][r] * d * kk[j][r] : 0.0f;
+        dc += pair;
+        across[r] = sum16(pair);
+        db -= s < t ? yu[j][r] * d * kk[j][r] : 0.0f;
       }
-      across = sum_rows(across);
-      if (quad == 0) down[wr][16 * (2 * half + j) + col] = across;
-      // M is stored [s][t]
-      put_column<NB>(ms + (16 * (2 * half + j) + col) * LDM + 16 * wr + 4 * quad, MP, m);
-      if (kBoth) put_column<NB>(bs + (16 * (2 * half + j) + col) * LDM + 16 * wr + 4 * quad, MP, b[j]);
+      if (col == 0) *reinterpret_cast<f32x4 *>(&down[wr][s0 + 16 * j]) = across;
+      put_four<NB>(ms + t * LDM + s0 + 16 * j, MP, m);
+      if (kBoth) put_four<NB>(bs + t * LDM + s0 + 16 * j, MP, b[j]);
     }
-    yv = half == 0 ? sum_rows(yv) : 0.0f;  // lane i: of row 16 wr + i % 16
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const int t = 16 * wr + 4 * quad + r;
-      const float x = sum16(dc[r]), y = sum16(db[r]) + __shfl(yv, 4 * quad + r, 64);
-      if (col == 0) {
-        row_c[half][t] = x;
-        row_b[half][t] = y;
-      }
+    dc = sum_rows(dc);
+    db = sum_rows(db);
+    if (quad == 0) {
+      row_c[half][t] = dc;
+      row_b[half][t] = db;
     }
     end = sum64(end + se * dec[63]);
     if (l == 0) total[w] = end;
@@ -458,44 +458,38 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
 #pragma unroll
     for (int t0 = 0; t0 < 64; t0 += 32) {
       if (t0 == 0 || wr >= 2) {  // M ends at the diagonal
-        const Frag<NB> f = frag_col<NB>(ms, MP, LDM, 16 * wr, t0);
-#pragma unroll
-        for (int j = 0; j < JK; j++) dq[j] = mma(dq[j], f, frag_col<NI>(ks, KP, LDK, 16 * (JK * half + j), t0));
-      }
-      if (t0 != 0 || wr < 2) {
         const Frag<NB> f = frag_row<NB>(ms, MP, LDM, 16 * wr, t0);
 #pragma unroll
-        for (int j = 0; j < JK; j++) dk[j] = mma(dk[j], f, frag_col<NI>(qs, KP, LDK, 16 * (JK * half + j), t0));
+        for (int j = 0; j < JK; j++) dq[j] = mma(dq[j], frag_col<NI>(ks, KP, LDK, 16 * (JK * half + j), t0), f);
+      }
+      if (t0 != 0 || wr < 2) {
+        const Frag<NB> f = frag_col<NB>(ms, MP, LDM, 16 * wr, t0);
+#pragma unroll
+        for (int j = 0; j < JK; j++) dk[j] = mma(dk[j], frag_col<NI>(qs, KP, LDK, 16 * (JK * half + j), t0), f);
       }
     }
     if (!kBoth) {
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < 2; j++)
-        put_column<NB>(bs + (16 * (2 * half + j) + col) * LDM + 16 * wr + 4 * quad, MP, b[j]);
+      for (int j = 0; j < 2; j++) put_four<NB>(bs + t * LDM + s0 + 16 * j, MP, b[j]);
       __syncthreads();
     }
 #pragma unroll
     for (int t0 = 0; t0 < 64; t0 += 32) {
-      const Frag<NB> fb = frag_col<NB>(bs, MP, LDM, 16 * wr, t0), ft = frag_row<NB>(bs, MP, LDM, 16 * wr, t0);
+      const Frag<NB> fb = frag_row<NB>(bs, MP, LDM, 16 * wr, t0), ft = frag_col<NB>(bs, MP, LDM, 16 * wr, t0);
 #pragma unroll
       for (int j = 0; j < JK; j++) {
         const Frag<NI> fk = frag_col<NI>(ks, KP, LDK, 16 * (JK * half + j), t0);
-        if (t0 == 0 || wr >= 2) dk[j] = mma(dk[j], fb, fk);
-        if (t0 != 0 || wr < 2) dk[j] = mma(dk[j], ft, fk);
+        if (t0 == 0 || wr >= 2) dk[j] = mma(dk[j], fk, fb);
+        if (t0 != 0 || wr < 2) dk[j] = mma(dk[j], fk, ft);
       }
     }
   }
 #pragma unroll
-  for (int j = 0; j < JK; j++)
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const int t = 16 * wr + 4 * quad + r, d = 16 * (JK * half + j) + col;
-      if (t < c.len && d < a.dk) {
-        out_at<T>(a.gq, c.row, c.first + t, hk)[d] = T(dq[j][r]);
-        out_at<T>(a.gk, c.row, c.first + t, hk)[d] = T(dk[j][r]);
-      }
-    }
+  for (int j = 0; j < JK; j++) {
+    store_head4<Fast, T>(a.gq, c, hk, t, x0 + 16 * j, a.dk, dq[j]);
+    store_head4<Fast, T>(a.gk, c, hk, t, x0 + 16 * j, a.dk, dk[j]);
+  }
 }
 
 }  // namespace

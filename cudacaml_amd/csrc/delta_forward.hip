@@ -8,8 +8,10 @@ namespace op {
 namespace {
 
 // A workgroup of four waves runs BV value columns of one head through the
-// chunks. Wave w holds rows w DK / 4 .. of S (f32, in the layout of a
-// product's result) and makes rows 16 w .. of K S, U and O. Only K, S, beta X
+// chunks. Wave w holds columns w DK / 4 .. of S^T in the layout of a
+// product's result (f32) and makes columns 16 w .. of (K S)^T, U^T and O^T:
+// products are taken transposed, so that a lane has 4 neighbouring value
+// columns of one token and reads and writes them at once. Only K, S, beta X
 // and U are shared through LDS: the rows of Q, T and P that a wave needs are
 // its own and go from memory to registers as matrix operands. Each of them is
 // asked for again for the next chunk as soon as this one has used it, so that
@@ -20,11 +22,11 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
   typedef typename M::T T;
   typedef typename M::Saved Saved;
   constexpr int NI = M::NI, NS = M::NS, NO = M::NO, NU = M::NU;
-  constexpr int LDK = DK + 8, LDT = 72;
-  constexpr int KP = 64 * LDK, SP = BV * LDK, XP = BV * LDT;
+  constexpr int LDK = DK + 8, LDV = BV + 8;
+  constexpr int KP = 64 * LDK, SP = DK * LDV, XP = 64 * LDV;
   constexpr int TK = DK / 64, TV = BV / 16;  // 16 x 16 tiles of S a wave holds
   typedef Record<M> R;
-  __shared__ __align__(16) bf16 ks[NI * KP], st[NS * SP], xt[NS * XP], ut[NU * XP], gt[NS * XP];
+  __shared__ __align__(16) bf16 ks[NI * KP], ss[NS * SP], xs[NS * XP], us[NU * XP], gs[NS * XP];
 
   // heads 8 apart share a chiplet's L2: a head's column blocks, which read
   // the same q, k, T and P, are 8 workgroups apart
@@ -38,18 +40,19 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
   const int chunks = int((sq.len + kChunk - 1) / kChunk);
 
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, quad = l >> 4, col = l & 15;
-  const int row0 = w * (DK / 4) + quad * 4;  // of S: this lane's rows are row0 + 16 i + r
+  const int x0 = w * (DK / 4) + col, y0 = 4 * TV * quad;  // this lane's part of S: rows x0 + 16 i, columns dv0 + y0 + 4 j + r
+  const int t = 16 * w + col;                        // and its token
 
   f32x4 s[TK][TV];
-  const int64_t state_at = lane_id * a.dk * a.dv;
+  const int64_t state_at = lane_id * a.dk * a.dv + dv0;
 #pragma unroll
   for (int i = 0; i < TK; i++)
 #pragma unroll
     for (int j = 0; j < TV; j++)
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const int x = row0 + 16 * i + r, y = dv0 + 16 * j + col;
-        s[i][j][r] = a.state && x < a.dk && y < a.dv ? a.state[state_at + int64_t(x) * a.dv + y] : 0.0f;
+        const int x = x0 + 16 * i, y = y0 + 4 * j + r;
+        s[i][j][r] = a.state && x < a.dk && dv0 + y < a.dv ? a.state[state_at + int64_t(x) * a.dv + y] : 0.0f;
       }
 
   auto chunk = [&](int i) {
@@ -58,10 +61,10 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
   };
   auto record = [&](int i) { return a.records + ((sq.slot + i) * a.hv + h) * R::bytes(Back); };
   Raw8<T> rk[DK / 32], rq[DK / 32];
-  T rv[TV][4];
+  RawV<T, TV> rv;
   Frag<NS> ft[2];
   Frag<NO> fp[2];
-  float gam[4], last[4], beta[4];
+  float gam, last, beta, end;
   auto fetch_k = [&](int i) {
     const Chunk c = chunk(i);
 #pragma unroll
@@ -73,37 +76,30 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
   auto fetch_qv = [&](int i) {
     const Chunk c = chunk(i);
 #pragma unroll
-    for (int j = 0; j < DK / 32; j++) rq[j] = load_head8<Fast, T>(a.q, c, hk, 16 * w + col, 32 * j + 8 * quad, a.dk);
-    const float *dec = reinterpret_cast<const float *>(record(i) + R::Decay);
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const int t = 16 * w + 4 * quad + r;
-#pragma unroll
-      for (int j = 0; j < TV; j++) rv[j][r] = load_head1<T>(a.v, c, h, t, dv0 + 16 * j + col, a.dv);
-      beta[r] = dec[128 + t];
-    }
+    for (int j = 0; j < DK / 32; j++) rq[j] = load_head8<Fast, T>(a.q, c, hk, t, 32 * j + 8 * quad, a.dk);
+    rv = load_v<Fast, T, TV>(a.v, c, h, t, dv0 + y0, a.dv);
+  };
+  auto fragment = [&](const char *from, int b) {  // rows 16 w .. of a matrix of the record, terms 32 b ..
+    return *reinterpret_cast<const bf16x8 *>(from + uint32_t((w * 2 + b) * 1024 + l * 16));
   };
   auto fetch_t = [&](int i) {
 #pragma unroll
     for (int b = 0; b < 2; b++)
       if (b == 0 || w >= 2)  // T and P end at the diagonal
 #pragma unroll
-        for (int p = 0; p < NS; p++)
-          ft[b].p[p] = reinterpret_cast<const bf16x8 *>(record(i) + R::T + p * 8192)[(w * 2 + b) * 64 + l];
+        for (int p = 0; p < NS; p++) ft[b].p[p] = fragment(record(i) + R::T + p * 8192, b);
   };
   auto fetch_p = [&](int i) {
 #pragma unroll
     for (int b = 0; b < 2; b++)
       if (b == 0 || w >= 2)
 #pragma unroll
-        for (int p = 0; p < NO; p++)
-          fp[b].p[p] = reinterpret_cast<const bf16x8 *>(record(i) + R::P + p * 8192)[(w * 2 + b) * 64 + l];
+        for (int p = 0; p < NO; p++) fp[b].p[p] = fragment(record(i) + R::P + p * 8192, b);
     const float *dec = reinterpret_cast<const float *>(record(i) + R::Decay);
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-      gam[r] = dec[16 * w + 4 * quad + r];
-      last[r] = dec[64 + 16 * w + 4 * quad + r];
-    }
+    gam = dec[t];
+    last = dec[64 + t];
+    beta = dec[128 + t];
+    end = dec[63];
   };
 
   if (chunks > 0) {
@@ -117,35 +113,41 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
     const int next = ci + 1 < chunks ? ci + 1 : ci;
 #pragma unroll
     for (int j = 0; j < DK / 32; j++) {
-      const int at = tid + 256 * j, t = at / (DK / 8), d = at % (DK / 8) * 8;
-      put_frag<NI>(ks + t * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rk[j], c, t, d, a.dk)));
+      const int at = tid + 256 * j, kt = at / (DK / 8), d = at % (DK / 8) * 8;
+      put_frag<NI>(ks + kt * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rk[j], c, kt, d, a.dk)));
     }
 #pragma unroll
     for (int i = 0; i < TK; i++)
 #pragma unroll
-      for (int j = 0; j < TV; j++) put_column<NS>(st + (16 * j + col) * LDK + row0 + 16 * i, SP, s[i][j]);
+      for (int j = 0; j < TV; j++) put_four<NS>(ss + (x0 + 16 * i) * LDV + y0 + 4 * j, SP, s[i][j]);
     __syncthreads();
     fetch_k(next);
     if (Back) {
-      Saved *to = reinterpret_cast<Saved *>(a.states) + ((sq.slot + ci) * a.hv + h) * DK * a.dvp + dv0;
+      char *to = a.states + (((sq.slot + ci) * a.hv + h) * a.dvp + dv0 / 32 * 32) * DK * int64_t(sizeof(Saved));
 #pragma unroll
-      for (int i = 0; i < TK; i++)
-#pragma unroll
-        for (int j = 0; j < TV; j++)
-#pragma unroll
-          for (int r = 0; r < 4; r++) to[(row0 + 16 * i + r) * a.dvp + 16 * j + col] = Saved(s[i][j][r]);
+      for (int i = 0; i < TK; i++) put_block<Saved, TV>(to, x0 + 16 * i, dv0 % 32 + y0, s[i]);
     }
 
-    f32x4 kS[TV] = {}, qS[TV] = {};
+    f32x4 kS[TV] = {}, o[TV] = {};
+    {
+      // operands first, products after: one wait for LDS, not one a product
+      Frag<NI> fk[DK / 32];
+      Frag<NS> fs[DK / 32][TV];
 #pragma unroll
-    for (int d = 0; d < DK; d += 32) {
-      const Frag<NI> fk = frag_row<NI>(ks, KP, LDK, 16 * w, d);
-      const Frag<NI> fq = frag_of<NI>(keep_head8<Fast>(rq[d / 32], c, 16 * w + col, d + 8 * quad, a.dk));
+      for (int d = 0; d < DK / 32; d++) {
+        fk[d] = frag_row<NI>(ks, KP, LDK, 16 * w, 32 * d);
 #pragma unroll
-      for (int j = 0; j < TV; j++) {
-        const Frag<NS> fs = frag_row<NS>(st, SP, LDK, 16 * j, d);
-        kS[j] = mma(kS[j], fk, fs);
-        qS[j] = mma(qS[j], fq, first_planes<NO>(fs));
+        for (int j = 0; j < TV; j++) fs[d][j] = frag_v<NS, TV>(ss, SP, LDV, j, 32 * d);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int d = 0; d < DK / 32; d++) {
+        const Frag<NI> fq = frag_of<NI>(keep_head8<Fast>(rq[d], c, t, 32 * d + 8 * quad, a.dk));
+#pragma unroll
+        for (int j = 0; j < TV; j++) {
+          kS[j] = mma(kS[j], fs[d][j], fk[d]);
+          o[j] = mma(o[j], first_planes<NO>(fs[d][j]), fq);
+        }
       }
     }
 #pragma unroll
@@ -153,72 +155,73 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
       f32x4 x;
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const int t = 16 * w + 4 * quad + r, y = dv0 + 16 * j + col;
-        const float v = t < c.len && y < a.dv ? float(rv[j][r]) : 0.0f;
-        x[r] = beta[r] * (v - gam[r] * kS[j][r]);
+        const float v = t < c.len && dv0 + y0 + 4 * j + r < a.dv ? float(rv.x[4 * j + r]) : 0.0f;
+        x[r] = beta * (v - gam * kS[j][r]);
       }
-      put_column<NS>(xt + (16 * j + col) * LDT + 16 * w + 4 * quad, XP, x);
+      put_four<NS>(xs + t * LDV + y0 + 4 * j, XP, x);
     }
     fetch_qv(next);
     __syncthreads();
     f32x4 u[TV] = {};
+    {
+      Frag<NS> fx[2][TV];
 #pragma unroll
-    for (int b = 0; b < 2; b++)
-      if (b == 0 || w >= 2)
+      for (int b = 0; b < 2; b++)
 #pragma unroll
-        for (int j = 0; j < TV; j++) u[j] = mma(u[j], ft[b], frag_row<NS>(xt, XP, LDT, 16 * j, 32 * b));
+        for (int j = 0; j < TV; j++) fx[b][j] = frag_v<NS, TV>(xs, XP, LDV, j, 32 * b);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+        if (b == 0 || w >= 2)
+#pragma unroll
+          for (int j = 0; j < TV; j++) u[j] = mma(u[j], fx[b][j], ft[b]);
+    }
     fetch_t(next);
 #pragma unroll
     for (int j = 0; j < TV; j++) {
-      f32x4 g;
-#pragma unroll
-      for (int r = 0; r < 4; r++) g[r] = last[r] * u[j][r];
-      put_column<NU>(ut + (16 * j + col) * LDT + 16 * w + 4 * quad, XP, u[j]);
-      put_column<NS>(gt + (16 * j + col) * LDT + 16 * w + 4 * quad, XP, g);
+      put_four<NU>(us + t * LDV + y0 + 4 * j, XP, u[j]);
+      put_four<NS>(gs + t * LDV + y0 + 4 * j, XP, last * u[j]);
     }
     if (Back) {
-      float *to = a.us + ((sq.slot + ci) * a.hv + h) * kChunk * a.dvp + dv0;
-#pragma unroll
-      for (int j = 0; j < TV; j++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) to[(16 * w + 4 * quad + r) * a.dvp + 16 * j + col] = u[j][r];
+      char *to = reinterpret_cast<char *>(a.us + (((sq.slot + ci) * a.hv + h) * a.dvp + dv0 / 32 * 32) * kChunk);
+      put_block<float, TV>(to, t, dv0 % 32 + y0, u);
     }
-    const float end = reinterpret_cast<const float *>(record(ci) + R::Decay)[63];
     __syncthreads();
-    f32x4 o[TV];
+    {
+      Frag<NS> fg[2][TV];
+      Frag<NI> fk[2][TK];
+      Frag<NU> fu[2][TV];
 #pragma unroll
-    for (int j = 0; j < TV; j++)
+      for (int b = 0; b < 2; b++) {
 #pragma unroll
-      for (int r = 0; r < 4; r++) o[j][r] = gam[r] * qS[j][r];
+        for (int j = 0; j < TV; j++) fg[b][j] = frag_v<NS, TV>(gs, XP, LDV, j, 32 * b);
 #pragma unroll
-    for (int b = 0; b < 2; b++)
-      if (b == 0 || w >= 2)
+        for (int i = 0; i < TK; i++) fk[b][i] = frag_col<NI>(ks, KP, LDK, w * (DK / 4) + 16 * i, 32 * b);
 #pragma unroll
-        for (int j = 0; j < TV; j++) o[j] = mma(o[j], fp[b], frag_row<NU>(ut, XP, LDT, 16 * j, 32 * b));
+        for (int j = 0; j < TV; j++) fu[b][j] = frag_v<NU, TV>(us, XP, LDV, j, 32 * b);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < TK; i++)
+#pragma unroll
+        for (int j = 0; j < TV; j++) s[i][j] *= end;
+#pragma unroll
+      for (int j = 0; j < TV; j++) o[j] *= gam;
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+#pragma unroll
+        for (int i = 0; i < TK; i++)
+#pragma unroll
+          for (int j = 0; j < TV; j++) s[i][j] = mma(s[i][j], fg[b][j], fk[b][i]);
+        if (b == 0 || w >= 2)
+#pragma unroll
+          for (int j = 0; j < TV; j++) o[j] = mma(o[j], fu[b][j], fp[b]);
+      }
+    }
     fetch_p(next);
 #pragma unroll
-    for (int i = 0; i < TK; i++)
-#pragma unroll
-      for (int j = 0; j < TV; j++) s[i][j] *= end;
-#pragma unroll
-    for (int b = 0; b < 2; b++) {
-      Frag<NS> fg[TV];
-#pragma unroll
-      for (int j = 0; j < TV; j++) fg[j] = frag_row<NS>(gt, XP, LDT, 16 * j, 32 * b);
-#pragma unroll
-      for (int i = 0; i < TK; i++) {
-        const Frag<NI> fk = frag_col<NI>(ks, KP, LDK, w * (DK / 4) + 16 * i, 32 * b);
-#pragma unroll
-        for (int j = 0; j < TV; j++) s[i][j] = mma(s[i][j], fk, fg[j]);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < TV; j++)
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int t = 16 * w + 4 * quad + r, y = dv0 + 16 * j + col;
-        if (t < c.len && y < a.dv) out_at<T>(a.o, c.row, c.first + t, h)[y] = T(a.scale * o[j][r]);
-      }
+    for (int j = 0; j < TV; j++) o[j] *= a.scale;
+    store_v<Fast, T, TV>(a.o, c, h, t, dv0 + y0, a.dv, o);
     __syncthreads();
   }
   if (a.state_out)
@@ -228,8 +231,8 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
       for (int j = 0; j < TV; j++)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-          const int x = row0 + 16 * i + r, y = dv0 + 16 * j + col;
-          if (x < a.dk && y < a.dv) a.state_out[state_at + int64_t(x) * a.dv + y] = s[i][j][r];
+          const int x = x0 + 16 * i, y = y0 + 4 * j + r;
+          if (x < a.dk && dv0 + y < a.dv) a.state_out[state_at + int64_t(x) * a.dv + y] = s[i][j][r];
         }
 }
 

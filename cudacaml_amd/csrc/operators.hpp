@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "internal.hpp"
 
@@ -65,18 +66,21 @@ struct Frag {
   bf16x8 p[N];
 };
 
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
 template <int N, typename T>
 __device__ __forceinline__ Frag<N> frag_of(const Raw8<T> &r) {
   Frag<N> f;
+  if constexpr (N == 1 && std::is_same<T, bf16>::value) {
+    f.p[0] = *reinterpret_cast<const bf16x8 *>(&r);
+  } else {
+    f32x8 x;
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    if constexpr (N == 1 && sizeof(T) == 2) {
-      f.p[0][i] = bf16(r.x[i]);
-    } else {
-      bf16 s[N];
-      split<N>(float(r.x[i]), s);
+    for (int i = 0; i < 8; i++) x[i] = float(r.x[i]);
 #pragma unroll
-      for (int n = 0; n < N; n++) f.p[n][i] = s[n];
+    for (int n = 0; n < N; n++) {
+      f.p[n] = __builtin_convertvector(x, bf16x8);
+      if (n + 1 < N) x -= __builtin_convertvector(f.p[n], f32x8);
     }
   }
   return f;
@@ -96,12 +100,15 @@ __device__ __forceinline__ Frag<N> frag_row(const bf16 *m, int plane, int ld, in
 
 // The same of a matrix stored [term][row]: the transposing LDS read. Of 16
 // lanes each gives the address of 4 neighbouring elements, 4 lanes to a
-// stored row; lane i gets column i of those 4 rows of 16.
-template <int N>
+// stored row; lane i gets column i of those 4 rows of 16. Row 4 i + r of the
+// fragment is stored column row0 + Apart i + r: with Apart 8 two fragments,
+// row0 4 apart, are 32 columns of which a lane of their products has 8 side
+// by side.
+template <int N, int Apart = 4>
 __device__ __forceinline__ Frag<N> frag_col(const bf16 *m, int plane, int ld, int row0, int term0) {
   typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
   const int l = threadIdx.x & 63;
-  const bf16 *p = m + (term0 + (l >> 4) * 8 + ((l >> 2) & 3)) * ld + row0 + (l & 3) * 4;
+  const bf16 *p = m + (term0 + (l >> 4) * 8 + ((l >> 2) & 3)) * ld + row0 + (l & 3) * Apart;
   Frag<N> f;
 #pragma unroll
   for (int n = 0; n < N; n++) {
@@ -133,19 +140,15 @@ __device__ __forceinline__ f32x4 mma(f32x4 c, const Frag<NA> &a, const Frag<NB> 
   return c;
 }
 
-// Four rows of one column of a product into LDS, stored [column][row].
+// The four values that a lane has of a product into LDS, side by side.
 template <int N>
-__device__ __forceinline__ void put_column(bf16 *at, int plane, const f32x4 &c) {
-  bf16x4 v[N];
+__device__ __forceinline__ void put_four(bf16 *at, int plane, f32x4 x) {
 #pragma unroll
-  for (int r = 0; r < 4; r++) {
-    bf16 s[N];
-    split<N>(c[r], s);
-#pragma unroll
-    for (int n = 0; n < N; n++) v[n][r] = s[n];
+  for (int n = 0; n < N; n++) {
+    const bf16x4 v = __builtin_convertvector(x, bf16x4);
+    *reinterpret_cast<bf16x4 *>(at + n * plane) = v;
+    if (n + 1 < N) x -= __builtin_convertvector(v, f32x4);
   }
-#pragma unroll
-  for (int n = 0; n < N; n++) *reinterpret_cast<bf16x4 *>(at + n * plane) = v[n];
 }
 
 template <int N>
