@@ -97,9 +97,6 @@ SIGNATURES = {
 
 # ---- cchip_operators.h --------------------------------------------------------
 
-c_i32 = ctypes.c_int32
-c_u64 = ctypes.c_uint64
-
 
 class GatedDeltaDesc(ctypes.Structure):
     _fields_ = [("dtype", c_int), ("batch", c_i64), ("tokens", c_i64), ("sequences", c_i64), ("key_heads", c_int),
@@ -107,41 +104,25 @@ class GatedDeltaDesc(ctypes.Structure):
                 ("scale", ctypes.c_float)]
 
 
-class Heads(ctypes.Structure):
-    _fields_ = [("data", c_vp), ("batch", c_i64), ("token", c_i64), ("head", c_i64)]
-
-
-class GatedDeltaIO(ctypes.Structure):
-    _fields_ = [(n, Heads) for n in ("q", "k", "v", "g", "beta", "o", "d_o", "dq", "dk", "dv", "dg", "dbeta")] + [
-        (n, c_vp) for n in ("offsets", "state", "state_out", "dstate_out", "dstate", "saved")]
-
-
-class DropDesc(ctypes.Structure):
-    _fields_ = [("p", ctypes.c_double), ("seed", c_u64), ("offset", c_u64), ("step", c_vp)]
-
-
-class Rows(ctypes.Structure):
-    _fields_ = [("data", c_vp), ("row", c_i64)]
+class DropoutDesc(ctypes.Structure):
+    _fields_ = [("dtype", c_int), ("rows", c_i64), ("cols", c_i64), ("p", ctypes.c_double), ("scale", ctypes.c_float)]
 
 
 class NormBlockDesc(ctypes.Structure):
     _fields_ = [("dtype", c_int), ("weight_dtype", c_int), ("rows", c_i64), ("width", c_i64), ("post", c_int),
-                ("pre", c_int), ("gate", c_int), ("scale", ctypes.c_float), ("eps", ctypes.c_float)]
+                ("pre", c_int), ("gate", c_int), ("scale", ctypes.c_float), ("eps", ctypes.c_float),
+                ("p", ctypes.c_double)]
 
 
-class NormParams(ctypes.Structure):
-    _fields_ = [(n, c_vp) for n in ("post_weight", "post_bias", "channel_scale", "pre_weight", "pre_bias")]
-
-
+# The io structures hold 64-bit words only; callers pack them into bytes.
 OPERATOR_SIGNATURES = {
-    "cchip_gated_delta_sizes": (c_int, [P(GatedDeltaDesc), P(c_size), P(c_size)]),
-    "cchip_gated_delta_forward": (c_int, [P(GatedDeltaDesc), P(GatedDeltaIO), c_vp, c_size, c_vp]),
-    "cchip_gated_delta_backward": (c_int, [P(GatedDeltaDesc), P(GatedDeltaIO), c_vp, c_size, c_vp]),
-    "cchip_dropout": (c_int, [c_int, c_i64, c_i64, P(DropDesc), ctypes.c_float, Rows, Rows, Rows, c_vp]),
-    "cchip_norm_block_forward": (c_int, [P(NormBlockDesc), P(DropDesc), P(NormParams)] + [Rows] * 5 + [c_vp]),
+    "cchip_gated_delta_sizes": (c_int, [P(GatedDeltaDesc), P(c_size), P(c_size), P(c_size)]),
+    "cchip_gated_delta_forward": (c_int, [P(GatedDeltaDesc), c_cp, c_vp, c_size, c_vp]),
+    "cchip_gated_delta_backward": (c_int, [P(GatedDeltaDesc), c_cp, c_vp, c_size, c_vp]),
+    "cchip_dropout_run": (c_int, [P(DropoutDesc), c_cp, c_vp]),
+    "cchip_norm_block_forward": (c_int, [P(NormBlockDesc), c_cp, c_vp]),
     "cchip_norm_block_workspace": (c_int, [P(NormBlockDesc), P(c_size)]),
-    "cchip_norm_block_backward": (c_int, [P(NormBlockDesc), P(DropDesc), P(NormParams), P(NormParams)] + [Rows] * 8
-                                  + [c_vp, c_size, c_vp]),
+    "cchip_norm_block_backward": (c_int, [P(NormBlockDesc), c_cp, c_vp, c_size, c_vp]),
 }
 
 _lib = None

@@ -56,9 +56,7 @@ Layout layout_of(const cchip_gated_delta &op) {
   return p;
 }
 
-bool steps(const cchip_gated_delta &op, const cchip_gated_delta_io &io) {
-  return !op.sequences && !io.saved && op.tokens <= kStepTokens;
-}
+bool steps(const cchip_gated_delta &op, bool saves) { return !op.sequences && !saves && op.tokens <= kStepTokens; }
 
 int element_size(const cchip_gated_delta &op) { return op.dtype == CCHIP_F32 ? 4 : 2; }
 
@@ -120,11 +118,6 @@ void check_workspace(const void *workspace, size_t have, size_t need) {
     throw InvalidArgument(strf("gated delta: the workspace needs %zu bytes aligned to 16, has %zu", need, workspace ? have : 0));
 }
 
-size_t workspace_bytes_of(const cchip_gated_delta &op, const Layout &p) {
-  (void)op;
-  return std::max(p.record, p.states + p.us);
-}
-
 void lay_out(DeltaArgs &a, const Layout &p, char *saved) {
   a.records = saved;
   a.states = saved + p.record_back;
@@ -135,11 +128,12 @@ void lay_out(DeltaArgs &a, const Layout &p, char *saved) {
 
 extern "C" {
 
-int cchip_gated_delta_sizes(const cchip_gated_delta *op, size_t *workspace, size_t *saved) {
+int cchip_gated_delta_sizes(const cchip_gated_delta *op, size_t *forward, size_t *backward, size_t *saved) {
   return guarded([&] {
     check_op(op);
     const Layout p = layout_of(*op);
-    if (workspace) *workspace = workspace_bytes_of(*op, p);
+    if (forward) *forward = steps(*op, false) ? 0 : p.record;
+    if (backward) *backward = p.states + p.us;
     if (saved) *saved = p.record_back + p.states + p.us;
   });
 }
@@ -153,7 +147,7 @@ int cchip_gated_delta_forward(const cchip_gated_delta *op, const cchip_gated_del
     DeltaArgs a = args_of(*op, *io, false);
     a.slots = p.slots;
     if (a.sequences == 0) return;
-    if (steps(*op, *io)) return delta_step_launch(*op, a, (hipStream_t)stream);
+    if (steps(*op, io->saved != nullptr)) return delta_step_launch(*op, a, (hipStream_t)stream);
     if (io->saved) {
       lay_out(a, p, static_cast<char *>(io->saved));
     } else {

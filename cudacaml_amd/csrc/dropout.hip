@@ -46,11 +46,11 @@ __global__ __launch_bounds__(256) void dropout(const DropoutArgs a) {
 
 }  // namespace
 
-Drop drop_of(const cchip_drop *d) {
-  if (!d) return {0, 0, nullptr, 0, 1.0f};
-  if (!(d->p >= 0.0 && d->p <= 1.0)) throw InvalidArgument(strf("dropout: p = %g is not in 0 .. 1", d->p));
-  const uint32_t bar = uint32_t(std::nearbyint(d->p * 65536.0));
-  return {d->seed, d->offset, d->step, bar, bar >= 65536 ? 0.0f : float(65536.0 / (65536 - bar))};
+Drop drop_of(const char *who, double p, uint64_t seed, uint64_t offset, const uint64_t *step) {
+  if (!(p >= 0.0 && p <= 1.0)) throw InvalidArgument(strf("%s: p = %g is not in 0 .. 1", who, p));
+  if (reinterpret_cast<uintptr_t>(step) % 8) throw InvalidArgument(strf("%s: step is not aligned to its 8 bytes", who));
+  const uint32_t bar = uint32_t(std::nearbyint(p * 65536.0));
+  return {seed, offset, step, bar, bar >= 65536 ? 0.0f : float(65536.0 / (65536 - bar))};
 }
 
 }  // namespace op
@@ -59,27 +59,26 @@ Drop drop_of(const cchip_drop *d) {
 using namespace cchip;
 using namespace cchip::op;
 
-extern "C" int cchip_dropout(int dtype, int64_t rows, int64_t cols, const cchip_drop *drop, float scale, cchip_rows x,
-                             cchip_rows residual, cchip_rows out, void *stream) {
+extern "C" int cchip_dropout_run(const cchip_dropout *op, const cchip_dropout_io *io, void *stream) {
   return guarded([&] {
     const char *who = "dropout";
-    check_rows_type(who, dtype);
-    if (!drop) throw InvalidArgument("dropout: no probability and seed");
-    if (rows < 0 || cols < 0 || rows >= (int64_t(1) << 32) || cols >= (int64_t(1) << 35))
+    if (!op || !io) throw InvalidArgument("dropout: no descriptor or tensors");
+    check_rows_type(who, op->dtype);
+    if (op->rows < 0 || op->cols < 0 || op->rows >= (int64_t(1) << 32) || op->cols >= (int64_t(1) << 35))
       throw InvalidArgument("dropout: rows are below 2^32 and columns below 2^35");
-    if (!std::isfinite(scale)) throw InvalidArgument("dropout: scale is not finite");
+    if (!std::isfinite(op->scale)) throw InvalidArgument("dropout: scale is not finite");
     DropoutArgs a = {};
-    a.drop = drop_of(drop);
-    if (rows == 0 || cols == 0) return;
-    a.x = rows_of(who, "x", dtype, rows, cols, x, false, true);
-    a.residual = rows_of(who, "residual", dtype, rows, cols, residual, false, false);
-    a.out = rows_of(who, "out", dtype, rows, cols, out, true, true);
-    a.per_row = uint32_t((cols + 7) / 8);
-    a.groups = uint64_t(rows) * a.per_row;
+    a.drop = drop_of(who, op->p, io->seed, io->offset, io->step);
+    if (op->rows == 0 || op->cols == 0) return;
+    a.x = rows_of(who, "x", op->dtype, op->rows, op->cols, io->x, false, true);
+    a.residual = rows_of(who, "residual", op->dtype, op->rows, op->cols, io->residual, false, false);
+    a.out = rows_of(who, "out", op->dtype, op->rows, op->cols, io->out, true, true);
+    a.per_row = uint32_t((op->cols + 7) / 8);
+    a.groups = uint64_t(op->rows) * a.per_row;
     if ((a.groups + 255) / 256 > uint64_t(INT32_MAX)) throw InvalidArgument("dropout: more elements than a launch can have");
-    a.cols = cols;
-    a.scale = scale;
-    with_rows_type(dtype, [&](auto t) {
+    a.cols = op->cols;
+    a.scale = op->scale;
+    with_rows_type(op->dtype, [&](auto t) {
       typedef decltype(t) T;
       hipLaunchKernelGGL((dropout<T>), dim3(unsigned((a.groups + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a);
     });

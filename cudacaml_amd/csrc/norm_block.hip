@@ -61,11 +61,13 @@ void check_op(const cchip_norm_block *op) {
       throw InvalidArgument(strf("norm block: unknown norm %d", kind));
   if (op->gate != CCHIP_GATE_NONE && op->gate != CCHIP_GATE_SIGMOID && op->gate != CCHIP_GATE_SILU)
     throw InvalidArgument(strf("norm block: unknown gate %d", op->gate));
+  if (!(op->p >= 0.0 && op->p <= 1.0)) throw InvalidArgument(strf("norm block: p = %g is not in 0 .. 1", op->p));
   if (!std::isfinite(op->scale) || !(op->eps >= 0.0f) || !std::isfinite(op->eps))
     throw InvalidArgument("norm block: scale is finite and eps finite and not negative");
 }
 
-NormArgs args_of(const cchip_norm_block &op, const cchip_drop *drop, const cchip_norm_params *params) {
+NormArgs args_of(const cchip_norm_block &op, const cchip_norm_block_io *io) {
+  if (!io) throw InvalidArgument("norm block: no tensors");
   NormArgs a = {};
   a.rows = uint32_t(op.rows);
   a.width = int(op.width);
@@ -75,14 +77,12 @@ NormArgs args_of(const cchip_norm_block &op, const cchip_drop *drop, const cchip
   a.scale = op.scale;
   a.eps = op.eps;
   a.weights_f32 = op.weight_dtype == CCHIP_F32;
-  a.drop = drop_of(drop);
-  if (params) {
-    a.post_weight = params->post_weight;
-    a.post_bias = params->post_bias;
-    a.channel_scale = params->channel_scale;
-    a.pre_weight = params->pre_weight;
-    a.pre_bias = params->pre_bias;
-  }
+  a.drop = drop_of("norm block", op.p, io->seed, io->offset, io->step);
+  a.post_weight = io->params.post_weight;
+  a.post_bias = io->params.post_bias;
+  a.channel_scale = io->params.channel_scale;
+  a.pre_weight = io->params.pre_weight;
+  a.pre_bias = io->params.pre_bias;
   for (const void *p : {a.post_weight, a.post_bias, a.channel_scale, a.pre_weight, a.pre_bias})
     if (reinterpret_cast<uintptr_t>(p) % (a.weights_f32 ? 4 : 2))
       throw InvalidArgument("norm block: a parameter is not aligned to its elements");
@@ -110,22 +110,20 @@ using namespace cchip::op;
 
 extern "C" {
 
-int cchip_norm_block_forward(const cchip_norm_block *op, const cchip_drop *drop, const cchip_norm_params *params,
-                             cchip_rows y, cchip_rows gate, cchip_rows residual, cchip_rows h, cchip_rows n,
-                             void *stream) {
+int cchip_norm_block_forward(const cchip_norm_block *op, const cchip_norm_block_io *io, void *stream) {
   return guarded([&] {
     const char *who = "norm block";
     check_op(op);
-    NormArgs a = args_of(*op, drop, params);
+    NormArgs a = args_of(*op, io);
     const bool pre = op->pre != CCHIP_NORM_NONE, gated = op->gate != CCHIP_GATE_NONE;
     if (op->rows == 0) return;
-    if (pre != (n.data != nullptr)) throw InvalidArgument("norm block: n is given if and only if there is a pre norm");
-    if (gated != (gate.data != nullptr)) throw InvalidArgument("norm block: a gate is given if and only if the operator has one");
-    a.y = rows_of(who, "y", op->dtype, op->rows, op->width, y, false, true);
-    a.gate = rows_of(who, "gate", op->dtype, op->rows, op->width, gate, false, false);
-    a.residual = rows_of(who, "residual", op->dtype, op->rows, op->width, residual, false, false);
-    a.h = rows_of(who, "h", op->dtype, op->rows, op->width, h, true, true);
-    a.n = rows_of(who, "n", op->dtype, op->rows, op->width, n, true, false);
+    if (pre != (io->n.data != nullptr)) throw InvalidArgument("norm block: n is given if and only if there is a pre norm");
+    if (gated != (io->gate.data != nullptr)) throw InvalidArgument("norm block: a gate is given if and only if the operator has one");
+    a.y = rows_of(who, "y", op->dtype, op->rows, op->width, io->y, false, true);
+    a.gate = rows_of(who, "gate", op->dtype, op->rows, op->width, io->gate, false, false);
+    a.residual = rows_of(who, "residual", op->dtype, op->rows, op->width, io->residual, false, false);
+    a.h = rows_of(who, "h", op->dtype, op->rows, op->width, io->h, true, true);
+    a.n = rows_of(who, "n", op->dtype, op->rows, op->width, io->n, true, false);
     with_rows_type(op->dtype, [&](auto t) { norm_forward_launch<decltype(t)>(a, (hipStream_t)stream); });
     check_launch(who);
   });
@@ -138,23 +136,19 @@ int cchip_norm_block_workspace(const cchip_norm_block *op, size_t *bytes) {
   });
 }
 
-int cchip_norm_block_backward(const cchip_norm_block *op, const cchip_drop *drop, const cchip_norm_params *params,
-                              const cchip_norm_grads *grads, cchip_rows y, cchip_rows gate, cchip_rows h,
-                              cchip_rows dh, cchip_rows dn, cchip_rows dy, cchip_rows dgate, cchip_rows dresidual,
-                              void *workspace, size_t workspace_bytes, void *stream) {
+int cchip_norm_block_backward(const cchip_norm_block *op, const cchip_norm_block_io *io, void *workspace,
+                              size_t workspace_bytes, void *stream) {
   return guarded([&] {
     const char *who = "norm block";
     check_op(op);
-    NormArgs a = args_of(*op, drop, params);
+    NormArgs a = args_of(*op, io);
     const bool pre = op->pre != CCHIP_NORM_NONE, gated = op->gate != CCHIP_GATE_NONE;
     ColumnArgs c = {};
-    if (grads) {
-      c.to[kPostWeight] = grads->post_weight;
-      c.to[kChannelScale] = grads->channel_scale;
-      c.to[kPreWeight] = grads->pre_weight;
-      c.to[kPostBias] = grads->post_bias;
-      c.to[kPreBias] = grads->pre_bias;
-    }
+    c.to[kPostWeight] = io->grads.post_weight;
+    c.to[kChannelScale] = io->grads.channel_scale;
+    c.to[kPreWeight] = io->grads.pre_weight;
+    c.to[kPostBias] = io->grads.post_bias;
+    c.to[kPreBias] = io->grads.pre_bias;
     bool any = false;
     for (void *p : c.to) {
       any = any || p;
@@ -166,18 +160,18 @@ int cchip_norm_block_backward(const cchip_norm_block *op, const cchip_drop *drop
     if ((c.to[kPreWeight] || c.to[kPreBias]) && !pre) throw InvalidArgument("norm block: gradients of a pre norm that there is not");
     const bool bias = c.to[kPostBias] || c.to[kPreBias] || a.post_bias;
     if (op->rows > 0) {
-      if (pre != (dn.data != nullptr) || pre != (h.data != nullptr))
+      if (pre != (io->dn.data != nullptr) || pre != (io->h.data != nullptr))
         throw InvalidArgument("norm block: h and dn are given if and only if there is a pre norm");
-      if (gated != (gate.data != nullptr)) throw InvalidArgument("norm block: a gate is given if and only if the operator has one");
-      if (!gated && dgate.data) throw InvalidArgument("norm block: the gradient of a gate that there is not");
-      a.y = rows_of(who, "y", op->dtype, op->rows, op->width, y, false, true);
-      a.gate = rows_of(who, "gate", op->dtype, op->rows, op->width, gate, false, false);
-      a.h = rows_of(who, "h", op->dtype, op->rows, op->width, h, false, false);
-      a.dh = rows_of(who, "dh", op->dtype, op->rows, op->width, dh, false, true);
-      a.dn = rows_of(who, "dn", op->dtype, op->rows, op->width, dn, false, false);
-      a.dy = rows_of(who, "dy", op->dtype, op->rows, op->width, dy, true, true);
-      a.dgate = rows_of(who, "dgate", op->dtype, op->rows, op->width, dgate, true, false);
-      a.dresidual = rows_of(who, "dresidual", op->dtype, op->rows, op->width, dresidual, true, false);
+      if (gated != (io->gate.data != nullptr)) throw InvalidArgument("norm block: a gate is given if and only if the operator has one");
+      if (!gated && io->dgate.data) throw InvalidArgument("norm block: the gradient of a gate that there is not");
+      a.y = rows_of(who, "y", op->dtype, op->rows, op->width, io->y, false, true);
+      a.gate = rows_of(who, "gate", op->dtype, op->rows, op->width, io->gate, false, false);
+      a.h = rows_of(who, "h", op->dtype, op->rows, op->width, io->h, false, false);
+      a.dh = rows_of(who, "dh", op->dtype, op->rows, op->width, io->dh, false, true);
+      a.dn = rows_of(who, "dn", op->dtype, op->rows, op->width, io->dn, false, false);
+      a.dy = rows_of(who, "dy", op->dtype, op->rows, op->width, io->dy, true, true);
+      a.dgate = rows_of(who, "dgate", op->dtype, op->rows, op->width, io->dgate, true, false);
+      a.dresidual = rows_of(who, "dresidual", op->dtype, op->rows, op->width, io->dresidual, true, false);
     }
     const int groups = groups_of(*op);
     if (any) {

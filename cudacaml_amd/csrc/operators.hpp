@@ -47,6 +47,16 @@ __device__ __forceinline__ Raw8<T> load8(const T *p, int valid) {
   return r;
 }
 
+// Two values rounded to bf16 in one instruction (the compiler makes one of
+// each), and those as f32 again.
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t u;
+  asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(u) : "v"(lo), "v"(hi));
+  return u;
+}
+__device__ __forceinline__ float low_bf16(uint32_t u) { return __builtin_bit_cast(float, u << 16); }
+__device__ __forceinline__ float high_bf16(uint32_t u) { return __builtin_bit_cast(float, u & 0xFFFF0000u); }
+
 // x as the sum of N bf16 values, each the rounding of what the ones before
 // it leave: 8, 16 and 24 bits of x for N = 1, 2 and 3 (24 hold every f32, 11
 // every f16).
@@ -66,21 +76,26 @@ struct Frag {
   bf16x8 p[N];
 };
 
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-
 template <int N, typename T>
 __device__ __forceinline__ Frag<N> frag_of(const Raw8<T> &r) {
   Frag<N> f;
   if constexpr (N == 1 && std::is_same<T, bf16>::value) {
     f.p[0] = *reinterpret_cast<const bf16x8 *>(&r);
   } else {
-    f32x8 x;
+    float x[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) x[i] = float(r.x[i]);
 #pragma unroll
     for (int n = 0; n < N; n++) {
-      f.p[n] = __builtin_convertvector(x, bf16x8);
-      if (n + 1 < N) x -= __builtin_convertvector(f.p[n], f32x8);
+      u32x4 u;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const uint32_t p = pack_bf16(x[2 * i], x[2 * i + 1]);
+        u[i] = p;
+        x[2 * i] -= low_bf16(p);
+        x[2 * i + 1] -= high_bf16(p);
+      }
+      f.p[n] = __builtin_bit_cast(bf16x8, u);
     }
   }
   return f;
@@ -145,9 +160,9 @@ template <int N>
 __device__ __forceinline__ void put_four(bf16 *at, int plane, f32x4 x) {
 #pragma unroll
   for (int n = 0; n < N; n++) {
-    const bf16x4 v = __builtin_convertvector(x, bf16x4);
-    *reinterpret_cast<bf16x4 *>(at + n * plane) = v;
-    if (n + 1 < N) x -= __builtin_convertvector(v, f32x4);
+    const uint32_t a = pack_bf16(x[0], x[1]), b = pack_bf16(x[2], x[3]);
+    *reinterpret_cast<uint2 *>(at + n * plane) = make_uint2(a, b);
+    x -= f32x4{low_bf16(a), high_bf16(a), low_bf16(b), high_bf16(b)};
   }
 }
 

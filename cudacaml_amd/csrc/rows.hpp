@@ -39,8 +39,8 @@ __device__ __forceinline__ void store8(T *p, const float (&x)[8], int n) {
 
 __device__ __forceinline__ uint64_t offset_of(const Drop &d) { return d.offset + (d.step ? *d.step : 0); }
 
-// The kernel's form of a probability and seed; null: nothing is dropped.
-Drop drop_of(const cchip_drop *d);
+// The kernel's form of a probability, seed and offset.
+Drop drop_of(const char *who, double p, uint64_t seed, uint64_t offset, const uint64_t *step);
 
 inline void check_rows_type(const char *who, int dtype) {
   if (dtype != CCHIP_F32 && dtype != CCHIP_BF16 && dtype != CCHIP_F16)

@@ -6,8 +6,8 @@ A handle is made once for its shapes, checks the arguments of each call and
 keeps the workspace, one for each stream it is called on. A call only issues
 work on ``stream`` (a ``runtime.Stream``, an object with ``cuda_stream``, a
 raw pointer, or None for the default stream) and may be captured into a HIP
-graph once its handle has been called on that stream (or ``reserve`` has);
-the arrays it is given have to live until the stream is past it.
+graph once the handle has its workspace there (``reserve``, or an earlier
+call); the arrays it is given have to live until the stream is past it.
 
 Arrays are ``Array``, ``backend_hip.Resident`` or anything with ``data_ptr()``,
 ``get_device()``, ``dtype``, ``shape`` and ``stride()``, such as a tensor of
@@ -19,6 +19,8 @@ work.
 from __future__ import annotations
 
 import ctypes
+import functools
+import struct
 
 from . import _lib
 from ._lib import check, lib
@@ -31,6 +33,7 @@ NORMS = {"none": 0, "rms": 1, "layer": 2}
 GATES = {"none": 0, "sigmoid": 1, "silu": 2}
 
 
+@functools.lru_cache(maxsize=1024)
 def _contiguous(shape):
     out, n = [], 1
     for d in reversed(shape):
@@ -94,12 +97,6 @@ def _dtype_name(d):
     return n
 
 
-def _as_array(x):
-    if isinstance(x, Resident):
-        return Array(x.buf, x.dtype.name, x.shape)
-    return x
-
-
 def _stream_ptr(stream):
     if stream is None or isinstance(stream, int):
         return stream
@@ -112,47 +109,49 @@ def _dims(shape):
     return "[" + ", ".join(str(d) for d in shape) + "]"
 
 
+_NO_ROWS = (0, 0)
+
+
 class _Operator:
     _who = ""
 
     def __init__(self):
         self._device = Device.current() if Device.available() else None
-        self._workspace_bytes = 0
         self._workspaces = {}
 
-    def _check(self, name, x, dtype, shape):
+    def _view(self, name, x, dtype, shape):
         """The array's pointer and strides, or ValueError."""
         if type(x) is Resident:
-            x = _as_array(x)
+            x = Array(x.buf, x.dtype.name, x.shape)
         if x.shape != shape and tuple(x.shape) != shape:
             raise ValueError("%s: %s has shape %s, expected %s" % (self._who, name, _dims(x.shape), _dims(shape)))
-        if _dtypes.get(x.dtype) != dtype and _dtype_name(x.dtype) != dtype:
-            raise ValueError("%s: %s has dtype %s, expected %s" % (self._who, name, _dtype_name(x.dtype), dtype))
+        d = x.dtype
+        if _dtypes.get(d) != dtype and _dtype_name(d) != dtype:
+            raise ValueError("%s: %s has dtype %s, expected %s" % (self._who, name, _dtype_name(d), dtype))
         d = x.get_device()
-        if d is not None and d != self._device:
+        if d != self._device and d is not None:
             raise ValueError("%s: %s is not on device %s" % (self._who, name, self._device))
         return x.data_ptr(), x.stride()
 
     def _whole(self, name, x, dtype, shape):
-        """The pointer of an array without gaps; None for None."""
+        """The pointer of an array without gaps; 0 for None."""
         if x is None:
-            return None
-        p, st = self._check(name, x, dtype, shape)
+            return 0
+        p, st = self._view(name, x, dtype, shape)
         if st != _contiguous(shape) and any(a != b for a, b, d in zip(st, _contiguous(shape), shape) if d > 1):
             raise ValueError("%s: %s is not contiguous" % (self._who, name))
         return p
 
-    def _workspace(self, stream):
-        if not self._workspace_bytes:
+    def _workspace(self, stream, nbytes):
+        """A workspace of at least nbytes of the stream's own."""
+        if not nbytes:
             return None
         w = self._workspaces.get(stream)
-        if w is None:
-            w = self._workspaces[stream] = Buffer.alloc(self._workspace_bytes)
+        if w is None or w.nbytes < nbytes:
+            if w is not None:
+                w.free()  # hipFree waits for the work that uses it
+            w = self._workspaces[stream] = Buffer.alloc(nbytes)
         return w.ptr
-
-    def reserve(self, stream=None):
-        """Allocate the workspace of a stream before the first call on it."""
-        self._workspace(_stream_ptr(stream))
 
     def free(self):
         """Free the workspaces; the streams have to be done with them."""
@@ -165,6 +164,12 @@ class _Operator:
             self.free()
         except Exception:
             pass
+
+
+def _check_dtype(who, *names):
+    for n in names:
+        if n not in CODES:
+            raise ValueError("%s: dtype %r is not f32, bf16 or f16" % (who, n))
 
 
 class GatedDelta(_Operator):
@@ -180,24 +185,25 @@ class GatedDelta(_Operator):
     """
 
     _who = "GatedDelta"
+    # cchip_gated_delta_io: twelve cchip_heads of four words, six pointers
+    _forward_io = struct.Struct("24q192x6q")
+    _backward_io = struct.Struct("20q32x24q6q")
 
     def __init__(self, dtype, batch, tokens, key_heads, value_heads, key_dim, value_dim, scale=None, sequences=None,
                  states=True):
         super().__init__()
-        if dtype not in CODES:
-            raise ValueError("GatedDelta: dtype %r is not f32, bf16 or f16" % (dtype,))
+        _check_dtype("GatedDelta", dtype)
         if sequences is not None and sequences < 1:
             raise ValueError("GatedDelta: sequences must be >= 1")
         self.dtype = dtype
         self._desc = _lib.GatedDeltaDesc(CODES[dtype], batch, tokens, sequences or 0, key_heads, value_heads, key_dim,
                                          value_dim, 1 if states else 0,
                                          key_dim ** -0.5 if scale is None and key_dim > 0 else scale or 0.0)
-        w, s = ctypes.c_size_t(), ctypes.c_size_t()
-        check(lib().cchip_gated_delta_sizes(self._desc, ctypes.byref(w), ctypes.byref(s)))
-        self._workspace_bytes, self._saved_bytes = w.value, s.value
-        self._qk = (batch, tokens, key_heads, key_dim)
-        self._v = (batch, tokens, value_heads, value_dim)
-        self._gates = (batch, tokens, value_heads)
+        sizes = [ctypes.c_size_t() for _ in range(3)]
+        check(lib().cchip_gated_delta_sizes(self._desc, *sizes))
+        self._forward_bytes, self._backward_bytes, self._saved_bytes = (x.value for x in sizes)
+        qk, v, gates = (batch, tokens, key_heads, key_dim), (batch, tokens, value_heads, value_dim), (batch, tokens, value_heads)
+        self._shapes = dict(q=qk, k=qk, dq=qk, dk=qk, v=v, o=v, do=v, dv=v, g=gates, beta=gates, dg=gates, dbeta=gates)
         self._state = (sequences or batch, value_heads, key_dim, value_dim)
         self._offsets = None if sequences is None else (sequences + 1,)
 
@@ -209,43 +215,54 @@ class GatedDelta(_Operator):
         """A fresh array for what a forward pass saves."""
         return Array.empty("u8", (self._saved_bytes,))
 
-    def _heads(self, io, name, x, shape):
-        p, st = self._check(name, x, self.dtype, shape)
-        if len(shape) == 4 and shape[3] > 1 and st[3] != 1:
-            raise ValueError("GatedDelta: the last dimension of %s is not contiguous" % name)
-        h = getattr(io, name)
-        h.data, h.batch, h.token, h.head = p, st[0], st[1], st[2]
+    def reserve(self, stream=None, backward=False):
+        """Allocate a stream's workspace ahead of the first call on it."""
+        self._workspace(_stream_ptr(stream), max(self._forward_bytes, self._backward_bytes if backward else 0))
 
-    def _io(self, q, k, v, g, beta, offsets, saved):
-        io = _lib.GatedDeltaIO()
-        self._heads(io, "q", q, self._qk)
-        self._heads(io, "k", k, self._qk)
-        self._heads(io, "v", v, self._v)
-        self._heads(io, "g", g, self._gates)
-        self._heads(io, "beta", beta, self._gates)
-        if self._offsets is None:
-            if offsets is not None:
-                raise ValueError("GatedDelta: offsets without packed sequences")
-        else:
-            if offsets is None:
-                raise ValueError("GatedDelta: packed sequences need offsets")
-            io.offsets = self._whole("offsets", offsets, "i32", self._offsets)
-        if saved is not None:
-            if saved.shape != (self._saved_bytes,):
-                raise ValueError("GatedDelta: saved has shape %s, expected %s" % (_dims(saved.shape), _dims((self._saved_bytes,))))
-            io.saved = self._whole("saved", saved, "u8", (self._saved_bytes,))
-        return io
+    def _words(self, **given):
+        """Pointer and three strides of each array. The loop does in one go what
+        _view does with words to say: a call on small arrays costs little more
+        than looking at them."""
+        words, device, dtype, shapes = [], self._device, self.dtype, self._shapes
+        for name, x in given.items():
+            shape = shapes[name]
+            try:
+                st = x.stride()
+                plain = x.shape == shape and _dtypes[x.dtype] == dtype and x.get_device() == device
+                p = x.data_ptr()
+            except (AttributeError, KeyError):
+                plain = False
+            if not plain:
+                p, st = self._view(name, x, dtype, shape)
+            if len(st) == 4:
+                if st[3] != 1 and shape[3] > 1:
+                    raise ValueError("GatedDelta: the last dimension of %s is not contiguous" % name)
+                st = st[:3]
+            words.append(p)
+            words += st
+        return words
+
+    def _bounds(self, offsets):
+        if (offsets is None) != (self._offsets is None):
+            raise ValueError("GatedDelta: packed sequences need offsets" if offsets is None else
+                             "GatedDelta: offsets without packed sequences")
+        return self._whole("offsets", offsets, "i32", self._offsets)
+
+    def _kept(self, saved):
+        return self._whole("saved", saved, "u8", (self._saved_bytes,))
 
     def forward(self, q, k, v, g, beta, o, *, state=None, state_out=None, offsets=None, saved=None, stream=None):
         """Write ``o``, and the sequences' last states to ``state_out`` if given
         (it may be ``state``, where they begin; without one, at zero).
         ``saved`` is written for a backward pass if given."""
-        io = self._io(q, k, v, g, beta, offsets, saved)
-        self._heads(io, "o", o, self._v)
-        io.state = self._whole("state", state, "f32", self._state)
-        io.state_out = self._whole("state_out", state_out, "f32", self._state)
+        words = self._words(q=q, k=k, v=v, g=g, beta=beta, o=o)
         s = _stream_ptr(stream)
-        check(lib().cchip_gated_delta_forward(self._desc, io, self._workspace(s), self._workspace_bytes, s))
+        io = self._forward_io.pack(*words, self._bounds(offsets), self._whole("state", state, "f32", self._state),
+                                   self._whole("state_out", state_out, "f32", self._state), 0, 0, self._kept(saved))
+        n = 0 if saved is not None else self._forward_bytes
+        rc = lib().cchip_gated_delta_forward(self._desc, io, self._workspace(s, n) if n else None, n, s)
+        if rc:
+            check(rc)
 
     def backward(self, q, k, v, g, beta, do, saved, dq, dk, dv, dg, dbeta, *, dstate_out=None, dstate=None, offsets=None,
                  stream=None):
@@ -254,59 +271,68 @@ class GatedDelta(_Operator):
         given. ``saved`` is what ``forward`` wrote for the same inputs."""
         if saved is None:
             raise ValueError("GatedDelta: the backward pass needs what the forward pass saved")
-        io = self._io(q, k, v, g, beta, offsets, saved)
-        self._heads(io, "d_o", do, self._v)
-        self._heads(io, "dq", dq, self._qk)
-        self._heads(io, "dk", dk, self._qk)
-        self._heads(io, "dv", dv, self._v)
-        self._heads(io, "dg", dg, self._gates)
-        self._heads(io, "dbeta", dbeta, self._gates)
-        io.dstate_out = self._whole("dstate_out", dstate_out, "f32", self._state)
-        io.dstate = self._whole("dstate", dstate, "f32", self._state)
-        s = _stream_ptr(stream)
-        check(lib().cchip_gated_delta_backward(self._desc, io, self._workspace(s), self._workspace_bytes, s))
+        words = self._words(q=q, k=k, v=v, g=g, beta=beta, do=do, dq=dq, dk=dk, dv=dv, dg=dg, dbeta=dbeta)
+        s, n = _stream_ptr(stream), self._backward_bytes
+        io = self._backward_io.pack(*words, self._bounds(offsets), 0, 0,
+                                    self._whole("dstate_out", dstate_out, "f32", self._state),
+                                    self._whole("dstate", dstate, "f32", self._state), self._kept(saved))
+        check(lib().cchip_gated_delta_backward(self._desc, io, self._workspace(s, n), n, s))
 
 
 class _RowOperator(_Operator):
-    def _rows(self, name, x, needed=False):
+    def _rows(self, name, x):
+        """An array's pointer and the distance of its rows; zeros for None."""
         if x is None:
-            if needed:
-                raise ValueError("%s: no %s" % (self._who, name))
-            return _lib.Rows(None, 0)
-        p, st = self._check(name, x, self.dtype, self._shape)
-        if self._shape[1] > 1 and st[1] != 1:
+            return _NO_ROWS
+        try:
+            st = x.stride()
+            plain = x.shape == self._shape and _dtypes[x.dtype] == self.dtype and x.get_device() == self._device
+            p = x.data_ptr()
+        except (AttributeError, KeyError):
+            plain = False
+        if not plain:
+            p, st = self._view(name, x, self.dtype, self._shape)
+        if st[1] != 1 and self._shape[1] > 1:
             raise ValueError("%s: rows of %s are not contiguous" % (self._who, name))
-        return _lib.Rows(p, st[0])
+        return p, st[0]
 
-    def _step(self, step):
-        return self._whole("step", step, "i64", ())
+    def _needed(self, name, x):
+        if x is None:
+            raise ValueError("%s: no %s" % (self._who, name))
+        return self._rows(name, x)
+
+    def _seed(self, seed, offset, step):
+        return (seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF,
+                0 if step is None else self._whole("step", step, "i64", ()))
+
+
+def _check_p(who, p):
+    if not 0.0 <= p <= 1.0:
+        raise ValueError("%s: p = %r is not in 0 .. 1" % (who, p))
 
 
 class Dropout(_RowOperator):
     """Dropout of ``[rows, cols]`` arrays by the counter-based generator, its
     mask drawn when needed and never stored: the same ``seed`` and ``offset``
-    give the same mask. ``step``, a one-element i64 array without dimensions,
-    is added to ``offset`` on the device."""
+    give the same mask. ``step``, an i64 array without dimensions, is added
+    to ``offset`` on the device."""
 
     _who = "Dropout"
+    _io = struct.Struct("3Q6q")  # cchip_dropout_io
 
     def __init__(self, dtype, rows, cols, p, scale=1.0):
         super().__init__()
-        if dtype not in CODES:
-            raise ValueError("Dropout: dtype %r is not f32, bf16 or f16" % (dtype,))
-        if not 0.0 <= p <= 1.0:
-            raise ValueError("Dropout: p = %r is not in 0 .. 1" % (p,))
+        _check_dtype("Dropout", dtype)
+        _check_p("Dropout", p)
         self.dtype = dtype
-        self.p = p
-        self.scale = scale
+        self._desc = _lib.DropoutDesc(CODES[dtype], rows, cols, p, scale)
         self._shape = (rows, cols)
 
     def forward(self, x, out, *, seed, offset=0, residual=None, step=None, stream=None):
         """``out = residual + scale drop(x)``; out may be x or residual."""
-        drop = _lib.DropDesc(self.p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, self._step(step))
-        check(lib().cchip_dropout(CODES[self.dtype], self._shape[0], self._shape[1], drop, self.scale,
-                                  self._rows("x", x, True), self._rows("residual", residual), self._rows("out", out, True),
-                                  _stream_ptr(stream)))
+        io = self._io.pack(*self._seed(seed, offset, step), *self._needed("x", x), *self._rows("residual", residual),
+                           *self._needed("out", out))
+        check(lib().cchip_dropout_run(self._desc, io, _stream_ptr(stream)))
 
     def backward(self, dout, dx, *, seed, offset=0, step=None, stream=None):
         """``dx = scale drop(dout)`` with the forward pass's mask; the residual's
@@ -314,7 +340,7 @@ class Dropout(_RowOperator):
         self.forward(dout, dx, seed=seed, offset=offset, step=step, stream=stream)
 
 
-_PARAMS = ("post_weight", "post_bias", "channel_scale", "pre_weight", "pre_bias")
+_PARAMS = {"post_weight": 0, "post_bias": 1, "channel_scale": 2, "pre_weight": 3, "pre_bias": 4}
 
 
 class NormBlock(_RowOperator):
@@ -327,45 +353,45 @@ class NormBlock(_RowOperator):
     ``weight_dtype`` ("f32" or ``dtype``); one that is not given is 1 or 0."""
 
     _who = "NormBlock"
+    _io = struct.Struct("3Q10q20q")  # cchip_norm_block_io
 
     def __init__(self, dtype, rows, width, norm="rms", pre="rms", gate="none", dropout=0.0, scale=1.0, eps=1e-6,
                  weight_dtype="f32"):
         super().__init__()
-        if dtype not in CODES or weight_dtype not in CODES:
-            raise ValueError("NormBlock: dtypes %r and %r are not f32, bf16 or f16" % (dtype, weight_dtype))
+        _check_dtype("NormBlock", dtype, weight_dtype)
+        _check_p("NormBlock", dropout)
         if norm not in NORMS or pre not in NORMS or gate not in GATES:
             raise ValueError("NormBlock: unknown norm %r, pre %r or gate %r" % (norm, pre, gate))
-        if not 0.0 <= dropout <= 1.0:
-            raise ValueError("NormBlock: dropout = %r is not in 0 .. 1" % (dropout,))
         self.dtype = dtype
         self.weight_dtype = weight_dtype
-        self.p = dropout
         self._shape = (rows, width)
+        self._vector = (width,)
         self._desc = _lib.NormBlockDesc(CODES[dtype], CODES[weight_dtype], rows, width, NORMS[norm], NORMS[pre], GATES[gate],
-                                        scale, eps)
+                                        scale, eps, dropout)
         w = ctypes.c_size_t()
         check(lib().cchip_norm_block_workspace(self._desc, ctypes.byref(w)))
-        self._workspace_bytes = w.value
+        self._backward_bytes = w.value
+
+    def reserve(self, stream=None):
+        """Allocate a stream's workspace ahead of the first backward call on it."""
+        self._workspace(_stream_ptr(stream), self._backward_bytes)
 
     def _vectors(self, given):
-        p = _lib.NormParams()
+        p = [0, 0, 0, 0, 0]
         for n, x in given.items():
             if n not in _PARAMS:
                 raise ValueError("NormBlock: unknown parameter %s" % n)
-            setattr(p, n, self._whole(n, x, self.weight_dtype, self._shape[1:]))
+            p[_PARAMS[n]] = self._whole(n, x, self.weight_dtype, self._vector)
         return p
-
-    def _drop(self, seed, offset, step):
-        return _lib.DropDesc(self.p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, self._step(step))
 
     def forward(self, y, h, n=None, *, gate=None, residual=None, seed=0, offset=0, step=None, stream=None, **params):
         """Write ``h``, and ``n`` if there is a norm of it. h may be residual or
         y, n may be y. ``params``: post_weight, post_bias, channel_scale,
         pre_weight, pre_bias. ``seed``, ``offset`` and ``step`` as for Dropout."""
-        check(lib().cchip_norm_block_forward(self._desc, self._drop(seed, offset, step), self._vectors(params),
-                                             self._rows("y", y, True), self._rows("gate", gate),
-                                             self._rows("residual", residual), self._rows("h", h, True),
-                                             self._rows("n", n), _stream_ptr(stream)))
+        io = self._io.pack(*self._seed(seed, offset, step), *self._vectors(params), 0, 0, 0, 0, 0,
+                           *self._needed("y", y), *self._rows("gate", gate), *self._rows("residual", residual),
+                           *self._needed("h", h), *self._rows("n", n), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+        check(lib().cchip_norm_block_forward(self._desc, io, _stream_ptr(stream)))
 
     def backward(self, y, dh, dy, *, dn=None, h=None, gate=None, dgate=None, dresidual=None, grads=None, seed=0, offset=0,
                  step=None, stream=None, **params):
@@ -373,9 +399,9 @@ class NormBlock(_RowOperator):
         gradients of h and n, write those of y, gate and residual and, for each
         name in ``grads``, of that parameter, summed over the rows."""
         s = _stream_ptr(stream)
-        check(lib().cchip_norm_block_backward(self._desc, self._drop(seed, offset, step), self._vectors(params),
-                                              self._vectors(grads or {}), self._rows("y", y, True), self._rows("gate", gate),
-                                              self._rows("h", h), self._rows("dh", dh, True), self._rows("dn", dn),
-                                              self._rows("dy", dy, True), self._rows("dgate", dgate),
-                                              self._rows("dresidual", dresidual), self._workspace(s), self._workspace_bytes,
-                                              s))
+        io = self._io.pack(*self._seed(seed, offset, step), *self._vectors(params), *self._vectors(grads or {}),
+                           *self._needed("y", y), *self._rows("gate", gate), 0, 0, *self._rows("h", h), 0, 0,
+                           *self._needed("dh", dh), *self._rows("dn", dn), *self._needed("dy", dy),
+                           *self._rows("dgate", dgate), *self._rows("dresidual", dresidual))
+        n = self._backward_bytes if grads else 0
+        check(lib().cchip_norm_block_backward(self._desc, io, self._workspace(s, n), n, s))

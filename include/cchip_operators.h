@@ -87,10 +87,12 @@ typedef struct {
   void *saved;                         /* forward: written (NULL: no backward pass follows); backward: read */
 } cchip_gated_delta_io;
 
-/* Bytes of workspace that a forward or backward call needs (it holds nothing
-   between calls; calls that overlap need one each) and of `saved`. Both are
-   aligned to 16 bytes. */
-int cchip_gated_delta_sizes(const cchip_gated_delta *op, size_t *workspace, size_t *saved);
+/* Bytes of workspace that a forward and a backward call need (a workspace
+   holds nothing between calls; calls that overlap need one each), and of
+   `saved`. All are aligned to 16 bytes. A forward call that saves needs no
+   workspace, nor does one of at most 8 tokens a sequence, not packed, that
+   does not: it runs the recurrence itself. */
+int cchip_gated_delta_sizes(const cchip_gated_delta *op, size_t *forward, size_t *backward, size_t *saved);
 int cchip_gated_delta_forward(const cchip_gated_delta *op, const cchip_gated_delta_io *io, void *workspace,
                               size_t workspace_bytes, void *stream);
 int cchip_gated_delta_backward(const cchip_gated_delta *op, const cchip_gated_delta_io *io, void *workspace,
@@ -108,10 +110,11 @@ int cchip_gated_delta_backward(const cchip_gated_delta *op, const cchip_gated_de
  * when the kernel runs, so that a captured graph draws anew on each replay.
  */
 typedef struct {
-  double p; /* 0 <= p <= 1 */
-  uint64_t seed, offset;
-  const uint64_t *step;
-} cchip_drop;
+  int dtype;
+  int64_t rows, cols; /* rows < 2^32, cols < 2^35 */
+  double p;           /* 0 <= p <= 1 */
+  float scale;
+} cchip_dropout;
 
 /* A matrix: rows `row` elements apart, the elements of a row adjacent. */
 typedef struct {
@@ -119,11 +122,16 @@ typedef struct {
   int64_t row;
 } cchip_rows;
 
-/* out = residual + scale drop(x), residual.data NULL: no residual. The
+typedef struct {
+  uint64_t seed, offset;
+  const uint64_t *step;
+  cchip_rows x, residual, out;
+} cchip_dropout_io;
+
+/* out = residual + scale drop(x); residual.data NULL: no residual. The
    gradient of x is the same call on the gradient of out, without residual.
-   out may be x or residual. rows < 2^32, cols < 2^35. */
-int cchip_dropout(int dtype, int64_t rows, int64_t cols, const cchip_drop *drop, float scale, cchip_rows x,
-                  cchip_rows residual, cchip_rows out, void *stream);
+   out may be x or residual. */
+int cchip_dropout_run(const cchip_dropout *op, const cchip_dropout_io *io, void *stream);
 
 /* ---- Norm block ---------------------------------------------------------- */
 
@@ -151,29 +159,34 @@ typedef struct {
   int64_t rows, width; /* rows < 2^32, width <= 32768 */
   int post, pre, gate;
   float scale, eps;
+  double p; /* of dropout */
 } cchip_norm_block;
 
 typedef struct {
-  const void *post_weight, *post_bias, *channel_scale, *pre_weight, *pre_bias;
+  void *post_weight, *post_bias, *channel_scale, *pre_weight, *pre_bias;
 } cchip_norm_params;
 
 typedef struct {
-  void *post_weight, *post_bias, *channel_scale, *pre_weight, *pre_bias; /* NULL: not wanted */
-} cchip_norm_grads;
+  uint64_t seed, offset; /* of dropout, as in cchip_dropout_io */
+  const uint64_t *step;
+  cchip_norm_params params;
+  cchip_norm_params grads;            /* backward: written; NULL: not wanted */
+  cchip_rows y, gate;                 /* read by both */
+  cchip_rows residual;                /* forward: read */
+  cchip_rows h, n;                    /* forward: written; backward: h is read */
+  cchip_rows dh, dn;                  /* backward: read */
+  cchip_rows dy, dgate, dresidual;    /* backward: written; dgate, dresidual NULL: not wanted */
+} cchip_norm_block_io;
 
 /* h may be `residual` or y, n may be y. n is NULL iff pre is none. */
-int cchip_norm_block_forward(const cchip_norm_block *op, const cchip_drop *drop, const cchip_norm_params *params,
-                             cchip_rows y, cchip_rows gate, cchip_rows residual, cchip_rows h, cchip_rows n,
-                             void *stream);
+int cchip_norm_block_forward(const cchip_norm_block *op, const cchip_norm_block_io *io, void *stream);
 /* From y, gate, the forward pass's h (needed iff pre is not none), and the
-   gradients dh and dn of its results: the gradients of y, gate and residual
-   (dresidual.data NULL: not wanted) and of the parameters, summed over rows
-   in f32 in an order that does not change from run to run. */
+   gradients dh and dn of its results: the gradients of y, gate, residual and
+   the parameters, those summed over rows in f32 in an order that does not
+   change from run to run. */
 int cchip_norm_block_workspace(const cchip_norm_block *op, size_t *bytes);
-int cchip_norm_block_backward(const cchip_norm_block *op, const cchip_drop *drop, const cchip_norm_params *params,
-                              const cchip_norm_grads *grads, cchip_rows y, cchip_rows gate, cchip_rows h,
-                              cchip_rows dh, cchip_rows dn, cchip_rows dy, cchip_rows dgate, cchip_rows dresidual,
-                              void *workspace, size_t workspace_bytes, void *stream);
+int cchip_norm_block_backward(const cchip_norm_block *op, const cchip_norm_block_io *io, void *workspace,
+                              size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
