@@ -15,7 +15,7 @@ constexpr int64_t kStepTokens = 8;
 
 struct Layout {
   int64_t slots, slot_heads;
-  size_t record, record_back, states, us;  // bytes, all slots and heads
+  size_t record, record_back, states, us, dots;  // bytes, all slots and heads
 };
 
 void check_op(const cchip_gated_delta *op) {
@@ -51,6 +51,7 @@ Layout layout_of(const cchip_gated_delta &op) {
     p.record = size_t(p.slot_heads) * record_bytes<M>(false);
     p.record_back = size_t(p.slot_heads) * record_bytes<M>(true);
     p.states = size_t(p.slot_heads) * padded_key_dim(op.key_dim) * padded_value_dim(op) * sizeof(typename M::Saved);
+    p.dots = size_t(p.slot_heads) * (padded_value_dim(op) / 16) * 4 * sizeof(float);
     p.us = size_t(p.slot_heads) * kChunk * padded_value_dim(op) * sizeof(float);
   });
   return p;
@@ -133,7 +134,7 @@ int cchip_gated_delta_sizes(const cchip_gated_delta *op, size_t *forward, size_t
     check_op(op);
     const Layout p = layout_of(*op);
     if (forward) *forward = steps(*op, false) ? 0 : p.record;
-    if (backward) *backward = p.states + p.us;
+    if (backward) *backward = p.states + p.us + p.dots;
     if (saved) *saved = p.record_back + p.states + p.us;
   });
 }
@@ -169,9 +170,10 @@ int cchip_gated_delta_backward(const cchip_gated_delta *op, const cchip_gated_de
     a.slots = p.slots;
     if (a.sequences == 0) return;
     lay_out(a, p, static_cast<char *>(io->saved));
-    check_workspace(workspace, workspace_bytes, p.states + p.us);
+    check_workspace(workspace, workspace_bytes, p.states + p.us + p.dots);
     a.grads = static_cast<char *>(workspace);
     a.ys = reinterpret_cast<float *>(a.grads + p.states);
+    a.dots = reinterpret_cast<float *>(a.grads + p.states + p.us);
     delta_backward_launch(*op, a, (hipStream_t)stream);
   });
 }

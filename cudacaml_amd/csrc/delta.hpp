@@ -49,6 +49,7 @@ struct DeltaArgs {
   float *us;      // saved U, 64 rows
   char *grads;    // backward: dS after the chunk
   float *ys;      // backward: Y
+  float *dots;    // backward: sums that make <S, dS>, four for each 16 value columns
   int64_t tokens, sequences;  // sequences: of the packed batch, or its rows
   int64_t slots;
   int chunks;  // of a row of the batch; unused where packed
@@ -309,6 +310,23 @@ __device__ __forceinline__ void put_block(char *rows, int row, int y, const f32x
   } else {
     *reinterpret_cast<uint64_t *>(to) = u.half;
   }
+}
+
+template <typename T, int TV>
+__device__ __forceinline__ RawV<T, TV> load_block(const char *rows, int row, int y) {
+  union {
+    RawV<T, TV> r;
+    u32x4 w[sizeof(RawV<T, TV>) >= 16 ? sizeof(RawV<T, TV>) / 16 : 1];
+    uint64_t half;
+  } u;
+  const char *from = rows + uint32_t(row * 32 + y) * uint32_t(sizeof(T));
+  if constexpr (sizeof(u.r) >= 16) {
+#pragma unroll
+    for (int i = 0; i < int(sizeof(u.r) / 16); i++) u.w[i] = reinterpret_cast<const u32x4 *>(from)[i];
+  } else {
+    u.half = *reinterpret_cast<const uint64_t *>(from);
+  }
+  return u.r;
 }
 
 template <typename T>

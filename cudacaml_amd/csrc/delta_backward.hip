@@ -28,7 +28,8 @@ namespace {
 
 // The counterpart of delta_forward, laid out like it: BV value columns of a
 // head, E in registers, each chunk's rows asked for while the one after it is
-// computed.
+// computed. <S, E> is summed here, where E still is f32: of the two in bf16
+// it would be off by both their roundings.
 template <typename M, int DK, int BV, bool Fast>
 __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int blocks) {
   typedef typename M::T T;
@@ -73,6 +74,7 @@ __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int b
   };
   auto record = [&](int i) { return a.records + ((sq.slot + i) * a.hv + h) * R::bytes(true); };
   Raw8<T> rk[DK / 32], rq[DK / 32], ro;
+  RawV<Saved, TV> rs[TK];
   Frag<NS> tt[2], pt[2];  // rows 16 w .. of T^T and P^T: terms from the diagonal on
   float og, gam, last, beta, end;
   auto fetch = [&](int i) {
@@ -83,6 +85,9 @@ __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int b
       rk[j] = load_head8<Fast, T>(a.k, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk);
       rq[j] = load_head8<Fast, T>(a.q, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk);
     }
+    const char *from = a.states + (((sq.slot + i) * a.hv + h) * a.dvp + dv0 / 32 * 32) * DK * int64_t(sizeof(Saved));
+#pragma unroll
+    for (int j = 0; j < TK; j++) rs[j] = load_block<Saved, TV>(from, x0 + 16 * j, dv0 % 32 + y0);
     if (has_o) {
       ro = load_head8<Fast, T>(a.d_o, c, h, ot, dv0 + od, a.dv);
       og = reinterpret_cast<const float *>(record(i) + R::Decay)[ot];
@@ -139,6 +144,17 @@ __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int b
     for (int i = 0; i < TK; i++)
 #pragma unroll
       for (int j = 0; j < TV; j++) put_four<NS>(es + (x0 + 16 * i) * LDV + y0 + 4 * j, EP, e[i][j]);
+    float dot = 0.0f;
+#pragma unroll
+    for (int i = 0; i < TK; i++)
+#pragma unroll
+      for (int j = 0; j < 4 * TV; j++) dot += float(rs[i].x[j]) * e[i][j / 4][j % 4];
+    dot = sum64(dot);
+    if (l == 0) {
+      float *dots = a.dots + (slot_head * (a.dvp / 16) + dv0 / 16) * 4;
+      dots[w] = dot;
+      if (TV == 2) dots[4 + w] = 0.0f;
+    }
     __syncthreads();
     fetch(next);
     char *to = a.grads + (slot_head * a.dvp + dv0 / 32 * 32) * DK * int64_t(sizeof(Saved));
@@ -345,6 +361,7 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
 
     f32x4 os[JK] = {}, ys[JK] = {}, ue[JK] = {}, ou[2] = {}, yu[2] = {};
     float yv = 0.0f, se = 0.0f;  // yv: this lane's columns
+    for (int i = tid; i < a.dvp / 4; i += 512) se += a.dots[slot_head * (a.dvp / 4) + i];
     for (int v0 = 0; v0 < a.dvp; v0 += 32) {
       const Frag<NI> fo = frag_of<NI>(keep_head8<Fast>(ro, c, t, v0 + 8 * quad, a.dv));
       const Frag<NU> fy = frag_of<NU>(ry);
@@ -354,8 +371,6 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
       if (has_u) put_frag<NU>(us + ux * LDS + sv, UP, frag_of<NU>(ru));
       Raw8<Saved> late = re;
       if (has_s) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) se += float(rs.x[i]) * float(re.x[i]);
         put_frag<NB>(ss + sx * LDS + sv, SP, frag_of<NB>(rs));
         if (kBoth) put_frag<NB>(es + sx * LDS + sv, SP, frag_of<NB>(re));
       }

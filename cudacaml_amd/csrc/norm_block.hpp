@@ -170,9 +170,12 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_forward(const 
 
 // d becomes the gradient of what `normalise` read, from that of what it
 // gave: (d - mean(d) - xhat mean(d xhat)) inv, the first mean of a layer norm.
+// Of a row of one value, or two centred ones, all of d lies along xhat and
+// what is left is eps inv^2 of it: there the projection is taken off twice
+// and that share put back, as the difference itself would be rounding.
 template <int LANES, int V>
 __device__ __forceinline__ void normalise_back(float (&d)[V][8], const float (&xhat)[V][8], int kind, float inv,
-                                               float inv_width, RowSum<LANES> &sum) {
+                                               float inv_width, float eps, int width, RowSum<LANES> &sum) {
   float p = 0.0f, q = 0.0f;
 #pragma unroll
   for (int v = 0; v < V; v++)
@@ -183,10 +186,24 @@ __device__ __forceinline__ void normalise_back(float (&d)[V][8], const float (&x
     }
   p = sum(p) * inv_width;
   q = kind == CCHIP_NORM_LAYER ? sum(q) * inv_width : 0.0f;
+  float back = 0.0f;
+  if (width <= 2) {
+    float s = 0.0f;
+    for (int i = 0; i < 8; i++) s += xhat[0][i] * xhat[0][i];
+    s = sum(s) * inv_width;  // mean of xhat^2, 1 - eps inv^2
+    const float once = s > 0.0f ? p / s : 0.0f;
+    float r = 0.0f;
+    for (int i = 0; i < 8; i++) r += (d[0][i] - q - xhat[0][i] * once) * xhat[0][i];
+    r = sum(r) * inv_width;
+    const float twice = s > 0.0f ? r / s : 0.0f;
+    for (int i = 0; i < 8; i++) d[0][i] = (d[0][i] - q - xhat[0][i] * once) - xhat[0][i] * twice;
+    back = once * eps * inv * inv;
+    p = q = 0.0f;
+  }
 #pragma unroll
   for (int v = 0; v < V; v++)
 #pragma unroll
-    for (int i = 0; i < 8; i++) d[v][i] = (d[v][i] - xhat[v][i] * p - q) * inv;
+    for (int i = 0; i < 8; i++) d[v][i] = (d[v][i] - xhat[v][i] * (p - back) - q) * inv;
 }
 
 // The parameters' gradients in the order of their sums; without Bias there
@@ -246,7 +263,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_backward(const
           d[v][i] = i < n[v] ? dn * pw[v][i] : 0.0f;
         }
       }
-      normalise_back<LANES, V>(d, x, a.pre, inv, inv_width, sum);
+      normalise_back<LANES, V>(d, x, a.pre, inv, inv_width, a.eps, a.width, sum);
 #pragma unroll
       for (int v = 0; v < V; v++)
 #pragma unroll
@@ -292,7 +309,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_backward(const
       }
       if (Gate && a.dgate.p) store8<T>(row_at<T>(a.dgate, row) + c, dz, n[v]);
     }
-    if (a.post != CCHIP_NORM_NONE) normalise_back<LANES, V>(d, x, a.post, inv, inv_width, sum);
+    if (a.post != CCHIP_NORM_NONE) normalise_back<LANES, V>(d, x, a.post, inv, inv_width, a.eps, a.width, sum);
 #pragma unroll
     for (int v = 0; v < V; v++) store8<T>(row_at<T>(a.dy, row) + (v * LANES + lane) * 8, d[v], n[v]);
   }

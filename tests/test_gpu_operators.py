@@ -1,0 +1,646 @@
+"""The layer operators on the device against the 64-bit references of
+operator_reference.py.
+
+Bounds, in the 2-norm over an output, from the formats alone:
+- f32 results: a result passes through at most five chained sums of up to 128
+  products; f32 sums of n terms are off by about sqrt(n) 2^-24 of their terms'
+  norm, 7e-7 each, and 3.4e-6 together: 4e-6. The gradient of g sums 64 of
+  such results once more: 8e-6.
+- bf16 results are rounded to at most 2^-9 of themselves, and in the gated
+  delta rule come through one operand that is rounded to as much: 2 x 2^-9.
+  f16 results likewise: 2 x 2^-12, operands being kept to 16 bits or more. No
+  f16 is nearer to a value below 2^-14 than half its step of 2^-24 there.
+- results that a single element could dominate are also held element by
+  element, to 16 times the bound of the larger of the value and the root mean
+  square: what a rounding of one operand can do to a sum of few terms.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+import operator_reference as R
+from cudacaml_amd import backend_hip as H
+from cudacaml_amd import operators as O
+from cudacaml_amd.runtime import Buffer, Device, Stream
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+BOUND = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 4e-6}
+
+
+def close(got, want, name, bound=None):
+    bound = bound or BOUND[got.dtype]
+    a, b = got.detach().double().cpu().numpy(), np.asarray(want, dtype=np.float64)
+    assert a.shape == b.shape, name
+    if not b.size:
+        return
+    assert np.isfinite(a).all(), name
+    norm = np.linalg.norm(b)
+    if norm == 0.0:
+        assert not a.any(), name
+        return
+    rms = norm / np.sqrt(b.size)
+    step = 2.0 ** -25 if got.dtype == torch.float16 else 0.0  # what the nearest f16 to a tiny value may be off
+    miss = np.maximum(np.abs(a - b) - step, 0.0)
+    off = np.linalg.norm(miss) / norm
+    assert off <= bound, "%s is %.3g off, %.3g allowed" % (name, off, bound)
+    most = (miss / np.maximum(np.abs(b), rms)).max()
+    assert most <= 16 * bound, "%s has an element %.3g off, %.3g allowed" % (name, most, 16 * bound)
+
+
+def arrays(dtype, batch, tokens, hk, hv, dk, dv, seed=0, states=0, back=False):
+    """What a layer feeds the rule: unit keys and queries, decays and rates in
+    0 .. 1, already rounded to the type."""
+    g = torch.Generator().manual_seed(seed)
+    n = lambda *s: torch.randn(s, generator=g)  # noqa: E731
+    x = dict(q=torch.nn.functional.normalize(n(batch, tokens, hk, dk), dim=-1),
+             k=torch.nn.functional.normalize(n(batch, tokens, hk, dk), dim=-1), v=n(batch, tokens, hv, dv),
+             g=-torch.nn.functional.softplus(n(batch, tokens, hv) - 1.0), beta=torch.sigmoid(n(batch, tokens, hv)))
+    if back:
+        x["do"] = n(batch, tokens, hv, dv)
+    x = {k: v.to(TYPES[dtype]) for k, v in x.items()}
+    if states:
+        x["state"] = n(states, hv, dk, dv) * 0.3
+        if back:
+            x["dstate_out"] = n(states, hv, dk, dv) * 0.3
+    return x
+
+
+def run_delta(x, dtype, cuts=None, back=False, layout=None, stream=None, handle=None, save=None):
+    """Every output of the operator for CPU arrays x, as device tensors."""
+    b, t, hk, dk = x["q"].shape
+    hv, dv = x["v"].shape[2:]
+    states = "state" in x
+    op = handle or O.GatedDelta(dtype, b, t, hk, hv, dk, dv, sequences=None if cuts is None else len(cuts) - 1,
+                                states=states)
+    dev = {k: v.cuda() for k, v in x.items()}
+    if layout:
+        dev = layout(dev)
+    e = torch.empty_like
+    offsets = None if cuts is None else torch.tensor(cuts, dtype=torch.int32, device="cuda")
+    out = {"o": torch.full((b, t, hv, dv), float("nan"), dtype=TYPES[dtype], device="cuda")}
+    if states:
+        out["state"] = torch.full_like(dev["state"], float("nan"))
+    saved = None
+    if back or save:
+        saved = torch.full((op.saved_bytes(),), 255, dtype=torch.uint8, device="cuda")
+    ins = [dev[n] for n in ("q", "k", "v", "g", "beta")]
+    op.forward(*ins, out["o"], state=dev.get("state"), state_out=out.get("state"), offsets=offsets, saved=saved,
+               stream=stream)
+    if back:
+        for n in ("q", "k", "v", "g", "beta"):
+            out["d" + n] = torch.full(x[n].shape, float("nan"), dtype=TYPES[dtype], device="cuda")
+        if states:
+            out["dstate"] = e(out["state"])
+        op.backward(*ins, dev["do"], saved, *(out["d" + n] for n in ("q", "k", "v", "g", "beta")),
+                    dstate_out=dev.get("dstate_out"), dstate=out.get("dstate"), offsets=offsets, stream=stream)
+    torch.cuda.synchronize()
+    return out
+
+
+def check_delta(x, dtype, cuts=None, back=False, **kw):
+    got = run_delta(x, dtype, cuts, back, **kw)
+    want = R.delta_batch({n: v.double().numpy() for n, v in x.items()}, cuts, x["q"].shape[3] ** -0.5,
+                         x["state"].double().numpy() if "state" in x else None, back)
+    for n, v in got.items():
+        close(v, want[n], n, 8e-6 if n == "dg" and v.dtype == torch.float32 else None)
+    return got
+
+
+SHAPES = [  # batch, tokens, key heads, value heads, key_dim, value_dim
+    (1, 1, 1, 1, 1, 1), (3, 1, 2, 4, 128, 128), (2, 2, 1, 2, 64, 64), (2, 8, 2, 2, 72, 100), (2, 9, 1, 1, 128, 64),
+    (1, 63, 1, 2, 64, 32), (1, 64, 2, 2, 128, 128), (2, 65, 1, 4, 17, 250), (1, 130, 3, 3, 40, 33), (2, 200, 2, 4, 128, 96),
+]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", SHAPES)
+def test_gated_delta_forward(device, dtype, shape):
+    check_delta(arrays(dtype, *shape, states=shape[0]), dtype)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", SHAPES)
+def test_gated_delta_backward(device, dtype, shape):
+    check_delta(arrays(dtype, *shape, seed=1, states=shape[0], back=True), dtype, back=True)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_gated_delta_without_states(device, dtype):
+    check_delta(arrays(dtype, 2, 150, 2, 4, 128, 128, seed=2, back=True), dtype, back=True)
+    check_delta(arrays(dtype, 2, 5, 2, 4, 64, 128, seed=2), dtype)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("cuts", [[0, 0], [0, 0, 1, 1, 64, 129, 129, 300], [0, 300], [0, 63, 64, 65, 192, 256, 299, 300]])
+def test_gated_delta_packed(device, dtype, cuts):
+    """Empty sequences, single tokens, ends inside and at chunks' ends; an
+    empty one's last state is its first."""
+    x = arrays(dtype, 1, max(cuts[-1], 1), 2, 4, 64, 72, seed=3, states=len(cuts) - 1, back=True)
+    if cuts[-1] == 0:
+        x = {k: v[:, :0] if v.dim() < 5 and "state" not in k else v for k, v in x.items()}
+    got = check_delta(x, dtype, cuts, back=True)
+    for i, (a, b) in enumerate(zip(cuts, cuts[1:])):
+        if a == b:
+            assert torch.equal(got["state"][i].cpu(), x["state"][i])
+            assert torch.equal(got["dstate"][i].cpu(), x["dstate_out"][i])
+
+
+def test_gated_delta_no_tokens(device):
+    x = arrays("bf16", 2, 0, 1, 2, 32, 32, states=2)
+    got = run_delta(x, "bf16")
+    assert torch.equal(got["state"].cpu(), x["state"])
+
+
+def test_gated_delta_state_in_place_and_one_token_at_a_time(device):
+    """A prompt, then tokens one by one on the same state: as one sequence."""
+    x = arrays("f32", 2, 100, 2, 4, 64, 64, seed=4, states=2)
+    want = R.delta_batch({n: v.double().numpy() for n, v in x.items()}, None, 64 ** -0.5, x["state"].double().numpy(), False)
+    dev = {k: v.cuda() for k, v in x.items()}
+    state, o = dev["state"].clone(), torch.empty_like(dev["v"])
+    part = lambda a, b: [dev[n][:, a:b] for n in ("q", "k", "v", "g", "beta")]  # noqa: E731
+    O.GatedDelta("f32", 2, 70, 2, 4, 64, 64).forward(*part(0, 70), o[:, :70], state=state, state_out=state)
+    one = O.GatedDelta("f32", 2, 1, 2, 4, 64, 64)
+    for t in range(70, 97):
+        one.forward(*part(t, t + 1), o[:, t:t + 1], state=state, state_out=state)
+    O.GatedDelta("f32", 2, 3, 2, 4, 64, 64).forward(*part(97, 100), o[:, 97:], state=state, state_out=state)
+    close(o, want["o"], "o")
+    close(state, want["state"], "state")
+
+
+def _from_one_projection(dev):
+    """q, k and v as slices of one tensor, an odd number of elements apart."""
+    b, t, hk, dk = dev["q"].shape
+    hv, dv = dev["v"].shape[2:]
+    whole = torch.full((b, t, 2 * hk * dk + hv * dv + 3), float("nan"), dtype=dev["q"].dtype, device="cuda")
+    at = 1
+    for n, h, d in (("q", hk, dk), ("k", hk, dk), ("v", hv, dv)):
+        part = whole[:, :, at:at + h * d].unflatten(2, (h, d))
+        part.copy_(dev[n])
+        dev[n] = part
+        at += h * d
+    return dev
+
+
+def _heads_first(dev):
+    """Everything stored [batch, heads, tokens, ...]."""
+    return {k: v.transpose(1, 2).contiguous().transpose(1, 2) if "state" not in k else v for k, v in dev.items()}
+
+
+@pytest.mark.parametrize("layout", [_from_one_projection, _heads_first])
+@pytest.mark.parametrize("shape", [(2, 70, 2, 4, 64, 96), (2, 70, 1, 2, 20, 12), (3, 3, 2, 2, 20, 12)])
+def test_gated_delta_strides(device, layout, shape):
+    """Views of any stride and alignment give what contiguous tensors give."""
+    x = arrays("bf16", *shape, seed=5, states=shape[0], back=True)
+    a = run_delta(x, "bf16", back=True)
+    b = run_delta(x, "bf16", back=True, layout=layout)
+    for n in a:
+        assert torch.equal(a[n], b[n]), n
+
+
+def test_gated_delta_writes_only_its_outputs(device):
+    """Strided outputs: what lies between their elements keeps its value."""
+    x = {k: v.cuda() for k, v in arrays("bf16", 2, 70, 2, 4, 40, 24, seed=6).items()}
+    op = O.GatedDelta("bf16", 2, 70, 2, 4, 40, 24, states=False)
+    wide = torch.full((2, 70, 4, 29), 7.0, dtype=torch.bfloat16, device="cuda")
+    op.forward(*x.values(), wide[..., 2:26])
+    plain = torch.empty(2, 70, 4, 24, dtype=torch.bfloat16, device="cuda")
+    op.forward(*x.values(), plain)
+    torch.cuda.synchronize()
+    assert torch.equal(wide[..., 2:26], plain)
+    assert bool((wide[..., :2] == 7).all()) and bool((wide[..., 26:] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_gated_delta_extreme_gates(device, dtype):
+    """Decays to nothing (g of -inf and of the type's lowest value forget the
+    state), no decay, rates of 0 (a token that writes nothing still has a
+    gradient of its rate) and of 1."""
+    x = arrays(dtype, 2, 140, 1, 2, 64, 64, seed=7, states=2, back=True)
+    x["g"][0, 10] = -float("inf")
+    x["g"][0, 70:73] = torch.finfo(TYPES[dtype]).min
+    x["g"][1, 20:90] = 0.0
+    x["beta"][0, 30:40] = 0.0
+    x["beta"][1, 64:100] = 1.0
+    x["beta"][1, 127] = 0.0
+    check_delta(x, dtype, back=True)
+
+
+def test_gated_delta_equal_keys(device):
+    """Keys that are all the same and rates of 1: the triangular systems are
+    as far from the identity as they get."""
+    x = arrays("f32", 1, 130, 1, 1, 32, 32, seed=8, states=1, back=True)
+    x["k"] = x["k"][:, :1].expand_as(x["k"]).clone()
+    x["beta"].fill_(1.0)
+    x["g"].fill_(-1e-3)
+    check_delta(x, "f32", back=True)
+
+
+def test_gated_delta_large_values(device):
+    """Values far from 1, as bf16 holds them: nothing inside has less range."""
+    x = arrays("bf16", 1, 100, 1, 2, 64, 64, seed=9, back=True)
+    x["v"] = (x["v"].float() * 1e20).bfloat16()
+    x["do"] = (x["do"].float() * 1e-18).bfloat16()
+    check_delta(x, "bf16", back=True)
+
+
+def test_gated_delta_nan_stays_in_its_sequence(device):
+    """A NaN reaches its own sequence and value heads and no chunk before its
+    own in the forward pass."""
+    cuts = [0, 100, 200, 300]
+    x = arrays("bf16", 1, 300, 1, 2, 64, 64, seed=10, states=3, back=True)
+    clean = run_delta(x, "bf16", cuts, back=True)
+    x["v"][0, 170, 1, 3] = float("nan")
+    got = run_delta(x, "bf16", cuts, back=True)
+    same = torch.ones(300, dtype=torch.bool)
+    same[100:200] = False
+    for n in ("o", "dq", "dk", "dv", "dg", "dbeta"):
+        assert torch.equal(got[n][:, same], clean[n][:, same]), n
+    assert torch.equal(got["o"][:, 100:164], clean["o"][:, 100:164])
+    assert torch.equal(got["o"][:, :, 0], clean["o"][:, :, 0])
+    assert got["o"][0, 170, 1].isnan().any()
+    assert torch.equal(got["state"][[0, 2]], clean["state"][[0, 2]])
+
+
+def test_gated_delta_is_deterministic_and_handles_keep_nothing(device):
+    """The same call twice gives the same bits, other calls between or not."""
+    x = arrays("bf16", 2, 300, 2, 8, 128, 64, seed=11, back=True)
+    y = arrays("bf16", 2, 300, 2, 8, 128, 64, seed=12, back=True)
+    op = O.GatedDelta("bf16", 2, 300, 2, 8, 128, 64, states=False)
+    a = run_delta(x, "bf16", back=True, handle=op)
+    run_delta(y, "bf16", back=True, handle=op)
+    b = run_delta(x, "bf16", back=True, handle=op)
+    for n in a:
+        assert torch.equal(a[n], b[n]), n
+
+
+def test_gated_delta_differences(device):
+    """The kernels' own forward pass against their gradient: a central
+    difference of step h is off by h^2 times third derivatives (1e-4 for unit
+    directions and h = 1e-2), and the f32 forward pass's rounding of about
+    4e-6 of a sum of 2e4 terms' norm over 2 h adds as much: 2e-2 of the norm
+    of gradient times direction."""
+    x = arrays("f32", 1, 150, 1, 2, 32, 32, seed=13, states=1, back=True)
+    got = run_delta(x, "f32", back=True)
+    w = {n: v.double() for n, v in x.items()}
+
+    def loss(name, value):
+        out = run_delta({**x, name: value.float()}, "f32")
+        return float((out["o"].double().cpu() * w["do"]).sum() + (out["state"].double().cpu() * w["dstate_out"]).sum())
+
+    g = torch.Generator().manual_seed(1)
+    for n, at in (("q", "dq"), ("k", "dk"), ("v", "dv"), ("g", "dg"), ("beta", "dbeta"), ("state", "dstate")):
+        d = torch.randn(x[n].shape, generator=g, dtype=torch.float64)
+        d /= d.norm()
+        h = 1e-2
+        want = (loss(n, w[n] + h * d) - loss(n, w[n] - h * d)) / (2 * h)
+        grad = got[at].double().cpu()
+        assert abs(float((grad * d).sum()) - want) <= 2e-2 * max(1.0, float(grad.norm())), n
+
+
+def test_gated_delta_on_another_stream(device):
+    """Work on a stream of its own, its workspace with it, next to other work
+    on the default stream with the same handle."""
+    x = arrays("bf16", 2, 200, 2, 4, 64, 64, seed=14, states=2, back=True)
+    op = O.GatedDelta("bf16", 2, 200, 2, 4, 64, 64)
+    want = run_delta(x, "bf16", back=True, handle=op)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for stream in (side, Stream.create(), side.cuda_stream):
+        got = run_delta(x, "bf16", back=True, handle=op, stream=stream)
+        for n in want:
+            assert torch.equal(got[n], want[n]), n
+
+
+def test_gated_delta_in_a_graph(device):
+    """Captured once and replayed on new inputs, with eager calls between."""
+    shape = (2, 130, 1, 2, 64, 64)
+    op = O.GatedDelta("bf16", *shape, states=False)
+    one, two = (arrays("bf16", *shape, seed=s, back=True) for s in (15, 16))
+    want = [run_delta(x, "bf16", back=True) for x in (one, two)]
+    dev = {k: v.cuda() for k, v in one.items()}
+    names = ("q", "k", "v", "g", "beta")
+    out = {"o": torch.empty_like(dev["v"]), **{"d" + n: torch.empty_like(dev[n]) for n in names}}
+    saved = torch.empty(op.saved_bytes(), dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.Stream()
+    op.reserve(stream, backward=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        op.forward(*(dev[n] for n in names), out["o"], saved=saved, stream=stream)
+        op.backward(*(dev[n] for n in names), dev["do"], saved, *(out["d" + n] for n in names), stream=stream)
+    for i in (0, 1, 0, 1):
+        for n, v in (one, two)[i].items():
+            dev[n].copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        for n in out:
+            assert torch.equal(out[n], want[i][n]), (i, n)
+        run_delta(two, "bf16", back=True)
+
+
+def test_operators_on_residents(device):
+    """The framework's own buffers, no other library's tensors."""
+    x = arrays("f32", 1, 70, 1, 1, 16, 16, seed=17)
+    live = Buffer.live_count()
+    res = {k: H.upload(np.ascontiguousarray(v.numpy())) for k, v in x.items()}
+    o = O.Array.empty("f32", (1, 70, 1, 16))
+    op = O.GatedDelta("f32", 1, 70, 1, 1, 16, 16, states=False)
+    op.forward(*res.values(), o)
+    Device.synchronize()
+    got = np.empty((1, 70, 1, 16), np.float32)
+    o.buf.download(got)
+    want = R.delta_batch({n: v.double().numpy() for n, v in x.items()}, None, 0.25, None, False)
+    close(torch.from_numpy(got), want["o"], "o")
+    for r in res.values():
+        H.free_resident(r)
+    o.free()
+    op.free()
+    assert Buffer.live_count() == live
+
+
+# ---- norm block --------------------------------------------------------------
+
+def norm_arrays(dtype, weight, rows, width, norm, pre, gate, residual=True, bias=True, channel=True, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    n = lambda *s: torch.randn(s, generator=g)  # noqa: E731
+    x = dict(y=n(rows, width), dh=n(rows, width))
+    if gate != "none":
+        x["gate"] = n(rows, width)
+    if residual:
+        x["residual"] = 2 * n(rows, width)
+    if pre != "none":
+        x.update(dn=n(rows, width), h=2 * n(rows, width) + 0.5)
+    x = {k: v.to(TYPES[dtype]) for k, v in x.items()}
+    w = {}
+    if norm != "none":
+        w["post_weight"] = 1 + 0.1 * n(width)
+        if bias:
+            w["post_bias"] = 0.1 * n(width)
+    if pre != "none":
+        w["pre_weight"] = 1 + 0.1 * n(width)
+        if bias:
+            w["pre_bias"] = 0.1 * n(width)
+    if channel:
+        w["channel_scale"] = 1 + 0.1 * n(width)
+    return x, {k: v.to(TYPES[weight]) for k, v in w.items()}
+
+
+def check_norm(dtype, weight, rows, width, norm, pre, gate, p=0.2, view=lambda t: t, change=None, **kw):
+    x, w = norm_arrays(dtype, weight, rows, width, norm, pre, gate, **kw)
+    if change:
+        change(x, w)
+    seed, offset = 0x1234567890ABCDEF, 1 << 33
+    op = O.NormBlock(dtype, rows, width, norm=norm, pre=pre, gate=gate, dropout=p, scale=0.7, eps=1e-5, weight_dtype=weight)
+    dev, wd = {k: view(v.cuda()) for k, v in x.items()}, {k: v.cuda() for k, v in w.items()}
+    wide = {k: v.double().numpy() for k, v in {**x, **w}.items()}
+    how = (norm, pre, gate, 0.7, 1e-5, p, seed, offset)
+    empty = lambda: view(torch.full((rows, width), float("nan"), dtype=TYPES[dtype], device="cuda"))  # noqa: E731
+    got = {"h": empty()}
+    if pre != "none":
+        got["n"] = empty()
+    op.forward(dev["y"], got["h"], got.get("n"), gate=dev.get("gate"), residual=dev.get("residual"), seed=seed,
+               offset=offset, **wd)
+    torch.cuda.synchronize()
+    for n, want in R.norm_block(wide, *how).items():
+        close(got[n], want, n)
+    out = {"y": empty()}
+    if "gate" in x:
+        out["gate"] = empty()
+    if "residual" in x:
+        out["residual"] = empty()
+    grads = {n: torch.full_like(v, float("nan")) for n, v in wd.items()}
+    op.backward(dev["y"], dev["dh"], out["y"], dn=dev.get("dn"), h=dev.get("h"), gate=dev.get("gate"),
+                dgate=out.get("gate"), dresidual=out.get("residual"), grads=grads, seed=seed, offset=offset, **wd)
+    torch.cuda.synchronize()
+    want = R.norm_block(wide, *how, back=True)
+    for n, v in {**out, **grads}.items():
+        close(v, want[n], n)
+
+
+NORMS = [  # rows, width, norm, pre, gate
+    (1, 1, "rms", "rms", "none"), (5, 3, "layer", "layer", "sigmoid"), (33, 16, "rms", "none", "silu"),
+    (70, 128, "rms", "rms", "silu"), (9, 129, "layer", "rms", "none"), (6, 512, "none", "layer", "silu"),
+    (5, 513, "rms", "rms", "sigmoid"), (3, 2048, "layer", "layer", "silu"), (4, 2049, "rms", "rms", "none"),
+    (3, 4096, "rms", "rms", "silu"), (2, 5000, "layer", "rms", "none"), (2, 8192, "rms", "layer", "sigmoid"),
+    (2, 10001, "rms", "rms", "silu"), (1, 16384, "layer", "layer", "none"), (1, 20000, "rms", "rms", "silu"),
+    (1, 32768, "layer", "layer", "silu"), (17, 40, "none", "none", "silu"),
+]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("case", NORMS)
+def test_norm_block(device, dtype, case):
+    check_norm(dtype, "f32", *case)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("kw", [dict(), dict(bias=False), dict(channel=False), dict(residual=False, p=0.0),
+                                dict(bias=False, channel=False, p=1.0)])
+def test_norm_block_parameters(device, dtype, kw):
+    """Parameters in the type of the rows, and each of them left out."""
+    check_norm(dtype, dtype, 37, 200, "layer", "rms", "silu", seed=1, **kw)
+    check_norm(dtype, dtype, 37, 1000, "rms", "layer", "none", seed=2, **kw)
+
+
+def test_norm_block_many_rows(device):
+    """More rows than workgroups: the parameters' gradients are sums over
+    workgroups, and two runs give the same bits."""
+    check_norm("f32", "f32", 5003, 24, "rms", "rms", "silu", seed=3)
+    x, w = norm_arrays("bf16", "f32", 6007, 640, "rms", "rms", "none", seed=4)
+    op = O.NormBlock("bf16", 6007, 640, dropout=0.1)
+    dev, wd = {k: v.cuda() for k, v in x.items()}, {k: v.cuda() for k, v in w.items()}
+    runs = []
+    for _ in range(2):
+        grads = {n: torch.empty_like(v) for n, v in wd.items()}
+        op.backward(dev["y"], dev["dh"], torch.empty_like(dev["y"]), dn=dev["dn"], h=dev["h"], grads=grads, seed=5, **wd)
+        torch.cuda.synchronize()
+        runs.append(grads)
+    for n in wd:
+        assert torch.equal(runs[0][n], runs[1][n]), n
+
+
+def test_norm_block_strided_rows(device):
+    """Rows an odd number of elements apart, at odd addresses."""
+    def view(t):
+        wide = torch.full((t.shape[0], t.shape[1] + 5), float("nan"), dtype=t.dtype, device="cuda")
+        part = wide[:, 3:3 + t.shape[1]]
+        part.copy_(t)
+        return part
+
+    check_norm("bf16", "f32", 11, 136, "rms", "layer", "silu", view=view, seed=6)
+    check_norm("f32", "f32", 11, 77, "layer", "rms", "none", view=view, seed=7)
+
+
+def test_norm_block_rows_of_zeros_and_constants(device):
+    """A row of zeros has eps to divide by; a layer norm centres a constant
+    row to nothing."""
+    def change(x, w):
+        x["y"][1] = 0.0
+        x["y"][2] = 5.0
+        x["h"][1] = 0.0
+
+    check_norm("f32", "f32", 4, 64, "layer", "rms", "none", change=change, seed=8)
+
+
+def test_norm_block_in_place(device):
+    """h over the residual and n over y, as an inference loop keeps them."""
+    x, w = norm_arrays("bf16", "f32", 20, 300, "rms", "rms", "none", seed=9)
+    op = O.NormBlock("bf16", 20, 300)
+    dev, wd = {k: v.cuda() for k, v in x.items()}, {k: v.cuda() for k, v in w.items()}
+    h, n = torch.empty_like(dev["y"]), torch.empty_like(dev["y"])
+    op.forward(dev["y"], h, n, residual=dev["residual"], **wd)
+    y, r = dev["y"].clone(), dev["residual"].clone()
+    op.forward(y, r, y, residual=r, **wd)
+    torch.cuda.synchronize()
+    assert torch.equal(r, h) and torch.equal(y, n)
+
+
+def test_norm_block_differences(device):
+    """As for the gated delta rule: a step of 1e-2 along unit directions; sums
+    of 1000 results of size 1 are off by 1e-7 x 30 / 2e-2 = 2e-4 and third
+    derivatives by 1e-4: 1e-2 of the norms."""
+    x, w = norm_arrays("f32", "f32", 12, 80, "layer", "rms", "silu", seed=10)
+    op = O.NormBlock("f32", 12, 80, norm="layer", pre="rms", gate="silu", dropout=0.3, scale=0.7, eps=1e-5)
+    inputs = {k: x[k] for k in ("y", "gate", "residual")}
+
+    def forward(a):
+        d = {k: v.float().cuda() for k, v in a.items()}
+        h, n = torch.empty(12, 80, device="cuda"), torch.empty(12, 80, device="cuda")
+        op.forward(d["y"], h, n, gate=d["gate"], residual=d["residual"], seed=3, **{k: d[k] for k in w})
+        torch.cuda.synchronize()
+        return h, n
+
+    h, _ = forward({**inputs, **w})
+    dev, wd = {k: v.cuda() for k, v in x.items()}, {k: v.cuda() for k, v in w.items()}
+    out = {k: torch.empty(12, 80, device="cuda") for k in inputs}
+    grads = {k: torch.empty_like(v) for k, v in wd.items()}
+    op.backward(dev["y"], dev["dh"], out["y"], dn=dev["dn"], h=h, gate=dev["gate"], dgate=out["gate"],
+                dresidual=out["residual"], grads=grads, seed=3, **wd)
+    torch.cuda.synchronize()
+    g = torch.Generator().manual_seed(2)
+    for n, grad in {**out, **grads}.items():
+        base = {k: v.double() for k, v in {**inputs, **w}.items()}
+        d = torch.randn(base[n].shape, generator=g, dtype=torch.float64)
+        d /= d.norm()
+        step = 1e-2
+
+        def loss(sign):
+            a, b = forward({**base, n: base[n] + sign * step * d})
+            return float((a.double().cpu() * x["dh"].double()).sum() + (b.double().cpu() * x["dn"].double()).sum())
+
+        want = (loss(1) - loss(-1)) / (2 * step)
+        grad = grad.double().cpu()
+        assert abs(float((grad * d).sum()) - want) <= 1e-2 * max(1.0, float(grad.norm())), n
+
+
+def test_norm_block_no_rows(device):
+    """No rows: parameters' gradients are zero, nothing else is written."""
+    op = O.NormBlock("f32", 0, 16)
+    z = torch.empty(0, 16, device="cuda")
+    grads = {n: torch.full((16,), float("nan"), device="cuda") for n in ("post_weight", "pre_weight")}
+    op.forward(z, z, z)
+    op.backward(z, z, z, dn=z, h=z, grads=grads)
+    torch.cuda.synchronize()
+    assert not grads["post_weight"].any() and not grads["pre_weight"].any()
+
+
+# ---- dropout -----------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", [(1, 1), (3, 7), (2, 8), (5, 21), (33, 64), (4, 1001), (700, 3)])
+@pytest.mark.parametrize("p", [0.0, 0.3, 1.0])
+def test_dropout(device, dtype, shape, p):
+    """The reference's mask exactly, forward and backward, with a residual."""
+    g = torch.Generator().manual_seed(4)
+    x, r = (torch.randn(shape, generator=g).to(TYPES[dtype]) for _ in range(2))
+    seed, offset = 0xFFFFFFFF00000001, 0x1FFFFFFFF
+    op = O.Dropout(dtype, *shape, p, scale=0.5)
+    xd, rd, out, dx = x.cuda(), r.cuda(), torch.empty(shape, dtype=TYPES[dtype], device="cuda"), None
+    op.forward(xd, out, seed=seed, offset=offset, residual=rd)
+    keep, up = R.kept(*shape, p, seed, offset)
+    want = r.double().numpy() + 0.5 * R.drop(x.double().numpy(), p, seed, offset)
+    torch.cuda.synchronize()
+    close(out, want, "out")
+    dx = torch.empty_like(out)
+    op.backward(xd, dx, seed=seed, offset=offset)
+    torch.cuda.synchronize()
+    assert np.array_equal(dx.double().cpu().numpy() != 0, keep & (x.double().numpy() != 0))
+    close(dx, 0.5 * R.drop(x.double().numpy(), p, seed, offset), "dx")
+
+
+def test_dropout_drops_what_is_not_a_number(device):
+    """A dropped infinity or NaN is zero; a kept one stays."""
+    x = torch.full((4, 64), float("inf"), device="cuda")
+    x[1::2] = float("nan")
+    out = torch.empty_like(x)
+    O.Dropout("f32", 4, 64, 0.5).forward(x, out, seed=9)
+    keep, _ = R.kept(4, 64, 0.5, 9, 0)
+    torch.cuda.synchronize()
+    got = out.cpu().numpy()
+    assert (got[~keep] == 0).all() and not np.isfinite(got[keep]).any()
+
+
+def test_dropout_rate_seeds_and_offsets(device):
+    """About p of many values are dropped (5 sigma), and other seeds and
+    offsets drop others: two masks agree where independent ones would."""
+    n, p = 1 << 20, 0.3
+    x = torch.ones(1024, 1024, device="cuda")
+    masks = []
+    for seed, offset in ((1, 0), (2, 0), (1, 1)):
+        out = torch.empty_like(x)
+        O.Dropout("f32", 1024, 1024, p).forward(x, out, seed=seed, offset=offset)
+        masks.append(out != 0)
+    torch.cuda.synchronize()
+    for m in masks:
+        assert abs(float(m.double().mean()) - (1 - p)) < 5 * (p * (1 - p) / n) ** 0.5
+    agree = p * p + (1 - p) * (1 - p)
+    for m in masks[1:]:
+        assert abs(float((m == masks[0]).double().mean()) - agree) < 5 * (agree * (1 - agree) / n) ** 0.5
+
+
+def test_dropout_step_on_the_device(device):
+    """A captured call draws anew on each replay through its step word, and as
+    an eager call with that offset; strides do not change a mask; in place."""
+    x = torch.randn(50, 70, device="cuda")
+    step = torch.zeros((), dtype=torch.int64, device="cuda")
+    out = torch.empty_like(x)
+    op = O.Dropout("f32", 50, 70, 0.4)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        op.forward(x, out, seed=3, offset=10, step=step, stream=stream)
+        step.add_(1)
+    for i in range(4):
+        graph.replay()
+        torch.cuda.synchronize()
+        wide = torch.zeros(50, 75, device="cuda")
+        wide[:, 2:72] = x
+        op.forward(wide[:, 2:72], wide[:, 2:72], seed=3, offset=10 + i)
+        torch.cuda.synchronize()
+        assert torch.equal(wide[:, 2:72], out), i
+        assert not wide[:, :2].any() and not wide[:, 72:].any()
+
+
+def test_the_example_learns_and_serves(device):
+    """A recurrent layer trained on graphs and operators: its loss falls, and
+    token by token it gives what whole sequences give."""
+    from cudacaml_amd.examples import delta_layer as E
+
+    z = E.Sizes()
+    live = Buffer.live_count()
+    layer = E.Layer(z)
+    x, target = E.recall_task(z, 1)
+    losses = [layer.step(x, target, seed=i) for i in range(12)]
+    assert losses[-1] < 0.75 * losses[0], losses
+    a, b = layer.predict(x), layer.evaluate(x)
+    assert np.abs(a - b).max() <= 1e-4 * np.abs(b).max()
+    layer.release()
+    del layer
+    import gc
+
+    gc.collect()
+    assert Buffer.live_count() <= live

@@ -1,0 +1,294 @@
+"""The layer operators without a device: the ABI, what the handles refuse, the
+generator against the array DSL's, and the 64-bit references' gradients
+against differences."""
+
+import ctypes
+import os
+import re
+import subprocess
+
+import numpy as np
+import pytest
+import torch
+
+import operator_reference as R
+from cudacaml_amd import _lib
+from cudacaml_amd import operators as O
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HEADER = os.path.join(ROOT, "include", "cchip_operators.h")
+
+
+def test_every_declared_operator_is_exported_and_bound():
+    text = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+    names = {m.group(1) for m in re.finditer(r"\b(cchip_[a-z_0-9]+)\s*\(", text)}
+    assert names == set(_lib.OPERATOR_SIGNATURES)
+    lib = ctypes.CDLL(_lib.LIB_PATH)
+    assert not [n for n in names if not hasattr(lib, n)]
+
+
+def test_structures_have_the_headers_sizes(tmp_path):
+    """The header is strict C99, and what Python packs is what C reads."""
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "cchip_operators.h"\n'
+                   "int main(void) { printf(\"%zu %zu %zu %zu %zu %zu %zu\\n\", sizeof(cchip_gated_delta), "
+                   "sizeof(cchip_gated_delta_io), offsetof(cchip_gated_delta_io, offsets), sizeof(cchip_dropout), "
+                   "sizeof(cchip_dropout_io), sizeof(cchip_norm_block), sizeof(cchip_norm_block_io)); return 0; }\n")
+    exe = str(tmp_path / "sizes")
+    subprocess.run(["gcc", "-std=c99", "-pedantic", "-Wall", "-Wextra", "-Werror", "-I" + os.path.join(ROOT, "include"),
+                    "-o", exe, str(src)], check=True)
+    got = [int(x) for x in subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [ctypes.sizeof(_lib.GatedDeltaDesc), O.GatedDelta._forward_io.size, 12 * 32,
+                   ctypes.sizeof(_lib.DropoutDesc), O.Dropout._io.size, ctypes.sizeof(_lib.NormBlockDesc),
+                   O.NormBlock._io.size]
+    assert O.GatedDelta._backward_io.size == O.GatedDelta._forward_io.size
+
+
+BAD_DELTA = [
+    (dict(dtype="f64"), "dtype"),
+    (dict(key_heads=3), "multiple"),
+    (dict(key_heads=0), "multiple"),
+    (dict(key_dim=129), "key_dim"),
+    (dict(key_dim=0), "key_dim"),
+    (dict(value_dim=0), "value_dim"),
+    (dict(value_dim=4097), "value_dim"),
+    (dict(batch=-1), "negative"),
+    (dict(tokens=1 << 31), "2\\^31"),
+    (dict(sequences=2), "batch of 1"),
+    (dict(sequences=0), "sequences"),
+    (dict(scale=float("nan")), "finite"),
+    (dict(batch=1 << 30, tokens=1 << 20), "launch"),
+]
+
+
+@pytest.mark.parametrize("change,why", BAD_DELTA)
+def test_gated_delta_refuses_its_shapes(change, why):
+    shape = dict(dtype="bf16", batch=2, tokens=100, key_heads=2, value_heads=4, key_dim=64, value_dim=64)
+    O.GatedDelta(**shape)
+    with pytest.raises(ValueError, match=why):
+        O.GatedDelta(**{**shape, **change})
+
+
+def test_sizes_grow_with_what_is_kept():
+    a = O.GatedDelta("bf16", 1, 640, 2, 4, 64, 64)
+    b = O.GatedDelta("bf16", 1, 1280, 2, 4, 64, 64)
+    assert b.saved_bytes() == 2 * a.saved_bytes() > 0
+    # a step needs no workspace, and packed sequences a slot each at the most
+    assert O.GatedDelta("bf16", 7, 8, 2, 4, 64, 64)._forward_bytes == 0
+    one = O.GatedDelta("bf16", 1, 64, 2, 4, 64, 64).saved_bytes()
+    assert O.GatedDelta("bf16", 1, 640, 2, 4, 64, 64, sequences=3).saved_bytes() == 13 * one
+
+
+def _delta_arrays(b=2, t=10, hk=2, hv=4, dk=16, dv=8, dtype=torch.float32):
+    z = lambda *s: torch.zeros(s, dtype=dtype)  # noqa: E731
+    return dict(q=z(b, t, hk, dk), k=z(b, t, hk, dk), v=z(b, t, hv, dv), g=z(b, t, hv), beta=z(b, t, hv), o=z(b, t, hv, dv))
+
+
+@pytest.mark.parametrize("name,bad,why", [
+    ("q", torch.zeros(2, 10, 2, 8), "shape"),
+    ("v", torch.zeros(2, 10, 4, 8, dtype=torch.float64), "dtype"),
+    ("k", torch.zeros(2, 10, 16, 2).transpose(2, 3), "contiguous"),
+    ("g", torch.zeros(2, 10, 4), "device"),
+])
+def test_gated_delta_refuses_arrays(name, bad, why):
+    """Wrong shapes, types and strides, and memory of the host, which the
+    operator must never hand to a kernel."""
+    op = O.GatedDelta("f32", 2, 10, 2, 4, 16, 8)
+    x = _delta_arrays()
+    op._device = -1 if why != "device" else 0  # as if these were the device's
+    x[name] = bad
+    with pytest.raises(ValueError, match=why):
+        op.forward(*x.values())
+
+
+def test_gated_delta_refuses_calls():
+    x = _delta_arrays()
+    op = O.GatedDelta("f32", 2, 10, 2, 4, 16, 8, states=False)
+    op._device = -1
+    grads = [x[n] for n in ("q", "k", "v", "g", "beta")]
+    with pytest.raises(ValueError, match="saved"):
+        op.backward(*grads, x["o"], None, *grads)
+    with pytest.raises(ValueError, match="offsets"):
+        op.forward(*x.values(), offsets=torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(ValueError, match="shape"):
+        op.forward(*x.values(), saved=torch.zeros(16, dtype=torch.uint8))
+    packed = O.GatedDelta("f32", 1, 10, 2, 4, 16, 8, sequences=3)
+    packed._device = -1
+    with pytest.raises(ValueError, match="offsets"):
+        packed.forward(*_delta_arrays(b=1).values())
+
+
+def _call(fn, *args):
+    rc = fn(*args)
+    return rc, _lib.lib().cchip_last_error().decode()
+
+
+def test_c_entries_refuse_before_any_device_work():
+    """Null pointers, misaligned and overlapping tensors, states that the
+    operator was made without, and a workspace that is too small."""
+    L = _lib.lib()
+    d = _lib.GatedDeltaDesc(0, 2, 100, 0, 2, 4, 16, 8, 0, 1.0)
+    F = O.GatedDelta._forward_io
+    t = lambda p=4096, h=8: (p, 100 * 4 * h, 4 * h, h)  # noqa: E731
+    good = [*t(h=16), *t(h=16), *t(), *t(h=1), *t(h=1), *t()]
+
+    def forward(words, tail=(0,) * 6, ws=None, n=0, desc=d):
+        return _call(L.cchip_gated_delta_forward, desc, F.pack(*words, *tail), ws, n, None)
+
+    rc, msg = forward(good)
+    assert rc == 1 and re.match(r"gated delta: the workspace needs \d+ bytes aligned to 16, has 0$", msg)
+    for at, value, why in [(0, 0, "no q"), (8, 4098, "v is not aligned"), (21, 0, "o overlap"), (22, 0, "o overlap"),
+                           (23, 4, "o overlap"), (6, 1 << 24, "tokens of k"), (2, -64, "tokens of q")]:
+        words = list(good)
+        words[at] = value
+        rc, msg = forward(words)
+        assert rc == 1 and why in msg, (at, msg)
+    rc, msg = forward(good, tail=(0, 4096, 0, 0, 0, 0))
+    assert rc == 1 and "without states" in msg
+    rc, msg = forward(good, tail=(4096, 0, 0, 0, 0, 0))
+    assert rc == 1 and "offsets without packed" in msg
+    rc, msg = forward(good, tail=(0, 0, 0, 0, 0, 4100))
+    assert rc == 1 and "saved is not aligned" in msg
+    rc, msg = _call(L.cchip_gated_delta_backward, d, bytes(F.size), None, 0, None)
+    assert rc == 1
+    rc, msg = _call(L.cchip_gated_delta_forward, None, None, None, 0, None)
+    assert rc == 1 and "no descriptor" in msg
+
+
+def test_nothing_to_do_is_no_error():
+    """No rows, no columns, no sequences: no launch, so no device is needed."""
+    L = _lib.lib()
+    d = _lib.GatedDeltaDesc(0, 0, 100, 0, 2, 4, 16, 8, 1, 1.0)
+    assert _call(L.cchip_gated_delta_forward, d, bytes(O.GatedDelta._forward_io.size), None, 0, None)[0] == 0
+    assert _call(L.cchip_dropout_run, _lib.DropoutDesc(0, 0, 7, 0.5, 1.0), bytes(O.Dropout._io.size), None)[0] == 0
+    n = _lib.NormBlockDesc(0, 0, 0, 8, 1, 1, 0, 1.0, 1e-6, 0.0)
+    assert _call(L.cchip_norm_block_forward, n, bytes(O.NormBlock._io.size), None)[0] == 0
+
+
+@pytest.mark.parametrize("kw,why", [
+    (dict(dtype="i32"), "dtype"), (dict(weight_dtype="f16"), "parameters"), (dict(width=0), "width"),
+    (dict(width=32769), "width"), (dict(rows=1 << 32), "rows"), (dict(norm="batch"), "unknown"),
+    (dict(gate="tanh"), "unknown"), (dict(dropout=1.5), "not in 0"), (dict(dropout=float("nan")), "not in 0"),
+    (dict(eps=-1.0), "eps"), (dict(scale=float("inf")), "finite"),
+])
+def test_norm_block_refuses_its_shapes(kw, why):
+    with pytest.raises(ValueError, match=why):
+        O.NormBlock(**{**dict(dtype="bf16", rows=4, width=8), **kw})
+
+
+def test_norm_block_refuses_calls():
+    z = lambda *s: torch.zeros(s)  # noqa: E731
+    op = O.NormBlock("f32", 4, 8)
+    op._device = -1
+    with pytest.raises(ValueError, match="if and only if"):
+        op.forward(z(4, 8), z(4, 8))
+    with pytest.raises(ValueError, match="a gate is given"):
+        op.forward(z(4, 8), z(4, 8), z(4, 8), gate=z(4, 8))
+    with pytest.raises(ValueError, match="unknown parameter"):
+        op.forward(z(4, 8), z(4, 8), z(4, 8), weight=z(8))
+    with pytest.raises(ValueError, match="rows of y are not contiguous"):
+        op.forward(z(8, 4).t(), z(4, 8), z(4, 8))
+    with pytest.raises(ValueError, match="rows of h overlap"):
+        op.forward(z(4, 8), z(1, 8).expand(4, 8), z(4, 8))
+    with pytest.raises(ValueError, match="h and dn"):
+        op.backward(z(4, 8), z(4, 8), z(4, 8))
+    plain = O.NormBlock("f32", 4, 8, norm="none", pre="none")
+    plain._device = -1
+    with pytest.raises(ValueError, match="post norm that there is not"):
+        plain.forward(z(4, 8), z(4, 8), post_weight=z(8))
+    with pytest.raises(ValueError, match="gate that there is not"):
+        plain.backward(z(4, 8), z(4, 8), z(4, 8), dgate=z(4, 8))
+
+
+def test_dropout_refuses():
+    for p in (-0.1, 1.1, float("nan")):
+        with pytest.raises(ValueError, match="not in 0"):
+            O.Dropout("f32", 4, 8, p)
+    op = O.Dropout("f32", 4, 8, 0.5)
+    op._device = -1
+    with pytest.raises(ValueError, match="no out"):
+        op.forward(torch.zeros(4, 8), None, seed=1)
+    with pytest.raises(ValueError, match="rows of out overlap"):
+        op.forward(torch.zeros(4, 8), torch.zeros(1, 8).expand(4, 8), seed=1)
+
+
+def test_arrays_lie_in_their_buffers():
+    class Memory:
+        ptr, nbytes = 4096, 64
+
+    O.Array(Memory(), "f32", (4, 4))
+    O.Array(Memory(), "bf16", (4, 4), strides=(8, 1), first=4)
+    with pytest.raises(ValueError, match="do not lie"):
+        O.Array(Memory(), "f32", (4, 5))
+    with pytest.raises(ValueError, match="do not lie"):
+        O.Array(Memory(), "f32", (2, 4), strides=(-4, 1))
+    with pytest.raises(ValueError, match="unknown dtype"):
+        O.Array(Memory(), "f8", (4, 4))
+
+
+def test_the_generator_is_the_array_languages():
+    """Words of the mask's generator against ``rng.round10`` as a graph, on the
+    interpreter: the same rounds, constants and key schedule."""
+    import oracle
+    from cudacaml_amd import dsl as D
+    from cudacaml_amd import rng
+    from cudacaml_amd.ir import I32, Graph
+
+    seed, offset, row = 0x123456789ABCDEF, 0xFEDCBA9876543210, 77
+
+    def word(i):
+        c = lambda x: D.const(I32, int(np.uint32(x).astype(np.int32)))  # noqa: E731
+        ctr = (lambda g: (g, c(row), c(offset & R.LOW), c(offset >> 32)))
+        return D.map(lambda g: rng.round10(ctr(g), (c(seed & R.LOW), c(seed >> 32)))[i], D.iota((9,)))
+
+    g = Graph.create("words", [("w%d" % i, word(i)) for i in range(4)])
+    got = dict(oracle.Interp.run(oracle.Interp.compile(g), []))
+    for group in range(9):
+        want = R.philox((group, row, offset & R.LOW, offset >> 32), (seed & R.LOW, seed >> 32))
+        assert [int(got["w%d" % i][group]) & R.LOW for i in range(4)] == want
+
+
+def _difference(f, x, direction, eps=1e-5):
+    return (f(x + eps * direction) - f(x - eps * direction)) / (2 * eps)
+
+
+def test_reference_gradients_against_differences():
+    """The references' hand-made gradients in 64 bits: a central difference of
+    step 1e-5 is off by about 1e-10 of the value for functions of these sizes,
+    and rounding by 1e-11; 1e-6 leaves room for their condition."""
+    g = np.random.default_rng(3)
+    x = dict(q=g.standard_normal((7, 2, 5)), k=g.standard_normal((7, 2, 5)) / 3, v=g.standard_normal((7, 4, 3)),
+             g=-g.random((7, 4)), beta=g.random((7, 4)), state=g.standard_normal((4, 5, 3)))
+    do, ds = g.standard_normal((7, 4, 3)), g.standard_normal((4, 5, 3))
+
+    def loss(**kw):
+        y = {**x, **kw}
+        o, s = R.delta(y["q"], y["k"], y["v"], y["g"], y["beta"], 0.3, y["state"])
+        return (o * do).sum() + (s * ds).sum()
+
+    d = R.delta(x["q"], x["k"], x["v"], x["g"], x["beta"], 0.3, x["state"], do, ds)[2]
+    for n in x:
+        r = g.standard_normal(x[n].shape)
+        want = _difference(lambda a: loss(**{n: a}), x[n], r)
+        assert abs((d["d" + n] * r).sum() - want) < 1e-6 * max(1.0, abs(want)), n
+
+    for post, pre, gate in (("rms", "layer", "silu"), ("layer", "rms", "sigmoid"), ("none", "none", "none")):
+        y = dict(y=g.standard_normal((3, 9)), residual=g.standard_normal((3, 9)), channel_scale=g.standard_normal(9))
+        if gate != "none":
+            y["gate"] = g.standard_normal((3, 9))
+        if post != "none":
+            y.update(post_weight=g.standard_normal(9), post_bias=g.standard_normal(9))
+        if pre != "none":
+            y.update(pre_weight=g.standard_normal(9), pre_bias=g.standard_normal(9))
+        dh, dn = g.standard_normal((3, 9)), g.standard_normal((3, 9))
+        how = (post, pre, gate, 0.7, 1e-3, 0.3, 5, 6)
+
+        def loss(**kw):
+            out = R.norm_block({**y, **kw}, *how)
+            return (out["h"] * dh).sum() + ((out["n"] * dn).sum() if pre != "none" else 0.0)
+
+        d = R.norm_block({**y, "h": R.norm_block(y, *how)["h"], "dh": dh, "dn": dn}, *how, back=True)
+        for n in y:
+            r = g.standard_normal(y[n].shape)
+            want = _difference(lambda a: loss(**{n: a}), y[n], r)
+            assert abs((d[n] * r).sum() - want) < 1e-6 * max(1.0, abs(want)), (post, n)
