@@ -35,7 +35,7 @@ __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int b
   typedef typename M::T T;
   typedef typename M::Saved Saved;
   constexpr int NI = M::NI, NS = M::NS;
-  constexpr int LDK = DK + 8, LDV = BV + 8;
+  constexpr int LDK = DK + 16, LDV = BV == 16 ? 24 : BV;
   constexpr int KP = 64 * LDK, EP = DK * LDV, XP = 64 * LDV;
   constexpr int TK = DK / 64, TV = BV / 16;
   typedef Record<M> R;
@@ -271,7 +271,7 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
   typedef typename M::T T;
   typedef typename M::Saved Saved;
   constexpr int NI = M::NI, NB = M::NB, NU = M::NU;
-  constexpr int LDK = DK + 8, KP = 64 * LDK, LDS = 40, SP = DK * LDS, UP = 64 * LDS, LDM = 72, MP = 64 * LDM;
+  constexpr int LDK = DK + 16, KP = 64 * LDK, LDS = 40, SP = DK * LDS, UP = 64 * LDS, LDM = 72, MP = 64 * LDM;
   constexpr int JK = DK / 32;        // 16-column tiles of a half of the keys' dimension
   constexpr bool kBoth = NB < 3;     // S and E in LDS at a time, M and B too
   typedef Record<M> R;

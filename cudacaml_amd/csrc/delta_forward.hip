@@ -22,7 +22,7 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
   typedef typename M::T T;
   typedef typename M::Saved Saved;
   constexpr int NI = M::NI, NS = M::NS, NO = M::NO, NU = M::NU;
-  constexpr int LDK = DK + 8, LDV = BV + 8;
+  constexpr int LDK = DK + 16, LDV = BV == 16 ? 24 : BV;
   constexpr int KP = 64 * LDK, SP = DK * LDV, XP = 64 * LDV;
   constexpr int TK = DK / 64, TV = BV / 16;  // 16 x 16 tiles of S a wave holds
   typedef Record<M> R;

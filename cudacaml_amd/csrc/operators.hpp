@@ -118,7 +118,9 @@ __device__ __forceinline__ Frag<N> frag_row(const bf16 *m, int plane, int ld, in
 // stored row; lane i gets column i of those 4 rows of 16. Row 4 i + r of the
 // fragment is stored column row0 + Apart i + r: with Apart 8 two fragments,
 // row0 4 apart, are 32 columns of which a lane of their products has 8 side
-// by side.
+// by side. 16 lanes read at a time: the four stored rows they touch lie in
+// banks of their own if rows are 8 to 56 banks of 64 apart (16 or 48 with
+// Apart 8).
 template <int N, int Apart = 4>
 __device__ __forceinline__ Frag<N> frag_col(const bf16 *m, int plane, int ld, int row0, int term0) {
   typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
