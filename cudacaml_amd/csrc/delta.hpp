@@ -246,23 +246,23 @@ __device__ __forceinline__ Frag<N> frag_v(const bf16 *m, int plane, int ld, int 
   return frag_col<N, 4 * TV>(m, plane, ld, 4 * j, term0);
 }
 
-// A lane's 4 TV elements of token t of a tensor, zero past the chunk or the
-// head, and their store.
+// A lane's 4 TV elements of token t of a tensor, and their store. Held as
+// words: elements taken apart on the way round a loop would be waited for
+// there.
 template <typename T, int TV>
 struct RawV {
-  T x[4 * TV];
+  uint32_t w[TV * sizeof(T)];
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, w[i]);
+    else if constexpr (std::is_same<T, bf16>::value) return i & 1 ? high_bf16(w[i / 2]) : low_bf16(w[i / 2]);
+    else return float(__builtin_bit_cast(f16, uint16_t(w[i / 2] >> (i & 1 ? 16 : 0))));
+  }
 };
 
 template <bool Fast, typename T, int TV>
 __device__ __forceinline__ RawV<T, TV> load_v(const Heads &x, const Chunk &c, int head, int t, int d, int dim) {
-  union {
-    RawV<T, TV> v;
-    Raw4<T> r4;
-    Raw8<T> r8;
-  } u;
-  if constexpr (TV == 2) u.r8 = load_head8<Fast, T>(x, c, head, t, d, dim);
-  else u.r4 = load_head4<Fast, T>(x, c, head, t, d, dim);
-  return u.v;
+  if constexpr (TV == 2) return __builtin_bit_cast(RawV<T, TV>, load_head8<Fast, T>(x, c, head, t, d, dim));
+  else return __builtin_bit_cast(RawV<T, TV>, load_head4<Fast, T>(x, c, head, t, d, dim));
 }
 
 template <bool Fast, typename T, int TV>
@@ -271,12 +271,12 @@ __device__ __forceinline__ void store_v(const Heads &x, const Chunk &c, int head
   char *base = x.p + (c.row * x.b + c.first * x.t + head * x.h) * int64_t(sizeof(T));
   char *to = base + (uint32_t(t) * uint32_t(x.t) + uint32_t(d)) * uint32_t(sizeof(T));
   union {
-    RawV<T, TV> r;
-    u32x4 w[sizeof(RawV<T, TV>) >= 16 ? sizeof(RawV<T, TV>) / 16 : 1];
+    T r[4 * TV];
+    u32x4 w[sizeof(T) * TV >= 4 ? sizeof(T) * TV / 4 : 1];
     uint64_t half;
   } u;
 #pragma unroll
-  for (int i = 0; i < 4 * TV; i++) u.r.x[i] = T(v[i / 4][i % 4]);
+  for (int i = 0; i < 4 * TV; i++) u.r[i] = T(v[i / 4][i % 4]);
   if (Fast) {
     if constexpr (sizeof(u.r) >= 16) {
 #pragma unroll
@@ -287,7 +287,7 @@ __device__ __forceinline__ void store_v(const Heads &x, const Chunk &c, int head
   } else {
 #pragma unroll
     for (int i = 0; i < 4 * TV; i++)
-      if (d + i < dim) reinterpret_cast<T *>(to)[i] = u.r.x[i];
+      if (d + i < dim) reinterpret_cast<T *>(to)[i] = u.r[i];
   }
 }
 
@@ -297,12 +297,12 @@ __device__ __forceinline__ void store_v(const Heads &x, const Chunk &c, int head
 template <typename T, int TV>
 __device__ __forceinline__ void put_block(char *rows, int row, int y, const f32x4 (&v)[TV]) {
   union {
-    RawV<T, TV> r;
-    u32x4 w[sizeof(RawV<T, TV>) >= 16 ? sizeof(RawV<T, TV>) / 16 : 1];
+    T r[4 * TV];
+    u32x4 w[sizeof(T) * TV >= 4 ? sizeof(T) * TV / 4 : 1];
     uint64_t half;
   } u;
 #pragma unroll
-  for (int i = 0; i < 4 * TV; i++) u.r.x[i] = T(v[i / 4][i % 4]);
+  for (int i = 0; i < 4 * TV; i++) u.r[i] = T(v[i / 4][i % 4]);
   char *to = rows + uint32_t(row * 32 + y) * uint32_t(sizeof(T));
   if constexpr (sizeof(u.r) >= 16) {
 #pragma unroll
@@ -314,19 +314,21 @@ __device__ __forceinline__ void put_block(char *rows, int row, int y, const f32x
 
 template <typename T, int TV>
 __device__ __forceinline__ RawV<T, TV> load_block(const char *rows, int row, int y) {
-  union {
-    RawV<T, TV> r;
-    u32x4 w[sizeof(RawV<T, TV>) >= 16 ? sizeof(RawV<T, TV>) / 16 : 1];
-    uint64_t half;
-  } u;
   const char *from = rows + uint32_t(row * 32 + y) * uint32_t(sizeof(T));
-  if constexpr (sizeof(u.r) >= 16) {
+  RawV<T, TV> r;
+  if constexpr (sizeof(r) >= 16) {
 #pragma unroll
-    for (int i = 0; i < int(sizeof(u.r) / 16); i++) u.w[i] = reinterpret_cast<const u32x4 *>(from)[i];
+    for (int i = 0; i < int(sizeof(r) / 16); i++) {
+      const u32x4 x = reinterpret_cast<const u32x4 *>(from)[i];
+#pragma unroll
+      for (int j = 0; j < 4; j++) r.w[4 * i + j] = x[j];
+    }
   } else {
-    u.half = *reinterpret_cast<const uint64_t *>(from);
+    const uint2 x = *reinterpret_cast<const uint2 *>(from);
+    r.w[0] = x.x;
+    r.w[1] = x.y;
   }
-  return u.r;
+  return r;
 }
 
 template <typename T>

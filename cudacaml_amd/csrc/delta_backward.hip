@@ -148,7 +148,7 @@ __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int b
 #pragma unroll
     for (int i = 0; i < TK; i++)
 #pragma unroll
-      for (int j = 0; j < 4 * TV; j++) dot += float(rs[i].x[j]) * e[i][j / 4][j % 4];
+      for (int j = 0; j < 4 * TV; j++) dot += rs[i][j] * e[i][j / 4][j % 4];
     dot = sum64(dot);
     if (l == 0) {
       float *dots = a.dots + (slot_head * (a.dvp / 16) + dv0 / 16) * 4;
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int b
 #pragma unroll
     for (int i = 0; i < TK; i++) put_block<Saved, TV>(to, x0 + 16 * i, dv0 % 32 + y0, e[i]);
 
-    f32x4 ke[TV] = {}, du[TV] = {};
+    Levels<NS> ke[TV], po[TV];
     {
       // operands first, products after: one wait for LDS, not one a product
       Frag<NI> fk[DK / 32], fo[2][TV];
@@ -180,22 +180,22 @@ __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int b
 #pragma unroll
       for (int d = 0; d < DK / 32; d++)
 #pragma unroll
-        for (int j = 0; j < TV; j++) ke[j] = mma(ke[j], fe[d][j], fk[d]);
+        for (int j = 0; j < TV; j++) ke[j].add(fe[d][j], fk[d]);
 #pragma unroll
       for (int b = 0; b < 2; b++)
         if (b == 1 || w < 2)
 #pragma unroll
-          for (int j = 0; j < TV; j++) du[j] = mma(du[j], fo[b][j], pt[b]);
+          for (int j = 0; j < TV; j++) po[j].add(fo[b][j], pt[b]);
     }
     fetch_p(next);
 #pragma unroll
     for (int j = 0; j < TV; j++) {
-      du[j] = a.scale * du[j] + last * ke[j];
-      put_four<NS>(xs + t * LDV + y0 + 4 * j, XP, du[j]);
+      put_four<NS>(xs + t * LDV + y0 + 4 * j, XP, a.scale * po[j].sum() + last * ke[j].sum());
     }
     __syncthreads();
-    f32x4 y[TV] = {};
+    f32x4 y[TV];
     {
+      Levels<NS> sum[TV];
       Frag<NS> fx[2][TV];
 #pragma unroll
       for (int b = 0; b < 2; b++)
@@ -206,7 +206,9 @@ __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int b
       for (int b = 0; b < 2; b++)
         if (b == 1 || w < 2)
 #pragma unroll
-          for (int j = 0; j < TV; j++) y[j] = mma(y[j], fx[b][j], tt[b]);
+          for (int j = 0; j < TV; j++) sum[j].add(fx[b][j], tt[b]);
+#pragma unroll
+      for (int j = 0; j < TV; j++) y[j] = sum[j].sum();
     }
     put_block<float, TV>(reinterpret_cast<char *>(a.ys + (slot_head * a.dvp + dv0 / 32 * 32) * kChunk), t, dv0 % 32 + y0, y);
 #pragma unroll

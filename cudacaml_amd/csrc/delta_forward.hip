@@ -26,7 +26,10 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
   constexpr int KP = 64 * LDK, SP = DK * LDV, XP = 64 * LDV;
   constexpr int TK = DK / 64, TV = BV / 16;  // 16 x 16 tiles of S a wave holds
   typedef Record<M> R;
-  __shared__ __align__(16) bf16 ks[NI * KP], ss[NS * SP], xs[NS * XP], us[NU * XP], gs[NS * XP];
+  // two sets of keys where LDS has room: the next chunk's are written while
+  // slower waves still read this one's
+  constexpr int kSets = NI == 1 ? 2 : 1;
+  __shared__ __align__(16) bf16 keys[kSets * NI * KP], ss[NS * SP], xs[NS * XP], us[NU * XP], gs[NS * XP];
 
   // heads 8 apart share a chiplet's L2: a head's column blocks, which read
   // the same q, k, T and P, are 8 workgroups apart
@@ -108,18 +111,29 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
     fetch_t(0);
     fetch_p(0);
   }
-  for (int ci = 0; ci < chunks; ci++) {
-    const Chunk c = chunk(ci);
-    const int next = ci + 1 < chunks ? ci + 1 : ci;
+  auto put_keys = [&](int i) {
+    const Chunk c = chunk(i);
+    bf16 *const to = keys + i % kSets * NI * KP;
 #pragma unroll
     for (int j = 0; j < DK / 32; j++) {
       const int at = tid + 256 * j, kt = at / (DK / 8), d = at % (DK / 8) * 8;
-      put_frag<NI>(ks + kt * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rk[j], c, kt, d, a.dk)));
+      put_frag<NI>(to + kt * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rk[j], c, kt, d, a.dk)));
     }
+  };
+  auto put_state = [&]() {
 #pragma unroll
     for (int i = 0; i < TK; i++)
 #pragma unroll
       for (int j = 0; j < TV; j++) put_four<NS>(ss + (x0 + 16 * i) * LDV + y0 + 4 * j, SP, s[i][j]);
+  };
+  if (chunks > 0) {
+    put_keys(0);
+    put_state();
+  }
+  for (int ci = 0; ci < chunks; ci++) {
+    const Chunk c = chunk(ci);
+    const int next = ci + 1 < chunks ? ci + 1 : ci;
+    const bf16 *const ks = keys + ci % kSets * NI * KP;
     __syncthreads();
     fetch_k(next);
     if (Back) {
@@ -128,8 +142,9 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
       for (int i = 0; i < TK; i++) put_block<Saved, TV>(to, x0 + 16 * i, dv0 % 32 + y0, s[i]);
     }
 
-    f32x4 kS[TV] = {}, o[TV] = {};
+    f32x4 kS[TV], o[TV] = {};
     {
+      Levels<NS> sum[TV];
       // operands first, products after: one wait for LDS, not one a product
       Frag<NI> fk[DK / 32];
       Frag<NS> fs[DK / 32][TV];
@@ -145,25 +160,28 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
         const Frag<NI> fq = frag_of<NI>(keep_head8<Fast>(rq[d], c, t, 32 * d + 8 * quad, a.dk));
 #pragma unroll
         for (int j = 0; j < TV; j++) {
-          kS[j] = mma(kS[j], fs[d][j], fk[d]);
+          sum[j].add(fs[d][j], fk[d]);
           o[j] = mma(o[j], first_planes<NO>(fs[d][j]), fq);
         }
       }
+#pragma unroll
+      for (int j = 0; j < TV; j++) kS[j] = sum[j].sum();
     }
 #pragma unroll
     for (int j = 0; j < TV; j++) {
       f32x4 x;
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const float v = t < c.len && dv0 + y0 + 4 * j + r < a.dv ? float(rv.x[4 * j + r]) : 0.0f;
+        const float v = t < c.len && dv0 + y0 + 4 * j + r < a.dv ? rv[4 * j + r] : 0.0f;
         x[r] = beta * (v - gam * kS[j][r]);
       }
       put_four<NS>(xs + t * LDV + y0 + 4 * j, XP, x);
     }
     fetch_qv(next);
     __syncthreads();
-    f32x4 u[TV] = {};
+    f32x4 u[TV];
     {
+      Levels<NS> sum[TV];
       Frag<NS> fx[2][TV];
 #pragma unroll
       for (int b = 0; b < 2; b++)
@@ -174,7 +192,9 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
       for (int b = 0; b < 2; b++)
         if (b == 0 || w >= 2)
 #pragma unroll
-          for (int j = 0; j < TV; j++) u[j] = mma(u[j], fx[b][j], ft[b]);
+          for (int j = 0; j < TV; j++) sum[j].add(fx[b][j], ft[b]);
+#pragma unroll
+      for (int j = 0; j < TV; j++) u[j] = sum[j].sum();
     }
     fetch_t(next);
 #pragma unroll
@@ -208,21 +228,33 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
 #pragma unroll
       for (int j = 0; j < TV; j++) o[j] *= gam;
 #pragma unroll
-      for (int b = 0; b < 2; b++) {
+      for (int b = 0; b < 2; b++)
 #pragma unroll
         for (int i = 0; i < TK; i++)
 #pragma unroll
           for (int j = 0; j < TV; j++) s[i][j] = mma(s[i][j], fg[b][j], fk[b][i]);
+      // the next chunk waits for S only: O comes after it
+      if (kSets == 2 && ci + 1 < chunks) {
+        put_state();
+        put_keys(ci + 1);
+      }
+#pragma unroll
+      for (int b = 0; b < 2; b++)
         if (b == 0 || w >= 2)
 #pragma unroll
           for (int j = 0; j < TV; j++) o[j] = mma(o[j], fu[b][j], fp[b]);
-      }
     }
     fetch_p(next);
 #pragma unroll
     for (int j = 0; j < TV; j++) o[j] *= a.scale;
     store_v<Fast, T, TV>(a.o, c, h, t, dv0 + y0, a.dv, o);
-    __syncthreads();
+    if (kSets == 1) {
+      __syncthreads();
+      if (ci + 1 < chunks) {
+        put_state();
+        put_keys(ci + 1);
+      }
+    }
   }
   if (a.state_out)
 #pragma unroll

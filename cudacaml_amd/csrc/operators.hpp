@@ -47,12 +47,14 @@ __device__ __forceinline__ Raw8<T> load8(const T *p, int valid) {
   return r;
 }
 
-// Two values rounded to bf16 in one instruction (the compiler makes one of
-// each), and those as f32 again.
+// Two values rounded to bf16, and those as f32 again. By conversions of the
+// language and not an asm instruction: what a product has just written must
+// not be read for some cycles, and only instructions that the compiler knows
+// are kept from it.
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  uint32_t u;
-  asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(u) : "v"(lo), "v"(hi));
-  return u;
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), bf16x2));
 }
 __device__ __forceinline__ float low_bf16(uint32_t u) { return __builtin_bit_cast(float, u << 16); }
 __device__ __forceinline__ float high_bf16(uint32_t u) { return __builtin_bit_cast(float, u & 0xFFFF0000u); }
@@ -167,6 +169,30 @@ __device__ __forceinline__ void put_four(bf16 *at, int plane, f32x4 x) {
     x -= f32x4{low_bf16(a), high_bf16(a), low_bf16(b), high_bf16(b)};
   }
 }
+
+// A sum of products that no product waits long for: the planes' levels i + j
+// (see mma) each have a sum of their own, added up at the end, small first.
+template <int L>
+struct Levels {
+  f32x4 s[L] = {};
+  template <int NA, int NB>
+  __device__ __forceinline__ void add(const Frag<NA> &a, const Frag<NB> &b) {
+    static_assert((NA > NB ? NA : NB) <= L, "a level has no sum");
+#pragma unroll
+    for (int k = (NA > NB ? NA : NB) - 1; k >= 0; k--)
+#pragma unroll
+      for (int i = 0; i < NA; i++) {
+        const int j = k - i;
+        if (j >= 0 && j < NB) s[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[j], s[k], 0, 0, 0);
+      }
+  }
+  __device__ __forceinline__ f32x4 sum() const {
+    f32x4 x = s[L - 1];
+#pragma unroll
+    for (int k = L - 2; k >= 0; k--) x += s[k];
+    return x;
+  }
+};
 
 template <int N>
 __device__ __forceinline__ void put_frag(bf16 *at, int plane, const Frag<N> &f) {
