@@ -265,50 +265,57 @@ __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int b
 // A workgroup of eight waves a chunk and key head, its value heads one after
 // another (so dQ and dK of a shared head are summed in registers, in an order
 // that is always the same). Products are taken transposed, as in the forward
-// pass: wave w has tokens 16 (w % 4) .. of each and half w / 4 of the rest,
-// and a lane one token. S, E and U pass through LDS 32 value columns at a
-// time, the next 32 being read while the products of these are made.
+// pass: wave w has tokens 16 (w % 4) .. of each and part w / 4 of the rest,
+// and a lane one token. S, E, U, Y and dO pass through LDS 32 value columns
+// at a time, the next 32 being read while the products of these are made.
+// Four parts and 16 waves would hide more but do not fit in 128 registers
+// (790 us where this takes 500, for 8192 chunks of 128-element heads).
 template <typename M, int DK, bool Fast>
 __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
   typedef typename M::T T;
   typedef typename M::Saved Saved;
-  constexpr int NI = M::NI, NB = M::NB, NU = M::NU;
+  constexpr int NI = M::NI, NB = M::NB, NU = M::NU, P = 2, kThreads = 256 * P;
   constexpr int LDK = DK + 16, KP = 64 * LDK, LDS = 40, SP = DK * LDS, UP = 64 * LDS, LDM = 72, MP = 64 * LDM;
-  constexpr int JK = DK / 32;        // 16-column tiles of a half of the keys' dimension
-  constexpr bool kBoth = NB < 3;     // S and E in LDS at a time, M and B too
+  constexpr int JK = DK / 16 / P, JS = 4 / P;  // 16-wide tiles of a part: of a key, of the tokens
+  constexpr bool kAll = NB < 3;               // everything in LDS at a time; else E after S, and Y and dO not
   typedef Record<M> R;
-  constexpr int kSlices = (kBoth ? 2 : 1) * NB * SP + NU * UP, kMs = (kBoth ? 2 : 1) * NB * MP;
+  constexpr int kSlices = (kAll ? 2 : 1) * NB * SP + NU * UP + (kAll ? (NU + NI) * UP : 0), kMs = (kAll ? 2 : 1) * NB * MP;
   __shared__ __align__(16) bf16 ks[NI * KP], qs[NI * KP], slice[kSlices > kMs ? kSlices : kMs];
   __shared__ double cs[64];
   __shared__ __align__(16) float down[4][64];
-  __shared__ float row_c[2][64], row_b[2][64], total[8];
-  bf16 *const us = slice, *const ss = slice + NU * UP, *const es = kBoth ? ss + NB * SP : ss;
-  bf16 *const ms = slice, *const bs = kBoth ? slice + NB * MP : slice;
+  __shared__ float row_c[P][64], row_b[P][64], row_y[64], total[4 * P];
+  bf16 *const us = slice, *const ss = slice + NU * UP, *const es = kAll ? ss + NB * SP : ss;
+  bf16 *const yl = es + NB * SP, *const ol = yl + NU * UP;  // Y and dO if kAll
+  bf16 *const ms = slice, *const bs = kAll ? slice + NB * MP : slice;
 
   const int64_t slot = blockIdx.x / a.hk;
   const int hk = int(blockIdx.x - slot * a.hk), per = a.hv / a.hk;
   const Chunk c = chunk_of(a, slot);
   if (c.len == 0) return;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, quad = l >> 4, col = l & 15;
-  const int wr = w & 3, half = w >> 2;
-  const int t = 16 * wr + col;                  // this lane's token
-  const int x0 = 16 * JK * half + 4 * quad;     // its part of a key: x0 + 16 j + r
-  const int s0 = 32 * half + 4 * quad;          // and of the tokens before it: s0 + 16 j + r
+  const int wr = w & 3, part = w >> 2;
+  const int t = 16 * wr + col;                    // this lane's token
+  const int x0 = 16 * JK * part + 4 * quad;       // its part of a key: x0 + 16 j + r
+  const int s0 = 16 * JS * part + 4 * quad;       // and of the tokens before it: s0 + 16 j + r
 
   {
-    Raw8<T> rk[DK / 64], rq[DK / 64];
+    constexpr int kRows = 64 * (DK / 8) / kThreads > 0 ? 64 * (DK / 8) / kThreads : 1;
+    const bool has = tid < 64 * (DK / 8);
+    Raw8<T> rk[kRows], rq[kRows];
 #pragma unroll
-    for (int j = 0; j < DK / 64; j++) {
-      const int at = tid + 512 * j;
-      rk[j] = load_head8<Fast, T>(a.k, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk);
-      rq[j] = load_head8<Fast, T>(a.q, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk);
-    }
+    for (int j = 0; j < kRows; j++)
+      if (has) {
+        const int at = tid + kThreads * j;
+        rk[j] = load_head8<Fast, T>(a.k, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk);
+        rq[j] = load_head8<Fast, T>(a.q, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk);
+      }
 #pragma unroll
-    for (int j = 0; j < DK / 64; j++) {
-      const int at = tid + 512 * j, kt = at / (DK / 8), d = at % (DK / 8) * 8;
-      put_frag<NI>(ks + kt * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rk[j], c, kt, d, a.dk)));
-      put_frag<NI>(qs + kt * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rq[j], c, kt, d, a.dk)));
-    }
+    for (int j = 0; j < kRows; j++)
+      if (has) {
+        const int at = tid + kThreads * j, kt = at / (DK / 8), d = at % (DK / 8) * 8;
+        put_frag<NI>(ks + kt * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rk[j], c, kt, d, a.dk)));
+        put_frag<NI>(qs + kt * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rq[j], c, kt, d, a.dk)));
+      }
   }
   // four elements of this lane's row of K or Q as their planes add up
   auto value4 = [&](const bf16 *m, int d) {
@@ -321,9 +328,10 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
     }
     return x;
   };
-  // this thread's pieces of a slice: of S and E (row sx), and of U (row ux)
-  const int sx = tid / 4, sv = tid % 4 * 8, ux = (tid & 255) / 4;
-  const bool has_s = sx < DK, has_u = tid < 256;
+  // this thread's pieces of a slice, 8 columns from sv on: row sx of S and E,
+  // and row ux of U and dO or, in the second half of the waves, of Y and v
+  const int sv = tid % 4 * 8, sx = tid / 4, ux = (tid & 255) / 4;
+  const bool has_s = sx < DK, second = w >= 4;
 
   f32x4 dq[JK] = {}, dk[JK] = {};
   for (int h = hk * per; h < (hk + 1) * per; h++) {
@@ -342,10 +350,15 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
         rs = load_block8<Saved>(S, uint32_t(v0 * DK + sx * 32 + sv));
         re = load_block8<Saved>(E, uint32_t(v0 * DK + sx * 32 + sv));
       }
-      if (has_u) ru = load_block8<float>(U, uint32_t(v0 * 64 + ux * 32 + sv));
-      ry = load_block8<float>(Y, uint32_t(v0 * 64 + t * 32 + 8 * quad));
-      ro = load_head8<Fast, T>(a.d_o, c, h, t, v0 + 8 * quad, a.dv);
-      rv = load_head8<Fast, T>(a.v, c, h, t, v0 + 8 * quad, a.dv);
+      if (kAll) {
+        ru = load_block8<float>(second ? Y : U, uint32_t(v0 * 64 + ux * 32 + sv));
+        ro = load_head8<Fast, T>(second ? a.v : a.d_o, c, h, ux, v0 + sv, a.dv);
+      } else {
+        if (!second) ru = load_block8<float>(U, uint32_t(v0 * 64 + ux * 32 + sv));
+        ry = load_block8<float>(Y, uint32_t(v0 * 64 + t * 32 + 8 * quad));
+        ro = load_head8<Fast, T>(a.d_o, c, h, t, v0 + 8 * quad, a.dv);
+        rv = load_head8<Fast, T>(a.v, c, h, t, v0 + 8 * quad, a.dv);
+      }
     };
     fetch(0);
     double run = 0.0;  // the running sum of g, as delta_chunk makes it
@@ -361,51 +374,76 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
     __syncthreads();  // the head before is done with LDS
     if (w == 0) cs[l] = run;
 
-    f32x4 os[JK] = {}, ys[JK] = {}, ue[JK] = {}, ou[2] = {}, yu[2] = {};
-    float yv = 0.0f, se = 0.0f;  // yv: this lane's columns
-    for (int i = tid; i < a.dvp / 4; i += 512) se += a.dots[slot_head * (a.dvp / 4) + i];
+    f32x4 os[JK] = {}, ys[JK] = {}, ue[JK] = {}, ou[JS] = {}, yu[JS] = {};
+    float yv = 0.0f, se = 0.0f;  // yv: of row ux (kAll) or t, this thread's columns
+    for (int i = tid; i < a.dvp / 4; i += kThreads) se += a.dots[slot_head * (a.dvp / 4) + i];
     for (int v0 = 0; v0 < a.dvp; v0 += 32) {
-      const Frag<NI> fo = frag_of<NI>(keep_head8<Fast>(ro, c, t, v0 + 8 * quad, a.dv));
-      const Frag<NU> fy = frag_of<NU>(ry);
-      const Raw8<T> v = keep_head8<Fast>(rv, c, t, v0 + 8 * quad, a.dv);
-#pragma unroll
-      for (int i = 0; i < 8; i++) yv += ry.x[i] * float(v.x[i]);
-      if (has_u) put_frag<NU>(us + ux * LDS + sv, UP, frag_of<NU>(ru));
-      Raw8<Saved> late = re;
+      Frag<NI> fo;
+      Frag<NU> fy;
+      const Raw8<Saved> late = re;
       if (has_s) {
         put_frag<NB>(ss + sx * LDS + sv, SP, frag_of<NB>(rs));
-        if (kBoth) put_frag<NB>(es + sx * LDS + sv, SP, frag_of<NB>(re));
+        if (kAll) put_frag<NB>(es + sx * LDS + sv, SP, frag_of<NB>(re));
+      }
+      if (kAll) {
+        put_frag<NU>((second ? yl : us) + ux * LDS + sv, UP, frag_of<NU>(ru));
+        const Raw8<T> x = keep_head8<Fast>(ro, c, ux, v0 + sv, a.dv);
+        if (second) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) yv += ru.x[i] * float(x.x[i]);
+        } else {
+          put_frag<NI>(ol + ux * LDS + sv, UP, frag_of<NI>(x));
+        }
+      } else {
+        if (!second) put_frag<NU>(us + ux * LDS + sv, UP, frag_of<NU>(ru));
+        fo = frag_of<NI>(keep_head8<Fast>(ro, c, t, v0 + 8 * quad, a.dv));
+        fy = frag_of<NU>(ry);
+        const Raw8<T> v = keep_head8<Fast>(rv, c, t, v0 + 8 * quad, a.dv);
+#pragma unroll
+        for (int i = 0; i < 8; i++) yv += ry.x[i] * float(v.x[i]);
       }
       __syncthreads();
       if (v0 + 32 < a.dvp) fetch(v0 + 32);
+      if (kAll) {
+        fo = frag_row<NI>(ol, UP, LDS, 16 * wr, 0);
+        fy = frag_row<NU>(yl, UP, LDS, 16 * wr, 0);
+      }
       const Frag<NU> fu = frag_row<NU>(us, UP, LDS, 16 * wr, 0);
 #pragma unroll
       for (int j = 0; j < JK; j++) {
-        const int x = 16 * (JK * half + j);
+        const int x = 16 * (JK * part + j);
         const Frag<NB> fs = frag_row<NB>(ss, SP, LDS, x, 0);
         os[j] = mma(os[j], fs, fo);
         ys[j] = mma(ys[j], fs, fy);
-        if (kBoth) ue[j] = mma(ue[j], frag_row<NB>(es, SP, LDS, x, 0), fu);
+        if (kAll) ue[j] = mma(ue[j], frag_row<NB>(es, SP, LDS, x, 0), fu);
       }
 #pragma unroll
-      for (int j = 0; j < 2; j++)
-        if (2 * half + j <= wr) {
-          const Frag<NU> f = frag_row<NU>(us, UP, LDS, 16 * (2 * half + j), 0);
+      for (int j = 0; j < JS; j++)
+        if (JS * part + j <= wr) {
+          const Frag<NU> f = frag_row<NU>(us, UP, LDS, 16 * (JS * part + j), 0);
           ou[j] = mma(ou[j], f, fo);
           yu[j] = mma(yu[j], f, fy);
         }
       __syncthreads();
-      if (!kBoth) {
+      if (!kAll) {
         if (has_s) put_frag<NB>(es + sx * LDS + sv, SP, frag_of<NB>(late));
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < JK; j++) ue[j] = mma(ue[j], frag_row<NB>(es, SP, LDS, 16 * (JK * half + j), 0), fu);
+        for (int j = 0; j < JK; j++) ue[j] = mma(ue[j], frag_row<NB>(es, SP, LDS, 16 * (JK * part + j), 0), fu);
         __syncthreads();
       }
     }
+    if (kAll) {
+      yv += __shfl_xor(yv, 1, 64);
+      yv += __shfl_xor(yv, 2, 64);
+      if (second && tid % 4 == 0) row_y[ux] = yv;
+    } else {
+      yv = sum_rows(yv);
+      if (part == 0 && quad == 0) row_y[t] = yv;
+    }
 
     const float gam = dec[t], last = dec[64 + t], beta = dec[128 + t];
-    float dc = 0.0f, db = half == 0 ? yv : 0.0f, end = 0.0f;
+    float dc = 0.0f, db = 0.0f, end = 0.0f;
 #pragma unroll
     for (int j = 0; j < JK; j++) {
       const f32x4 kv = value4(ks, x0 + 16 * j), qv = value4(qs, x0 + 16 * j);
@@ -419,21 +457,21 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
         end += kv[r] * u[r];
       }
     }
-    f32x4 kk[2] = {}, qk[2] = {};
+    f32x4 kk[JS] = {}, qk[JS] = {};
 #pragma unroll
     for (int d = 0; d < DK; d += 32) {
       const Frag<NI> fk = frag_row<NI>(ks, KP, LDK, 16 * wr, d), fq = frag_row<NI>(qs, KP, LDK, 16 * wr, d);
 #pragma unroll
-      for (int j = 0; j < 2; j++)
-        if (2 * half + j <= wr) {
-          const Frag<NI> fs = frag_row<NI>(ks, KP, LDK, 16 * (2 * half + j), d);
+      for (int j = 0; j < JS; j++)
+        if (JS * part + j <= wr) {
+          const Frag<NI> fs = frag_row<NI>(ks, KP, LDK, 16 * (JS * part + j), d);
           kk[j] = mma(kk[j], fs, fk);
           qk[j] = mma(qk[j], fs, fq);
         }
     }
-    f32x4 b[2];
+    f32x4 b[JS];
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
+    for (int j = 0; j < JS; j++) {
       f32x4 m, across;
 #pragma unroll
       for (int r = 0; r < 4; r++) {
@@ -448,20 +486,27 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
       }
       if (col == 0) *reinterpret_cast<f32x4 *>(&down[wr][s0 + 16 * j]) = across;
       put_four<NB>(ms + t * LDM + s0 + 16 * j, MP, m);
-      if (kBoth) put_four<NB>(bs + t * LDM + s0 + 16 * j, MP, b[j]);
+      if (kAll) put_four<NB>(bs + t * LDM + s0 + 16 * j, MP, b[j]);
     }
     dc = sum_rows(dc);
     db = sum_rows(db);
     if (quad == 0) {
-      row_c[half][t] = dc;
-      row_b[half][t] = db;
+      row_c[part][t] = dc;
+      row_b[part][t] = db;
     }
     end = sum64(end + se * dec[63]);
     if (l == 0) total[w] = end;
     __syncthreads();
     if (w == 0) {
-      float x = row_c[0][l] + row_c[1][l] - (down[0][l] + down[1][l] + down[2][l] + down[3][l]);
-      if (l == 63) x += ((total[0] + total[1]) + (total[2] + total[3])) + ((total[4] + total[5]) + (total[6] + total[7]));
+      float x = -(down[0][l] + down[1][l] + down[2][l] + down[3][l]), y = row_y[l], all = 0.0f;
+#pragma unroll
+      for (int p = 0; p < P; p++) {
+        x += row_c[p][l];
+        y += row_b[p][l];
+      }
+#pragma unroll
+      for (int i = 0; i < 4 * P; i++) all += total[i];
+      if (l == 63) x += all;
 #pragma unroll
       for (int d = 1; d < 64; d *= 2) {
         const float up = __shfl_down(x, d, 64);
@@ -469,7 +514,7 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
       }
       if (l < c.len) {
         *out_at<T>(a.gg, c.row, c.first + l, h) = T(x);
-        *out_at<T>(a.gbeta, c.row, c.first + l, h) = T(row_b[0][l] + row_b[1][l]);
+        *out_at<T>(a.gbeta, c.row, c.first + l, h) = T(y);
       }
     }
 #pragma unroll
@@ -477,18 +522,18 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
       if (t0 == 0 || wr >= 2) {  // M ends at the diagonal
         const Frag<NB> f = frag_row<NB>(ms, MP, LDM, 16 * wr, t0);
 #pragma unroll
-        for (int j = 0; j < JK; j++) dq[j] = mma(dq[j], frag_col<NI>(ks, KP, LDK, 16 * (JK * half + j), t0), f);
+        for (int j = 0; j < JK; j++) dq[j] = mma(dq[j], frag_col<NI>(ks, KP, LDK, 16 * (JK * part + j), t0), f);
       }
       if (t0 != 0 || wr < 2) {
         const Frag<NB> f = frag_col<NB>(ms, MP, LDM, 16 * wr, t0);
 #pragma unroll
-        for (int j = 0; j < JK; j++) dk[j] = mma(dk[j], frag_col<NI>(qs, KP, LDK, 16 * (JK * half + j), t0), f);
+        for (int j = 0; j < JK; j++) dk[j] = mma(dk[j], frag_col<NI>(qs, KP, LDK, 16 * (JK * part + j), t0), f);
       }
     }
-    if (!kBoth) {
+    if (!kAll) {
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < 2; j++) put_four<NB>(bs + t * LDM + s0 + 16 * j, MP, b[j]);
+      for (int j = 0; j < JS; j++) put_four<NB>(bs + t * LDM + s0 + 16 * j, MP, b[j]);
       __syncthreads();
     }
 #pragma unroll
@@ -496,7 +541,7 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
       const Frag<NB> fb = frag_row<NB>(bs, MP, LDM, 16 * wr, t0), ft = frag_col<NB>(bs, MP, LDM, 16 * wr, t0);
 #pragma unroll
       for (int j = 0; j < JK; j++) {
-        const Frag<NI> fk = frag_col<NI>(ks, KP, LDK, 16 * (JK * half + j), t0);
+        const Frag<NI> fk = frag_col<NI>(ks, KP, LDK, 16 * (JK * part + j), t0);
         if (t0 == 0 || wr >= 2) dk[j] = mma(dk[j], fk, fb);
         if (t0 != 0 || wr < 2) dk[j] = mma(dk[j], fk, ft);
       }
