@@ -15,7 +15,7 @@ constexpr int64_t kStepTokens = 8;
 
 struct Layout {
   int64_t slots, slot_heads;
-  size_t record, record_back, states, us, dots;  // bytes, all slots and heads
+  size_t record, record_back, states, us, scales, dots;  // bytes, all slots and heads
 };
 
 void check_op(const cchip_gated_delta *op) {
@@ -52,7 +52,8 @@ Layout layout_of(const cchip_gated_delta &op) {
     p.record_back = size_t(p.slot_heads) * record_bytes<M>(true);
     p.states = size_t(p.slot_heads) * padded_key_dim(op.key_dim) * padded_value_dim(op) * sizeof(typename M::Saved);
     p.dots = size_t(p.slot_heads) * (padded_value_dim(op) / 16) * 4 * sizeof(float);
-    p.us = size_t(p.slot_heads) * kChunk * padded_value_dim(op) * sizeof(float);
+    p.us = size_t(p.slot_heads) * kChunk * padded_value_dim(op) * sizeof(typename M::Kept);
+    p.scales = sizeof(typename M::Kept) == 4 ? 0 : size_t(p.slot_heads) * kChunk * (padded_value_dim(op) / 16) * sizeof(float);
   });
   return p;
 }
@@ -122,7 +123,8 @@ void check_workspace(const void *workspace, size_t have, size_t need) {
 void lay_out(DeltaArgs &a, const Layout &p, char *saved) {
   a.records = saved;
   a.states = saved + p.record_back;
-  a.us = reinterpret_cast<float *>(a.states + p.states);
+  a.us = a.states + p.states;
+  a.u_scales = reinterpret_cast<float *>(a.us + p.us);
 }
 
 }  // namespace
@@ -134,8 +136,8 @@ int cchip_gated_delta_sizes(const cchip_gated_delta *op, size_t *forward, size_t
     check_op(op);
     const Layout p = layout_of(*op);
     if (forward) *forward = steps(*op, false) ? 0 : p.record;
-    if (backward) *backward = p.states + p.us + p.dots;
-    if (saved) *saved = p.record_back + p.states + p.us;
+    if (backward) *backward = p.states + p.us + p.scales + p.dots;
+    if (saved) *saved = p.record_back + p.states + p.us + p.scales;
   });
 }
 
@@ -170,10 +172,11 @@ int cchip_gated_delta_backward(const cchip_gated_delta *op, const cchip_gated_de
     a.slots = p.slots;
     if (a.sequences == 0) return;
     lay_out(a, p, static_cast<char *>(io->saved));
-    check_workspace(workspace, workspace_bytes, p.states + p.us + p.dots);
+    check_workspace(workspace, workspace_bytes, p.states + p.us + p.scales + p.dots);
     a.grads = static_cast<char *>(workspace);
-    a.ys = reinterpret_cast<float *>(a.grads + p.states);
-    a.dots = reinterpret_cast<float *>(a.grads + p.states + p.us);
+    a.ys = a.grads + p.states;
+    a.y_scales = reinterpret_cast<float *>(a.ys + p.us);
+    a.dots = reinterpret_cast<float *>(a.ys + p.us + p.scales);
     delta_backward_launch(*op, a, (hipStream_t)stream);
   });
 }

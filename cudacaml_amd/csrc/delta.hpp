@@ -46,9 +46,10 @@ struct DeltaArgs {
   // of each (slot, value head), in blocks of 32 value columns (put_block);
   // what pads a head is zero
   char *states;   // saved S before the chunk, DK rows; null if there is no backward pass
-  float *us;      // saved U, 64 rows
+  char *us;       // saved U, 64 rows
   char *grads;    // backward: dS after the chunk
-  float *ys;      // backward: Y
+  char *ys;       // backward: Y
+  float *u_scales, *y_scales;  // of U and Y in f16: [16 columns][64]
   float *dots;    // backward: sums that make <S, dS>, four for each 16 value columns
   int64_t tokens, sequences;  // sequences: of the packed batch, or its rows
   int64_t slots;
@@ -61,23 +62,26 @@ struct DeltaArgs {
 // Element type, then the planes: NI of an input, NS of what makes a state
 // (S, T, X and U in their products), NO of S and P where they make only an
 // output, NU of U and Y where they make only outputs. Saved is the type that
-// S and dS are kept in for the backward pass, read back in NB planes.
+// S and dS are kept in for the backward pass, read back in NB planes, and
+// Kept that of U and Y: f16 with a power of two for each token and 16
+// columns (11 bits, which two planes hold) or f32.
 //
 // A product loses the most precise operand's worth of the other's rounding:
 // 2^-9 of a value in one plane of bf16, 2^-17 in two. bf16 results are
 // rounded to 2^-9 themselves, and each of theirs comes through one operand
 // in one plane and no more (2.3e-3 in the 2-norm where their own rounding
 // alone is 1.7e-3); states in f32 take three planes.
-template <typename T_, int NI_, int NS_, int NO_, int NU_, typename Saved_, int NB_>
+template <typename T_, int NI_, int NS_, int NO_, int NU_, typename Saved_, int NB_, typename Kept_>
 struct Mode {
   typedef T_ T;
   typedef Saved_ Saved;
+  typedef Kept_ Kept;
   static constexpr int NI = NI_, NS = NS_, NO = NO_, NU = NU_, NB = NB_;
 };
-typedef Mode<bf16, 1, 2, 1, 2, bf16, 1> ModeBf16;   // bf16 in and out
-typedef Mode<bf16, 1, 3, 1, 2, bf16, 1> ModeBf16S;  // with f32 states in or out
-typedef Mode<f16, 2, 3, 2, 2, float, 2> ModeF16;
-typedef Mode<float, 3, 3, 3, 3, float, 3> ModeF32;
+typedef Mode<bf16, 1, 2, 1, 2, bf16, 1, f16> ModeBf16;   // bf16 in and out
+typedef Mode<bf16, 1, 3, 1, 2, bf16, 1, f16> ModeBf16S;  // with f32 states in or out
+typedef Mode<f16, 2, 3, 2, 2, float, 2, float> ModeF16;
+typedef Mode<float, 3, 3, 3, 3, float, 3, float> ModeF32;
 
 // What a chunk and value head have that depends on no state: matrices as
 // fragments of 16 rows and 32 terms, [row block][term block][lane][8], in
@@ -329,6 +333,28 @@ __device__ __forceinline__ RawV<T, TV> load_block(const char *rows, int row, int
     r.w[1] = x.y;
   }
   return r;
+}
+
+// A token's share of U or Y as it is kept. Every lane of the token takes part.
+template <typename Kept, int TV>
+__device__ __forceinline__ void keep_block(char *all, float *scales, int64_t slot_head, int dvp, int v0, int t, int quad, int y,
+                                           const f32x4 (&v)[TV]) {
+  char *rows = all + (slot_head * dvp + v0 / 32 * 32) * (kChunk * int64_t(sizeof(Kept)));
+  if constexpr (sizeof(Kept) == 4) {
+    put_block<float, TV>(rows, t, v0 % 32 + y, v);
+  } else {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4 * TV; i++) m = fmaxf(m, fabsf(v[i / 4][i % 4]));
+    const uint32_t e = __builtin_bit_cast(uint32_t, max_rows(m)) >> 23;
+    const uint32_t x = e < 1 ? 127 : e > 253 ? 253 : e;  // the largest becomes 1 .. 2 (zeros stay, the last binade 2 .. 8)
+    const float down = __builtin_bit_cast(float, (254 - x) << 23);
+    f32x4 s[TV];
+#pragma unroll
+    for (int j = 0; j < TV; j++) s[j] = v[j] * down;
+    put_block<f16, TV>(rows, t, v0 % 32 + y, s);
+    if (quad < TV) scales[(slot_head * dvp + v0) * (kChunk / 16) + quad * kChunk + t] = __builtin_bit_cast(float, x << 23);
+  }
 }
 
 template <typename T>

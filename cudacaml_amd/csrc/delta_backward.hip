@@ -210,7 +210,7 @@ __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int b
 #pragma unroll
       for (int j = 0; j < TV; j++) y[j] = sum[j].sum();
     }
-    put_block<float, TV>(reinterpret_cast<char *>(a.ys + (slot_head * a.dvp + dv0 / 32 * 32) * kChunk), t, dv0 % 32 + y0, y);
+    keep_block<typename M::Kept, TV>(a.ys, a.y_scales, slot_head, a.dvp, dv0, t, quad, y0, y);
 #pragma unroll
     for (int j = 0; j < TV; j++) {
       put_four<NS>(zs + t * LDV + y0 + 4 * j, EP, (-gam * beta) * y[j]);
@@ -274,6 +274,7 @@ template <typename M, int DK, bool Fast>
 __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
   typedef typename M::T T;
   typedef typename M::Saved Saved;
+  typedef typename M::Kept Kept;
   constexpr int NI = M::NI, NB = M::NB, NU = M::NU, P = 2, kThreads = 256 * P;
   constexpr int LDK = DK + 16, KP = 64 * LDK, LDS = 40, SP = DK * LDS, UP = 64 * LDS, LDM = 72, MP = 64 * LDM;
   constexpr int JK = DK / 16 / P, JS = 4 / P;  // 16-wide tiles of a part: of a key, of the tokens
@@ -339,22 +340,26 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
     const float *dec = reinterpret_cast<const float *>(a.records + slot_head * R::bytes(true) + R::Decay);
     const char *S = a.states + slot_head * DK * a.dvp * int64_t(sizeof(Saved));
     const char *E = a.grads + slot_head * DK * a.dvp * int64_t(sizeof(Saved));
-    const char *U = reinterpret_cast<const char *>(a.us + slot_head * kChunk * a.dvp);
-    const char *Y = reinterpret_cast<const char *>(a.ys + slot_head * kChunk * a.dvp);
+    const char *U = a.us + slot_head * kChunk * a.dvp * int64_t(sizeof(Kept));
+    const char *Y = a.ys + slot_head * kChunk * a.dvp * int64_t(sizeof(Kept));
+    const float *u_scales = a.u_scales + slot_head * (kChunk / 16) * a.dvp, *y_scales = a.y_scales + slot_head * (kChunk / 16) * a.dvp;
 
     Raw8<Saved> rs, re;
-    Raw8<float> ru, ry;
+    Raw8<Kept> ru;
+    Raw8<float> ry;
     Raw8<T> ro, rv;
+    float scale = 1.0f;
     auto fetch = [&](int v0) {
       if (has_s) {
         rs = load_block8<Saved>(S, uint32_t(v0 * DK + sx * 32 + sv));
         re = load_block8<Saved>(E, uint32_t(v0 * DK + sx * 32 + sv));
       }
       if (kAll) {
-        ru = load_block8<float>(second ? Y : U, uint32_t(v0 * 64 + ux * 32 + sv));
+        ru = load_block8<Kept>(second ? Y : U, uint32_t(v0 * 64 + ux * 32 + sv));
+        if (sizeof(Kept) < 4) scale = (second ? y_scales : u_scales)[(v0 + sv) / 16 * kChunk + ux];
         ro = load_head8<Fast, T>(second ? a.v : a.d_o, c, h, ux, v0 + sv, a.dv);
       } else {
-        if (!second) ru = load_block8<float>(U, uint32_t(v0 * 64 + ux * 32 + sv));
+        if (!second) ru = load_block8<Kept>(U, uint32_t(v0 * 64 + ux * 32 + sv));
         ry = load_block8<float>(Y, uint32_t(v0 * 64 + t * 32 + 8 * quad));
         ro = load_head8<Fast, T>(a.d_o, c, h, t, v0 + 8 * quad, a.dv);
         rv = load_head8<Fast, T>(a.v, c, h, t, v0 + 8 * quad, a.dv);
@@ -386,11 +391,14 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
         if (kAll) put_frag<NB>(es + sx * LDS + sv, SP, frag_of<NB>(re));
       }
       if (kAll) {
-        put_frag<NU>((second ? yl : us) + ux * LDS + sv, UP, frag_of<NU>(ru));
+        Raw8<float> u;
+#pragma unroll
+        for (int i = 0; i < 8; i++) u.x[i] = sizeof(Kept) < 4 ? scale * float(ru.x[i]) : float(ru.x[i]);
+        put_frag<NU>((second ? yl : us) + ux * LDS + sv, UP, frag_of<NU>(u));
         const Raw8<T> x = keep_head8<Fast>(ro, c, ux, v0 + sv, a.dv);
         if (second) {
 #pragma unroll
-          for (int i = 0; i < 8; i++) yv += ru.x[i] * float(x.x[i]);
+          for (int i = 0; i < 8; i++) yv += u.x[i] * float(x.x[i]);
         } else {
           put_frag<NI>(ol + ux * LDS + sv, UP, frag_of<NI>(x));
         }

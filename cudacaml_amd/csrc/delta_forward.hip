@@ -202,10 +202,7 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
       put_four<NU>(us + t * LDV + y0 + 4 * j, XP, u[j]);
       put_four<NS>(gs + t * LDV + y0 + 4 * j, XP, last * u[j]);
     }
-    if (Back) {
-      char *to = reinterpret_cast<char *>(a.us + (((sq.slot + ci) * a.hv + h) * a.dvp + dv0 / 32 * 32) * kChunk);
-      put_block<float, TV>(to, t, dv0 % 32 + y0, u);
-    }
+    if (Back) keep_block<typename M::Kept, TV>(a.us, a.u_scales, (sq.slot + ci) * a.hv + h, a.dvp, dv0, t, quad, y0, u);
     __syncthreads();
     {
       Frag<NS> fg[2][TV];

@@ -225,6 +225,18 @@ __device__ __forceinline__ float sum_rows(float x) {
   return __builtin_bit_cast(float, b0) + __builtin_bit_cast(float, b1);
 }
 
+// The largest of the four rows' x of a column.
+__device__ __forceinline__ float max_rows(float x) {
+  uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  x = fmaxf(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1));
+  u = __builtin_bit_cast(uint32_t, x);
+  const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return fmaxf(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+}
+
 __device__ __forceinline__ float sum64(float x) { return sum_rows(sum16(x)); }
 
 // Philox-4x32-10 (Salmon, Moraes, Dror and Shaw, SC'11), the generator of
