@@ -147,20 +147,22 @@ __device__ __forceinline__ T *out_at(const Heads &x, int64_t row, int64_t token,
 }
 
 // Eight elements of token `t` of a chunk from element `d` on, of a head of
-// `dim` (a multiple of 8 if Fast): always loads, of an element that exists
-// where the one asked for does not, so that nothing branches and loads stay
-// in flight; keep_head8 makes what is past the chunk or the head zero once
-// they are needed.
+// `dim` (Fast: whole pieces of 16 bytes): always loads, of an element that
+// exists where the one asked for does not, so that nothing branches and loads
+// stay in flight; keep_head8 makes what is past the chunk or the head zero
+// once they are needed.
 template <bool Fast, typename T>
 __device__ __forceinline__ Raw8<T> load_head8(const Heads &x, const Chunk &c, int head, int t, int d, int dim) {
+  constexpr int E = 16 / sizeof(T);
   const char *base = x.p + (c.row * x.b + c.first * x.t + head * x.h) * int64_t(sizeof(T));
   const uint32_t row = uint32_t(t < c.len ? t : c.len - 1) * uint32_t(x.t);
   Raw8<T> r;
   if (Fast) {
-    const u32x4_any *s = reinterpret_cast<const u32x4_any *>(base + (row + uint32_t(d < dim ? d : dim - 8)) * uint32_t(sizeof(T)));
-    u32x4 *to = reinterpret_cast<u32x4 *>(&r);
 #pragma unroll
-    for (int i = 0; i < int(sizeof(T) * 8 / 16); i++) to[i] = s[i];
+    for (int i = 0; i < 8 / E; i++) {
+      const int at = d + i * E < dim ? d + i * E : dim - E;
+      reinterpret_cast<u32x4 *>(&r)[i] = *reinterpret_cast<const u32x4_any *>(base + (row + uint32_t(at)) * uint32_t(sizeof(T)));
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; i++)
@@ -171,21 +173,16 @@ __device__ __forceinline__ Raw8<T> load_head8(const Heads &x, const Chunk &c, in
 
 template <bool Fast, typename T>
 __device__ __forceinline__ Raw8<T> keep_head8(Raw8<T> r, const Chunk &c, int t, int d, int dim) {
+  constexpr int E = 16 / sizeof(T);
   if (Fast) {
-    const bool live = t < c.len && d < dim;
     u32x4 *x = reinterpret_cast<u32x4 *>(&r);
 #pragma unroll
-    for (int i = 0; i < int(sizeof(T) * 8 / 16); i++) x[i] = live ? x[i] : u32x4{};
+    for (int i = 0; i < 8 / E; i++) x[i] = t < c.len && d + i * E < dim ? x[i] : u32x4{};
   } else {
 #pragma unroll
     for (int i = 0; i < 8; i++) r.x[i] = t < c.len && d + i < dim ? r.x[i] : T(0.0f);
   }
   return r;
-}
-
-template <bool Fast, typename T>
-__device__ __forceinline__ Raw8<T> head8(const Heads &x, const Chunk &c, int head, int t, int d, int dim) {
-  return keep_head8<Fast>(load_head8<Fast, T>(x, c, head, t, d, dim), c, t, d, dim);
 }
 
 // Four in the same way, as f32, and the store of four.
@@ -284,7 +281,8 @@ __device__ __forceinline__ void store_v(const Heads &x, const Chunk &c, int head
   if (Fast) {
     if constexpr (sizeof(u.r) >= 16) {
 #pragma unroll
-      for (int i = 0; i < int(sizeof(u.r) / 16); i++) reinterpret_cast<u32x4_any *>(to)[i] = u.w[i];
+      for (int i = 0; i < int(sizeof(u.r) / 16); i++)
+        if (d + i * int(16 / sizeof(T)) < dim) reinterpret_cast<u32x4_any *>(to)[i] = u.w[i];
     } else {
       *reinterpret_cast<u32x2_any *>(to) = __builtin_bit_cast(u32x2_any, u.half);
     }
@@ -387,8 +385,11 @@ void delta_step_launch(const cchip_gated_delta &op, const DeltaArgs &a, hipStrea
 
 inline int padded_key_dim(int dk) { return dk <= 64 ? 64 : 128; }
 
-// Whether heads are read 8 elements at a time.
-inline bool fast(const DeltaArgs &a) { return a.dk % 8 == 0 && a.dv % 8 == 0; }
+// Whether heads are whole pieces of 16 bytes (and, of f32, keys whole eights).
+template <typename T>
+bool fast(const DeltaArgs &a) {
+  return a.dk % 8 == 0 && a.dv % int(16 / sizeof(T)) == 0;
+}
 
 template <typename F>
 void with_bool(bool x, F &&f) {

@@ -574,7 +574,7 @@ void delta_backward_launch(const cchip_gated_delta &op, const DeltaArgs &a, hipS
     typedef decltype(m) M;
     constexpr int DK = decltype(dk)::value, BV = decltype(bv)::value;
     const int blocks = a.dvp / BV;  // what pads a head is written too
-    with_bool(fast(a), [&](auto f) {
+    with_bool(fast<typename M::T>(a), [&](auto f) {
       constexpr bool F = decltype(f)::value;
       hipLaunchKernelGGL((delta_reverse<M, DK, BV, F>), dim3(unsigned((lanes + 7) / 8 * 8 * blocks)), dim3(256), 0, stream,
                          a, blocks);

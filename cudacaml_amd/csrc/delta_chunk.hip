@@ -180,7 +180,7 @@ void delta_chunk_launch(const cchip_gated_delta &op, const DeltaArgs &a, bool ba
   with_mode(op, [&](auto m) {
     typedef decltype(m) M;
     with_bool(back, [&](auto b) {
-      with_bool(fast(a), [&](auto f) {
+      with_bool(fast<typename M::T>(a), [&](auto f) {
         constexpr bool B = decltype(b)::value, F = decltype(f)::value;
         auto *k = a.dk <= 64 ? delta_chunk<M, 64, B, F> : delta_chunk<M, 128, B, F>;
         hipLaunchKernelGGL(k, dim3(unsigned(grid)), dim3(256), 0, stream, a);

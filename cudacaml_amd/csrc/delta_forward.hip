@@ -274,7 +274,7 @@ void delta_forward_launch(const cchip_gated_delta &op, const DeltaArgs &a, bool 
     constexpr int DK = decltype(dk)::value, BV = decltype(bv)::value;
     const int blocks = back ? a.dvp / BV : (a.dv + BV - 1) / BV;  // saved columns that pad a head are written too
     with_bool(back, [&](auto b) {
-      with_bool(fast(a), [&](auto f) {
+      with_bool(fast<typename M::T>(a), [&](auto f) {
         hipLaunchKernelGGL((delta_forward<M, DK, BV, decltype(b)::value, decltype(f)::value>),
                            dim3(unsigned((lanes + 7) / 8 * 8 * blocks)), dim3(256), 0, stream, a, blocks);
       });
