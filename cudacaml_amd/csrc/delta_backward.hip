@@ -30,7 +30,7 @@ namespace {
 // head, E in registers, each chunk's rows asked for while the one after it is
 // computed. <S, E> is summed here, where E still is f32: of the two in bf16
 // it would be off by both their roundings.
-template <typename M, int DK, int BV, bool Fast>
+template <typename M, int DK, int BV, int A>
 __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int blocks) {
   typedef typename M::T T;
   typedef typename M::Saved Saved;
@@ -82,14 +82,14 @@ __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int b
 #pragma unroll
     for (int j = 0; j < DK / 32; j++) {
       const int at = tid + 256 * j;
-      rk[j] = load_head8<Fast, T>(a.k, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk);
-      rq[j] = load_head8<Fast, T>(a.q, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk);
+      rk[j] = load_head8<A, T>(a.k, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk);
+      rq[j] = load_head8<A, T>(a.q, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk);
     }
     const char *from = a.states + (((sq.slot + i) * a.hv + h) * a.dvp + dv0 / 32 * 32) * DK * int64_t(sizeof(Saved));
 #pragma unroll
     for (int j = 0; j < TK; j++) rs[j] = load_block<Saved, TV>(from, x0 + 16 * j, dv0 % 32 + y0);
     if (has_o) {
-      ro = load_head8<Fast, T>(a.d_o, c, h, ot, dv0 + od, a.dv);
+      ro = load_head8<A, T>(a.d_o, c, h, ot, dv0 + od, a.dv);
       og = reinterpret_cast<const float *>(record(i) + R::Decay)[ot];
     }
   };
@@ -128,11 +128,11 @@ __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int b
 #pragma unroll
     for (int j = 0; j < DK / 32; j++) {
       const int at = tid + 256 * j, kt = at / (DK / 8), d = at % (DK / 8) * 8;
-      put_frag<NI>(ks + kt * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rk[j], c, kt, d, a.dk)));
-      put_frag<NI>(qs + kt * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rq[j], c, kt, d, a.dk)));
+      put_frag<NI>(ks + kt * LDK + d, KP, frag_of<NI>(keep_head8<A>(rk[j], c, kt, d, a.dk)));
+      put_frag<NI>(qs + kt * LDK + d, KP, frag_of<NI>(keep_head8<A>(rq[j], c, kt, d, a.dk)));
     }
     if (has_o) {
-      const Raw8<T> raw = keep_head8<Fast>(ro, c, ot, dv0 + od, a.dv);
+      const Raw8<T> raw = keep_head8<A>(ro, c, ot, dv0 + od, a.dv);
       put_frag<NI>(os + ot * LDV + od, XP, frag_of<NI>(raw));
       const float f = a.scale * og;
       Raw8<float> up;
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int b
       put_four<NS>(zs + t * LDV + y0 + 4 * j, EP, (-gam * beta) * y[j]);
       y[j] *= beta;
     }
-    store_v<Fast, T, TV>(a.gv, c, h, t, dv0 + y0, a.dv, y);
+    store_v<A, T, TV>(a.gv, c, h, t, dv0 + y0, a.dv, y);
     fetch_t(next);
     __syncthreads();
 #pragma unroll
@@ -270,7 +270,7 @@ __global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int b
 // at a time, the next 32 being read while the products of these are made.
 // Four parts and 16 waves would hide more but do not fit in 128 registers
 // (790 us where this takes 500, for 8192 chunks of 128-element heads).
-template <typename M, int DK, bool Fast>
+template <typename M, int DK, int A>
 __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
   typedef typename M::T T;
   typedef typename M::Saved Saved;
@@ -307,15 +307,15 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
     for (int j = 0; j < kRows; j++)
       if (has) {
         const int at = tid + kThreads * j;
-        rk[j] = load_head8<Fast, T>(a.k, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk);
-        rq[j] = load_head8<Fast, T>(a.q, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk);
+        rk[j] = load_head8<A, T>(a.k, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk);
+        rq[j] = load_head8<A, T>(a.q, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk);
       }
 #pragma unroll
     for (int j = 0; j < kRows; j++)
       if (has) {
         const int at = tid + kThreads * j, kt = at / (DK / 8), d = at % (DK / 8) * 8;
-        put_frag<NI>(ks + kt * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rk[j], c, kt, d, a.dk)));
-        put_frag<NI>(qs + kt * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rq[j], c, kt, d, a.dk)));
+        put_frag<NI>(ks + kt * LDK + d, KP, frag_of<NI>(keep_head8<A>(rk[j], c, kt, d, a.dk)));
+        put_frag<NI>(qs + kt * LDK + d, KP, frag_of<NI>(keep_head8<A>(rq[j], c, kt, d, a.dk)));
       }
   }
   // four elements of this lane's row of K or Q as their planes add up
@@ -357,12 +357,12 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
       if (kAll) {
         ru = load_block8<Kept>(second ? Y : U, uint32_t(v0 * 64 + ux * 32 + sv));
         if (sizeof(Kept) < 4) scale = (second ? y_scales : u_scales)[(v0 + sv) / 16 * kChunk + ux];
-        ro = load_head8<Fast, T>(second ? a.v : a.d_o, c, h, ux, v0 + sv, a.dv);
+        ro = load_head8<A, T>(second ? a.v : a.d_o, c, h, ux, v0 + sv, a.dv);
       } else {
         if (!second) ru = load_block8<Kept>(U, uint32_t(v0 * 64 + ux * 32 + sv));
         ry = load_block8<float>(Y, uint32_t(v0 * 64 + t * 32 + 8 * quad));
-        ro = load_head8<Fast, T>(a.d_o, c, h, t, v0 + 8 * quad, a.dv);
-        rv = load_head8<Fast, T>(a.v, c, h, t, v0 + 8 * quad, a.dv);
+        ro = load_head8<A, T>(a.d_o, c, h, t, v0 + 8 * quad, a.dv);
+        rv = load_head8<A, T>(a.v, c, h, t, v0 + 8 * quad, a.dv);
       }
     };
     fetch(0);
@@ -395,7 +395,7 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; i++) u.x[i] = sizeof(Kept) < 4 ? scale * float(ru.x[i]) : float(ru.x[i]);
         put_frag<NU>((second ? yl : us) + ux * LDS + sv, UP, frag_of<NU>(u));
-        const Raw8<T> x = keep_head8<Fast>(ro, c, ux, v0 + sv, a.dv);
+        const Raw8<T> x = keep_head8<A>(ro, c, ux, v0 + sv, a.dv);
         if (second) {
 #pragma unroll
           for (int i = 0; i < 8; i++) yv += u.x[i] * float(x.x[i]);
@@ -404,9 +404,9 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
         }
       } else {
         if (!second) put_frag<NU>(us + ux * LDS + sv, UP, frag_of<NU>(ru));
-        fo = frag_of<NI>(keep_head8<Fast>(ro, c, t, v0 + 8 * quad, a.dv));
+        fo = frag_of<NI>(keep_head8<A>(ro, c, t, v0 + 8 * quad, a.dv));
         fy = frag_of<NU>(ry);
-        const Raw8<T> v = keep_head8<Fast>(rv, c, t, v0 + 8 * quad, a.dv);
+        const Raw8<T> v = keep_head8<A>(rv, c, t, v0 + 8 * quad, a.dv);
 #pragma unroll
         for (int i = 0; i < 8; i++) yv += ry.x[i] * float(v.x[i]);
       }
@@ -557,8 +557,8 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
   }
 #pragma unroll
   for (int j = 0; j < JK; j++) {
-    store_head4<Fast, T>(a.gq, c, hk, t, x0 + 16 * j, a.dk, dq[j]);
-    store_head4<Fast, T>(a.gk, c, hk, t, x0 + 16 * j, a.dk, dk[j]);
+    store_head4<A, T>(a.gq, c, hk, t, x0 + 16 * j, a.dk, dq[j]);
+    store_head4<A, T>(a.gk, c, hk, t, x0 + 16 * j, a.dk, dk[j]);
   }
 }
 
@@ -574,8 +574,8 @@ void delta_backward_launch(const cchip_gated_delta &op, const DeltaArgs &a, hipS
     typedef decltype(m) M;
     constexpr int DK = decltype(dk)::value, BV = decltype(bv)::value;
     const int blocks = a.dvp / BV;  // what pads a head is written too
-    with_bool(fast<typename M::T>(a), [&](auto f) {
-      constexpr bool F = decltype(f)::value;
+    with_access<typename M::T>(a, [&](auto f) {
+      constexpr int F = decltype(f)::value;
       hipLaunchKernelGGL((delta_reverse<M, DK, BV, F>), dim3(unsigned((lanes + 7) / 8 * 8 * blocks)), dim3(256), 0, stream,
                          a, blocks);
       if (a.slots) hipLaunchKernelGGL((delta_gradients<M, DK, F>), dim3(unsigned(a.slots * a.hk)), dim3(512), 0, stream, a);

@@ -49,7 +49,7 @@ __device__ __forceinline__ void put_block(float *to, const f32x4 &c, float sign)
 // lower triangle T_ij = -T_ii sum_m A_im T_mj, a diagonal of blocks at a
 // time. All of it is f32: entries of T add up 64 products deep, and every
 // state after the chunk carries what they lose.
-template <typename M, int DK, bool Back, bool Fast>
+template <typename M, int DK, bool Back, int A>
 __global__ __launch_bounds__(256) void delta_chunk(const DeltaArgs a) {
   typedef typename M::T T;
   constexpr int NI = M::NI, LD = DK + 8, KPlane = 64 * LD;
@@ -91,13 +91,13 @@ __global__ __launch_bounds__(256) void delta_chunk(const DeltaArgs a) {
 #pragma unroll
   for (int j = 0; j < DK / 32; j++) {
     const int i = tid + 256 * j;
-    rk[j] = load_head8<Fast, T>(a.k, c, hk, i / (DK / 8), i % (DK / 8) * 8, a.dk);
-    rq[j] = load_head8<Fast, T>(a.q, c, hk, 16 * w + col, 32 * j + quad * 8, a.dk);
+    rk[j] = load_head8<A, T>(a.k, c, hk, i / (DK / 8), i % (DK / 8) * 8, a.dk);
+    rq[j] = load_head8<A, T>(a.q, c, hk, 16 * w + col, 32 * j + quad * 8, a.dk);
   }
 #pragma unroll
   for (int j = 0; j < DK / 32; j++) {
     const int i = tid + 256 * j, t = i / (DK / 8), d = i % (DK / 8) * 8;
-    put_frag<NI>(ks + t * LD + d, KPlane, frag_of<NI>(keep_head8<Fast>(rk[j], c, t, d, a.dk)));
+    put_frag<NI>(ks + t * LD + d, KPlane, frag_of<NI>(keep_head8<A>(rk[j], c, t, d, a.dk)));
   }
   for (int i = tid; i < 64 * kPad; i += 256) tm[i] = 0.0f;
   __syncthreads();
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(256) void delta_chunk(const DeltaArgs a) {
 #pragma unroll
   for (int d = 0; d < DK; d += 32) {
     const Frag<NI> fk = frag_row<NI>(ks, KPlane, LD, 16 * w, d);
-    const Frag<NI> fq = frag_of<NI>(keep_head8<Fast>(rq[d / 32], c, 16 * w + col, d + quad * 8, a.dk));
+    const Frag<NI> fq = frag_of<NI>(keep_head8<A>(rq[d / 32], c, 16 * w + col, d + quad * 8, a.dk));
 #pragma unroll
     for (int j = 0; j < 4; j++)
       if (j <= w) {
@@ -180,8 +180,9 @@ void delta_chunk_launch(const cchip_gated_delta &op, const DeltaArgs &a, bool ba
   with_mode(op, [&](auto m) {
     typedef decltype(m) M;
     with_bool(back, [&](auto b) {
-      with_bool(fast<typename M::T>(a), [&](auto f) {
-        constexpr bool B = decltype(b)::value, F = decltype(f)::value;
+      with_access<typename M::T>(a, [&](auto f) {
+        constexpr bool B = decltype(b)::value;
+        constexpr int F = decltype(f)::value;
         auto *k = a.dk <= 64 ? delta_chunk<M, 64, B, F> : delta_chunk<M, 128, B, F>;
         hipLaunchKernelGGL(k, dim3(unsigned(grid)), dim3(256), 0, stream, a);
       });

@@ -17,7 +17,7 @@ namespace {
 // asked for again for the next chunk as soon as this one has used it, so that
 // memory answers while the chain of products, three waits for the other
 // waves long, goes on.
-template <typename M, int DK, int BV, bool Back, bool Fast>
+template <typename M, int DK, int BV, bool Back, int A>
 __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int blocks) {
   typedef typename M::T T;
   typedef typename M::Saved Saved;
@@ -73,14 +73,14 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
 #pragma unroll
     for (int j = 0; j < DK / 32; j++) {
       const int at = tid + 256 * j;
-      rk[j] = load_head8<Fast, T>(a.k, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk);
+      rk[j] = load_head8<A, T>(a.k, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk);
     }
   };
   auto fetch_qv = [&](int i) {
     const Chunk c = chunk(i);
 #pragma unroll
-    for (int j = 0; j < DK / 32; j++) rq[j] = load_head8<Fast, T>(a.q, c, hk, t, 32 * j + 8 * quad, a.dk);
-    rv = load_v<Fast, T, TV>(a.v, c, h, t, dv0 + y0, a.dv);
+    for (int j = 0; j < DK / 32; j++) rq[j] = load_head8<A, T>(a.q, c, hk, t, 32 * j + 8 * quad, a.dk);
+    rv = load_v<A, T, TV>(a.v, c, h, t, dv0 + y0, a.dv);
   };
   auto fragment = [&](const char *from, int b) {  // rows 16 w .. of a matrix of the record, terms 32 b ..
     return *reinterpret_cast<const bf16x8 *>(from + uint32_t((w * 2 + b) * 1024 + l * 16));
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
 #pragma unroll
     for (int j = 0; j < DK / 32; j++) {
       const int at = tid + 256 * j, kt = at / (DK / 8), d = at % (DK / 8) * 8;
-      put_frag<NI>(to + kt * LDK + d, KP, frag_of<NI>(keep_head8<Fast>(rk[j], c, kt, d, a.dk)));
+      put_frag<NI>(to + kt * LDK + d, KP, frag_of<NI>(keep_head8<A>(rk[j], c, kt, d, a.dk)));
     }
   };
   auto put_state = [&]() {
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int d = 0; d < DK / 32; d++) {
-        const Frag<NI> fq = frag_of<NI>(keep_head8<Fast>(rq[d], c, t, 32 * d + 8 * quad, a.dk));
+        const Frag<NI> fq = frag_of<NI>(keep_head8<A>(rq[d], c, t, 32 * d + 8 * quad, a.dk));
 #pragma unroll
         for (int j = 0; j < TV; j++) {
           sum[j].add(fs[d][j], fk[d]);
@@ -167,12 +167,13 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
 #pragma unroll
       for (int j = 0; j < TV; j++) kS[j] = sum[j].sum();
     }
+    const RawV<T, TV> v4 = settle_v<A>(rv, dv0 + y0, a.dv);
 #pragma unroll
     for (int j = 0; j < TV; j++) {
       f32x4 x;
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const float v = t < c.len && dv0 + y0 + 4 * j + r < a.dv ? rv[4 * j + r] : 0.0f;
+        const float v = t < c.len && dv0 + y0 + 4 * j + r < a.dv ? v4[4 * j + r] : 0.0f;
         x[r] = beta * (v - gam * kS[j][r]);
       }
       put_four<NS>(xs + t * LDV + y0 + 4 * j, XP, x);
@@ -244,7 +245,7 @@ __global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int b
     fetch_p(next);
 #pragma unroll
     for (int j = 0; j < TV; j++) o[j] *= a.scale;
-    store_v<Fast, T, TV>(a.o, c, h, t, dv0 + y0, a.dv, o);
+    store_v<A, T, TV>(a.o, c, h, t, dv0 + y0, a.dv, o);
     if (kSets == 1) {
       __syncthreads();
       if (ci + 1 < chunks) {
@@ -274,7 +275,7 @@ void delta_forward_launch(const cchip_gated_delta &op, const DeltaArgs &a, bool 
     constexpr int DK = decltype(dk)::value, BV = decltype(bv)::value;
     const int blocks = back ? a.dvp / BV : (a.dv + BV - 1) / BV;  // saved columns that pad a head are written too
     with_bool(back, [&](auto b) {
-      with_bool(fast<typename M::T>(a), [&](auto f) {
+      with_access<typename M::T>(a, [&](auto f) {
         hipLaunchKernelGGL((delta_forward<M, DK, BV, decltype(b)::value, decltype(f)::value>),
                            dim3(unsigned((lanes + 7) / 8 * 8 * blocks)), dim3(256), 0, stream, a, blocks);
       });
