@@ -93,15 +93,25 @@ NormArgs args_of(const cchip_norm_block &op, const cchip_norm_block_io *io) {
   return a;
 }
 
-// Workgroups of a backward pass: as many as run at once, and at least 4 rows
-// each so that the sums they leave stay small beside the rows.
-int groups_of(const cchip_norm_block &op) {
-  const int64_t at_a_time = rows_at_a_time(int(op.width));
-  const int64_t sets = (op.rows + at_a_time - 1) / at_a_time;
-  return int(std::min<int64_t>(resident_groups(int(op.width)), (sets + 3) / 4));
+// A backward pass leaves a workgroup's sums in memory: of 4 rows at least,
+// so that they stay small beside the rows.
+int backward_groups(const cchip_norm_block &op, bool bias) {
+  int waves = 0;
+  with_shape(int(op.width), [&](auto lanes, auto) {
+    waves = waves_of(decltype(lanes)::value, op.gate != CCHIP_GATE_NONE, op.pre != CCHIP_NORM_NONE, bias);
+  });
+  return groups_of(op.rows, int(op.width), waves, 4);
 }
 
 }  // namespace
+
+int groups_of(int64_t rows, int width, int waves, int least) {
+  const int64_t at_a_time = rows_at_a_time(width), sets = (rows + at_a_time - 1) / at_a_time;
+  const int64_t most = 256 * (waves * 256 / threads_of(width));
+  const int64_t each = std::max<int64_t>(least, (sets + most - 1) / most);
+  return int((sets + each - 1) / each);
+}
+
 }  // namespace op
 }  // namespace cchip
 
@@ -132,7 +142,7 @@ int cchip_norm_block_forward(const cchip_norm_block *op, const cchip_norm_block_
 int cchip_norm_block_workspace(const cchip_norm_block *op, size_t *bytes) {
   return guarded([&] {
     check_op(op);
-    if (bytes) *bytes = size_t(groups_of(*op)) * kParams * op->width * sizeof(float);
+    if (bytes) *bytes = size_t(std::max(backward_groups(*op, false), backward_groups(*op, true))) * kParams * op->width * sizeof(float);
   });
 }
 
@@ -173,7 +183,7 @@ int cchip_norm_block_backward(const cchip_norm_block *op, const cchip_norm_block
       a.dgate = rows_of(who, "dgate", op->dtype, op->rows, op->width, io->dgate, true, false);
       a.dresidual = rows_of(who, "dresidual", op->dtype, op->rows, op->width, io->dresidual, true, false);
     }
-    const int groups = groups_of(*op);
+    const int groups = backward_groups(*op, bias);
     if (any) {
       const size_t need = size_t(groups) * (bias ? 5 : 3) * op->width * sizeof(float);
       if (workspace_bytes < need || (need && !workspace) || reinterpret_cast<uintptr_t>(workspace) % 4)

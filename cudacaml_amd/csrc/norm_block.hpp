@@ -19,12 +19,19 @@ struct NormArgs {
   Drop drop;
 };
 
-// Row sums over LANES threads: every one gets the sum. `at` is a scratch of
-// a float a wave and set, two sets, used in turn.
+// Row sums over LANES threads, or a workgroup of at most LANES: every one
+// gets the sum. `at` is a scratch of a float a wave and set, two sets, used
+// in turn, zero where there is no such wave.
 template <int LANES>
 struct RowSum {
   float (*at)[LANES > 64 ? LANES / 64 : 1];
   int set;
+  __device__ __forceinline__ void begin() {
+    if (LANES <= 64) return;
+    set = 0;
+    if (threadIdx.x < 2 * LANES / 64) at[0][threadIdx.x] = 0.0f;
+    __syncthreads();
+  }
   __device__ __forceinline__ float operator()(float x) {
     if (LANES == 16) return sum16(x);
     x = sum64(x);
@@ -87,7 +94,13 @@ __device__ __forceinline__ float normalise(float (&x)[V][8], int kind, float inv
   return inv;
 }
 
-__device__ __forceinline__ float sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }
+// For 16-bit elements by the exponential and reciprocal instructions, 1e-7
+// off for each unit of z where the element's rounding is 2e-4 or more.
+template <typename T>
+__device__ __forceinline__ float sigmoid(float z) {
+  if (sizeof(T) == 4) return 1.0f / (1.0f + expf(-z));
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f));
+}
 
 // A row to LANES threads, 8 neighbouring columns a thread and step, held in
 // registers from the one read of it to the writes. A workgroup takes every
@@ -97,6 +110,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_forward(const 
   constexpr int kRows = LANES < 256 ? 256 / LANES : 1;
   __shared__ float scratch[2][LANES > 64 ? LANES / 64 : 1];
   RowSum<LANES> sum = {scratch, 0};
+  sum.begin();
   const int lane = threadIdx.x % LANES;
   const float inv_width = 1.0f / float(a.width);
   const float up = a.scale * a.drop.up;
@@ -148,7 +162,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_forward(const 
       for (int i = 0; i < 8; i++) {
         float e = h[v][i] * w[v][i] + b[v][i];
         if (a.act != CCHIP_GATE_NONE) {
-          const float zi = float(z[v].x[i]), s = sigmoid(zi);
+          const float zi = float(z[v].x[i]), s = sigmoid<T>(zi);
           e *= a.act == CCHIP_GATE_SILU ? zi * s : s;
         }
         e = bits[v] >> i & 1 ? e : 0.0f;
@@ -210,30 +224,59 @@ __device__ __forceinline__ void normalise_back(float (&d)[V][8], const float (&x
 // are no biases and the last two are not made.
 enum Param { kPostWeight, kChannelScale, kPreWeight, kPostBias, kPreBias, kParams };
 
+// Waves a SIMD holds of a backward pass: 4 of at most 128 registers; with two
+// norms and a gate or biases, what a thread holds does not fit in those and
+// is not spilled for a fourth wave: 16384 rows of 4096 with all of it take
+// 374 us so and 593 spilled, without gate and biases 174 us of four waves and
+// 228 of three.
+constexpr int waves_of(int lanes, bool gate, bool pre, bool bias) {
+  return lanes > 512 || !(pre && (gate || bias)) ? 4 : lanes > 256 ? 2 : 3;
+}
+
 // As norm_forward, a workgroup taking every gridDim-th set of rows so that it
 // can sum the parameters' gradients of its columns in registers; they are
 // left in `partial` and added up by norm_columns.
 template <typename T, int LANES, int V, bool Gate, bool Pre, bool Bias>
-__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_backward(const NormArgs a) {
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES, waves_of(LANES, Gate, Pre, Bias)) void norm_backward(const NormArgs a) {
   constexpr int kRows = LANES < 256 ? 256 / LANES : 1, kThreads = LANES < 256 ? 256 : LANES;
   constexpr int kSums = Bias ? 5 : 3;
   __shared__ float scratch[2][LANES > 64 ? LANES / 64 : 1];
   RowSum<LANES> sum = {scratch, 0};
+  sum.begin();
   const int lane = threadIdx.x % LANES;
   const float inv_width = 1.0f / float(a.width);
   const float up = a.scale * a.drop.up;
   const uint64_t offset = a.drop.bar ? offset_of(a.drop) : 0;
   float acc[kSums][V][8] = {};
-  float w[V][8], b[V][8], t[V][8], pw[V][8];
   int n[V];
 #pragma unroll
   for (int v = 0; v < V; v++) {
     const int c = (v * LANES + lane) * 8;
     n[v] = a.width - c < 0 ? 0 : a.width - c > 8 ? 8 : a.width - c;
-    load_params<T>(w[v], a.post_weight, a.weights_f32, c, n[v], 1.0f);
-    load_params<T>(b[v], Bias ? a.post_bias : nullptr, a.weights_f32, c, n[v], 0.0f);
-    load_params<T>(t[v], a.channel_scale, a.weights_f32, c, n[v], 1.0f);
-    if (Pre) load_params<T>(pw[v], a.pre_weight, a.weights_f32, c, n[v], 1.0f);
+  }
+  // Parameters of this thread's columns: in LDS where a workgroup's fit.
+  extern __shared__ f32x4 held[];
+  const int lanes = LANES < 256 ? LANES : int(blockDim.x);
+  auto from_memory = [&](int k, int v, float(&x)[8]) {
+    const void *p = k == kPostWeight ? a.post_weight : k == kChannelScale ? a.channel_scale : k == kPreWeight ? a.pre_weight : a.post_bias;
+    load_params<T>(x, p, a.weights_f32, (v * LANES + lane) * 8, n[v], k == kPostBias ? 0.0f : 1.0f);
+  };
+  auto param = [&](int k, int v, int half) {
+    if (V == 1) return held[(k * 2 + half) * lanes + lane];
+    float x[8];
+    from_memory(k, v, x);
+    return f32x4{x[4 * half], x[4 * half + 1], x[4 * half + 2], x[4 * half + 3]};
+  };
+  if (V == 1) {
+#pragma unroll
+    for (int k = 0; k < (Bias ? 4 : 3); k++) {
+      float x[8];
+      from_memory(k, 0, x);
+      if (threadIdx.x < lanes)
+#pragma unroll
+        for (int i = 0; i < 2; i++) held[(k * 2 + i) * lanes + lane] = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+    }
+    __syncthreads();
   }
   for (int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / LANES; row < a.rows; row += int64_t(gridDim.x) * kRows) {
     Raw8<T> ry[V], rz[V], rh[V], rdh[V], rdn[V];
@@ -256,11 +299,15 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_backward(const
 #pragma unroll
       for (int v = 0; v < V; v++) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const float dn = float(rdn[v].x[i]);
-          acc[kPreWeight][v][i] += dn * x[v][i];
-          if (Bias) acc[kPreBias][v][i] += dn;
-          d[v][i] = i < n[v] ? dn * pw[v][i] : 0.0f;
+        for (int half = 0; half < 2; half++) {
+          const f32x4 pw = param(kPreWeight, v, half);
+#pragma unroll
+          for (int i = 4 * half; i < 4 * half + 4; i++) {
+            const float dn = float(rdn[v].x[i]);
+            acc[kPreWeight][v][i] += dn * x[v][i];
+            if (Bias) acc[kPreBias][v][i] += dn;
+            d[v][i] = i < n[v] ? dn * pw[i % 4] : 0.0f;
+          }
         }
       }
       normalise_back<LANES, V>(d, x, a.pre, inv, inv_width, a.eps, a.width, sum);
@@ -290,23 +337,30 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_backward(const
       float dz[8];
       const uint32_t bits = a.drop.bar ? keep_bits(a.drop, offset, uint32_t(row), g) : 0xFFu;
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const bool keep = bits >> i & 1 && i < n[v];
-        const float e = Bias ? x[v][i] * w[v][i] + b[v][i] : x[v][i] * w[v][i];
-        float act = 1.0f, slope = 0.0f;
-        if (Gate) {
-          const float z = float(rz[v].x[i]), s = sigmoid(z);
-          act = a.act == CCHIP_GATE_SILU ? z * s : s;
-          slope = a.act == CCHIP_GATE_SILU ? s * (1.0f + z * (1.0f - s)) : s * (1.0f - s);
+      for (int half = 0; half < 2; half++) {
+        __builtin_amdgcn_sched_barrier(0);  // four at a time: all eight hold more registers than there are
+        const f32x4 w = param(kPostWeight, v, half), t = param(kChannelScale, v, half);
+        const f32x4 b = Bias ? param(kPostBias, v, half) : f32x4{};
+#pragma unroll
+        for (int i = 4 * half; i < 4 * half + 4; i++) {
+          const bool keep = bits >> i & 1 && i < n[v];
+          const float e = Bias ? x[v][i] * w[i % 4] + b[i % 4] : x[v][i] * w[i % 4];
+          float act = 1.0f, slope = 0.0f;
+          if (Gate) {
+            const float z = float(rz[v].x[i]), s = sigmoid<T>(z);
+            act = a.act == CCHIP_GATE_SILU ? z * s : s;
+            slope = a.act == CCHIP_GATE_SILU ? s * (1.0f + z * (1.0f - s)) : s * (1.0f - s);
+          }
+          const float du = keep ? d[v][i] * up : 0.0f;
+          acc[kChannelScale][v][i] += keep ? du * e * act : 0.0f;
+          const float db = du * t[i % 4], da = db * act;
+          if (Gate) dz[i] = keep ? db * e * slope : 0.0f;
+          acc[kPostWeight][v][i] += da * x[v][i];
+          if (Bias) acc[kPostBias][v][i] += da;
+          d[v][i] = da * w[i % 4];
         }
-        const float du = keep ? d[v][i] * up : 0.0f;
-        acc[kChannelScale][v][i] += keep ? du * e * act : 0.0f;
-        const float db = du * t[v][i], da = db * act;
-        if (Gate) dz[i] = keep ? db * e * slope : 0.0f;
-        acc[kPostWeight][v][i] += da * x[v][i];
-        if (Bias) acc[kPostBias][v][i] += da;
-        d[v][i] = da * w[v][i];
       }
+      __builtin_amdgcn_sched_barrier(0);
       if (Gate && a.dgate.p) store8<T>(row_at<T>(a.dgate, row) + c, dz, n[v]);
     }
     if (a.post != CCHIP_NORM_NONE) normalise_back<LANES, V>(d, x, a.post, inv, inv_width, a.eps, a.width, sum);
@@ -351,12 +405,16 @@ void norm_backward_launch(const NormArgs &a, bool bias, int groups, hipStream_t 
 // Rows a workgroup takes at a time for a width.
 inline int rows_at_a_time(int width) { return width <= 128 ? 16 : width <= 512 ? 4 : 1; }
 
-// Workgroups that run at once: 8 of 256 threads a unit, fewer of more.
-inline int resident_groups(int width) { return width <= 2048 ? 1024 : width <= 4096 ? 512 : 256; }
+// Threads of a workgroup: a wave for each 512 columns where a row is one's.
+inline int threads_of(int width) { return width <= 512 ? 256 : width <= 8192 ? (width + 511) / 512 * 64 : 1024; }
+
+// Workgroups that take `rows` evenly, `least` at least each, as many as run
+// at once with `waves` a SIMD.
+int groups_of(int64_t rows, int width, int waves, int least);
 
 // Calls f(lanes, steps) with the smallest shape that holds a row: few lanes
 // for short rows, so that none idles, and 8 columns a thread up to 8192, so
-// that a backward pass's parameters and sums stay in registers.
+// that a backward pass's sums stay in registers.
 template <typename F>
 void with_shape(int width, F &&f) {
   if (width <= 128) f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
@@ -373,11 +431,8 @@ void with_shape(int width, F &&f) {
   void norm_forward_launch<T>(const NormArgs &a, hipStream_t stream) {                                             \
     with_shape(a.width, [&](auto lanes, auto steps) {                                                              \
       constexpr int L = decltype(lanes)::value, V = decltype(steps)::value;                                        \
-      constexpr int kRows = L < 256 ? 256 / L : 1;                                                                 \
-      const int64_t sets = (int64_t(a.rows) + kRows - 1) / kRows;                                                  \
-      const int most = 2 * resident_groups(a.width);                                                               \
-      hipLaunchKernelGGL((norm_forward<T, L, V>), dim3(unsigned(sets < most ? sets : most)),                       \
-                         dim3(L < 256 ? 256 : L), 0, stream, a);                                                   \
+      hipLaunchKernelGGL((norm_forward<T, L, V>), dim3(unsigned(groups_of(a.rows, a.width, 8, 1))),                \
+                         dim3(threads_of(a.width)), 0, stream, a);                                                 \
     });                                                                                                            \
   }                                                                                                                \
   template <>                                                                                                      \
@@ -389,7 +444,8 @@ void with_shape(int width, F &&f) {
                             : (bias ? norm_backward<T, L, V, true, false, true> : norm_backward<T, L, V, true, false, false>))   \
                      : (pre ? (bias ? norm_backward<T, L, V, false, true, true> : norm_backward<T, L, V, false, true, false>)    \
                             : (bias ? norm_backward<T, L, V, false, false, true> : norm_backward<T, L, V, false, false, false>));\
-      hipLaunchKernelGGL(k, dim3(unsigned(groups)), dim3(L < 256 ? 256 : L), 0, stream, a);                        \
+      const int threads = threads_of(a.width), held = V > 1 ? 0 : (bias ? 8 : 6) * 16 * (L < 256 ? L : threads);   \
+      hipLaunchKernelGGL(k, dim3(unsigned(groups)), dim3(threads), held, stream, a);                               \
     });                                                                                                            \
   }
 
