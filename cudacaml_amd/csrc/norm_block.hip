@@ -93,14 +93,23 @@ NormArgs args_of(const cchip_norm_block &op, const cchip_norm_block_io *io) {
   return a;
 }
 
+bool wide(const cchip_norm_block &op) { return op.width > 8192; }
+
 // A backward pass leaves a workgroup's sums in memory: of 4 rows at least,
-// so that they stay small beside the rows.
+// so that they stay small beside the rows. Those of wide rows are of 2048
+// columns each, four to a unit.
 int backward_groups(const cchip_norm_block &op, bool bias) {
+  if (wide(op)) return int(std::min<int64_t>((op.rows + 3) / 4, 1024 / ((op.width + 2047) / 2048)));
   int waves = 0;
   with_shape(int(op.width), [&](auto lanes, auto) {
     waves = waves_of(decltype(lanes)::value, op.gate != CCHIP_GATE_NONE, op.pre != CCHIP_NORM_NONE, bias);
   });
   return groups_of(op.rows, int(op.width), waves, 4);
+}
+
+// Sums of each workgroup, and wide rows' statistics after them.
+size_t workspace_of(const cchip_norm_block &op, bool bias) {
+  return size_t(backward_groups(op, bias)) * (bias ? 5 : 3) * op.width * sizeof(float) + (wide(op) ? size_t(op.rows) * sizeof(RowStat) : 0);
 }
 
 }  // namespace
@@ -142,7 +151,7 @@ int cchip_norm_block_forward(const cchip_norm_block *op, const cchip_norm_block_
 int cchip_norm_block_workspace(const cchip_norm_block *op, size_t *bytes) {
   return guarded([&] {
     check_op(op);
-    if (bytes) *bytes = size_t(std::max(backward_groups(*op, false), backward_groups(*op, true))) * kParams * op->width * sizeof(float);
+    if (bytes) *bytes = std::max(workspace_of(*op, false), workspace_of(*op, true));
   });
 }
 
@@ -185,10 +194,11 @@ int cchip_norm_block_backward(const cchip_norm_block *op, const cchip_norm_block
     }
     const int groups = backward_groups(*op, bias);
     if (any) {
-      const size_t need = size_t(groups) * (bias ? 5 : 3) * op->width * sizeof(float);
+      const size_t need = workspace_of(*op, bias);
       if (workspace_bytes < need || (need && !workspace) || reinterpret_cast<uintptr_t>(workspace) % 4)
         throw InvalidArgument(strf("norm block: the workspace needs %zu bytes aligned to 4, has %zu", need, workspace ? workspace_bytes : 0));
       a.partial = static_cast<float *>(workspace);
+      a.stats = reinterpret_cast<RowStat *>(a.partial + size_t(groups) * (bias ? 5 : 3) * op->width);
     }
     if (groups)
       with_rows_type(op->dtype, [&](auto t) { norm_backward_launch<decltype(t)>(a, bias, groups, (hipStream_t)stream); });

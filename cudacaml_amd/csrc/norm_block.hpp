@@ -7,11 +7,18 @@
 namespace cchip {
 namespace op {
 
+// What a row's norms leave for norm_sums: xhat is (x - mean) inv, and the
+// gradient through the pre norm (d - xhat along - share) inv.
+struct RowStat {
+  float pre_mean, pre_inv, along, share, post_mean, post_inv;
+};
+
 struct NormArgs {
   Rows y, gate, residual, h, n;                 // forward
   Rows dh, dn, dy, dgate, dresidual;            // backward (reads y, gate, h)
   const void *post_weight, *post_bias, *channel_scale, *pre_weight, *pre_bias;
   float *partial;  // backward: [workgroup][parameter][width]
+  RowStat *stats;  // backward of wide rows: [row]
   uint32_t rows;
   int width, post, pre, act;
   bool weights_f32;
@@ -68,7 +75,7 @@ __device__ __forceinline__ void load_params(float (&w)[8], const void *p, bool f
 // multiplied by. Sums of squares are of centred values: nothing cancels.
 template <int LANES, int V>
 __device__ __forceinline__ float normalise(float (&x)[V][8], int kind, float inv_width, float eps, RowSum<LANES> &sum,
-                                           int lane, int width) {
+                                           int lane, int width, float *of = nullptr) {
   if (kind == CCHIP_NORM_LAYER) {
     float s = 0.0f;
 #pragma unroll
@@ -76,6 +83,7 @@ __device__ __forceinline__ float normalise(float (&x)[V][8], int kind, float inv
 #pragma unroll
       for (int i = 0; i < 8; i++) s += x[v][i];
     const float mean = sum(s) * inv_width;
+    if (of) *of = mean;
 #pragma unroll
     for (int v = 0; v < V; v++)
 #pragma unroll
@@ -102,6 +110,14 @@ __device__ __forceinline__ float sigmoid(float z) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f));
 }
 
+// A gate's value for z and its slope.
+template <typename T>
+__device__ __forceinline__ void gate_of(int kind, float z, float &act, float &slope) {
+  const float s = sigmoid<T>(z);
+  act = kind == CCHIP_GATE_SILU ? z * s : s;
+  slope = kind == CCHIP_GATE_SILU ? s * (1.0f + z * (1.0f - s)) : s * (1.0f - s);
+}
+
 // A row to LANES threads, 8 neighbouring columns a thread and step, held in
 // registers from the one read of it to the writes. A workgroup takes every
 // gridDim-th set of rows and keeps the parameters of its columns.
@@ -116,24 +132,35 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_forward(const 
   const float up = a.scale * a.drop.up;
   const uint64_t offset = a.drop.bar ? offset_of(a.drop) : 0;
 
-  // (yhat w + b) up t, as one product and sum
+  // (yhat w + b) up t, as one product and sum. One row of parameters stays
+  // in registers, more are read again for each row.
   float w[V][8], b[V][8], pw[V][8], pb[V][8];
   int n[V];
 #pragma unroll
   for (int v = 0; v < V; v++) {
     const int c = (v * LANES + lane) * 8;
     n[v] = a.width - c < 0 ? 0 : a.width - c > 8 ? 8 : a.width - c;
+  }
+  auto post_params = [&](int v) {
+    const int c = (v * LANES + lane) * 8;
     float t[8];
     load_params<T>(t, a.channel_scale, a.weights_f32, c, n[v], 1.0f);
     load_params<T>(w[v], a.post_weight, a.weights_f32, c, n[v], 1.0f);
     load_params<T>(b[v], a.post_bias, a.weights_f32, c, n[v], 0.0f);
-    load_params<T>(pw[v], a.pre_weight, a.weights_f32, c, n[v], 1.0f);
-    load_params<T>(pb[v], a.pre_bias, a.weights_f32, c, n[v], 0.0f);
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       w[v][i] *= up * t[i];
       b[v][i] *= up * t[i];
     }
+  };
+  auto pre_params = [&](int v) {
+    const int c = (v * LANES + lane) * 8;
+    load_params<T>(pw[v], a.pre_weight, a.weights_f32, c, n[v], 1.0f);
+    load_params<T>(pb[v], a.pre_bias, a.weights_f32, c, n[v], 0.0f);
+  };
+  if (V == 1) {
+    post_params(0);
+    pre_params(0);
   }
   for (int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / LANES; row < a.rows; row += int64_t(gridDim.x) * kRows) {
     Raw8<T> y[V], z[V], x[V];
@@ -158,6 +185,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_forward(const 
     if (a.post != CCHIP_NORM_NONE) normalise<LANES, V>(h, a.post, inv_width, a.eps, sum, lane, a.width);
 #pragma unroll
     for (int v = 0; v < V; v++) {
+      if (V > 1) post_params(v);
 #pragma unroll
       for (int i = 0; i < 8; i++) {
         float e = h[v][i] * w[v][i] + b[v][i];
@@ -175,6 +203,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_forward(const 
     normalise<LANES, V>(h, a.pre, inv_width, a.eps, sum, lane, a.width);
 #pragma unroll
     for (int v = 0; v < V; v++) {
+      if (V > 1) pre_params(v);
 #pragma unroll
       for (int i = 0; i < 8; i++) h[v][i] = h[v][i] * pw[v][i] + pb[v][i];
       store8<T>(row_at<T>(a.n, row) + (v * LANES + lane) * 8, h[v], n[v]);
@@ -189,7 +218,8 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_forward(const 
 // and that share put back, as the difference itself would be rounding.
 template <int LANES, int V>
 __device__ __forceinline__ void normalise_back(float (&d)[V][8], const float (&xhat)[V][8], int kind, float inv,
-                                               float inv_width, float eps, int width, RowSum<LANES> &sum) {
+                                               float inv_width, float eps, int width, RowSum<LANES> &sum,
+                                               RowStat *of = nullptr) {
   float p = 0.0f, q = 0.0f;
 #pragma unroll
   for (int v = 0; v < V; v++)
@@ -214,6 +244,10 @@ __device__ __forceinline__ void normalise_back(float (&d)[V][8], const float (&x
     back = once * eps * inv * inv;
     p = q = 0.0f;
   }
+  if (of) {
+    of->along = p;
+    of->share = q;
+  }
 #pragma unroll
   for (int v = 0; v < V; v++)
 #pragma unroll
@@ -235,7 +269,9 @@ constexpr int waves_of(int lanes, bool gate, bool pre, bool bias) {
 
 // As norm_forward, a workgroup taking every gridDim-th set of rows so that it
 // can sum the parameters' gradients of its columns in registers; they are
-// left in `partial` and added up by norm_columns.
+// left in `partial` and added up by norm_columns. Rows of over 8192 columns
+// (V > 1) leave no registers for that: each leaves its statistics, and
+// norm_sums reads it again.
 template <typename T, int LANES, int V, bool Gate, bool Pre, bool Bias>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES, waves_of(LANES, Gate, Pre, Bias)) void norm_backward(const NormArgs a) {
   constexpr int kRows = LANES < 256 ? 256 / LANES : 1, kThreads = LANES < 256 ? 256 : LANES;
@@ -247,7 +283,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES, waves_of(LANES, Gate, Pr
   const float inv_width = 1.0f / float(a.width);
   const float up = a.scale * a.drop.up;
   const uint64_t offset = a.drop.bar ? offset_of(a.drop) : 0;
-  float acc[kSums][V][8] = {};
+  float acc[kSums][V][8] = {};  // of one step
   int n[V];
 #pragma unroll
   for (int v = 0; v < V; v++) {
@@ -286,16 +322,18 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES, waves_of(LANES, Gate, Pr
       if (Pre) rh[v] = load8<T>(row_at<T>(a.h, row) + c, n[v]);
       if (Pre) rdn[v] = load8<T>(row_at<T>(a.dn, row) + c, n[v]);
       rdh[v] = load8<T>(row_at<T>(a.dh, row) + c, n[v]);
-      ry[v] = load8<T>(row_at<T>(a.y, row) + c, n[v]);
-      if (Gate) rz[v] = load8<T>(row_at<T>(a.gate, row) + c, n[v]);
+      if (V < 4) ry[v] = load8<T>(row_at<T>(a.y, row) + c, n[v]);
+      if (V < 4 && Gate) rz[v] = load8<T>(row_at<T>(a.gate, row) + c, n[v]);
     }
+    RowStat stat = {0.0f, 1.0f, 0.0f, 0.0f, 0.0f, 1.0f};
     float d[V][8], x[V][8];
     if (Pre) {
 #pragma unroll
       for (int v = 0; v < V; v++)
 #pragma unroll
         for (int i = 0; i < 8; i++) x[v][i] = float(rh[v].x[i]);
-      const float inv = normalise<LANES, V>(x, a.pre, inv_width, a.eps, sum, lane, a.width);
+      const float inv = normalise<LANES, V>(x, a.pre, inv_width, a.eps, sum, lane, a.width, &stat.pre_mean);
+      stat.pre_inv = inv;
 #pragma unroll
       for (int v = 0; v < V; v++) {
 #pragma unroll
@@ -304,13 +342,13 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES, waves_of(LANES, Gate, Pr
 #pragma unroll
           for (int i = 4 * half; i < 4 * half + 4; i++) {
             const float dn = float(rdn[v].x[i]);
-            acc[kPreWeight][v][i] += dn * x[v][i];
-            if (Bias) acc[kPreBias][v][i] += dn;
+            if (V == 1) acc[kPreWeight][v][i] += dn * x[v][i];
+            if (V == 1 && Bias) acc[kPreBias][v][i] += dn;
             d[v][i] = i < n[v] ? dn * pw[i % 4] : 0.0f;
           }
         }
       }
-      normalise_back<LANES, V>(d, x, a.pre, inv, inv_width, a.eps, a.width, sum);
+      normalise_back<LANES, V>(d, x, a.pre, inv, inv_width, a.eps, a.width, sum, &stat);
 #pragma unroll
       for (int v = 0; v < V; v++)
 #pragma unroll
@@ -325,12 +363,20 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES, waves_of(LANES, Gate, Pr
 #pragma unroll
       for (int v = 0; v < V; v++) store8<T>(row_at<T>(a.dresidual, row) + (v * LANES + lane) * 8, d[v], n[v]);
 
+    if (V == 4)
+#pragma unroll
+      for (int v = 0; v < V; v++) {
+        ry[v] = load8<T>(row_at<T>(a.y, row) + (v * LANES + lane) * 8, n[v]);
+        if (Gate) rz[v] = load8<T>(row_at<T>(a.gate, row) + (v * LANES + lane) * 8, n[v]);
+      }
 #pragma unroll
     for (int v = 0; v < V; v++)
 #pragma unroll
       for (int i = 0; i < 8; i++) x[v][i] = float(ry[v].x[i]);
     float inv = 1.0f;
-    if (a.post != CCHIP_NORM_NONE) inv = normalise<LANES, V>(x, a.post, inv_width, a.eps, sum, lane, a.width);
+    if (a.post != CCHIP_NORM_NONE) inv = normalise<LANES, V>(x, a.post, inv_width, a.eps, sum, lane, a.width, &stat.post_mean);
+    stat.post_inv = inv;
+    if (V > 1 && a.partial && threadIdx.x == 0) a.stats[row] = stat;
 #pragma unroll
     for (int v = 0; v < V; v++) {
       const int g = v * LANES + lane, c = g * 8;
@@ -346,17 +392,13 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES, waves_of(LANES, Gate, Pr
           const bool keep = bits >> i & 1 && i < n[v];
           const float e = Bias ? x[v][i] * w[i % 4] + b[i % 4] : x[v][i] * w[i % 4];
           float act = 1.0f, slope = 0.0f;
-          if (Gate) {
-            const float z = float(rz[v].x[i]), s = sigmoid<T>(z);
-            act = a.act == CCHIP_GATE_SILU ? z * s : s;
-            slope = a.act == CCHIP_GATE_SILU ? s * (1.0f + z * (1.0f - s)) : s * (1.0f - s);
-          }
+          if (Gate) gate_of<T>(a.act, float(rz[v].x[i]), act, slope);
           const float du = keep ? d[v][i] * up : 0.0f;
-          acc[kChannelScale][v][i] += keep ? du * e * act : 0.0f;
+          if (V == 1) acc[kChannelScale][v][i] += keep ? du * e * act : 0.0f;
           const float db = du * t[i % 4], da = db * act;
           if (Gate) dz[i] = keep ? db * e * slope : 0.0f;
-          acc[kPostWeight][v][i] += da * x[v][i];
-          if (Bias) acc[kPostBias][v][i] += da;
+          if (V == 1) acc[kPostWeight][v][i] += da * x[v][i];
+          if (V == 1 && Bias) acc[kPostBias][v][i] += da;
           d[v][i] = da * w[i % 4];
         }
       }
@@ -367,7 +409,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES, waves_of(LANES, Gate, Pr
 #pragma unroll
     for (int v = 0; v < V; v++) store8<T>(row_at<T>(a.dy, row) + (v * LANES + lane) * 8, d[v], n[v]);
   }
-  if (!a.partial) return;
+  if (V > 1 || !a.partial) return;
   if (kRows > 1) {
     // the workgroup's rows side by side: sum them in the order of the rows
     __shared__ float side[kThreads * 8];
@@ -395,6 +437,57 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES, waves_of(LANES, Gate, Pr
         for (int i = 0; i < 8; i++)
           if (i < n[v]) a.partial[(int64_t(blockIdx.x) * kSums + s) * a.width + (v * LANES + lane) * 8 + i] = acc[s][v][i];
   }
+}
+
+// The parameters' gradients of wide rows: a workgroup sums 2048 columns of
+// every gridDim.y-th row from what the rows' statistics make of them.
+template <typename T, bool Gate, bool Pre, bool Bias>
+__global__ __launch_bounds__(256, 4) void norm_sums(const NormArgs a) {
+  constexpr int kSums = Bias ? 5 : 3;
+  const int group = int(blockIdx.x) * 256 + int(threadIdx.x), c = group * 8;
+  const int n = a.width - c < 0 ? 0 : a.width - c > 8 ? 8 : a.width - c;
+  if (!n) return;
+  const float up = a.scale * a.drop.up;
+  const uint64_t offset = a.drop.bar ? offset_of(a.drop) : 0;
+  float acc[kSums][8] = {};
+  float w[8], t[8], b[8], pw[8];
+  load_params<T>(w, a.post_weight, a.weights_f32, c, n, 1.0f);
+  load_params<T>(t, a.channel_scale, a.weights_f32, c, n, 1.0f);
+  if (Bias) load_params<T>(b, a.post_bias, a.weights_f32, c, n, 0.0f);
+  if (Pre) load_params<T>(pw, a.pre_weight, a.weights_f32, c, n, 1.0f);
+  for (uint32_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    Raw8<T> ry, rz, rh, rdh, rdn;
+    if (Pre) rh = load8<T>(row_at<T>(a.h, row) + c, n);
+    if (Pre) rdn = load8<T>(row_at<T>(a.dn, row) + c, n);
+    rdh = load8<T>(row_at<T>(a.dh, row) + c, n);
+    ry = load8<T>(row_at<T>(a.y, row) + c, n);
+    if (Gate) rz = load8<T>(row_at<T>(a.gate, row) + c, n);
+    const RowStat s = a.stats[row];
+    const uint32_t bits = a.drop.bar ? keep_bits(a.drop, offset, row, group) : 0xFFu;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      float d = float(rdh.x[i]);
+      if (Pre) {
+        const float dn = float(rdn.x[i]), xhat = (float(rh.x[i]) - s.pre_mean) * s.pre_inv;
+        acc[kPreWeight][i] += dn * xhat;
+        if (Bias) acc[kPreBias][i] += dn;
+        d += (dn * pw[i] - xhat * s.along - s.share) * s.pre_inv;
+      }
+      const float x = (float(ry.x[i]) - s.post_mean) * s.post_inv, e = Bias ? x * w[i] + b[i] : x * w[i];
+      float act = 1.0f, slope = 0.0f;
+      if (Gate) gate_of<T>(a.act, float(rz.x[i]), act, slope);
+      const float du = bits >> i & 1 ? d * up : 0.0f;
+      acc[kChannelScale][i] += bits >> i & 1 ? du * e * act : 0.0f;
+      const float da = du * t[i] * act;
+      acc[kPostWeight][i] += da * x;
+      if (Bias) acc[kPostBias][i] += da;
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < kSums; s++)
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (i < n) a.partial[(int64_t(blockIdx.y) * kSums + s) * a.width + c + i] = acc[s][i];
 }
 
 template <typename T>
@@ -426,6 +519,21 @@ void with_shape(int width, F &&f) {
   else f(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
 }
 
+// Calls f with whether there are a gate, a pre norm and biases.
+template <typename F>
+void with_parts(const NormArgs &a, bool bias, F &&f) {
+  auto third = [&](auto gate, auto pre) {
+    if (bias) f(gate, pre, std::true_type());
+    else f(gate, pre, std::false_type());
+  };
+  auto second = [&](auto gate) {
+    if (a.pre != CCHIP_NORM_NONE) third(gate, std::true_type());
+    else third(gate, std::false_type());
+  };
+  if (a.act != CCHIP_GATE_NONE) second(std::true_type());
+  else second(std::false_type());
+}
+
 #define CCHIP_NORM_BLOCK_LAUNCHERS(T)                                                                              \
   template <>                                                                                                      \
   void norm_forward_launch<T>(const NormArgs &a, hipStream_t stream) {                                             \
@@ -439,13 +547,20 @@ void with_shape(int width, F &&f) {
   void norm_backward_launch<T>(const NormArgs &a, bool bias, int groups, hipStream_t stream) {                     \
     with_shape(a.width, [&](auto lanes, auto steps) {                                                              \
       constexpr int L = decltype(lanes)::value, V = decltype(steps)::value;                                        \
-      const bool gate = a.act != CCHIP_GATE_NONE, pre = a.pre != CCHIP_NORM_NONE;                                  \
-      auto *k = gate ? (pre ? (bias ? norm_backward<T, L, V, true, true, true> : norm_backward<T, L, V, true, true, false>)      \
-                            : (bias ? norm_backward<T, L, V, true, false, true> : norm_backward<T, L, V, true, false, false>))   \
-                     : (pre ? (bias ? norm_backward<T, L, V, false, true, true> : norm_backward<T, L, V, false, true, false>)    \
-                            : (bias ? norm_backward<T, L, V, false, false, true> : norm_backward<T, L, V, false, false, false>));\
-      const int threads = threads_of(a.width), held = V > 1 ? 0 : (bias ? 8 : 6) * 16 * (L < 256 ? L : threads);   \
-      hipLaunchKernelGGL(k, dim3(unsigned(groups)), dim3(threads), held, stream, a);                               \
+      with_parts(a, bias, [&](auto g, auto p, auto b) {                                                            \
+        constexpr bool G = decltype(g)::value, P = decltype(p)::value, B = decltype(b)::value;                     \
+        const int threads = threads_of(a.width);                                                                   \
+        if constexpr (V == 1) {                                                                                    \
+          hipLaunchKernelGGL((norm_backward<T, L, V, G, P, B>), dim3(unsigned(groups)), dim3(threads),             \
+                             (B ? 8 : 6) * 16 * (L < 256 ? L : threads), stream, a);                               \
+        } else {                                                                                                   \
+          hipLaunchKernelGGL((norm_backward<T, L, V, G, P, B>), dim3(unsigned(groups_of(a.rows, a.width, 4, 1))),  \
+                             dim3(threads), 0, stream, a);                                                         \
+          if (a.partial)                                                                                           \
+            hipLaunchKernelGGL((norm_sums<T, G, P, B>), dim3(unsigned((a.width + 2047) / 2048), unsigned(groups)),     \
+                               dim3(256), 0, stream, a);                                                           \
+        }                                                                                                          \
+      });                                                                                                          \
     });                                                                                                            \
   }
 
