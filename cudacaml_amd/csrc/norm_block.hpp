@@ -31,12 +31,12 @@ struct NormArgs {
 // in turn, zero where there is no such wave.
 template <int LANES>
 struct RowSum {
-  float (*at)[LANES > 64 ? LANES / 64 : 1];
+  f32x2 (*at)[LANES > 64 ? LANES / 64 : 1];
   int set;
   __device__ __forceinline__ void begin() {
     if (LANES <= 64) return;
     set = 0;
-    if (threadIdx.x < 2 * LANES / 64) at[0][threadIdx.x] = 0.0f;
+    if (threadIdx.x < 2 * LANES / 64) at[0][threadIdx.x] = f32x2{};
     __syncthreads();
   }
   __device__ __forceinline__ float operator()(float x) {
@@ -44,15 +44,44 @@ struct RowSum {
     x = sum64(x);
     if (LANES == 64) return x;
     const int w = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) at[set][w] = x;
+    if ((threadIdx.x & 63) == 0) at[set][w].x = x;
     __syncthreads();
     float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < (LANES > 64 ? LANES / 64 : 1); i++) s += at[set][i];
+    for (int i = 0; i < (LANES > 64 ? LANES / 64 : 1); i++) s += at[set][i].x;
     set ^= 1;
     return s;
   }
+  // Two at once.
+  __device__ __forceinline__ void operator()(float &x, float &y) {
+    if (LANES <= 64) {
+      x = (*this)(x);
+      y = (*this)(y);
+      return;
+    }
+    x = sum64(x);
+    y = sum64(y);
+    const int w = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) at[set][w] = f32x2{x, y};
+    __syncthreads();
+    f32x2 s = {};
+#pragma unroll
+    for (int i = 0; i < (LANES > 64 ? LANES / 64 : 1); i++) {
+      s.x += at[set][i].x;
+      s.y += at[set][i].y;
+    }
+    set ^= 1;
+    x = s.x;
+    y = s.y;
+  }
 };
+
+// 1 / sqrt(x) by the instruction, which knows no subnormal x.
+__device__ __forceinline__ float inverse_root(float x) {
+  const bool small = x < 0x1p-100f;
+  const float r = __builtin_amdgcn_rsqf(small ? x * 0x1p100f : x);
+  return small ? r * 0x1p50f : r;
+}
 
 // Eight of a parameter vector; `none` where there is none.
 template <typename T>
@@ -94,7 +123,7 @@ __device__ __forceinline__ float normalise(float (&x)[V][8], int kind, float inv
   for (int v = 0; v < V; v++)
 #pragma unroll
     for (int i = 0; i < 8; i++) q += x[v][i] * x[v][i];
-  const float inv = 1.0f / sqrtf(sum(q) * inv_width + eps);
+  const float inv = inverse_root(sum(q) * inv_width + eps);
 #pragma unroll
   for (int v = 0; v < V; v++)
 #pragma unroll
@@ -124,7 +153,7 @@ __device__ __forceinline__ void gate_of(int kind, float z, float &act, float &sl
 template <typename T, int LANES, int V>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_forward(const NormArgs a) {
   constexpr int kRows = LANES < 256 ? 256 / LANES : 1;
-  __shared__ float scratch[2][LANES > 64 ? LANES / 64 : 1];
+  __shared__ f32x2 scratch[2][LANES > 64 ? LANES / 64 : 1];
   RowSum<LANES> sum = {scratch, 0};
   sum.begin();
   const int lane = threadIdx.x % LANES;
@@ -228,8 +257,10 @@ __device__ __forceinline__ void normalise_back(float (&d)[V][8], const float (&x
       p += d[v][i] * xhat[v][i];
       q += d[v][i];
     }
-  p = sum(p) * inv_width;
-  q = kind == CCHIP_NORM_LAYER ? sum(q) * inv_width : 0.0f;
+  if (kind == CCHIP_NORM_LAYER) sum(p, q);
+  else p = sum(p);
+  p *= inv_width;
+  q = kind == CCHIP_NORM_LAYER ? q * inv_width : 0.0f;
   float back = 0.0f;
   if (width <= 2) {
     float s = 0.0f;
@@ -261,8 +292,8 @@ enum Param { kPostWeight, kChannelScale, kPreWeight, kPostBias, kPreBias, kParam
 // Waves a SIMD holds of a backward pass: 4 of at most 128 registers; with two
 // norms and a gate or biases, what a thread holds does not fit in those and
 // is not spilled for a fourth wave: 16384 rows of 4096 with all of it take
-// 374 us so and 593 spilled, without gate and biases 174 us of four waves and
-// 228 of three.
+// 347 us so and 593 spilled, without gate and biases 174 us of four waves and
+// 228 of three. (bf16; floors of 220 and 165 us by the bytes.)
 constexpr int waves_of(int lanes, bool gate, bool pre, bool bias) {
   return lanes > 512 || !(pre && (gate || bias)) ? 4 : lanes > 256 ? 2 : 3;
 }
@@ -271,12 +302,15 @@ constexpr int waves_of(int lanes, bool gate, bool pre, bool bias) {
 // can sum the parameters' gradients of its columns in registers; they are
 // left in `partial` and added up by norm_columns. Rows of over 8192 columns
 // (V > 1) leave no registers for that: each leaves its statistics, and
-// norm_sums reads it again.
+// norm_sums reads it again, 4096 rows of 16384 taking 357 us in both kernels
+// where one that spilled its sums took 678. Up to 8192 columns one kernel is
+// the faster: 16384 rows of 5000 with two norms and a gate take 567 us, and
+// 715 in two.
 template <typename T, int LANES, int V, bool Gate, bool Pre, bool Bias>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES, waves_of(LANES, Gate, Pre, Bias)) void norm_backward(const NormArgs a) {
   constexpr int kRows = LANES < 256 ? 256 / LANES : 1, kThreads = LANES < 256 ? 256 : LANES;
   constexpr int kSums = Bias ? 5 : 3;
-  __shared__ float scratch[2][LANES > 64 ? LANES / 64 : 1];
+  __shared__ f32x2 scratch[2][LANES > 64 ? LANES / 64 : 1];
   RowSum<LANES> sum = {scratch, 0};
   sum.begin();
   const int lane = threadIdx.x % LANES;
