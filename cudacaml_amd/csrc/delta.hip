@@ -10,8 +10,12 @@ using namespace cchip::op;
 
 namespace {
 
-// Up to this many tokens a sequence the recurrence runs token by token.
-constexpr int64_t kStepTokens = 8;
+// Up to this many tokens a sequence the recurrence runs token by token, which
+// grows with them while a chunk costs the same for 1 token and 64: 8 x 16
+// heads of 128 x 128 take 17.6 us for 8 tokens, 30.2 for 16 and 55.9 for 32,
+// the chunk's kernels 31; 256 x 32 heads 619 us for 8, 1085 for 16, the
+// chunk's 1268.
+constexpr int64_t kStepTokens = 16;
 
 struct Layout {
   int64_t slots, slot_heads;

@@ -1,6 +1,6 @@
 // The gated delta rule: arguments, chunk records and sequence lookup shared
 // by its kernels (delta_chunk.hip, delta_forward.hip, delta_backward.hip,
-// delta_step.hip) and their host side (delta.cpp).
+// delta_step.hip) and their host side (delta.hip).
 //
 // A sequence is cut into chunks of 64 tokens. With c the running sum of g in
 // a chunk, D_ts = exp(c_t - c_s) for s <= t, Gam_t = exp(c_t), G_s =
@@ -424,6 +424,14 @@ void delta_chunk_launch(const cchip_gated_delta &op, const DeltaArgs &a, bool ba
 void delta_forward_launch(const cchip_gated_delta &op, const DeltaArgs &a, bool back, hipStream_t stream);
 void delta_backward_launch(const cchip_gated_delta &op, const DeltaArgs &a, hipStream_t stream);
 void delta_step_launch(const cchip_gated_delta &op, const DeltaArgs &a, hipStream_t stream);
+
+// Whether forward and reverse take 16 value columns a workgroup and not 32:
+// where so many workgroups still find a unit each, as a chunk of 16 columns
+// takes less time than one of 32 (forward of 16384 tokens, 32 bf16 heads of
+// 128: 515 us in 256 workgroups, 855 in 128). Beyond that 32 do more at once:
+// forward and reverse of 3 x 4096 tokens, 16 heads, take 508 us in 192
+// workgroups and 555 in 384, of 4 x 4096 and 32 heads 750 and 1080.
+inline bool narrow_blocks(const DeltaArgs &a) { return a.sequences * a.hv * ((a.dv + 31) / 32) <= 128; }
 
 inline int padded_key_dim(int dk) { return dk <= 64 ? 64 : 128; }
 

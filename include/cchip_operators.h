@@ -51,8 +51,8 @@ extern "C" {
  * `states` non-zero: sequences begin from `state` (NULL: zeros) and their
  * last states or the gradients of their first ones are wanted; the products
  * that make a state then keep 24 bits of f32 operands. With `states` zero,
- * those arguments are NULL and bf16 operands are rounded to 8 bits once per
- * 64 tokens. Sums and states are f32 either way.
+ * those arguments are NULL and a bf16 operator keeps 16 bits of them. Sums
+ * and the states that go from chunk to chunk are f32 either way.
  *
  * A NaN or infinity in a token reaches the outputs of its own sequence and
  * value heads from the 64-token chunk it stands in onwards, in the backward
@@ -90,7 +90,7 @@ typedef struct {
 /* Bytes of workspace that a forward and a backward call need (a workspace
    holds nothing between calls; calls that overlap need one each), and of
    `saved`. All are aligned to 16 bytes. A forward call that saves needs no
-   workspace, nor does one of at most 8 tokens a sequence, not packed, that
+   workspace, nor does one of at most 16 tokens a sequence, not packed, that
    does not: it runs the recurrence itself. */
 int cchip_gated_delta_sizes(const cchip_gated_delta *op, size_t *forward, size_t *backward, size_t *saved);
 int cchip_gated_delta_forward(const cchip_gated_delta *op, const cchip_gated_delta_io *io, void *workspace,
@@ -183,7 +183,7 @@ int cchip_norm_block_forward(const cchip_norm_block *op, const cchip_norm_block_
 /* From y, gate, the forward pass's h (needed iff pre is not none), and the
    gradients dh and dn of its results: the gradients of y, gate, residual and
    the parameters, those summed over rows in f32 in an order that does not
-   change from run to run. */
+   change from run to run. What it writes overlaps nothing that it reads. */
 int cchip_norm_block_workspace(const cchip_norm_block *op, size_t *bytes);
 int cchip_norm_block_backward(const cchip_norm_block *op, const cchip_norm_block_io *io, void *workspace,
                               size_t workspace_bytes, void *stream);

@@ -110,7 +110,7 @@ def check_delta(x, dtype, cuts=None, back=False, **kw):
 
 
 SHAPES = [  # batch, tokens, key heads, value heads, key_dim, value_dim
-    (1, 1, 1, 1, 1, 1), (3, 1, 2, 4, 128, 128), (2, 2, 1, 2, 64, 64), (2, 8, 2, 2, 72, 100), (2, 9, 1, 1, 128, 64),
+    (1, 1, 1, 1, 1, 1), (3, 1, 2, 4, 128, 128), (2, 2, 1, 2, 64, 64), (2, 8, 2, 2, 72, 100), (2, 9, 1, 1, 128, 64), (2, 16, 1, 2, 64, 96), (3, 17, 1, 1, 100, 40),
     (1, 63, 1, 2, 64, 32), (1, 64, 2, 2, 128, 128), (2, 65, 1, 4, 17, 250), (1, 130, 3, 3, 40, 33), (2, 200, 2, 4, 128, 96),
 ]
 
