@@ -433,6 +433,14 @@ void delta_step_launch(const cchip_gated_delta &op, const DeltaArgs &a, hipStrea
 // workgroups and 555 in 384, of 4 x 4096 and 32 heads 750 and 1080.
 inline bool narrow_blocks(const DeltaArgs &a) { return a.sequences * a.hv * ((a.dv + 31) / 32) <= 128; }
 
+// Workgroups of delta_forward and delta_reverse a unit is to hold: two where
+// their LDS leaves room. (With keys of up to 64 elements f32 and f16 would
+// have it too, but not the registers: they spill, and run no faster.)
+template <typename M>
+constexpr int groups_a_unit(int dk, int bv) {
+  return M::NI > 1 || (M::NS > 2 && dk * bv > 128 * 16) ? 1 : 2;
+}
+
 inline int padded_key_dim(int dk) { return dk <= 64 ? 64 : 128; }
 
 template <typename F>

@@ -33,7 +33,7 @@ namespace {
 // one more wait a chunk and the states read too: 390 us for 4 x 4096 tokens,
 // 32 bf16 heads of 128, 1.3 GB at 3.4 TB/s.
 template <typename M, int DK, int BV, int A>
-__global__ __launch_bounds__(256, 2) void delta_reverse(const DeltaArgs a, int blocks) {
+__global__ __launch_bounds__(256, groups_a_unit<M>(DK, BV)) void delta_reverse(const DeltaArgs a, int blocks) {
   typedef typename M::T T;
   typedef typename M::Saved Saved;
   constexpr int NI = M::NI, NS = M::NS;

@@ -25,7 +25,7 @@ namespace {
 // MFLOP of products a chunk and head, in planes twice that, at a quarter of
 // the matrix rate: neither is at its limit, the waits between are the rest.
 template <typename M, int DK, int BV, bool Back, int A>
-__global__ __launch_bounds__(256, 2) void delta_forward(const DeltaArgs a, int blocks) {
+__global__ __launch_bounds__(256, groups_a_unit<M>(DK, BV)) void delta_forward(const DeltaArgs a, int blocks) {
   typedef typename M::T T;
   typedef typename M::Saved Saved;
   constexpr int NI = M::NI, NS = M::NS, NO = M::NO, NU = M::NU;

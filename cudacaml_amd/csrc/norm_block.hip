@@ -191,6 +191,10 @@ int cchip_norm_block_backward(const cchip_norm_block *op, const cchip_norm_block
       a.dy = rows_of(who, "dy", op->dtype, op->rows, op->width, io->dy, true, true);
       a.dgate = rows_of(who, "dgate", op->dtype, op->rows, op->width, io->dgate, true, false);
       a.dresidual = rows_of(who, "dresidual", op->dtype, op->rows, op->width, io->dresidual, true, false);
+      // norm_sums reads its inputs after the others are written
+      for (const char *out : {a.dy.p, a.dgate.p, a.dresidual.p})
+        for (const char *in : {a.y.p, a.gate.p, a.h.p, a.dh.p, a.dn.p})
+          if (out && out == in) throw InvalidArgument("norm block: a gradient is written over what the backward pass reads");
     }
     const int groups = backward_groups(*op, bias);
     if (any) {

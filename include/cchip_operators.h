@@ -66,7 +66,8 @@ typedef struct {
   float scale;
 } cchip_gated_delta;
 
-/* A tensor [batch][token][head][dim]: the distances, in elements, of
+/* What a call writes overlaps nothing that it reads, but for state_out.
+   A tensor [batch][token][head][dim]: the distances, in elements, of
    neighbours along the first three; the elements of a head are adjacent. g
    and beta have no last dimension. */
 typedef struct {

@@ -148,6 +148,14 @@ def test_gated_delta_packed(device, dtype, cuts):
             assert torch.equal(got["dstate"][i].cpu(), x["dstate_out"][i])
 
 
+def test_gated_delta_offsets_are_clamped(device):
+    """Offsets below 0 or past the tokens count as those."""
+    x = arrays("bf16", 1, 150, 1, 2, 32, 32, seed=17, states=3, back=True)
+    a, b = run_delta(x, "bf16", [-7, 70, 150, 2000000000], back=True), run_delta(x, "bf16", [0, 70, 150, 150], back=True)
+    for n in a:
+        assert torch.equal(a[n], b[n]), n
+
+
 def test_gated_delta_no_tokens(device):
     x = arrays("bf16", 2, 0, 1, 2, 32, 32, states=2)
     got = run_delta(x, "bf16")
@@ -196,6 +204,31 @@ def test_gated_delta_strides(device, layout, shape):
     x = arrays("bf16", *shape, seed=5, states=shape[0], back=True)
     a = run_delta(x, "bf16", back=True)
     b = run_delta(x, "bf16", back=True, layout=layout)
+    for n in a:
+        assert torch.equal(a[n], b[n]), n
+
+
+def _far_apart(tokens):
+    """v, o's gradient and dv with tokens or rows of the batch so far apart
+    that their last elements lie past 2^32 bytes (and 2^31 elements)."""
+    def far(t):
+        b, n, h, d = t.shape
+        step = (1 << 23) if tokens else h * d
+        row = n * step if tokens else (1 << 31) + 8
+        whole = torch.empty((b - 1) * row + (n - 1) * step + h * d, dtype=t.dtype, device="cuda")
+        part = whole.as_strided((b, n, h, d), (row, step, d, 1))
+        part.copy_(t)
+        return part
+
+    return lambda dev: {k: far(v) if k in ("v", "do") else v for k, v in dev.items()}
+
+
+@pytest.mark.parametrize("shape,tokens", [((2, 3, 1, 2, 32, 32), False), ((2, 300, 1, 2, 32, 32), False),
+                                          ((2, 300, 1, 2, 32, 32), True)])
+def test_gated_delta_tensors_past_32_bits(device, shape, tokens):
+    x = arrays("bf16", *shape, seed=15, states=shape[0], back=True)
+    a = run_delta(x, "bf16", back=shape[1] > 3)
+    b = run_delta(x, "bf16", back=shape[1] > 3, layout=_far_apart(tokens))
     for n in a:
         assert torch.equal(a[n], b[n]), n
 
@@ -472,6 +505,29 @@ def test_norm_block_strided_rows(device):
 
     check_norm("bf16", "f32", 11, 136, "rms", "layer", "silu", view=view, seed=6)
     check_norm("f32", "f32", 11, 77, "layer", "rms", "none", view=view, seed=7)
+
+
+def test_rows_past_32_bits(device):
+    """Rows 2^30 + 9 elements apart: the last of them past 2^32 bytes."""
+    def view(t):
+        whole = torch.empty((t.shape[0] - 1) * ((1 << 30) + 9) + t.shape[1], dtype=t.dtype, device="cuda")
+        part = whole.as_strided(tuple(t.shape), ((1 << 30) + 9, 1))
+        part.copy_(t)
+        return part
+
+    check_norm("bf16", "f32", 4, 136, "rms", "layer", "silu", view=view, seed=6)
+    x = torch.randn(4, 100, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    far, out = view(x.cuda()), view(torch.zeros(4, 100, dtype=torch.bfloat16, device="cuda"))
+    O.Dropout("bf16", 4, 100, 0.3).forward(far, out, seed=5, offset=6)
+    torch.cuda.synchronize()
+    close(out, R.drop(x.double().numpy(), 0.3, 5, 6), "out")
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("how", [("rms", "rms", "none"), ("layer", "layer", "silu"), ("layer", "none", "sigmoid")])
+def test_norm_block_many_wide_rows(device, dtype, how):
+    """Over 8192 columns the parameters' gradients are summed apart."""
+    check_norm(dtype, "f32", 70, 8200, *how, seed=16)
 
 
 def test_norm_block_rows_of_zeros_and_constants(device):

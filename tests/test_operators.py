@@ -192,6 +192,9 @@ def test_norm_block_refuses_calls():
         op.forward(z(4, 8), z(1, 8).expand(4, 8), z(4, 8))
     with pytest.raises(ValueError, match="h and dn"):
         op.backward(z(4, 8), z(4, 8), z(4, 8))
+    dh = z(4, 8)
+    with pytest.raises(ValueError, match="written over"):
+        op.backward(z(4, 8), dh, dh, dn=z(4, 8), h=z(4, 8))
     plain = O.NormBlock("f32", 4, 8, norm="none", pre="none")
     plain._device = -1
     with pytest.raises(ValueError, match="post norm that there is not"):
