@@ -60,28 +60,29 @@ struct DeltaArgs {
 };
 
 // Element type, then the planes: NI of an input, NS of what makes a state
-// (S, T, X and U in their products), NO of S and P where they make only an
-// output, NU of U and Y where they make only outputs. Saved is the type that
-// S and dS are kept in for the backward pass, read back in NB planes, and
-// Kept that of U and Y: f16 with a power of two for each token and 16
-// columns (11 bits, which two planes hold) or f32.
+// (S, T, X and U in their products), NO of S, P, U and Y where they make only
+// outputs. Saved is the type that S and dS are kept in for the backward pass,
+// read back in NB planes, and Kept that of U and Y: f16 with a power of two
+// for each token and 16 columns (11 bits, which two planes hold) or f32.
 //
 // A product loses the most precise operand's worth of the other's rounding:
-// 2^-9 of a value in one plane of bf16, 2^-17 in two. bf16 results are
-// rounded to 2^-9 themselves, and each of theirs comes through one operand
-// in one plane and no more (2.3e-3 in the 2-norm where their own rounding
-// alone is 1.7e-3); states in f32 take three planes.
-template <typename T_, int NI_, int NS_, int NO_, int NU_, typename Saved_, int NB_, typename Kept_>
+// 2^-9 of a value in one plane of bf16, 2^-17 in two; states in f32 take
+// three. bf16 results are rounded to 2^-9 themselves, 1.7e-3 in the 2-norm.
+// o adds nothing to that; in one plane it would be 2.4e-3 off, for 363 us in
+// place of 376 (forward of 4 x 4096 tokens, 32 heads of 128). The gradients
+// of q, k, g and beta add the rounding of the saved S and dS, 2.4e-3 in all:
+// kept as f32 these would be another 0.5 GB there to write and to read.
+template <typename T_, int NI_, int NS_, int NO_, typename Saved_, int NB_, typename Kept_>
 struct Mode {
   typedef T_ T;
   typedef Saved_ Saved;
   typedef Kept_ Kept;
-  static constexpr int NI = NI_, NS = NS_, NO = NO_, NU = NU_, NB = NB_;
+  static constexpr int NI = NI_, NS = NS_, NO = NO_, NB = NB_;
 };
-typedef Mode<bf16, 1, 2, 1, 2, bf16, 1, f16> ModeBf16;   // bf16 in and out
-typedef Mode<bf16, 1, 3, 1, 2, bf16, 1, f16> ModeBf16S;  // with f32 states in or out
-typedef Mode<f16, 2, 3, 2, 2, float, 2, float> ModeF16;
-typedef Mode<float, 3, 3, 3, 3, float, 3, float> ModeF32;
+typedef Mode<bf16, 1, 2, 2, bf16, 1, f16> ModeBf16;   // bf16 in and out
+typedef Mode<bf16, 1, 3, 2, bf16, 1, f16> ModeBf16S;  // with f32 states in or out
+typedef Mode<f16, 2, 3, 2, float, 2, float> ModeF16;
+typedef Mode<float, 3, 3, 3, float, 3, float> ModeF32;
 
 // What a chunk and value head have that depends on no state: matrices as
 // fragments of 16 rows and 32 terms, [row block][term block][lane][8], in

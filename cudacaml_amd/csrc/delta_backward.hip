@@ -279,18 +279,18 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
   typedef typename M::T T;
   typedef typename M::Saved Saved;
   typedef typename M::Kept Kept;
-  constexpr int NI = M::NI, NB = M::NB, NU = M::NU, P = 2, kThreads = 256 * P;
+  constexpr int NI = M::NI, NB = M::NB, NO = M::NO, P = 2, kThreads = 256 * P;
   constexpr int LDK = DK + 16, KP = 64 * LDK, LDS = 40, SP = DK * LDS, UP = 64 * LDS, LDM = 72, MP = 64 * LDM;
   constexpr int JK = DK / 16 / P, JS = 4 / P;  // 16-wide tiles of a part: of a key, of the tokens
   constexpr bool kAll = NB < 3;               // everything in LDS at a time; else E after S, and Y and dO not
   typedef Record<M> R;
-  constexpr int kSlices = (kAll ? 2 : 1) * NB * SP + NU * UP + (kAll ? (NU + NI) * UP : 0), kMs = (kAll ? 2 : 1) * NB * MP;
+  constexpr int kSlices = (kAll ? 2 : 1) * NB * SP + NO * UP + (kAll ? (NO + NI) * UP : 0), kMs = (kAll ? 2 : 1) * NB * MP;
   __shared__ __align__(16) bf16 ks[NI * KP], qs[NI * KP], slice[kSlices > kMs ? kSlices : kMs];
   __shared__ double cs[64];
   __shared__ __align__(16) float down[4][64];
   __shared__ float row_c[P][64], row_b[P][64], row_y[64], total[4 * P];
-  bf16 *const us = slice, *const ss = slice + NU * UP, *const es = kAll ? ss + NB * SP : ss;
-  bf16 *const yl = es + NB * SP, *const ol = yl + NU * UP;  // Y and dO if kAll
+  bf16 *const us = slice, *const ss = slice + NO * UP, *const es = kAll ? ss + NB * SP : ss;
+  bf16 *const yl = es + NB * SP, *const ol = yl + NO * UP;  // Y and dO if kAll
   bf16 *const ms = slice, *const bs = kAll ? slice + NB * MP : slice;
 
   const int64_t slot = blockIdx.x / a.hk;
@@ -388,7 +388,7 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
     for (int i = tid; i < a.dvp / 4; i += kThreads) se += a.dots[slot_head * (a.dvp / 4) + i];
     for (int v0 = 0; v0 < a.dvp; v0 += 32) {
       Frag<NI> fo;
-      Frag<NU> fy;
+      Frag<NO> fy;
       const Raw8<Saved> late = re;
       if (has_s) {
         put_frag<NB>(ss + sx * LDS + sv, SP, frag_of<NB>(rs));
@@ -398,7 +398,7 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
         Raw8<float> u;
 #pragma unroll
         for (int i = 0; i < 8; i++) u.x[i] = sizeof(Kept) < 4 ? scale * float(ru.x[i]) : float(ru.x[i]);
-        put_frag<NU>((second ? yl : us) + ux * LDS + sv, UP, frag_of<NU>(u));
+        put_frag<NO>((second ? yl : us) + ux * LDS + sv, UP, frag_of<NO>(u));
         const Raw8<T> x = keep_head8<A>(ro, c, ux, v0 + sv, a.dv);
         if (second) {
 #pragma unroll
@@ -407,9 +407,9 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
           put_frag<NI>(ol + ux * LDS + sv, UP, frag_of<NI>(x));
         }
       } else {
-        if (!second) put_frag<NU>(us + ux * LDS + sv, UP, frag_of<NU>(ru));
+        if (!second) put_frag<NO>(us + ux * LDS + sv, UP, frag_of<NO>(ru));
         fo = frag_of<NI>(keep_head8<A>(ro, c, t, v0 + 8 * quad, a.dv));
-        fy = frag_of<NU>(ry);
+        fy = frag_of<NO>(ry);
         const Raw8<T> v = keep_head8<A>(rv, c, t, v0 + 8 * quad, a.dv);
 #pragma unroll
         for (int i = 0; i < 8; i++) yv += ry.x[i] * float(v.x[i]);
@@ -418,9 +418,9 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
       if (v0 + 32 < a.dvp) fetch(v0 + 32);
       if (kAll) {
         fo = frag_row<NI>(ol, UP, LDS, 16 * wr, 0);
-        fy = frag_row<NU>(yl, UP, LDS, 16 * wr, 0);
+        fy = frag_row<NO>(yl, UP, LDS, 16 * wr, 0);
       }
-      const Frag<NU> fu = frag_row<NU>(us, UP, LDS, 16 * wr, 0);
+      const Frag<NO> fu = frag_row<NO>(us, UP, LDS, 16 * wr, 0);
 #pragma unroll
       for (int j = 0; j < JK; j++) {
         const int x = 16 * (JK * part + j);
@@ -432,7 +432,7 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
 #pragma unroll
       for (int j = 0; j < JS; j++)
         if (JS * part + j <= wr) {
-          const Frag<NU> f = frag_row<NU>(us, UP, LDS, 16 * (JS * part + j), 0);
+          const Frag<NO> f = frag_row<NO>(us, UP, LDS, 16 * (JS * part + j), 0);
           ou[j] = mma(ou[j], f, fo);
           yu[j] = mma(yu[j], f, fy);
         }

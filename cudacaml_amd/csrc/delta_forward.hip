@@ -28,7 +28,7 @@ template <typename M, int DK, int BV, bool Back, int A>
 __global__ __launch_bounds__(256, groups_a_unit<M>(DK, BV)) void delta_forward(const DeltaArgs a, int blocks) {
   typedef typename M::T T;
   typedef typename M::Saved Saved;
-  constexpr int NI = M::NI, NS = M::NS, NO = M::NO, NU = M::NU;
+  constexpr int NI = M::NI, NS = M::NS, NO = M::NO;
   constexpr int LDK = DK + 16, LDV = BV == 16 ? 24 : BV;
   constexpr int KP = 64 * LDK, SP = DK * LDV, XP = 64 * LDV;
   constexpr int TK = DK / 64, TV = BV / 16;  // 16 x 16 tiles of S a wave holds
@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256, groups_a_unit<M>(DK, BV)) void delta_forward(c
   // two sets of keys where LDS has room: the next chunk's are written while
   // slower waves still read this one's
   constexpr int kSets = NI == 1 ? 2 : 1;
-  __shared__ __align__(16) bf16 keys[kSets * NI * KP], ss[NS * SP], xs[NS * XP], us[NU * XP], gs[NS * XP];
+  __shared__ __align__(16) bf16 keys[kSets * NI * KP], ss[NS * SP], xs[NS * XP], us[NO * XP], gs[NS * XP];
 
   // heads 8 apart share a chiplet's L2: a head's column blocks, which read
   // the same q, k, T and P, are 8 workgroups apart
@@ -207,7 +207,7 @@ __global__ __launch_bounds__(256, groups_a_unit<M>(DK, BV)) void delta_forward(c
     fetch_t(next);
 #pragma unroll
     for (int j = 0; j < TV; j++) {
-      put_four<NU>(us + t * LDV + y0 + 4 * j, XP, u[j]);
+      put_four<NO>(us + t * LDV + y0 + 4 * j, XP, u[j]);
       put_four<NS>(gs + t * LDV + y0 + 4 * j, XP, last * u[j]);
     }
     if (Back) keep_block<typename M::Kept, TV>(a.us, a.u_scales, (sq.slot + ci) * a.hv + h, a.dvp, dv0, t, quad, y0, u);
@@ -215,7 +215,7 @@ __global__ __launch_bounds__(256, groups_a_unit<M>(DK, BV)) void delta_forward(c
     {
       Frag<NS> fg[2][TV];
       Frag<NI> fk[2][TK];
-      Frag<NU> fu[2][TV];
+      Frag<NO> fu[2][TV];
 #pragma unroll
       for (int b = 0; b < 2; b++) {
 #pragma unroll
@@ -223,7 +223,7 @@ __global__ __launch_bounds__(256, groups_a_unit<M>(DK, BV)) void delta_forward(c
 #pragma unroll
         for (int i = 0; i < TK; i++) fk[b][i] = frag_col<NI>(ks, KP, LDK, w * (DK / 4) + 16 * i, 32 * b);
 #pragma unroll
-        for (int j = 0; j < TV; j++) fu[b][j] = frag_v<NU, TV>(us, XP, LDV, j, 32 * b);
+        for (int j = 0; j < TV; j++) fu[b][j] = frag_v<NO, TV>(us, XP, LDV, j, 32 * b);
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll

@@ -489,7 +489,7 @@ __global__ __launch_bounds__(256, 4) void norm_sums(const NormArgs a) {
   load_params<T>(t, a.channel_scale, a.weights_f32, c, n, 1.0f);
   if (Bias) load_params<T>(b, a.post_bias, a.weights_f32, c, n, 0.0f);
   if (Pre) load_params<T>(pw, a.pre_weight, a.weights_f32, c, n, 1.0f);
-  for (uint32_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
     Raw8<T> ry, rz, rh, rdh, rdn;
     if (Pre) rh = load8<T>(row_at<T>(a.h, row) + c, n);
     if (Pre) rdn = load8<T>(row_at<T>(a.dn, row) + c, n);
@@ -497,7 +497,7 @@ __global__ __launch_bounds__(256, 4) void norm_sums(const NormArgs a) {
     ry = load8<T>(row_at<T>(a.y, row) + c, n);
     if (Gate) rz = load8<T>(row_at<T>(a.gate, row) + c, n);
     const RowStat s = a.stats[row];
-    const uint32_t bits = a.drop.bar ? keep_bits(a.drop, offset, row, group) : 0xFFu;
+    const uint32_t bits = a.drop.bar ? keep_bits(a.drop, offset, uint32_t(row), group) : 0xFFu;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       float d = float(rdh.x[i]);
@@ -532,7 +532,9 @@ void norm_backward_launch(const NormArgs &a, bool bias, int groups, hipStream_t 
 // Rows a workgroup takes at a time for a width.
 inline int rows_at_a_time(int width) { return width <= 128 ? 16 : width <= 512 ? 4 : 1; }
 
-// Threads of a workgroup: a wave for each 512 columns where a row is one's.
+// Threads of a workgroup: a wave for each 512 columns where a row is one's
+// (the backward pass of 65536 rows of 1000 takes 404 us in two waves, 670 in
+// four of which two have no columns).
 inline int threads_of(int width) { return width <= 512 ? 256 : width <= 8192 ? (width + 511) / 512 * 64 : 1024; }
 
 // Workgroups that take `rows` evenly, `least` at least each, as many as run
