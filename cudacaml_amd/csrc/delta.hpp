@@ -429,9 +429,9 @@ void delta_step_launch(const cchip_gated_delta &op, const DeltaArgs &a, hipStrea
 // Whether forward and reverse take 16 value columns a workgroup and not 32:
 // where so many workgroups still find a unit each, as a chunk of 16 columns
 // takes less time than one of 32 (forward of 16384 tokens, 32 bf16 heads of
-// 128: 515 us in 256 workgroups, 855 in 128). Beyond that 32 do more at once:
-// forward and reverse of 3 x 4096 tokens, 16 heads, take 508 us in 192
-// workgroups and 555 in 384, of 4 x 4096 and 32 heads 750 and 1080.
+// 128: 570 us in 256 workgroups, 878 in 128). Beyond that 32 do more at once:
+// forward and reverse of 3 x 4096 tokens, 16 heads, take 533 us in 192
+// workgroups and 573 in 384, of 4 x 4096 and 32 heads 767 and 1107.
 inline bool narrow_blocks(const DeltaArgs &a) { return a.sequences * a.hv * ((a.dv + 31) / 32) <= 128; }
 
 // Workgroups of delta_forward and delta_reverse a unit is to hold: two where
@@ -450,10 +450,10 @@ void with_bool(bool x, F &&f) {
   else f(std::false_type());
 }
 
-// Calls f with how the heads of an operator are read. The four kernels of a
-// bf16 training step of 2 x 4096 tokens, 8 heads of 100 x 100, take 458 us in
-// pieces and 1086 us an element at a time; of an f32 step of 2 x 2048 tokens,
-// 8 heads of 70 x 90, 461 and 668. Whole heads spare the shifts: 8 heads of
+// Calls f with how the heads of an operator are read. The four kernels of an
+// f32 training step of 2 x 2048 tokens, 8 heads of 70 x 90, take 461 us in
+// pieces and 668 us an element at a time; of a bf16 step of 2 x 4096 tokens, 8
+// heads of 100 x 100, 464 and over 1080. Whole heads spare the shifts: 8 heads of
 // 72 x 100 of 5003 tokens in f32 take 497 us whole and 565 in pieces.
 template <typename T, typename F>
 void with_access(const DeltaArgs &a, F &&f) {

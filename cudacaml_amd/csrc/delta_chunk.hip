@@ -50,8 +50,8 @@ __device__ __forceinline__ void put_block(float *to, const f32x4 &c, float sign)
 // time. All of it is f32: entries of T add up 64 products deep, and every
 // state after the chunk carries what they lose. The substitution's 15 steps,
 // each on the last, bound it, and three workgroups a unit cover each other's:
-// 155 us for 256 chunks of 32 bf16 heads of 128 with what the backward pass
-// reads (0.6 GB, 3.9 TB/s), 134 us with f32 states and no backward pass.
+// 163 us for 256 chunks of 32 bf16 heads of 128 with what the backward pass
+// reads (0.67 GB, 4.1 TB/s), 142 us with f32 states and no backward pass.
 template <typename M, int DK, bool Back, int A>
 __global__ __launch_bounds__(256) void delta_chunk(const DeltaArgs a) {
   typedef typename M::T T;

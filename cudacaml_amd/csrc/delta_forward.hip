@@ -18,11 +18,11 @@ namespace {
 // memory answers while the chain of products, three waits for the other
 // waves long, goes on.
 //
-// That chain bounds it where workgroups have a unit each: 2 us a chunk (515
+// That chain bounds it where workgroups have a unit each: 2.2 us a chunk (570
 // us for 16384 tokens, 32 bf16 heads of 128 with f32 states; their bytes take
-// 84). With two a unit (4 x 4096 tokens, saving for a backward pass, 365 us)
-// it moves 0.9 GB of records, tokens, states and U at 2.5 TB/s and makes 8.4
-// MFLOP of products a chunk and head, in planes twice that, at a quarter of
+// 84). With two a unit (4 x 4096 tokens, saving for a backward pass, 376 us)
+// it moves 0.95 GB of records, tokens, states and U at 2.5 TB/s and makes 8.4
+// MFLOP of products a chunk and head, in planes over twice that, at a third of
 // the matrix rate: neither is at its limit, the waits between are the rest.
 template <typename M, int DK, int BV, bool Back, int A>
 __global__ __launch_bounds__(256, groups_a_unit<M>(DK, BV)) void delta_forward(const DeltaArgs a, int blocks) {
