@@ -3,11 +3,18 @@ delta rule, the norm block and dropout, over the C-ABI of
 ``include/cchip_operators.h`` (which states what each computes).
 
 A handle is made once for its shapes, checks the arguments of each call and
-keeps the workspace, one for each stream it is called on. A call only issues
-work on ``stream`` (a ``runtime.Stream``, an object with ``cuda_stream``, a
-raw pointer, or None for the default stream) and may be captured into a HIP
-graph once the handle has its workspace there (``reserve``, or an earlier
-call); the arrays it is given have to live until the stream is past it.
+keeps the workspaces, one for each direction and stream it is called on; they
+stay where they are until ``free``. A call only issues work on ``stream`` (a
+``runtime.Stream``, an object with ``cuda_stream``, a raw pointer, or None for
+the default stream) and may be captured into a HIP graph once the handle has
+its workspace there (``reserve``, or an earlier call); the arrays it is given
+have to live until the stream is past it.
+
+A graph uses the workspace that its call was captured with: the handle has to
+outlive the graph, and a replay must not run while another replay or a call
+on the capture stream uses the same workspace. A call with a ``workspace`` of
+the caller's own (u8, ``workspace_bytes`` at least, aligned to 16 bytes) is
+free of both.
 
 Arrays are ``Array``, ``backend_hip.Resident`` or anything with ``data_ptr()``,
 ``get_device()``, ``dtype``, ``shape`` and ``stride()``, such as a tensor of
@@ -142,19 +149,31 @@ class _Operator:
             raise ValueError("%s: %s is not contiguous" % (self._who, name))
         return p
 
-    def _workspace(self, stream, nbytes):
-        """A workspace of at least nbytes of the stream's own."""
-        if not nbytes:
-            return None
-        w = self._workspaces.get(stream)
-        if w is None or w.nbytes < nbytes:
-            if w is not None:
-                w.free()  # hipFree waits for the work that uses it
-            w = self._workspaces[stream] = Buffer.alloc(nbytes)
-        return w.ptr
+    _forward_bytes = 0
+    _backward_bytes = 0
+
+    def workspace_bytes(self, backward=False):
+        """Bytes of workspace that a call of a direction needs."""
+        return self._backward_bytes if backward else self._forward_bytes
+
+    def _workspace(self, stream, backward=False, given=None):
+        """The pointer and bytes of a call's workspace: the one given, or the
+        stream's own for this direction. That one is never replaced, as a
+        captured graph may hold it."""
+        n = self.workspace_bytes(backward)
+        if given is not None:
+            have = given.shape[0] if len(given.shape) == 1 else 0
+            return self._whole("workspace", given, "u8", (have,)), have
+        if not n:
+            return None, 0
+        w = self._workspaces.get((stream, backward))
+        if w is None:
+            w = self._workspaces[stream, backward] = Buffer.alloc(n)
+        return w.ptr, n
 
     def free(self):
-        """Free the workspaces; the streams have to be done with them."""
+        """Free the workspaces; streams and captured graphs have to be done
+        with them."""
         for w in self._workspaces.values():
             w.free()
         self._workspaces.clear()
@@ -216,8 +235,10 @@ class GatedDelta(_Operator):
         return Array.empty("u8", (self._saved_bytes,))
 
     def reserve(self, stream=None, backward=False):
-        """Allocate a stream's workspace ahead of the first call on it."""
-        self._workspace(_stream_ptr(stream), max(self._forward_bytes, self._backward_bytes if backward else 0))
+        """Allocate a stream's workspace for forward calls, and that for
+        backward calls, ahead of the first of them."""
+        for back in (False, True)[:1 + bool(backward)]:
+            self._workspace(_stream_ptr(stream), back)
 
     def _words(self, **given):
         """Pointer and three strides of each array. The loop does in one go what
@@ -251,7 +272,8 @@ class GatedDelta(_Operator):
     def _kept(self, saved):
         return self._whole("saved", saved, "u8", (self._saved_bytes,))
 
-    def forward(self, q, k, v, g, beta, o, *, state=None, state_out=None, offsets=None, saved=None, stream=None):
+    def forward(self, q, k, v, g, beta, o, *, state=None, state_out=None, offsets=None, saved=None, workspace=None,
+                stream=None):
         """Write ``o``, and the sequences' last states to ``state_out`` if given
         (it may be ``state``, where they begin; without one, at zero).
         ``saved`` is written for a backward pass if given."""
@@ -259,24 +281,24 @@ class GatedDelta(_Operator):
         s = _stream_ptr(stream)
         io = self._forward_io.pack(*words, self._bounds(offsets), self._whole("state", state, "f32", self._state),
                                    self._whole("state_out", state_out, "f32", self._state), 0, 0, self._kept(saved))
-        n = 0 if saved is not None else self._forward_bytes
-        rc = lib().cchip_gated_delta_forward(self._desc, io, self._workspace(s, n) if n else None, n, s)
+        w, n = (None, 0) if saved is not None or not self._forward_bytes else self._workspace(s, False, workspace)
+        rc = lib().cchip_gated_delta_forward(self._desc, io, w, n, s)
         if rc:
             check(rc)
 
     def backward(self, q, k, v, g, beta, do, saved, dq, dk, dv, dg, dbeta, *, dstate_out=None, dstate=None, offsets=None,
-                 stream=None):
+                 workspace=None, stream=None):
         """From the gradients of ``o`` and of the last states (None: zero) write
         those of q, k, v, g, beta, and of the first states to ``dstate`` if
         given. ``saved`` is what ``forward`` wrote for the same inputs."""
         if saved is None:
             raise ValueError("GatedDelta: the backward pass needs what the forward pass saved")
         words = self._words(q=q, k=k, v=v, g=g, beta=beta, do=do, dq=dq, dk=dk, dv=dv, dg=dg, dbeta=dbeta)
-        s, n = _stream_ptr(stream), self._backward_bytes
+        s = _stream_ptr(stream)
         io = self._backward_io.pack(*words, self._bounds(offsets), 0, 0,
                                     self._whole("dstate_out", dstate_out, "f32", self._state),
                                     self._whole("dstate", dstate, "f32", self._state), self._kept(saved))
-        check(lib().cchip_gated_delta_backward(self._desc, io, self._workspace(s, n), n, s))
+        check(lib().cchip_gated_delta_backward(self._desc, io, *self._workspace(s, True, workspace), s))
 
 
 class _RowOperator(_Operator):
@@ -374,7 +396,7 @@ class NormBlock(_RowOperator):
 
     def reserve(self, stream=None):
         """Allocate a stream's workspace ahead of the first backward call on it."""
-        self._workspace(_stream_ptr(stream), self._backward_bytes)
+        self._workspace(_stream_ptr(stream), True)
 
     def _vectors(self, given):
         p = [0, 0, 0, 0, 0]
@@ -394,7 +416,7 @@ class NormBlock(_RowOperator):
         check(lib().cchip_norm_block_forward(self._desc, io, _stream_ptr(stream)))
 
     def backward(self, y, dh, dy, *, dn=None, h=None, gate=None, dgate=None, dresidual=None, grads=None, seed=0, offset=0,
-                 step=None, stream=None, **params):
+                 step=None, workspace=None, stream=None, **params):
         """From y, gate, the forward pass's h (where it is normed again) and the
         gradients of h and n, write those of y, gate and residual and, for each
         name in ``grads``, of that parameter, summed over the rows."""
@@ -403,5 +425,5 @@ class NormBlock(_RowOperator):
                            *self._needed("y", y), *self._rows("gate", gate), 0, 0, *self._rows("h", h), 0, 0,
                            *self._needed("dh", dh), *self._rows("dn", dn), *self._needed("dy", dy),
                            *self._rows("dgate", dgate), *self._rows("dresidual", dresidual))
-        n = self._backward_bytes if grads else 0
-        check(lib().cchip_norm_block_backward(self._desc, io, self._workspace(s, n), n, s))
+        w, n = self._workspace(s, True, workspace) if grads else (None, 0)
+        check(lib().cchip_norm_block_backward(self._desc, io, w, n, s))

@@ -700,3 +700,65 @@ def test_the_example_learns_and_serves(device):
 
     gc.collect()
     assert Buffer.live_count() <= live
+
+
+# ---- workspaces of captured calls --------------------------------------------
+
+def test_a_graph_keeps_its_workspace(device):
+    """A captured forward pass with eager backward passes of the same handle on
+    the same stream between its replays, which need a larger workspace."""
+    shape = (2, 130, 1, 2, 64, 64)
+    op = O.GatedDelta("bf16", *shape, states=False)
+    one, two = (arrays("bf16", *shape, seed=s, back=True) for s in (31, 32))
+    want = [run_delta(x, "bf16", back=True) for x in (one, two)]
+    dev = {k: v.cuda() for k, v in one.items()}
+    names = ("q", "k", "v", "g", "beta")
+    o = torch.empty_like(dev["v"])
+    stream = torch.cuda.Stream()
+    op.reserve(stream)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        op.forward(*(dev[n] for n in names), o, stream=stream)
+    for i in (0, 1, 0, 1):
+        for n, v in (one, two)[i].items():
+            dev[n].copy_(v)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, want[i]["o"]), i
+        with torch.cuda.stream(stream):
+            got = run_delta(two, "bf16", back=True, handle=op, stream=stream)
+            run_delta(two, "bf16", handle=op, stream=stream)
+        for n in got:
+            assert torch.equal(got[n], want[1][n]), n
+
+
+def test_a_graph_with_the_callers_workspace(device):
+    """Such a graph outlives its handle and may run on any stream, with calls
+    on the capture stream next to it."""
+    shape = (2, 130, 1, 2, 64, 64)
+    op = O.GatedDelta("f32", *shape, states=False)
+    x = arrays("f32", *shape, seed=33)
+    want = run_delta(x, "f32")["o"]
+    dev = {k: v.cuda() for k, v in x.items()}
+    o = torch.empty_like(want)
+    work = torch.empty(op.workspace_bytes(), dtype=torch.uint8, device="cuda")
+    stream, other = torch.cuda.Stream(), torch.cuda.Stream()
+    live = Buffer.live_count()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        op.forward(*dev.values(), o, workspace=work, stream=stream)
+    assert Buffer.live_count() == live
+    op.free()
+    del op
+    for _ in range(3):
+        o.fill_(float("nan"))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(other):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, want)
+        with torch.cuda.stream(stream):
+            assert torch.equal(run_delta(x, "f32", stream=stream)["o"], want)

@@ -295,3 +295,67 @@ def test_reference_gradients_against_differences():
             r = g.standard_normal(y[n].shape)
             want = _difference(lambda a: loss(**{n: a}), y[n], r)
             assert abs((d[n] * r).sum() - want) < 1e-6 * max(1.0, abs(want)), (post, n)
+
+
+# ---- workspaces --------------------------------------------------------------
+
+class _Memory:
+    """Buffers of host addresses, in the order they are made."""
+
+    made = []
+
+    def __init__(self, nbytes):
+        self.ptr, self.nbytes, self.freed = 4096 * (len(self.made) + 1), nbytes, False
+        self.made.append(self)
+
+    def free(self):
+        self.freed = True
+
+
+@pytest.fixture
+def memory(monkeypatch):
+    monkeypatch.setattr(_Memory, "made", [])
+    monkeypatch.setattr(O.Buffer, "alloc", staticmethod(_Memory))
+    return _Memory.made
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_a_workspace_stays_where_a_graph_may_hold_it(memory, dtype):
+    """A backward pass that needs more than a forward call leaves the forward
+    call's workspace alone: a graph captured with it may be replayed yet."""
+    op = O.GatedDelta(dtype, 1, 4096, 8, 32, 128, 128)
+    assert op.workspace_bytes(backward=True) > op.workspace_bytes() > 0
+    op.reserve(77)
+    held = op._workspace(77)
+    op.reserve(77, backward=True)
+    assert op._workspace(77) == held and op._workspace(77, True) != held
+    assert not any(m.freed for m in memory)
+    assert [m.nbytes for m in memory] == [op.workspace_bytes(), op.workspace_bytes(backward=True)]
+    op._workspace(78)
+    assert len(memory) == 3  # another stream's is its own
+    op.free()
+    assert all(m.freed for m in memory)
+
+
+def test_a_callers_workspace(memory):
+    """The caller's memory is handed on, checked, and nothing is allocated."""
+    op = O.GatedDelta("f32", 2, 100, 2, 4, 16, 8, states=False)
+    op._device = -1
+    n = op.workspace_bytes()
+    w = torch.zeros(n + 16, dtype=torch.uint8)
+    assert op._workspace(5, False, w) == (w.data_ptr(), n + 16) and not memory
+    x = _delta_arrays(t=100)
+    with pytest.raises(ValueError, match="workspace needs"):
+        op.forward(*x.values(), workspace=w[:n - 16])
+    with pytest.raises(ValueError, match="workspace needs"):
+        op.forward(*x.values(), workspace=w[8:])
+    with pytest.raises(ValueError, match="workspace has dtype"):
+        op.forward(*x.values(), workspace=torch.zeros(n))
+    block = O.NormBlock("f32", 4, 8)
+    block._device = -1
+    assert block.workspace_bytes() == 0 < block.workspace_bytes(backward=True)
+    z = torch.zeros(4, 8)
+    with pytest.raises(ValueError, match="workspace needs"):
+        block.backward(z, z.clone(), z.clone(), dn=z, h=z, grads=dict(pre_weight=torch.zeros(8)),
+                       workspace=torch.zeros(4, dtype=torch.uint8))
+    assert not memory
