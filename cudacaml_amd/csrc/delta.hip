@@ -78,7 +78,7 @@ Heads heads_of(const cchip_gated_delta &op, const cchip_heads &x, const char *na
   return {static_cast<char *>(x.data), x.batch, x.token, x.head};
 }
 
-DeltaArgs args_of(const cchip_gated_delta &op, const cchip_gated_delta_io &io, bool back) {
+DeltaArgs args_of(const cchip_gated_delta &op, const cchip_gated_delta_io &io, const Layout &p, bool back) {
   DeltaArgs a = {};
   const int hk = op.key_heads, hv = op.value_heads, dk = op.key_dim, dv = op.value_dim;
   a.q = heads_of(op, io.q, "q", false, hk, dk);
@@ -91,7 +91,7 @@ DeltaArgs args_of(const cchip_gated_delta &op, const cchip_gated_delta_io &io, b
   if (!op.states && (io.state || io.state_out || io.dstate || io.dstate_out))
     throw InvalidArgument("gated delta: a state for an operator made without states");
   if (back) {
-    if (!io.saved) throw InvalidArgument("gated delta: the backward pass needs what the forward pass saved");
+    if (!io.saved && p.slots) throw InvalidArgument("gated delta: the backward pass needs what the forward pass saved");
     a.d_o = heads_of(op, io.d_o, "the gradient of o", false, hv, dv);
     a.gq = heads_of(op, io.dq, "dq", true, hk, dk);
     a.gk = heads_of(op, io.dk, "dk", true, hk, dk);
@@ -108,6 +108,7 @@ DeltaArgs args_of(const cchip_gated_delta &op, const cchip_gated_delta_io &io, b
   if (!aligned16(io.saved)) throw InvalidArgument("gated delta: saved is not aligned to 16 bytes");
   a.offsets = io.offsets;
   a.tokens = op.tokens;
+  a.slots = p.slots;
   a.sequences = count_sequences(op);
   a.chunks = int((op.tokens + kChunk - 1) / kChunk);
   a.hk = hk;
@@ -151,8 +152,7 @@ int cchip_gated_delta_forward(const cchip_gated_delta *op, const cchip_gated_del
     check_op(op);
     if (!io) throw InvalidArgument("gated delta: no tensors");
     const Layout p = layout_of(*op);
-    DeltaArgs a = args_of(*op, *io, false);
-    a.slots = p.slots;
+    DeltaArgs a = args_of(*op, *io, p, false);
     if (a.sequences == 0) return;
     if (steps(*op, io->saved != nullptr)) return delta_step_launch(*op, a, (hipStream_t)stream);
     if (io->saved) {
@@ -172,8 +172,7 @@ int cchip_gated_delta_backward(const cchip_gated_delta *op, const cchip_gated_de
     check_op(op);
     if (!io) throw InvalidArgument("gated delta: no tensors");
     const Layout p = layout_of(*op);
-    DeltaArgs a = args_of(*op, *io, true);
-    a.slots = p.slots;
+    DeltaArgs a = args_of(*op, *io, p, true);
     if (a.sequences == 0) return;
     lay_out(a, p, static_cast<char *>(io->saved));
     check_workspace(workspace, workspace_bytes, p.states + p.us + p.scales + p.dots);

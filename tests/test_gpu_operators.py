@@ -762,3 +762,16 @@ def test_a_graph_with_the_callers_workspace(device):
         assert torch.equal(o, want)
         with torch.cuda.stream(stream):
             assert torch.equal(run_delta(x, "f32", stream=stream)["o"], want)
+
+
+# ---- nothing to go back through ----------------------------------------------
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", [(2, 0, 1, 2, 32, 32), (3, 0, 2, 2, 100, 40)])
+def test_gated_delta_backward_of_no_tokens(device, dtype, shape):
+    """Rows without tokens: the last states' gradient is that of the first."""
+    x = arrays(dtype, *shape, states=shape[0], back=True)
+    got = run_delta(x, dtype, back=True)
+    assert torch.equal(got["dstate"].cpu(), x["dstate_out"]) and torch.equal(got["state"].cpu(), x["state"])
+    got = run_delta({n: v for n, v in x.items() if n != "dstate_out"}, dtype, back=True)
+    assert not got["dstate"].any()

@@ -297,6 +297,21 @@ def test_reference_gradients_against_differences():
             assert abs((d[n] * r).sum() - want) < 1e-6 * max(1.0, abs(want)), (post, n)
 
 
+def test_backward_of_no_sequences_is_no_error():
+    """A batch of none has nothing saved, and its backward pass nothing to do.
+    Where there are chunks, what the forward pass saved is still asked for."""
+    L, sizes = _lib.lib(), [ctypes.c_size_t() for _ in range(3)]
+    io = bytes(O.GatedDelta._backward_io.size)
+    none = _lib.GatedDeltaDesc(0, 0, 100, 0, 2, 4, 16, 8, 1, 1.0)
+    assert L.cchip_gated_delta_sizes(none, *sizes) == 0 and [s.value for s in sizes] == [0, 0, 0]
+    assert _call(L.cchip_gated_delta_backward, none, io, None, 0, None)[0] == 0
+    t = lambda h=8: (4096, 100 * 4 * h, 4 * h, h)  # noqa: E731
+    some = _lib.GatedDeltaDesc(0, 2, 100, 0, 4, 4, 8, 8, 1, 1.0)
+    words = [*t(), *t(), *t(), *t(1), *t(1), *[w for h in (8, 8, 8, 8, 1, 1) for w in t(h)], *(0,) * 6]
+    rc, msg = _call(L.cchip_gated_delta_backward, some, O.GatedDelta._backward_io.pack(*words), None, 0, None)
+    assert rc == 1 and "what the forward pass saved" in msg
+
+
 # ---- workspaces --------------------------------------------------------------
 
 class _Memory:
