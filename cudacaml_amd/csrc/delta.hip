@@ -78,6 +78,33 @@ Heads heads_of(const cchip_gated_delta &op, const cchip_heads &x, const char *na
   return {static_cast<char *>(x.data), x.batch, x.token, x.head};
 }
 
+// What a call writes is read by other workgroups of the same call, and in the
+// backward pass by later kernels too. Of two tensors whose elements may lie
+// between one another's, those of the first token and head are looked at.
+void check_apart(const cchip_gated_delta &op, const cchip_gated_delta_io &io, bool back) {
+  if (op.batch * op.tokens == 0) return;
+  struct Head {
+    const char *name;
+    const void *data;
+    size_t bytes;
+  };
+  const size_t size = element_size(op), key = size * op.key_dim, value = size * op.value_dim;
+  const Head in[] = {{"q", io.q.data, key}, {"k", io.k.data, key}, {"v", io.v.data, value}, {"g", io.g.data, size},
+                     {"beta", io.beta.data, size}, {"the gradient of o", io.d_o.data, value}};
+  const Head forward[] = {{"o", io.o.data, value}};
+  const Head backward[] = {{"dq", io.dq.data, key}, {"dk", io.dk.data, key}, {"dv", io.dv.data, value}, {"dg", io.dg.data, size},
+                           {"dbeta", io.dbeta.data, size}};
+  const Head *out = back ? backward : forward;
+  for (int i = 0; i < (back ? 5 : 1); i++) {
+    for (int j = 0; j < (back ? 6 : 5); j++)
+      if (meet(out[i].data, out[i].bytes, in[j].data, in[j].bytes))
+        throw InvalidArgument(strf("gated delta: %s is written over %s, which the call reads", out[i].name, in[j].name));
+    for (int j = 0; j < i; j++)
+      if (meet(out[i].data, out[i].bytes, out[j].data, out[j].bytes))
+        throw InvalidArgument(strf("gated delta: %s and %s are written to one place", out[j].name, out[i].name));
+  }
+}
+
 DeltaArgs args_of(const cchip_gated_delta &op, const cchip_gated_delta_io &io, const Layout &p, bool back) {
   DeltaArgs a = {};
   const int hk = op.key_heads, hv = op.value_heads, dk = op.key_dim, dv = op.value_dim;
@@ -154,13 +181,15 @@ int cchip_gated_delta_forward(const cchip_gated_delta *op, const cchip_gated_del
     const Layout p = layout_of(*op);
     DeltaArgs a = args_of(*op, *io, p, false);
     if (a.sequences == 0) return;
-    if (steps(*op, io->saved != nullptr)) return delta_step_launch(*op, a, (hipStream_t)stream);
+    const bool step = steps(*op, io->saved != nullptr);
     if (io->saved) {
       lay_out(a, p, static_cast<char *>(io->saved));
-    } else {
+    } else if (!step) {
       check_workspace(workspace, workspace_bytes, p.record);
       a.records = static_cast<char *>(workspace);
     }
+    check_apart(*op, *io, false);
+    if (step) return delta_step_launch(*op, a, (hipStream_t)stream);
     if (p.slots) delta_chunk_launch(*op, a, io->saved != nullptr, (hipStream_t)stream);
     delta_forward_launch(*op, a, io->saved != nullptr, (hipStream_t)stream);
   });
@@ -176,6 +205,8 @@ int cchip_gated_delta_backward(const cchip_gated_delta *op, const cchip_gated_de
     if (a.sequences == 0) return;
     lay_out(a, p, static_cast<char *>(io->saved));
     check_workspace(workspace, workspace_bytes, p.states + p.us + p.scales + p.dots);
+    check_apart(*op, *io, true);
+    if (p.slots && workspace == io->saved) throw InvalidArgument("gated delta: the workspace is what the forward pass saved");
     a.grads = static_cast<char *>(workspace);
     a.ys = a.grads + p.states;
     a.y_scales = reinterpret_cast<float *>(a.ys + p.us);

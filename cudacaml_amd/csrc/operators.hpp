@@ -277,6 +277,12 @@ __device__ __forceinline__ uint32_t keep_bits(const Drop &d, uint64_t offset, ui
 
 // ---- host side --------------------------------------------------------------
 
+// Whether two stretches of memory share a byte.
+inline bool meet(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + b_bytes && y < x + a_bytes;
+}
+
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 inline void check_launch(const char *what) { check_hip(hipGetLastError(), what); }

@@ -312,6 +312,49 @@ def test_backward_of_no_sequences_is_no_error():
     assert rc == 1 and "what the forward pass saved" in msg
 
 
+def test_gated_delta_refuses_to_write_over_what_it_reads():
+    """Other workgroups and later kernels read q, k, v, g, beta and the
+    gradient of o after the first results are written."""
+    x = _delta_arrays(t=100)
+    op = O.GatedDelta("f32", 2, 100, 2, 4, 16, 8, states=False)
+    op._device = -1
+    names = ("q", "k", "v", "g", "beta")
+    ins = [x[n] for n in names]
+
+    def room(n):
+        whole = torch.zeros(n + 16, dtype=torch.uint8)
+        return whole[-whole.data_ptr() % 16:][:n]
+
+    work, saved = room(op.workspace_bytes(backward=True)), room(op.saved_bytes())
+    with pytest.raises(ValueError, match="o is written over v, which"):
+        op.forward(*ins, x["v"], saved=saved)
+    with pytest.raises(ValueError, match="o is written over v, which"):
+        _one_token(op).forward(*(t[:, :1] for t in ins), x["v"][:, :1])
+
+    def backward(workspace=work, **over):
+        grads = {n: over.get(n, torch.zeros_like(x[n])) for n in names}
+        op.backward(*ins, x["o"], saved, *grads.values(), workspace=workspace)
+
+    for n in names:
+        with pytest.raises(ValueError, match="d%s is written over %s, which" % (n, n)):
+            backward(**{n: x[n]})
+    with pytest.raises(ValueError, match="dv is written over the gradient of o"):
+        backward(v=x["o"])
+    z = torch.zeros_like(x["k"])
+    with pytest.raises(ValueError, match="dq and dk are written to one place"):
+        backward(q=z, k=z)
+    big = room(max(op.workspace_bytes(backward=True), op.saved_bytes()))
+    saved = big[:op.saved_bytes()]
+    with pytest.raises(ValueError, match="the workspace is what"):
+        backward(workspace=big)
+
+
+def _one_token(op):
+    one = O.GatedDelta("f32", 2, 1, 2, 4, 16, 8, states=False)
+    one._device = op._device
+    return one
+
+
 # ---- workspaces --------------------------------------------------------------
 
 class _Memory:
