@@ -37,6 +37,13 @@ __device__ __forceinline__ f32x4 block_product(f32x4 c, const float *x, const fl
   return c;
 }
 
+// What a wave's lanes have written to LDS is there for its other lanes.
+__device__ __forceinline__ void wave_settles() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 __device__ __forceinline__ void put_block(float *to, const f32x4 &c, float sign) {
   const int l = threadIdx.x & 63;
 #pragma unroll
@@ -163,7 +170,7 @@ __global__ __launch_bounds__(256) void delta_chunk(const DeltaArgs a) {
         sum = block_product(sum, am + 16 * w * kPad + 16 * m, tm + 16 * m * kPad + 16 * (w - d));
       float *tmp = am + 16 * (w - d) * kPad + 16 * w;
       put_block(tmp, sum, 1.0f);
-      __builtin_amdgcn_wave_barrier();
+      wave_settles();
       f32x4 t = {};
       t = block_product(t, tm + 16 * w * kPad + 16 * w, tmp);
       put_block(tm + 16 * w * kPad + 16 * (w - d), t, -1.0f);

@@ -775,3 +775,18 @@ def test_gated_delta_backward_of_no_tokens(device, dtype, shape):
     assert torch.equal(got["dstate"].cpu(), x["dstate_out"]) and torch.equal(got["state"].cpu(), x["state"])
     got = run_delta({n: v for n, v in x.items() if n != "dstate_out"}, dtype, back=True)
     assert not got["dstate"].any()
+
+
+# ---- the triangular systems --------------------------------------------------
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("dims", [(64, 32), (128, 64), (40, 20)])
+def test_gated_delta_inverses_reach_across_a_chunk(device, dtype, dims):
+    """Equal keys, rates of 0.05 and hardly a decay: (I + A)^-1 falls by 5% a
+    token, so that every block of it, the one 48 tokens off the diagonal too,
+    is in the results."""
+    x = arrays(dtype, 2, 130, 1, 2, *dims, seed=34, states=2, back=True)
+    x["k"] = x["k"][:, :1].expand_as(x["k"]).clone()
+    x["beta"].fill_(0.05)
+    x["g"].fill_(-1e-3)
+    check_delta(x, dtype, back=True)
