@@ -121,8 +121,10 @@ __global__ __launch_bounds__(256) void delta_chunk(const DeltaArgs a) {
     for (int j = 0; j < 4; j++)
       if (j <= w) {
         const Frag<NI> fs = frag_row<NI>(ks, KPlane, LD, 16 * j, d);
-        kk[j] = mma(kk[j], fk, fs);
-        qk[j] = mma(qk[j], fq, fs);
+        // T and P^T go into f32 states: products of f16 inputs are whole
+        constexpr int kLevels = NI == 2 ? 3 : 0;
+        kk[j] = mma<kLevels>(kk[j], fk, fs);
+        qk[j] = mma<kLevels>(qk[j], fq, fs);
       }
   }
   float *pm = reinterpret_cast<float *>(ks);  // the keys are done with

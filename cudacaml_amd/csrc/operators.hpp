@@ -143,12 +143,14 @@ __device__ __forceinline__ Frag<N> frag_col(const bf16 *m, int plane, int ld, in
 }
 
 // c += a b^T over 32 terms. Planes i and j are multiplied while i + j is
-// below the larger count: the terms left out are as small as what splitting
-// dropped. Small terms first. Lane l holds rows 4 (l / 16) .. + 3 of column
-// l % 16.
-template <int NA, int NB>
+// below `Levels`: the larger count of planes unless given, which leaves out
+// terms of at most 2^-18 of a product for two planes (as small as what two
+// drop of an f32) and 2^-27 for three. Two planes hold an f16 whole, and with
+// Levels 3 its products are exact too. Small terms first. Lane l holds rows
+// 4 (l / 16) .. + 3 of column l % 16.
+template <int Levels = 0, int NA, int NB>
 __device__ __forceinline__ f32x4 mma(f32x4 c, const Frag<NA> &a, const Frag<NB> &b) {
-  constexpr int M = NA > NB ? NA : NB;
+  constexpr int M = Levels ? Levels : NA > NB ? NA : NB;
 #pragma unroll
   for (int s = M - 1; s >= 0; s--)
 #pragma unroll
