@@ -43,12 +43,14 @@ int padded_value_dim(const cchip_gated_delta &op) { return (op.value_dim + 31) /
 
 Layout layout_of(const cchip_gated_delta &op) {
   Layout p;
-  // batch and sequences below 2^31, so nothing here overflows
-  if (op.batch >= (int64_t(1) << 31) || op.sequences >= (int64_t(1) << 31)) throw InvalidArgument("gated delta: too many sequences");
+  // batch and sequences below 2^31 and heads of all of them too, so nothing here overflows
+  if (op.batch >= (int64_t(1) << 31) || op.sequences >= (int64_t(1) << 31) || count_sequences(op) * op.value_heads > INT32_MAX)
+    throw InvalidArgument("gated delta: too many sequences and heads for a launch");
   p.slots = op.sequences ? op.tokens / kChunk + op.sequences : op.batch * ((op.tokens + kChunk - 1) / kChunk);
+  if (p.slots > INT32_MAX) throw InvalidArgument("gated delta: more chunks than a launch can have");
   p.slot_heads = p.slots * op.value_heads;
   const int64_t blocks = padded_value_dim(op) / 16;
-  if (p.slots > INT32_MAX || p.slot_heads > INT32_MAX || (count_sequences(op) * op.value_heads + 8) * blocks > INT32_MAX)
+  if (p.slot_heads > INT32_MAX || (count_sequences(op) * op.value_heads + 8) * blocks > INT32_MAX)
     throw InvalidArgument("gated delta: more chunks, heads and value columns than a launch can have");
   with_mode(op, [&](auto m) {
     typedef decltype(m) M;

@@ -44,8 +44,8 @@ __global__ __launch_bounds__(256, groups_a_unit<M>(DK, BV)) void delta_reverse(c
   __shared__ __align__(16) bf16 ks[NI * KP], qs[NI * KP], es[NS * EP], xs[NS * XP], os[NI * XP], gs[NS * XP];
   bf16 *const zs = es;  // E is done with when Z is made
 
-  const int64_t group = blockIdx.x / (8 * blocks);
-  const int rest = int(blockIdx.x - group * 8 * blocks);
+  const int64_t group = block_index() / (8 * blocks);
+  const int rest = int(block_index() - group * 8 * blocks);
   const int64_t lane_id = group * 8 + rest % 8;
   if (lane_id >= a.sequences * a.hv) return;
   const int64_t sid = lane_id / a.hv;
@@ -293,8 +293,9 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
   bf16 *const yl = es + NB * SP, *const ol = yl + NO * UP;  // Y and dO if kAll
   bf16 *const ms = slice, *const bs = kAll ? slice + NB * MP : slice;
 
-  const int64_t slot = blockIdx.x / a.hk;
-  const int hk = int(blockIdx.x - slot * a.hk), per = a.hv / a.hk;
+  const int64_t slot = block_index() / a.hk;
+  if (slot >= a.slots) return;
+  const int hk = int(block_index() - slot * a.hk), per = a.hv / a.hk;
   const Chunk c = chunk_of(a, slot);
   if (c.len == 0) return;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, quad = l >> 4, col = l & 15;
@@ -580,9 +581,9 @@ void delta_backward_launch(const cchip_gated_delta &op, const DeltaArgs &a, hipS
     const int blocks = a.dvp / BV;  // what pads a head is written too
     with_access<typename M::T>(a, [&](auto f) {
       constexpr int F = decltype(f)::value;
-      hipLaunchKernelGGL((delta_reverse<M, DK, BV, F>), dim3(unsigned((lanes + 7) / 8 * 8 * blocks)), dim3(256), 0, stream,
+      hipLaunchKernelGGL((delta_reverse<M, DK, BV, F>), grid_of((lanes + 7) / 8 * 8 * blocks), dim3(256), 0, stream,
                          a, blocks);
-      if (a.slots) hipLaunchKernelGGL((delta_gradients<M, DK, F>), dim3(unsigned(a.slots * a.hk)), dim3(512), 0, stream, a);
+      if (a.slots) hipLaunchKernelGGL((delta_gradients<M, DK, F>), grid_of(a.slots * a.hk), dim3(512), 0, stream, a);
     });
   };
   with_mode(op, [&](auto m) {

@@ -69,8 +69,9 @@ __global__ __launch_bounds__(256) void delta_chunk(const DeltaArgs a) {
   __shared__ double cs[64];
   __shared__ float bs[64];
 
-  const int64_t slot = blockIdx.x / a.hv;
-  const int h = int(blockIdx.x - slot * a.hv), hk = h / (a.hv / a.hk);
+  const int64_t slot = block_index() / a.hv;
+  if (slot >= a.slots) return;
+  const int h = int(block_index() - slot * a.hv), hk = h / (a.hv / a.hk);
   const Chunk c = chunk_of(a, slot);
   if (c.len == 0) return;
   char *rec = a.records + (slot * a.hv + h) * R::bytes(Back);
@@ -196,7 +197,7 @@ void delta_chunk_launch(const cchip_gated_delta &op, const DeltaArgs &a, bool ba
         constexpr bool B = decltype(b)::value;
         constexpr int F = decltype(f)::value;
         auto *k = a.dk <= 64 ? delta_chunk<M, 64, B, F> : delta_chunk<M, 128, B, F>;
-        hipLaunchKernelGGL(k, dim3(unsigned(grid)), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(k, grid_of(grid), dim3(256), 0, stream, a);
       });
     });
   });

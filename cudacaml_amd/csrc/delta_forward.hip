@@ -40,8 +40,8 @@ __global__ __launch_bounds__(256, groups_a_unit<M>(DK, BV)) void delta_forward(c
 
   // heads 8 apart share a chiplet's L2: a head's column blocks, which read
   // the same q, k, T and P, are 8 workgroups apart
-  const int64_t group = blockIdx.x / (8 * blocks);
-  const int rest = int(blockIdx.x - group * 8 * blocks);
+  const int64_t group = block_index() / (8 * blocks);
+  const int rest = int(block_index() - group * 8 * blocks);
   const int64_t lane_id = group * 8 + rest % 8;
   if (lane_id >= a.sequences * a.hv) return;
   const int64_t sid = lane_id / a.hv;
@@ -284,7 +284,7 @@ void delta_forward_launch(const cchip_gated_delta &op, const DeltaArgs &a, bool 
     with_bool(back, [&](auto b) {
       with_access<typename M::T>(a, [&](auto f) {
         hipLaunchKernelGGL((delta_forward<M, DK, BV, decltype(b)::value, decltype(f)::value>),
-                           dim3(unsigned((lanes + 7) / 8 * 8 * blocks)), dim3(256), 0, stream, a, blocks);
+                           grid_of((lanes + 7) / 8 * 8 * blocks), dim3(256), 0, stream, a, blocks);
       });
     });
   };

@@ -27,10 +27,11 @@ __device__ __forceinline__ f32x4 load_state4(const float *p, int n, bool vec) {
 template <typename T, int ROWS>
 __global__ __launch_bounds__(256) void delta_step(const DeltaArgs a, int blocks, bool vec) {
   __shared__ float qs[2][ROWS * 32], ks[2][ROWS * 32], part[2][4][2 * kColumns + 1];
-  const int64_t lane_id = blockIdx.x / blocks;
+  const int64_t lane_id = block_index() / blocks;
+  if (lane_id >= a.sequences * a.hv) return;
   const int64_t row = lane_id / a.hv;
   const int h = int(lane_id - row * a.hv), hk = h / (a.hv / a.hk);
-  const int v0 = int(blockIdx.x - lane_id * blocks) * kColumns;
+  const int v0 = int(block_index() - lane_id * blocks) * kColumns;
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, y = v0 + tid % 8 * 4, n = a.dv - y;
 
   f32x4 s[ROWS];
@@ -118,7 +119,7 @@ void delta_step_launch(const cchip_gated_delta &op, const DeltaArgs &a, hipStrea
   auto launch = [&](auto t) {
     typedef decltype(t) T;
     auto *k = a.dk <= 64 ? delta_step<T, 2> : delta_step<T, 4>;
-    hipLaunchKernelGGL(k, dim3(unsigned(a.sequences * a.hv * blocks)), dim3(256), 0, stream, a, blocks, vec);
+    hipLaunchKernelGGL(k, grid_of(a.sequences * a.hv * blocks), dim3(256), 0, stream, a, blocks, vec);
   };
   if (op.dtype == CCHIP_F32) launch(float());
   else if (op.dtype == CCHIP_F16) launch(f16());

@@ -14,7 +14,7 @@ namespace {
 struct DropoutArgs {
   Rows x, residual, out;
   uint64_t groups;   // rows times groups of 8 columns
-  uint32_t per_row;  // groups a row
+  uint64_t per_row;  // groups a row, up to 2^32
   int64_t cols;
   float scale;
   Drop drop;
@@ -28,9 +28,9 @@ struct DropoutArgs {
 // over a copy's 4.9 as the second finds some of its input in the cache.
 template <typename T>
 __global__ __launch_bounds__(256) void dropout(const DropoutArgs a) {
-  const uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x;
+  const uint64_t i = uint64_t(block_index()) * 256 + threadIdx.x;
   if (i >= a.groups) return;
-  const uint64_t row = a.groups <= 0xFFFFFFFFu ? uint32_t(i) / a.per_row : i / a.per_row;
+  const uint64_t row = a.groups <= 0xFFFFFFFFu ? uint32_t(i) / uint32_t(a.per_row) : i / a.per_row;
   const uint32_t group = uint32_t(i - row * a.per_row);
   const int64_t col = int64_t(group) * 8;
   const int n = a.cols - col > 8 ? 8 : int(a.cols - col);
@@ -75,14 +75,14 @@ extern "C" int cchip_dropout_run(const cchip_dropout *op, const cchip_dropout_io
     a.x = rows_of(who, "x", op->dtype, op->rows, op->cols, io->x, false, true);
     a.residual = rows_of(who, "residual", op->dtype, op->rows, op->cols, io->residual, false, false);
     a.out = rows_of(who, "out", op->dtype, op->rows, op->cols, io->out, true, true);
-    a.per_row = uint32_t((op->cols + 7) / 8);
+    a.per_row = uint64_t(op->cols + 7) / 8;
+    if (a.per_row > (uint64_t(1) << 39) / uint64_t(op->rows)) throw InvalidArgument("dropout: more than 2^42 elements");
     a.groups = uint64_t(op->rows) * a.per_row;
-    if ((a.groups + 255) / 256 > uint64_t(INT32_MAX)) throw InvalidArgument("dropout: more elements than a launch can have");
     a.cols = op->cols;
     a.scale = op->scale;
     with_rows_type(op->dtype, [&](auto t) {
       typedef decltype(t) T;
-      hipLaunchKernelGGL((dropout<T>), dim3(unsigned((a.groups + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a);
+      hipLaunchKernelGGL((dropout<T>), grid_of(int64_t((a.groups + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a);
     });
     check_launch("dropout");
   });

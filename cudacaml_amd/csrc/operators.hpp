@@ -277,12 +277,24 @@ __device__ __forceinline__ uint32_t keep_bits(const Drop &d, uint64_t offset, ui
   return bits;
 }
 
+// A launch has fewer than 2^32 work items along an axis: workgroups (of at
+// most 512 here) past the first 2^22 go on along y. The last row of y may have
+// some over.
+constexpr uint32_t kGridRow = 1u << 22;
+
+__device__ __forceinline__ uint32_t block_index() { return blockIdx.y * kGridRow + blockIdx.x; }
+
 // ---- host side --------------------------------------------------------------
 
 // Whether two stretches of memory share a byte.
 inline bool meet(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
   return x < y + b_bytes && y < x + a_bytes;
+}
+
+inline dim3 grid_of(int64_t workgroups) {
+  const int64_t rows = (workgroups + kGridRow - 1) / kGridRow;
+  return dim3(unsigned(rows > 1 ? kGridRow : workgroups), unsigned(rows));
 }
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

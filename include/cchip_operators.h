@@ -112,7 +112,7 @@ int cchip_gated_delta_backward(const cchip_gated_delta *op, const cchip_gated_de
  */
 typedef struct {
   int dtype;
-  int64_t rows, cols; /* rows < 2^32, cols < 2^35 */
+  int64_t rows, cols; /* rows < 2^32, cols < 2^35, at most 2^42 elements */
   double p;           /* 0 <= p <= 1 */
   float scale;
 } cchip_dropout;

@@ -809,3 +809,72 @@ def test_gated_delta_f16_products_are_whole(device, dims, back):
     x["beta"].fill_(1.0)
     x["g"].fill_(-0.05)
     check_delta(x, "f16", back=back)
+
+
+# ---- more workgroups than a launch has along one axis ------------------------
+
+def test_dropout_of_more_rows_than_a_launch_has_work_items(device):
+    """2^32 - 1 rows of one column, in place: rows at the ends and around each
+    2^30th against the generator, and about p of all of them dropped."""
+    rows, p, seed, offset = (1 << 32) - 1, 0.25, 0x123456789, 7
+    x = torch.ones(rows, 1, dtype=torch.bfloat16, device="cuda")
+    O.Dropout("bf16", rows, 1, p).forward(x, x, seed=seed, offset=offset)
+    torch.cuda.synchronize()
+    for at in (0, (1 << 30) - 50, (1 << 31) - 50, 3 * (1 << 30) - 50, rows - 100):
+        got = x[at:at + 100, 0].float().cpu().numpy()
+        low = [R.philox((0, r, offset, 0), (seed & R.LOW, seed >> 32))[0] & 0xFFFF for r in range(at, at + 100)]
+        want = np.where(np.array(low) >= 16384, float(torch.tensor(4 / 3).bfloat16()), 0.0)
+        assert np.array_equal(got, want), at
+    kept = sum(int((x[at:at + (1 << 28)] != 0).sum()) for at in range(0, rows, 1 << 28))
+    assert abs(kept / rows - 0.75) < 5 * (0.1875 / rows) ** 0.5
+    del x
+    torch.cuda.empty_cache()
+
+
+def test_dropout_of_the_longest_rows(device):
+    """2^35 - 3 columns, in place: 2^32 groups of eight, the last one short."""
+    cols, seed = (1 << 35) - 3, 99
+    x = torch.ones(1, cols, dtype=torch.float16, device="cuda")
+    O.Dropout("f16", 1, cols, 0.5).forward(x, x, seed=seed)
+    torch.cuda.synchronize()
+    for group in (0, (1 << 30) + 1, 1 << 31, (1 << 32) - 1):
+        got = x[0, 8 * group:8 * group + 8].float().cpu().numpy()
+        words = R.philox((group, 0, 0, 0), (seed, 0))
+        halves = [h for w in words for h in (w & 0xFFFF, w >> 16)][:len(got)]
+        assert np.array_equal(got, [2.0 * (h >= 32768) for h in halves]), group
+    assert len(got) == 5
+    del x
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_gated_delta_more_heads_than_a_launch_has_workgroups(device, dtype):
+    """One token of 2^24 + 32 states of one element."""
+    b, h = (1 << 19) + 1, 32
+    g = torch.Generator(device="cuda").manual_seed(3)
+    r = lambda *s: torch.randn(s, generator=g, device="cuda").to(TYPES[dtype])  # noqa: E731
+    q, k, v, a, beta = r(b, 1, 1, 1), r(b, 1, 1, 1), r(b, 1, h, 1), -r(b, 1, h).abs(), r(b, 1, h).sigmoid()
+    state = torch.randn(b, h, 1, 1, generator=g, device="cuda")
+    o, end = torch.empty_like(v), torch.empty_like(state)
+    O.GatedDelta(dtype, b, 1, 1, h, 1, 1, scale=0.5).forward(q, k, v, a, beta, o, state=state, state_out=end)
+    torch.cuda.synchronize()
+    s = a.double().exp()[:, 0] * state.double()[..., 0, 0]
+    s = s + k.double()[:, 0, :, 0] * beta.double()[:, 0] * (v.double()[:, 0, :, 0] - s * k.double()[:, 0, :, 0])
+    close(end[..., 0, 0], s.cpu().numpy(), "state")
+    close(o[:, 0, :, 0], (0.5 * s * q.double()[:, 0, :, 0]).cpu().numpy(), "o")
+
+
+def test_gated_delta_more_column_blocks_than_a_launch_has_workgroups(device):
+    """4096 sequences, all but a few empty, of 32 heads of 4096 columns."""
+    n, hv, dv, tokens = 4096, 32, 4096, 70
+    x = {k: v.cuda() for k, v in arrays("bf16", 1, tokens, 1, hv, 16, dv, seed=36).items()}
+    cuts = [0, 3] + [3] * (n // 2) + [20] * (n // 2 - 2) + [tokens]
+    out = []
+    for c in (cuts, [0, 3, 20, tokens]):
+        o = torch.full_like(x["v"], float("nan"))
+        op = O.GatedDelta("bf16", 1, tokens, 1, hv, 16, dv, sequences=len(c) - 1, states=False)
+        op.forward(*x.values(), o, offsets=torch.tensor(c, dtype=torch.int32, device="cuda"))
+        torch.cuda.synchronize()
+        op.free()
+        out.append(o)
+    assert torch.equal(out[0], out[1])

@@ -355,6 +355,19 @@ def _one_token(op):
     return one
 
 
+def test_sizes_past_a_launch_are_refused():
+    """What overflows no count on the way to its refusal."""
+    for change in (dict(batch=1 << 30, value_heads=1 << 30, key_heads=1, tokens=0), dict(batch=1, tokens=0, value_heads=(1 << 31) - 1,
+                                                                                     key_heads=1, value_dim=4096)):
+        with pytest.raises(ValueError, match="launch"):
+            O.GatedDelta(**{**dict(dtype="bf16", key_dim=64, value_dim=64), **change})
+    rows = (1 << 32) - 1
+    words = O.Dropout._io.pack(1, 0, 0, *(4096, 1 << 34) * 3)
+    for cols in (1 << 34, (1 << 35) - 1):
+        rc, msg = _call(_lib.lib().cchip_dropout_run, _lib.DropoutDesc(5, rows, cols, 0.5, 1.0), words, None)
+        assert rc == 1 and ("more than 2^42 elements" in msg or "rows of out overlap" in msg), msg
+
+
 # ---- workspaces --------------------------------------------------------------
 
 class _Memory:
