@@ -878,3 +878,115 @@ def test_gated_delta_more_column_blocks_than_a_launch_has_workgroups(device):
         op.free()
         out.append(o)
     assert torch.equal(out[0], out[1])
+
+
+# ---- 32 value columns a workgroup, wide heads --------------------------------
+
+MANY = [  # more than 128 blocks of 32 value columns, so that a workgroup takes 32 (whole heads, pieces, single elements)
+    (3, 100, 8, 24, 128, 64), (5, 70, 4, 32, 64, 32), (4, 66, 4, 12, 128, 100), (5, 70, 4, 32, 100, 40), (3, 130, 2, 16, 61, 90),
+    (5, 70, 8, 32, 5, 7), (5, 65, 16, 32, 3, 3), (1, 70, 1, 5, 24, 4096),
+]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("states", [False, True])
+@pytest.mark.parametrize("shape", MANY)
+def test_gated_delta_many_blocks(device, dtype, shape, states):
+    """Forward with and without what a backward pass needs, and backward."""
+    assert shape[0] * shape[3] * -(-shape[5] // 32) > 128
+    x = arrays(dtype, *shape, seed=41, states=shape[0] if states else 0, back=True)
+    check_delta(x, dtype, back=True)
+    check_delta({n: v for n, v in x.items() if n not in ("do", "dstate_out")}, dtype)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_gated_delta_many_packed_sequences(device, dtype):
+    cuts = [0, 1, 1, 65, 66, 130, 258, 259, 300, 300, 320]
+    check_delta(arrays(dtype, 1, 320, 4, 16, 48, 40, seed=42, states=len(cuts) - 1, back=True), dtype, cuts, back=True)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", [(1, 130, 1, 1, 16, 1001), (1, 70, 1, 2, 128, 512), (2, 1, 1, 1, 20, 1500)])
+def test_gated_delta_wide_values(device, dtype, shape):
+    """Few heads of many columns: 16 columns a workgroup, and single tokens."""
+    check_delta(arrays(dtype, *shape, seed=43, states=shape[0], back=True), dtype, back=True)
+    check_delta(arrays(dtype, *shape, seed=43, states=shape[0]), dtype)
+
+
+# ---- where gradients are written ---------------------------------------------
+
+def _between_guards(like):
+    """A place for a result at an odd element, its heads a few elements apart,
+    and the whole that it lies in, of sevens."""
+    b, t, h = like.shape[:3]
+    if like.dim() == 3:
+        whole = torch.full((b, t, 2 * h + 3), 7.0, dtype=like.dtype, device="cuda")
+        return whole[..., 1:2 * h + 1:2], whole
+    whole = torch.full((b, t, h, like.shape[3] + 5), 7.0, dtype=like.dtype, device="cuda")
+    return whole[..., 3:3 + like.shape[3]], whole
+
+
+def _heads_first_place(like):
+    whole = torch.full(tuple(like.shape[i] for i in (0, 2, 1)) + tuple(like.shape[3:]), 7.0, dtype=like.dtype, device="cuda")
+    return whole.transpose(1, 2), whole
+
+
+def run_delta_into(x, dtype, place):
+    """``run_delta`` of the backward pass with its results placed; also how
+    many elements of each whole are none of its result and not seven."""
+    b, t, hk, dk = x["q"].shape
+    hv, dv = x["v"].shape[2:]
+    op = O.GatedDelta(dtype, b, t, hk, hv, dk, dv, states=False)
+    dev = {k: v.cuda() for k, v in x.items()}
+    names = ("q", "k", "v", "g", "beta")
+    ins = [dev[n] for n in names]
+    out, whole = {}, {}
+    for n in ("o",) + tuple("d" + n for n in names):
+        out[n], whole[n] = place(dev["v" if n == "o" else n[1:]])
+    saved = torch.full((op.saved_bytes(),), 255, dtype=torch.uint8, device="cuda")
+    op.forward(*ins, out["o"], saved=saved)
+    op.backward(*ins, dev["do"], saved, *(out["d" + n] for n in names))
+    torch.cuda.synchronize()
+    touched = {}
+    for n in out:
+        got = out[n].clone()
+        out[n].fill_(7.0)
+        touched[n] = int((whole[n] != 7.0).sum())
+        out[n] = got
+    return out, touched
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("place", [_between_guards, _heads_first_place])
+@pytest.mark.parametrize("shape", [(2, 70, 2, 4, 64, 96), (2, 130, 1, 2, 100, 40), (2, 70, 1, 2, 5, 3), (1, 65, 1, 1, 33, 17),
+                                   (3, 70, 8, 48, 64, 32), (3, 70, 8, 48, 40, 27), (3, 67, 8, 48, 5, 7)])
+def test_gated_delta_writes_gradients_where_they_belong(device, dtype, place, shape):
+    """Results of any stride and alignment are those of contiguous ones, and
+    what lies between their elements keeps its value."""
+    x = arrays(dtype, *shape, seed=44, back=True)
+    want = run_delta(x, dtype, back=True)
+    got, touched = run_delta_into(x, dtype, place)
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+        assert touched[n] == 0, n
+
+
+def test_gated_delta_results_past_32_bits(device):
+    """o, dq, dk and dv with tokens 2^23 elements apart: the last ones lie past
+    2^32 bytes and 2^31 elements."""
+    x = arrays("bf16", 2, 300, 1, 2, 32, 32, seed=45, back=True)
+    want = run_delta(x, "bf16", back=True)
+
+    def place(like):
+        b, n, h = like.shape[:3]
+        if like.dim() == 3:
+            t = torch.empty_like(like)
+            return t, torch.full((1,), 7.0)
+        whole = torch.empty((b * n - 1) * (1 << 23) + h * like.shape[3], dtype=like.dtype, device="cuda")
+        return whole.as_strided(tuple(like.shape), (n << 23, 1 << 23, like.shape[3], 1)), torch.full((1,), 7.0)
+
+    got, _ = run_delta_into(x, "bf16", place)
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+    del got
+    torch.cuda.empty_cache()
