@@ -427,9 +427,9 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES, waves_of(LANES, Gate, Pr
           const float e = Bias ? x[v][i] * w[i % 4] + b[i % 4] : x[v][i] * w[i % 4];
           float act = 1.0f, slope = 0.0f;
           if (Gate) gate_of<T>(a.act, float(rz[v].x[i]), act, slope);
-          const float du = keep ? d[v][i] * up : 0.0f;
+          // selected last: what was dropped may be no number
+          const float du = d[v][i] * up, db = du * t[i % 4], da = keep ? db * act : 0.0f;
           if (V == 1) acc[kChannelScale][v][i] += keep ? du * e * act : 0.0f;
-          const float db = du * t[i % 4], da = db * act;
           if (Gate) dz[i] = keep ? db * e * slope : 0.0f;
           if (V == 1) acc[kPostWeight][v][i] += da * x[v][i];
           if (V == 1 && Bias) acc[kPostBias][v][i] += da;
@@ -510,9 +510,8 @@ __global__ __launch_bounds__(256, 4) void norm_sums(const NormArgs a) {
       const float x = (float(ry.x[i]) - s.post_mean) * s.post_inv, e = Bias ? x * w[i] + b[i] : x * w[i];
       float act = 1.0f, slope = 0.0f;
       if (Gate) gate_of<T>(a.act, float(rz.x[i]), act, slope);
-      const float du = bits >> i & 1 ? d * up : 0.0f;
+      const float du = d * up, da = bits >> i & 1 ? du * t[i] * act : 0.0f;
       acc[kChannelScale][i] += bits >> i & 1 ? du * e * act : 0.0f;
-      const float da = du * t[i] * act;
       acc[kPostWeight][i] += da * x;
       if (Bias) acc[kPostBias][i] += da;
     }

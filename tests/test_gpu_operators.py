@@ -990,3 +990,41 @@ def test_gated_delta_results_past_32_bits(device):
         assert torch.equal(got[n], want[n]), n
     del got
     torch.cuda.empty_cache()
+
+
+# ---- what a norm block's dropout drops ---------------------------------------
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("width", [40, 1000, 5000, 9001])
+@pytest.mark.parametrize("how", [("rms", "rms", "silu"), ("layer", "none", "sigmoid"), ("none", "rms", "silu")])
+def test_norm_block_drops_what_is_not_a_number(device, dtype, width, how):
+    """Gates that are infinite or NaN where they are dropped (and values of y,
+    where no norm reads them): results and gradients are those of any other
+    gate there, and theirs are zero."""
+    rows, p, seed, offset = 6, 0.4, 0x1234567890ABCDEF, 1 << 33
+    x, w = norm_arrays(dtype, "f32", rows, width, *how, seed=46)
+    drop = torch.from_numpy(~R.kept(rows, width, p, seed, offset)[0])
+    clean = {k: v.clone() for k, v in x.items()}
+    bad = torch.tensor([float("inf"), -float("inf"), float("nan")]).to(TYPES[dtype]).repeat(rows * width)[:rows * width].view(rows, width)
+    for n in ("gate",) + (("y",) if how[0] == "none" else ()):
+        x[n] = torch.where(drop, bad, x[n])
+        clean[n] = torch.where(drop, torch.zeros_like(x[n]), x[n])
+    op = O.NormBlock(dtype, rows, width, norm=how[0], pre=how[1], gate=how[2], dropout=p, scale=0.7, eps=1e-5)
+    dev, wd = {k: v.cuda() for k, v in x.items()}, {k: v.cuda() for k, v in w.items()}
+    wide = {k: v.double().numpy() for k, v in {**clean, **w}.items()}
+    got = {n: torch.empty_like(dev["y"]) for n in (("h", "n") if how[1] != "none" else ("h",))}
+    op.forward(dev["y"], got["h"], got.get("n"), gate=dev["gate"], residual=dev["residual"], seed=seed, offset=offset, **wd)
+    out = {n: torch.empty_like(dev["y"]) for n in ("y", "gate", "residual")}
+    grads = {n: torch.empty_like(v) for n, v in wd.items()}
+    op.backward(dev["y"], dev["dh"], out["y"], dn=dev.get("dn"), h=dev.get("h"), gate=dev["gate"], dgate=out["gate"],
+                dresidual=out["residual"], grads=grads, seed=seed, offset=offset, **wd)
+    torch.cuda.synchronize()
+    want = R.norm_block(wide, *how, 0.7, 1e-5, p, seed, offset)
+    for n, v in got.items():
+        close(v, want[n], n)
+    want = R.norm_block(wide, *how, 0.7, 1e-5, p, seed, offset, back=True)
+    for n, v in {**out, **grads}.items():
+        close(v, want[n], n)
+    assert not out["gate"].cpu()[drop].any()
+    if how[0] == "none":
+        assert not out["y"].cpu()[drop].any()
