@@ -2888,8 +2888,8 @@ struct Lowering {
     // off (cc_sum): each further tile is a rounding more in plain ones. Root
     // mean square error of the sums of uniform values, in such tiles plain /
     // carried / large tiles plain: 900001 f32 5.1e-8 / 3.6e-8 / 4.6e-8, 6M
-    // f32 5.4e-8 / 4.4e-8 / 4.9e-8, 900001 f64 1.02e-16 / 7.0e-17 / 9.2e-17,
-    // 60M f64 4.5e-16 / 2.3e-16 / 3.5e-16; the times are the same.
+    // f32 5.4e-8 / 4.4e-8 / 4.9e-8, 900001 f64 1.02e-16 / 6.6e-17 / 9.2e-17,
+    // 60M f64 4.5e-16 / 6.4e-17 / 3.5e-16; the times are the same.
     const bool carried = (two_pass || small_tiles || GW == 2) && (n.dt == DT::F32 || n.dt == DT::F64) && g.xs[n.body].op == B_ADD &&
                          any_order(n.body, n.dt, true);
     const std::string CT = carried ? "cc_sum<" + T + ">" : T, ccmb = carried ? "cc_sum_add" : cmb,
@@ -2904,6 +2904,14 @@ struct Lowering {
     bool uvec = !vec && len >= GW && dt_size(n.dt) >= 4;
     for (int b : f.ident) uvec = uvec && dt_size(prog.bufs[b].dt) >= 4;
     int words = wide ? 2 : 1;
+    // Chains of doubles publish what their additions rounded off too: the
+    // upper 30 bits of it stand above the flag in the first word, 18 bits of
+    // what is at most half a unit of the sum's last place. A prefix is then
+    // rounded where it is read and not at every hop, of which a long row has
+    // as many as its look-backs happen to take (2^25 f64, in roundings of the
+    // exact sums: 2.3 to 6.9 without it, other bits in every run, 1.42 with,
+    // the same bits in five; 2^27 f64 take 435 us either way).
+    const bool low_word = carried && wide;
     const bool selfsched = chained && !wide && tune("lb_counter", 0) == 0;
     int status = -1, ctr = -1, kinit = -1;
     if (two_pass) status = add_buf("t" + id + "_totals", n.dt, tpr - 1, BufRole::Scratch);
@@ -2956,12 +2964,12 @@ struct Lowering {
     } else {
       pub =
           "{ const cc_u64 bb = cc_bits(VAL); "
-          "__hip_atomic_store(&st[2 * (TILE)], ((cc_u64)(FLAG) << 32) | (bb & 0xffffffffull), __ATOMIC_RELAXED, "
+          "__hip_atomic_store(&st[2 * (TILE)], LOW((cc_u64)(FLAG) << 32) | (bb & 0xffffffffull), __ATOMIC_RELAXED, "
           "__HIP_MEMORY_SCOPE_AGENT); "
           "__hip_atomic_store(&st[2 * (TILE) + 1], ((cc_u64)(FLAG) << 32) | (bb >> 32), __ATOMIC_RELAXED, "
           "__HIP_MEMORY_SCOPE_AGENT); }";
     }
-    auto publish = [&](const std::string &tl, const std::string &flag, const std::string &val) {
+    auto publish = [&](const std::string &tl, const std::string &flag, const std::string &val, const std::string &low) {
       std::string r = pub;
       auto rep = [&](const std::string &a, const std::string &b) {
         size_t q = 0;
@@ -2973,6 +2981,7 @@ struct Lowering {
       rep("TILE", tl);
       rep("FLAG", flag);
       rep("VAL", val);
+      rep("LOW", low_word && !low.empty() ? "((cc_bits(" + low + ") >> 34) << 34) | " : "");
       return r;
     };
     // Buffer-resource loads and stores (one shared offset register for the
@@ -3236,7 +3245,7 @@ struct Lowering {
         << "    b" << rout[j] << "[row] = th ? " << rcmb[j] << "(" << rini[j] << "(), t) : " << rini[j] << "();\n"
         << "  }\n";
     if (chained) {
-      k << "  if (threadIdx.x == 0) " << publish("tile", "tin == 0 ? 2 : 1", "run") << ";\n"
+      k << "  if (threadIdx.x == 0) " << publish("tile", "tin == 0 ? 2 : 1", "run", "") << ";\n"
         << "  if (tin > 0) {\n"
         << "    if (wid == 0) {\n"
         << "      const int rowstart = row * " << tpr << ";\n"
@@ -3339,22 +3348,23 @@ struct Lowering {
       } else {
         k << "        const int q = j - lane;\n"
           << "        int flag = 2;\n"
-          << "        " << T << " val = " << ini << "();\n"
+          << "        " << T << " val = " << ini << "()" << (low_word ? ", low = 0" : "") << ";\n"
           << "        if (q >= rowstart) {\n"
           << "          while (true) {\n"
           << "            const cc_u64 w0 = __hip_atomic_load(&st[2 * q], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);\n"
           << "            const cc_u64 w1 = __hip_atomic_load(&st[2 * q + 1], __ATOMIC_RELAXED, "
              "__HIP_MEMORY_SCOPE_AGENT);\n"
-          << "            flag = (int)(w0 >> 32);\n"
+          << "            flag = (int)(w0 >> 32)" << (low_word ? " & 3" : "") << ";\n"
           << "            if (flag != 0 && flag == (int)(w1 >> 32)) { val = cc_from_bits<" << T
-          << ">((w0 & 0xffffffffull) | (w1 << 32)); break; }\n"
+          << ">((w0 & 0xffffffffull) | (w1 << 32)); "
+          << (low_word ? "low = cc_from_bits<" + T + ">((w0 >> 34) << 34); " : "") << "break; }\n"
           << "            if (++spins > (1u << 24)) { cc_flag(err, 4); flag = 2; break; }\n"
           << "            __builtin_amdgcn_s_sleep(1);\n"
           << "          }\n"
           << "        }\n"
           << "        const cc_u64 pm = __ballot(flag == 2);\n"
           << "        const int L = pm ? (__ffsll((long long)pm) - 1) : 63;\n"
-          << "        " << CT << " w = " << cof << "(val);\n"
+          << "        " << CT << " w = " << (low_word ? "{val, low}" : cof + "(val)") << ";\n"
           << "        bool hw = lane <= L;\n";
         k << lookback_tree(ccmb, CT)
           << "        w = __shfl(w, 0);\n"
@@ -3367,8 +3377,9 @@ struct Lowering {
       k
         << "      if (lane == 0) {\n"
         << "        s_prefix = " << cval << "(acc);\n"
-        << "        const " << T << " incl = " << cval << "(" << ccmb << "(acc, " << cof << "(run)));\n"
-        << "        " << publish("tile", "2", "incl") << ";\n"
+        << "        const " << CT << " total = " << ccmb << "(acc, " << cof << "(run));\n"
+        << "        const " << T << " incl = " << cval << "(total);\n"
+        << "        " << publish("tile", "2", "incl", "total.l - (incl - total.h)") << ";\n"
         << "      }\n"
         << "    }\n"
         << "    __syncthreads();\n"
