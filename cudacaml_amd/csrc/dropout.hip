@@ -75,6 +75,8 @@ extern "C" int cchip_dropout_run(const cchip_dropout *op, const cchip_dropout_io
     a.x = rows_of(who, "x", op->dtype, op->rows, op->cols, io->x, false, true);
     a.residual = rows_of(who, "residual", op->dtype, op->rows, op->cols, io->residual, false, false);
     a.out = rows_of(who, "out", op->dtype, op->rows, op->cols, io->out, true, true);
+    check_place(who, op->dtype, op->rows, op->cols, "out", a.out, "x", a.x, true);
+    check_place(who, op->dtype, op->rows, op->cols, "out", a.out, "residual", a.residual, true);
     a.per_row = uint64_t(op->cols + 7) / 8;
     if (a.per_row > (uint64_t(1) << 39) / uint64_t(op->rows)) throw InvalidArgument("dropout: more than 2^42 elements");
     a.groups = uint64_t(op->rows) * a.per_row;

@@ -4,6 +4,7 @@
 #include "norm_block.hpp"
 
 #include <cmath>
+#include <utility>
 
 namespace cchip {
 namespace op {
@@ -143,6 +144,12 @@ int cchip_norm_block_forward(const cchip_norm_block *op, const cchip_norm_block_
     a.residual = rows_of(who, "residual", op->dtype, op->rows, op->width, io->residual, false, false);
     a.h = rows_of(who, "h", op->dtype, op->rows, op->width, io->h, true, true);
     a.n = rows_of(who, "n", op->dtype, op->rows, op->width, io->n, true, false);
+    const std::pair<const char *, const Rows &> in[] = {{"y", a.y}, {"gate", a.gate}, {"residual", a.residual}};
+    for (auto &i : in) {
+      check_place(who, op->dtype, op->rows, op->width, "h", a.h, i.first, i.second, true);
+      check_place(who, op->dtype, op->rows, op->width, "n", a.n, i.first, i.second, true);
+    }
+    check_place(who, op->dtype, op->rows, op->width, "n", a.n, "h", a.h, false);
     with_rows_type(op->dtype, [&](auto t) { norm_forward_launch<decltype(t)>(a, (hipStream_t)stream); });
     check_launch(who);
   });
@@ -192,9 +199,13 @@ int cchip_norm_block_backward(const cchip_norm_block *op, const cchip_norm_block
       a.dgate = rows_of(who, "dgate", op->dtype, op->rows, op->width, io->dgate, true, false);
       a.dresidual = rows_of(who, "dresidual", op->dtype, op->rows, op->width, io->dresidual, true, false);
       // norm_sums reads its inputs after the others are written
-      for (const char *out : {a.dy.p, a.dgate.p, a.dresidual.p})
-        for (const char *in : {a.y.p, a.gate.p, a.h.p, a.dh.p, a.dn.p})
-          if (out && out == in) throw InvalidArgument("norm block: a gradient is written over what the backward pass reads");
+      const std::pair<const char *, const Rows &> out[] = {{"dy", a.dy}, {"dgate", a.dgate}, {"dresidual", a.dresidual}},
+                                                  in[] = {{"y", a.y}, {"gate", a.gate}, {"h", a.h}, {"dh", a.dh}, {"dn", a.dn}};
+      for (auto &o : out) {
+        for (auto &i : in) check_place(who, op->dtype, op->rows, op->width, o.first, o.second, i.first, i.second, false);
+        for (auto *other = out; other != &o; other++)
+          check_place(who, op->dtype, op->rows, op->width, o.first, o.second, other->first, other->second, false);
+      }
     }
     const int groups = backward_groups(*op, bias);
     if (any) {

@@ -59,6 +59,17 @@ inline Rows rows_of(const char *who, const char *name, int dtype, int64_t rows, 
   return {static_cast<char *>(x.data), x.row};
 }
 
+// What a call reads and writes may lie in one place where each thread reads an
+// element before it writes it: row for row. Any other overlap is refused, as
+// far as the first rows show it.
+inline void check_place(const char *who, int dtype, int64_t rows, int64_t cols, const char *out_name, const Rows &out,
+                        const char *in_name, const Rows &in, bool in_place) {
+  const size_t bytes = size_t(cols) * (dtype == CCHIP_F32 ? 4 : 2);
+  if (!out.p || !in.p || !meet(out.p, bytes, in.p, bytes)) return;
+  if (in_place && out.p == in.p && (rows == 1 || out.row == in.row)) return;
+  throw InvalidArgument(strf("%s: %s is written over %s%s", who, out_name, in_name, in_place ? ", and not row for row" : ""));
+}
+
 template <typename F>
 void with_rows_type(int dtype, F &&f) {
   if (dtype == CCHIP_F32) f(float());

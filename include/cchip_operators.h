@@ -131,7 +131,7 @@ typedef struct {
 
 /* out = residual + scale drop(x); residual.data NULL: no residual. The
    gradient of x is the same call on the gradient of out, without residual.
-   out may be x or residual. */
+   out may be x or residual, row for row. */
 int cchip_dropout_run(const cchip_dropout *op, const cchip_dropout_io *io, void *stream);
 
 /* ---- Norm block ---------------------------------------------------------- */
@@ -179,7 +179,8 @@ typedef struct {
   cchip_rows dy, dgate, dresidual;    /* backward: written; dgate, dresidual NULL: not wanted */
 } cchip_norm_block_io;
 
-/* h may be `residual` or y, n may be y. n is NULL iff pre is none. */
+/* h and n may each be `residual`, y or the gate, row for row, but not both the
+   same. n is NULL iff pre is none. */
 int cchip_norm_block_forward(const cchip_norm_block *op, const cchip_norm_block_io *io, void *stream);
 /* From y, gate, the forward pass's h (needed iff pre is not none), and the
    gradients dh and dn of its results: the gradients of y, gate, residual and

@@ -1028,3 +1028,24 @@ def test_norm_block_drops_what_is_not_a_number(device, dtype, width, how):
     assert not out["gate"].cpu()[drop].any()
     if how[0] == "none":
         assert not out["y"].cpu()[drop].any()
+
+
+# ---- results over inputs -----------------------------------------------------
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("width", [100, 3000, 9001])
+def test_norm_block_over_any_of_its_inputs(device, dtype, width):
+    """h and n each over y, the gate or the residual, row for row."""
+    x, w = norm_arrays(dtype, "f32", 9, width, "layer", "rms", "silu", seed=47)
+    op = O.NormBlock(dtype, 9, width, norm="layer", pre="rms", gate="silu", dropout=0.2)
+    dev, wd = {k: v.cuda() for k, v in x.items()}, {k: v.cuda() for k, v in w.items()}
+    h, n = torch.empty_like(dev["y"]), torch.empty_like(dev["y"])
+    op.forward(dev["y"], h, n, gate=dev["gate"], residual=dev["residual"], seed=2, **wd)
+    names = ("y", "gate", "residual")
+    for a in names:
+        for b in names:
+            if a != b:
+                t = {k: dev[k].clone() for k in names}
+                op.forward(t["y"], t[a], t[b], gate=t["gate"], residual=t["residual"], seed=2, **wd)
+                torch.cuda.synchronize()
+                assert torch.equal(t[a], h) and torch.equal(t[b], n), (a, b)

@@ -215,6 +215,34 @@ def test_dropout_refuses():
         op.forward(torch.zeros(4, 8), torch.zeros(1, 8).expand(4, 8), seed=1)
 
 
+def test_rows_are_written_in_place_row_for_row_only():
+    """A result over an input by other strides or a few elements on would be
+    read by threads after others wrote it; h and n have a place each."""
+    z = lambda *s: torch.zeros(s)  # noqa: E731
+    op = O.Dropout("f32", 4, 8, 0.5)
+    op._device = -1
+    w = z(200)
+    at = lambda first, row: w.as_strided((4, 8), (row, 1), first)  # noqa: E731
+    for out in (at(0, 9), at(3, 8), at(7, 8)):
+        with pytest.raises(ValueError, match="out is written over x, and not row for row"):
+            op.forward(at(0, 8), out, seed=1)
+        with pytest.raises(ValueError, match="out is written over residual"):
+            op.forward(z(4, 8), out, residual=at(0, 8), seed=1)
+    op = O.NormBlock("f32", 4, 8, gate="silu")
+    op._device = -1
+    with pytest.raises(ValueError, match="h is written over residual"):
+        op.forward(z(4, 8), at(0, 9), z(4, 8), gate=z(4, 8), residual=at(0, 8))
+    with pytest.raises(ValueError, match="n is written over y"):
+        op.forward(at(4, 8), z(4, 8), at(0, 8), gate=z(4, 8))
+    with pytest.raises(ValueError, match="n is written over h"):
+        op.forward(z(4, 8), at(0, 8), at(0, 8), gate=z(4, 8))
+    back = dict(dn=z(4, 8), h=z(4, 8), gate=z(4, 8))
+    with pytest.raises(ValueError, match="dgate is written over dy"):
+        op.backward(z(4, 8), z(4, 8), at(0, 8), dgate=at(0, 8), **back)
+    with pytest.raises(ValueError, match="dresidual is written over h"):
+        op.backward(z(4, 8), z(4, 8), z(4, 8), dresidual=at(5, 8), **{**back, "h": at(0, 8)})
+
+
 def test_arrays_lie_in_their_buffers():
     class Memory:
         ptr, nbytes = 4096, 64
