@@ -68,6 +68,22 @@ bool steps(const cchip_gated_delta &op, bool saves) { return !op.sequences && !s
 
 int element_size(const cchip_gated_delta &op) { return op.dtype == CCHIP_F32 ? 4 : 2; }
 
+// Whether two heads' elements of a tensor share a place, as far as one step
+// along an axis, or one and some along another, shows it.
+bool overlaps(const cchip_gated_delta &op, const cchip_heads &x, int heads, int dim) {
+  const int64_t count[] = {op.batch, op.tokens, heads}, step[] = {std::llabs(x.batch), std::llabs(x.token), std::llabs(x.head)};
+  for (int i = 0; i < 3; i++) {
+    if (count[i] < 2) continue;
+    if (step[i] < dim) return true;
+    for (int j = 0; j < 3; j++) {
+      if (i == j || count[j] < 2 || step[j] < dim || step[j] > step[i]) continue;
+      const int64_t n = step[i] / step[j], over = step[i] % step[j];
+      if ((over < dim && n < count[j]) || (step[j] - over < dim && n + 1 < count[j])) return true;
+    }
+  }
+  return false;
+}
+
 Heads heads_of(const cchip_gated_delta &op, const cchip_heads &x, const char *name, bool written, int heads, int dim) {
   if (op.batch * op.tokens == 0) return {static_cast<char *>(x.data), x.batch, x.token, x.head};
   if (!x.data) throw InvalidArgument(strf("gated delta: no %s", name));
@@ -75,7 +91,7 @@ Heads heads_of(const cchip_gated_delta &op, const cchip_heads &x, const char *na
     throw InvalidArgument(strf("gated delta: %s is not aligned to its elements", name));
   // within a chunk elements are counted in 32 bits
   if (x.token < 0 || x.token > (int64_t(1) << 23)) throw InvalidArgument(strf("gated delta: tokens of %s are not 0 to 2^23 elements apart", name));
-  if (written && ((op.batch > 1 && x.batch == 0) || (op.tokens > 1 && x.token == 0) || (heads > 1 && std::llabs(x.head) < dim)))
+  if (written && overlaps(op, x, heads, dim))
     throw InvalidArgument(strf("gated delta: elements of %s overlap", name));
   return {static_cast<char *>(x.data), x.batch, x.token, x.head};
 }

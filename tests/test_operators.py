@@ -155,6 +155,35 @@ def test_c_entries_refuse_before_any_device_work():
     assert rc == 1 and "no descriptor" in msg
 
 
+def test_gated_delta_refuses_results_that_share_elements():
+    """Against all heads written out, for strides of all orders: what is
+    refused does overlap, and what is taken does not but by several steps along
+    one axis against several along others."""
+    L, F = _lib.lib(), O.GatedDelta._forward_io
+    b, t, h, dv = 2, 3, 4, 5
+    d = _lib.GatedDeltaDesc(0, b, t, 0, 1, h, 5, dv, 0, 1.0)
+    x = lambda at, n: (at << 20, 3 * n, n, dv if n > h else 1)  # noqa: E731
+    ins = [*x(1, dv), *x(2, dv), *x(3, h * dv), *x(4, h), *x(5, h)]
+    rng, refused, taken = np.random.default_rng(5), 0, 0
+    steps = [(60, 20, 5), (15, 5, 30), (20, 40, 5), (60, 20, -5), (60, 19, 5), (5, 10, 30), (100, 0, 5), (100, 33, 11), (40, 60, 10)]
+    steps += [tuple(int(v) for v in rng.integers(0, 70, 3)) for _ in range(300)]
+    for s in steps:
+        heads = np.add.outer(np.add.outer(np.arange(b) * s[0], np.arange(t) * s[1]), np.arange(h) * s[2]).ravel()
+        gaps = np.diff(np.sort(heads))
+        # `saved` off its alignment: what is taken is refused for that
+        rc, msg = _call(L.cchip_gated_delta_forward, d, F.pack(*ins, 6 << 20, *s, 0, 0, 0, 0, 0, 4100), None, 0, None)
+        assert rc == 1
+        if "overlap" in msg:
+            refused += 1
+            assert (gaps < dv).any(), s
+        else:
+            taken += 1
+            assert "saved is not aligned" in msg
+            if (gaps < dv).any():
+                assert all(abs(v) >= dv for v in s), s
+    assert refused > 50 and taken > 5
+
+
 def test_nothing_to_do_is_no_error():
     """No rows, no columns, no sequences: no launch, so no device is needed."""
     L = _lib.lib()
