@@ -4,6 +4,7 @@
 #include "delta.hpp"
 
 #include <cmath>
+#include <utility>
 
 using namespace cchip;
 using namespace cchip::op;
@@ -150,6 +151,10 @@ DeltaArgs args_of(const cchip_gated_delta &op, const cchip_gated_delta_io &io, c
     a.state = io.state;
     a.state_out = io.state_out;
   }
+  const std::pair<const char *, const void *> words[] = {{"offsets", io.offsets}, {"state", io.state}, {"state_out", io.state_out},
+                                                        {"dstate", io.dstate}, {"dstate_out", io.dstate_out}};
+  for (auto &w : words)
+    if (reinterpret_cast<uintptr_t>(w.second) % 4) throw InvalidArgument(strf("gated delta: %s is not aligned to its elements", w.first));
   if (!aligned16(io.saved)) throw InvalidArgument("gated delta: saved is not aligned to 16 bytes");
   a.offsets = io.offsets;
   a.tokens = op.tokens;

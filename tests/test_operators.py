@@ -184,6 +184,22 @@ def test_gated_delta_refuses_results_that_share_elements():
     assert refused > 50 and taken > 5
 
 
+def test_gated_delta_refuses_misaligned_words():
+    L = _lib.lib()
+    t = lambda p, h=8: (p << 20, 100 * 4 * h, 4 * h, h)  # noqa: E731
+    some = [w for i, h in enumerate((8, 8, 8, 1, 1, 8)) for w in t(i + 1, h)]
+    for sequences, tail, why in [(0, (0, 4098, 0, 0, 0, 4096), "state is"), (0, (0, 0, 4097, 0, 0, 4096), "state_out is"),
+                                 (1, (4098, 0, 0, 0, 0, 4096), "offsets is")]:
+        d = _lib.GatedDeltaDesc(0, 1, 100, sequences, 4, 4, 8, 8, 1, 1.0)
+        rc, msg = _call(L.cchip_gated_delta_forward, d, O.GatedDelta._forward_io.pack(*some, *tail), None, 0, None)
+        assert rc == 1 and why + " not aligned" in msg, msg
+    back = [w for i, h in enumerate((8, 8, 8, 1, 1)) for w in t(i + 1, h)] + [w for i, h in enumerate((8, 8, 8, 8, 1, 1)) for w in t(i + 7, h)]
+    d = _lib.GatedDeltaDesc(0, 1, 100, 0, 4, 4, 8, 8, 1, 1.0)
+    for tail, why in [((0, 0, 0, 4098, 0, 4096), "dstate_out is"), ((0, 0, 0, 0, 4099, 4096), "dstate is")]:
+        rc, msg = _call(L.cchip_gated_delta_backward, d, O.GatedDelta._backward_io.pack(*back, *tail), None, 0, None)
+        assert rc == 1 and why + " not aligned" in msg, msg
+
+
 def test_nothing_to_do_is_no_error():
     """No rows, no columns, no sequences: no launch, so no device is needed."""
     L = _lib.lib()
