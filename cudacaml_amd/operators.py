@@ -128,8 +128,12 @@ class _Operator:
 
     def _view(self, name, x, dtype, shape):
         """The array's pointer and strides, or ValueError."""
+        if x is None:
+            raise ValueError("%s: no %s" % (self._who, name))
         if type(x) is Resident:
             x = Array(x.buf, x.dtype.name, x.shape)
+        if not all(hasattr(x, a) for a in ("shape", "dtype", "stride", "data_ptr", "get_device")):
+            raise ValueError("%s: %s is no array on a device" % (self._who, name))
         if x.shape != shape and tuple(x.shape) != shape:
             raise ValueError("%s: %s has shape %s, expected %s" % (self._who, name, _dims(x.shape), _dims(shape)))
         d = x.dtype

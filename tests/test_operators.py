@@ -288,6 +288,28 @@ def test_rows_are_written_in_place_row_for_row_only():
         op.backward(z(4, 8), z(4, 8), z(4, 8), dresidual=at(5, 8), **{**back, "h": at(0, 8)})
 
 
+def test_what_is_no_array_is_refused():
+    """None, and arrays of the host, by name."""
+    delta, block, drop = O.GatedDelta("f32", 2, 10, 2, 4, 16, 8), O.NormBlock("f32", 4, 8), O.Dropout("f32", 4, 8, 0.5)
+    for op in (delta, block, drop):
+        op._device = -1
+    x = _delta_arrays()
+    z = torch.zeros(4, 8)
+    for name in x:
+        with pytest.raises(ValueError, match="GatedDelta: no %s$" % name):
+            delta.forward(*{**x, name: None}.values())
+        with pytest.raises(ValueError, match="GatedDelta: %s is no array on a device" % name):
+            delta.forward(*{**x, name: x[name].numpy()}.values())
+    with pytest.raises(ValueError, match="no array on a device"):
+        delta.forward(*x.values(), state=np.zeros((2, 4, 16, 8), np.float32))
+    with pytest.raises(ValueError, match="NormBlock: no y"):
+        block.forward(None, z, z.clone())
+    with pytest.raises(ValueError, match="NormBlock: h is no array on a device"):
+        block.forward(z, z.numpy(), z.clone())
+    with pytest.raises(ValueError, match="Dropout: x is no array on a device"):
+        drop.forward(z.numpy(), z, seed=1)
+
+
 def test_arrays_lie_in_their_buffers():
     class Memory:
         ptr, nbytes = 4096, 64
