@@ -124,7 +124,15 @@ class _Operator:
 
     def __init__(self):
         self._device = Device.current() if Device.available() else None
+        self._others = self._device is not None and Device.count() > 1
         self._workspaces = {}
+
+    def _on(self, stream):
+        """The stream's pointer; a call on another device than the handle's is
+        refused, as its kernels would run there."""
+        if self._others and Device.current() != self._device:
+            raise ValueError("%s: made for device %d, called on device %d" % (self._who, self._device, Device.current()))
+        return _stream_ptr(stream)
 
     def _view(self, name, x, dtype, shape):
         """The array's pointer and strides, or ValueError."""
@@ -242,7 +250,7 @@ class GatedDelta(_Operator):
         """Allocate a stream's workspace for forward calls, and that for
         backward calls, ahead of the first of them."""
         for back in (False, True)[:1 + bool(backward)]:
-            self._workspace(_stream_ptr(stream), back)
+            self._workspace(self._on(stream), back)
 
     def _words(self, **given):
         """Pointer and three strides of each array. The loop does in one go what
@@ -282,7 +290,7 @@ class GatedDelta(_Operator):
         (it may be ``state``, where they begin; without one, at zero).
         ``saved`` is written for a backward pass if given."""
         words = self._words(q=q, k=k, v=v, g=g, beta=beta, o=o)
-        s = _stream_ptr(stream)
+        s = self._on(stream)
         io = self._forward_io.pack(*words, self._bounds(offsets), self._whole("state", state, "f32", self._state),
                                    self._whole("state_out", state_out, "f32", self._state), 0, 0, self._kept(saved))
         w, n = (None, 0) if saved is not None or not self._forward_bytes else self._workspace(s, False, workspace)
@@ -298,7 +306,7 @@ class GatedDelta(_Operator):
         if saved is None:
             raise ValueError("GatedDelta: the backward pass needs what the forward pass saved")
         words = self._words(q=q, k=k, v=v, g=g, beta=beta, do=do, dq=dq, dk=dk, dv=dv, dg=dg, dbeta=dbeta)
-        s = _stream_ptr(stream)
+        s = self._on(stream)
         io = self._backward_io.pack(*words, self._bounds(offsets), 0, 0,
                                     self._whole("dstate_out", dstate_out, "f32", self._state),
                                     self._whole("dstate", dstate, "f32", self._state), self._kept(saved))
@@ -358,7 +366,7 @@ class Dropout(_RowOperator):
         """``out = residual + scale drop(x)``; out may be x or residual."""
         io = self._io.pack(*self._seed(seed, offset, step), *self._needed("x", x), *self._rows("residual", residual),
                            *self._needed("out", out))
-        check(lib().cchip_dropout_run(self._desc, io, _stream_ptr(stream)))
+        check(lib().cchip_dropout_run(self._desc, io, self._on(stream)))
 
     def backward(self, dout, dx, *, seed, offset=0, step=None, stream=None):
         """``dx = scale drop(dout)`` with the forward pass's mask; the residual's
@@ -400,7 +408,7 @@ class NormBlock(_RowOperator):
 
     def reserve(self, stream=None):
         """Allocate a stream's workspace ahead of the first backward call on it."""
-        self._workspace(_stream_ptr(stream), True)
+        self._workspace(self._on(stream), True)
 
     def _vectors(self, given):
         p = [0, 0, 0, 0, 0]
@@ -417,14 +425,14 @@ class NormBlock(_RowOperator):
         io = self._io.pack(*self._seed(seed, offset, step), *self._vectors(params), 0, 0, 0, 0, 0,
                            *self._needed("y", y), *self._rows("gate", gate), *self._rows("residual", residual),
                            *self._needed("h", h), *self._rows("n", n), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
-        check(lib().cchip_norm_block_forward(self._desc, io, _stream_ptr(stream)))
+        check(lib().cchip_norm_block_forward(self._desc, io, self._on(stream)))
 
     def backward(self, y, dh, dy, *, dn=None, h=None, gate=None, dgate=None, dresidual=None, grads=None, seed=0, offset=0,
                  step=None, workspace=None, stream=None, **params):
         """From y, gate, the forward pass's h (where it is normed again) and the
         gradients of h and n, write those of y, gate and residual and, for each
         name in ``grads``, of that parameter, summed over the rows."""
-        s = _stream_ptr(stream)
+        s = self._on(stream)
         io = self._io.pack(*self._seed(seed, offset, step), *self._vectors(params), *self._vectors(grads or {}),
                            *self._needed("y", y), *self._rows("gate", gate), 0, 0, *self._rows("h", h), 0, 0,
                            *self._needed("dh", dh), *self._rows("dn", dn), *self._needed("dy", dy),

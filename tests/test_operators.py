@@ -310,6 +310,16 @@ def test_what_is_no_array_is_refused():
         drop.forward(z.numpy(), z, seed=1)
 
 
+def test_a_call_on_another_device_is_refused(monkeypatch):
+    """The arrays are on the handle's device; kernels would run on the one
+    that is current."""
+    op = O.Dropout("f32", 4, 8, 0.5)
+    op._device, op._others = -1, True
+    monkeypatch.setattr(O.Device, "current", staticmethod(lambda: 3))
+    with pytest.raises(ValueError, match="made for device -1, called on device 3"):
+        op.forward(torch.zeros(4, 8), torch.zeros(4, 8), seed=1)
+
+
 def test_arrays_lie_in_their_buffers():
     class Memory:
         ptr, nbytes = 4096, 64
