@@ -140,17 +140,17 @@ class _Operator:
             raise ValueError("%s: no %s" % (self._who, name))
         if type(x) is Resident:
             x = Array(x.buf, x.dtype.name, x.shape)
-        if not all(hasattr(x, a) for a in ("shape", "dtype", "stride", "data_ptr", "get_device")):
-            raise ValueError("%s: %s is no array on a device" % (self._who, name))
-        if x.shape != shape and tuple(x.shape) != shape:
-            raise ValueError("%s: %s has shape %s, expected %s" % (self._who, name, _dims(x.shape), _dims(shape)))
-        d = x.dtype
+        try:
+            have, d, device, p, st = x.shape, x.dtype, x.get_device(), x.data_ptr(), x.stride()
+        except AttributeError:
+            raise ValueError("%s: %s is no array on a device" % (self._who, name)) from None
+        if have != shape and tuple(have) != shape:
+            raise ValueError("%s: %s has shape %s, expected %s" % (self._who, name, _dims(have), _dims(shape)))
         if _dtypes.get(d) != dtype and _dtype_name(d) != dtype:
             raise ValueError("%s: %s has dtype %s, expected %s" % (self._who, name, _dtype_name(d), dtype))
-        d = x.get_device()
-        if d != self._device and d is not None:
+        if device != self._device and device is not None:
             raise ValueError("%s: %s is not on device %s" % (self._who, name, self._device))
-        return x.data_ptr(), x.stride()
+        return p, st
 
     def _whole(self, name, x, dtype, shape):
         """The pointer of an array without gaps; 0 for None."""
