@@ -1049,3 +1049,44 @@ def test_norm_block_over_any_of_its_inputs(device, dtype, width):
                 op.forward(t["y"], t[a], t[b], gate=t["gate"], residual=t["residual"], seed=2, **wd)
                 torch.cuda.synchronize()
                 assert torch.equal(t[a], h) and torch.equal(t[b], n), (a, b)
+
+
+# ---- 16-bit results to their own rounding ------------------------------------
+
+# Half a unit of the last place, and what f32 sums (4e-6) or products of 16-bit
+# planes (three of 2^-17) add before it.
+ROUNDING = {"bf16": 2.0 ** -9, "f16": 2.0 ** -12}
+
+
+@pytest.mark.parametrize("dtype", list(ROUNDING))
+@pytest.mark.parametrize("case", [(50, 128, "rms", "none", "silu"), (40, 700, "layer", "rms", "sigmoid"), (30, 4096, "rms", "rms", "none"),
+                                  (12, 9000, "layer", "layer", "silu")])
+def test_norm_block_rounds_its_results_once(device, dtype, case):
+    x, w = norm_arrays(dtype, "f32", *case, seed=48)
+    how = (*case[2:], 0.7, 1e-5, 0.2, 11, 12)
+    op = O.NormBlock(dtype, *case[:2], norm=case[2], pre=case[3], gate=case[4], dropout=0.2, scale=0.7, eps=1e-5)
+    dev, wd = {k: v.cuda() for k, v in x.items()}, {k: v.cuda() for k, v in w.items()}
+    wide = {k: v.double().numpy() for k, v in {**x, **w}.items()}
+    got = {n: torch.empty_like(dev["y"]) for n in (("h", "n") if case[3] != "none" else ("h",))}
+    op.forward(dev["y"], got["h"], got.get("n"), gate=dev.get("gate"), residual=dev["residual"], seed=11, offset=12, **wd)
+    out = {n: torch.empty_like(dev["y"]) for n in ("y", "residual") + (("gate",) if "gate" in x else ())}
+    op.backward(dev["y"], dev["dh"], out["y"], dn=dev.get("dn"), h=dev.get("h"), gate=dev.get("gate"), dgate=out.get("gate"),
+                dresidual=out["residual"], seed=11, offset=12, **wd)
+    torch.cuda.synchronize()
+    for want, results in ((R.norm_block(wide, *how), got), (R.norm_block(wide, *how, back=True), out)):
+        for n, v in results.items():
+            close(v, want[n], n, ROUNDING[dtype] + 4e-6)
+
+
+@pytest.mark.parametrize("dtype", list(ROUNDING))
+@pytest.mark.parametrize("shape", [(2, 200, 2, 4, 128, 96), (3, 100, 8, 24, 128, 64), (2, 130, 1, 2, 100, 40), (3, 5, 2, 4, 64, 64)])
+@pytest.mark.parametrize("states", [False, True])
+def test_gated_delta_rounds_o_and_dv_once(device, dtype, shape, states):
+    x = arrays(dtype, *shape, seed=49, states=shape[0] if states else 0, back=True)
+    got = run_delta(x, dtype, back=True)
+    want = R.delta_batch({n: v.double().numpy() for n, v in x.items()}, None, shape[4] ** -0.5,
+                         x["state"].double().numpy() if states else None, True)
+    for n in ("o", "dv", "dbeta"):
+        close(got[n], want[n], n, ROUNDING[dtype] + 3 * 2.0 ** -17)
+    got = run_delta({n: v for n, v in x.items() if n not in ("do", "dstate_out")}, dtype)
+    close(got["o"], want["o"], "o", ROUNDING[dtype] + 3 * 2.0 ** -17)
