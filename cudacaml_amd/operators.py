@@ -112,6 +112,14 @@ def _stream_ptr(stream):
     return stream.cuda_stream
 
 
+def _stream_on(who, device, stream):
+    """The same for a handle of one device of several: a call while another is
+    current is refused, as its kernels would run there."""
+    if Device.current() != device:
+        raise ValueError("%s: made for device %d, called on device %d" % (who, device, Device.current()))
+    return _stream_ptr(stream)
+
+
 def _dims(shape):
     return "[" + ", ".join(str(d) for d in shape) + "]"
 
@@ -121,18 +129,13 @@ _NO_ROWS = (0, 0)
 
 class _Operator:
     _who = ""
+    _on = staticmethod(_stream_ptr)
 
     def __init__(self):
         self._device = Device.current() if Device.available() else None
-        self._others = self._device is not None and Device.count() > 1
+        if self._device is not None and Device.count() > 1:
+            self._on = functools.partial(_stream_on, self._who, self._device)
         self._workspaces = {}
-
-    def _on(self, stream):
-        """The stream's pointer; a call on another device than the handle's is
-        refused, as its kernels would run there."""
-        if self._others and Device.current() != self._device:
-            raise ValueError("%s: made for device %d, called on device %d" % (self._who, self._device, Device.current()))
-        return _stream_ptr(stream)
 
     def _view(self, name, x, dtype, shape):
         """The array's pointer and strides, or ValueError."""

@@ -313,9 +313,13 @@ def test_what_is_no_array_is_refused():
 def test_a_call_on_another_device_is_refused(monkeypatch):
     """The arrays are on the handle's device; kernels would run on the one
     that is current."""
-    op = O.Dropout("f32", 4, 8, 0.5)
-    op._device, op._others = -1, True
-    monkeypatch.setattr(O.Device, "current", staticmethod(lambda: 3))
+    now = [-1]
+    monkeypatch.setattr(O.Device, "available", staticmethod(lambda: True))
+    monkeypatch.setattr(O.Device, "count", staticmethod(lambda: 2))
+    monkeypatch.setattr(O.Device, "current", staticmethod(lambda: now[0]))
+    op = O.Dropout("f32", 4, 8, 0.5)  # on device -1, where the host's tensors are
+    assert op._on(5) == 5
+    now[0] = 3
     with pytest.raises(ValueError, match="made for device -1, called on device 3"):
         op.forward(torch.zeros(4, 8), torch.zeros(4, 8), seed=1)
 
