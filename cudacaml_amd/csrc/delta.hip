@@ -20,7 +20,7 @@ constexpr int64_t kStepTokens = 16;
 
 struct Layout {
   int64_t slots, slot_heads;
-  size_t record, record_back, states, us, scales, dots;  // bytes, all slots and heads
+  size_t record, record_back, states, us, scales, powers, o_powers, dots;  // bytes, all slots and heads
 };
 
 void check_op(const cchip_gated_delta *op) {
@@ -58,7 +58,9 @@ Layout layout_of(const cchip_gated_delta &op) {
     p.record = size_t(p.slot_heads) * record_bytes<M>(false);
     p.record_back = size_t(p.slot_heads) * record_bytes<M>(true);
     p.states = size_t(p.slot_heads) * padded_key_dim(op.key_dim) * padded_value_dim(op) * sizeof(typename M::Saved);
-    p.dots = size_t(p.slot_heads) * (padded_value_dim(op) / 16) * 4 * sizeof(float);
+    p.powers = sizeof(typename M::Saved) == 4 ? 0 : size_t(p.slot_heads) * 4 * (padded_value_dim(op) / 16);
+    p.dots = sizeof(typename M::Saved) == 4 ? size_t(p.slot_heads) * (padded_value_dim(op) / 16) * 4 * sizeof(float) : 0;
+    p.o_powers = sizeof(typename M::Saved) == 4 ? 0 : size_t(p.slot_heads) * kChunk * (padded_value_dim(op) / 16);
     p.us = size_t(p.slot_heads) * kChunk * padded_value_dim(op) * sizeof(typename M::Kept);
     p.scales = sizeof(typename M::Kept) == 4 ? 0 : size_t(p.slot_heads) * kChunk * (padded_value_dim(op) / 16) * sizeof(float);
   });
@@ -175,11 +177,14 @@ void check_workspace(const void *workspace, size_t have, size_t need) {
     throw InvalidArgument(strf("gated delta: the workspace needs %zu bytes aligned to 16, has %zu", need, workspace ? have : 0));
 }
 
+size_t backward_bytes(const Layout &p) { return p.states + p.us + p.scales + p.dots + p.o_powers + p.powers; }
+
 void lay_out(DeltaArgs &a, const Layout &p, char *saved) {
   a.records = saved;
   a.states = saved + p.record_back;
   a.us = a.states + p.states;
   a.u_scales = reinterpret_cast<float *>(a.us + p.us);
+  a.state_powers = reinterpret_cast<uint8_t *>(a.us + p.us + p.scales);
 }
 
 }  // namespace
@@ -191,8 +196,8 @@ int cchip_gated_delta_sizes(const cchip_gated_delta *op, size_t *forward, size_t
     check_op(op);
     const Layout p = layout_of(*op);
     if (forward) *forward = steps(*op, false) ? 0 : p.record;
-    if (backward) *backward = p.states + p.us + p.scales + p.dots;
-    if (saved) *saved = p.record_back + p.states + p.us + p.scales;
+    if (backward) *backward = backward_bytes(p);
+    if (saved) *saved = p.record_back + p.states + p.us + p.scales + p.powers;
   });
 }
 
@@ -227,13 +232,15 @@ int cchip_gated_delta_backward(const cchip_gated_delta *op, const cchip_gated_de
     DeltaArgs a = args_of(*op, *io, p, true);
     if (a.sequences == 0) return;
     lay_out(a, p, static_cast<char *>(io->saved));
-    check_workspace(workspace, workspace_bytes, p.states + p.us + p.scales + p.dots);
+    check_workspace(workspace, workspace_bytes, backward_bytes(p));
     check_apart(*op, *io, true);
     if (p.slots && workspace == io->saved) throw InvalidArgument("gated delta: the workspace is what the forward pass saved");
     a.grads = static_cast<char *>(workspace);
     a.ys = a.grads + p.states;
     a.y_scales = reinterpret_cast<float *>(a.ys + p.us);
     a.dots = reinterpret_cast<float *>(a.ys + p.us + p.scales);
+    a.o_powers = reinterpret_cast<uint8_t *>(a.ys + p.us + p.scales + p.dots);
+    a.grad_powers = a.o_powers + p.o_powers;
     delta_backward_launch(*op, a, (hipStream_t)stream);
   });
 }

@@ -50,7 +50,9 @@ struct DeltaArgs {
   char *grads;    // backward: dS after the chunk
   char *ys;       // backward: Y
   float *u_scales, *y_scales;  // of U and Y in f16: [16 columns][64]
-  float *dots;    // backward: sums that make <S, dS>, four for each 16 value columns
+  float *dots;                  // backward: sums that make <S, dS>, four for each 16 value columns, where those are f32
+  uint8_t *o_powers;            // backward: of the gradient of o, [16 columns][64]
+  uint8_t *state_powers, *grad_powers;  // of S and dS in f16: [16 columns][4 blocks of DK / 4 rows], the exponents of f32
   int64_t tokens, sequences;  // sequences: of the packed batch, or its rows
   int64_t slots;
   int chunks;  // of a row of the batch; unused where packed
@@ -61,17 +63,22 @@ struct DeltaArgs {
 
 // Element type, then the planes: NI of an input, NS of what makes a state
 // (S, T, X and U in their products), NO of S, P, U and Y where they make only
-// outputs. Saved is the type that S and dS are kept in for the backward pass,
-// read back in NB planes, and Kept that of U and Y: f16 with a power of two
-// for each token and 16 columns (11 bits, which two planes hold) or f32.
+// outputs. Saved is the type that S and dS are kept in for the backward pass
+// and Kept that of U and Y: f32 or, with powers of two (half_exponent), f16,
+// one for each token of U and Y and each DK / 4 rows of S and dS in the 16 or
+// 32 columns of a workgroup. NB: planes of M and B and, in f32, of S and dS
+// where the gradients of q and k are made.
 //
 // A product loses the most precise operand's worth of the other's rounding:
 // 2^-9 of a value in one plane of bf16, 2^-17 in two; states in f32 take
 // three. bf16 results are rounded to 2^-9 themselves, 1.7e-3 in the 2-norm.
 // o adds nothing to that; in one plane it would be 2.4e-3 off, for 363 us in
-// place of 376 (forward of 4 x 4096 tokens, 32 heads of 128). The gradients
-// of q, k, g and beta add the rounding of the saved S and dS, 2.4e-3 in all:
-// kept as f32 these would be another 0.5 GB there to write and to read.
+// place of 376 (forward of 4 x 4096 tokens, 32 heads of 128). Nor do the
+// gradients add to it: the 11 bits of f16 are exact on the f16 matrix
+// instruction. S and dS as bf16, and M and B in one plane, made dq and dk 2.4e-3
+// off, 3.5e-3 where keys are alike, and the four kernels of a training step
+// there 1410 us in place of 1440. Value columns of a head that are more than
+// 2^24 apart lose bits of the smaller ones' share in dq, dk, dg and dbeta.
 template <typename T_, int NI_, int NS_, int NO_, typename Saved_, int NB_, typename Kept_>
 struct Mode {
   typedef T_ T;
@@ -79,8 +86,8 @@ struct Mode {
   typedef Kept_ Kept;
   static constexpr int NI = NI_, NS = NS_, NO = NO_, NB = NB_;
 };
-typedef Mode<bf16, 1, 2, 2, bf16, 1, f16> ModeBf16;   // bf16 in and out
-typedef Mode<bf16, 1, 3, 2, bf16, 1, f16> ModeBf16S;  // with f32 states in or out
+typedef Mode<bf16, 1, 2, 2, f16, 2, f16> ModeBf16;   // bf16 in and out
+typedef Mode<bf16, 1, 3, 2, f16, 2, f16> ModeBf16S;  // with f32 states in or out
 typedef Mode<f16, 2, 3, 2, float, 2, float> ModeF16;
 typedef Mode<float, 3, 3, 3, float, 3, float> ModeF32;
 
@@ -376,7 +383,51 @@ __device__ __forceinline__ RawV<T, TV> load_block(const char *rows, int row, int
   return r;
 }
 
-// A token's share of U or Y as it is kept. Every lane of the token takes part.
+// What is kept in f16 is kept with a power of two, by which the largest of
+// the values that share it becomes 2^14 .. 2^15: those down to 2^-28 of it
+// have all of f16's 11 bits. `half_exponent` is the largest's, as f32 has it
+// and in the range that the powers have; the values are multiplied by
+// half_down of it and, read, by half_up.
+__device__ __forceinline__ float power(uint32_t x) { return __builtin_bit_cast(float, x << 23); }
+__device__ __forceinline__ uint32_t exponent(float x) { return __builtin_bit_cast(uint32_t, x) >> 23 & 0xFF; }
+__device__ __forceinline__ uint32_t half_exponent(float largest) {
+  const uint32_t e = exponent(largest);
+  return e < 15 ? 15 : e > 254 ? 254 : e;
+}
+__device__ __forceinline__ float half_down(uint32_t x) { return power(268 - x); }
+__device__ __forceinline__ float half_up(uint32_t x) { return power(x - 14); }
+constexpr int kHalfZero = 127 + 14;  // the half_exponent whose half_up is 1
+
+// A wave's rows of S or dS as they are kept, of a workgroup's columns from v0
+// on: one power for all of them.
+template <typename Saved, int DK, int TK, int TV>
+__device__ __forceinline__ void keep_state(char *all, uint8_t *powers, int64_t slot_head, int dvp, int v0, int w, int row, int y,
+                                           const f32x4 (&v)[TK][TV]) {
+  char *rows = all + (slot_head * dvp + v0 / 32 * 32) * (DK * int64_t(sizeof(Saved)));
+  if constexpr (sizeof(Saved) == 4) {
+#pragma unroll
+    for (int i = 0; i < TK; i++) put_block<float, TV>(rows, row + 16 * i, v0 % 32 + y, v[i]);
+  } else {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < TK; i++)
+#pragma unroll
+      for (int j = 0; j < 4 * TV; j++) m = fmaxf(m, fabsf(v[i][j / 4][j % 4]));
+    const uint32_t x = half_exponent(max_rows(max16(m)));
+#pragma unroll
+    for (int i = 0; i < TK; i++) {
+      f32x4 s[TV];
+#pragma unroll
+      for (int j = 0; j < TV; j++) s[j] = v[i][j] * half_down(x);
+      put_block<f16, TV>(rows, row + 16 * i, v0 % 32 + y, s);
+    }
+    const int l = threadIdx.x & 63;
+    if (l < TV) powers[(slot_head * (dvp / 16) + v0 / 16 + l) * 4 + w] = uint8_t(x);
+  }
+}
+
+// A token's share of U or Y as it is kept, of a workgroup's columns: one power
+// for all of them. Every lane of the token takes part.
 template <typename Kept, int TV>
 __device__ __forceinline__ void keep_block(char *all, float *scales, int64_t slot_head, int dvp, int v0, int t, int quad, int y,
                                            const f32x4 (&v)[TV]) {
@@ -387,14 +438,12 @@ __device__ __forceinline__ void keep_block(char *all, float *scales, int64_t slo
     float m = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4 * TV; i++) m = fmaxf(m, fabsf(v[i / 4][i % 4]));
-    const uint32_t e = __builtin_bit_cast(uint32_t, max_rows(m)) >> 23;
-    const uint32_t x = e < 1 ? 127 : e > 253 ? 253 : e;  // the largest becomes 1 .. 2 (zeros stay, the last binade 2 .. 8)
-    const float down = __builtin_bit_cast(float, (254 - x) << 23);
+    const uint32_t x = half_exponent(max_rows(m));
     f32x4 s[TV];
 #pragma unroll
-    for (int j = 0; j < TV; j++) s[j] = v[j] * down;
+    for (int j = 0; j < TV; j++) s[j] = v[j] * half_down(x);
     put_block<f16, TV>(rows, t, v0 % 32 + y, s);
-    if (quad < TV) scales[(slot_head * dvp + v0) * (kChunk / 16) + quad * kChunk + t] = __builtin_bit_cast(float, x << 23);
+    if (quad < TV) scales[(slot_head * dvp + v0) * (kChunk / 16) + quad * kChunk + t] = half_up(x);
   }
 }
 
@@ -405,6 +454,15 @@ __device__ __forceinline__ Raw8<T> load_block8(const char *rows, uint32_t at) {
   for (int i = 0; i < int(sizeof(T) * 8 / 16); i++)
     reinterpret_cast<u32x4 *>(&r)[i] = reinterpret_cast<const u32x4 *>(rows + at * uint32_t(sizeof(T)))[i];
   return r;
+}
+
+// Eight values that are kept in f16 with a power of two, or in f32.
+template <typename Kept>
+__device__ __forceinline__ Raw8<float> kept8(const Raw8<Kept> &r, float power) {
+  Raw8<float> x;
+#pragma unroll
+  for (int i = 0; i < 8; i++) x.x[i] = sizeof(Kept) < 4 ? power * float(r.x[i]) : float(r.x[i]);
+  return x;
 }
 
 // The first N planes of a fragment.

@@ -28,10 +28,9 @@ namespace {
 
 // The counterpart of delta_forward, laid out like it: BV value columns of a
 // head, E in registers, each chunk's rows asked for while the one after it is
-// computed. <S, E> is summed here, where E still is f32: of the two in bf16
-// it would be off by both their roundings. Bounded as delta_forward is, with
-// one more wait a chunk and the states read too: 390 us for 4 x 4096 tokens,
-// 32 bf16 heads of 128, 1.3 GB at 3.4 TB/s.
+// computed. Where they are kept as f32, <S, E> is summed here, with E at hand.
+// Bounded as delta_forward is, with one more wait a chunk: 375 us for 4 x 4096
+// tokens, 32 bf16 heads of 128, 1.0 GB at 2.7 TB/s.
 template <typename M, int DK, int BV, int A>
 __global__ __launch_bounds__(256, groups_a_unit<M>(DK, BV)) void delta_reverse(const DeltaArgs a, int blocks) {
   typedef typename M::T T;
@@ -40,6 +39,7 @@ __global__ __launch_bounds__(256, groups_a_unit<M>(DK, BV)) void delta_reverse(c
   constexpr int LDK = DK + 16, LDV = BV == 16 ? 24 : BV;
   constexpr int KP = 64 * LDK, EP = DK * LDV, XP = 64 * LDV;
   constexpr int TK = DK / 64, TV = BV / 16;
+  constexpr bool kDots = sizeof(Saved) == 4;
   typedef Record<M> R;
   __shared__ __align__(16) bf16 ks[NI * KP], qs[NI * KP], es[NS * EP], xs[NS * XP], os[NI * XP], gs[NS * XP];
   bf16 *const zs = es;  // E is done with when Z is made
@@ -76,7 +76,7 @@ __global__ __launch_bounds__(256, groups_a_unit<M>(DK, BV)) void delta_reverse(c
   };
   auto record = [&](int i) { return a.records + ((sq.slot + i) * a.hv + h) * R::bytes(true); };
   Raw8<T> rk[DK / 32], rq[DK / 32], ro;
-  RawV<Saved, TV> rs[TK];
+  RawV<float, TV> rs[kDots ? TK : 1];
   Frag<NS> tt[2], pt[2];  // rows 16 w .. of T^T and P^T: terms from the diagonal on
   float og, gam, last, beta, end;
   auto fetch = [&](int i) {
@@ -87,9 +87,11 @@ __global__ __launch_bounds__(256, groups_a_unit<M>(DK, BV)) void delta_reverse(c
       rk[j] = load_head8<A, T>(a.k, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk);
       rq[j] = load_head8<A, T>(a.q, c, hk, at / (DK / 8), at % (DK / 8) * 8, a.dk);
     }
-    const char *from = a.states + (((sq.slot + i) * a.hv + h) * a.dvp + dv0 / 32 * 32) * DK * int64_t(sizeof(Saved));
+    if constexpr (kDots) {
+      const char *from = a.states + (((sq.slot + i) * a.hv + h) * a.dvp + dv0 / 32 * 32) * DK * int64_t(sizeof(Saved));
 #pragma unroll
-    for (int j = 0; j < TK; j++) rs[j] = load_block<Saved, TV>(from, x0 + 16 * j, dv0 % 32 + y0);
+      for (int j = 0; j < TK; j++) rs[j] = load_block<float, TV>(from, x0 + 16 * j, dv0 % 32 + y0);
+    }
     if (has_o) {
       ro = load_head8<A, T>(a.d_o, c, h, ot, dv0 + od, a.dv);
       og = reinterpret_cast<const float *>(record(i) + R::Decay)[ot];
@@ -136,6 +138,14 @@ __global__ __launch_bounds__(256, groups_a_unit<M>(DK, BV)) void delta_reverse(c
     if (has_o) {
       const Raw8<T> raw = keep_head8<A>(ro, c, ot, dv0 + od, a.dv);
       put_frag<NI>(os + ot * LDV + od, XP, frag_of<NI>(raw));
+      if (sizeof(Saved) < 4) {  // the largest of a token's in these columns, for delta_gradients
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(float(raw.x[i])));
+        m = fmaxf(m, CCHIP_QUAD(m, 0xB1));
+        if (TV == 2) m = fmaxf(m, CCHIP_QUAD(m, 0x4E));
+        if (od < 8 * TV) a.o_powers[(slot_head * (a.dvp / 16) + dv0 / 16 + od / 8) * kChunk + ot] = uint8_t(half_exponent(m));
+      }
       const float f = a.scale * og;
       Raw8<float> up;
 #pragma unroll
@@ -146,22 +156,22 @@ __global__ __launch_bounds__(256, groups_a_unit<M>(DK, BV)) void delta_reverse(c
     for (int i = 0; i < TK; i++)
 #pragma unroll
       for (int j = 0; j < TV; j++) put_four<NS>(es + (x0 + 16 * i) * LDV + y0 + 4 * j, EP, e[i][j]);
-    float dot = 0.0f;
+    if constexpr (kDots) {
+      float dot = 0.0f;
 #pragma unroll
-    for (int i = 0; i < TK; i++)
+      for (int i = 0; i < TK; i++)
 #pragma unroll
-      for (int j = 0; j < 4 * TV; j++) dot += rs[i][j] * e[i][j / 4][j % 4];
-    dot = sum64(dot);
-    if (l == 0) {
-      float *dots = a.dots + (slot_head * (a.dvp / 16) + dv0 / 16) * 4;
-      dots[w] = dot;
-      if (TV == 2) dots[4 + w] = 0.0f;
+        for (int j = 0; j < 4 * TV; j++) dot += rs[i][j] * e[i][j / 4][j % 4];
+      dot = sum64(dot);
+      if (l == 0) {
+        float *dots = a.dots + (slot_head * (a.dvp / 16) + dv0 / 16) * 4;
+        dots[w] = dot;
+        if (TV == 2) dots[4 + w] = 0.0f;
+      }
     }
     __syncthreads();
     fetch(next);
-    char *to = a.grads + (slot_head * a.dvp + dv0 / 32 * 32) * DK * int64_t(sizeof(Saved));
-#pragma unroll
-    for (int i = 0; i < TK; i++) put_block<Saved, TV>(to, x0 + 16 * i, dv0 % 32 + y0, e[i]);
+    keep_state<Saved, DK, TK, TV>(a.grads, a.grad_powers, slot_head, a.dvp, dv0, w, x0, y0, e);
 
     Levels<NS> ke[TV], po[TV];
     {
@@ -264,16 +274,38 @@ __global__ __launch_bounds__(256, groups_a_unit<M>(DK, BV)) void delta_reverse(c
         }
 }
 
+// Eight values in f16 into LDS, times 2^n for n <= 0.
+__device__ __forceinline__ void put_lower(bf16 *to, const Raw8<f16> &x, int n) {
+  const f16 down = f16(n < -126 ? 0.0f : power(uint32_t(127 + n)));
+  *reinterpret_cast<f16x8 *>(to) = __builtin_bit_cast(f16x8, x) * down;
+}
+template <typename T>
+__device__ __forceinline__ void put_lower(bf16 *, const Raw8<T> &, int) {}
+
+// The operand of 16 rows from row0 on of f16 rows in LDS, and a product of two.
+__device__ __forceinline__ f16x8 half_row(const bf16 *m, int ld, int row0) {
+  const int l = threadIdx.x & 63;
+  return *reinterpret_cast<const f16x8 *>(m + (row0 + (l & 15)) * ld + (l >> 4) * 8);
+}
+__device__ __forceinline__ f32x4 mma_half(f32x4 c, f16x8 a, f16x8 b) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
 // A workgroup of eight waves a chunk and key head, its value heads one after
 // another (so dQ and dK of a shared head are summed in registers, in an order
 // that is always the same). Products are taken transposed, as in the forward
 // pass: wave w has tokens 16 (w % 4) .. of each and part w / 4 of the rest,
 // and a lane one token. S, E, U, Y and dO pass through LDS 32 value columns
 // at a time, the next 32 being read while the products of these are made.
-// Four parts and 16 waves would hide more but do not fit in 128 registers
-// (790 us where this takes 475, for 256 chunks of 32 bf16 heads of 128, which
-// reads and writes 1.3 GB). One workgroup a unit is what LDS and registers
-// allow, so its waits for LDS and memory are not covered by another's work.
+// Where they are f16 (kHalf, dO made so), the values of a token or of a block
+// of rows of S and E are brought to the largest power of two that they have in
+// any columns, so that products add up over all columns and are scaled once
+// for a head: 525 us for 256 chunks of 32 bf16 heads of 128, 1.3 GB at 2.5
+// TB/s, where the same accuracy from pairs of bf16 planes took 555 and single
+// ones 480. Four parts and 16 waves would hide more but do not fit in 128
+// registers (790 us with single planes). One workgroup a unit is what
+// registers allow, so its waits for LDS and memory are not covered by
+// another's work.
 template <typename M, int DK, int A>
 __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
   typedef typename M::T T;
@@ -283,14 +315,18 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
   constexpr int LDK = DK + 16, KP = 64 * LDK, LDS = 40, SP = DK * LDS, UP = 64 * LDS, LDM = 72, MP = 64 * LDM;
   constexpr int JK = DK / 16 / P, JS = 4 / P;  // 16-wide tiles of a part: of a key, of the tokens
   constexpr bool kAll = NB < 3;               // everything in LDS at a time; else E after S, and Y and dO not
+  constexpr bool kHalf = sizeof(Saved) == 2;  // slices as f16 with powers of two, on the f16 matrix instruction
+  constexpr int PB = kHalf ? 1 : NB, PO = kHalf ? 1 : NO, PI = kHalf ? 1 : NI;  // planes of a slice
   typedef Record<M> R;
-  constexpr int kSlices = (kAll ? 2 : 1) * NB * SP + NO * UP + (kAll ? (NO + NI) * UP : 0), kMs = (kAll ? 2 : 1) * NB * MP;
+  constexpr int kSlices = (kAll ? 2 : 1) * PB * SP + PO * UP + (kAll ? (PO + PI) * UP : 0), kMs = (kAll ? 2 : 1) * NB * MP;
   __shared__ __align__(16) bf16 ks[NI * KP], qs[NI * KP], slice[kSlices > kMs ? kSlices : kMs];
   __shared__ double cs[64];
   __shared__ __align__(16) float down[4][64];
   __shared__ float row_c[P][64], row_b[P][64], row_y[64], total[4 * P];
-  bf16 *const us = slice, *const ss = slice + NO * UP, *const es = kAll ? ss + NB * SP : ss;
-  bf16 *const yl = es + NB * SP, *const ol = yl + NO * UP;  // Y and dO if kAll
+  // kHalf: the powers that hold in all columns of a head, of the tokens and of the blocks of DK / 4 rows of S and E
+  __shared__ __align__(16) uint32_t u_top[64], y_top[64], o_top[64], s_top[8];
+  bf16 *const us = slice, *const ss = slice + PO * UP, *const es = kAll ? ss + PB * SP : ss;
+  bf16 *const yl = es + PB * SP, *const ol = yl + PO * UP;  // Y and dO if kAll
   bf16 *const ms = slice, *const bs = kAll ? slice + NB * MP : slice;
 
   const int64_t slot = block_index() / a.hk;
@@ -349,15 +385,24 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
     const char *Y = a.ys + slot_head * kChunk * a.dvp * int64_t(sizeof(Kept));
     const float *u_scales = a.u_scales + slot_head * (kChunk / 16) * a.dvp, *y_scales = a.y_scales + slot_head * (kChunk / 16) * a.dvp;
 
+    const int groups = a.dvp / 16;
+    const uint8_t *s_powers = a.state_powers + slot_head * groups * 4, *e_powers = a.grad_powers + slot_head * groups * 4;
+    const uint8_t *o_powers = a.o_powers + slot_head * groups * kChunk;
+
     Raw8<Saved> rs, re;
     Raw8<Kept> ru;
     Raw8<float> ry;
     Raw8<T> ro, rv;
     float scale = 1.0f;
+    uint8_t ps = 0, pe = 0;  // S and E's exponents
     auto fetch = [&](int v0) {
       if (has_s) {
         rs = load_block8<Saved>(S, uint32_t(v0 * DK + sx * 32 + sv));
         re = load_block8<Saved>(E, uint32_t(v0 * DK + sx * 32 + sv));
+        if (kHalf) {
+          ps = s_powers[(v0 + sv) / 16 * 4 + sx / (DK / 4)];
+          pe = e_powers[(v0 + sv) / 16 * 4 + sx / (DK / 4)];
+        }
       }
       if (kAll) {
         ru = load_block8<Kept>(second ? Y : U, uint32_t(v0 * 64 + ux * 32 + sv));
@@ -381,70 +426,158 @@ __global__ __launch_bounds__(512, 2) void delta_gradients(const DeltaArgs a) {
         if (l >= d) run += up;
       }
     }
+    if (kHalf && w >= 4) {
+      // eight groups' at a time, so that they are waited for at once
+      auto largest = [&](auto of) {
+        uint32_t top = 1;
+        for (int g = 0; g < groups; g += 8) {
+          uint32_t x[8];
+#pragma unroll
+          for (int i = 0; i < 8; i++) x[i] = of(min(g + i, groups - 1));
+#pragma unroll
+          for (int i = 0; i < 8; i++) top = max(top, x[i]);
+        }
+        return top;
+      };
+      if (w < 6) {
+        const float *scales = (w == 4 ? u_scales : y_scales) + l;
+        (w == 4 ? u_top : y_top)[l] = largest([&](int g) { return exponent(scales[g * kChunk]); });
+      } else if (w == 6) {
+        o_top[l] = largest([&](int g) { return uint32_t(o_powers[g * kChunk + l]); });
+      } else if (l < 8) {
+        const uint8_t *powers = l < 4 ? s_powers + l : e_powers + l - 4;
+        s_top[l] = largest([&](int g) { return uint32_t(powers[g * 4]); });
+      }
+    }
     __syncthreads();  // the head before is done with LDS
     if (w == 0) cs[l] = run;
 
     f32x4 os[JK] = {}, ys[JK] = {}, ue[JK] = {}, ou[JS] = {}, yu[JS] = {};
     float yv = 0.0f, se = 0.0f;  // yv: of row ux (kAll) or t, this thread's columns
-    for (int i = tid; i < a.dvp / 4; i += kThreads) se += a.dots[slot_head * (a.dvp / 4) + i];
+    if (!kHalf)
+      for (int i = tid; i < a.dvp / 4; i += kThreads) se += a.dots[slot_head * (a.dvp / 4) + i];
     for (int v0 = 0; v0 < a.dvp; v0 += 32) {
       Frag<NI> fo;
       Frag<NO> fy;
       const Raw8<Saved> late = re;
-      if (has_s) {
-        put_frag<NB>(ss + sx * LDS + sv, SP, frag_of<NB>(rs));
-        if (kAll) put_frag<NB>(es + sx * LDS + sv, SP, frag_of<NB>(re));
-      }
-      if (kAll) {
-        Raw8<float> u;
+      if constexpr (kHalf) {
+        if (has_s) {
+          const int at = sx / (DK / 4);
+          float dot = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) u.x[i] = sizeof(Kept) < 4 ? scale * float(ru.x[i]) : float(ru.x[i]);
-        put_frag<NO>((second ? yl : us) + ux * LDS + sv, UP, frag_of<NO>(u));
+          for (int i = 0; i < 8; i++) dot += float(rs.x[i]) * float(re.x[i]);
+          se += ldexpf(dot, int(ps) + int(pe) - 2 * kHalfZero);
+          put_lower(ss + sx * LDS + sv, rs, int(ps) - int(s_top[at]));
+          put_lower(es + sx * LDS + sv, re, int(pe) - int(s_top[4 + at]));
+        }
+        put_lower((second ? yl : us) + ux * LDS + sv, ru, int(exponent(scale)) - int((second ? y_top : u_top)[ux]));
         const Raw8<T> x = keep_head8<A>(ro, c, ux, v0 + sv, a.dv);
         if (second) {
+          const Raw8<float> u = kept8(ru, scale);
 #pragma unroll
           for (int i = 0; i < 8; i++) yv += u.x[i] * float(x.x[i]);
         } else {
-          put_frag<NI>(ol + ux * LDS + sv, UP, frag_of<NI>(x));
+          const float down = half_down(o_top[ux]);
+          f16x8 o;
+#pragma unroll
+          for (int i = 0; i < 8; i++) o[i] = f16(float(x.x[i]) * down);
+          *reinterpret_cast<f16x8 *>(ol + ux * LDS + sv) = o;
         }
       } else {
-        if (!second) put_frag<NO>(us + ux * LDS + sv, UP, frag_of<NO>(ru));
-        fo = frag_of<NI>(keep_head8<A>(ro, c, t, v0 + 8 * quad, a.dv));
-        fy = frag_of<NO>(ry);
-        const Raw8<T> v = keep_head8<A>(rv, c, t, v0 + 8 * quad, a.dv);
+        if (has_s) {
+          put_frag<NB>(ss + sx * LDS + sv, SP, frag_of<NB>(rs));
+          if (kAll) put_frag<NB>(es + sx * LDS + sv, SP, frag_of<NB>(re));
+        }
+        if (kAll) {
+          put_frag<NO>((second ? yl : us) + ux * LDS + sv, UP, frag_of<NO>(ru));
+          const Raw8<T> x = keep_head8<A>(ro, c, ux, v0 + sv, a.dv);
+          if (second) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) yv += ry.x[i] * float(v.x[i]);
+            for (int i = 0; i < 8; i++) yv += ru.x[i] * float(x.x[i]);
+          } else {
+            put_frag<NI>(ol + ux * LDS + sv, UP, frag_of<NI>(x));
+          }
+        } else {
+          if (!second) put_frag<NO>(us + ux * LDS + sv, UP, frag_of<NO>(ru));
+          fo = frag_of<NI>(keep_head8<A>(ro, c, t, v0 + 8 * quad, a.dv));
+          fy = frag_of<NO>(ry);
+          const Raw8<T> v = keep_head8<A>(rv, c, t, v0 + 8 * quad, a.dv);
+#pragma unroll
+          for (int i = 0; i < 8; i++) yv += ry.x[i] * float(v.x[i]);
+        }
       }
       __syncthreads();
       if (v0 + 32 < a.dvp) fetch(v0 + 32);
-      if (kAll) {
-        fo = frag_row<NI>(ol, UP, LDS, 16 * wr, 0);
-        fy = frag_row<NO>(yl, UP, LDS, 16 * wr, 0);
+      if constexpr (kHalf) {
+        const f16x8 ho = half_row(ol, LDS, 16 * wr), hy = half_row(yl, LDS, 16 * wr), hu = half_row(us, LDS, 16 * wr);
+#pragma unroll
+        for (int j = 0; j < JK; j++) {
+          const int x = 16 * (JK * part + j);
+          const f16x8 hs = half_row(ss, LDS, x);
+          os[j] = mma_half(os[j], hs, ho);
+          ys[j] = mma_half(ys[j], hs, hy);
+          ue[j] = mma_half(ue[j], half_row(es, LDS, x), hu);
+        }
+#pragma unroll
+        for (int j = 0; j < JS; j++)
+          if (JS * part + j <= wr) {
+            const f16x8 h = half_row(us, LDS, 16 * (JS * part + j));
+            ou[j] = mma_half(ou[j], h, ho);
+            yu[j] = mma_half(yu[j], h, hy);
+          }
+        __syncthreads();
+      } else {
+        if (kAll) {
+          fo = frag_row<NI>(ol, UP, LDS, 16 * wr, 0);
+          fy = frag_row<NO>(yl, UP, LDS, 16 * wr, 0);
+        }
+        const Frag<NO> fu = frag_row<NO>(us, UP, LDS, 16 * wr, 0);
+#pragma unroll
+        for (int j = 0; j < JK; j++) {
+          const int x = 16 * (JK * part + j);
+          const Frag<NB> fs = frag_row<NB>(ss, SP, LDS, x, 0);
+          os[j] = mma(os[j], fs, fo);
+          ys[j] = mma(ys[j], fs, fy);
+          if (kAll) ue[j] = mma(ue[j], frag_row<NB>(es, SP, LDS, x, 0), fu);
+        }
+#pragma unroll
+        for (int j = 0; j < JS; j++)
+          if (JS * part + j <= wr) {
+            const Frag<NO> f = frag_row<NO>(us, UP, LDS, 16 * (JS * part + j), 0);
+            ou[j] = mma(ou[j], f, fo);
+            yu[j] = mma(yu[j], f, fy);
+          }
+        __syncthreads();
+        if (!kAll) {
+          if (has_s) put_frag<NB>(es + sx * LDS + sv, SP, frag_of<NB>(late));
+          __syncthreads();
+#pragma unroll
+          for (int j = 0; j < JK; j++) ue[j] = mma(ue[j], frag_row<NB>(es, SP, LDS, 16 * (JK * part + j), 0), fu);
+          __syncthreads();
+        }
       }
-      const Frag<NO> fu = frag_row<NO>(us, UP, LDS, 16 * wr, 0);
+    }
+    if constexpr (kHalf) {
+      const int u = int(u_top[t]) - 127, y = int(y_top[t]) - 127, o = int(o_top[t]) - kHalfZero;
 #pragma unroll
       for (int j = 0; j < JK; j++) {
-        const int x = 16 * (JK * part + j);
-        const Frag<NB> fs = frag_row<NB>(ss, SP, LDS, x, 0);
-        os[j] = mma(os[j], fs, fo);
-        ys[j] = mma(ys[j], fs, fy);
-        if (kAll) ue[j] = mma(ue[j], frag_row<NB>(es, SP, LDS, x, 0), fu);
+        const int at = 16 * (JK * part + j) / (DK / 4);
+        const int sn = int(s_top[at]) - kHalfZero, en = int(s_top[4 + at]) - kHalfZero;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          os[j][r] = ldexpf(os[j][r], sn + o);
+          ys[j][r] = ldexpf(ys[j][r], sn + y);
+          ue[j][r] = ldexpf(ue[j][r], en + u);
+        }
       }
 #pragma unroll
       for (int j = 0; j < JS; j++)
-        if (JS * part + j <= wr) {
-          const Frag<NO> f = frag_row<NO>(us, UP, LDS, 16 * (JS * part + j), 0);
-          ou[j] = mma(ou[j], f, fo);
-          yu[j] = mma(yu[j], f, fy);
-        }
-      __syncthreads();
-      if (!kAll) {
-        if (has_s) put_frag<NB>(es + sx * LDS + sv, SP, frag_of<NB>(late));
-        __syncthreads();
 #pragma unroll
-        for (int j = 0; j < JK; j++) ue[j] = mma(ue[j], frag_row<NB>(es, SP, LDS, 16 * (JK * part + j), 0), fu);
-        __syncthreads();
-      }
+        for (int r = 0; r < 4; r++) {
+          const int n = int(u_top[s0 + 16 * j + r]) - 127;
+          ou[j][r] = ldexpf(ou[j][r], n + o);
+          yu[j][r] = ldexpf(yu[j][r], n + y);
+        }
     }
     if (kAll) {
       yv += __shfl_xor(yv, 1, 64);

@@ -144,9 +144,7 @@ __global__ __launch_bounds__(256, groups_a_unit<M>(DK, BV)) void delta_forward(c
     __syncthreads();
     fetch_k(next);
     if (Back) {
-      char *to = a.states + (((sq.slot + ci) * a.hv + h) * a.dvp + dv0 / 32 * 32) * DK * int64_t(sizeof(Saved));
-#pragma unroll
-      for (int i = 0; i < TK; i++) put_block<Saved, TV>(to, x0 + 16 * i, dv0 % 32 + y0, s[i]);
+      keep_state<Saved, DK, TK, TV>(a.states, a.state_powers, (sq.slot + ci) * a.hv + h, a.dvp, dv0, w, x0, y0, s);
     }
 
     f32x4 kS[TV], o[TV] = {};

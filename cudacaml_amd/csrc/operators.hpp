@@ -17,6 +17,7 @@ typedef __bf16 bf16;
 typedef _Float16 f16;
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
@@ -205,15 +206,26 @@ __device__ __forceinline__ void put_frag(bf16 *at, int plane, const Frag<N> &f) 
 // Sum over the 16 lanes of a row of lanes by rotations within it, and over
 // the wave by swapping its rows and then its halves: every lane gets it, and
 // nothing goes through LDS.
-__device__ __forceinline__ float sum16(float x) {
 #define CCHIP_ROTATED(x, n) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + n, 0xf, 0xf, true))
+__device__ __forceinline__ float sum16(float x) {
   x += CCHIP_ROTATED(x, 8);
   x += CCHIP_ROTATED(x, 4);
   x += CCHIP_ROTATED(x, 2);
   x += CCHIP_ROTATED(x, 1);
-#undef CCHIP_ROTATED
   return x;
 }
+
+// The largest of the 16 lanes of a row.
+__device__ __forceinline__ float max16(float x) {
+  x = fmaxf(x, CCHIP_ROTATED(x, 8));
+  x = fmaxf(x, CCHIP_ROTATED(x, 4));
+  x = fmaxf(x, CCHIP_ROTATED(x, 2));
+  return fmaxf(x, CCHIP_ROTATED(x, 1));
+}
+#undef CCHIP_ROTATED
+
+// x of another lane of the same four: 0xB1 the neighbour's, 0x4E that two on.
+#define CCHIP_QUAD(x, order) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), order, 0xf, 0xf, true))
 
 // x of the same column summed over the four rows of 16 lanes.
 __device__ __forceinline__ float sum_rows(float x) {

@@ -1090,3 +1090,56 @@ def test_gated_delta_rounds_o_and_dv_once(device, dtype, shape, states):
         close(got[n], want[n], n, ROUNDING[dtype] + 3 * 2.0 ** -17)
     got = run_delta({n: v for n, v in x.items() if n not in ("do", "dstate_out")}, dtype)
     close(got["o"], want["o"], "o", ROUNDING[dtype] + 3 * 2.0 ** -17)
+
+
+# ---- gradients of 16-bit heads to their own rounding -------------------------
+
+# What a bf16 or f16 gradient of q and k adds to its rounding: S, dS, U and Y in
+# 11 bits and M and B in 16, a few roundings of 2^-12 in 2^-9 or of as much in
+# 2^-12 (where S and dS are f32): 2^-9 (1 + 1/8), and twice 2^-12.
+GRADIENT = {"bf16": 2.0 ** -9 * 1.125, "f16": 2.0 ** -11}
+
+
+@pytest.mark.parametrize("dtype", list(GRADIENT))
+@pytest.mark.parametrize("alike", [0.0, 1.0, 4.0])
+@pytest.mark.parametrize("shape", [(2, 200, 2, 4, 128, 96), (3, 100, 8, 24, 128, 64), (2, 130, 1, 2, 64, 40)])
+def test_gated_delta_gradients_of_keys_that_are_alike(device, dtype, alike, shape):
+    """Keys and queries around one direction: differences of the parts that
+    make dq and dk are smaller than the parts, and what those lose shows."""
+    x = arrays(dtype, *shape, seed=51, back=True)
+    g = torch.Generator().manual_seed(52)
+    mean = alike * torch.randn(1, 1, shape[2], shape[4], generator=g)
+    for n in ("q", "k"):
+        x[n] = torch.nn.functional.normalize(torch.randn(x[n].shape, generator=g) + mean, dim=-1).to(TYPES[dtype])
+    got = run_delta(x, dtype, back=True)
+    want = R.delta_batch({n: v.double().numpy() for n, v in x.items()}, None, shape[4] ** -0.5, None, True)
+    for n in ("dq", "dk"):
+        close(got[n], want[n], n, GRADIENT[dtype])
+
+
+@pytest.mark.parametrize("up", [1e33, 1e-33])
+def test_gated_delta_values_as_far_from_one_as_bf16_has_them(device, up):
+    """v far up and the gradient of o as far down, and the other way round:
+    the gradients of q, k, g and beta, products of the two, are about 1."""
+    x = arrays("bf16", 2, 130, 1, 2, 64, 64, seed=53, back=True)
+    x["v"] = (x["v"].float() * up).bfloat16()
+    x["do"] = (x["do"].float() / up).bfloat16()
+    check_delta(x, "bf16", back=True)
+
+
+@pytest.mark.parametrize("shape", [(2, 130, 1, 2, 64, 96), (3, 100, 8, 24, 128, 96)])
+def test_gated_delta_columns_of_different_size(device, shape):
+    """Value columns 2^20 apart whose gradients of o are as far apart the other
+    way: every column has its share of dq, dk, dg and dbeta."""
+    x = arrays("bf16", *shape, seed=54, back=True)
+    size = torch.ones(shape[5])
+    size[:32], size[32:48] = 2.0 ** 10, 2.0 ** -10
+    x["v"] = (x["v"].float() * size).bfloat16()
+    x["do"] = (x["do"].float() / size).bfloat16()
+    got = run_delta(x, "bf16", back=True)
+    want = R.delta_batch({n: v.double().numpy() for n, v in x.items()}, None, shape[4] ** -0.5, None, True)
+    for n in ("dq", "dk", "dg", "dbeta"):
+        close(got[n], want[n], n)
+    for lo, hi in ((0, 32), (32, 48), (48, 96)):
+        for n in ("o", "dv"):
+            close(got[n][..., lo:hi], want[n][..., lo:hi], "%s %d" % (n, lo))
