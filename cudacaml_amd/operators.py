@@ -19,7 +19,7 @@ free of both.
 Arrays are ``Array``, ``backend_hip.Resident`` or anything with ``data_ptr()``,
 ``get_device()``, ``dtype``, ``shape`` and ``stride()``, such as a tensor of
 a GPU framework; their last dimension is contiguous, the others may have any
-stride. A wrong shape, type or stride raises ``ValueError`` before any device
+stride (tokens of the gated delta rule one of 0 to 2^23 elements). A wrong shape, type or stride raises ``ValueError`` before any device
 work.
 """
 

@@ -66,10 +66,10 @@ typedef struct {
   float scale;
 } cchip_gated_delta;
 
-/* What a call writes overlaps nothing that it reads, but for state_out.
-   A tensor [batch][token][head][dim]: the distances, in elements, of
-   neighbours along the first three; the elements of a head are adjacent. g
-   and beta have no last dimension. */
+/* What a call writes overlaps nothing that it reads, but for state_out, nor
+   itself. A tensor [batch][token][head][dim]: the distances, in elements, of
+   neighbours along the first three, of tokens 0 to 2^23; the elements of a
+   head are adjacent. g and beta have no last dimension. */
 typedef struct {
   void *data;
   int64_t batch, token, head;
