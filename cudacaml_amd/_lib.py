@@ -104,6 +104,11 @@ class GatedDeltaDesc(ctypes.Structure):
                 ("scale", ctypes.c_float)]
 
 
+class AttentionDesc(ctypes.Structure):
+    _fields_ = [("dtype", c_int), ("batch", c_i64), ("tokens", c_i64), ("sequences", c_i64), ("keys", c_i64),
+                ("heads", c_int), ("kv_heads", c_int), ("head_dim", c_int), ("scale", ctypes.c_float)]
+
+
 class DropoutDesc(ctypes.Structure):
     _fields_ = [("dtype", c_int), ("rows", c_i64), ("cols", c_i64), ("p", ctypes.c_double), ("scale", ctypes.c_float)]
 
@@ -114,15 +119,35 @@ class NormBlockDesc(ctypes.Structure):
                 ("p", ctypes.c_double)]
 
 
+class HeadNormDesc(ctypes.Structure):
+    _fields_ = [("dtype", c_int), ("weight_dtype", c_int), ("batch", c_i64), ("tokens", c_i64), ("keys", c_i64),
+                ("heads", c_int), ("kv_heads", c_int), ("head_dim", c_int), ("rotary", c_int), ("interleaved", c_int),
+                ("norm", c_int), ("eps", ctypes.c_float)]
+
+
+class EmbeddingDesc(ctypes.Structure):
+    _fields_ = [("dtype", c_int), ("weight_dtype", c_int), ("tokens", c_i64), ("vocab", c_i64), ("width", c_i64),
+                ("scale", ctypes.c_float)]
+
+
 # The io structures hold 64-bit words only; callers pack them into bytes.
 OPERATOR_SIGNATURES = {
     "cchip_gated_delta_sizes": (c_int, [P(GatedDeltaDesc), P(c_size), P(c_size), P(c_size)]),
     "cchip_gated_delta_forward": (c_int, [P(GatedDeltaDesc), c_cp, c_vp, c_size, c_vp]),
     "cchip_gated_delta_backward": (c_int, [P(GatedDeltaDesc), c_cp, c_vp, c_size, c_vp]),
+    "cchip_attention_sizes": (c_int, [P(AttentionDesc), P(c_size), P(c_size), P(c_size)]),
+    "cchip_attention_forward": (c_int, [P(AttentionDesc), c_cp, c_vp, c_size, c_vp]),
+    "cchip_attention_backward": (c_int, [P(AttentionDesc), c_cp, c_vp, c_size, c_vp]),
     "cchip_dropout_run": (c_int, [P(DropoutDesc), c_cp, c_vp]),
     "cchip_norm_block_forward": (c_int, [P(NormBlockDesc), c_cp, c_vp]),
     "cchip_norm_block_workspace": (c_int, [P(NormBlockDesc), P(c_size)]),
     "cchip_norm_block_backward": (c_int, [P(NormBlockDesc), c_cp, c_vp, c_size, c_vp]),
+    "cchip_head_norm_forward": (c_int, [P(HeadNormDesc), c_cp, c_vp]),
+    "cchip_head_norm_workspace": (c_int, [P(HeadNormDesc), P(c_size)]),
+    "cchip_head_norm_backward": (c_int, [P(HeadNormDesc), c_cp, c_vp, c_size, c_vp]),
+    "cchip_embedding_forward": (c_int, [P(EmbeddingDesc), c_cp, c_vp]),
+    "cchip_embedding_workspace": (c_int, [P(EmbeddingDesc), P(c_size)]),
+    "cchip_embedding_backward": (c_int, [P(EmbeddingDesc), c_cp, c_vp, c_size, c_vp]),
 }
 
 _lib = None

@@ -21,17 +21,13 @@
 #include <type_traits>
 
 #include "../../include/cchip_operators.h"
+#include "heads.hpp"
 #include "operators.hpp"
 
 namespace cchip {
 namespace op {
 
 constexpr int kChunk = 64;
-
-struct Heads {
-  char *p;  // elements of the operator's type
-  int64_t b, t, h;
-};
 
 struct DeltaArgs {
   Heads q, k, v, g, beta, o;

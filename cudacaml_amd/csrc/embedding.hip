@@ -1,0 +1,423 @@
+// Embedding: rows of a table by token, and the table's gradient, which sums
+// the rows of equal tokens in the tokens' order: they are sorted first, so
+// that no sum depends on which workgroup comes first.
+
+#include "../../include/cchip_operators.h"
+#include "operators.hpp"
+#include "rows.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+namespace cchip {
+namespace op {
+namespace {
+
+struct EmbeddingArgs {
+  const int32_t *ids;
+  Rows weight, out, dout, dweight;
+  int64_t tokens, vocab, width;
+  uint32_t per_row;  // groups of 8 columns
+  uint64_t groups;   // of all tokens' rows
+  float scale;
+  bool accumulate;
+  // sorting
+  uint2 *from, *to;        // (word, token); null `from`: the ids themselves
+  uint32_t *counts, *next;  // [block][kBins] of this pass and the one after; null: there is none
+  int blocks, shift;
+  // sums
+  const uint2 *sorted;
+  float *partial;  // [piece][first run, last run][width]
+  int pieces;
+};
+
+template <typename W, typename T>
+__global__ __launch_bounds__(256) void embed(const EmbeddingArgs a) {
+  const uint64_t i = uint64_t(block_index()) * 256 + threadIdx.x;
+  if (i >= a.groups) return;
+  const uint64_t token = i / a.per_row;
+  const int64_t col = int64_t(i - token * a.per_row) * 8;
+  const int n = a.width - col < 8 ? int(a.width - col) : 8;
+  const int64_t id = a.ids[token];
+  float x[8] = {};
+  if (id >= 0 && id < a.vocab) {
+    const Raw8<W> r = load8<W>(row_at<W>(a.weight, id) + col, n);
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = a.scale * float(r.x[j]);
+  }
+  store8<T>(row_at<T>(a.out, token) + col, x, n);
+}
+
+// ---- sorting tokens by word ------------------------------------------------------
+
+// A stable radix sort, kBits of the word a pass. A block of kBlock tokens is a
+// workgroup's; its place in each bin is the sum of what all blocks have of
+// the bins before and the blocks before of this one, which every workgroup
+// adds up for itself from the counts in memory (they are 2 KB a block).
+constexpr int kBits = 9, kBins = 1 << kBits, kSortThreads = 512, kSortWaves = kSortThreads / 64, kEach = 4;
+constexpr int kBlock = kSortThreads * kEach;
+
+__device__ __forceinline__ uint32_t word_of(const EmbeddingArgs &a, int64_t token) {
+  const int64_t id = a.ids[token];
+  return id >= 0 && id < a.vocab ? uint32_t(id) : uint32_t(a.vocab);  // words that are none come last
+}
+
+// What the first pass's blocks have in each bin; the workgroups behind them
+// clear the gradient, which takes longer than the sorting, and the counts of
+// the passes to come.
+template <typename W>
+__global__ __launch_bounds__(kSortThreads) void count_words(const EmbeddingArgs a, uint32_t *clear, int64_t clear_words) {
+  __shared__ uint32_t bins[kBins];
+  const int t = threadIdx.x;
+  if (int(blockIdx.x) < a.blocks) {
+    for (int i = t; i < kBins; i += kSortThreads) bins[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+      const int64_t token = int64_t(blockIdx.x) * kBlock + i * kSortThreads + t;
+      if (token < a.tokens) atomicAdd(&bins[word_of(a, token) & (kBins - 1)], 1u);
+    }
+    __syncthreads();
+    for (int i = t; i < kBins; i += kSortThreads) a.counts[int64_t(blockIdx.x) * kBins + i] = bins[i];
+    return;
+  }
+  const int64_t first = int64_t(blockIdx.x - a.blocks) * kSortThreads + t, step = int64_t(gridDim.x - a.blocks) * kSortThreads;
+  for (int64_t i = first; i < clear_words; i += step) clear[i] = 0;
+  if (a.accumulate) return;
+  const float zeros[8] = {};
+  const uint64_t all = uint64_t(a.vocab) * a.per_row;
+  for (uint64_t i = first; i < all; i += step) {
+    const uint64_t row = i / a.per_row;
+    const int64_t col = int64_t(i - row * a.per_row) * 8;
+    store8<W>(row_at<W>(a.dweight, row) + col, zeros, a.width - col < 8 ? int(a.width - col) : 8);
+  }
+}
+
+__global__ __launch_bounds__(kSortThreads) void sort_words(const EmbeddingArgs a) {
+  __shared__ uint32_t bins[kSortWaves][kBins], base[kBins], sums[kSortWaves];
+  static_assert(kBins == kSortThreads, "a thread a bin");
+  const int t = threadIdx.x, l = t & 63, w = t >> 6;
+  const int64_t block = blockIdx.x;
+
+  // this thread's bin: what blocks before have of it, and what all have
+  uint32_t before = 0, all = 0;
+  for (int64_t b = 0; b < a.blocks; b++) {
+    const uint32_t n = a.counts[b * kBins + t];
+    if (b < block) before += n;
+    all += n;
+  }
+  uint32_t upto = all;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint32_t x = __shfl_up(upto, d, 64);
+    if (l >= d) upto += x;
+  }
+  if (l == 63) sums[w] = upto;
+#pragma unroll
+  for (int i = 0; i < kSortWaves; i++) bins[i][t] = 0;
+  __syncthreads();
+  for (int i = 0; i < w; i++) upto += sums[i];
+  base[t] = upto - all + before;
+
+  // ranks among a wave's equal digits, tokens in order
+  uint2 item[kEach];
+  uint32_t rank[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; i++) {
+    const int64_t at = block * kBlock + (w * kEach + i) * 64 + l;
+    const bool live = at < a.tokens;
+    item[i] = make_uint2(0, 0);
+    if (live) item[i] = a.from ? a.from[at] : make_uint2(word_of(a, at), uint32_t(at));
+    const uint32_t digit = (item[i].x >> a.shift) & (kBins - 1);
+    uint64_t same = __ballot(live);
+#pragma unroll
+    for (int b = 0; b < kBits; b++) {
+      const uint64_t set = __ballot(digit >> b & 1);
+      same &= digit >> b & 1 ? set : ~set;
+    }
+    const uint32_t ahead = uint32_t(__popcll(same & ((uint64_t(1) << l) - 1)));
+    uint32_t had = 0;
+    if (live) had = bins[w][digit];
+    rank[i] = had + ahead;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (live && ahead == 0) bins[w][digit] = had + uint32_t(__popcll(same));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  uint32_t waves = base[t];
+#pragma unroll
+  for (int i = 0; i < kSortWaves; i++) {
+    const uint32_t n = bins[i][t];
+    bins[i][t] = waves;
+    waves += n;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kEach; i++) {
+    const int64_t at = block * kBlock + (w * kEach + i) * 64 + l;
+    if (at >= a.tokens) continue;
+    const uint32_t to = bins[w][(item[i].x >> a.shift) & (kBins - 1)] + rank[i];
+    a.to[to] = item[i];
+    if (a.next) atomicAdd(&a.next[int64_t(to / kBlock) * kBins + ((item[i].x >> (a.shift + kBits)) & (kBins - 1))], 1u);
+  }
+}
+
+// ---- sums over runs of equal words -------------------------------------------------
+
+// Rows of kPiece sorted tokens, 8 columns a thread. A run that lies in the
+// piece is finished here; of one that goes on before or behind it the piece's
+// part is left for join_words: before first, behind last, and a piece that is
+// all one run's counts as first.
+constexpr int kPiece = 32;
+
+template <typename W>
+__device__ __forceinline__ void add_row(const EmbeddingArgs &a, uint32_t word, int64_t col, int n, const float (&sum)[8]) {
+  W *p = row_at<W>(a.dweight, word) + col;
+  float x[8];
+  if (a.accumulate) {
+    const Raw8<W> r = load8<W>(p, n);
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = float(r.x[j]) + a.scale * sum[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = a.scale * sum[j];
+  }
+  store8<W>(p, x, n);
+}
+
+template <typename W, typename T>
+__global__ __launch_bounds__(256) void sum_words(const EmbeddingArgs a) {
+  __shared__ uint2 items[kPiece + 2];  // the piece's, and its neighbours'
+  const int t = threadIdx.x;
+  const int64_t piece = block_index();
+  if (piece >= a.pieces) return;
+  const int64_t at0 = piece * kPiece;
+  for (int i = t; i < kPiece + 2; i += blockDim.x) {
+    const int64_t at = at0 + i - 1;
+    items[i] = at >= 0 && at < a.tokens ? a.sorted[at] : make_uint2(0xFFFFFFFFu, 0);
+  }
+  __syncthreads();
+  const int64_t col = (int64_t(blockIdx.z) * blockDim.x + t) * 8;
+  if (col >= a.width) return;
+  const int n = a.width - col < 8 ? int(a.width - col) : 8;
+  const int count = a.tokens - at0 < kPiece ? int(a.tokens - at0) : kPiece;
+  float sum[8] = {};
+  bool from_before = items[1].x == items[0].x;
+  for (int i0 = 0; i0 < count; i0 += 8) {
+    Raw8<T> r[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const uint2 item = items[1 + (i0 + i < count ? i0 + i : 0)];
+      r[i] = load8<T>(row_at<T>(a.dout, item.y) + col, i0 + i < count && item.x < a.vocab ? n : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if (i0 + i >= count) break;
+      const uint32_t word = items[1 + i0 + i].x, after = items[2 + i0 + i].x;
+#pragma unroll
+      for (int j = 0; j < 8; j++) sum[j] += float(r[i].x[j]);
+      const bool last = i0 + i + 1 == count;
+      if (word == after && !last) continue;
+      if (word < a.vocab) {
+        if (from_before || word == after) {
+          float *p = a.partial + (piece * 2 + (from_before ? 0 : 1)) * a.width + col;
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            if (j < n) p[j] = sum[j];
+        } else {
+          add_row<W>(a, word, col, n, sum);
+        }
+      }
+      from_before = false;
+#pragma unroll
+      for (int j = 0; j < 8; j++) sum[j] = 0.0f;
+    }
+  }
+}
+
+// Runs that begin in one piece and end in another, by the piece they begin in.
+template <typename W>
+__global__ __launch_bounds__(256) void join_words(const EmbeddingArgs a) {
+  const int64_t piece = block_index();
+  if (piece + 1 >= a.pieces) return;
+  const int64_t last = piece * kPiece + kPiece - 1;
+  const uint32_t word = a.sorted[last].x;
+  if (word >= a.vocab || a.sorted[last + 1].x != word) return;
+  // a run that began before this piece and fills it is another workgroup's
+  if (piece > 0 && a.sorted[last - kPiece].x == word) return;
+  const int64_t col = (int64_t(blockIdx.z) * blockDim.x + threadIdx.x) * 8;
+  if (col >= a.width) return;
+  const int n = a.width - col < 8 ? int(a.width - col) : 8;
+  // the piece that it ends in: the last whose first token is the run's
+  int64_t lo = piece + 1, hi = a.pieces - 1;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi + 1) / 2;
+    if (a.sorted[mid * kPiece].x == word) lo = mid;
+    else hi = mid - 1;
+  }
+  float sum[8];
+  const float *p = a.partial + (piece * 2 + 1) * a.width + col;
+#pragma unroll
+  for (int j = 0; j < 8; j++) sum[j] = j < n ? p[j] : 0.0f;
+#pragma unroll 4
+  for (int64_t i = piece + 1; i <= lo; i++) {
+    const Raw8<float> r = load8<float>(a.partial + i * 2 * a.width + col, n);
+#pragma unroll
+    for (int j = 0; j < 8; j++) sum[j] += r.x[j];
+  }
+  add_row<W>(a, word, col, n, sum);
+}
+
+// ---- host ----------------------------------------------------------------------------
+
+struct Layout {
+  int passes, blocks, pieces;
+  size_t counts, items, partial;  // bytes
+  size_t bytes() const { return counts + 2 * items + partial; }
+};
+
+Layout layout_of(const cchip_embedding &op) {
+  Layout p = {};
+  while (op.vocab >> (p.passes * kBits)) p.passes++;  // words 0 .. vocab
+  p.blocks = int((op.tokens + kBlock - 1) / kBlock);
+  p.pieces = int((op.tokens + kPiece - 1) / kPiece);
+  p.counts = size_t(p.passes) * p.blocks * kBins * sizeof(uint32_t);
+  p.items = (size_t(op.tokens) * sizeof(uint2) + 15) / 16 * 16;
+  p.partial = size_t(p.pieces) * 2 * op.width * sizeof(float);
+  return p;
+}
+
+void check_op(const cchip_embedding *op) {
+  const char *who = "embedding";
+  if (!op) throw InvalidArgument("embedding: no descriptor");
+  check_rows_type(who, op->dtype);
+  if (op->weight_dtype != op->dtype && op->weight_dtype != CCHIP_F32)
+    throw InvalidArgument("embedding: the table is of the operator's dtype or f32");
+  if (op->tokens < 0 || op->tokens > (int64_t(1) << 30)) throw InvalidArgument("embedding: tokens are not in 0 .. 2^30");
+  if (op->vocab < 1 || op->vocab > INT32_MAX) throw InvalidArgument("embedding: vocab is not in 1 .. 2^31 - 1");
+  if (op->width < 1 || op->width > (int64_t(1) << 20)) throw InvalidArgument("embedding: width is not in 1 .. 2^20");
+  if (!std::isfinite(op->scale)) throw InvalidArgument("embedding: scale is not finite");
+}
+
+const int32_t *ids_of(const cchip_embedding_io &io) {
+  if (!io.ids) throw InvalidArgument("embedding: no ids");
+  if (reinterpret_cast<uintptr_t>(io.ids) % 4) throw InvalidArgument("embedding: ids are not aligned to their elements");
+  return io.ids;
+}
+
+template <typename F>
+void with_types(const cchip_embedding &op, F &&f) {
+  with_rows_type(op.dtype, [&](auto t) {
+    if (op.weight_dtype == CCHIP_F32) f(float(), t);
+    else f(t, t);
+  });
+}
+
+}  // namespace
+}  // namespace op
+}  // namespace cchip
+
+using namespace cchip;
+using namespace cchip::op;
+
+extern "C" {
+
+int cchip_embedding_forward(const cchip_embedding *op, const cchip_embedding_io *io, void *stream) {
+  return guarded([&] {
+    const char *who = "embedding";
+    check_op(op);
+    if (!io) throw InvalidArgument("embedding: no tensors");
+    if (op->tokens == 0) return;
+    EmbeddingArgs a = {};
+    a.ids = ids_of(*io);
+    a.weight = rows_of(who, "weight", op->weight_dtype, op->vocab, op->width, io->weight, false, true);
+    a.out = rows_of(who, "out", op->dtype, op->tokens, op->width, io->out, true, true);
+    check_place(who, op->dtype, op->tokens, op->width, "out", a.out, "weight", a.weight, false);
+    a.tokens = op->tokens;
+    a.vocab = op->vocab;
+    a.width = op->width;
+    a.per_row = uint32_t((op->width + 7) / 8);
+    a.groups = uint64_t(op->tokens) * a.per_row;
+    if (a.groups > (uint64_t(1) << 39)) throw InvalidArgument("embedding: more than 2^42 elements");
+    a.scale = op->scale;
+    with_types(*op, [&](auto w, auto t) {
+      hipLaunchKernelGGL((embed<decltype(w), decltype(t)>), grid_of(int64_t((a.groups + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a);
+    });
+    check_launch(who);
+  });
+}
+
+int cchip_embedding_workspace(const cchip_embedding *op, size_t *bytes) {
+  return guarded([&] {
+    check_op(op);
+    if (bytes) *bytes = layout_of(*op).bytes();
+  });
+}
+
+int cchip_embedding_backward(const cchip_embedding *op, const cchip_embedding_io *io, void *workspace, size_t workspace_bytes,
+                             void *stream) {
+  return guarded([&] {
+    const char *who = "embedding";
+    check_op(op);
+    if (!io) throw InvalidArgument("embedding: no tensors");
+    EmbeddingArgs a = {};
+    a.dweight = rows_of(who, "dweight", op->weight_dtype, op->vocab, op->width, io->dweight, true, true);
+    if (op->tokens) {
+      a.ids = ids_of(*io);
+      a.dout = rows_of(who, "dout", op->dtype, op->tokens, op->width, io->dout, false, true);
+      check_place(who, op->dtype, op->tokens, op->width, "dweight", a.dweight, "dout", a.dout, false);
+    }
+    const Layout p = layout_of(*op);
+    if (workspace_bytes < p.bytes() || (p.bytes() && (!workspace || !aligned16(workspace))))
+      throw InvalidArgument(strf("embedding: the workspace needs %zu bytes aligned to 16, has %zu", p.bytes(), workspace ? workspace_bytes : 0));
+    a.tokens = op->tokens;
+    a.vocab = op->vocab;
+    a.width = op->width;
+    a.per_row = uint32_t((op->width + 7) / 8);
+    a.scale = op->scale;
+    a.accumulate = io->accumulate != 0;
+    a.blocks = p.blocks;
+    a.pieces = p.pieces;
+    char *at = static_cast<char *>(workspace);
+    uint32_t *counts = reinterpret_cast<uint32_t *>(at);
+    uint2 *items[2] = {reinterpret_cast<uint2 *>(at + p.counts), reinterpret_cast<uint2 *>(at + p.counts + p.items)};
+    a.partial = reinterpret_cast<float *>(at + p.counts + 2 * p.items);
+    const size_t pass_words = size_t(p.blocks) * kBins;
+    hipStream_t s = (hipStream_t)stream;
+    if (!op->tokens && a.accumulate) return;
+
+    a.counts = counts;
+    const int64_t clear = int64_t(p.passes - 1) * pass_words, fill = a.accumulate ? 0 : op->vocab * int64_t(a.per_row);
+    const int64_t clearing = std::min<int64_t>(2048, std::max((clear + kSortThreads - 1) / kSortThreads, (fill + kSortThreads - 1) / kSortThreads));
+    with_types(*op, [&](auto w, auto) {
+      hipLaunchKernelGGL((count_words<decltype(w)>), dim3(unsigned(p.blocks + clearing)), dim3(kSortThreads), 0, s, a, counts + pass_words, clear);
+    });
+    check_launch(who);
+    if (!op->tokens) return;
+    for (int i = 0; i < p.passes; i++) {
+      a.from = i ? items[(i - 1) & 1] : nullptr;
+      a.to = items[i & 1];
+      a.counts = counts + i * pass_words;
+      a.next = i + 1 < p.passes ? a.counts + pass_words : nullptr;
+      a.shift = i * kBits;
+      hipLaunchKernelGGL(sort_words, dim3(unsigned(p.blocks)), dim3(kSortThreads), 0, s, a);
+      check_launch(who);
+    }
+    a.sorted = a.to;
+    const int threads = int(std::min<int64_t>(256, (int64_t(a.per_row) + 63) / 64 * 64));
+    dim3 grid = grid_of(p.pieces);
+    grid.z = unsigned((a.per_row + threads - 1) / threads);
+    with_types(*op, [&](auto w, auto t) {
+      typedef decltype(w) W;
+      typedef decltype(t) T;
+      hipLaunchKernelGGL((sum_words<W, T>), grid, dim3(threads), 0, s, a);
+      check_launch(who);
+      if (p.pieces > 1) hipLaunchKernelGGL((join_words<W>), grid, dim3(threads), 0, s, a);
+    });
+    check_launch(who);
+  });
+}
+
+}  // extern "C"

@@ -206,7 +206,60 @@ def _check_dtype(who, *names):
             raise ValueError("%s: dtype %r is not f32, bf16 or f16" % (who, n))
 
 
-class GatedDelta(_Operator):
+class _HeadOperator(_Operator):
+    """Operators on ``[batch, tokens, heads, dim]`` arrays, whose shapes
+    ``_shapes`` has by name."""
+
+    def _words(self, **given):
+        """Pointer and three strides of each array. The loop does in one go what
+        _view does with words to say: a call on small arrays costs little more
+        than looking at them."""
+        words, device, dtype, shapes = [], self._device, self.dtype, self._shapes
+        for name, x in given.items():
+            shape = shapes[name]
+            try:
+                st = x.stride()
+                plain = x.shape == shape and _dtypes[x.dtype] == dtype and x.get_device() == device
+                p = x.data_ptr()
+            except (AttributeError, KeyError):
+                plain = False
+            if not plain:
+                p, st = self._view(name, x, dtype, shape)
+            if len(st) == 4:
+                if st[3] != 1 and shape[3] > 1:
+                    raise ValueError("%s: the last dimension of %s is not contiguous" % (self._who, name))
+                st = st[:3]
+            words.append(p)
+            words += st
+        return words
+
+    def _bounds(self, offsets):
+        if (offsets is None) != (self._offsets is None):
+            raise ValueError("%s: packed sequences need offsets" % self._who if offsets is None else
+                             "%s: offsets without packed sequences" % self._who)
+        return self._whole("offsets", offsets, "i32", self._offsets)
+
+    _saved_bytes = 0
+
+    def saved_bytes(self):
+        """Bytes of what a forward pass saves for its backward pass."""
+        return self._saved_bytes
+
+    def saved(self):
+        """A fresh array for what a forward pass saves."""
+        return Array.empty("u8", (self._saved_bytes,))
+
+    def _kept(self, saved):
+        return self._whole("saved", saved, "u8", (self._saved_bytes,))
+
+    def reserve(self, stream=None, backward=False):
+        """Allocate a stream's workspace for forward calls, and that for
+        backward calls, ahead of the first of them."""
+        for back in (False, True)[:1 + bool(backward)]:
+            self._workspace(self._on(stream), back)
+
+
+class GatedDelta(_HeadOperator):
     """The gated delta rule over ``[batch, tokens, heads, dim]`` arrays.
 
     ``u = beta (v - exp(g) S^T k)``, ``S = exp(g) S + k u^T``,
@@ -241,52 +294,6 @@ class GatedDelta(_Operator):
         self._state = (sequences or batch, value_heads, key_dim, value_dim)
         self._offsets = None if sequences is None else (sequences + 1,)
 
-    def saved_bytes(self):
-        """Bytes of what a forward pass saves for its backward pass."""
-        return self._saved_bytes
-
-    def saved(self):
-        """A fresh array for what a forward pass saves."""
-        return Array.empty("u8", (self._saved_bytes,))
-
-    def reserve(self, stream=None, backward=False):
-        """Allocate a stream's workspace for forward calls, and that for
-        backward calls, ahead of the first of them."""
-        for back in (False, True)[:1 + bool(backward)]:
-            self._workspace(self._on(stream), back)
-
-    def _words(self, **given):
-        """Pointer and three strides of each array. The loop does in one go what
-        _view does with words to say: a call on small arrays costs little more
-        than looking at them."""
-        words, device, dtype, shapes = [], self._device, self.dtype, self._shapes
-        for name, x in given.items():
-            shape = shapes[name]
-            try:
-                st = x.stride()
-                plain = x.shape == shape and _dtypes[x.dtype] == dtype and x.get_device() == device
-                p = x.data_ptr()
-            except (AttributeError, KeyError):
-                plain = False
-            if not plain:
-                p, st = self._view(name, x, dtype, shape)
-            if len(st) == 4:
-                if st[3] != 1 and shape[3] > 1:
-                    raise ValueError("GatedDelta: the last dimension of %s is not contiguous" % name)
-                st = st[:3]
-            words.append(p)
-            words += st
-        return words
-
-    def _bounds(self, offsets):
-        if (offsets is None) != (self._offsets is None):
-            raise ValueError("GatedDelta: packed sequences need offsets" if offsets is None else
-                             "GatedDelta: offsets without packed sequences")
-        return self._whole("offsets", offsets, "i32", self._offsets)
-
-    def _kept(self, saved):
-        return self._whole("saved", saved, "u8", (self._saved_bytes,))
-
     def forward(self, q, k, v, g, beta, o, *, state=None, state_out=None, offsets=None, saved=None, workspace=None,
                 stream=None):
         """Write ``o``, and the sequences' last states to ``state_out`` if given
@@ -316,6 +323,159 @@ class GatedDelta(_Operator):
         check(lib().cchip_gated_delta_backward(self._desc, io, *self._workspace(s, True, workspace), s))
 
 
+class Attention(_HeadOperator):
+    """Causal attention over ``[batch, tokens, heads, head_dim]`` queries and
+    ``[batch, tokens, kv_heads, head_dim]`` keys and values; heads ``h`` of
+    ``heads`` go with key head ``h // (heads // kv_heads)``. scale is
+    ``head_dim ** -0.5`` unless given.
+
+    ``sequences``: that many sequences packed into a batch of 1, which every
+    call says the bounds of (``offsets``, i32, ``sequences + 1`` values from 0
+    to ``tokens``). ``keys``: k and v are caches of that many tokens a row, of
+    which every call says how many they hold (``lengths``, i32, ``[batch]``),
+    the queries' own ``tokens``, the last, among them: single tokens and
+    chunks of a prompt. Without either, prompts and training."""
+
+    _who = "Attention"
+    # cchip_attention_io: eight cchip_heads of four words, three pointers
+    _forward_io = struct.Struct("16q128x3q")
+    _backward_io = struct.Struct("32q3q")
+
+    def __init__(self, dtype, batch, tokens, heads, kv_heads, head_dim, scale=None, sequences=None, keys=None):
+        super().__init__()
+        _check_dtype("Attention", dtype)
+        if sequences is not None and sequences < 1:
+            raise ValueError("Attention: sequences must be >= 1")
+        if keys is not None and keys < 1:
+            raise ValueError("Attention: keys must be >= 1")
+        self.dtype = dtype
+        self._desc = _lib.AttentionDesc(CODES[dtype], batch, tokens, sequences or 0, keys or 0, heads, kv_heads, head_dim,
+                                        head_dim ** -0.5 if scale is None and head_dim > 0 else scale or 0.0)
+        sizes = [ctypes.c_size_t() for _ in range(3)]
+        check(lib().cchip_attention_sizes(self._desc, *sizes))
+        self._forward_bytes, self._backward_bytes, self._saved_bytes = (x.value for x in sizes)
+        q, k = (batch, tokens, heads, head_dim), (batch, keys or tokens, kv_heads, head_dim)
+        self._shapes = dict(q=q, o=q, do=q, dq=q, k=k, v=k, dk=k, dv=k)
+        self._offsets = None if sequences is None else (sequences + 1,)
+        self._lengths = None if keys is None else (batch,)
+
+    def forward(self, q, k, v, o, *, offsets=None, lengths=None, saved=None, workspace=None, stream=None):
+        """Write ``o``, and ``saved`` for a backward pass if given."""
+        words = self._words(q=q, k=k, v=v, o=o)
+        if (lengths is None) != (self._lengths is None):
+            raise ValueError("Attention: a cache needs lengths" if lengths is None else "Attention: lengths without a cache")
+        s = self._on(stream)
+        io = self._forward_io.pack(*words, self._bounds(offsets), self._whole("lengths", lengths, "i32", self._lengths),
+                                   self._kept(saved))
+        w, n = self._workspace(s, False, workspace) if self._forward_bytes else (None, 0)
+        rc = lib().cchip_attention_forward(self._desc, io, w, n, s)
+        if rc:
+            check(rc)
+
+    def backward(self, q, k, v, o, do, saved, dq, dk, dv, *, offsets=None, workspace=None, stream=None):
+        """From ``o`` and its gradient ``do`` write those of q, k and v. ``saved``
+        is what ``forward`` wrote for the same inputs."""
+        if self._lengths is not None:
+            raise ValueError("Attention: there is no backward pass over a cache")
+        if saved is None:
+            raise ValueError("Attention: the backward pass needs what the forward pass saved")
+        words = self._words(q=q, k=k, v=v, o=o, do=do, dq=dq, dk=dk, dv=dv)
+        s = self._on(stream)
+        io = self._backward_io.pack(*words, self._bounds(offsets), 0, self._kept(saved))
+        check(lib().cchip_attention_backward(self._desc, io, *self._workspace(s, True, workspace), s))
+
+
+class HeadNorm(_HeadOperator):
+    """The norm of each head of q ``[batch, tokens, heads, head_dim]`` and k
+    ``[batch, tokens, kv_heads, head_dim]`` ("rms", with a weight of
+    ``head_dim`` for each of the two, or "none") and the rotation of its first
+    ``rotary`` elements (all unless given) by the token's position: pairs are
+    the halves of these or, ``interleaved``, neighbours.
+
+    Every call is given the ``frequencies``, radians a position of each of the
+    ``rotary // 2`` pairs (f32), and may be given ``positions`` (i32,
+    ``[batch, tokens]``; without them rows count from 0). ``keys``: forward
+    calls also write k and v to caches ``[batch, keys, kv_heads, head_dim]``
+    at the tokens' positions (those outside the cache nowhere)."""
+
+    _who = "HeadNorm"
+    _io = struct.Struct("44q6q")  # cchip_head_norm_io: eleven cchip_heads, six pointers
+    _NONE = (0, 0, 0, 0)
+
+    def __init__(self, dtype, batch, tokens, heads, kv_heads, head_dim, norm="rms", rotary=None, interleaved=False, eps=1e-6,
+                 weight_dtype="f32", keys=None):
+        super().__init__()
+        _check_dtype("HeadNorm", dtype, weight_dtype)
+        if norm not in ("rms", "none"):
+            raise ValueError("HeadNorm: unknown norm %r" % (norm,))
+        if keys is not None and keys < 1:
+            raise ValueError("HeadNorm: keys must be >= 1")
+        self.dtype = dtype
+        self.weight_dtype = weight_dtype
+        rotary = head_dim // 2 * 2 if rotary is None else rotary
+        self._desc = _lib.HeadNormDesc(CODES[dtype], CODES[weight_dtype], batch, tokens, keys or 0, heads, kv_heads, head_dim,
+                                       rotary, 1 if interleaved else 0, NORMS[norm], eps)
+        w = ctypes.c_size_t()
+        check(lib().cchip_head_norm_workspace(self._desc, ctypes.byref(w)))
+        self._backward_bytes = w.value
+        q, k = (batch, tokens, heads, head_dim), (batch, tokens, kv_heads, head_dim)
+        self._shapes = dict(q=q, q_out=q, dq_out=q, dq=q, k=k, v=k, k_out=k, dk_out=k, dk=k)
+        self._cache = keys is not None
+        if self._cache:
+            self._shapes["k_cache"] = self._shapes["v_cache"] = (batch, keys, kv_heads, head_dim)
+        self._positions = (batch, tokens)
+        self._frequencies = (rotary // 2,)
+        self._vector = (head_dim,)
+
+    def reserve(self, stream=None):
+        """Allocate a stream's workspace ahead of the first backward call on it."""
+        self._workspace(self._on(stream), True)
+
+    def _tables(self, frequencies, positions, q_weight, k_weight):
+        return (self._whole("positions", positions, "i32", self._positions),
+                self._whole("frequencies", frequencies, "f32", self._frequencies),
+                self._whole("q_weight", q_weight, self.weight_dtype, self._vector),
+                self._whole("k_weight", k_weight, self.weight_dtype, self._vector))
+
+    def forward(self, q, k, q_out, k_out=None, *, frequencies=None, positions=None, q_weight=None, k_weight=None, v=None,
+                k_cache=None, v_cache=None, stream=None):
+        """Write ``q_out`` and ``k_out``, which may be q and k; with caches those
+        are written from k and ``v``, and k_out need not be given."""
+        none = self._NONE
+        if self._cache:
+            words = self._words(q=q, k=k, v=v, q_out=q_out)
+            out = self._words(k_out=k_out) if k_out is not None else none
+            io = self._io.pack(*words, *out, *self._words(k_cache=k_cache, v_cache=v_cache), *none, *none, *none, *none,
+                               *self._tables(frequencies, positions, q_weight, k_weight), 0, 0)
+        else:
+            if not v is k_cache is v_cache is None:
+                raise ValueError("HeadNorm: a cache for an operator made without keys")
+            words = self._words(q=q, k=k)
+            io = self._io.pack(*words, *none, *self._words(q_out=q_out, k_out=k_out), *none, *none, *none, *none, *none, *none,
+                               *self._tables(frequencies, positions, q_weight, k_weight), 0, 0)
+        rc = lib().cchip_head_norm_forward(self._desc, io, self._on(stream))
+        if rc:
+            check(rc)
+
+    def backward(self, q, k, dq_out, dk_out, dq, dk, *, frequencies=None, positions=None, q_weight=None, k_weight=None,
+                 grads=None, workspace=None, stream=None):
+        """From q, k and the gradients of what ``forward`` wrote the gradients of
+        q and k (they may be ``dq_out`` and ``dk_out``) and, for each name in
+        ``grads`` ("q_weight", "k_weight"), of that weight, summed over tokens
+        and heads."""
+        none, s = self._NONE, self._on(stream)
+        grads = grads or {}
+        for n in grads:
+            if n not in ("q_weight", "k_weight"):
+                raise ValueError("HeadNorm: unknown parameter %s" % n)
+        words = self._words(q=q, k=k), self._words(dq_out=dq_out, dk_out=dk_out, dq=dq, dk=dk)
+        io = self._io.pack(*words[0], *none, *none, *none, *none, *none, *words[1],
+                           *self._tables(frequencies, positions, q_weight, k_weight),
+                           *(self._whole(n, grads.get(n), self.weight_dtype, self._vector) for n in ("q_weight", "k_weight")))
+        w, n = self._workspace(s, True, workspace) if grads else (None, 0)
+        check(lib().cchip_head_norm_backward(self._desc, io, w, n, s))
+
+
 class _RowOperator(_Operator):
     def _rows(self, name, x):
         """An array's pointer and the distance of its rows; zeros for None."""
@@ -341,6 +501,60 @@ class _RowOperator(_Operator):
     def _seed(self, seed, offset, step):
         return (seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF,
                 0 if step is None else self._whole("step", step, "i64", ()))
+
+
+class Embedding(_RowOperator):
+    """Rows of a table ``[vocab, width]`` by the tokens' ``ids`` (i32,
+    ``[tokens]``), times ``scale``, and the table's gradient. Ids outside 0 ..
+    vocab - 1 have rows of zeros and no gradient. The table and its gradient
+    are of ``weight_dtype`` ("f32" or ``dtype``, which it is unless given)."""
+
+    _who = "Embedding"
+    _io = struct.Struct("10q")  # cchip_embedding_io
+
+    def __init__(self, dtype, tokens, vocab, width, scale=1.0, weight_dtype=None):
+        super().__init__()
+        weight_dtype = weight_dtype or dtype
+        _check_dtype("Embedding", dtype, weight_dtype)
+        self.dtype = dtype
+        self.weight_dtype = weight_dtype
+        self._desc = _lib.EmbeddingDesc(CODES[dtype], CODES[weight_dtype], tokens, vocab, width, scale)
+        w = ctypes.c_size_t()
+        check(lib().cchip_embedding_workspace(self._desc, ctypes.byref(w)))
+        self._backward_bytes = w.value
+        self._ids = (tokens,)
+        self._shape = (tokens, width)
+        self._table = (vocab, width)
+
+    def reserve(self, stream=None):
+        """Allocate a stream's workspace ahead of the first backward call on it."""
+        self._workspace(self._on(stream), True)
+
+    def _words_of(self, ids):
+        if ids is None:
+            raise ValueError("Embedding: no ids")
+        return self._whole("ids", ids, "i32", self._ids)
+
+    def _table_of(self, name, x):
+        p, st = self._view(name, x, self.weight_dtype, self._table)
+        if st[1] != 1 and self._table[1] > 1:
+            raise ValueError("Embedding: rows of %s are not contiguous" % name)
+        return p, st[0]
+
+    def forward(self, ids, weight, out, *, stream=None):
+        """``out[t] = scale weight[ids[t]]``."""
+        io = self._io.pack(self._words_of(ids), *self._table_of("weight", weight), *self._needed("out", out), 0, 0, 0, 0, 0)
+        rc = lib().cchip_embedding_forward(self._desc, io, self._on(stream))
+        if rc:
+            check(rc)
+
+    def backward(self, ids, dout, dweight, *, accumulate=False, workspace=None, stream=None):
+        """Write the table's gradient, of all words, or with ``accumulate`` add
+        to the rows of those there are."""
+        s = self._on(stream)
+        io = self._io.pack(self._words_of(ids), 0, 0, 0, 0, *self._needed("dout", dout), *self._table_of("dweight", dweight),
+                           1 if accumulate else 0)
+        check(lib().cchip_embedding_backward(self._desc, io, *self._workspace(s, True, workspace), s))
 
 
 def _check_p(who, p):

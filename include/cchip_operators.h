@@ -99,6 +99,58 @@ int cchip_gated_delta_forward(const cchip_gated_delta *op, const cchip_gated_del
 int cchip_gated_delta_backward(const cchip_gated_delta *op, const cchip_gated_delta_io *io, void *workspace,
                                size_t workspace_bytes, void *stream);
 
+/* ---- Attention ----------------------------------------------------------- */
+
+/*
+ * Causal attention with grouped heads: query t of head h sees, of key head
+ * h / (heads / kv_heads), the keys up to its own token, counted from the end
+ * of both,
+ *
+ *   j <= t + (keys of the sequence) - (tokens of the sequence)
+ *   p_j = softmax_j(scale q_t . k_j),   o_t = sum_j p_j v_j
+ *
+ * heads is a multiple of kv_heads; sums, maxima and scores are f32. A query
+ * that sees no key, or whose every score is -infinity, has zeros for o. Three
+ * kinds of batches:
+ *
+ *   `sequences` and `keys` 0: the rows of the batch are the sequences, with a
+ *   key for each token.
+ *   `sequences` > 0: batch is 1 and sequence i is the tokens offsets[i] ..
+ *   offsets[i + 1] - 1, as for the gated delta rule; tokens of no sequence
+ *   are left as they were in all that is written.
+ *   `keys` > 0: k and v are caches of `keys` tokens a row of the batch, of
+ *   which row i holds lengths[i] (i32 on the device, clamped to 0 .. keys),
+ *   and q the last `tokens` of them; what a cache has behind its length is
+ *   not looked at. Forward only.
+ *
+ * A NaN or infinity in k or v reaches the queries that see it and no others.
+ * In the backward pass one in q, k, v or the gradient of o may reach the
+ * gradients of other tokens of its sequence that stand within 128 of it.
+ */
+typedef struct {
+  int dtype;
+  int64_t batch, tokens, sequences, keys;
+  int heads, kv_heads, head_dim; /* head_dim <= 128 */
+  float scale;
+} cchip_attention;
+
+/* Tensors as in cchip_gated_delta_io; k, v, dk and dv have kv_heads heads and,
+   with a cache, `keys` tokens. */
+typedef struct {
+  cchip_heads q, k, v;
+  cchip_heads o;            /* forward: written; backward: read */
+  cchip_heads d_o;          /* backward: read */
+  cchip_heads dq, dk, dv;   /* backward: written */
+  const int32_t *offsets, *lengths;
+  void *saved;              /* forward: written (NULL: no backward pass follows); backward: read */
+} cchip_attention_io;
+
+int cchip_attention_sizes(const cchip_attention *op, size_t *forward, size_t *backward, size_t *saved);
+int cchip_attention_forward(const cchip_attention *op, const cchip_attention_io *io, void *workspace, size_t workspace_bytes,
+                            void *stream);
+int cchip_attention_backward(const cchip_attention *op, const cchip_attention_io *io, void *workspace, size_t workspace_bytes,
+                             void *stream);
+
 /* ---- Dropout ------------------------------------------------------------- */
 
 /*
@@ -189,6 +241,81 @@ int cchip_norm_block_forward(const cchip_norm_block *op, const cchip_norm_block_
 int cchip_norm_block_workspace(const cchip_norm_block *op, size_t *bytes);
 int cchip_norm_block_backward(const cchip_norm_block *op, const cchip_norm_block_io *io, void *workspace,
                               size_t workspace_bytes, void *stream);
+
+/* ---- Norm and rotation of heads ------------------------------------------ */
+
+/*
+ * What stands between the projections of q and k and attention, on each head:
+ *
+ *   n = x / sqrt(mean(x^2) + eps) weight          (norm rms; none: n = x)
+ *   (y_i, y_j) = (n_i cos a - n_j sin a, n_j cos a + n_i sin a),  a = position frequency_p
+ *
+ * for the rotary / 2 pairs p of the first `rotary` elements (even), (i, j) =
+ * (p, p + rotary / 2) or, interleaved, (2 p, 2 p + 1); the others are n. The
+ * angle is made in 64 bits. Weights are vectors of head_dim, of dtype or f32,
+ * one of q and one of k (NULL: ones).
+ *
+ * With `keys` a call also writes to caches of `keys` tokens a row of the
+ * batch: a token's y of k to k_cache and its v to v_cache, at its position;
+ * one whose position is not in 0 .. keys - 1 is not written. Positions of a
+ * row differ there.
+ */
+typedef struct {
+  int dtype, weight_dtype;
+  int64_t batch, tokens, keys; /* batch * tokens < 2^31 */
+  int heads, kv_heads, head_dim, rotary; /* head_dim <= 512 */
+  int interleaved, norm;       /* CCHIP_NORM_NONE or CCHIP_NORM_RMS */
+  float eps;
+} cchip_head_norm;
+
+typedef struct {
+  cchip_heads q, k;            /* read by both */
+  cchip_heads v;               /* forward with keys: read */
+  cchip_heads q_out, k_out;    /* forward: written, may be q and k; with keys k_out may be NULL */
+  cchip_heads k_cache, v_cache; /* forward with keys: written at the tokens' positions */
+  cchip_heads dq_out, dk_out;  /* backward: read */
+  cchip_heads dq, dk;          /* backward: written, may be dq_out and dk_out */
+  const int32_t *positions;    /* [batch][tokens]; NULL: 0, 1, 2, ... in each row */
+  const float *frequencies;    /* radians a position, rotary / 2 */
+  const void *q_weight, *k_weight;
+  void *dq_weight, *dk_weight; /* backward: written; NULL: not wanted */
+} cchip_head_norm_io;
+
+int cchip_head_norm_forward(const cchip_head_norm *op, const cchip_head_norm_io *io, void *stream);
+/* Gradients of the weights are summed over tokens and heads in f32, in an
+   order that does not change from run to run. */
+int cchip_head_norm_workspace(const cchip_head_norm *op, size_t *bytes);
+int cchip_head_norm_backward(const cchip_head_norm *op, const cchip_head_norm_io *io, void *workspace, size_t workspace_bytes,
+                             void *stream);
+
+/* ---- Embedding ----------------------------------------------------------- */
+
+/*
+ *   out[t] = scale weight[ids[t]]
+ *   dweight[w] = scale sum over t with ids[t] = w of dout[t]
+ *
+ * ids are i32; one that is not in 0 .. vocab - 1, such as a padding token's,
+ * has a row of zeros and no gradient. The table is of dtype or f32. Sums are
+ * f32, in the order of the tokens. The backward pass writes all of dweight,
+ * or, with `accumulate`, adds to the rows of the words that there are.
+ */
+typedef struct {
+  int dtype, weight_dtype;
+  int64_t tokens, vocab, width; /* tokens <= 2^30, vocab < 2^31, width <= 2^20 */
+  float scale;
+} cchip_embedding;
+
+typedef struct {
+  const int32_t *ids;
+  cchip_rows weight, out;    /* forward: read, written */
+  cchip_rows dout, dweight;  /* backward: read, written */
+  int64_t accumulate;
+} cchip_embedding_io;
+
+int cchip_embedding_forward(const cchip_embedding *op, const cchip_embedding_io *io, void *stream);
+int cchip_embedding_workspace(const cchip_embedding *op, size_t *bytes);
+int cchip_embedding_backward(const cchip_embedding *op, const cchip_embedding_io *io, void *workspace, size_t workspace_bytes,
+                             void *stream);
 
 #ifdef __cplusplus
 }
