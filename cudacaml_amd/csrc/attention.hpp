@@ -135,24 +135,45 @@ __device__ __forceinline__ Raw8<T> negated(Raw8<T> r) {
 // ---- tiles in LDS ---------------------------------------------------------------
 
 // A tile of rows of D elements of 16 bits, a plane after another, a row's
-// pieces of 16 bytes exchanged by a number of the row's: 16 rows' pieces of
-// one column lie in banks of their own, as do four neighbouring rows' 64
-// bytes, which is what the two kinds of reads below take at a time.
+// pieces of 16 bytes exchanged by a number of the row's. Rows lie in groups of
+// 1 KB, which are 16 bytes apart: 16 rows' pieces of one column lie in banks of
+// their own, as do four neighbouring rows' 64 bytes, which is what the two
+// kinds of reads below take at a time, and groups of rows are a constant apart,
+// so that few registers address them all.
+constexpr int kGroup = 520;  // elements from group to group
+
 template <int D>
 __device__ __forceinline__ int twist(int row) {
-  return D == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+  return D == 128 ? (row & 3) << 2 : (((row >> 1) & 1) << 2) | (((row >> 2) & 1) << 1);
 }
 
 template <int D>
 __device__ __forceinline__ int piece_at(int row, int piece) {
-  return (row * (D / 8) + (piece ^ twist<D>(row))) * 8;
+  constexpr int kRows = 512 / D;
+  return row / kRows * kGroup + (row % kRows * (D / 8) + (piece ^ twist<D>(row))) * 8;
 }
+
+template <int D>
+constexpr int tile_elements(int rows) { return rows * D / 512 * kGroup; }
+
+// A lane's places in a tile of the operands that it reads.
+template <int D>
+struct Places {
+  int rows[4], columns[D / 32];
+  __device__ __forceinline__ Places() {
+    const int l = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < 4; i++) rows[i] = piece_at<D>(l & 31, (D == 128 ? 4 * i : 2 * i) + (l >> 5));
+    const int row = 4 * (l >> 5) + ((l >> 2) & 3), col = (l & 16) + (l & 3) * 4;
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) columns[i] = piece_at<D>(row, 4 * i + (col >> 3)) + (col & 4);
+  }
+};
 
 // Rows row0 + l % 32, terms 16 step + 8 (l / 32) .. + 7.
 template <int N, int D, typename E>
-__device__ __forceinline__ Bits<N> rows_of_tile(const E *m, int plane, int row0, int step) {
-  const int l = threadIdx.x & 63;
-  const E *p = m + piece_at<D>(row0 + (l & 31), 2 * step + (l >> 5));
+__device__ __forceinline__ Bits<N> rows_of_tile(const Places<D> &at, const E *m, int plane, int row0, int step) {
+  const E *p = m + (D == 128 ? at.rows[step / 2] + step % 2 * 16 : at.rows[step]) + row0 * D / 512 * kGroup;
   Bits<N> f;
 #pragma unroll
   for (int n = 0; n < N; n++) f.p[n] = *reinterpret_cast<const u32x4 *>(p + n * plane);
@@ -164,11 +185,9 @@ __device__ __forceinline__ Bits<N> rows_of_tile(const E *m, int plane, int row0,
 // gives lane i of 16 column i of the four rows whose 4 elements each the 16
 // lanes address.
 template <int N, int D, typename E>
-__device__ __forceinline__ Bits<N> columns_of_tile(const E *m, int plane, int row0, int col0) {
+__device__ __forceinline__ Bits<N> columns_of_tile(const Places<D> &at, const E *m, int plane, int row0, int col0) {
   typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
-  const int l = threadIdx.x & 63;
-  const int row = row0 + 4 * (l >> 5) + ((l >> 2) & 3), col = col0 + (l & 16) + (l & 3) * 4;
-  const E *a = m + piece_at<D>(row, col >> 3) + (col & 4), *b = m + piece_at<D>(row + 8, col >> 3) + (col & 4);
+  const E *a = m + at.columns[col0 / 32] + row0 * D / 512 * kGroup;
   Bits<N> f;
 #pragma unroll
   for (int n = 0; n < N; n++) {
@@ -177,10 +196,17 @@ __device__ __forceinline__ Bits<N> columns_of_tile(const E *m, int plane, int ro
       u32x4 v;
     } u;
     u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(a + n * plane));
-    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(b + n * plane));
+    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(a + n * plane + 8 * D / 512 * kGroup));
     f.p[n] = u.v;
   }
   return f;
+}
+
+// What is on its way from memory is there.
+__device__ __forceinline__ void copies_done() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0F70);
+  asm volatile("" ::: "memory");
 }
 
 // Rows of a tensor on their way to a tile: pieces of 8 elements, `Threads`
@@ -199,12 +225,21 @@ struct Staged {
     if (rows >= Rows && dim == D) {
 #pragma unroll
       for (int i = 0; i < kEach; i++) r[i] = load8<T>(p + row(t, i) * stride + piece(t, i) * 8, 8);
+    } else if (dim % 8 == 0) {
+#pragma unroll
+      for (int i = 0; i < kEach; i++) {
+        r[i] = Raw8<T>{};
+        if (row(t, i) < rows && piece(t, i) * 8 < dim) r[i] = load8<T>(p + row(t, i) * stride + piece(t, i) * 8, 8);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < kEach; i++) {
         const int left = dim - piece(t, i) * 8;
         r[i] = load8<T>(p + row(t, i) * stride + piece(t, i) * 8, row(t, i) < rows && left > 0 ? (left < 8 ? left : 8) : 0);
       }
+      // the elements' registers are used otherwise where rows are whole: a
+      // wait here, or there it would be for what is on its way
+      copies_done();
     }
   }
 
@@ -215,12 +250,10 @@ struct Staged {
     for (int i = 0; i < kEach; i++) {
       const Bits<N> b = bits_of<T>(r[i]);
 #pragma unroll
-      for (int n = 0; n < N; n++) *reinterpret_cast<u32x4 *>(m + n * Rows * D + piece_at<D>(row(t, i), piece(t, i))) = b.p[n];
+      for (int n = 0; n < N; n++) *reinterpret_cast<u32x4 *>(m + n * tile_elements<D>(Rows) + piece_at<D>(row(t, i), piece(t, i))) = b.p[n];
     }
   }
 };
-
-// ---- lanes ------------------------------------------------------------------------
 
 // The wave of the workgroup, in a scalar register as all that follows from it.
 __device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)); }
@@ -228,6 +261,97 @@ __device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstl
 // In a branch that most waves do not take: keeps the compiler from taking it
 // always and selecting.
 __device__ __forceinline__ void stay_branch() { asm volatile(""); }
+
+// 16 bytes a lane from memory to LDS without registers, lane after lane from
+// `to`, which is the wave's; `offset` bytes, below 2^32, are the lane's. As the
+// compiler sees it every read of LDS after such a copy has to wait for all of
+// them, also those that go to other tiles; an instruction that it does not see
+// leaves the waiting to copies_left. It writes no vector register, so nothing
+// that is in use can be overwritten by it, and m0, which the compiler keeps
+// nothing in.
+__device__ __forceinline__ void copy_lanes(const void *from, uint32_t offset, void *to) {
+  const uint32_t at = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)to));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(offset), "s"(from) : "memory");
+}
+
+// All but the last Left copies and loads of the wave are there.
+template <int Left>
+__device__ __forceinline__ void copies_left() {
+  static_assert(Left < 64, "as many as the counter has");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"i"(Left) : "memory");
+}
+
+// The same rows, of 16-bit elements at 16-byte places, copied to a tile
+// directly. Pieces behind dim are not written: the tile has zeros there from
+// the start. Rows from `rows` on are the last one again: what they give has to
+// be masked.
+template <int D, int Rows, int Threads>
+struct Copied {
+  static constexpr int kPieces = D / 8, kEach = Rows * kPieces / Threads;
+  uint32_t offset[kEach];  // bytes from the tile's first row
+  bool live[kEach];
+
+  static __device__ __forceinline__ int row(int i) { return (i * Threads + int(threadIdx.x)) / kPieces; }
+
+  __device__ __forceinline__ void start(int64_t stride, int dim) {
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+      const int piece = (i * Threads + int(threadIdx.x)) % kPieces ^ twist<D>(row(i));
+      live[i] = piece * 8 < dim;
+      offset[i] = (uint32_t(row(i)) * uint32_t(stride) + piece * 8) * 2;
+    }
+  }
+  __device__ __forceinline__ void copy(const char *from, uint32_t stride, int rows, int dim, char *to) const {
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+      uint32_t at = offset[i];
+      if (rows < Rows) {
+        stay_branch();
+        if (row(i) >= rows) at -= uint32_t(row(i) - rows + 1) * stride * 2;
+      }
+      char *const there = to + (i * Threads / 64 + wave_index()) * (kGroup * 2);
+      if (dim == D) {
+        copy_lanes(from, at, there);
+      } else if (live[i]) {
+        copy_lanes(from, at, there);
+      }
+    }
+  }
+};
+
+// ---- lanes ------------------------------------------------------------------------
+
+// A kernel of so many threads whose registers are for exactly so many waves a
+// SIMD: the compiler knows nothing of the LDS that a launch asks for, and would
+// save registers, and keep loads next to their uses, for waves that never come.
+#define CCHIP_WAVES(threads, waves) __launch_bounds__(threads, waves) __attribute__((amdgpu_waves_per_eu(waves, waves)))
+
+// All waves are here, and what they wrote to LDS is there; loads from memory
+// stay on their way.
+__device__ __forceinline__ void phase_done() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// use(i, operand) for i below Count, each operand read(i) from LDS Depth of
+// them ahead. The compiler would read each just before its product and wait.
+template <int Count, int Depth, int N>
+struct Ahead {
+  static constexpr int kDepth = Depth < Count ? Depth : Count;
+  Bits<N> f[kDepth];
+  template <typename Read>
+  __device__ __forceinline__ void start(const Read &read) {
+#pragma unroll
+    for (int i = 0; i < kDepth; i++) f[i] = read(i);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  template <typename Read, typename Use>
+  __device__ __forceinline__ void run(const Read &read, const Use &use) {
+#pragma unroll
+    for (int i = 0; i < Count; i++) {
+      use(i, f[i % kDepth]);
+      if (i + kDepth < Count) f[i % kDepth] = read(i + kDepth);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+};
 
 // x of the lane 32 on or before.
 __device__ __forceinline__ float other_half(float x) {

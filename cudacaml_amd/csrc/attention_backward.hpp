@@ -111,14 +111,14 @@ __device__ __forceinline__ void lay_tile(const AttentionArgs &a, const Heads &x,
       u32x4 u;
 #pragma unroll
       for (int j = 0; j < 4; j++) u[j] = pack_f16(float(r[i].x[2 * j]) * up, float(r[i].x[2 * j + 1]) * up);
-      to[piece_at<D>((t + i * 256) / kPieces, piece) / 8] = u;
+      to[(t + i * 256) / kPieces * kPieces + (piece ^ twist<D>((t + i * 256) / kPieces))] = u;
     }
   } else {
 #pragma unroll
     for (int i = 0; i < kEach; i++) {
       const Bits<B::N> b = bits_of<T>(r[i]);
 #pragma unroll
-      for (int n = 0; n < B::N; n++) to[(n * B::kHigh * D + piece_at<D>((t + i * 256) / kPieces, piece)) / 8] = b.p[n];
+      for (int n = 0; n < B::N; n++) to[(n * B::kHigh + (t + i * 256) / kPieces) * kPieces + (piece ^ twist<D>((t + i * 256) / kPieces))] = b.p[n];
     }
   }
 }
@@ -153,22 +153,14 @@ __global__ __launch_bounds__(256) void lay_out(const AttentionArgs a) {
 
 // ---- products -------------------------------------------------------------------------
 
-// What a wave copies of a piece of memory to the same place of LDS, 1 KB an
-// instruction, without registers; Waves waves share it. It is there after
-// copies_done and a barrier.
-template <int Bytes, int Waves>
-__device__ __forceinline__ void copy_to_lds(const u32x4 *from, u32x4 *to) {
-  const int w = wave_index(), l = threadIdx.x & 63;
-  static_assert(Bytes % (Waves * 1024) == 0, "every wave copies as much");
+// A tile in memory to LDS, 1 KB an instruction and group of rows, which four
+// waves share.
+template <int Pieces>
+__device__ __forceinline__ void copy_tile(const u32x4 *from, char *to) {
+  static_assert(Pieces % 256 == 0, "every wave copies as much");
 #pragma unroll
-  for (int i = 0; i < Bytes / (Waves * 1024); i++) {
-    const int at = (i * Waves + w) * 64;
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(from + at + l),
-                                     (__attribute__((address_space(3))) void *)(to + at), 16, 0, 0);
-  }
+  for (int i = 0; i < Pieces / 256; i++) copy_lanes(from, (i * 256 + threadIdx.x) * 16, to + (i * 4 + wave_index()) * (kGroup * 2));
 }
-
-__device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // Rows at + l % 32 of a tile in memory as an operand.
 template <typename T, int D>
@@ -178,7 +170,7 @@ __device__ __forceinline__ void load_operand(Bits<Backward<T>::N> (&q)[D / 16], 
   for (int i = 0; i < D / 16; i++)
 #pragma unroll
     for (int n = 0; n < Backward<T>::N; n++)
-      q[i].p[n] = tile[(n * Backward<T>::kHigh * D + piece_at<D>(at + (l & 31), 2 * i + (l >> 5))) / 8];
+      q[i].p[n] = tile[(n * Backward<T>::kHigh + at + (l & 31)) * (D / 8) + ((2 * i + (l >> 5)) ^ twist<D>(l & 31))];
 }
 
 // A column's dS in f16 has a power of two, so that the largest so far is
@@ -218,12 +210,13 @@ __device__ __forceinline__ void operands_of(Bits<Planes<M>::N> (&p)[2], const f3
 
 // kUnit rows, 32 a wave, over the keys that they see.
 template <typename T, int D>
-__global__ __launch_bounds__(256, Planes<T>::kWaves) void attend_back_rows(const AttentionArgs a) {
+__global__ CCHIP_WAVES(256, Planes<T>::kWaves) void attend_back_rows(const AttentionArgs a) {
   typedef Backward<T> B;
   typedef typename B::M M;
   typedef typename Planes<M>::E E;
-  constexpr int N = B::N, kHigh = B::kHigh, kPlane = kHigh * D, kPieces = kTilePieces<T, D>, kTiles = kUnit / kHigh;
-  extern __shared__ u32x4 lds[];  // [2][keys, values][tile]
+  constexpr int N = B::N, kHigh = B::kHigh, kPlane = tile_elements<D>(kHigh), kBytes = N * kPlane * 2, kPieces = kTilePieces<T, D>, kTiles = kUnit / kHigh;
+  extern __shared__ u32x4 lds_[];  // [2][keys, values][tile]
+  char *const lds = reinterpret_cast<char *>(lds_);
 
   const int t = threadIdx.x, l = t & 63, half = l >> 5, w = wave_index();
   const uint32_t id = block_index();
@@ -242,8 +235,8 @@ __global__ __launch_bounds__(256, Planes<T>::kWaves) void attend_back_rows(const
   const int64_t row_tile = (s.row_base + s.tile) * kTiles + w * 32 / kHigh, key_tile = s.key_base * kTiles;
   const u32x4 *k = a.tiles[2] + key_tile * kPieces, *v = a.tiles[3] + key_tile * kPieces;
   const int32_t *ke = a.powers[2] + key_tile, *ve = a.powers[3] + key_tile;
-  copy_to_lds<kPieces * 16, 4>(k, lds);
-  copy_to_lds<kPieces * 16, 4>(v, lds + kPieces);
+  copy_tile<kPieces>(k, lds);
+  copy_tile<kPieces>(v, lds + kBytes);
 
   Bits<N> q[D / 16], g[D / 16];
   const int in_tile = w * 32 % kHigh;
@@ -254,16 +247,17 @@ __global__ __launch_bounds__(256, Planes<T>::kWaves) void attend_back_rows(const
   if constexpr (B::kScaled) qe = a.powers[0][row_tile], ge = a.powers[1][row_tile];
   const float scale = a.negate ? -a.scale : a.scale;
 
+  const Places<D> at;
   f32x16 out[D / 32] = {};
   int power = kFirstPower;
   copies_done();
   __syncthreads();
   for (int tile = 0; tile < end; tile++) {
-    const E *km = reinterpret_cast<const E *>(lds + (tile & 1) * 2 * kPieces), *vm = km + kPieces * 8;
+    const E *km = reinterpret_cast<const E *>(lds + (tile & 1) * 2 * kBytes), *vm = km + N * kPlane;
     if (tile + 1 < end) {
-      u32x4 *next = lds + ((tile + 1) & 1) * 2 * kPieces;
-      copy_to_lds<kPieces * 16, 4>(k + int64_t(tile + 1) * kPieces, next);
-      copy_to_lds<kPieces * 16, 4>(v + int64_t(tile + 1) * kPieces, next + kPieces);
+      char *next = lds + ((tile + 1) & 1) * 2 * kBytes;
+      copy_tile<kPieces>(k + int64_t(tile + 1) * kPieces, next);
+      copy_tile<kPieces>(v + int64_t(tile + 1) * kPieces, next + kBytes);
     }
     const int64_t key0 = int64_t(tile) * kHigh;
     if (key0 < wave_any) {
@@ -279,8 +273,8 @@ __global__ __launch_bounds__(256, Planes<T>::kWaves) void attend_back_rows(const
         f32x16 x = {}, y = {};
 #pragma unroll
         for (int j = 0; j < D / 16; j++) {
-          x = product<M, N>(x, rows_of_tile<N, D>(km, kPlane, 32 * part, j), q[j]);
-          y = product<M, N>(y, rows_of_tile<N, D>(vm, kPlane, 32 * part, j), g[j]);
+          x = product<M, N>(x, rows_of_tile<N, D>(at, km, kPlane, 32 * part, j), q[j]);
+          y = product<M, N>(y, rows_of_tile<N, D>(at, vm, kPlane, 32 * part, j), g[j]);
         }
 #pragma unroll
         for (int i = 0; i < 16; i++)
@@ -303,7 +297,7 @@ __global__ __launch_bounds__(256, Planes<T>::kWaves) void attend_back_rows(const
         for (int d = 0; d < D / 32; d++)
 #pragma unroll
           for (int h = 0; h < 2; h++)
-            out[d] = product<M, N>(out[d], columns_of_tile<N, D>(km, kPlane, 32 * part + 16 * h, 32 * d), p[h]);
+            out[d] = product<M, N>(out[d], columns_of_tile<N, D>(at, km, kPlane, 32 * part + 16 * h, 32 * d), p[h]);
       }
     }
     copies_done();
@@ -318,12 +312,13 @@ __global__ __launch_bounds__(256, Planes<T>::kWaves) void attend_back_rows(const
 // kUnit keys, 32 a wave, over the rows that see them. Keys and values stay in
 // registers as second operands.
 template <typename T, int D>
-__global__ __launch_bounds__(256, 1) void attend_back_keys(const AttentionArgs a) {
+__global__ CCHIP_WAVES(256, 1) void attend_back_keys(const AttentionArgs a) {
   typedef Backward<T> B;
   typedef typename B::M M;
   typedef typename Planes<M>::E E;
-  constexpr int N = B::N, kHigh = B::kHigh, kPlane = kHigh * D, kPieces = kTilePieces<T, D>, kTiles = kUnit / kHigh;
-  extern __shared__ u32x4 lds[];  // [2][queries, gradients of o][tile]
+  constexpr int N = B::N, kHigh = B::kHigh, kPlane = tile_elements<D>(kHigh), kBytes = N * kPlane * 2, kPieces = kTilePieces<T, D>, kTiles = kUnit / kHigh;
+  extern __shared__ u32x4 lds_[];  // [2][queries, gradients of o][tile]
+  char *const lds = reinterpret_cast<char *>(lds_);
   __shared__ f32x4 lses[2][kHigh / 4], dots[2][kHigh / 4];
 
   const int t = threadIdx.x, l = t & 63, half = l >> 5, w = wave_index();
@@ -346,9 +341,9 @@ __global__ __launch_bounds__(256, 1) void attend_back_keys(const AttentionArgs a
 
   float row_value = 0.0f;  // a thread's lse or dot of a tile
   const auto fetch = [&](int tile) {
-    u32x4 *to = lds + (tile & 1) * 2 * kPieces;
-    copy_to_lds<kPieces * 16, 4>(q + int64_t(tile) * kPieces, to);
-    copy_to_lds<kPieces * 16, 4>(g + int64_t(tile) * kPieces, to + kPieces);
+    char *to = lds + (tile & 1) * 2 * kBytes;
+    copy_tile<kPieces>(q + int64_t(tile) * kPieces, to);
+    copy_tile<kPieces>(g + int64_t(tile) * kPieces, to + kBytes);
     if (t < 2 * kHigh) row_value = t < kHigh ? lse_of[int64_t(tile) * kHigh + t] : dot_of[int64_t(tile) * kHigh + t - kHigh];
   };
   const auto put = [&](int tile) {
@@ -364,6 +359,7 @@ __global__ __launch_bounds__(256, 1) void attend_back_keys(const AttentionArgs a
   if constexpr (B::kScaled) ke = a.powers[2][key_tile], ve = a.powers[3][key_tile];
   const float scale = a.negate ? -a.scale : a.scale;
 
+  const Places<D> at;
   f32x16 gk[D / 32] = {}, gv[D / 32] = {};
   int power = kFirstPower;
   int lift = 127;  // terms are 2^lift P over the power of two of the gradients' tile
@@ -374,7 +370,7 @@ __global__ __launch_bounds__(256, 1) void attend_back_keys(const AttentionArgs a
     if (tile + 1 < end) fetch(tile + 1);
     const int64_t tile_row = int64_t(tile) * kHigh;
     if (tile_row + kHigh > wave_first && wave_key < s.keys) {
-      const E *qm = reinterpret_cast<const E *>(lds + (tile & 1) * 2 * kPieces), *gm = qm + kPieces * 8;
+      const E *qm = reinterpret_cast<const E *>(lds + (tile & 1) * 2 * kBytes), *gm = qm + N * kPlane;
       float s_scale = scale, p_scale = 1.0f, more = 0.0f;
       int besides = 0;
       if constexpr (B::kScaled) {
@@ -396,8 +392,8 @@ __global__ __launch_bounds__(256, 1) void attend_back_keys(const AttentionArgs a
         f32x16 x = {}, y = {};
 #pragma unroll
         for (int j = 0; j < D / 16; j++) {
-          x = product<M, N>(x, rows_of_tile<N, D>(qm, kPlane, 32 * part, j), k[j]);
-          y = product<M, N>(y, rows_of_tile<N, D>(gm, kPlane, 32 * part, j), v[j]);
+          x = product<M, N>(x, rows_of_tile<N, D>(at, qm, kPlane, 32 * part, j), k[j]);
+          y = product<M, N>(y, rows_of_tile<N, D>(at, gm, kPlane, 32 * part, j), v[j]);
         }
         const bool masked = row0 < wave_full;
         const int from = int(clamped(mine - row0, 32)) - 4 * half;  // rows of the lane's from here on
@@ -429,8 +425,8 @@ __global__ __launch_bounds__(256, 1) void attend_back_keys(const AttentionArgs a
         for (int d = 0; d < D / 32; d++)
 #pragma unroll
           for (int h = 0; h < 2; h++) {
-            gv[d] = product<M, N>(gv[d], columns_of_tile<N, D>(gm, kPlane, 32 * part + 16 * h, 32 * d), p[h]);
-            gk[d] = product<M, N>(gk[d], columns_of_tile<N, D>(qm, kPlane, 32 * part + 16 * h, 32 * d), ds[h]);
+            gv[d] = product<M, N>(gv[d], columns_of_tile<N, D>(at, gm, kPlane, 32 * part + 16 * h, 32 * d), p[h]);
+            gk[d] = product<M, N>(gk[d], columns_of_tile<N, D>(at, qm, kPlane, 32 * part + 16 * h, 32 * d), ds[h]);
           }
       }
     }
@@ -438,9 +434,9 @@ __global__ __launch_bounds__(256, 1) void attend_back_keys(const AttentionArgs a
     copies_done();
     __syncthreads();
   }
-  const int64_t at = s.key0 + (live ? key : 0);
-  T *kp = reinterpret_cast<T *>(const_cast<char *>(element(a.gk, s.batch, at, s.kv, sizeof(T))));
-  T *vp = reinterpret_cast<T *>(const_cast<char *>(element(a.gv, s.batch, at, s.kv, sizeof(T))));
+  const int64_t place = s.key0 + (live ? key : 0);
+  T *kp = reinterpret_cast<T *>(const_cast<char *>(element(a.gk, s.batch, place, s.kv, sizeof(T))));
+  T *vp = reinterpret_cast<T *>(const_cast<char *>(element(a.gv, s.batch, place, s.kv, sizeof(T))));
   store_row<T, D>(kp, gk, B::kScaled ? a.plain_scale * power_of_two(-power) : a.plain_scale, a.dim, live);
   store_row<T, D>(vp, gv, B::kScaled ? power_of_two(-lift) : 1.0f, a.dim, live);
 }
@@ -471,7 +467,7 @@ inline BackSizes back_sizes(int dtype, int dim, int64_t pairs, int64_t row_slots
 
 template <typename T, int D>
 void launch_attend_back(AttentionArgs a, hipStream_t stream) {
-  constexpr size_t bytes = size_t(4) * kTilePieces<T, D> * 16;
+  constexpr size_t bytes = size_t(4) * Backward<T>::N * tile_elements<D>(Backward<T>::kHigh) * 2;
   constexpr uint32_t kTiles = kUnit / Backward<T>::kHigh;
   check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(&attend_back_rows<T, D>), hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)), "attention");
   check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(&attend_back_keys<T, D>), hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)), "attention");

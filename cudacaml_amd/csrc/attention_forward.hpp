@@ -186,6 +186,33 @@ __device__ __forceinline__ bool take_finite(Raw8<T> &r) {
   return all;
 }
 
+// The same of eight 16-bit elements as they are: exponents of ones only.
+template <typename T>
+__device__ __forceinline__ bool some_infinite(uint32_t u) {
+  const uint32_t e = std::is_same<T, f16>::value ? 0x7C007C00u : 0x7F807F80u, one = std::is_same<T, f16>::value ? 0x04000400u : 0x00800080u;
+  return ((u & e) + one) & 0x80008000u;
+}
+
+template <typename T>
+__device__ __forceinline__ u32x4 finite_only(u32x4 u) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if (some_infinite<T>(u[i] & 0xFFFFu)) u[i] &= 0xFFFF0000u;
+    if (some_infinite<T>(u[i] & 0xFFFF0000u)) u[i] &= 0xFFFFu;
+  }
+  return u;
+}
+
+template <typename T>
+__device__ __forceinline__ bool tile_finite(const u32x4 *tile, int pieces) {
+  bool some = false;
+  for (int i = threadIdx.x & 63; i < pieces; i += 64) {
+    const u32x4 u = tile[i];
+    some = some || some_infinite<T>(u[0]) || some_infinite<T>(u[1]) || some_infinite<T>(u[2]) || some_infinite<T>(u[3]);
+  }
+  return __ballot(some) == 0;
+}
+
 // Values of a tile that are not finite, and that the tile has zeros for,
 // where a row sees them: an infinity or NaN times the term's sign. A product
 // would bring them to the rows that do not, as zero times infinity.
@@ -206,19 +233,22 @@ __device__ __forceinline__ void add_infinite(Running<D> &r, const T *v, int64_t 
   }
 }
 
-// 32 Waves rows of a sequence and key head, a split of the keys they see.
-// Tiles of Keys keys and values go from memory through registers to one half
-// of LDS while the other is computed with; every wave reads all of both
-// (32 KB a tile of 64 for D = 128), which at 128 bytes a cycle of the unit
-// takes as long as the tile's products: waves are 8 where there are rows for
-// them, as they share what is loaded.
-template <typename T, int D, int Waves, int Keys>
-__global__ __launch_bounds__(Waves * 64, Planes<T>::kWaves) void attend(const AttentionArgs a) {
-  constexpr int N = Planes<T>::N, kTile = Keys * D, kBuffer = 2 * N * kTile;
+// 32 Waves rows of a sequence and key head, a split of the keys they see, in
+// tiles of Keys keys that go from memory through registers to LDS. A wave goes
+// through two phases a tile: products (what the terms of the tile before give
+// of its values, and this tile's scores) and terms. Of eight waves, two a SIMD,
+// four are a phase behind, so that the matrix units have one half's products
+// while the vector units make the other half's terms; with all in step each
+// would wait for the other.
+template <typename T, int D, int Waves, int Keys, bool Direct>
+__global__ CCHIP_WAVES(Waves * 64, Planes<T>::kWaves) void attend(const AttentionArgs a) {
+  constexpr int N = Planes<T>::N, kTile = tile_elements<D>(Keys), kBuffer = N * kTile;
+  constexpr bool kTwo = Waves == 8;
+  constexpr int kSlots = Direct ? 4 : 2;
   typedef typename Planes<T>::E E;
   extern __shared__ u32x4 lds[];
-  E *tiles = reinterpret_cast<E *>(lds);  // [2][keys, values][plane][Keys][D]
-  __shared__ int bad[2];                  // the tile, counted from 1, in a buffer some of whose values were not finite
+  E *const kt = reinterpret_cast<E *>(lds), *const vt = kt + kSlots * kBuffer;  // [kSlots][plane][Keys][D] of keys and of values
+  __shared__ int bad[2];  // the tile, counted from 1, in a buffer some of whose values were not finite
 
   const int t = threadIdx.x, l = t & 63, half = l >> 5, w = wave_index();
   const uint32_t block = block_index(), id = block / uint32_t(a.splits);
@@ -229,72 +259,193 @@ __global__ __launch_bounds__(Waves * 64, Planes<T>::kWaves) void attend(const At
   const int64_t row0 = int64_t(s.tile) * 32 * Waves, wave_row = row0 + w * 32, row = wave_row + (l & 31);
   if (row0 >= s.rows) return;
 
-  // keys that rows see: all of the workgroup's, all of the wave's, any of the
+  // keys that rows see: all of the workgroup's, all of the
   // wave's, the lane's
   const int64_t last_row = s.rows - 1 < row0 + 32 * Waves - 1 ? s.rows - 1 : row0 + 32 * Waves - 1;
-  const int64_t wave_last = s.rows - 1 < wave_row + 31 ? s.rows - 1 : wave_row + 31;
-  const int64_t to = clamped(last_row / a.group + s.ahead + 1, s.keys);
-  const int64_t all = clamped(row0 / a.group + s.ahead + 1, s.keys);
-  const int64_t wave_all = clamped(wave_row / a.group + s.ahead + 1, s.keys);
-  const int64_t wave_any = wave_row < s.rows ? clamped(wave_last / a.group + s.ahead + 1, s.keys) : 0;
-  const int64_t mine = clamped(row / a.group + s.ahead + 1, s.keys);
-  const int64_t count = (to + Keys - 1) / Keys;
-  const int64_t first = count * split / a.splits, end = count * (split + 1) / a.splits;
+  const int to = int(clamped(last_row / a.group + s.ahead + 1, s.keys));
+  const int all = int(clamped(row0 / a.group + s.ahead + 1, s.keys));
+  const int wave_all = int(clamped(wave_row / a.group + s.ahead + 1, s.keys));
+  const int mine = int(clamped(row / a.group + s.ahead + 1, s.keys));
+  const int count = (to + Keys - 1) / Keys;
+  const int first = int(int64_t(count) * split / a.splits), end = int(int64_t(count) * (split + 1) / a.splits);
 
   Bits<N> q[D / 16];
   load_queries<T, D>(q, a, a.q, s, row, a.negate);
   Running<D> r;
-  const T *k = reinterpret_cast<const T *>(element(a.k, s.batch, s.key0 + first * Keys, s.kv, sizeof(T)));
-  const T *v = reinterpret_cast<const T *>(element(a.v, s.batch, s.key0 + first * Keys, s.kv, sizeof(T)));
+  const T *const k = reinterpret_cast<const T *>(element(a.k, s.batch, s.key0, s.kv, sizeof(T)));
+  const T *const v = reinterpret_cast<const T *>(element(a.v, s.batch, s.key0, s.kv, sizeof(T)));
   if (t < 2) bad[t] = 0;
 
   Staged<T, D, Keys, Waves * 64> ks, vs;
-  const auto put = [&](int64_t tile) {
-    E *m = tiles + (tile & 1) * kBuffer;
-    ks.store(t, m);
-    if ((tile + 1) * Keys > all) {
-      bool finite = true;
-#pragma unroll
-      for (int i = 0; i < vs.kEach; i++) finite = take_finite(vs.r[i]) && finite;
-      if (!finite) bad[tile & 1] = int(tile) + 1;
-    }
-    vs.store(t, m + N * kTile);
+  const auto load = [&](int k_tile, int v_tile) {
+    if (k_tile < end) ks.load(t, k + int64_t(k_tile) * Keys * a.k.t, a.k.t, to - k_tile * Keys, a.dim);
+    if (v_tile < end) vs.load(t, v + int64_t(v_tile) * Keys * a.v.t, a.v.t, to - v_tile * Keys, a.dim);
   };
-  if (first < end) {
-    ks.load(t, k, a.k.t, to - first * Keys, a.dim);
-    vs.load(t, v, a.v.t, to - first * Keys, a.dim);
-    __syncthreads();
-    put(first);
-  }
-  __syncthreads();
-  for (int64_t tile = first; tile < end; tile++) {
-    const int64_t key0 = tile * Keys;
-    k += Keys * a.k.t;
-    v += Keys * a.v.t;
-    if (tile + 1 < end) {
-      ks.load(t, k, a.k.t, to - key0 - Keys, a.dim);
-      vs.load(t, v, a.v.t, to - key0 - Keys, a.dim);
-    }
-    if (key0 < wave_any) {
-      const E *km = tiles + (tile & 1) * kBuffer, *vm = km + N * kTile;
-      f32x16 x[Keys / 32];
+  const auto put = [&](int k_tile, int v_tile) {
+    if (k_tile < end) ks.store(t, kt + (k_tile & 1) * kBuffer);
+    if (v_tile < end) {
+      if ((v_tile + 1) * Keys > all) {
+        stay_branch();
+        bool finite = true;
 #pragma unroll
-      for (int i = 0; i < Keys / 32; i++) {
-        x[i] = f32x16{};
-#pragma unroll
-        for (int j = 0; j < D / 16; j++) x[i] = product<T, N>(x[i], rows_of_tile<N, D>(km, kTile, 32 * i, j), q[j]);
+        for (int i = 0; i < vs.kEach; i++) finite = take_finite(vs.r[i]) && finite;
+        if (!finite) bad[v_tile & 1] = v_tile + 1;
       }
-      Bits<N> p[Keys / 16];
-      terms_of<T, D, Keys / 32>(r, x, p, a.scale, key0 + Keys > wave_all, int(clamped(mine - key0, Keys)) - 4 * half);
-#pragma unroll
-      for (int d = 0; d < D / 32; d++)
-#pragma unroll
-        for (int i = 0; i < Keys / 16; i++) r.out[d] = product<T, N>(r.out[d], columns_of_tile<N, D>(vm, kTile, 16 * i, 32 * d), p[i]);
-      if (key0 + Keys > all && bad[tile & 1] == int(tile) + 1)
-        add_infinite<T, D>(r, v - Keys * a.v.t, a.v.t, to - key0 < Keys ? to - key0 : Keys, mine - key0, a.dim);
+      vs.store(t, vt + (v_tile & 1) * kBuffer);
     }
-    if (tile + 1 < end) put(tile + 1);
-    __syncthreads();
+  };
+  const Places<D> at;
+  f32x16 x[Keys / 32];
+  Bits<N> p[Keys / 16];
+  constexpr int kValues = D / 32 * (Keys / 16), kScores = Keys / 32 * (D / 16);
+  const auto read_values = [&](int tile, int i) {
+    return columns_of_tile<N, D>(at, vt + tile % kSlots * kBuffer, kTile, 16 * (i / (D / 32)), 32 * (i % (D / 32)));
+  };
+  const auto read_keys = [&](int tile, int i) {
+    return rows_of_tile<N, D>(at, kt + tile % kSlots * kBuffer, kTile, 32 * (i % (Keys / 32)), i / (Keys / 32));
+  };
+  const auto use_values = [&](int i, const Bits<N> &f) { r.out[i % (D / 32)] = product<T, N>(r.out[i % (D / 32)], f, p[i / (D / 32)]); };
+  const auto use_keys = [&](int i, const Bits<N> &f) { x[i % (Keys / 32)] = product<T, N>(x[i % (Keys / 32)], f, q[i / (Keys / 32)]); };
+  const auto scores = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < Keys / 32; i++) x[i] = f32x16{};
+    const auto read = [&](int i) { return read_keys(tile, i); };
+    Ahead<kScores, 6 / N, N> ahead;
+    ahead.start(read);
+    ahead.run(read, use_keys);
+  };
+  // products of the terms of tile - 1 and, between, the scores of tile
+  const auto both = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < Keys / 32; i++) x[i] = f32x16{};
+    const auto read = [&](int i) { return i < kValues ? read_values(tile - 1, i) : read_keys(tile, i - kValues); };
+    Ahead<kValues + kScores, 6 / N, N> ahead;
+    ahead.start(read);
+    ahead.run(read, [&](int i, const Bits<N> &f) { i < kValues ? use_values(i, f) : use_keys(i - kValues, f); });
+  };
+  const auto values = [&](int tile) {
+    const auto read = [&](int i) { return read_values(tile, i); };
+    Ahead<kValues, 6 / N, N> ahead;
+    ahead.start(read);
+    ahead.run(read, use_values);
+  };
+  const auto infinite = [&](int tile) {
+    stay_branch();
+    add_infinite<T, D>(r, v + int64_t(tile) * Keys * a.v.t, a.v.t, to - tile * Keys < Keys ? to - tile * Keys : Keys, mine - tile * Keys, a.dim);
+  };
+  // `some` rows may not see all of the tile
+  const auto terms = [&](int tile, bool some) {
+    terms_of<T, D, Keys / 32>(r, x, p, a.scale, some && (tile + 1) * Keys > wave_all, (mine - tile * Keys < Keys ? mine - tile * Keys : Keys) - 4 * half);
+  };
+
+  const bool behind = kTwo && w >= Waves / 2;
+  if constexpr (Direct) {
+    // Tiles are copied three ahead, in the first phase of a tile's two, and
+    // are there when the second ends: the slot that one goes to was done with
+    // then. Behind the last tile copies go on, so that those on their way can
+    // be counted.
+    Copied<D, Keys, Waves * 64> kc, vc;
+    kc.start(a.k.t, a.dim);
+    vc.start(a.v.t, a.dim);
+    const auto copy_keys = [&](int tile) {
+      const int at = tile < end ? tile : end - 1;
+      kc.copy(reinterpret_cast<const char *>(k + int64_t(at) * Keys * a.k.t), uint32_t(a.k.t), to - at * Keys, a.dim,
+              reinterpret_cast<char *>(kt + tile % kSlots * kBuffer));
+    };
+    const auto copy_values = [&](int tile) {
+      const int at = tile < end ? tile : end - 1;
+      vc.copy(reinterpret_cast<const char *>(v + int64_t(at) * Keys * a.v.t), uint32_t(a.v.t), to - at * Keys, a.dim,
+              reinterpret_cast<char *>(vt + tile % kSlots * kBuffer));
+    };
+    const auto copy = [&](int tile) { copy_keys(tile + 3), copy_values(tile + 2); };
+    constexpr int kLeft = 2 * (kc.kEach + vc.kEach);
+    // values that rows see and others do not have to be finite for a product
+    const auto values_of = [&](int tile) {
+      if ((tile + 1) * Keys <= all || tile_finite<T>(reinterpret_cast<const u32x4 *>(vt + tile % kSlots * kBuffer), kTile / 8)) return values(tile);
+      stay_branch();
+#pragma unroll
+      for (int i = 0; i < kValues; i++) {
+        Bits<N> f = read_values(tile, i);
+        f.p[0] = finite_only<T>(f.p[0]);
+        use_values(i, f);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      infinite(tile);
+    };
+    if (first < end) {
+      if (a.dim < D) {
+        for (int i = t; i < 2 * kSlots * kBuffer / 8; i += Waves * 64) lds[i] = u32x4{};
+        __syncthreads();
+      }
+      copy_keys(first), copy_keys(first + 1), copy_values(first);
+      copy_keys(first + 2), copy_values(first + 1);
+      copies_left<kLeft>();
+      __syncthreads();
+      if (kTwo && behind) copy(first), phase_done();
+      const auto step = [&](int tile, bool some) {
+        if (behind) copies_left<kLeft>();
+        if (kTwo) phase_done();
+        if (behind) copy(tile + 1);
+        terms(tile, some);
+        if (!behind) copies_left<kLeft>();
+        phase_done();
+      };
+      if (!behind) copy(first);
+      scores(first);
+      step(first, true);
+      const int full = all / Keys < end ? all / Keys : end;  // tiles that all rows see
+      int tile = first + 1;
+      for (; tile < full; tile++) {
+        if (!behind) copy(tile);
+        both(tile);
+        step(tile, false);
+      }
+      for (; tile < end; tile++) {
+        if (!behind) copy(tile);
+        values_of(tile - 1);
+        scores(tile);
+        step(tile, true);
+      }
+      values_of(end - 1);
+      if (kTwo && !behind) phase_done();
+      copies_done();
+    }
+  } else {
+    // waves that are behind have the tiles after theirs on their way one phase
+    // earlier, as all that a phase of the others needs is there at its start
+    const int lead = behind ? 1 : 0;
+    const auto step = [&](int tile) {
+      if (kTwo) phase_done();
+      terms(tile, true);
+      put(tile + 1 + lead, tile + lead);
+      phase_done();
+    };
+    const auto mend = [&](int tile) {
+      if ((tile + 1) * Keys > all && bad[tile & 1] == tile + 1) infinite(tile);
+    };
+    if (first < end) {
+      load(first, end);
+      copies_done();  // the queries too: a wait within the loop would be for the keys on their way as well
+      put(first, end);
+      if (behind) {
+        load(first + 1, first);
+        put(first + 1, first);
+      }
+      __syncthreads();
+      if (behind) phase_done();
+      load(first + 1 + lead, first + lead);
+      scores(first);
+      step(first);
+      for (int tile = first + 1; tile < end; tile++) {
+        load(tile + 1 + lead, tile + lead);
+        both(tile);
+        mend(tile - 1);
+        step(tile);
+      }
+      values(end - 1);
+      mend(end - 1);
+      if (kTwo && !behind) phase_done();
+    }
   }
   finish<T, D>(a, s, r, row, split, sum_halves(r.sum));
 }
@@ -304,8 +455,8 @@ __global__ __launch_bounds__(Waves * 64, Planes<T>::kWaves) void attend(const At
 // to four waves in turn, each with its own part of LDS and no barrier; what
 // they have is joined at the end.
 template <typename T, int D>
-__global__ __launch_bounds__(256, Planes<T>::kWaves) void attend_few(const AttentionArgs a) {
-  constexpr int N = Planes<T>::N, kTile = 32 * D, kWaves = 4;
+__global__ CCHIP_WAVES(256, Planes<T>::kWaves) void attend_few(const AttentionArgs a) {
+  constexpr int N = Planes<T>::N, kTile = tile_elements<D>(32), kWaves = 4;
   typedef typename Planes<T>::E E;
   extern __shared__ u32x4 lds[];
   const int t = threadIdx.x, l = t & 63, w = wave_index(), half = l >> 5;
@@ -327,6 +478,7 @@ __global__ __launch_bounds__(256, Planes<T>::kWaves) void attend_few(const Atten
   load_queries<T, D>(q, a, a.q, s, row, a.negate);
   Running<D> r;
   E *m = reinterpret_cast<E *>(lds) + w * N * kTile;
+  const Places<D> at;
   Staged<T, D, 32, 64> ks, vs;
   const T *k = reinterpret_cast<const T *>(element(a.k, s.batch, s.key0 + first * 32, s.kv, sizeof(T)));
   const T *v = reinterpret_cast<const T *>(element(a.v, s.batch, s.key0 + first * 32, s.kv, sizeof(T)));
@@ -344,7 +496,7 @@ __global__ __launch_bounds__(256, Planes<T>::kWaves) void attend_few(const Atten
     __builtin_amdgcn_wave_barrier();
     f32x16 x[1] = {};
 #pragma unroll
-    for (int j = 0; j < D / 16; j++) x[0] = product<T, N>(x[0], rows_of_tile<N, D>(m, kTile, 0, j), q[j]);
+    for (int j = 0; j < D / 16; j++) x[0] = product<T, N>(x[0], rows_of_tile<N, D>(at, m, kTile, 0, j), q[j]);
     Bits<N> p[2];
     terms_of<T, D, 1>(r, x, p, a.scale, masked, int(clamped(mine - key0, 32)) - 4 * half);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -364,7 +516,7 @@ __global__ __launch_bounds__(256, Planes<T>::kWaves) void attend_few(const Atten
 #pragma unroll
     for (int d = 0; d < D / 32; d++)
 #pragma unroll
-      for (int i = 0; i < 2; i++) r.out[d] = product<T, N>(r.out[d], columns_of_tile<N, D>(m, kTile, 16 * i, 32 * d), p[i]);
+      for (int i = 0; i < 2; i++) r.out[d] = product<T, N>(r.out[d], columns_of_tile<N, D>(at, m, kTile, 16 * i, 32 * d), p[i]);
     if (some_bad) add_infinite<T, D>(r, here, a.v.t, to - key0 < 32 ? to - key0 : 32, mine - key0, a.dim);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -402,25 +554,25 @@ __global__ __launch_bounds__(256, Planes<T>::kWaves) void attend_few(const Atten
   // eight elements a thread, D / 8 threads a row; every thread of a wave
   // goes on, as a row's sum comes from another lane
   for (int i = t; i < (rows * (D / 8) + 63) / 64 * 64; i += 256) {
-    const int at_row = i / (D / 8), at = i % (D / 8) * 8;
+    const int at_row = i / (D / 8), col = i % (D / 8) * 8;
     const float its = __shfl(total, at_row & 31, 64), its_top = __shfl(top, at_row & 31, 64);
-    if (at_row >= rows || at >= a.dim) continue;
+    if (at_row >= rows || col >= a.dim) continue;
     float y[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-      const int c = at_row * D + ((at + j) ^ ((at_row & 7) * 4));
+      const int c = at_row * D + ((col + j) ^ ((at_row & 7) * 4));
       y[j] = 0.0f;
 #pragma unroll
       for (int wave = 0; wave < kWaves; wave++) y[j] += outs[wave * 32 * D + c];
     }
-    const int n = a.dim - at < 8 ? a.dim - at : 8;
+    const int n = a.dim - col < 8 ? a.dim - col : 8;
     const int64_t all_at = row_values(a, s) + row0 + at_row;
     if (a.splits > 1) {
-      float *p = a.partial + (all_at * a.splits + split) * a.dim + at;
+      float *p = a.partial + (all_at * a.splits + split) * a.dim + col;
 #pragma unroll
       for (int j = 0; j < 8; j++)
         if (j < n) p[j] = y[j];
-      if (!at) {
+      if (!col) {
         float *ms = a.partial + all_rows * a.splits * a.dim + (all_at * a.splits + split) * 2;
         ms[0] = its_top;
         ms[1] = its;
@@ -429,15 +581,15 @@ __global__ __launch_bounds__(256, Planes<T>::kWaves) void attend_few(const Atten
     }
     const int64_t token = (row0 + at_row) / a.group;
     const int head = int(row0 + at_row - token * a.group);
-    T *p = reinterpret_cast<T *>(const_cast<char *>(element(a.o, s.batch, s.first + token, int64_t(s.kv) * a.group + head, sizeof(T)))) + at;
+    T *p = reinterpret_cast<T *>(const_cast<char *>(element(a.o, s.batch, s.first + token, int64_t(s.kv) * a.group + head, sizeof(T)))) + col;
     const float up = its == 0.0f ? 0.0f : 1.0f / its;
 #pragma unroll
     for (int j = 0; j < 8; j++)
       if (j < n) {
         p[j] = T(y[j] * up);
-        if (a.o_rest) a.o_rest[all_at * a.dim + at + j] = bf16(y[j] * up - float(p[j]));
+        if (a.o_rest) a.o_rest[all_at * a.dim + col + j] = bf16(y[j] * up - float(p[j]));
       }
-    if (a.lse && !at) a.lse[all_at] = its == 0.0f ? INFINITY : its_top - Powers<T>::kLift + __builtin_log2f(its);
+    if (a.lse && !col) a.lse[all_at] = its == 0.0f ? INFINITY : its_top - Powers<T>::kLift + __builtin_log2f(its);
   }
 }
 
@@ -474,17 +626,30 @@ __global__ __launch_bounds__(256) void join_splits(const AttentionArgs a) {
   if (a.lse && !l) a.lse[at] = sum == 0.0f ? INFINITY : top - Powers<T>::kLift + __builtin_log2f(sum);
 }
 
+// Whether rows are of whole pieces of 16 bytes, at places of them.
+inline bool whole_pieces(const AttentionArgs &a, const Heads &x) {
+  return a.dim % 8 == 0 && aligned16(x.p) && x.t % 8 == 0 && (x.h % 8 == 0 || a.kv_heads == 1) && (x.b % 8 == 0 || a.batch == 1);
+}
+
+template <typename T, int D, int Waves, int Keys, bool Direct>
+void launch_attend_as(const AttentionArgs &a, hipStream_t stream) {
+  constexpr size_t bytes = size_t(Direct ? 4 : 2) * 2 * Planes<T>::N * tile_elements<D>(Keys) * 2;
+  check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(&attend<T, D, Waves, Keys, Direct>), hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)),
+            "attention");
+  hipLaunchKernelGGL((attend<T, D, Waves, Keys, Direct>), grid_of(a.workgroups), dim3(Waves * 64), bytes, stream, a);
+}
+
 template <typename T, int D, int Waves, int Keys>
 void launch_attend(const AttentionArgs &a, hipStream_t stream) {
-  constexpr size_t bytes = size_t(2) * 2 * Planes<T>::N * Keys * D * 2;
-  check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(&attend<T, D, Waves, Keys>), hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)),
-            "attention");
-  hipLaunchKernelGGL((attend<T, D, Waves, Keys>), grid_of(a.workgroups), dim3(Waves * 64), bytes, stream, a);
+  if constexpr (!std::is_same<T, float>::value) {
+    if (whole_pieces(a, a.k) && whole_pieces(a, a.v)) return launch_attend_as<T, D, Waves, Keys, true>(a, stream);
+  }
+  launch_attend_as<T, D, Waves, Keys, false>(a, stream);
 }
 
 template <typename T, int D>
 void launch_attend_few(const AttentionArgs &a, hipStream_t stream) {
-  constexpr size_t tiles = size_t(4) * Planes<T>::N * 32 * D * 2, outs = size_t(4) * 32 * D * 4, bytes = tiles > outs ? tiles : outs;
+  constexpr size_t tiles = size_t(4) * Planes<T>::N * tile_elements<D>(32) * 2, outs = size_t(4) * 32 * D * 4, bytes = tiles > outs ? tiles : outs;
   check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(&attend_few<T, D>), hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)), "attention");
   hipLaunchKernelGGL((attend_few<T, D>), grid_of(a.workgroups), dim3(256), bytes, stream, a);
 }
