@@ -3,6 +3,7 @@
 
 #include "attention_backward.hpp"
 
+#include <algorithm>
 #include <cmath>
 #include <utility>
 
@@ -82,6 +83,7 @@ size_t saved_bytes(const cchip_attention &op) {
 
 struct BackCut {
   int64_t pairs, row_slots, key_slots;
+  int chunks, chunk_tiles;
   BackSizes sizes;
 };
 
@@ -92,7 +94,13 @@ BackCut back_cut_of(const cchip_attention &op) {
   c.key_slots = (op.tokens + kUnit - 1) / kUnit + op.sequences;
   if (c.row_slots > (int64_t(1) << 24) || c.pairs * c.row_slots > (int64_t(1) << 27))
     throw InvalidArgument("attention: more tokens and heads than a launch can have");
-  c.sizes = back_sizes(op.dtype, op.head_dim, c.pairs, c.row_slots, c.key_slots);
+  // chunks of rows that there are four workgroups to a unit, of 2048 rows at
+  // least: a chunk's sums cost what 30 of its rows do
+  const int64_t high = op.dtype == CCHIP_F32 ? 32 : 64, tiles = (op.tokens * (op.heads / op.kv_heads) + high - 1) / high;
+  const int64_t jobs = c.pairs * c.key_slots;
+  c.chunks = int(std::max<int64_t>(1, std::min<int64_t>({8, (1024 + jobs - 1) / std::max<int64_t>(1, jobs), tiles * high / 2048})));
+  c.chunk_tiles = int((tiles + c.chunks - 1) / c.chunks);
+  c.sizes = back_sizes(op.dtype, op.head_dim, c.pairs, c.row_slots, c.key_slots, c.chunks);
   return c;
 }
 
@@ -222,12 +230,12 @@ int cchip_attention_backward(const cchip_attention *op, const cchip_attention_io
       a.tiles[i] = reinterpret_cast<u32x4 *>(at);
       at += c.sizes.tiles[i];
     }
-    for (int i = 0; i < 4; i++) {
-      a.powers[i] = reinterpret_cast<int32_t *>(at);
-      at += c.sizes.powers[i];
-    }
-    a.lses = reinterpret_cast<float *>(at);
-    a.dots = reinterpret_cast<float *>(at + c.sizes.values);
+    a.row_heads = reinterpret_cast<float *>(at);
+    a.key_heads = reinterpret_cast<int32_t *>(at + c.sizes.row_heads);
+    a.partial = reinterpret_cast<float *>(at + c.sizes.row_heads + c.sizes.key_heads);
+    a.queues = reinterpret_cast<uint32_t *>(at + c.sizes.row_heads + c.sizes.key_heads + c.sizes.partial);
+    a.chunks = c.chunks;
+    a.chunk_tiles = c.chunk_tiles;
     a.pairs = uint32_t(c.pairs);
     a.row_slots = int(c.row_slots);
     a.key_slots = int(c.key_slots);

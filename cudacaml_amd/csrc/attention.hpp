@@ -30,13 +30,17 @@ struct AttentionArgs {
   float *lse;              // log2 of a row's sum: [batch][key head][token][head of the group], or null
   bf16 *o_rest;            // what rounding o to 16 bits left, as lse with `dim` a row, or null
   // backward (attention_backward.hpp): tiles of q, the gradient of o, k and v,
-  // their powers of two, and of the rows in tiles the lse and do . o
+  // and what belongs to a tile of rows and of keys
   u32x4 *tiles[4];
-  int32_t *powers[4];
-  float *lses, *dots;
+  float *row_heads;
+  int32_t *key_heads;
   int row_slots, key_slots;
+  int chunks;        // of the rows that see a key, kept apart until they are summed
+  int chunk_tiles;   // tiles of rows in a chunk
+  uint32_t *queues;  // kQueues of the rows' workgroups, then of the keys'
   uint32_t pairs;
-  float *partial;          // of splits: [slot of rows][split][rows][dim], then the maximum and sum of each
+  float *partial;          // of splits: [row][split][dim], then the maximum and sum of each; backward: of
+                           // chunks, [slot of keys][chunk][dk, dv][kUnit][dim]
   int64_t tokens, keys;    // of a row of the batch; keys: of the cache, or the tokens
   int64_t sequences;       // packed; 0: the batch's rows
   int64_t batch;
@@ -344,10 +348,16 @@ struct Ahead {
   }
   template <typename Read, typename Use>
   __device__ __forceinline__ void run(const Read &read, const Use &use) {
+    run(read, use, [](int) {});
+  }
+  // With work(i) after each product: vector instructions while it is made.
+  template <typename Read, typename Use, typename Work>
+  __device__ __forceinline__ void run(const Read &read, const Use &use, const Work &work) {
 #pragma unroll
     for (int i = 0; i < Count; i++) {
       use(i, f[i % kDepth]);
       if (i + kDepth < Count) f[i % kDepth] = read(i + kDepth);
+      work(i);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -389,6 +399,7 @@ struct Span {
   int64_t key0;        // row of k and v that the sequence's keys begin at
   int kv;
   int tile;            // of rows (or keys, backward), heavy ones first; < 0: nothing to do
+  int chunk;
   int64_t row_base, key_base;  // tiles of rows and of keys of the pairs and sequences before, as tall as this one
 };
 
@@ -405,11 +416,15 @@ __device__ __forceinline__ void pair_and_slot(uint32_t id, uint32_t pairs, uint3
 __device__ __forceinline__ int64_t clamped(int64_t x, int64_t most) { return x < 0 ? 0 : x > most ? most : x; }
 
 // Tiles of `height` rows, `per_token` to a token; `last_first`: tiles of a
-// sequence are counted from its end. `slots` are what the pair has tiles for.
-__device__ __forceinline__ Span span_of(const AttentionArgs &a, uint32_t id, uint32_t slots, int per_token, int height, bool last_first) {
+// sequence are counted from its end. `slots` are what the pair has tiles for;
+// with `chunks` of each there are those of the last chunk first.
+__device__ __forceinline__ Span span_of(const AttentionArgs &a, uint32_t id, uint32_t slots, int per_token, int height, bool last_first,
+                                        uint32_t chunks = 1) {
   Span s;
   uint32_t pair, slot;
-  pair_and_slot(id, uint32_t((a.sequences ? 1 : a.batch) * a.kv_heads), slots, pair, slot);
+  pair_and_slot(id, uint32_t((a.sequences ? 1 : a.batch) * a.kv_heads), slots * chunks, pair, slot);
+  s.chunk = int(chunks - 1 - slot / slots);
+  slot %= slots;
   int64_t tokens = a.tokens, tiles = slots;
   s.kv = int(pair % uint32_t(a.kv_heads));
   s.batch = pair / uint32_t(a.kv_heads);
@@ -468,6 +483,35 @@ __device__ __forceinline__ Span span_of(const AttentionArgs &a, uint32_t id, uin
   if (s.tile >= 0 && last_first) s.tile = int(tiles) - 1 - s.tile;
   return s;
 }
+
+// Workgroups that take one job after another: the hardware hands its own out in
+// order, each to the next of a die's four engines, so that one of them waits
+// for a unit of its engine while others idle, which costs half the time where
+// jobs differ in length. A die has a queue of every eighth job (see above) and
+// goes on with the next one's when that is empty. What a job does is the same
+// whoever has it.
+constexpr uint32_t kQueues = 8;
+
+struct Jobs {
+  uint32_t *queue;
+  uint32_t count, tried, die;
+  __device__ __forceinline__ Jobs(uint32_t *queues, uint32_t jobs) : queue(queues), count(jobs), tried(0), die(blockIdx.x % kQueues) {}
+  // the next, or all of them; `place` is in LDS
+  __device__ __forceinline__ uint32_t next(uint32_t &place) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      uint32_t job = count;
+      while (tried < kQueues && job >= count) {
+        const uint32_t q = (die + tried) % kQueues;
+        job = q + kQueues * atomicAdd(&queue[q], 1u);
+        if (job >= count) tried++;
+      }
+      place = job;
+    }
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(place);
+  }
+};
 
 __device__ __forceinline__ const char *element(const Heads &x, int64_t b, int64_t t, int64_t h, int size) {
   return x.p + (b * x.b + t * x.t + h * x.h) * size;
