@@ -57,15 +57,20 @@ struct Cut {
 Cut cut_of(const cchip_attention &op) {
   Cut p = {};
   const int64_t group = op.heads / op.kv_heads, rows = op.tokens * group, keys = op.keys ? op.keys : op.tokens;
-  const int64_t pairs = (op.sequences ? 1 : op.batch) * op.kv_heads;
+  const int64_t pairs = (op.sequences ? 1 : op.batch) * op.kv_heads, of_one = op.sequences ? rows / op.sequences : rows;
   const auto slots_of = [&](int height) { return (rows + height - 1) / height + op.sequences; };
-  p.waves = !op.sequences && rows <= 64 ? 0 : op.dtype != CCHIP_F32 && pairs * slots_of(256) >= 256 ? 8 : 4;
+  // Eight waves where there are rows for more than four: they share what is
+  // read, and four would leave half of a unit's registers idle, as there is
+  // LDS for one workgroup.
+  p.waves = !op.sequences && rows <= 64 ? 0 : op.dtype != CCHIP_F32 && of_one > 128 ? 8 : 4;
   const int64_t slots = slots_of(p.waves ? 32 * p.waves : 32);
   if (slots > (int64_t(1) << 27) || pairs * slots > (int64_t(1) << 30))
     throw InvalidArgument("attention: more tokens and heads than a launch can have");
   p.slots = int(slots);
   p.splits = 1;
-  const int64_t base = std::max<int64_t>(1, pairs * slots), least = p.waves ? 256 : 128, wanted = p.waves ? 512 : 1024;
+  // Keys are split where there are too few workgroups for the chip, but into
+  // parts that are long beside what joining them costs.
+  const int64_t base = std::max<int64_t>(1, pairs * slots), least = p.waves ? 512 : 128, wanted = p.waves ? 512 : 1024;
   if (!op.sequences && base < wanted) p.splits = int(std::max<int64_t>(1, std::min((wanted + base - 1) / base, keys / least)));
   p.workgroups = pairs * slots * p.splits;  // at most 2^30: splits are few where it is much
   if (p.splits > 1) p.bytes = size_t(op.batch) * op.tokens * op.heads * p.splits * (op.head_dim + 2) * sizeof(float);

@@ -136,6 +136,13 @@ __device__ __forceinline__ Raw8<T> negated(Raw8<T> r) {
   return r;
 }
 
+// Made here, among the products that it stands between, and not where it is
+// used.
+__device__ __forceinline__ float stay(float x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // ---- tiles in LDS ---------------------------------------------------------------
 
 // A tile of rows of D elements of 16 bits, a plane after another, a row's
@@ -274,8 +281,11 @@ __device__ __forceinline__ void stay_branch() { asm volatile(""); }
 // that is in use can be overwritten by it, and m0, which the compiler keeps
 // nothing in.
 __device__ __forceinline__ void copy_lanes(const void *from, uint32_t offset, void *to) {
-  const uint32_t at = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)to));
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(offset), "s"(from) : "memory");
+  // both are the wave's; the instruction takes them from scalar registers
+  const uint64_t source = reinterpret_cast<uint64_t>(from);
+  const uint64_t base = uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(source >> 32)))) << 32 | uint32_t(__builtin_amdgcn_readfirstlane(int(source)));
+  const uint32_t at = __builtin_amdgcn_readfirstlane(int(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)to)));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(offset), "s"(base) : "memory");
 }
 
 // All but the last Left copies and loads of the wave are there.
@@ -403,10 +413,10 @@ struct Span {
   int64_t row_base, key_base;  // tiles of rows and of keys of the pairs and sequences before, as tall as this one
 };
 
-// Tiles are numbered so that those of one sequence and key head, which read
-// the same keys, run on one of the eight dies (workgroups go to them in
-// turn): eight pairs at a time, each die all tiles of its own.
-__device__ __forceinline__ void pair_and_slot(uint32_t id, uint32_t pairs, uint32_t slots, uint32_t &pair, uint32_t &slot) {
+// Workgroups go to the eight dies in turn, each with a second-level cache of
+// its own: those of one sequence and key head, which read the same keys, run on
+// one die; eight pairs at a time, each die all tiles of its own.
+__device__ __forceinline__ void pair_a_die(uint32_t id, uint32_t pairs, uint32_t slots, uint32_t &pair, uint32_t &slot) {
   const uint32_t set = id / (8 * slots), in = id - set * 8 * slots;
   const uint32_t here = pairs - set * 8 < 8 ? pairs - set * 8 : 8;
   slot = in / here;
@@ -417,13 +427,13 @@ __device__ __forceinline__ int64_t clamped(int64_t x, int64_t most) { return x <
 
 // Tiles of `height` rows, `per_token` to a token; `last_first`: tiles of a
 // sequence are counted from its end. `slots` are what the pair has tiles for;
-// with `chunks` of each there are those of the last chunk first.
+// with `chunks` of each there are those of the first chunk first.
 __device__ __forceinline__ Span span_of(const AttentionArgs &a, uint32_t id, uint32_t slots, int per_token, int height, bool last_first,
                                         uint32_t chunks = 1) {
   Span s;
   uint32_t pair, slot;
-  pair_and_slot(id, uint32_t((a.sequences ? 1 : a.batch) * a.kv_heads), slots * chunks, pair, slot);
-  s.chunk = int(chunks - 1 - slot / slots);
+  pair_a_die(id, uint32_t((a.sequences ? 1 : a.batch) * a.kv_heads), slots * chunks, pair, slot);
+  s.chunk = int(slot / slots);
   slot %= slots;
   int64_t tokens = a.tokens, tiles = slots;
   s.kv = int(pair % uint32_t(a.kv_heads));
@@ -485,18 +495,21 @@ __device__ __forceinline__ Span span_of(const AttentionArgs &a, uint32_t id, uin
 }
 
 // Workgroups that take one job after another: the hardware hands its own out in
-// order, each to the next of a die's four engines, so that one of them waits
-// for a unit of its engine while others idle, which costs half the time where
-// jobs differ in length. A die has a queue of every eighth job (see above) and
-// goes on with the next one's when that is empty. What a job does is the same
-// whoever has it.
+// order, each to the next of a die's four engines, so that one waits for a unit
+// of its engine while others idle: up to half the time where jobs differ in
+// length, and two thirds where engines differ in units. A die has a queue of
+// every eighth job (see above) and goes on with the next one's when that is
+// empty. What a job does is the same whoever has it. There are some more
+// workgroups than units, as those of an engine that has no room find nothing
+// left.
+constexpr uint32_t kTakers = 320;
 constexpr uint32_t kQueues = 8;
 
 struct Jobs {
   uint32_t *queue;
   uint32_t count, tried, die;
   __device__ __forceinline__ Jobs(uint32_t *queues, uint32_t jobs) : queue(queues), count(jobs), tried(0), die(blockIdx.x % kQueues) {}
-  // the next, or all of them; `place` is in LDS
+  // the next, or `count`; `place` is in LDS
   __device__ __forceinline__ uint32_t next(uint32_t &place) {
     __syncthreads();
     if (threadIdx.x == 0) {

@@ -229,17 +229,13 @@ __device__ __forceinline__ void operands_of(Bits<Planes<M>::N> (&p)[2], const f3
 
 // kUnit rows, 32 a wave, over the keys that they see.
 template <typename T, int D>
-__global__ CCHIP_WAVES(256, Planes<T>::kWaves) void attend_back_rows(const AttentionArgs a) {
+__device__ __forceinline__ void back_rows_job(const AttentionArgs &a, uint32_t id, char *lds, int (&heads)[2][kKeyHead]) {
   typedef Backward<T> B;
   typedef typename B::M M;
   typedef typename Planes<M>::E E;
   constexpr int N = B::N, kHigh = B::kHigh, kPlane = tile_elements<D>(kHigh), kBytes = N * kPlane * 2, kPieces = kTilePieces<T, D>, kTiles = kUnit / kHigh;
-  extern __shared__ u32x4 lds_[];  // [2][keys, values][tile]
-  char *const lds = reinterpret_cast<char *>(lds_);
 
   const int t = threadIdx.x, l = t & 63, half = l >> 5, w = wave_index();
-  const uint32_t id = block_index();
-  if (id >= a.workgroups) return;
   const Span s = span_of(a, id, uint32_t(a.row_slots), a.group, kUnit, true);
   if (s.tile < 0) return;
   const int64_t row0 = int64_t(s.tile) * kUnit, wave_row = row0 + w * 32, row = wave_row + (l & 31);
@@ -254,7 +250,6 @@ __global__ CCHIP_WAVES(256, Planes<T>::kWaves) void attend_back_rows(const Atten
   const int64_t row_tile = (s.row_base + s.tile) * kTiles + w * 32 / kHigh, key_tile = s.key_base * kTiles;
   const u32x4 *k = a.tiles[2] + key_tile * kPieces, *v = a.tiles[3] + key_tile * kPieces;
   const int32_t *head_of = a.key_heads + key_tile * kKeyHead;
-  __shared__ int heads[2][kKeyHead];
   int head = 0;
   if (t < kKeyHead) heads[0][t] = head_of[t];
   copy_tile<kPieces>(k, lds);
@@ -336,6 +331,16 @@ __global__ CCHIP_WAVES(256, Planes<T>::kWaves) void attend_back_rows(const Atten
   const int64_t token = live ? row / a.group : 0, in = int64_t(s.kv) * a.group + (live ? int(row - token * a.group) : 0);
   T *p = reinterpret_cast<T *>(const_cast<char *>(element(a.gq, s.batch, s.first + token, in, sizeof(T))));
   store_row<T, D>(p, out, B::kScaled ? a.plain_scale * power_of_two(-power) : a.plain_scale, a.dim, live);
+}
+
+template <typename T, int D>
+__global__ CCHIP_WAVES(256, Planes<T>::kWaves) void attend_back_rows(const AttentionArgs a) {
+  extern __shared__ u32x4 lds[];  // [2][keys, values][tile]
+  __shared__ int heads[2][kKeyHead];
+  __shared__ uint32_t place;
+  Jobs jobs(a.queues, a.workgroups);
+  for (uint32_t job = jobs.next(place); job < a.workgroups; job = jobs.next(place))
+    back_rows_job<T, D>(a, job, reinterpret_cast<char *>(lds), heads);
 }
 
 constexpr int kBackSlots = 3;  // tiles of rows in LDS: in use, the one before, and on its way
@@ -477,7 +482,7 @@ __device__ __forceinline__ void back_keys_job(const AttentionArgs &a, uint32_t j
   float most = 0.0f;  // of dS
   const auto term = [&](int part, int i) {
     x[part][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[part][i], s_scale, more - lse[i / 4][i % 4]));
-    y[part][i] = x[part][i] * __builtin_fmaf(y[part][i], p_scale, -dot[i / 4][i % 4]);
+    y[part][i] = stay(x[part][i] * __builtin_fmaf(y[part][i], p_scale, -dot[i / 4][i % 4]));
     if constexpr (B::kScaled) most = fmaxf(most, __builtin_fabsf(y[part][i]));
   };
   // What is seldom, in one branch: rows that do not see all keys, the
@@ -674,16 +679,16 @@ template <typename T, int D>
 void launch_attend_back(AttentionArgs a, hipStream_t stream) {
   constexpr size_t bytes = size_t(4) * Backward<T>::N * tile_elements<D>(Backward<T>::kHigh) * 2, key_bytes = bytes / 4 * 6;
   constexpr uint32_t kTiles = kUnit / Backward<T>::kHigh;
-  check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(&attend_back_rows<T, D>), hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)), "attention");
-  check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(&attend_back_keys<T, D>), hipFuncAttributeMaxDynamicSharedMemorySize, int(key_bytes)), "attention");
+  allow_lds<&attend_back_rows<T, D>>(int(bytes));
+  allow_lds<&attend_back_keys<T, D>>(int(key_bytes));
   a.workgroups = 2 * a.pairs * uint32_t(a.row_slots + a.key_slots) * kTiles;
   hipLaunchKernelGGL((lay_out<T, D>), grid_of(a.workgroups), dim3(256), 0, stream, a);
   check_launch("attention");
   a.workgroups = a.pairs * uint32_t(a.row_slots);
-  hipLaunchKernelGGL((attend_back_rows<T, D>), grid_of(a.workgroups), dim3(256), bytes, stream, a);
+  hipLaunchKernelGGL((attend_back_rows<T, D>), dim3(std::min(a.workgroups, 2 * kTakers)), dim3(256), bytes, stream, a);
   check_launch("attention");
   a.workgroups = a.pairs * uint32_t(a.key_slots) * uint32_t(a.chunks);
-  hipLaunchKernelGGL((attend_back_keys<T, D>), dim3(std::min(a.workgroups, 256u)), dim3(256), key_bytes, stream, a);
+  hipLaunchKernelGGL((attend_back_keys<T, D>), dim3(std::min(a.workgroups, kTakers)), dim3(256), key_bytes, stream, a);
   check_launch("attention");
   if (a.chunks == 1) return;
   a.workgroups = a.pairs * uint32_t(a.key_slots) * 8;

@@ -1,6 +1,8 @@
 // Attention, forward: the kernel over tiles of rows, and the one for few rows
 // whose waves share the keys out.
 
+#include <atomic>
+
 #include "attention.hpp"
 
 namespace cchip {
@@ -247,8 +249,8 @@ __global__ CCHIP_WAVES(Waves * 64, Planes<T>::kWaves) void attend(const Attentio
   constexpr int kSlots = Direct ? 4 : 2;
   typedef typename Planes<T>::E E;
   extern __shared__ u32x4 lds[];
-  E *const kt = reinterpret_cast<E *>(lds), *const vt = kt + kSlots * kBuffer;  // [kSlots][plane][Keys][D] of keys and of values
   __shared__ int bad[2];  // the tile, counted from 1, in a buffer some of whose values were not finite
+  E *const kt = reinterpret_cast<E *>(lds), *const vt = kt + kSlots * kBuffer;  // [kSlots][plane][Keys][D] of keys and of values
 
   const int t = threadIdx.x, l = t & 63, half = l >> 5, w = wave_index();
   const uint32_t block = block_index(), id = block / uint32_t(a.splits);
@@ -626,6 +628,18 @@ __global__ __launch_bounds__(256) void join_splits(const AttentionArgs a) {
   if (a.lse && !l) a.lse[at] = sum == 0.0f ? INFINITY : top - Powers<T>::kLift + __builtin_log2f(sum);
 }
 
+// More than 64 KB of LDS have to be allowed, once for a kernel and device.
+template <auto Kernel>
+void allow_lds(int bytes) {
+  static std::atomic<uint64_t> allowed{0};
+  int device = 0;
+  check_hip(hipGetDevice(&device), "attention");
+  const uint64_t bit = uint64_t(1) << (device & 63);
+  if (device < 64 && (allowed.load(std::memory_order_relaxed) & bit)) return;
+  check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "attention");
+  allowed.fetch_or(bit, std::memory_order_relaxed);
+}
+
 // Whether rows are of whole pieces of 16 bytes, at places of them.
 inline bool whole_pieces(const AttentionArgs &a, const Heads &x) {
   return a.dim % 8 == 0 && aligned16(x.p) && x.t % 8 == 0 && (x.h % 8 == 0 || a.kv_heads == 1) && (x.b % 8 == 0 || a.batch == 1);
@@ -634,8 +648,7 @@ inline bool whole_pieces(const AttentionArgs &a, const Heads &x) {
 template <typename T, int D, int Waves, int Keys, bool Direct>
 void launch_attend_as(const AttentionArgs &a, hipStream_t stream) {
   constexpr size_t bytes = size_t(Direct ? 4 : 2) * 2 * Planes<T>::N * tile_elements<D>(Keys) * 2;
-  check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(&attend<T, D, Waves, Keys, Direct>), hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)),
-            "attention");
+  allow_lds<&attend<T, D, Waves, Keys, Direct>>(int(bytes));
   hipLaunchKernelGGL((attend<T, D, Waves, Keys, Direct>), grid_of(a.workgroups), dim3(Waves * 64), bytes, stream, a);
 }
 
@@ -650,7 +663,7 @@ void launch_attend(const AttentionArgs &a, hipStream_t stream) {
 template <typename T, int D>
 void launch_attend_few(const AttentionArgs &a, hipStream_t stream) {
   constexpr size_t tiles = size_t(4) * Planes<T>::N * tile_elements<D>(32) * 2, outs = size_t(4) * 32 * D * 4, bytes = tiles > outs ? tiles : outs;
-  check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(&attend_few<T, D>), hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)), "attention");
+  allow_lds<&attend_few<T, D>>(int(bytes));
   hipLaunchKernelGGL((attend_few<T, D>), grid_of(a.workgroups), dim3(256), bytes, stream, a);
 }
 
