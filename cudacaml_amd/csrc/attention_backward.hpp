@@ -679,8 +679,8 @@ template <typename T, int D>
 void launch_attend_back(AttentionArgs a, hipStream_t stream) {
   constexpr size_t bytes = size_t(4) * Backward<T>::N * tile_elements<D>(Backward<T>::kHigh) * 2, key_bytes = bytes / 4 * 6;
   constexpr uint32_t kTiles = kUnit / Backward<T>::kHigh;
-  allow_lds<&attend_back_rows<T, D>>(int(bytes));
-  allow_lds<&attend_back_keys<T, D>>(int(key_bytes));
+  allow_lds<&attend_back_rows<T, D>>(int(bytes), "attention");
+  allow_lds<&attend_back_keys<T, D>>(int(key_bytes), "attention");
   a.workgroups = 2 * a.pairs * uint32_t(a.row_slots + a.key_slots) * kTiles;
   hipLaunchKernelGGL((lay_out<T, D>), grid_of(a.workgroups), dim3(256), 0, stream, a);
   check_launch("attention");

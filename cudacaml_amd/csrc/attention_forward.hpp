@@ -1,8 +1,6 @@
 // Attention, forward: the kernel over tiles of rows, and the one for few rows
 // whose waves share the keys out.
 
-#include <atomic>
-
 #include "attention.hpp"
 
 namespace cchip {
@@ -628,18 +626,6 @@ __global__ __launch_bounds__(256) void join_splits(const AttentionArgs a) {
   if (a.lse && !l) a.lse[at] = sum == 0.0f ? INFINITY : top - Powers<T>::kLift + __builtin_log2f(sum);
 }
 
-// More than 64 KB of LDS have to be allowed, once for a kernel and device.
-template <auto Kernel>
-void allow_lds(int bytes) {
-  static std::atomic<uint64_t> allowed{0};
-  int device = 0;
-  check_hip(hipGetDevice(&device), "attention");
-  const uint64_t bit = uint64_t(1) << (device & 63);
-  if (device < 64 && (allowed.load(std::memory_order_relaxed) & bit)) return;
-  check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "attention");
-  allowed.fetch_or(bit, std::memory_order_relaxed);
-}
-
 // Whether rows are of whole pieces of 16 bytes, at places of them.
 inline bool whole_pieces(const AttentionArgs &a, const Heads &x) {
   return a.dim % 8 == 0 && aligned16(x.p) && x.t % 8 == 0 && (x.h % 8 == 0 || a.kv_heads == 1) && (x.b % 8 == 0 || a.batch == 1);
@@ -648,7 +634,7 @@ inline bool whole_pieces(const AttentionArgs &a, const Heads &x) {
 template <typename T, int D, int Waves, int Keys, bool Direct>
 void launch_attend_as(const AttentionArgs &a, hipStream_t stream) {
   constexpr size_t bytes = size_t(Direct ? 4 : 2) * 2 * Planes<T>::N * tile_elements<D>(Keys) * 2;
-  allow_lds<&attend<T, D, Waves, Keys, Direct>>(int(bytes));
+  allow_lds<&attend<T, D, Waves, Keys, Direct>>(int(bytes), "attention");
   hipLaunchKernelGGL((attend<T, D, Waves, Keys, Direct>), grid_of(a.workgroups), dim3(Waves * 64), bytes, stream, a);
 }
 
@@ -663,7 +649,7 @@ void launch_attend(const AttentionArgs &a, hipStream_t stream) {
 template <typename T, int D>
 void launch_attend_few(const AttentionArgs &a, hipStream_t stream) {
   constexpr size_t tiles = size_t(4) * Planes<T>::N * tile_elements<D>(32) * 2, outs = size_t(4) * 32 * D * 4, bytes = tiles > outs ? tiles : outs;
-  allow_lds<&attend_few<T, D>>(int(bytes));
+  allow_lds<&attend_few<T, D>>(int(bytes), "attention");
   hipLaunchKernelGGL((attend_few<T, D>), grid_of(a.workgroups), dim3(256), bytes, stream, a);
 }
 

@@ -31,21 +31,35 @@ struct EmbeddingArgs {
   int pieces;
 };
 
+// A thread has four groups of 8 columns, so that four tokens' ids, and then
+// their rows, are on their way at once.
+constexpr int kAtOnce = 4;
+
 template <typename W, typename T>
 __global__ __launch_bounds__(256) void embed(const EmbeddingArgs a) {
-  const uint64_t i = uint64_t(block_index()) * 256 + threadIdx.x;
-  if (i >= a.groups) return;
-  const uint64_t token = i / a.per_row;
-  const int64_t col = int64_t(i - token * a.per_row) * 8;
-  const int n = a.width - col < 8 ? int(a.width - col) : 8;
-  const int64_t id = a.ids[token];
-  float x[8] = {};
-  if (id >= 0 && id < a.vocab) {
-    const Raw8<W> r = load8<W>(row_at<W>(a.weight, id) + col, n);
+  const uint64_t first = uint64_t(block_index()) * (256 * kAtOnce) + threadIdx.x;
+  uint64_t token[kAtOnce];
+  int64_t col[kAtOnce], id[kAtOnce];
+  int n[kAtOnce];
 #pragma unroll
-    for (int j = 0; j < 8; j++) x[j] = a.scale * float(r.x[j]);
+  for (int k = 0; k < kAtOnce; k++) {
+    const uint64_t i = first + k * 256;
+    token[k] = a.groups <= 0xFFFFFFFFu ? uint32_t(i) / a.per_row : i / a.per_row;
+    col[k] = int64_t(i - token[k] * a.per_row) * 8;
+    n[k] = i >= a.groups ? 0 : a.width - col[k] < 8 ? int(a.width - col[k]) : 8;
+    id[k] = n[k] ? a.ids[token[k]] : -1;
   }
-  store8<T>(row_at<T>(a.out, token) + col, x, n);
+  Raw8<W> r[kAtOnce];
+#pragma unroll
+  for (int k = 0; k < kAtOnce; k++)
+    r[k] = load8<W>(row_at<W>(a.weight, id[k] < 0 ? 0 : id[k]) + col[k], id[k] >= 0 && id[k] < a.vocab ? n[k] : 0);
+#pragma unroll
+  for (int k = 0; k < kAtOnce; k++) {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = id[k] >= 0 && id[k] < a.vocab ? a.scale * float(r[k].x[j]) : 0.0f;
+    if (n[k]) store8<T>(row_at<T>(a.out, token[k]) + col[k], x, n[k]);
+  }
 }
 
 // ---- sorting tokens by word ------------------------------------------------------
@@ -62,9 +76,22 @@ __device__ __forceinline__ uint32_t word_of(const EmbeddingArgs &a, int64_t toke
   return id >= 0 && id < a.vocab ? uint32_t(id) : uint32_t(a.vocab);  // words that are none come last
 }
 
+// Zeros for the whole gradient from some workgroups of a launch: the
+// `turn`-th of `turns`.
+template <typename W>
+__device__ __forceinline__ void clear_gradient(const EmbeddingArgs &a, uint32_t turn, uint32_t turns) {
+  if (a.accumulate) return;
+  const float zeros[8] = {};
+  const uint64_t all = uint64_t(a.vocab) * a.per_row;
+  for (uint64_t i = uint64_t(turn) * blockDim.x + threadIdx.x; i < all; i += uint64_t(turns) * blockDim.x) {
+    const uint64_t row = all <= 0xFFFFFFFFu ? uint32_t(i) / a.per_row : i / a.per_row;
+    const int64_t col = int64_t(i - row * a.per_row) * 8;
+    store8<W>(row_at<W>(a.dweight, row) + col, zeros, a.width - col < 8 ? int(a.width - col) : 8);
+  }
+}
+
 // What the first pass's blocks have in each bin; the workgroups behind them
-// clear the gradient, which takes longer than the sorting, and the counts of
-// the passes to come.
+// clear the gradient and the counts of the passes to come.
 template <typename W>
 __global__ __launch_bounds__(kSortThreads) void count_words(const EmbeddingArgs a, uint32_t *clear, int64_t clear_words) {
   __shared__ uint32_t bins[kBins];
@@ -81,16 +108,31 @@ __global__ __launch_bounds__(kSortThreads) void count_words(const EmbeddingArgs 
     for (int i = t; i < kBins; i += kSortThreads) a.counts[int64_t(blockIdx.x) * kBins + i] = bins[i];
     return;
   }
-  const int64_t first = int64_t(blockIdx.x - a.blocks) * kSortThreads + t, step = int64_t(gridDim.x - a.blocks) * kSortThreads;
-  for (int64_t i = first; i < clear_words; i += step) clear[i] = 0;
-  if (a.accumulate) return;
-  const float zeros[8] = {};
-  const uint64_t all = uint64_t(a.vocab) * a.per_row;
-  for (uint64_t i = first; i < all; i += step) {
-    const uint64_t row = i / a.per_row;
-    const int64_t col = int64_t(i - row * a.per_row) * 8;
-    store8<W>(row_at<W>(a.dweight, row) + col, zeros, a.width - col < 8 ? int(a.width - col) : 8);
+  const uint32_t turn = blockIdx.x - a.blocks, turns = gridDim.x - a.blocks;
+  for (int64_t i = int64_t(turn) * kSortThreads + t; i < clear_words; i += int64_t(turns) * kSortThreads) clear[i] = 0;
+  clear_gradient<W>(a, turn, turns);
+}
+
+// A lane's rank among the wave's items of its digit, those counted before
+// included, which it adds these to.
+template <int Bits>
+__device__ __forceinline__ uint32_t rank_of(bool live, uint32_t digit, uint32_t *counts) {
+  const int l = threadIdx.x & 63;
+  uint64_t same = __ballot(live);
+#pragma unroll
+  for (int b = 0; b < Bits; b++) {
+    const uint64_t set = __ballot(digit >> b & 1);
+    same &= digit >> b & 1 ? set : ~set;
   }
+  const uint32_t ahead = uint32_t(__popcll(same & ((uint64_t(1) << l) - 1)));
+  uint32_t had = 0;
+  if (live) had = counts[digit];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  if (live && ahead == 0) counts[digit] = had + uint32_t(__popcll(same));
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  return had + ahead;
 }
 
 __global__ __launch_bounds__(kSortThreads) void sort_words(const EmbeddingArgs a) {
@@ -129,21 +171,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_words(const EmbeddingArgs a
     item[i] = make_uint2(0, 0);
     if (live) item[i] = a.from ? a.from[at] : make_uint2(word_of(a, at), uint32_t(at));
     const uint32_t digit = (item[i].x >> a.shift) & (kBins - 1);
-    uint64_t same = __ballot(live);
-#pragma unroll
-    for (int b = 0; b < kBits; b++) {
-      const uint64_t set = __ballot(digit >> b & 1);
-      same &= digit >> b & 1 ? set : ~set;
-    }
-    const uint32_t ahead = uint32_t(__popcll(same & ((uint64_t(1) << l) - 1)));
-    uint32_t had = 0;
-    if (live) had = bins[w][digit];
-    rank[i] = had + ahead;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (live && ahead == 0) bins[w][digit] = had + uint32_t(__popcll(same));
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    rank[i] = rank_of<kBits>(live, digit, bins[w]);
   }
   __syncthreads();
   uint32_t waves = base[t];
@@ -164,9 +192,78 @@ __global__ __launch_bounds__(kSortThreads) void sort_words(const EmbeddingArgs a
   }
 }
 
+// All tokens in one workgroup, where they fit into LDS, while the others of
+// the launch clear the gradient, which takes longer: 16384 tokens are sorted in
+// the 38 us that 268 MB of zeros take, in place of 27 us of their own.
+constexpr int kInOne = 16384, kOneThreads = 1024, kOneWaves = kOneThreads / 64, kOneEach = kInOne / kOneThreads;
+constexpr int kOneBits = 8, kOneBins = 1 << kOneBits;
+constexpr size_t kOneBytes = size_t(kInOne) * sizeof(uint2) + size_t(kOneWaves) * kOneBins * sizeof(uint32_t);
+
+template <typename W>
+__global__ __launch_bounds__(kOneThreads) void sort_in_one(const EmbeddingArgs a, int passes) {
+  extern __shared__ uint2 held[];  // the items, then the counts of each wave
+  __shared__ uint32_t sums[kOneWaves];
+  if (blockIdx.x) return clear_gradient<W>(a, blockIdx.x - 1, gridDim.x - 1);
+  uint32_t(*bins)[kOneBins] = reinterpret_cast<uint32_t(*)[kOneBins]>(held + kInOne);
+  const int t = threadIdx.x, l = t & 63, w = t >> 6, count = int(a.tokens);
+  // a wave has as many rounds of 64 tokens side by side
+  const int rounds = (count + kOneThreads - 1) / kOneThreads, first = w * rounds * 64 + l;
+  uint2 item[kOneEach];
+#pragma unroll
+  for (int i = 0; i < kOneEach; i++) {
+    const int at = first + i * 64;
+    item[i] = make_uint2(0, 0);
+    if (i < rounds && at < count) item[i] = make_uint2(word_of(a, at), uint32_t(at));
+  }
+  for (int pass = 0; pass < passes; pass++) {
+    for (int i = l; i < kOneBins; i += 64) bins[w][i] = 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    uint32_t rank[kOneEach];
+#pragma unroll
+    for (int i = 0; i < kOneEach; i++)
+      if (i < rounds) rank[i] = rank_of<kOneBits>(first + i * 64 < count, item[i].x >> (pass * kOneBits) & (kOneBins - 1), bins[w]);
+    __syncthreads();
+    uint32_t all = 0, upto = 0;
+    if (t < kOneBins) {
+      for (int i = 0; i < kOneWaves; i++) all += bins[i][t];
+      upto = all;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const uint32_t x = __shfl_up(upto, d, 64);
+        if (l >= d) upto += x;
+      }
+      if (l == 63) sums[w] = upto;
+    }
+    __syncthreads();
+    if (t < kOneBins) {
+      for (int i = 0; i < w; i++) upto += sums[i];
+      uint32_t from = upto - all;
+      for (int i = 0; i < kOneWaves; i++) {
+        const uint32_t n = bins[i][t];
+        bins[i][t] = from;
+        from += n;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kOneEach; i++)
+      if (i < rounds && first + i * 64 < count) held[bins[w][item[i].x >> (pass * kOneBits) & (kOneBins - 1)] + rank[i]] = item[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kOneEach; i++)
+      if (i < rounds && first + i * 64 < count) item[i] = held[first + i * 64];
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < kOneEach; i++)
+    if (i < rounds && first + i * 64 < count) a.to[first + i * 64] = item[i];
+}
+
 // ---- sums over runs of equal words -------------------------------------------------
 
-// Rows of kPiece sorted tokens, 8 columns a thread. A run that lies in the
+// Rows of kPiece sorted tokens, 8 columns a thread, half of them (of f32 a
+// quarter) on their way at once. A run that lies in the
 // piece is finished here; of one that goes on before or behind it the piece's
 // part is left for join_words: before first, behind last, and a piece that is
 // all one run's counts as first.
@@ -205,15 +302,21 @@ __global__ __launch_bounds__(256) void sum_words(const EmbeddingArgs a) {
   const int count = a.tokens - at0 < kPiece ? int(a.tokens - at0) : kPiece;
   float sum[8] = {};
   bool from_before = items[1].x == items[0].x;
-  for (int i0 = 0; i0 < count; i0 += 8) {
-    Raw8<T> r[8];
+  constexpr int kRows = sizeof(T) == 2 ? 16 : 8;
+  for (int i0 = 0; i0 < count; i0 += kRows) {
+    Raw8<T> r[kRows];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < kRows; i++) {
       const uint2 item = items[1 + (i0 + i < count ? i0 + i : 0)];
-      r[i] = load8<T>(row_at<T>(a.dout, item.y) + col, i0 + i < count && item.x < a.vocab ? n : 0);
+      const bool live = i0 + i < count && item.x < a.vocab;
+      if (n == 8) {  // one load and no branch
+        r[i] = load8<T>(row_at<T>(a.dout, live ? item.y : items[1].y) + col, 8);
+      } else {
+        r[i] = load8<T>(row_at<T>(a.dout, item.y) + col, live ? n : 0);
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < kRows; i++) {
       if (i0 + i >= count) break;
       const uint32_t word = items[1 + i0 + i].x, after = items[2 + i0 + i].x;
 #pragma unroll
@@ -261,11 +364,62 @@ __global__ __launch_bounds__(256) void join_words(const EmbeddingArgs a) {
   const float *p = a.partial + (piece * 2 + 1) * a.width + col;
 #pragma unroll
   for (int j = 0; j < 8; j++) sum[j] = j < n ? p[j] : 0.0f;
-#pragma unroll 4
-  for (int64_t i = piece + 1; i <= lo; i++) {
-    const Raw8<float> r = load8<float>(a.partial + i * 2 * a.width + col, n);
+  for (int64_t i0 = piece + 1; i0 <= lo; i0 += 8) {
+    Raw8<float> r[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++) sum[j] += r.x[j];
+    for (int i = 0; i < 8; i++) r[i] = load8<float>(a.partial + (i0 + i <= lo ? i0 + i : lo) * 2 * a.width + col, i0 + i <= lo ? n : 0);
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) sum[j] += r[i].x[j];
+  }
+  add_row<W>(a, word, col, n, sum);
+}
+
+// Few tokens: a workgroup a token, which is done where an earlier one has its
+// word and adds up the later ones' rows otherwise, in their order; which they
+// are every wave finds for itself. One launch, or two with the zeros, where
+// sorting takes three.
+constexpr int kFew = 512;
+
+template <typename W>
+__global__ __launch_bounds__(256) void clear_words(const EmbeddingArgs a) {
+  clear_gradient<W>(a, blockIdx.x, gridDim.x);
+}
+
+template <typename W, typename T>
+__global__ __launch_bounds__(256) void sum_few(const EmbeddingArgs a) {
+  const int l = threadIdx.x & 63, token = blockIdx.x, count = int(a.tokens);
+  const uint32_t word = word_of(a, token);
+  if (word >= a.vocab) return;
+  uint64_t equal[kFew / 64];
+#pragma unroll
+  for (int i = 0; i < kFew / 64; i++) equal[i] = __ballot(i * 64 + l < count && a.ids[i * 64 + l < count ? i * 64 + l : 0] == int32_t(word));
+  const int64_t col = (int64_t(blockIdx.z) * blockDim.x + threadIdx.x) * 8;
+  const int n = a.width - col < 8 ? int(a.width - col) : 8;
+  bool first = true;
+#pragma unroll
+  for (int i = 0; i < kFew / 64; i++) {
+    const uint64_t before = i * 64 > token ? 0 : token - i * 64 >= 64 ? ~uint64_t(0) : (uint64_t(1) << (token - i * 64)) - 1;
+    first = first && !(equal[i] & before);
+  }
+  if (!first || col >= a.width) return;
+  float sum[8] = {};
+#pragma unroll
+  for (int i = 0; i < kFew / 64; i++) {
+    uint64_t left = equal[i];
+    while (left) {
+      Raw8<T> r[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        r[j] = load8<T>(row_at<T>(a.dout, i * 64 + (left ? __builtin_ctzll(left) : 0)) + col, left ? n : 0);
+        left &= left - 1;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int k = 0; k < 8; k++) sum[k] += float(r[j].x[k]);
+    }
   }
   add_row<W>(a, word, col, n, sum);
 }
@@ -273,14 +427,16 @@ __global__ __launch_bounds__(256) void join_words(const EmbeddingArgs a) {
 // ---- host ----------------------------------------------------------------------------
 
 struct Layout {
-  int passes, blocks, pieces;
+  int passes, one_passes, blocks, pieces;
   size_t counts, items, partial;  // bytes
   size_t bytes() const { return counts + 2 * items + partial; }
 };
 
 Layout layout_of(const cchip_embedding &op) {
   Layout p = {};
+  if (op.tokens <= kFew) return p;
   while (op.vocab >> (p.passes * kBits)) p.passes++;  // words 0 .. vocab
+  while (op.vocab >> (p.one_passes * kOneBits)) p.one_passes++;
   p.blocks = int((op.tokens + kBlock - 1) / kBlock);
   p.pieces = int((op.tokens + kPiece - 1) / kPiece);
   p.counts = size_t(p.passes) * p.blocks * kBins * sizeof(uint32_t);
@@ -343,7 +499,7 @@ int cchip_embedding_forward(const cchip_embedding *op, const cchip_embedding_io 
     if (a.groups > (uint64_t(1) << 39)) throw InvalidArgument("embedding: more than 2^42 elements");
     a.scale = op->scale;
     with_types(*op, [&](auto w, auto t) {
-      hipLaunchKernelGGL((embed<decltype(w), decltype(t)>), grid_of(int64_t((a.groups + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a);
+      hipLaunchKernelGGL((embed<decltype(w), decltype(t)>), grid_of(int64_t((a.groups + 256 * kAtOnce - 1) / (256 * kAtOnce))), dim3(256), 0, (hipStream_t)stream, a);
     });
     check_launch(who);
   });
@@ -386,29 +542,50 @@ int cchip_embedding_backward(const cchip_embedding *op, const cchip_embedding_io
     a.partial = reinterpret_cast<float *>(at + p.counts + 2 * p.items);
     const size_t pass_words = size_t(p.blocks) * kBins;
     hipStream_t s = (hipStream_t)stream;
-    if (!op->tokens && a.accumulate) return;
-
-    a.counts = counts;
-    const int64_t clear = int64_t(p.passes - 1) * pass_words, fill = a.accumulate ? 0 : op->vocab * int64_t(a.per_row);
-    const int64_t clearing = std::min<int64_t>(2048, std::max((clear + kSortThreads - 1) / kSortThreads, (fill + kSortThreads - 1) / kSortThreads));
-    with_types(*op, [&](auto w, auto) {
-      hipLaunchKernelGGL((count_words<decltype(w)>), dim3(unsigned(p.blocks + clearing)), dim3(kSortThreads), 0, s, a, counts + pass_words, clear);
-    });
-    check_launch(who);
-    if (!op->tokens) return;
-    for (int i = 0; i < p.passes; i++) {
-      a.from = i ? items[(i - 1) & 1] : nullptr;
-      a.to = items[i & 1];
-      a.counts = counts + i * pass_words;
-      a.next = i + 1 < p.passes ? a.counts + pass_words : nullptr;
-      a.shift = i * kBits;
-      hipLaunchKernelGGL(sort_words, dim3(unsigned(p.blocks)), dim3(kSortThreads), 0, s, a);
+    const int64_t fill = a.accumulate ? 0 : op->vocab * int64_t(a.per_row);
+    const auto turns = [&](int64_t work, int threads) { return unsigned(std::min<int64_t>(2048, (work + threads - 1) / threads)); };
+    const int threads = int(std::min<int64_t>(256, (int64_t(a.per_row) + 63) / 64 * 64));
+    const unsigned columns = unsigned((a.per_row + threads - 1) / threads);
+    if (op->tokens <= kFew) {
+      with_types(*op, [&](auto w, auto t) {
+        typedef decltype(w) W;
+        typedef decltype(t) T;
+        if (fill) hipLaunchKernelGGL((clear_words<W>), dim3(turns(fill, 256)), dim3(256), 0, s, a);
+        check_launch(who);
+        if (op->tokens) hipLaunchKernelGGL((sum_few<W, T>), dim3(unsigned(op->tokens), 1, columns), dim3(threads), 0, s, a);
+      });
       check_launch(who);
+      return;
+    }
+    if (op->tokens <= kInOne) {
+      a.to = items[0];
+      with_types(*op, [&](auto w, auto) {
+        typedef decltype(w) W;
+        allow_lds<&sort_in_one<W>>(int(kOneBytes), who);
+        hipLaunchKernelGGL((sort_in_one<W>), dim3(1 + turns(fill, kOneThreads)), dim3(kOneThreads), kOneBytes, s, a, p.one_passes);
+      });
+      check_launch(who);
+    } else {
+      const int64_t clear = int64_t(p.passes - 1) * pass_words;
+      a.counts = counts;
+      with_types(*op, [&](auto w, auto) {
+        hipLaunchKernelGGL((count_words<decltype(w)>), dim3(unsigned(p.blocks) + std::max(1u, turns(std::max(clear, fill), kSortThreads))), dim3(kSortThreads), 0, s, a,
+                           counts + pass_words, clear);
+      });
+      check_launch(who);
+      for (int i = 0; i < p.passes; i++) {
+        a.from = i ? items[(i - 1) & 1] : nullptr;
+        a.to = items[i & 1];
+        a.counts = counts + i * pass_words;
+        a.next = i + 1 < p.passes ? a.counts + pass_words : nullptr;
+        a.shift = i * kBits;
+        hipLaunchKernelGGL(sort_words, dim3(unsigned(p.blocks)), dim3(kSortThreads), 0, s, a);
+        check_launch(who);
+      }
     }
     a.sorted = a.to;
-    const int threads = int(std::min<int64_t>(256, (int64_t(a.per_row) + 63) / 64 * 64));
     dim3 grid = grid_of(p.pieces);
-    grid.z = unsigned((a.per_row + threads - 1) / threads);
+    grid.z = columns;
     with_types(*op, [&](auto w, auto t) {
       typedef decltype(w) W;
       typedef decltype(t) T;

@@ -5,6 +5,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <type_traits>
 
@@ -310,6 +311,18 @@ inline dim3 grid_of(int64_t workgroups) {
 }
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// More than 64 KB of LDS have to be allowed, once for a kernel and device.
+template <auto Kernel>
+void allow_lds(int bytes, const char *what) {
+  static std::atomic<uint64_t> allowed{0};
+  int device = 0;
+  check_hip(hipGetDevice(&device), what);
+  const uint64_t bit = uint64_t(1) << (device & 63);
+  if (device < 64 && (allowed.load(std::memory_order_relaxed) & bit)) return;
+  check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes), what);
+  allowed.fetch_or(bit, std::memory_order_relaxed);
+}
 
 inline void check_launch(const char *what) { check_hip(hipGetLastError(), what); }
 
