@@ -117,12 +117,6 @@ AttentionArgs args_of(const cchip_attention &op, const cchip_attention_io &io, b
   a.k = heads_of(kWho, "k", op.dtype, b, n, hk, d, io.k, false);
   a.v = heads_of(kWho, "v", op.dtype, b, n, hk, d, io.v, false);
   a.o = heads_of(kWho, "o", op.dtype, b, t, h, d, io.o, !back);
-  struct Named {
-    const char *name;
-    const void *p;
-  };
-  const Named in[] = {{"q", io.q.data}, {"k", io.k.data}, {"v", io.v.data}, {"the gradient of o", io.d_o.data}, {"o", io.o.data}};
-  const Named out[] = {{"dq", io.dq.data}, {"dk", io.dk.data}, {"dv", io.dv.data}};
   if (back) {
     a.d_o = heads_of(kWho, "the gradient of o", op.dtype, b, t, h, d, io.d_o, false);
     a.gq = heads_of(kWho, "dq", op.dtype, b, t, h, d, io.dq, true);
@@ -131,25 +125,21 @@ AttentionArgs args_of(const cchip_attention &op, const cchip_attention_io &io, b
   }
   // other workgroups read what one of a call writes; of tensors that lie
   // between one another the first heads are looked at
-  if (b * t > 0) {
-    const size_t bytes = size_t(d) * (op.dtype == CCHIP_F32 ? 4 : 2);
-    for (const Named &i : in) {
-      if (!back) {
-        if (i.p != io.o.data && i.p && i.p != io.d_o.data && meet(io.o.data, bytes, i.p, bytes))
-          throw InvalidArgument(strf("attention: o is written over %s, which the call reads", i.name));
-        continue;
-      }
-      for (const Named &o : out)
-        if (meet(o.p, bytes, i.p, bytes)) throw InvalidArgument(strf("attention: %s is written over %s, which the call reads", o.name, i.name));
-    }
-    if (!back)
-      for (int i = 0; i < 3; i++)
-        if (in[i].p == io.o.data) throw InvalidArgument(strf("attention: o is written over %s, which the call reads", in[i].name));
-    if (back)
-      for (int i = 0; i < 3; i++)
-        for (int j = 0; j < i; j++)
-          if (meet(out[i].p, bytes, out[j].p, bytes))
-            throw InvalidArgument(strf("attention: %s and %s are written to one place", out[j].name, out[i].name));
+  struct Named {
+    const char *name;
+    const void *p;
+  };
+  const Named in[] = {{"q", io.q.data}, {"k", io.k.data}, {"v", io.v.data}, {"the gradient of o", io.d_o.data}, {"o", io.o.data}};
+  const Named out[] = {{"dq", io.dq.data}, {"dk", io.dk.data}, {"dv", io.dv.data}}, o[] = {{"o", io.o.data}};
+  const size_t bytes = b * t ? size_t(d) * (op.dtype == CCHIP_F32 ? 4 : 2) : 0;
+  for (int i = 0; i < (back ? 3 : 1); i++) {
+    const Named &to = back ? out[i] : o[i];
+    for (int j = 0; j < (back ? 5 : 3); j++)
+      if (meet(to.p, bytes, in[j].p, bytes))
+        throw InvalidArgument(strf("attention: %s is written over %s, which the call reads", to.name, in[j].name));
+    for (int j = 0; j < i; j++)
+      if (meet(to.p, bytes, out[j].p, bytes))
+        throw InvalidArgument(strf("attention: %s and %s are written to one place", out[j].name, to.name));
   }
   if (op.sequences ? !io.offsets : io.offsets != nullptr)
     throw InvalidArgument(op.sequences ? "attention: packed sequences need offsets" : "attention: offsets without packed sequences");

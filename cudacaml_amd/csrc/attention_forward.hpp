@@ -8,7 +8,8 @@ namespace op {
 
 // A row's maximum follows the largest score only when that is kSlack (a power
 // of two) ahead of it: what the row has so far is rescaled in the first tile
-// and hardly ever again. Terms are 2^(score - maximum + kLift): f16 has normal
+// and hardly ever again, and never for another row's sake, so that a row's
+// result does not depend on its neighbours. Terms are 2^(score - maximum + kLift): f16 has normal
 // values from 2^-14, so that what is dropped there is below 2^-24 of the
 // largest term, and nothing reaches 2^16.
 template <typename T>
@@ -68,7 +69,7 @@ __device__ __forceinline__ void terms_of(Running<D> &r, f32x16 (&s)[Tiles], Bits
     for (int i = t ? 0 : 1; i < 16; i++) most = fmaxf(most, s[t][i]);
   most = max_halves(most) * scale;
   if (__ballot(most > r.top + Powers<T>::kSlack)) {
-    const float top = most > r.top ? most : r.top;
+    const float top = most > r.top + Powers<T>::kSlack ? most : r.top;
     const float factor = top == r.top ? 1.0f : __builtin_amdgcn_exp2f(r.top - top);
     r.top = top;
     r.sum *= factor;
@@ -85,6 +86,34 @@ __device__ __forceinline__ void terms_of(Running<D> &r, f32x16 (&s)[Tiles], Bits
       for (int i = 0; i < 8; i++) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][half * 8 + i], scale, -from));
       p[2 * t + half] = operand_of<T>(x);
       r.sum = sum_of<T>(r.sum, x, p[2 * t + half]);
+    }
+}
+
+// Planes of f32 cannot hold an infinity: the scores of 32 Tiles keys that came
+// out as NaN are made again from q and k themselves.
+template <int Tiles>
+__device__ __forceinline__ void plain_scores(f32x16 (&s)[Tiles], const AttentionArgs &a, const Span &span, int64_t row, const float *k, int64_t keys) {
+  bool some = false;
+#pragma unroll
+  for (int t = 0; t < Tiles; t++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) some = some || s[t][i] != s[t][i];
+  if (!__ballot(some)) return;
+  stay_branch();
+  if (row >= span.rows) return;
+  const int half = (threadIdx.x & 63) >> 5;
+  const int64_t token = row / a.group;
+  const float *q = reinterpret_cast<const float *>(element(a.q, span.batch, span.first + token, int64_t(span.kv) * a.group + (row - token * a.group), sizeof(float)));
+#pragma unroll
+  for (int t = 0; t < Tiles; t++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const int key = t * 32 + 8 * (i / 4) + 4 * half + i % 4;
+      if (s[t][i] == s[t][i] || key >= keys) continue;
+      float sum = 0.0f;
+#pragma unroll 1
+      for (int d = 0; d < a.dim; d++) sum = __builtin_fmaf(a.negate ? -q[d] : q[d], k[key * a.k.t + d], sum);
+      s[t][i] = sum;
     }
 }
 
@@ -335,6 +364,7 @@ __global__ CCHIP_WAVES(Waves * 64, Planes<T>::kWaves) void attend(const Attentio
   };
   // `some` rows may not see all of the tile
   const auto terms = [&](int tile, bool some) {
+    if constexpr (std::is_same<T, float>::value) plain_scores(x, a, s, row, k + int64_t(tile) * Keys * a.k.t, to - tile * Keys);
     terms_of<T, D, Keys / 32>(r, x, p, a.scale, some && (tile + 1) * Keys > wave_all, (mine - tile * Keys < Keys ? mine - tile * Keys : Keys) - 4 * half);
   };
 
@@ -497,6 +527,7 @@ __global__ CCHIP_WAVES(256, Planes<T>::kWaves) void attend_few(const AttentionAr
     f32x16 x[1] = {};
 #pragma unroll
     for (int j = 0; j < D / 16; j++) x[0] = product<T, N>(x[0], rows_of_tile<N, D>(at, m, kTile, 0, j), q[j]);
+    if constexpr (std::is_same<T, float>::value) plain_scores(x, a, s, row, k - 32 * kWaves * a.k.t, to - key0);
     Bits<N> p[2];
     terms_of<T, D, 1>(r, x, p, a.scale, masked, int(clamped(mine - key0, 32)) - 4 * half);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

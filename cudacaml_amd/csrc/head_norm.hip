@@ -401,7 +401,8 @@ void launch(const cchip_head_norm &op, HeadArgs &a, const Cut &c, bool back, hip
       case 4: return launch_lanes<T, 4>(a, op.interleaved, back, grid, stream);
       case 8: return launch_lanes<T, 8>(a, op.interleaved, back, grid, stream);
       case 16: return launch_lanes<T, 16>(a, op.interleaved, back, grid, stream);
-      default: return launch_lanes<T, 32>(a, op.interleaved, back, grid, stream);
+      case 32: return launch_lanes<T, 32>(a, op.interleaved, back, grid, stream);
+      default: return launch_lanes<T, 64>(a, op.interleaved, back, grid, stream);
     }
   });
   check_launch(kWho);
