@@ -70,7 +70,7 @@ Cut cut_of(const cchip_attention &op) {
   p.splits = 1;
   // Keys are split where there are too few workgroups for the chip, but into
   // parts that are long beside what joining them costs.
-  const int64_t base = std::max<int64_t>(1, pairs * slots), least = p.waves ? 512 : 128, wanted = p.waves ? 512 : 1024;
+  const int64_t base = std::max<int64_t>(1, pairs * slots), least = !p.waves ? 128 : op.dtype == CCHIP_F32 ? 256 : 512, wanted = p.waves ? 512 : 1024;
   if (!op.sequences && base < wanted) p.splits = int(std::max<int64_t>(1, std::min((wanted + base - 1) / base, keys / least)));
   p.workgroups = pairs * slots * p.splits;  // at most 2^30: splits are few where it is much
   if (p.splits > 1) p.bytes = size_t(op.batch) * op.tokens * op.heads * p.splits * (op.head_dim + 2) * sizeof(float);
@@ -99,11 +99,13 @@ BackCut back_cut_of(const cchip_attention &op) {
   c.key_slots = (op.tokens + kUnit - 1) / kUnit + op.sequences;
   if (c.row_slots > (int64_t(1) << 24) || c.pairs * c.row_slots > (int64_t(1) << 27))
     throw InvalidArgument("attention: more tokens and heads than a launch can have");
-  // chunks of rows that there are four workgroups to a unit, of 2048 rows at
-  // least: a chunk's sums cost what 30 of its rows do
+  // Chunks of rows that there are four workgroups to a unit, of 2048 rows at
+  // least: a chunk's sums cost what 30 of its rows do. Where all keys are too few
+  // workgroups for the chip, what they leave idle costs more: of 256 rows.
   const int64_t high = op.dtype == CCHIP_F32 ? 32 : 64, tiles = (op.tokens * (op.heads / op.kv_heads) + high - 1) / high;
   const int64_t jobs = c.pairs * c.key_slots;
   c.chunks = int(std::max<int64_t>(1, std::min<int64_t>({8, (1024 + jobs - 1) / std::max<int64_t>(1, jobs), tiles * high / 2048})));
+  if (jobs > 0 && jobs * c.chunks < 256) c.chunks = int(std::max<int64_t>(c.chunks, std::min<int64_t>({8, 256 / jobs, tiles * high / 256})));
   c.chunk_tiles = int((tiles + c.chunks - 1) / c.chunks);
   c.sizes = back_sizes(op.dtype, op.head_dim, c.pairs, c.row_slots, c.key_slots, c.chunks);
   return c;

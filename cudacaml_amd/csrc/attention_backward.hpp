@@ -629,6 +629,7 @@ __global__ __launch_bounds__(256) void sum_chunks(const AttentionArgs a) {
       to = c + 1;
     }
   }
+  if (to == 0) from = 0;
   const float *p = a.partial + (s.key_base + s.tile) * a.chunks * 2 * kUnit * a.dim;
   const int pieces = (a.dim + 3) / 4;
   for (int i = threadIdx.x; i < 2 * (kUnit / 8) * pieces; i += 256) {
@@ -638,10 +639,22 @@ __global__ __launch_bounds__(256) void sum_chunks(const AttentionArgs a) {
     float sum[4] = {};
     const float *x = p + int64_t(which) * kUnit * a.dim + (block % 8 * (kUnit / 8) + row) * a.dim + col;
     const int n = a.dim - col < 4 ? a.dim - col : 4;
-    for (int c = from; c < to; c++)
+    const int64_t step = int64_t(2) * kUnit * a.dim;
+    if (n == 4 && a.dim % 4 == 0) {  // all on their way at once: there are eight at most
+      f32x4 y[8];
 #pragma unroll
-      for (int j = 0; j < 4; j++)
-        if (j < n) sum[j] += x[int64_t(c) * 2 * kUnit * a.dim + j];
+      for (int c = 0; c < 8; c++) y[c] = *reinterpret_cast<const f32x4 *>(x + (from + c < to ? from + c : from) * step);
+#pragma unroll
+      for (int c = 0; c < 8; c++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (from + c < to) sum[j] += y[c][j];
+    } else {
+      for (int c = from; c < to; c++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (j < n) sum[j] += x[c * step + j];
+    }
     T *out = reinterpret_cast<T *>(const_cast<char *>(element(which ? a.gv : a.gk, s.batch, s.key0 + key, s.kv, sizeof(T)))) + col;
 #pragma unroll
     for (int j = 0; j < 4; j++)

@@ -635,13 +635,13 @@ __global__ __launch_bounds__(256) void join_splits(const AttentionArgs a) {
   for (int i = 0; i < a.splits; i++) top = fmaxf(top, ms[2 * i]);
   const float from = top == -INFINITY ? 0.0f : top;
   float sum = 0.0f, y[2] = {};
+#pragma unroll 4
   for (int i = 0; i < a.splits; i++) {
     const float f = __builtin_amdgcn_exp2f(ms[2 * i] - from);
     sum += ms[2 * i + 1] * f;
     const float *p = a.partial + (at * a.splits + i) * a.dim;
 #pragma unroll
-    for (int j = 0; j < 2; j++)
-      if (l + 64 * j < a.dim) y[j] += p[l + 64 * j] * f;
+    for (int j = 0; j < 2; j++) y[j] += p[l + 64 * j < a.dim ? l + 64 * j : 0] * f;
   }
   // at = ((batch x kv heads + kv) x tokens + token) x group + head of the group
   const int64_t per_head = a.tokens * a.group, pair = at / per_head, in = at - pair * per_head, token = in / a.group;

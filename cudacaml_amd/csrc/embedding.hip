@@ -31,35 +31,21 @@ struct EmbeddingArgs {
   int pieces;
 };
 
-// A thread has four groups of 8 columns, so that four tokens' ids, and then
-// their rows, are on their way at once.
-constexpr int kAtOnce = 4;
-
+// A thread has eight columns of a row; four rows a thread took as long for
+// 16384 rows of 4096 and 4.4 us in place of 3.1 for 301 of 520.
 template <typename W, typename T>
 __global__ __launch_bounds__(256) void embed(const EmbeddingArgs a) {
-  const uint64_t first = uint64_t(block_index()) * (256 * kAtOnce) + threadIdx.x;
-  uint64_t token[kAtOnce];
-  int64_t col[kAtOnce], id[kAtOnce];
-  int n[kAtOnce];
+  const uint64_t i = uint64_t(block_index()) * 256 + threadIdx.x;
+  if (i >= a.groups) return;
+  const uint64_t token = a.groups <= 0xFFFFFFFFu ? uint32_t(i) / a.per_row : i / a.per_row;
+  const int64_t col = int64_t(i - token * a.per_row) * 8, id = a.ids[token];
+  const int n = a.width - col < 8 ? int(a.width - col) : 8;
+  const bool there = id >= 0 && id < a.vocab;
+  const Raw8<W> r = load8<W>(row_at<W>(a.weight, there ? id : 0) + col, there ? n : 0);
+  float x[8];
 #pragma unroll
-  for (int k = 0; k < kAtOnce; k++) {
-    const uint64_t i = first + k * 256;
-    token[k] = a.groups <= 0xFFFFFFFFu ? uint32_t(i) / a.per_row : i / a.per_row;
-    col[k] = int64_t(i - token[k] * a.per_row) * 8;
-    n[k] = i >= a.groups ? 0 : a.width - col[k] < 8 ? int(a.width - col[k]) : 8;
-    id[k] = n[k] ? a.ids[token[k]] : -1;
-  }
-  Raw8<W> r[kAtOnce];
-#pragma unroll
-  for (int k = 0; k < kAtOnce; k++)
-    r[k] = load8<W>(row_at<W>(a.weight, id[k] < 0 ? 0 : id[k]) + col[k], id[k] >= 0 && id[k] < a.vocab ? n[k] : 0);
-#pragma unroll
-  for (int k = 0; k < kAtOnce; k++) {
-    float x[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) x[j] = id[k] >= 0 && id[k] < a.vocab ? a.scale * float(r[k].x[j]) : 0.0f;
-    if (n[k]) store8<T>(row_at<T>(a.out, token[k]) + col[k], x, n[k]);
-  }
+  for (int j = 0; j < 8; j++) x[j] = there ? a.scale * float(r.x[j]) : 0.0f;
+  store8<T>(row_at<T>(a.out, token) + col, x, n);
 }
 
 // ---- sorting tokens by word ------------------------------------------------------
@@ -499,7 +485,7 @@ int cchip_embedding_forward(const cchip_embedding *op, const cchip_embedding_io 
     if (a.groups > (uint64_t(1) << 39)) throw InvalidArgument("embedding: more than 2^42 elements");
     a.scale = op->scale;
     with_types(*op, [&](auto w, auto t) {
-      hipLaunchKernelGGL((embed<decltype(w), decltype(t)>), grid_of(int64_t((a.groups + 256 * kAtOnce - 1) / (256 * kAtOnce))), dim3(256), 0, (hipStream_t)stream, a);
+      hipLaunchKernelGGL((embed<decltype(w), decltype(t)>), grid_of(int64_t((a.groups + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a);
     });
     check_launch(who);
   });
