@@ -1032,3 +1032,56 @@ def test_attending_on_residents(device):
     heads.free()
     attend.free()
     assert Buffer.live_count() == live
+
+
+# ---- the example -------------------------------------------------------------------
+
+def _example_loss(z, w, ids, target, frequencies):
+    """The example's layer in 64 bits."""
+    rms = lambda x: x / np.sqrt((x * x).mean(-1, keepdims=True) + 1e-6)  # noqa: E731
+    split = lambda x, h: x.reshape(z.batch, z.tokens, h, z.head_dim)  # noqa: E731
+    x = z.width ** 0.5 * w["words"][ids]
+    n = rms(x) * w["first"]
+    angle = np.arange(z.tokens)[None, :, None, None] * frequencies
+    q, k = (A.head_norm(split(n @ w[a], h), w[b], angle, z.head_dim, False, True, 1e-6)
+            for a, b, h in (("wq", "qn", z.heads), ("wk", "kn", z.kv_heads)))
+    v = split(n @ w["wv"], z.kv_heads)
+    o = np.stack([A.attention(q[i], k[i], v[i], z.head_dim ** -0.5) for i in range(z.batch)])
+    y = o.reshape(len(ids), -1) @ w["wo"]
+    m = rms(x + rms(y) * w["post"]) * w["pre"]
+    return ((m @ w["we"] - target) ** 2).mean()
+
+
+def test_the_example_runs_and_its_gradients(device):
+    """Gradients of all weights against differences of the layer in 64 bits,
+    whose own error is their step's square: with half the step a quarter, and
+    so a third of what halving changes. What f32 is off by, in a chain of some
+    twenty sums: 1e-5 of the gradient's norm."""
+    from cudacaml_amd.examples import attention_layer as E
+
+    z = E.Sizes()
+    live = Buffer.live_count()
+    layer = E.Layer(z)
+    ids, target = E.recall_task(z, 1)
+    for _ in range(3):
+        assert np.isfinite(layer.step(ids, target))
+    loss, grads = layer.gradients(ids, target)
+    w = {n: v.astype(np.float64) for n, v in layer.weights.items()}
+    f = lambda w: _example_loss(z, w, ids, target.astype(np.float64), layer.frequencies.astype(np.float64))  # noqa: E731
+    assert abs(loss - f(w)) <= 1e-5 * abs(loss)
+    assert set(grads) == set(w)
+    g = np.random.default_rng(2)
+    for n in grads:
+        way = g.standard_normal(w[n].shape)
+        slopes = [(f({**w, n: w[n] + h * way}) - f({**w, n: w[n] - h * way})) / (2 * h) for h in (1e-4, 5e-5)]
+        off = abs((grads[n] * way).sum() - slopes[1])
+        allowed = abs(slopes[0] - slopes[1]) + 1e-9 + 1e-5 * np.linalg.norm(grads[n]) * np.linalg.norm(way)
+        assert off <= allowed, (n, off, allowed)
+    a, b = layer.predict(ids), layer.evaluate(ids)
+    assert np.abs(a - b).max() <= 1e-5 * np.abs(b).max()
+    layer.release()
+    del layer
+    import gc
+
+    gc.collect()
+    assert Buffer.live_count() <= live
