@@ -475,6 +475,9 @@ __device__ __forceinline__ Span span_of(const AttentionArgs &a, uint32_t id, uin
         tile = int(at) - (of_lane(upto, w) - int(tiles));
         s.row_base += of_lane(upto_rows - rows, w);
         s.key_base += of_lane(upto_keys - keys, w);
+        // offsets that decrease: what lies behind the tiles there is room for
+        const int64_t past = int64_t(pair) + 1;
+        if (a.row_slots && (s.row_base + of_lane(rows, w) > past * a.row_slots || s.key_base + of_lane(keys, w) > past * a.key_slots)) tile = -1;
         break;
       }
       before += of_lane(upto, 63);

@@ -227,6 +227,13 @@ __device__ __forceinline__ void operands_of(Bits<Planes<M>::N> (&p)[2], const f3
   }
 }
 
+// Elements from `at` on are padding: here six products of f32 are worth a
+// branch (heads of 72: 76 us in place of 82), one of 16 bits is not. The other
+// kernels' instructions are in an order that branches would break (of the keys'
+// gradients 74 us in place of 62).
+template <int N>
+__device__ __forceinline__ bool no_product(int at, int dim) { return N > 1 && at >= dim; }
+
 // kUnit rows, 32 a wave, over the keys that they see.
 template <typename T, int D>
 __device__ __forceinline__ void back_rows_job(const AttentionArgs &a, uint32_t id, char *lds, int (&heads)[2][kKeyHead]) {
@@ -296,6 +303,7 @@ __device__ __forceinline__ void back_rows_job(const AttentionArgs &a, uint32_t i
           Ahead<D / 8, N == 1 ? 6 : 2, N> rows;
           rows.start(read);
           rows.run(read, [&](int i, const Bits<N> &f) {
+            if (no_product<N>(16 * (i / 2), a.dim)) return;
             if (i % 2) y = product<M, N>(y, f, g[i / 2]);
             else x = product<M, N>(x, f, q[i / 2]);
           });
@@ -320,7 +328,10 @@ __device__ __forceinline__ void back_rows_job(const AttentionArgs &a, uint32_t i
         }
         Bits<N> p[2];
         operands_of<M>(p, x);
-        columns.run(read, [&](int i, const Bits<N> &f) { out[i % (D / 32)] = product<M, N>(out[i % (D / 32)], f, p[i / (D / 32)]); });
+        columns.run(read, [&](int i, const Bits<N> &f) {
+          if (no_product<N>(32 * (i % (D / 32)), a.dim)) return;
+          out[i % (D / 32)] = product<M, N>(out[i % (D / 32)], f, p[i / (D / 32)]);
+        });
       }
     }
     if (tile + 1 < end && t < kKeyHead) heads[(tile + 1) & 1][t] = head;

@@ -1,6 +1,7 @@
 """Layer operators of language models on device-resident data: the gated
-delta rule, the norm block and dropout, over the C-ABI of
-``include/cchip_operators.h`` (which states what each computes).
+delta rule, attention, the norm and rotation of its heads, the embedding, the
+norm block and dropout, over the C-ABI of ``include/cchip_operators.h`` (which
+states what each computes).
 
 A handle is made once for its shapes, checks the arguments of each call and
 keeps the workspaces, one for each direction and stream it is called on; they
@@ -19,8 +20,8 @@ free of both.
 Arrays are ``Array``, ``backend_hip.Resident`` or anything with ``data_ptr()``,
 ``get_device()``, ``dtype``, ``shape`` and ``stride()``, such as a tensor of
 a GPU framework; their last dimension is contiguous, the others may have any
-stride (tokens of the gated delta rule one of 0 to 2^23 elements). A wrong shape, type or stride raises ``ValueError`` before any device
-work.
+stride (tokens of heads one of 0 to 2^23 elements). A wrong shape, type or
+stride raises ``ValueError`` before any device work.
 """
 
 from __future__ import annotations

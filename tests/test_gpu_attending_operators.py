@@ -160,6 +160,21 @@ def test_attention_offsets_are_clamped(device):
         assert same(a[n], b[n]), n
 
 
+def test_attention_offsets_that_decrease_stay_in_bounds(device):
+    """Sequences that lie over one another have no result to speak of, but
+    need no more of the workspace than others."""
+    x = attention_arrays("bf16", 1, 1000, 2, 1, 32, seed=4)
+    op = O.Attention("bf16", 1, 1000, 2, 1, 32, sequences=3)
+    need = op.workspace_bytes(backward=True)
+    guard = torch.full((need + (1 << 22),), 99, dtype=torch.uint8, device="cuda")
+    for cuts in ([0, 1000, 0, 1000], [1000, 0, 1000, 0], [900, 500, 1000, 100]):
+        run_attention(x, "bf16", cuts=cuts, op=op, backward=guard[:need])
+    assert (guard[need:] == 99).all()
+    a, b = run_attention(x, "bf16", cuts=[0, 10, 10, 1000], op=op), run_attention(x, "bf16", cuts=[0, 10, 10, 1000])
+    for n in a:
+        assert same(a[n], b[n]), n
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("shape", [(0, 10, 2, 1, 8), (2, 0, 2, 1, 8)])
 def test_attention_of_nothing(device, dtype, shape):
