@@ -232,11 +232,12 @@ __device__ __forceinline__ u32x4 finite_only(u32x4 u) {
   return u;
 }
 
+// Of a tile, without what lies between its groups, which nothing writes.
 template <typename T>
-__device__ __forceinline__ bool tile_finite(const u32x4 *tile, int pieces) {
+__device__ __forceinline__ bool tile_finite(const u32x4 *tile, int groups) {
   bool some = false;
-  for (int i = threadIdx.x & 63; i < pieces; i += 64) {
-    const u32x4 u = tile[i];
+  for (int i = 0; i < groups; i++) {
+    const u32x4 u = tile[i * (kGroup / 8) + (threadIdx.x & 63)];
     some = some || some_infinite<T>(u[0]) || some_infinite<T>(u[1]) || some_infinite<T>(u[2]) || some_infinite<T>(u[3]);
   }
   return __ballot(some) == 0;
@@ -391,7 +392,7 @@ __global__ CCHIP_WAVES(Waves * 64, Planes<T>::kWaves) void attend(const Attentio
     constexpr int kLeft = 2 * (kc.kEach + vc.kEach);
     // values that rows see and others do not have to be finite for a product
     const auto values_of = [&](int tile) {
-      if ((tile + 1) * Keys <= all || tile_finite<T>(reinterpret_cast<const u32x4 *>(vt + tile % kSlots * kBuffer), kTile / 8)) return values(tile);
+      if ((tile + 1) * Keys <= all || tile_finite<T>(reinterpret_cast<const u32x4 *>(vt + tile % kSlots * kBuffer), kTile / kGroup)) return values(tile);
       stay_branch();
 #pragma unroll
       for (int i = 0; i < kValues; i++) {
