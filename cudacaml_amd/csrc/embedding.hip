@@ -32,7 +32,7 @@ struct EmbeddingArgs {
 };
 
 // A thread has eight columns of a row; four rows a thread took as long for
-// 16384 rows of 4096 and 4.4 us in place of 3.1 for 301 of 520.
+// 16384 rows of 2048 and 4.4 us in place of 3.1 for 301 of 520.
 template <typename W, typename T>
 __global__ __launch_bounds__(256) void embed(const EmbeddingArgs a) {
   const uint64_t i = uint64_t(block_index()) * 256 + threadIdx.x;
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_words(const EmbeddingArgs a
 
 // All tokens in one workgroup, where they fit into LDS, while the others of
 // the launch clear the gradient, which takes longer: 16384 tokens are sorted in
-// the 38 us that 268 MB of zeros take, in place of 27 us of their own.
+// the 39 us that 268 MB of zeros take, in place of 27 us of their own.
 constexpr int kInOne = 16384, kOneThreads = 1024, kOneWaves = kOneThreads / 64, kOneEach = kInOne / kOneThreads;
 constexpr int kOneBits = 8, kOneBins = 1 << kOneBits;
 constexpr size_t kOneBytes = size_t(kInOne) * sizeof(uint2) + size_t(kOneWaves) * kOneBins * sizeof(uint32_t);
@@ -188,17 +188,18 @@ constexpr size_t kOneBytes = size_t(kInOne) * sizeof(uint2) + size_t(kOneWaves) 
 template <typename W>
 __global__ __launch_bounds__(kOneThreads) void sort_in_one(const EmbeddingArgs a, int passes) {
   extern __shared__ uint2 held[];  // the items, then the counts of each wave
-  __shared__ uint32_t sums[kOneWaves];
+  __shared__ uint32_t sums[kOneWaves], there;
   if (blockIdx.x) return clear_gradient<W>(a, blockIdx.x - 1, gridDim.x - 1);
   uint32_t(*bins)[kOneBins] = reinterpret_cast<uint32_t(*)[kOneBins]>(held + kInOne);
   const int t = threadIdx.x, l = t & 63, w = t >> 6, count = int(a.tokens);
+  const uint32_t none = uint32_t(a.vocab);
   // a wave has as many rounds of 64 tokens side by side
   const int rounds = (count + kOneThreads - 1) / kOneThreads, first = w * rounds * 64 + l;
   uint2 item[kOneEach];
 #pragma unroll
   for (int i = 0; i < kOneEach; i++) {
     const int at = first + i * 64;
-    item[i] = make_uint2(0, 0);
+    item[i] = make_uint2(none, 0);
     if (i < rounds && at < count) item[i] = make_uint2(word_of(a, at), uint32_t(at));
   }
   for (int pass = 0; pass < passes; pass++) {
@@ -208,7 +209,7 @@ __global__ __launch_bounds__(kOneThreads) void sort_in_one(const EmbeddingArgs a
     uint32_t rank[kOneEach];
 #pragma unroll
     for (int i = 0; i < kOneEach; i++)
-      if (i < rounds) rank[i] = rank_of<kOneBits>(first + i * 64 < count, item[i].x >> (pass * kOneBits) & (kOneBins - 1), bins[w]);
+      if (i < rounds) rank[i] = rank_of<kOneBits>(item[i].x != none, item[i].x >> (pass * kOneBits) & (kOneBins - 1), bins[w]);
     __syncthreads();
     uint32_t all = 0, upto = 0;
     if (t < kOneBins) {
@@ -224,6 +225,7 @@ __global__ __launch_bounds__(kOneThreads) void sort_in_one(const EmbeddingArgs a
     __syncthreads();
     if (t < kOneBins) {
       for (int i = 0; i < w; i++) upto += sums[i];
+      if (t == kOneBins - 1) there = upto;
       uint32_t from = upto - all;
       for (int i = 0; i < kOneWaves; i++) {
         const uint32_t n = bins[i][t];
@@ -234,11 +236,12 @@ __global__ __launch_bounds__(kOneThreads) void sort_in_one(const EmbeddingArgs a
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kOneEach; i++)
-      if (i < rounds && first + i * 64 < count) held[bins[w][item[i].x >> (pass * kOneBits) & (kOneBins - 1)] + rank[i]] = item[i];
+      if (i < rounds && item[i].x != none) held[bins[w][item[i].x >> (pass * kOneBits) & (kOneBins - 1)] + rank[i]] = item[i];
     __syncthreads();
+    // what has no word is dropped here, and comes last as such
 #pragma unroll
     for (int i = 0; i < kOneEach; i++)
-      if (i < rounds && first + i * 64 < count) item[i] = held[first + i * 64];
+      if (i < rounds) item[i] = first + i * 64 < int(there) ? held[first + i * 64] : make_uint2(none, 0);
     __syncthreads();
   }
 #pragma unroll
@@ -422,7 +425,7 @@ Layout layout_of(const cchip_embedding &op) {
   Layout p = {};
   if (op.tokens <= kFew) return p;
   while (op.vocab >> (p.passes * kBits)) p.passes++;  // words 0 .. vocab
-  while (op.vocab >> (p.one_passes * kOneBits)) p.one_passes++;
+  for (p.one_passes = 1; (op.vocab - 1) >> (p.one_passes * kOneBits);) p.one_passes++;  // words that there are
   p.blocks = int((op.tokens + kBlock - 1) / kBlock);
   p.pieces = int((op.tokens + kPiece - 1) / kPiece);
   p.counts = size_t(p.passes) * p.blocks * kBins * sizeof(uint32_t);
