@@ -248,18 +248,30 @@ __device__ __forceinline__ bool tile_finite(const u32x4 *tile, int groups) {
 // would bring them to the rows that do not, as zero times infinity.
 template <typename T, int D>
 __device__ __forceinline__ void add_infinite(Running<D> &r, const T *v, int64_t stride, int64_t keys, int64_t seen, int dim) {
-  const int half = (threadIdx.x & 63) >> 5;
+  const int l = threadIdx.x & 63, half = l >> 5;
 #pragma unroll 1
-  for (int64_t j = 0; j < keys; j++) {
+  for (int64_t j0 = 0; j0 < keys; j0 += 8) {
+    uint32_t rows = 0;  // of eight, that have any
 #pragma unroll
-    for (int d = 0; d < D / 32; d++)
+    for (int i = 0; i < 8; i++) {
+      const T *row = v + (j0 + i < keys ? j0 + i : j0) * stride;
+      bool some = false;
 #pragma unroll
-      for (int i = 0; i < 16; i++) {
-        const int at = 32 * d + 8 * (i / 4) + 4 * half + i % 4;
-        if (at >= dim) continue;
-        const float x = float(v[j * stride + at]);
-        if (!(__builtin_fabsf(x) < INFINITY) && j < seen) r.out[d][i] += x;
-      }
+      for (int d = 0; d < D; d += 64) some = some || (l + d < dim && !(__builtin_fabsf(float(row[l + d])) < INFINITY));
+      if (__ballot(some) && j0 + i < keys) rows |= 1u << i;
+    }
+    for (; rows; rows &= rows - 1) {
+      const int64_t j = j0 + __builtin_ctz(rows);
+#pragma unroll
+      for (int d = 0; d < D / 32; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const int at = 32 * d + 8 * (i / 4) + 4 * half + i % 4;
+          if (at >= dim) continue;
+          const float x = float(v[j * stride + at]);
+          if (!(__builtin_fabsf(x) < INFINITY) && j < seen) r.out[d][i] += x;
+        }
+    }
   }
 }
 
