@@ -1,5 +1,5 @@
-// What the layer operators (delta*.hip, norm_block.hip, dropout.hip) share:
-// element types, raw loads at any alignment, matrix-core fragments held in
+// What the layer operators (delta*.hip, attention*.hip, head_norm.hip,
+// embedding.hip, norm_block*.hip, dropout.hip) share: element types, raw loads at any alignment, matrix-core fragments held in
 // one to three bf16 planes, and the counter-based generator.
 #pragma once
 

@@ -1,5 +1,6 @@
-// Matrices of rows for the dropout and the norm block: addressing, stores,
-// dropout's parameters and the checks of arguments they share.
+// Matrices of rows for the dropout, the norm block and the embedding:
+// addressing, stores, dropout's parameters and the checks of arguments they
+// share.
 #pragma once
 
 #include <cstdlib>
