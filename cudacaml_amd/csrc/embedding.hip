@@ -343,16 +343,19 @@ __global__ __launch_bounds__(256) void join_words(const EmbeddingArgs a) {
   if (word >= a.vocab || a.sorted[last + 1].x != word) return;
   // a run that began before this piece and fills it is another workgroup's
   if (piece > 0 && a.sorted[last - kPiece].x == word) return;
-  const int64_t col = (int64_t(blockIdx.z) * blockDim.x + threadIdx.x) * 8;
-  if (col >= a.width) return;
-  const int n = a.width - col < 8 ? int(a.width - col) : 8;
-  // the piece that it ends in: the last whose first token is the run's
-  int64_t lo = piece + 1, hi = a.pieces - 1;
+  // the piece that it ends in: the last whose first token is the run's, among
+  // the next 64 by a lane each, beyond them by halves
+  const int64_t at = piece + 2 + (threadIdx.x & 63);
+  const uint64_t others = ~__ballot(at < a.pieces && a.sorted[at < a.pieces ? at * kPiece : last].x == word);
+  int64_t lo = piece + 1 + (others ? __builtin_ctzll(others) : 64), hi = others ? lo : a.pieces - 1;
   while (lo < hi) {
     const int64_t mid = (lo + hi + 1) / 2;
     if (a.sorted[mid * kPiece].x == word) lo = mid;
     else hi = mid - 1;
   }
+  const int64_t col = (int64_t(blockIdx.z) * blockDim.x + threadIdx.x) * 8;
+  if (col >= a.width) return;
+  const int n = a.width - col < 8 ? int(a.width - col) : 8;
   float sum[8];
   const float *p = a.partial + (piece * 2 + 1) * a.width + col;
 #pragma unroll
