@@ -33,6 +33,7 @@ struct EmbeddingArgs {
   const uint2 *sorted;
   float *partial;  // [piece][first run, last run][width]
   int pieces;
+  int lanes;  // threads of a row, a power of two in 4 .. 256; 256 threads have as many pieces at a time as they have room for
 };
 
 // A thread has eight columns of a row; four rows a thread took as long for
@@ -279,18 +280,18 @@ __device__ __forceinline__ void add_row(const EmbeddingArgs &a, uint32_t word, i
 
 template <typename W, typename T>
 __global__ __launch_bounds__(256) void sum_words(const EmbeddingArgs a) {
-  __shared__ uint2 items[kPiece + 2];  // the piece's, and its neighbours'
-  const int t = threadIdx.x;
-  const int64_t piece = block_index();
-  if (piece >= a.pieces) return;
+  extern __shared__ uint2 pieces[];  // [piece][its items, and its neighbours']
+  const int t = threadIdx.x & (a.lanes - 1), g = threadIdx.x / a.lanes;
+  const int64_t piece = int64_t(block_index()) * (256 / a.lanes) + g;
+  uint2 *const items = pieces + g * (kPiece + 2);
   const int64_t at0 = piece * kPiece;
-  for (int i = t; i < kPiece + 2; i += blockDim.x) {
+  for (int i = t; i < kPiece + 2; i += a.lanes) {
     const int64_t at = at0 + i - 1;
     items[i] = at >= 0 && at < a.tokens ? a.sorted[at] : make_uint2(0xFFFFFFFFu, 0);
   }
   __syncthreads();
-  const int64_t col = (int64_t(blockIdx.z) * blockDim.x + t) * 8;
-  if (col >= a.width) return;
+  const int64_t col = (int64_t(blockIdx.z) * a.lanes + t) * 8;
+  if (piece >= a.pieces || col >= a.width) return;
   const int n = a.width - col < 8 ? int(a.width - col) : 8;
   const int count = a.tokens - at0 < kPiece ? int(a.tokens - at0) : kPiece;
   float sum[8] = {};
@@ -334,6 +335,8 @@ __global__ __launch_bounds__(256) void sum_words(const EmbeddingArgs a) {
 }
 
 // Runs that begin in one piece and end in another, by the piece they begin in.
+// A word of 45000 of 406000 tokens, rows of 57: 313 us by 8 threads in one
+// chain of its 1400 pieces, 26 as the workgroup shares them out.
 template <typename W>
 __global__ __launch_bounds__(256) void join_words(const EmbeddingArgs a) {
   const int64_t piece = block_index();
@@ -353,22 +356,38 @@ __global__ __launch_bounds__(256) void join_words(const EmbeddingArgs a) {
     if (a.sorted[mid * kPiece].x == word) lo = mid;
     else hi = mid - 1;
   }
-  const int64_t col = (int64_t(blockIdx.z) * blockDim.x + threadIdx.x) * 8;
-  if (col >= a.width) return;
+  // its pieces' parts by the groups of threads in turn, then the groups'
+  __shared__ float sums[256][8];
+  const int t = threadIdx.x & (a.lanes - 1), g = threadIdx.x / a.lanes, groups = 256 / a.lanes;
+  const int64_t col = (int64_t(blockIdx.z) * a.lanes + t) * 8;
   const int n = a.width - col < 8 ? int(a.width - col) : 8;
-  float sum[8];
-  const float *p = a.partial + (piece * 2 + 1) * a.width + col;
+  float sum[8] = {};
+  if (n > 0) {
+    if (g == 0) {
+      const Raw8<float> r = load8<float>(a.partial + (piece * 2 + 1) * a.width + col, n);
 #pragma unroll
-  for (int j = 0; j < 8; j++) sum[j] = j < n ? p[j] : 0.0f;
-  for (int64_t i0 = piece + 1; i0 <= lo; i0 += 8) {
-    Raw8<float> r[8];
+      for (int j = 0; j < 8; j++) sum[j] = r.x[j];
+    }
+    for (int64_t i0 = piece + 1 + g; i0 <= lo; i0 += 8 * groups) {
+      Raw8<float> r[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) r[i] = load8<float>(a.partial + (i0 + i <= lo ? i0 + i : lo) * 2 * a.width + col, i0 + i <= lo ? n : 0);
+      for (int i = 0; i < 8; i++) {
+        const int64_t at = i0 + i * groups;
+        r[i] = load8<float>(a.partial + (at <= lo ? at : lo) * 2 * a.width + col, at <= lo ? n : 0);
+      }
 #pragma unroll
-    for (int i = 0; i < 8; i++)
+      for (int i = 0; i < 8; i++)
 #pragma unroll
-      for (int j = 0; j < 8; j++) sum[j] += r[i].x[j];
+        for (int j = 0; j < 8; j++) sum[j] += r[i].x[j];
+    }
   }
+#pragma unroll
+  for (int j = 0; j < 8; j++) sums[threadIdx.x][j] = sum[j];
+  __syncthreads();
+  if (g > 0 || n <= 0) return;
+  for (int i = 1; i < groups; i++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) sum[j] += sums[i * a.lanes + t][j];
   add_row<W>(a, word, col, n, sum);
 }
 
@@ -580,14 +599,17 @@ int cchip_embedding_backward(const cchip_embedding *op, const cchip_embedding_io
       }
     }
     a.sorted = a.to;
-    dim3 grid = grid_of(p.pieces);
-    grid.z = columns;
+    a.lanes = 4;
+    while (a.lanes < 256 && uint32_t(a.lanes) < a.per_row) a.lanes *= 2;
+    const int at_once = 256 / a.lanes;
+    dim3 grid = grid_of((p.pieces + at_once - 1) / at_once), join_grid = grid_of(p.pieces);
+    grid.z = join_grid.z = unsigned((a.per_row + a.lanes - 1) / a.lanes);
     with_types(*op, [&](auto w, auto t) {
       typedef decltype(w) W;
       typedef decltype(t) T;
-      hipLaunchKernelGGL((sum_words<W, T>), grid, dim3(threads), 0, s, a);
+      hipLaunchKernelGGL((sum_words<W, T>), grid, dim3(256), size_t(at_once) * (kPiece + 2) * sizeof(uint2), s, a);
       check_launch(who);
-      if (p.pieces > 1) hipLaunchKernelGGL((join_words<W>), grid, dim3(threads), 0, s, a);
+      if (p.pieces > 1) hipLaunchKernelGGL((join_words<W>), join_grid, dim3(256), 0, s, a);
     });
     check_launch(who);
   });
