@@ -134,10 +134,15 @@ __global__ __launch_bounds__(kSortThreads) void sort_words(const EmbeddingArgs a
 
   // this thread's bin: what blocks before have of it, and what all have
   uint32_t before = 0, all = 0;
-  for (int64_t b = 0; b < a.blocks; b++) {
-    const uint32_t n = a.counts[b * kBins + t];
-    if (b < block) before += n;
-    all += n;
+  for (int64_t b0 = 0; b0 < a.blocks; b0 += 16) {
+    uint32_t n[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) n[i] = a.counts[(b0 + i < a.blocks ? b0 + i : b0) * kBins + t];
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      if (b0 + i < block) before += n[i];
+      if (b0 + i < a.blocks) all += n[i];
+    }
   }
   uint32_t upto = all;
 #pragma unroll
