@@ -17,10 +17,10 @@
 // would make it 1.5 times as much). f32 becomes three bf16 planes.
 //
 // 8192 packed tokens, 16 heads of 128 over 4, bf16, 407 GFLOP with the forward
-// pass's 199 us: 45 us for laying out, 225 for the rows, 359 for the keys and
-// 20 for the sums of chunks, 840 together. The rows' kernel has two waves a
-// SIMD; the keys' has registers for one, and vector instructions (one in two is a
-// term's) in the way of its products: 2.5 us for 64 rows and 128 keys, of
+// pass's 192 us: 45 us for laying out, 227 for the rows, 367 for the keys and
+// 20 for the sums of chunks, 838 together. The rows' kernel has two waves a
+// SIMD; the keys' has registers for one, with vector instructions in the way
+// of its products: 2.5 us for 64 rows and 128 keys, of
 // which the products are 0.9.
 
 #include <algorithm>
