@@ -345,6 +345,34 @@ def test_attention_strides(device, dtype, layout, shape):
         assert same(a[n], b[n]), n
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_attention_inputs_read_again(device, dtype):
+    """Keys of one row and head for all of them, values of one token."""
+    x = attention_arrays(dtype, 2, 150, 4, 2, 64, seed=30)
+    x["k"] = x["k"][:1, :, :1].expand_as(x["k"]).contiguous()
+    x["v"] = x["v"][:, :1].expand_as(x["v"]).contiguous()
+    again = lambda d: {**d, "k": d["k"][:1, :, :1].expand(d["k"].shape), "v": d["v"][:, :1].expand(d["v"].shape)}  # noqa: E731
+    a, b = run_attention(x, dtype), run_attention(x, dtype, layout=again)
+    for n in a:
+        assert same(a[n], b[n]), n
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_attention_rows_do_not_depend_on_one_another(device, dtype):
+    """A sequence alone, among others and behind one that is much longer: its
+    rows lie with others in a tile or alone, with the same results."""
+    x = attention_arrays(dtype, 1, 700, 6, 2, 64, seed=31)
+    a = run_attention(x, dtype, cuts=[0, 450, 530, 700])
+    parts = {n: v[:, 450:530].contiguous() for n, v in x.items()}
+    b = run_attention(parts, dtype, cuts=[0, 80])
+    for n in ("o", "dq"):
+        assert same(a[n][:, 450:530], b[n]), n
+    q = x["q"].clone()
+    q[:, ::2] *= 30  # every other query's scores rise far more
+    c = run_attention({**x, "q": q}, dtype, cuts=[0, 450, 530, 700])
+    assert same(a["o"][:, 1::2], c["o"][:, 1::2])
+
+
 @pytest.mark.parametrize("shape,tokens", [((2, 300, 2, 1, 64), False), ((1, 600, 2, 1, 64), True)])
 def test_attention_tensors_past_32_bits(device, shape, tokens):
     x = attention_arrays("bf16", *shape, seed=12)
