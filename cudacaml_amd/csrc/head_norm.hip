@@ -215,7 +215,9 @@ __global__ __launch_bounds__(kWaves * 64) void head_norm(const HeadArgs a) {
             sum += lo[i] * lo[i] + hi[i] * hi[i];
             dot += gl[i] * wl[i] * lo[i] + gh[i] * wh[i] * hi[i];
           }
-          const float inv = 1.0f / __builtin_sqrtf(sum_lanes<Lanes>(sum) / float(a.dim) + a.eps);
+          // behind the last head there is nothing to add, with an eps of zero 0 times an infinity
+          sum = sum_lanes<Lanes>(sum);
+          const float inv = live ? 1.0f / __builtin_sqrtf(sum / float(a.dim) + a.eps) : 0.0f;
           const float mean = sum_lanes<Lanes>(dot) / float(a.dim) * inv * inv;
 #pragma unroll
           for (int i = 0; i < 8; i++) {

@@ -1,0 +1,44 @@
+"""Attention, the norm and rotation of its heads and the embedding where a
+formula is still defined but little is left of it: no eps, infinities, the
+largest values, counts of tokens that few calls have. Tolerances are those of
+test_gpu_attending_operators.py."""
+
+import numpy as np
+import pytest
+import torch
+
+import attending_reference as A
+from cudacaml_amd import operators as O
+from test_gpu_attending_operators import TYPES, f64, nans, normal, same
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- norm and rotation of heads --------------------------------------------------
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("h,hk,d,rotary,tokens", [(3, 1, 64, 64, 7), (2, 4, 128, 128, 7), (5, 3, 40, 16, 7), (9, 2, 64, 64, 2100)])
+def test_head_norm_without_eps(device, dtype, h, hk, d, rotary, tokens):
+    """Heads that do not fill a wave: what is beyond the last one adds nothing
+    to the gradients of the weights, with an eps of zero either."""
+    op = O.HeadNorm(dtype, 1, tokens, h, hk, d, rotary=rotary, eps=0.0)
+    x = {n: normal(dtype, 1, tokens, c, d, seed=40 + i) for i, (n, c) in enumerate((("q", h), ("k", hk), ("dq", h), ("dk", hk)))}
+    freq = torch.exp(-torch.arange(rotary // 2) * 0.4).float()
+    w = {n: 1.0 + 0.3 * normal("f32", d, seed=44 + i) for i, n in enumerate(("q_weight", "k_weight"))}
+    dev = {n: v.cuda() for n, v in x.items()}
+    given = dict(frequencies=freq.cuda(), **{n: v.cuda() for n, v in w.items()})
+    out, grads = {n: nans(v.shape, dtype) for n, v in x.items()}, {n: nans((d,), "f32") for n in w}
+    op.forward(dev["q"], dev["k"], out["q"], out["k"], **given)
+    op.backward(dev["q"], dev["k"], dev["dq"], dev["dk"], out["dq"], out["dk"], grads=grads, **given)
+    torch.cuda.synchronize()
+    angle = np.arange(tokens)[None, :, None, None] * f64(freq)
+    for n in ("q", "k"):
+        a, g, ww = f64(x[n]), f64(x["d" + n]), f64(w[n + "_weight"])
+        how = (rotary, False, True, 0.0)
+        plain = A.head_norm(a, ww, angle * 0, *how)
+        A.near(f64(out[n]), A.head_norm(a, ww, angle, *how), n, A.HALF[dtype], 2.0 ** -19 * np.abs(plain).max(-1, keepdims=True))
+        dx, dw, terms = A.head_norm(a, ww, angle, *how, dy=g)
+        inv = 1.0 / np.sqrt((a * a).mean(-1, keepdims=True))
+        big = np.abs(g).max(-1, keepdims=True) * np.abs(ww).max() * inv
+        A.near(f64(out["d" + n]), dx, "d" + n, A.HALF[dtype], 2.0 ** -19 * big * (1 + np.abs(a * inv).max(-1, keepdims=True)))
+        A.near(f64(grads[n + "_weight"]), dw, n + "_weight", A.HALF["f32"], 2.0 ** -18 * terms)
