@@ -63,7 +63,9 @@ __device__ __forceinline__ float sum_lanes(float x) {
 }
 
 // A lane's pairs: `count` elements from first on and `seconds` from second on,
-// the elements of a pair side by side in both (alternate) or one in each.
+// the elements of a pair side by side in both (alternate) or one in each. Those
+// that are not rotated have nothing to do with one another: no turn of zero,
+// in which an infinity in one would be a NaN in the other.
 struct Pairs {
   int first, second, count, seconds;
   bool rotated, alternate;
@@ -187,7 +189,7 @@ __global__ __launch_bounds__(kWaves * 64) void head_norm(const HeadArgs a) {
 #pragma unroll
           for (int i = 0; i < 8; i++) lo[i] *= inv * wl[i], hi[i] *= inv * wh[i];
         }
-        if (!plain) {
+        if (at.rotated && !plain) {
 #pragma unroll
           for (int i = 0; i < 8; i++) {
             const float x = lo[i] * cs[i] - hi[i] * sn[i];
@@ -202,11 +204,13 @@ __global__ __launch_bounds__(kWaves * 64) void head_norm(const HeadArgs a) {
       } else {
         float gl[8], gh[8];
         load_pairs<T, Interleaved>(reinterpret_cast<const T *>(part.g.p) + batch * part.g.b + in * part.g.t + h * part.g.h, at, live, gl, gh);
+        if (at.rotated) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const float x = gl[i] * cs[i] + gh[i] * sn[i];
-          gh[i] = gh[i] * cs[i] - gl[i] * sn[i];
-          gl[i] = x;
+          for (int i = 0; i < 8; i++) {
+            const float x = gl[i] * cs[i] + gh[i] * sn[i];
+            gh[i] = gh[i] * cs[i] - gl[i] * sn[i];
+            gl[i] = x;
+          }
         }
         if (a.norm) {
           float sum = 0.0f, dot = 0.0f;

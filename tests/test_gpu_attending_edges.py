@@ -42,3 +42,35 @@ def test_head_norm_without_eps(device, dtype, h, hk, d, rotary, tokens):
         big = np.abs(g).max(-1, keepdims=True) * np.abs(ww).max() * inv
         A.near(f64(out["d" + n]), dx, "d" + n, A.HALF[dtype], 2.0 ** -19 * big * (1 + np.abs(a * inv).max(-1, keepdims=True)))
         A.near(f64(grads[n + "_weight"]), dw, n + "_weight", A.HALF["f32"], 2.0 ** -18 * terms)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("d,rotary", [(40, 0), (64, 16), (37, 20), (64, 64)])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_head_norm_elements_that_are_not_rotated_stand_alone(device, dtype, d, rotary, bad):
+    """Without a norm they are copied: what is not finite in one changes no
+    other, forward or back, and in a rotated one its pair alone."""
+    op = O.HeadNorm(dtype, 1, 5, 3, 2, d, rotary=rotary, norm="none")
+    x = [normal(dtype, 1, 5, c, d, seed=50 + i).cuda() for i, c in enumerate((3, 2, 3, 2))]
+    freq = torch.linspace(1.0, 0.1, rotary // 2, device="cuda")
+
+    def run():
+        out = [nans(v.shape, dtype) for v in x]
+        op.forward(*x[:2], *out[:2], frequencies=freq)
+        op.backward(*x, *out[2:], frequencies=freq)
+        torch.cuda.synchronize()
+        return out
+
+    want = run()
+    for at in {0, rotary // 2, max(rotary - 1, 0), rotary % d, d - 1}:
+        mates = {at} if at >= rotary else {at, (at + rotary // 2) % rotary}
+        keep = [v[0, 3, 1, at].item() for v in x]
+        for v in x:
+            v[0, 3, 1, at] = bad
+        for got, before in zip(run(), want):
+            for i in mates:
+                assert not torch.isfinite(got[0, 3, 1, i]), (at, i)
+                got[0, 3, 1, i] = before[0, 3, 1, i]
+            assert same(got, before), at
+        for v, k in zip(x, keep):
+            v[0, 3, 1, at] = k
