@@ -473,6 +473,7 @@ __global__ CCHIP_WAVES(Waves * 64, Planes<T>::kWaves) void attend(const Attentio
     if (first < end) {
       load(first, end);
       copies_done();  // the queries too: a wait within the loop would be for the keys on their way as well
+      if (kTwo) __syncthreads();  // `bad` is clear before a wave that is behind says what it found in the first values
       put(first, end);
       if (behind) {
         load(first + 1, first);

@@ -74,3 +74,51 @@ def test_head_norm_elements_that_are_not_rotated_stand_alone(device, dtype, d, r
             assert same(got, before), at
         for v, k in zip(x, keep):
             v[0, 3, 1, at] = k
+
+
+# ---- attention -------------------------------------------------------------------
+
+def _apart(x, odd):
+    """The array, or a copy whose heads begin off all 16-byte places."""
+    if not odd:
+        return x
+    b, t, h, d = x.shape
+    return torch.empty(b, t, h * d + 3, dtype=x.dtype, device="cuda")[..., 1:1 + h * d].view(x.shape).copy_(x)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("d,odd", [(41, False), (64, True), (128, True), (72, True), (64, False)])
+@pytest.mark.parametrize("tokens,keys", [(300, None), (200, 330)])
+def test_attention_values_not_finite_wherever_they_stand(device, dtype, d, odd, tokens, keys):
+    """In the first tile of keys and later ones, alone and with others, in heads
+    that are copied to their tile and in those that pass through registers,
+    with eight waves a workgroup: who sees one has it in its column, all else is
+    as it was."""
+    n = keys or tokens
+    q, k, v = (normal(dtype, 1, t, c, d, seed=60 + i).cuda() for i, (t, c) in enumerate(((tokens, 4), (n, 2), (n, 2))))
+    k, v = _apart(k, odd), _apart(v, odd)
+    op = O.Attention(dtype, 1, tokens, 4, 2, d, keys=keys)
+    lengths = None if keys is None else torch.tensor([n], dtype=torch.int32, device="cuda")
+
+    def run():
+        o = nans(q.shape, dtype)
+        op.forward(q, k, v, o, lengths=lengths)
+        torch.cuda.synchronize()
+        return o
+
+    want = run()
+    assert torch.isfinite(want).all()
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        for places in ([0], [3], [31, 32], [63], [64], [5, 127], [2, 130, 200], [n - 1], [n - 70, n - 3]):
+            keep = v.clone()
+            for i, at in enumerate(places):
+                v[0, at, 1, (7 + 5 * i) % d] = bad
+            got = run()
+            assert same(got[0, :, :2], want[0, :, :2]), places
+            changed = torch.zeros(tokens, d, dtype=torch.bool, device="cuda")
+            for i, at in enumerate(places):
+                changed[max(0, at - (n - tokens)):, (7 + 5 * i) % d] = True
+            changed = changed[:, None].expand(tokens, 2, d)
+            assert not torch.isfinite(got[0, :, 2:][changed]).any(), places
+            assert same(got[0, :, 2:][~changed], want[0, :, 2:][~changed]), places
+            v.copy_(keep)
