@@ -95,9 +95,10 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), f16x2));
 }
 
-// Eight values as an operand's.
+// Eight values as an operand's; `first` is what the first of several planes is
+// rounded from.
 template <typename T>
-__device__ __forceinline__ Bits<Planes<T>::N> operand_of(const float *x) {
+__device__ __forceinline__ Bits<Planes<T>::N> planes_of(const float *x, const float *first) {
   Bits<Planes<T>::N> r;
   if constexpr (std::is_same<T, f16>::value) {
 #pragma unroll
@@ -110,12 +111,17 @@ __device__ __forceinline__ Bits<Planes<T>::N> operand_of(const float *x) {
     for (int n = 0; n < Planes<T>::N; n++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const uint32_t u = pack_bf16(y[2 * i], y[2 * i + 1]);
+        const uint32_t u = n ? pack_bf16(y[2 * i], y[2 * i + 1]) : pack_bf16(first[2 * i], first[2 * i + 1]);
         r.p[n][i] = u;
         if (n + 1 < Planes<T>::N) y[2 * i] -= low_bf16(u), y[2 * i + 1] -= high_bf16(u);
       }
   }
   return r;
+}
+
+template <typename T>
+__device__ __forceinline__ Bits<Planes<T>::N> operand_of(const float *x) {
+  return planes_of<T>(x, x);
 }
 
 template <typename T>

@@ -178,6 +178,48 @@ __device__ __forceinline__ void store_row(T *p, const f32x16 (&out)[D / 32], flo
     }
 }
 
+// Whether an element is infinite or NaN; and zero in its place. Planes cannot
+// hold one, so that values of f32 are looked at in all tiles, others only in
+// those that some rows do not see all of. As they pass here anyway, values of
+// f32 are made small, and a row's output large again as its sum is divided:
+// a sum over 2^16 keys of any of them, which terms of up to 2^kSlack multiply,
+// stays finite.
+template <typename T>
+constexpr bool kPlanar = Planes<T>::N > 1;
+template <typename T>
+constexpr float kValueScale = kPlanar<T> ? 0x1p-24f : 1.0f;
+
+template <typename T>
+__device__ __forceinline__ bool take_finite(Raw8<T> &r) {
+  if constexpr (kPlanar<T>) {
+    float any = 0.0f;  // NaN: an element is not finite
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      r.x[i] *= kValueScale<T>;
+      any = __builtin_fmaf(r.x[i], 0.0f, any);
+    }
+    if (any == 0.0f) return true;
+    stay_branch();
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (!(__builtin_fabsf(r.x[i]) < INFINITY)) r.x[i] = 0.0f;
+    return false;
+  } else {
+    bool all = true;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const bool finite = __builtin_fabsf(float(r.x[i])) < INFINITY;
+      all = all && finite;
+      if (!finite) r.x[i] = T(0.0f);
+    }
+    return all;
+  }
+}
+
+// What a row's sum of values is multiplied by.
+template <typename T>
+__device__ __forceinline__ float of_sum(float sum) { return sum == 0.0f ? 0.0f : 1.0f / kValueScale<T> / sum; }
+
 // Rows' outputs: to o, or as they are for the sum over splits.
 template <typename T, int D>
 __device__ __forceinline__ void finish(const AttentionArgs &a, const Span &s, Running<D> &r, int64_t row, int split, float sum) {
@@ -197,22 +239,9 @@ __device__ __forceinline__ void finish(const AttentionArgs &a, const Span &s, Ru
   const int64_t token = live ? row / a.group : 0;
   const int head = live ? int(row - token * a.group) : 0;
   T *p = reinterpret_cast<T *>(const_cast<char *>(element(a.o, s.batch, s.first + token, int64_t(s.kv) * a.group + head, sizeof(T))));
-  store_row<T, D>(p, r.out, sum == 0.0f ? 0.0f : 1.0f / sum, a.dim, live, a.o_rest ? a.o_rest + (row_values(a, s) + row) * a.dim : nullptr);
+  store_row<T, D>(p, r.out, of_sum<T>(sum), a.dim, live, a.o_rest ? a.o_rest + (row_values(a, s) + row) * a.dim : nullptr);
   if (a.lse && live && !half)
     a.lse[row_values(a, s) + row] = sum == 0.0f ? INFINITY : r.top - Powers<T>::kLift + __builtin_log2f(sum);
-}
-
-// Whether an element is infinite or NaN; and zero in its place.
-template <typename T>
-__device__ __forceinline__ bool take_finite(Raw8<T> &r) {
-  bool all = true;
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const bool finite = __builtin_fabsf(float(r.x[i])) < INFINITY;
-    all = all && finite;
-    if (!finite) r.x[i] = T(0.0f);
-  }
-  return all;
 }
 
 // The same of eight 16-bit elements as they are: exponents of ones only.
@@ -330,7 +359,7 @@ __global__ CCHIP_WAVES(Waves * 64, Planes<T>::kWaves) void attend(const Attentio
   const auto put = [&](int k_tile, int v_tile) {
     if (k_tile < end) ks.store(t, kt + (k_tile & 1) * kBuffer);
     if (v_tile < end) {
-      if ((v_tile + 1) * Keys > all) {
+      if (kPlanar<T> || (v_tile + 1) * Keys > all) {
         stay_branch();
         bool finite = true;
 #pragma unroll
@@ -468,7 +497,7 @@ __global__ CCHIP_WAVES(Waves * 64, Planes<T>::kWaves) void attend(const Attentio
       phase_done();
     };
     const auto mend = [&](int tile) {
-      if ((tile + 1) * Keys > all && bad[tile & 1] == tile + 1) infinite(tile);
+      if ((kPlanar<T> || (tile + 1) * Keys > all) && bad[tile & 1] == tile + 1) infinite(tile);
     };
     if (first < end) {
       load(first, end);
@@ -554,12 +583,12 @@ __global__ CCHIP_WAVES(256, Planes<T>::kWaves) void attend_few(const AttentionAr
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     bool finite = true;
-    if (masked) {
+    if (kPlanar<T> || masked) {
 #pragma unroll
       for (int i = 0; i < vs.kEach; i++) finite = take_finite(vs.r[i]) && finite;
     }
     vs.store(l, m);
-    const bool some_bad = masked && __ballot(!finite);
+    const bool some_bad = (kPlanar<T> || masked) && __ballot(!finite);
     const T *here = v;
     v += 32 * kWaves * a.v.t;
     if (more) vs.load(l, v, a.v.t, to - next, a.dim);
@@ -634,7 +663,7 @@ __global__ CCHIP_WAVES(256, Planes<T>::kWaves) void attend_few(const AttentionAr
     const int64_t token = (row0 + at_row) / a.group;
     const int head = int(row0 + at_row - token * a.group);
     T *p = reinterpret_cast<T *>(const_cast<char *>(element(a.o, s.batch, s.first + token, int64_t(s.kv) * a.group + head, sizeof(T)))) + col;
-    const float up = its == 0.0f ? 0.0f : 1.0f / its;
+    const float up = of_sum<T>(its);
 #pragma unroll
     for (int j = 0; j < 8; j++)
       if (j < n) {
@@ -669,7 +698,7 @@ __global__ __launch_bounds__(256) void join_splits(const AttentionArgs a) {
   const int64_t per_head = a.tokens * a.group, pair = at / per_head, in = at - pair * per_head, token = in / a.group;
   const int64_t batch = pair / a.kv_heads, head = (pair - batch * a.kv_heads) * a.group + (in - token * a.group);
   T *p = reinterpret_cast<T *>(const_cast<char *>(element(a.o, batch, token, head, sizeof(T))));
-  const float up = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const float up = of_sum<T>(sum);
 #pragma unroll
   for (int j = 0; j < 2; j++)
     if (l + 64 * j < a.dim) {

@@ -9,7 +9,7 @@ import torch
 
 import attending_reference as A
 from cudacaml_amd import operators as O
-from test_gpu_attending_operators import TYPES, f64, nans, normal, same
+from test_gpu_attending_operators import TYPES, attention_arrays, check_attention, f64, nans, normal, run_attention, same
 
 pytestmark = pytest.mark.gpu
 
@@ -122,3 +122,43 @@ def test_attention_values_not_finite_wherever_they_stand(device, dtype, d, odd, 
             assert not torch.isfinite(got[0, :, 2:][changed]).any(), places
             assert same(got[0, :, 2:][~changed], want[0, :, 2:][~changed]), places
             v.copy_(keep)
+
+
+@pytest.mark.parametrize("d,odd", [(41, False), (128, False), (64, True)])
+@pytest.mark.parametrize("tokens,keys", [(300, None), (40, 700), (1, 700)])
+def test_attention_infinities_of_f32_are_infinities(device, d, odd, tokens, keys):
+    """A query that sees one has it, of whatever tile the key is; of both signs,
+    or NaN, it has NaN."""
+    n = keys or tokens
+    inf, nan = float("inf"), float("nan")
+    q, k, v = (normal("f32", 1, t, c, d, seed=70 + i).cuda() for i, (t, c) in enumerate(((tokens, 2), (n, 1), (n, 1))))
+    k, v = _apart(k, odd), _apart(v, odd)
+    op = O.Attention("f32", 1, tokens, 2, 1, d, keys=keys)
+    lengths = None if keys is None else torch.tensor([n], dtype=torch.int32, device="cuda")
+    out = [nans(q.shape, "f32") for _ in range(2)]
+    op.forward(q, k, v, out[0], lengths=lengths)
+    want = out[0].clone()
+    for places in ([(3, inf)], [(0, -inf)], [(100, nan)], [(40, inf), (45, -inf)], [(10, inf), (n - 2, inf)], [(n - 1, -inf)], [(9, inf), (n - 3, nan)]):
+        keep = v.clone()
+        column = want[0, :, :, 7].clone()
+        for at, x in places:
+            v[0, at, 0, 7] = x
+            column[max(0, at - (n - tokens)):] += x
+        op.forward(q, k, v, out[1], lengths=lengths)
+        torch.cuda.synchronize()
+        assert torch.equal(torch.nan_to_num(out[1][0, :, :, 7], nan=7.0), torch.nan_to_num(column, nan=7.0)), places
+        rest = torch.arange(d, device="cuda") != 7
+        assert same(out[1][..., rest], want[..., rest]), places
+        v.copy_(keep)
+
+
+@pytest.mark.parametrize("tokens,d", [(20, 64), (150, 41), (150, 128)])
+def test_attention_largest_f32_values(device, tokens, d):
+    """Next to what f32 holds, which no 16 bits hold: forward where the sums
+    stay below it, and back. Scores are zeros, so no term is larger than 1."""
+    x = attention_arrays("f32", 1, tokens, 2, 1, d, seed=8)
+    x["q"].zero_()
+    x["do"] *= 2.0 ** -20
+    most = torch.finfo(torch.float32).max
+    x["v"][0, 2, 0, 3], x["v"][0, tokens - 7, 0, 5], x["v"][0, 5, 0, 6] = most, -most, 3.395e38
+    check_attention(x, "f32", run_attention(x, "f32"))
