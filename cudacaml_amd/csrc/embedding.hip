@@ -29,6 +29,8 @@ struct EmbeddingArgs {
   uint2 *from, *to;        // (word, token); null `from`: the ids themselves
   uint32_t *counts, *next;  // [block][kBins] of this pass and the one after; null: there is none
   int blocks, shift;
+  uint32_t *totals;  // [group of blocks][kBins]
+  int group;         // blocks of a group; 0: each block adds all blocks' counts up
   // sums
   const uint2 *sorted;
   float *partial;  // [piece][first run, last run][width]
@@ -57,10 +59,17 @@ __global__ __launch_bounds__(256) void embed(const EmbeddingArgs a) {
 
 // A stable radix sort, kBits of the word a pass. A block of kBlock tokens is a
 // workgroup's; its place in each bin is the sum of what all blocks have of
-// the bins before and the blocks before of this one, which every workgroup
-// adds up for itself from the counts in memory (they are 2 KB a block).
+// the bins before and the blocks before of this one. Up to kAddUp blocks every
+// workgroup adds that up for itself from the counts in memory (they are 2 KB a
+// block). Beyond that, as such reads grow with the square of the tokens (2^30
+// would read 560 TB), two kernels before it do so for groups of blocks.
 constexpr int kBits = 9, kBins = 1 << kBits, kSortThreads = 512, kSortWaves = kSortThreads / 64, kEach = 4;
 constexpr int kBlock = kSortThreads * kEach;
+// Both ways take as long for 192 blocks: 94.5 us, in place of 102, for 128 (262144
+// tokens, rows of 64), 134 in place of 129 for 256, 253 and 206 for 512, 4385 and
+// 1102 for 4096 (rows of 8). Groups are of 64 blocks, or of more where there
+// would be over 1024 of them.
+constexpr int kAddUp = 192, kGroup = 64, kGroups = 1024;
 
 __device__ __forceinline__ uint32_t word_of(const EmbeddingArgs &a, int64_t token) {
   const int64_t id = a.ids[token];
@@ -126,22 +135,20 @@ __device__ __forceinline__ uint32_t rank_of(bool live, uint32_t digit, uint32_t 
   return had + ahead;
 }
 
-__global__ __launch_bounds__(kSortThreads) void sort_words(const EmbeddingArgs a) {
-  __shared__ uint32_t bins[kSortWaves][kBins], base[kBins], sums[kSortWaves];
-  static_assert(kBins == kSortThreads, "a thread a bin");
+// Where the items of the thread's bin begin that row `row` of `rows` rows of
+// counts has: behind all rows' of the bins before and the rows' before of this
+// one. For all threads of a workgroup; `sums` is in LDS.
+__device__ __forceinline__ uint32_t place_of(const uint32_t *counts, int64_t rows, int64_t row, uint32_t (&sums)[kSortWaves]) {
   const int t = threadIdx.x, l = t & 63, w = t >> 6;
-  const int64_t block = blockIdx.x;
-
-  // this thread's bin: what blocks before have of it, and what all have
   uint32_t before = 0, all = 0;
-  for (int64_t b0 = 0; b0 < a.blocks; b0 += 16) {
+  for (int64_t r0 = 0; r0 < rows; r0 += 16) {
     uint32_t n[16];
 #pragma unroll
-    for (int i = 0; i < 16; i++) n[i] = a.counts[(b0 + i < a.blocks ? b0 + i : b0) * kBins + t];
+    for (int i = 0; i < 16; i++) n[i] = counts[(r0 + i < rows ? r0 + i : r0) * kBins + t];
 #pragma unroll
     for (int i = 0; i < 16; i++) {
-      if (b0 + i < block) before += n[i];
-      if (b0 + i < a.blocks) all += n[i];
+      if (r0 + i < row) before += n[i];
+      if (r0 + i < rows) all += n[i];
     }
   }
   uint32_t upto = all;
@@ -151,11 +158,50 @@ __global__ __launch_bounds__(kSortThreads) void sort_words(const EmbeddingArgs a
     if (l >= d) upto += x;
   }
   if (l == 63) sums[w] = upto;
+  __syncthreads();
+  for (int i = 0; i < w; i++) upto += sums[i];
+  return upto - all + before;
+}
+
+// Many blocks: what a group of them has in each bin, and then each block's
+// places in the place of its counts.
+__global__ __launch_bounds__(kSortThreads) void sum_groups(const EmbeddingArgs a) {
+  const int t = threadIdx.x;
+  const int64_t first = int64_t(blockIdx.x) * a.group, end = first + a.group < a.blocks ? first + a.group : a.blocks;
+  uint32_t sum = 0;
+#pragma unroll 16
+  for (int64_t b = first; b < end; b++) sum += a.counts[b * kBins + t];
+  a.totals[int64_t(blockIdx.x) * kBins + t] = sum;
+}
+
+__global__ __launch_bounds__(kSortThreads) void place_blocks(const EmbeddingArgs a) {
+  __shared__ uint32_t sums[kSortWaves];
+  const int t = threadIdx.x;
+  const int64_t first = int64_t(blockIdx.x) * a.group, end = first + a.group < a.blocks ? first + a.group : a.blocks;
+  uint32_t place = place_of(a.totals, gridDim.x, blockIdx.x, sums);
+  for (int64_t b0 = first; b0 < end; b0 += 16) {
+    uint32_t n[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) n[i] = a.counts[(b0 + i < end ? b0 + i : b0) * kBins + t];
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      if (b0 + i >= end) break;
+      a.counts[(b0 + i) * kBins + t] = place;
+      place += n[i];
+    }
+  }
+}
+
+__global__ __launch_bounds__(kSortThreads) void sort_words(const EmbeddingArgs a) {
+  __shared__ uint32_t bins[kSortWaves][kBins], base[kBins], sums[kSortWaves];
+  static_assert(kBins == kSortThreads, "a thread a bin");
+  const int t = threadIdx.x, l = t & 63, w = t >> 6;
+  const int64_t block = blockIdx.x;
+
+  base[t] = a.group ? a.counts[block * kBins + t] : place_of(a.counts, a.blocks, block, sums);
 #pragma unroll
   for (int i = 0; i < kSortWaves; i++) bins[i][t] = 0;
   __syncthreads();
-  for (int i = 0; i < w; i++) upto += sums[i];
-  base[t] = upto - all + before;
 
   // ranks among a wave's equal digits, tokens in order
   uint2 item[kEach];
@@ -447,9 +493,9 @@ __global__ __launch_bounds__(256) void sum_few(const EmbeddingArgs a) {
 // ---- host ----------------------------------------------------------------------------
 
 struct Layout {
-  int passes, one_passes, blocks, pieces;
-  size_t counts, items, partial;  // bytes
-  size_t bytes() const { return counts + 2 * items + partial; }
+  int passes, one_passes, blocks, group, groups, pieces;
+  size_t counts, totals, items, partial;  // bytes
+  size_t bytes() const { return counts + totals + 2 * items + partial; }
 };
 
 Layout layout_of(const cchip_embedding &op) {
@@ -458,6 +504,11 @@ Layout layout_of(const cchip_embedding &op) {
   while (op.vocab >> (p.passes * kBits)) p.passes++;  // words 0 .. vocab
   for (p.one_passes = 1; (op.vocab - 1) >> (p.one_passes * kOneBits);) p.one_passes++;  // words that there are
   p.blocks = int((op.tokens + kBlock - 1) / kBlock);
+  if (p.blocks > kAddUp) {
+    p.group = std::max(kGroup, (p.blocks + kGroups - 1) / kGroups);
+    p.groups = (p.blocks + p.group - 1) / p.group;
+  }
+  p.totals = size_t(p.groups) * kBins * sizeof(uint32_t);
   p.pieces = int((op.tokens + kPiece - 1) / kPiece);
   p.counts = size_t(p.passes) * p.blocks * kBins * sizeof(uint32_t);
   p.items = (size_t(op.tokens) * sizeof(uint2) + 15) / 16 * 16;
@@ -558,8 +609,11 @@ int cchip_embedding_backward(const cchip_embedding *op, const cchip_embedding_io
     a.pieces = p.pieces;
     char *at = static_cast<char *>(workspace);
     uint32_t *counts = reinterpret_cast<uint32_t *>(at);
-    uint2 *items[2] = {reinterpret_cast<uint2 *>(at + p.counts), reinterpret_cast<uint2 *>(at + p.counts + p.items)};
-    a.partial = reinterpret_cast<float *>(at + p.counts + 2 * p.items);
+    a.totals = reinterpret_cast<uint32_t *>(at + p.counts);
+    a.group = p.group;
+    at += p.counts + p.totals;
+    uint2 *items[2] = {reinterpret_cast<uint2 *>(at), reinterpret_cast<uint2 *>(at + p.items)};
+    a.partial = reinterpret_cast<float *>(at + 2 * p.items);
     const size_t pass_words = size_t(p.blocks) * kBins;
     hipStream_t s = (hipStream_t)stream;
     const int64_t fill = a.accumulate ? 0 : op->vocab * int64_t(a.per_row);
@@ -599,6 +653,12 @@ int cchip_embedding_backward(const cchip_embedding *op, const cchip_embedding_io
         a.counts = counts + i * pass_words;
         a.next = i + 1 < p.passes ? a.counts + pass_words : nullptr;
         a.shift = i * kBits;
+        if (p.groups) {
+          hipLaunchKernelGGL(sum_groups, dim3(unsigned(p.groups)), dim3(kSortThreads), 0, s, a);
+          check_launch(who);
+          hipLaunchKernelGGL(place_blocks, dim3(unsigned(p.groups)), dim3(kSortThreads), 0, s, a);
+          check_launch(who);
+        }
         hipLaunchKernelGGL(sort_words, dim3(unsigned(p.blocks)), dim3(kSortThreads), 0, s, a);
         check_launch(who);
       }

@@ -9,7 +9,8 @@ import torch
 
 import attending_reference as A
 from cudacaml_amd import operators as O
-from test_gpu_attending_operators import TYPES, attention_arrays, check_attention, f64, nans, normal, run_attention, same
+from test_gpu_attending_operators import (TYPES, attention_arrays, check_attention, f64, ids_of, nans, normal, run_attention,
+                                          run_embedding, same)
 
 pytestmark = pytest.mark.gpu
 
@@ -162,3 +163,31 @@ def test_attention_largest_f32_values(device, tokens, d):
     most = torch.finfo(torch.float32).max
     x["v"][0, 2, 0, 3], x["v"][0, tokens - 7, 0, 5], x["v"][0, 5, 0, 6] = most, -most, 3.395e38
     check_attention(x, "f32", run_attention(x, "f32"))
+
+
+# ---- embedding -------------------------------------------------------------------
+
+@pytest.mark.parametrize("tokens,vocab,width", [(192 * 2048, 5000, 3), (192 * 2048 + 1, 5000, 3), (257 * 2048 + 9, 600000, 8), ((1 << 20) + 2047, 70, 1)])
+def test_embedding_of_many_tokens(device, tokens, vocab, width):
+    """On both sides of where blocks' places are made by groups of blocks, the
+    last group and block whole and not, in one to three passes."""
+    ids = ids_of(tokens, vocab, seed=tokens)
+    ids[::1000] = -1
+    run_embedding("f32", ids, vocab, width, seed=7)
+    run_embedding("bf16", ids, vocab, width, seed=8, accumulate=True, weight="f32")
+
+
+def test_embedding_of_a_hundred_million_tokens(device):
+    """Groups of more than 64 blocks. Rows of whole numbers, whose sums f32
+    holds, so that the order of a sum does not count."""
+    tokens, vocab = (1 << 27) + 3 * 2048 + 77, 3000
+    g = torch.Generator(device="cuda").manual_seed(9)
+    ids = torch.randint(-2, vocab, (tokens,), generator=g, dtype=torch.int32, device="cuda")
+    dout = torch.randint(-8, 9, (tokens, 1), generator=g, device="cuda", dtype=torch.int32)
+    want = torch.zeros(vocab + 2, dtype=torch.int64, device="cuda").index_add_(0, (ids + 2).long(), dout[:, 0].long())[2:]
+    dout, dw = dout.to(torch.bfloat16), nans((vocab, 1), "f32")
+    op = O.Embedding("bf16", tokens, vocab, 1, weight_dtype="f32")
+    op.backward(ids, dout, dw)
+    torch.cuda.synchronize()
+    assert torch.equal(dw[:, 0].long(), want)
+    op.free()
