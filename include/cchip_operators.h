@@ -299,7 +299,8 @@ int cchip_head_norm_backward(const cchip_head_norm *op, const cchip_head_norm_io
  *
  * ids are i32; one that is not in 0 .. vocab - 1, such as a padding token's,
  * has a row of zeros and no gradient. The table is of dtype or f32. Sums are
- * f32, in the order of the tokens. The backward pass writes all of dweight,
+ * f32, in an order that does not change from run to run (pieces of a word's
+ * tokens, then the pieces). The backward pass writes all of dweight,
  * or, with `accumulate`, adds to the rows of the words that there are.
  */
 typedef struct {
