@@ -127,22 +127,23 @@ AttentionArgs args_of(const cchip_attention &op, const cchip_attention_io &io, b
     a.gk = heads_of(kWho, "dk", op.dtype, b, n, hk, d, io.dk, true);
     a.gv = heads_of(kWho, "dv", op.dtype, b, n, hk, d, io.dv, true);
   }
-  // other workgroups read what one of a call writes; of tensors that lie
-  // between one another the first heads are looked at
+  // other workgroups read what one of a call writes
   struct Named {
     const char *name;
-    const void *p;
+    const Heads *x;
+    HeadCounts n;
   };
-  const Named in[] = {{"q", io.q.data}, {"k", io.k.data}, {"v", io.v.data}, {"the gradient of o", io.d_o.data}, {"o", io.o.data}};
-  const Named out[] = {{"dq", io.dq.data}, {"dk", io.dk.data}, {"dv", io.dv.data}}, o[] = {{"o", io.o.data}};
-  const size_t bytes = b * t ? size_t(d) * (op.dtype == CCHIP_F32 ? 4 : 2) : 0;
-  for (int i = 0; i < (back ? 3 : 1); i++) {
-    const Named &to = back ? out[i] : o[i];
+  const HeadCounts qs = {{b, t, h}}, ks = {{b, n, hk}};
+  const Named in[] = {{"q", &a.q, qs}, {"k", &a.k, ks}, {"v", &a.v, ks}, {"the gradient of o", &a.d_o, qs}, {"o", &a.o, qs}};
+  const Named out[] = {{"dq", &a.gq, qs}, {"dk", &a.gk, ks}, {"dv", &a.gv, ks}}, o = in[4];
+  const int size = op.dtype == CCHIP_F32 ? 4 : 2;
+  for (int i = 0; i < (back ? 3 : 1) && b * t; i++) {
+    const Named &to = back ? out[i] : o;
     for (int j = 0; j < (back ? 5 : 3); j++)
-      if (meet(to.p, bytes, in[j].p, bytes))
+      if (heads_meet(d, size, to.n, *to.x, in[j].n, *in[j].x))
         throw InvalidArgument(strf("attention: %s is written over %s, which the call reads", to.name, in[j].name));
     for (int j = 0; j < i; j++)
-      if (meet(to.p, bytes, out[j].p, bytes))
+      if (heads_meet(d, size, to.n, *to.x, out[j].n, *out[j].x))
         throw InvalidArgument(strf("attention: %s and %s are written to one place", out[j].name, to.name));
   }
   if (op.sequences ? !io.offsets : io.offsets != nullptr)

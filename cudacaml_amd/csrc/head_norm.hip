@@ -342,11 +342,17 @@ void check_aligned(const char *name, const void *p, size_t to) {
   if (reinterpret_cast<uintptr_t>(p) % to) throw InvalidArgument(strf("head norm: %s is not aligned to its elements", name));
 }
 
-// Written over what is read, as far as the first heads show it: in one place
-// only where `in_place` says that each head is read before it is written.
-void check_place(const cchip_head_norm &op, const char *out, const Heads &y, const char *in, const Heads &x, bool in_place) {
-  const size_t bytes = size_t(op.head_dim) * (op.dtype == CCHIP_F32 ? 4 : 2);
-  if (!y.p || !x.p || !meet(y.p, bytes, x.p, bytes)) return;
+// Written over what is read: in one place only where `in_place` says that each
+// head is read before it is written. Of caches, whose places are the
+// positions', the first heads are looked at.
+void check_place(const cchip_head_norm &op, const char *out, const Heads &y, int64_t y_heads, const char *in, const Heads &x, int64_t x_heads,
+                 bool in_place, bool cache) {
+  const int size = op.dtype == CCHIP_F32 ? 4 : 2;
+  if (!y.p || !x.p) return;
+  const size_t bytes = size_t(op.head_dim) * size;
+  if (cache ? !meet(y.p, bytes, x.p, bytes)
+            : !heads_meet(op.head_dim, size, {{op.batch, op.tokens, y_heads}}, y, {{op.batch, op.tokens, x_heads}}, x))
+    return;
   if (in_place && y.p == x.p && (op.batch < 2 || y.b == x.b) && (op.tokens < 2 || y.t == x.t) && y.h == x.h) return;
   throw InvalidArgument(strf("head norm: %s is written over %s%s", out, in, in_place ? ", and not head for head" : ""));
 }
@@ -447,11 +453,14 @@ int cchip_head_norm_forward(const cchip_head_norm *op, const cchip_head_norm_io 
     struct Named {
       const char *name;
       const Heads *x;
+      int heads;
     };
-    const Named in[] = {{"q", &q.x}, {"k", &k.x}, {"v", &v.x}}, out[] = {{"q_out", &q.y}, {"k_out", &k.y}, {"k_cache", &k.cache}, {"v_cache", &v.cache}};
+    const int h = op->heads, hk = op->kv_heads;
+    const Named in[] = {{"q", &q.x, h}, {"k", &k.x, hk}, {"v", &v.x, hk}},
+                out[] = {{"q_out", &q.y, h}, {"k_out", &k.y, hk}, {"k_cache", &k.cache, hk}, {"v_cache", &v.cache, hk}};
     for (int i = 0; i < 4; i++) {
-      for (int j = 0; j < 3; j++) check_place(*op, out[i].name, *out[i].x, in[j].name, *in[j].x, i == j && i < 2);
-      for (int j = 0; j < i; j++) check_place(*op, out[i].name, *out[i].x, out[j].name, *out[j].x, false);
+      for (int j = 0; j < 3; j++) check_place(*op, out[i].name, *out[i].x, out[i].heads, in[j].name, *in[j].x, in[j].heads, i == j && i < 2, i > 1);
+      for (int j = 0; j < i; j++) check_place(*op, out[i].name, *out[i].x, out[i].heads, out[j].name, *out[j].x, out[j].heads, false, i > 1);
     }
     launch(*op, a, cut_of(*op, false), false, (hipStream_t)stream);
   });
@@ -483,12 +492,14 @@ int cchip_head_norm_backward(const cchip_head_norm *op, const cchip_head_norm_io
       struct Named {
         const char *name;
         const Heads *x;
+        int heads;
       };
-      const Named in[] = {{"the gradient of q_out", &q.g}, {"the gradient of k_out", &k.g}, {"q", &q.x}, {"k", &k.x}},
-                  out[] = {{"dq", &q.y}, {"dk", &k.y}};
+      const int h = op->heads, hk = op->kv_heads;
+      const Named in[] = {{"the gradient of q_out", &q.g, h}, {"the gradient of k_out", &k.g, hk}, {"q", &q.x, h}, {"k", &k.x, hk}},
+                  out[] = {{"dq", &q.y, h}, {"dk", &k.y, hk}};
       for (int i = 0; i < 2; i++)
-        for (int j = 0; j < 4; j++) check_place(*op, out[i].name, *out[i].x, in[j].name, *in[j].x, i == j);
-      check_place(*op, "dk", k.y, "dq", q.y, false);
+        for (int j = 0; j < 4; j++) check_place(*op, out[i].name, *out[i].x, out[i].heads, in[j].name, *in[j].x, in[j].heads, i == j, false);
+      check_place(*op, "dk", k.y, hk, "dq", q.y, h, false, false);
       if (any) {
         const size_t need = partial_bytes(*op);
         if (workspace_bytes < need || !workspace || !aligned16(workspace))

@@ -31,6 +31,46 @@ inline bool heads_overlap(int64_t batch, int64_t tokens, const cchip_heads &x, i
   return false;
 }
 
+// A tensor's counts along its axes.
+struct HeadCounts {
+  int64_t n[3];  // batch, tokens, heads
+};
+
+// Whether elements of one tensor lie in another's. Of tensors with other
+// distances along an axis that both go along, which may lie between one
+// another, the first heads are looked at. Otherwise heads of the two are as far
+// apart as the tensors and a whole number of steps along each axis. Where a
+// step is longer than all that the shorter ones reach together, as it is
+// unless a tensor reads elements twice, the whole number nearest to what is
+// left is the one, or one beside it.
+inline bool heads_meet(int dim, int size, const HeadCounts &nx, const Heads &x, const HeadCounts &ny, const Heads &y) {
+  const int64_t sx[] = {x.b, x.t, x.h}, sy[] = {y.b, y.t, y.h};
+  int64_t step[3], least[3], most[3];
+  int axes = 0;
+  __int128 low = 0, high = 0;
+  for (int i = 0; i < 3; i++) {
+    if (nx.n[i] < 1 || ny.n[i] < 1) return false;
+    if (nx.n[i] > 1 && ny.n[i] > 1 && sx[i] != sy[i]) return meet(x.p, size_t(dim) * size, y.p, size_t(dim) * size);
+    const int64_t s = nx.n[i] > 1 ? sx[i] : sy[i];
+    if ((nx.n[i] < 2 && ny.n[i] < 2) || s == 0) continue;
+    int at = axes++;
+    for (; at > 0 && std::llabs(step[at - 1]) < std::llabs(s); at--) step[at] = step[at - 1], least[at] = least[at - 1], most[at] = most[at - 1];
+    step[at] = s, least[at] = 1 - ny.n[i], most[at] = nx.n[i] - 1;
+    low += __int128(s) * (s > 0 ? least[at] : most[at]);
+    high += __int128(s) * (s > 0 ? most[at] : least[at]);
+  }
+  const __int128 apart = (reinterpret_cast<intptr_t>(y.p) - reinterpret_cast<intptr_t>(x.p)) / size;
+  if (apart <= low - dim || apart >= high + dim) return false;
+  const auto among = [&](const auto &self, int axis, __int128 left) -> bool {
+    if (axis == axes) return left < dim && left > -dim;
+    const __int128 near = left / step[axis];
+    for (int i = -1; i <= 1; i++)
+      if (near + i >= least[axis] && near + i <= most[axis] && self(self, axis + 1, left - (near + i) * step[axis])) return true;
+    return false;
+  };
+  return among(among, 0, apart);
+}
+
 // What a kernel takes of an operator's tensor. The distance of tokens is
 // bounded so that a kernel may count the elements of some hundred of them in
 // 32 bits.

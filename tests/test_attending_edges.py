@@ -1,0 +1,93 @@
+"""What attention and the norm of its heads refuse of arrays that lie in one
+another, against every address, without a device."""
+
+import numpy as np
+import pytest
+
+from cudacaml_amd import _lib
+from cudacaml_amd import operators as O
+
+DIM, SIZE, BASE = 4, 4, 1 << 20
+
+
+def _places(at, counts, steps):
+    """The first places, in elements, of all heads of an array."""
+    i = np.indices(counts).reshape(3, -1)
+    return at + (i * np.array(steps)[:, None]).sum(0)
+
+
+def _meet(x, y):
+    return bool((np.abs(x[:, None] - y[None, :]) < DIM).any())
+
+
+def _steps(g, counts):
+    """Distances along the axes in an order of their own, with something between
+    neighbours or not, and of any sign but the tokens'."""
+    steps, reach = [0, 0, 0], DIM
+    for axis in g.permutation(3):
+        steps[axis] = int(reach + g.choice([0, 0, 3, DIM, 2 * DIM]))
+        reach += steps[axis] * (max(counts[axis], 2) - 1)
+        if axis != 1 and g.random() < 0.2:
+            steps[axis] *= -1
+    return steps, reach
+
+
+def _heads(at, steps):
+    return (BASE + at * SIZE, *steps)
+
+
+def _far(at):
+    return (at << 24, 1 << 16, 1 << 10, 1 << 6)
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_attention_refuses_results_within_inputs_wherever_they_meet(seed):
+    """o moved along q by any distance, with q's steps: refused if a head of one
+    lies in a head of the other, and not otherwise; of two results too."""
+    g = np.random.default_rng(seed)
+    L, seen = _lib.lib(), [0, 0]
+    for _ in range(400):
+        b, t, hk, group = (int(x) for x in g.integers(1, 5, 4))
+        h = hk * group
+        counts = (b, t, h)
+        steps, reach = _steps(g, counts)
+        desc = _lib.AttentionDesc(0, b, t, 0, 0, h, hk, DIM, 1.0)
+        # about as far as the array reaches, mostly by whole steps and a little
+        by = int(sum(int(g.integers(-n, n + 1)) * s for n, s in zip(counts, steps)) + g.integers(-DIM, DIM + 1)) if g.random() < 0.8 else int(
+            g.integers(-reach, reach))
+        at = 4 * reach
+        io = O.Attention._forward_io.pack(*_heads(at, steps), *_far(2), *_far(3), *_heads(at + by, steps), 0, 0, 4098)
+        rc, msg = L.cchip_attention_forward(desc, io, None, 0, None), _lib.lib().cchip_last_error().decode()
+        met = _meet(_places(at, counts, steps), _places(at + by, counts, steps))
+        assert rc == 1 and ("o is written over q" if met else "saved is not aligned") in msg, (counts, steps, by, msg)
+        seen[met] += 1
+        # dk beside dq: fewer heads, with the same steps
+        back = [*_far(2), *_far(3), *_far(4), *_far(5), *_far(6), *_heads(at, steps), *_heads(at + by, steps), *_far(7)]
+        rc, msg = L.cchip_attention_backward(desc, O.Attention._backward_io.pack(*back, 0, 0, 4098), None, 0, None), _lib.lib().cchip_last_error().decode()
+        met = _meet(_places(at, counts, steps), _places(at + by, (b, t, hk), steps))
+        assert rc == 1 and ("dq and dk are written to one place" if met else "saved is not aligned") in msg, (counts, hk, steps, by, msg)
+    assert min(seen) > 50
+
+
+@pytest.mark.parametrize("seed", range(2))
+def test_head_norm_refuses_results_within_inputs_wherever_they_meet(seed):
+    """All but the very place."""
+    g = np.random.default_rng(10 + seed)
+    L = _lib.lib()
+    none = (0, 0, 0, 0)
+    for _ in range(300):
+        b, t, h, hk = (int(x) for x in g.integers(1, 5, 4))
+        counts = (b, t, h)
+        steps, reach = _steps(g, counts)
+        desc = _lib.HeadNormDesc(0, 0, b, t, 0, h, hk, DIM, DIM, 0, 1, 1e-6)
+        by = int(sum(int(g.integers(-n, n + 1)) * s for n, s in zip(counts, steps)) + (g.integers(-DIM, DIM + 1) if g.random() < 0.5 else 0))
+        at = 4 * reach
+        # the sum of a weight's gradient has no workspace, which is refused last
+        back = [*_heads(at, steps), *_far(2), *none, *none, *none, *none, *none, *_far(3), *_far(4), *_heads(at + by, steps), *_far(5),
+                0, 4096, 0, 0, 4096, 0]
+        rc, msg = L.cchip_head_norm_backward(desc, O.HeadNorm._io.pack(*back), None, 0, None), _lib.lib().cchip_last_error().decode()
+        met = _meet(_places(at, counts, steps), _places(at + by, counts, steps))
+        assert rc == 1 and ("dq is written over q" if met else "workspace needs") in msg, (counts, steps, by, msg)
+        back[0:4], back[28:32] = _far(3), _heads(at, steps)  # the gradient, which dq may take the place of
+        rc, msg = L.cchip_head_norm_backward(desc, O.HeadNorm._io.pack(*back), None, 0, None), _lib.lib().cchip_last_error().decode()
+        assert rc == 1 and ("not head for head" if met and by else "workspace needs") in msg, (counts, steps, by, msg)
