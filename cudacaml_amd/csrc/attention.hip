@@ -173,9 +173,18 @@ AttentionArgs args_of(const cchip_attention &op, const cchip_attention_io &io, b
   return a;
 }
 
-void check_workspace(const void *workspace, size_t have, size_t need) {
+// The workspace is large enough, and neither it nor `saved` is where a tensor
+// begins or the other is.
+void check_workspace(const cchip_attention &op, const cchip_attention_io &io, const void *workspace, size_t have, size_t need) {
   if (have < need || (need && !workspace) || (need && !aligned16(workspace)))
     throw InvalidArgument(strf("attention: the workspace needs %zu bytes aligned to 16, has %zu", need, workspace ? have : 0));
+  const size_t saved = io.saved ? saved_bytes(op) : 0, head = size_t(op.head_dim) * (op.dtype == CCHIP_F32 ? 4 : 2);
+  if (meet(workspace, need, io.saved, saved)) throw InvalidArgument("attention: the workspace is what the forward pass saved");
+  const std::pair<const char *, const void *> tensors[] = {{"q", io.q.data}, {"k", io.k.data}, {"v", io.v.data}, {"o", io.o.data},
+                                                           {"the gradient of o", io.d_o.data}, {"dq", io.dq.data}, {"dk", io.dk.data}, {"dv", io.dv.data}};
+  for (auto &x : tensors)
+    if (x.second && (meet(workspace, need, x.second, head) || meet(io.saved, saved, x.second, head)))
+      throw InvalidArgument(strf("attention: %s lies in %s", x.first, meet(workspace, need, x.second, head) ? "the workspace" : "what the forward pass saves"));
 }
 
 }  // namespace
@@ -200,8 +209,8 @@ int cchip_attention_forward(const cchip_attention *op, const cchip_attention_io 
     AttentionArgs a = args_of(*op, *io, false);
     if (op->keys && io->saved) throw InvalidArgument("attention: there is no backward pass over a cache");
     const Cut p = cut_of(*op);
-    check_workspace(workspace, workspace_bytes, p.bytes);
     if (op->batch * op->tokens == 0) return;
+    check_workspace(*op, *io, workspace, workspace_bytes, p.bytes);
     a.partial = static_cast<float *>(workspace);
     a.slots = p.slots;
     a.splits = p.splits;
@@ -222,9 +231,7 @@ int cchip_attention_backward(const cchip_attention *op, const cchip_attention_io
     if (op->batch * op->tokens == 0) return;
     if (!io->saved) throw InvalidArgument("attention: the backward pass needs what the forward pass saved");
     const BackCut c = back_cut_of(*op);
-    check_workspace(workspace, workspace_bytes, c.sizes.bytes());
-    if (meet(workspace, c.sizes.bytes(), io->saved, saved_bytes(*op)))
-      throw InvalidArgument("attention: the workspace is what the forward pass saved");
+    check_workspace(*op, *io, workspace, workspace_bytes, c.sizes.bytes());
     char *at = static_cast<char *>(workspace);
     for (int i = 0; i < 4; i++) {
       a.tiles[i] = reinterpret_cast<u32x4 *>(at);

@@ -91,3 +91,26 @@ def test_head_norm_refuses_results_within_inputs_wherever_they_meet(seed):
         back[0:4], back[28:32] = _far(3), _heads(at, steps)  # the gradient, which dq may take the place of
         rc, msg = L.cchip_head_norm_backward(desc, O.HeadNorm._io.pack(*back), None, 0, None), _lib.lib().cchip_last_error().decode()
         assert rc == 1 and ("not head for head" if met and by else "workspace needs") in msg, (counts, steps, by, msg)
+
+
+def test_attention_refuses_tensors_in_its_workspace():
+    L = _lib.lib()
+    t = lambda p, h=4: (p << 24, 100 * 8 * h, 8 * h, 8)  # noqa: E731
+    desc = _lib.AttentionDesc(0, 2, 100, 0, 0, 4, 2, 8, 1.0)
+    back = [*t(1), *t(2, 2), *t(3, 2), *t(4), *t(5), *t(6), *t(7, 2), *t(8, 2)]
+    need = O.Attention("f32", 2, 100, 4, 2, 8).workspace_bytes(backward=True)
+    assert need < 1 << 24  # the first address that a tensor has
+    for at in range(8):
+        io = O.Attention._backward_io.pack(*back, 0, 0, 1 << 28)
+        rc, msg = L.cchip_attention_backward(desc, io, ((at + 1) << 24) - need + 16, need, None), L.cchip_last_error().decode()
+        assert rc == 1 and "lies in the workspace" in msg
+    cache = _lib.AttentionDesc(0, 2, 1, 0, 4096, 4, 2, 8, 1.0)
+    need = O.Attention("f32", 2, 1, 4, 2, 8, keys=4096).workspace_bytes()
+    words = [*t(1), 2 << 24, 1 << 16, 16, 8, 3 << 24, 1 << 16, 16, 8, *t(4)]
+    for p in (1 << 24, 2 << 24, 3 << 24, 4 << 24):
+        io = O.Attention._forward_io.pack(*words, 0, 4096, 0)
+        rc, msg = L.cchip_attention_forward(cache, io, p - need + 16, need, None), L.cchip_last_error().decode()
+        assert need > 0 and rc == 1 and "lies in the workspace" in msg
+    for p in (1, 2, 3, 4):  # and `saved`, which a forward call writes
+        rc, msg = L.cchip_attention_forward(desc, O.Attention._forward_io.pack(*back[:16], 0, 0, p << 24), None, 0, None), L.cchip_last_error().decode()
+        assert rc == 1 and "what the forward pass saves" in msg
