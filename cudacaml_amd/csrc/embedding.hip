@@ -8,6 +8,7 @@
 // cache behind the second level), 34 the sums, 7 those over pieces.
 
 #include "../../include/cchip_operators.h"
+#include "heads.hpp"
 #include "operators.hpp"
 #include "rows.hpp"
 
@@ -529,6 +530,16 @@ void check_op(const cchip_embedding *op) {
   if (!std::isfinite(op->scale)) throw InvalidArgument("embedding: scale is not finite");
 }
 
+// The table's rows, one of which is a word's, and the tokens', one of which is
+// written or read, lie apart; those of two types as far as the first rows show it.
+void check_apart(const cchip_embedding &op, const char *out_name, const Rows &out, const char *in_name, const Rows &in, bool table_written) {
+  const int64_t rows[] = {op.vocab, op.tokens};
+  const int size = op.dtype == CCHIP_F32 ? 4 : 2;
+  if (op.weight_dtype != op.dtype) return check_place("embedding", op.dtype, op.tokens, op.width, out_name, out, in_name, in, false);
+  if (heads_meet(int(op.width), size, {{1, rows[!table_written], 1}}, {out.p, 0, out.row, 0}, {{1, rows[table_written], 1}}, {in.p, 0, in.row, 0}))
+    throw InvalidArgument(strf("embedding: %s is written over %s", out_name, in_name));
+}
+
 const int32_t *ids_of(const cchip_embedding_io &io) {
   if (!io.ids) throw InvalidArgument("embedding: no ids");
   if (reinterpret_cast<uintptr_t>(io.ids) % 4) throw InvalidArgument("embedding: ids are not aligned to their elements");
@@ -562,7 +573,7 @@ int cchip_embedding_forward(const cchip_embedding *op, const cchip_embedding_io 
     a.ids = ids_of(*io);
     a.weight = rows_of(who, "weight", op->weight_dtype, op->vocab, op->width, io->weight, false, true);
     a.out = rows_of(who, "out", op->dtype, op->tokens, op->width, io->out, true, true);
-    check_place(who, op->dtype, op->tokens, op->width, "out", a.out, "weight", a.weight, false);
+    check_apart(*op, "out", a.out, "weight", a.weight, false);
     a.tokens = op->tokens;
     a.vocab = op->vocab;
     a.width = op->width;
@@ -595,7 +606,7 @@ int cchip_embedding_backward(const cchip_embedding *op, const cchip_embedding_io
     if (op->tokens) {
       a.ids = ids_of(*io);
       a.dout = rows_of(who, "dout", op->dtype, op->tokens, op->width, io->dout, false, true);
-      check_place(who, op->dtype, op->tokens, op->width, "dweight", a.dweight, "dout", a.dout, false);
+      check_apart(*op, "dweight", a.dweight, "dout", a.dout, true);
     }
     const Layout p = layout_of(*op);
     if (workspace_bytes < p.bytes() || (p.bytes() && (!workspace || !aligned16(workspace))))

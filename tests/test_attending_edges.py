@@ -1,5 +1,5 @@
-"""What attention and the norm of its heads refuse of arrays that lie in one
-another, against every address, without a device."""
+"""What attention, the norm of its heads and the embedding refuse of arrays that
+lie in one another, against every address, without a device."""
 
 import numpy as np
 import pytest
@@ -114,3 +114,23 @@ def test_attention_refuses_tensors_in_its_workspace():
     for p in (1, 2, 3, 4):  # and `saved`, which a forward call writes
         rc, msg = L.cchip_attention_forward(desc, O.Attention._forward_io.pack(*back[:16], 0, 0, p << 24), None, 0, None), L.cchip_last_error().decode()
         assert rc == 1 and "what the forward pass saves" in msg
+
+
+@pytest.mark.parametrize("seed", range(2))
+def test_embedding_refuses_rows_within_its_table(seed):
+    g = np.random.default_rng(20 + seed)
+    L, seen = _lib.lib(), [0, 0]
+    for _ in range(300):
+        vocab, tokens = (int(x) for x in g.integers(1, 9, 2))
+        step, by = int(DIM + g.choice([0, 0, 2, DIM, 9])), int(g.integers(-120, 120))
+        desc = _lib.EmbeddingDesc(0, 0, tokens, vocab, DIM, 1.0)
+        met = _meet(_places(0, (1, vocab, 1), (0, step, 0)), _places(by, (1, tokens, 1), (0, step, 0)))
+        table, rows = BASE, BASE + by * SIZE
+        seen[met] += 1
+        if not met:  # taken, which only a device can show
+            continue
+        for fn, words in ((L.cchip_embedding_forward, [4096, table, step, rows, step, 0, 0, 0, 0, 0]),
+                          (L.cchip_embedding_backward, [4096, 0, 0, 0, 0, rows, step, table, step, 0])):
+            rc = fn(desc, O.Embedding._io.pack(*words), *((None,) if fn is L.cchip_embedding_forward else (None, 0, None)))
+            assert rc == 1 and "is written over" in L.cchip_last_error().decode(), (vocab, tokens, step, by)
+    assert min(seen) > 30
