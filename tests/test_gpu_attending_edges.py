@@ -9,7 +9,7 @@ import torch
 
 import attending_reference as A
 from cudacaml_amd import operators as O
-from test_gpu_attending_operators import (TYPES, attention_arrays, check_attention, f64, ids_of, nans, normal, run_attention,
+from test_gpu_attending_operators import (BOUND, TYPES, attention_arrays, check_attention, f64, ids_of, nans, normal, run_attention,
                                           run_embedding, same)
 
 pytestmark = pytest.mark.gpu
@@ -163,6 +163,23 @@ def test_attention_largest_f32_values(device, tokens, d):
     most = torch.finfo(torch.float32).max
     x["v"][0, 2, 0, 3], x["v"][0, tokens - 7, 0, 5], x["v"][0, 5, 0, 6] = most, -most, 3.395e38
     check_attention(x, "f32", run_attention(x, "f32"))
+
+
+@pytest.mark.parametrize("dtype,large,small", [("bf16", 1.0, 2.0 ** -24), ("f16", 2.0 ** 8, 2.0 ** -8)])
+def test_attention_gradients_of_rows_far_smaller_than_their_neighbours(device, dtype, large, small):
+    """Every other token's gradient of o: a tile's elements are whole down to
+    2^-28 of its largest, which those here are but for few, and those to
+    2^-38; so its queries' gradients are as exact as the others'."""
+    x = attention_arrays(dtype, 1, 200, 4, 2, 64, seed=32)
+    x["do"][:, ::2] *= large
+    x["do"][:, 1::2] *= small
+    got = f64(run_attention(x, dtype)["dq"])[0]
+    a = {n: f64(v)[0] for n, v in x.items()}
+    want = A.attention(a["q"], a["k"], a["v"], 64 ** -0.5, a["do"])[1]
+    tiny = 2.0 ** -25 if dtype == "f16" else 0.0  # half of f16's least step
+    for rows in (slice(0, None, 2), slice(1, None, 2)):
+        off = np.linalg.norm(got[rows] - want[rows])
+        assert off <= BOUND[dtype] * np.linalg.norm(want[rows]) + tiny * want[rows].size ** 0.5
 
 
 # ---- embedding -------------------------------------------------------------------
