@@ -68,10 +68,15 @@ Cut cut_of(const cchip_attention &op) {
     throw InvalidArgument("attention: more tokens and heads than a launch can have");
   p.slots = int(slots);
   p.splits = 1;
-  // Keys are split where there are too few workgroups for the chip (512: twice
-  // its units, as many of the kernel for few rows as run at once; with 1024 a step of
-  // 16 sequences over 2048 keys took 39.7 us in place of 32.7, of one over 32768
-  // 56.8 in place of 41.8), but into parts that are long beside what joining them costs.
+  // Keys are split where there are too few workgroups for the chip, but into
+  // parts that are long beside what joining them costs. 512 are wanted: of the
+  // kernel for few rows as many as run at once (with 1024 a step of 16
+  // sequences over 2048 keys took 39.7 us in place of 32.7, of one over 32768 56.8 in
+  // place of 41.8). Of the others 256 run at once, but parts follow each
+  // sequence's own length: for sequences as long as one another 256 are better
+  // (chunks of 512 tokens over 8192 keys 163 us in place of 174, four of 256
+  // over 4096 98 in place of 114), for others 512 (512 over 8192 and 4352 keys
+  // 145 in place of 158).
   const int64_t base = std::max<int64_t>(1, pairs * slots), least = !p.waves ? 128 : op.dtype == CCHIP_F32 ? 256 : 512, wanted = 512;
   if (!op.sequences && base < wanted) p.splits = int(std::max<int64_t>(1, std::min((wanted + base - 1) / base, keys / least)));
   p.workgroups = pairs * slots * p.splits;  // at most 2^30: splits are few where it is much

@@ -8,8 +8,8 @@
 // of two: 8 for 128 elements, 8 heads to a wave at a time. A wave goes through
 // the heads of a token; the cosines and sines, which all of them share, are
 // made by its lanes, one each, and handed round through LDS. Bound by memory:
-// 16384 tokens, 32 and 8 heads of 128, bf16: 73.6 us for 336 MB forward, 108.8
-// for 503 MB backward and 5.2 for the sums of the weights' gradients: 4.6 TB/s
+// 16384 tokens, 32 and 8 heads of 128, bf16: 73.6 us for 336 MB forward, 107.1
+// for 503 MB backward and 5.1 for the sums of the weights' gradients: 4.6 and 4.7 TB/s
 // (a copy of 2 GiB: 4.86).
 
 #include "heads.hpp"

@@ -109,7 +109,9 @@ int cchip_gated_delta_backward(const cchip_gated_delta *op, const cchip_gated_de
  *   j <= t + (keys of the sequence) - (tokens of the sequence)
  *   p_j = softmax_j(scale q_t . k_j),   o_t = sum_j p_j v_j
  *
- * heads is a multiple of kv_heads; sums, maxima and scores are f32. A query
+ * heads is a multiple of kv_heads; sums, maxima and scores are f32. Weights
+ * of 16-bit types are rounded to them on their way to the values, and the sum
+ * that divides is of the rounded ones. A query
  * that sees no key, or whose every score is -infinity, has zeros for o. Three
  * kinds of batches:
  *
@@ -128,7 +130,10 @@ int cchip_gated_delta_backward(const cchip_gated_delta *op, const cchip_gated_de
  * values are summed in f32 before the division by the weights' sum, which
  * those of 16 bits beyond 2^96 may overflow.
  * In the backward pass one in q, k, v or the gradient of o may reach the
- * gradients of other tokens of its sequence that stand within 128 of it.
+ * gradients of other tokens of its sequence that stand within 128 of it, and
+ * 16-bit elements there are taken in steps of 2^-38 of the largest among 64
+ * neighbouring rows (tokens, for q and the gradient of o times the heads of a
+ * group): whole down to 2^-28 of it.
  */
 typedef struct {
   int dtype;
