@@ -135,6 +135,21 @@ __device__ __forceinline__ Bits<Planes<T>::N> bits_of(const Raw8<T> &r) {
   }
 }
 
+// The same of finite elements however large: what would round to an infinity
+// has the largest bf16 as its first plane, and the others hold the rest.
+template <typename T>
+__device__ __forceinline__ Bits<Planes<T>::N> whole_bits_of(const Raw8<T> &r) {
+  if constexpr (std::is_same<T, float>::value) {
+    constexpr float kMost = 0x1.FEp127f;
+    float first[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) first[i] = __builtin_amdgcn_fmed3f(r.x[i], -kMost, kMost);
+    return planes_of<T>(r.x, first);
+  } else {
+    return bits_of<T>(r);
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ Raw8<T> negated(Raw8<T> r) {
 #pragma unroll
@@ -262,13 +277,19 @@ struct Staged {
 
   template <typename E>
   __device__ __forceinline__ void store(int t, E *m) const {
-    constexpr int N = Planes<T>::N;
 #pragma unroll
-    for (int i = 0; i < kEach; i++) {
-      const Bits<N> b = bits_of<T>(r[i]);
+    for (int i = 0; i < kEach; i++) store_piece(t, i, m, bits_of<T>(r[i]));
+  }
+  template <typename E>
+  __device__ __forceinline__ void store_whole(int t, E *m) const {
 #pragma unroll
-      for (int n = 0; n < N; n++) *reinterpret_cast<u32x4 *>(m + n * tile_elements<D>(Rows) + piece_at<D>(row(t, i), piece(t, i))) = b.p[n];
-    }
+    for (int i = 0; i < kEach; i++) store_piece(t, i, m, whole_bits_of<T>(r[i]));
+  }
+  template <typename E>
+  static __device__ __forceinline__ void store_piece(int t, int i, E *m, const Bits<Planes<T>::N> &b) {
+#pragma unroll
+    for (int n = 0; n < Planes<T>::N; n++)
+      *reinterpret_cast<u32x4 *>(m + n * tile_elements<D>(Rows) + piece_at<D>(row(t, i), piece(t, i))) = b.p[n];
   }
 };
 

@@ -132,13 +132,7 @@ __device__ __forceinline__ void lay_tile(const AttentionArgs &a, const Heads &x,
   } else {
 #pragma unroll
     for (int i = 0; i < kEach; i++) {
-      // what would round to an infinity has the largest bf16 as its first
-      // plane, and the others hold the rest; an infinity becomes NaN
-      constexpr float kMost = 0x1.FEp127f;
-      float first[8];
-#pragma unroll
-      for (int j = 0; j < 8; j++) first[j] = __builtin_amdgcn_fmed3f(r[i].x[j], -kMost, kMost);
-      const Bits<B::N> b = planes_of<T>(r[i].x, first);
+      const Bits<B::N> b = whole_bits_of<T>(r[i]);  // an infinity's are NaN
 #pragma unroll
       for (int n = 0; n < B::N; n++) to[(n * B::kHigh + (t + i * 256) / kPieces) * kPieces + (piece ^ twist<D>((t + i * 256) / kPieces))] = b.p[n];
     }

@@ -188,24 +188,16 @@ __device__ __forceinline__ void store_row(T *p, const f32x16 (&out)[D / 32], flo
 
 // Whether an element is infinite or NaN; and zero in its place. Planes cannot
 // hold one, so that values of f32 are looked at in all tiles, others only in
-// those that some rows do not see all of. As they pass here anyway, values of
-// f32 are made small, and a row's output large again as its sum is divided:
-// a sum over 2^16 keys of any of them, which terms of up to 2^kSlack multiply,
-// stays finite.
+// those that some rows do not see all of.
 template <typename T>
 constexpr bool kPlanar = Planes<T>::N > 1;
-template <typename T>
-constexpr float kValueScale = kPlanar<T> ? 0x1p-24f : 1.0f;
 
 template <typename T>
 __device__ __forceinline__ bool take_finite(Raw8<T> &r) {
   if constexpr (kPlanar<T>) {
     float any = 0.0f;  // NaN: an element is not finite
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      r.x[i] *= kValueScale<T>;
-      any = __builtin_fmaf(r.x[i], 0.0f, any);
-    }
+    for (int i = 0; i < 8; i++) any = __builtin_fmaf(r.x[i], 0.0f, any);
     if (any == 0.0f) return true;
     stay_branch();
 #pragma unroll
@@ -223,10 +215,6 @@ __device__ __forceinline__ bool take_finite(Raw8<T> &r) {
     return all;
   }
 }
-
-// What a row's sum of values is multiplied by.
-template <typename T>
-__device__ __forceinline__ float of_sum(float sum) { return sum == 0.0f ? 0.0f : 1.0f / kValueScale<T> / sum; }
 
 // Rows' outputs: to o, or as they are for the sum over splits.
 template <typename T, int D>
@@ -247,7 +235,7 @@ __device__ __forceinline__ void finish(const AttentionArgs &a, const Span &s, Ru
   const int64_t token = live ? row / a.group : 0;
   const int head = live ? int(row - token * a.group) : 0;
   T *p = reinterpret_cast<T *>(const_cast<char *>(element(a.o, s.batch, s.first + token, int64_t(s.kv) * a.group + head, sizeof(T))));
-  store_row<T, D>(p, r.out, of_sum<T>(sum), a.dim, live, a.o_rest ? a.o_rest + (row_values(a, s) + row) * a.dim : nullptr);
+  store_row<T, D>(p, r.out, sum == 0.0f ? 0.0f : 1.0f / sum, a.dim, live, a.o_rest ? a.o_rest + (row_values(a, s) + row) * a.dim : nullptr);
   if (a.lse && live && !half)
     a.lse[row_values(a, s) + row] = sum == 0.0f ? INFINITY : r.top - Powers<T>::kLift + __builtin_log2f(sum);
 }
@@ -378,7 +366,7 @@ __global__ CCHIP_WAVES(Waves * 64, Planes<T>::kWaves) void attend(const Attentio
         for (int i = 0; i < vs.kEach; i++) finite = take_finite(vs.r[i]) && finite;
         if (!finite) bad[v_tile & 1] = v_tile + 1;
       }
-      vs.store(t, vt + (v_tile & 1) * kBuffer);
+      vs.store_whole(t, vt + (v_tile & 1) * kBuffer);
     }
   };
   const Places<D> at;
@@ -599,7 +587,7 @@ __global__ CCHIP_WAVES(256, Planes<T>::kWaves) void attend_few(const AttentionAr
 #pragma unroll
       for (int i = 0; i < vs.kEach; i++) finite = take_finite(vs.r[i]) && finite;
     }
-    vs.store(l, m);
+    vs.store_whole(l, m);
     const bool some_bad = (kPlanar<T> || masked) && __ballot(!finite);
     const T *here = v;
     v += 32 * kWaves * a.v.t;
@@ -675,7 +663,7 @@ __global__ CCHIP_WAVES(256, Planes<T>::kWaves) void attend_few(const AttentionAr
     const int64_t token = (row0 + at_row) / a.group;
     const int head = int(row0 + at_row - token * a.group);
     T *p = reinterpret_cast<T *>(const_cast<char *>(element(a.o, s.batch, s.first + token, int64_t(s.kv) * a.group + head, sizeof(T)))) + col;
-    const float up = of_sum<T>(its);
+    const float up = its == 0.0f ? 0.0f : 1.0f / its;
 #pragma unroll
     for (int j = 0; j < 8; j++)
       if (j < n) {
@@ -710,7 +698,7 @@ __global__ __launch_bounds__(256) void join_splits(const AttentionArgs a) {
   const int64_t per_head = a.tokens * a.group, pair = at / per_head, in = at - pair * per_head, token = in / a.group;
   const int64_t batch = pair / a.kv_heads, head = (pair - batch * a.kv_heads) * a.group + (in - token * a.group);
   T *p = reinterpret_cast<T *>(const_cast<char *>(element(a.o, batch, token, head, sizeof(T))));
-  const float up = of_sum<T>(sum);
+  const float up = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
   for (int j = 0; j < 2; j++)
     if (l + 64 * j < a.dim) {

@@ -128,7 +128,7 @@ int cchip_gated_delta_backward(const cchip_gated_delta *op, const cchip_gated_de
  * A NaN or infinity in k or v reaches the queries that see it and no others:
  * one in v as it is in f32, and in 16 bits as one or the other. Weighted
  * values are summed in f32 before the division by the weights' sum, which
- * those of 16 bits beyond 2^96 may overflow.
+ * values beyond 2^96 may overflow.
  * In the backward pass one in q, k, v or the gradient of o may reach the
  * gradients of other tokens of its sequence that stand within 128 of it, and
  * 16-bit elements there are taken in steps of 2^-38 of the largest among 64

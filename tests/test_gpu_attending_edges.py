@@ -155,14 +155,28 @@ def test_attention_infinities_of_f32_are_infinities(device, d, odd, tokens, keys
 
 @pytest.mark.parametrize("tokens,d", [(20, 64), (150, 41), (150, 128)])
 def test_attention_largest_f32_values(device, tokens, d):
-    """Next to what f32 holds, which no 16 bits hold: forward where the sums
-    stay below it, and back. Scores are zeros, so no term is larger than 1."""
+    """Next to what f32 holds, which no 16 bits hold, where their sums stay
+    below it: one to a column, which the others' do not take beyond the largest
+    f32, 3.4028e38. Forward and back; scores are zeros, so no term is larger
+    than 1."""
     x = attention_arrays("f32", 1, tokens, 2, 1, d, seed=8)
     x["q"].zero_()
     x["do"] *= 2.0 ** -20
-    most = torch.finfo(torch.float32).max
-    x["v"][0, 2, 0, 3], x["v"][0, tokens - 7, 0, 5], x["v"][0, 5, 0, 6] = most, -most, 3.395e38
+    x["v"][0, 2, 0, 3], x["v"][0, tokens - 7, 0, 5], x["v"][0, 5, 0, 6] = 3.402e38, -3.402e38, 3.395e38
     check_attention(x, "f32", run_attention(x, "f32"))
+
+
+@pytest.mark.parametrize("tokens,keys", [(150, None), (1, 300), (70, 700)])
+@pytest.mark.parametrize("power", [-104, 80])
+def test_attention_small_and_large_f32_values(device, tokens, keys, power):
+    """As exact as others: three planes hold all bits of values from 2^-110 on."""
+    x = attention_arrays("f32", 1, tokens, 2, 1, 64, seed=33, keys=keys)
+    x["v"] *= 2.0 ** power
+    o = nans(x["q"].shape, "f32")
+    op = O.Attention("f32", 1, tokens, 2, 1, 64, keys=keys)
+    op.forward(*(x[n].cuda() for n in ("q", "k", "v")), o, lengths=None if keys is None else torch.tensor([keys], dtype=torch.int32, device="cuda"))
+    a = {n: f64(v)[0] for n, v in x.items()}
+    A.close(f64(o)[0], A.attention(a["q"], a["k"], a["v"], 64 ** -0.5), "o", BOUND["f32"] * (2 if a["q"].size < 256 else 1))
 
 
 @pytest.mark.parametrize("dtype,large,small", [("bf16", 1.0, 2.0 ** -24), ("f16", 2.0 ** 8, 2.0 ** -8)])
